@@ -458,6 +458,97 @@ int mcb_cross_entropy_chunk(void* logits, const int32_t* targets, float* nll, co
                             int64_t V, int write_grad, int dtype, void* stream);
 int mcb_cross_entropy_finish(const float* nll, const int32_t* count, float* loss, int64_t M, void* stream);
 
+/* ---- losses over the logits of given tokens ---------------------------------------------------- */
+
+/* Post-training beside mcb_cross_entropy: log-probabilities of given tokens, and the losses built on them (preference pairs,
+ * clipped policy) or on a teacher's top logits (distillation), each with its gradient towards the logits in the same call.
+ * The reference has cross-entropy only (src/training/loss.rs:58-147); targets and masks follow it.  The descriptors are HOST
+ * structs, read during the call; everything they point to is device memory.
+ *
+ * Logits [batch, seq, vocab] of MCB_F32 or MCB_BF16: rows of contiguous elements, any non-negative strides (in elements)
+ * between them.  y = logits / temperature throughout.  Gradients are dense [batch * seq, vocab] of the logits' type, and may
+ * lie over dense logits (in place); null: none is computed. */
+typedef struct {
+  const void* logits;
+  int64_t batch, seq, vocab, batch_stride, token_stride;
+  float temperature;
+  int32_t dtype;
+} mcb_token_logits;
+/* targets [batch * seq] int32 or int64 (target_bytes 4 or 8).  -1 and, with has_ignore, ignore_index leave a position out: its
+ * log-probability and gradient are 0 and its logits are not read.  Any other target outside [0, vocab) makes the position's
+ * outputs and gradient, and so the loss, NaN: nothing is checked on the host, every call can be captured into a graph. */
+typedef struct {
+  const void* targets;
+  int32_t target_bytes, has_ignore;
+  int64_t ignore_index;
+} mcb_token_targets;
+/* The clipped policy term of a token: with r = exp(logp - old) (old_logp null: r = 1, the policy that is being trained), advantage A of row i =
+ * advantages[i / advantage_rows] and d = ref - logp:  -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(d) - d - 1);
+ * ref_logp null: no KL is computed.  old_logp and ref_logp are float [batch * seq]. */
+typedef struct {
+  const float* advantages;
+  int64_t advantage_rows;
+  const float* old_logp;
+  const float* ref_logp;
+  float clip_low, clip_high, kl_coef;
+  int32_t pad_;
+} mcb_policy_terms;
+/* A teacher's `top` (1 to 1024) largest logits of each row and their vocabulary ids, [batch * seq, top].  An entry whose logit is
+ * -inf counts for nothing, whatever its id; another id outside [0, vocab) makes the row NaN; an id that comes twice has the sum. */
+typedef struct {
+  const void* ids;      /* int32 or int64 (id_bytes 4 or 8) */
+  const void* logits;   /* MCB_F32 or MCB_BF16, by dtype */
+  int64_t top;
+  int32_t id_bytes, dtype;
+} mcb_teacher_top;
+
+/* logp [batch * seq] = y[target] - lse and, unless null, lse [batch * seq] = log sum exp(y).  unit_grad, unless null:
+ * d logp / d logits of each row in the same pass, for a caller that scales what comes of it later (mcb_scale_rows). */
+int mcb_token_logprob_fwd(const mcb_token_logits* logits, const mcb_token_targets* targets, float* logp, float* lse,
+                          void* unit_grad, void* stream);
+/* The reverse: dlogits = dlogp / temperature * (onehot(target) - softmax(y)), dlogp of row i = dlogp[i / dlogp_rows]; logp and lse as
+ * mcb_token_logprob_fwd left them. */
+int mcb_token_logprob_bwd(const mcb_token_logits* logits, const mcb_token_targets* targets, const float* logp, const float* lse,
+                          const float* dlogp, int64_t dlogp_rows, void* dlogits, void* stream);
+
+/* Workspace of the three calls below; a call's own, like every workspace. */
+size_t mcb_token_loss_workspace_bytes(int64_t batch, int64_t seq);
+/* Preference loss of batch / 2 pairs, the chosen sequences first: with L = sum (average: mean) of a sequence's log-probabilities,
+ * z = beta ((L_c - ref_c) - (L_r - ref_r)):  loss[0] = mean of -(1 - label_smoothing) log sigma(z) - label_smoothing log sigma(-z).
+ * ref_logp [batch]: the frozen reference's L; seq_logp [batch] receives the policy's.  label_smoothing in [0, 0.5]. */
+int mcb_preference_loss(const mcb_token_logits* logits, const mcb_token_targets* targets, const float* ref_logp, float beta,
+                        float label_smoothing, int average, float* seq_logp, float* loss, void* dlogits, void* workspace,
+                        size_t workspace_bytes, void* stream);
+/* out[0] = the mean policy term over kept tokens (sequence_mean: of each sequence first, then over the sequences that keep
+ * any), out[1] = the same mean of exp(d) - d - 1, out[2] = of the tokens whose ratio is bounded.  logp [batch * seq]. */
+int mcb_policy_loss(const mcb_token_logits* logits, const mcb_token_targets* targets, const mcb_policy_terms* policy, int sequence_mean,
+                    float* logp, float* out, void* dlogits, void* workspace, size_t workspace_bytes, void* stream);
+/* loss[0] = mean over kept rows (mask, a byte each, not 0; null: all) of temperature^2 KL(q || softmax(y)) with q = softmax(teacher / temperature) over
+ * the teacher's entries. */
+int mcb_distill_loss(const mcb_token_logits* logits, const mcb_teacher_top* teacher, const uint8_t* mask, float* loss, void* dlogits,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* The stages of these losses, for a caller that produces the logits a chunk of tokens at a time (see mcb_cross_entropy_chunk):
+ * mcb_loss_weights over all rows, the _rows call for each chunk (every per-row pointer at the chunk's first row; a chunk is
+ * batch = 1, seq = its rows; terms: 3 (policy) or 1 (distillation) contiguous arrays of the CHUNK's rows), mcb_loss_sums over
+ * each; for preference pairs mcb_token_logprob_fwd per chunk, then mcb_preference_finish (coef[s]: d loss / d logp of every
+ * token of sequence s, [2 pairs]).
+ * weight [batch * seq]: a row's share of the mean, 0 where it is left out; kept are the rows of `mask`, or else of `targets`, or
+ * else all. */
+int mcb_loss_weights(const mcb_token_targets* targets, const uint8_t* mask, float* weight, int64_t batch, int64_t seq, int64_t vocab,
+                     int sequence_mean, void* stream);
+int mcb_policy_loss_rows(const mcb_token_logits* logits, const mcb_token_targets* targets, const mcb_policy_terms* policy,
+                         const float* weight, float* logp, float* terms, void* dlogits, void* stream);
+int mcb_distill_loss_rows(const mcb_token_logits* logits, const mcb_teacher_top* teacher, const float* weight, float* terms,
+                          void* dlogits, void* stream);
+/* out[i] = sum of terms[i * rows .. (i + 1) * rows), i < n <= 8, in a fixed order. */
+int mcb_loss_sums(const float* terms, int64_t rows, int n, float* out, void* stream);
+int mcb_preference_finish(const float* logp, const mcb_token_targets* targets, const float* ref_logp, float* seq_logp, float* coef,
+                          float* loss, int64_t pairs, int64_t seq, int64_t vocab, float beta, float label_smoothing, int average,
+                          void* stream);
+/* x[i, :] *= coef[i / coef_rows], in place; x [rows, D]. */
+int mcb_scale_rows(void* x, const float* coef, int64_t rows, int64_t D, int64_t coef_rows, int dtype, void* stream);
+
 /* ---- the training step as one engine ------------------------------------------------------------ */
 
 /* TrainingStep::execute (src/training/trainer.rs:368-414) over Qwen::forward (src/models/qwen.rs:95-143,236-251) for

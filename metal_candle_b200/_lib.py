@@ -70,6 +70,24 @@ class QwenLayerCall(C.Structure):
                 ("saved", C.c_void_p), ("scratch", C.c_void_p), ("saved_bytes", C.c_size_t), ("scratch_bytes", C.c_size_t)]
 
 
+class TokenLogits(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("batch", C.c_int64), ("seq", C.c_int64), ("vocab", C.c_int64), ("batch_stride", C.c_int64),
+                ("token_stride", C.c_int64), ("temperature", C.c_float), ("dtype", C.c_int32)]
+
+
+class TokenTargets(C.Structure):
+    _fields_ = [("targets", C.c_void_p), ("target_bytes", C.c_int32), ("has_ignore", C.c_int32), ("ignore_index", C.c_int64)]
+
+
+class PolicyTerms(C.Structure):
+    _fields_ = [("advantages", C.c_void_p), ("advantage_rows", C.c_int64), ("old_logp", C.c_void_p), ("ref_logp", C.c_void_p),
+                ("clip_low", C.c_float), ("clip_high", C.c_float), ("kl_coef", C.c_float), ("pad_", C.c_int32)]
+
+
+class TeacherTop(C.Structure):
+    _fields_ = [("ids", C.c_void_p), ("logits", C.c_void_p), ("top", C.c_int64), ("id_bytes", C.c_int32), ("dtype", C.c_int32)]
+
+
 _vp, _i64, _i32, _f32, _sz = C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_size_t
 
 # name -> (restype, argtypes); every symbol include/mcb200.h declares
@@ -154,6 +172,18 @@ SIGNATURES = {
     "mcb_cross_entropy_count": (_i32, [_vp, _vp, _i64, _i64, _vp]),
     "mcb_cross_entropy_chunk": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _vp]),
     "mcb_cross_entropy_finish": (_i32, [_vp, _vp, _vp, _i64, _vp]),
+    "mcb_token_logprob_fwd": (_i32, [C.POINTER(TokenLogits), C.POINTER(TokenTargets), _vp, _vp, _vp, _vp]),
+    "mcb_token_logprob_bwd": (_i32, [C.POINTER(TokenLogits), C.POINTER(TokenTargets), _vp, _vp, _vp, _i64, _vp, _vp]),
+    "mcb_token_loss_workspace_bytes": (_sz, [_i64, _i64]),
+    "mcb_preference_loss": (_i32, [C.POINTER(TokenLogits), C.POINTER(TokenTargets), _vp, _f32, _f32, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mcb_policy_loss": (_i32, [C.POINTER(TokenLogits), C.POINTER(TokenTargets), C.POINTER(PolicyTerms), _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mcb_distill_loss": (_i32, [C.POINTER(TokenLogits), C.POINTER(TeacherTop), _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mcb_loss_weights": (_i32, [C.POINTER(TokenTargets), _vp, _vp, _i64, _i64, _i64, _i32, _vp]),
+    "mcb_policy_loss_rows": (_i32, [C.POINTER(TokenLogits), C.POINTER(TokenTargets), C.POINTER(PolicyTerms), _vp, _vp, _vp, _vp, _vp]),
+    "mcb_distill_loss_rows": (_i32, [C.POINTER(TokenLogits), C.POINTER(TeacherTop), _vp, _vp, _vp, _vp]),
+    "mcb_loss_sums": (_i32, [_vp, _i64, _i32, _vp, _vp]),
+    "mcb_preference_finish": (_i32, [_vp, C.POINTER(TokenTargets), _vp, _vp, _vp, _vp, _i64, _i64, _i64, _f32, _f32, _i32, _vp]),
+    "mcb_scale_rows": (_i32, [_vp, _vp, _i64, _i64, _i64, _i32, _vp]),
     "mcb_qwen_arena_bytes": (_sz, [C.POINTER(QwenConfig), C.POINTER(QwenAdapterEntry), _i32, _i32, _i64, _i64]),
     "mcb_qwen_create": (_i32, [C.POINTER(_vp), C.POINTER(QwenConfig), C.POINTER(QwenWeights), C.POINTER(QwenAdapterEntry), _i32, _i32,
                                _f32, _vp, _sz, _vp]),

@@ -1,0 +1,164 @@
+// What the losses over the logits of given tokens share: the arguments of a row, the arithmetic of its softmax, and what each
+// loss makes of a row's log-probability.
+//
+// A row x [V] at temperature T has y = x / T, p_j = exp(y_j) / sum exp(y).  Exponentials are taken in base 2 of differences,
+// 2^((x_j - m) k) with k = log2(e) / T: exact for x_j = m whatever its magnitude, and 0 for masked logits (-inf, or the type's
+// lowest value, whose difference may overflow to -inf).  The target is kept out of the sum: with m, s over the other columns,
+// p_t / (1 - p_t) = 2^((x_t - m) k) / s, so that neither log p_t near 0 nor 1 - p_t, the gradient's factor, is a difference of
+// nearly equal numbers.
+#pragma once
+
+#include "common.cuh"
+
+namespace mcb {
+namespace tokenloss {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kMaxTeacher = 1024;   // teacher entries a row
+
+enum Op { kStats = 0, kUnit = 1, kPolicy = 2, kDistill = 3 };
+
+struct RowArgs {
+  const void* logits;      // row r starts (r / S) * batch_stride + (r % S) * token_stride elements in
+  void* grad;              // [M, V] dense, or null
+  int64_t M, S, batch_stride, token_stride;
+  int V;
+  float k, inv_t, temperature;
+  // the target of each row (kStats, kUnit, kPolicy); -1 and, with has_ignore, `ignore` leave the row out
+  const void* targets;
+  int target_bytes, has_ignore;
+  int64_t ignore;
+  const float* weight;     // kPolicy, kDistill: [M]; 0 leaves the row out, NaN marks a target out of range
+  // kPolicy
+  const float* advantages; // of row r: advantages[r / advantage_rows]
+  int64_t advantage_rows;
+  const float* old_logp;   // null: the policy that is being trained
+  const float* ref_logp;   // null: no KL term
+  float ratio_min, ratio_max, kl_coef;
+  // kDistill
+  const void* teacher_ids; // [M, K]
+  const void* teacher;     // [M, K]
+  int id_bytes, teacher_f32, K;
+  // what a row leaves behind
+  float* logp;             // [M] (kDistill: none)
+  float* lse;              // [M], or null
+  float* terms;            // kPolicy: [3, M]: loss, KL, clipped; kDistill: [M]; each times the row's weight
+};
+
+__device__ __forceinline__ int64_t row_offset(const RowArgs& a, int64_t row) {
+  const int64_t b = row / a.S;
+  return b * a.batch_stride + (row - b * a.S) * a.token_stride;
+}
+
+// The row's target, -1 where the row is left out, -2 where it is none of the vocabulary.
+__device__ __forceinline__ int read_target(const void* targets, int target_bytes, int has_ignore, int64_t ignore, int64_t row, int V) {
+  const int64_t t = target_bytes == 8 ? static_cast<const int64_t*>(targets)[row] : static_cast<const int32_t*>(targets)[row];
+  if (t == -1 || (has_ignore && t == ignore)) return -1;
+  return t >= 0 && t < V ? static_cast<int>(t) : -2;
+}
+
+// 2^x, denormal results flushed to zero (one instruction, relative error about 2^-22)
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// maximum m and sum s of 2^((x - m) k) of two sets of logits; an empty or wholly masked set is (-inf, 0), or (-inf, NaN) if it
+// holds nothing but NaN besides
+__device__ __forceinline__ void combine(float& m, float& s, float m2, float s2, float k) {
+  const float mm = fmaxf(m, m2);
+  if (mm == -INFINITY) { s += s2; return; }
+  s = s * ex2((m - mm) * k) + s2 * ex2((m2 - mm) * k);
+  m = mm;
+}
+
+// A row's softmax around its target: (m, s) are those of the other columns.
+struct TargetStats {
+  float top, sum;       // of the whole row
+  float logp, rest;     // log p_t and 1 - p_t
+};
+__device__ __forceinline__ TargetStats target_stats(float m, float s, float xt, float k) {
+  TargetStats r;
+  if (m == -INFINITY && s == 0.0f) {   // nothing but the target (which, masked itself, has no probability: NaN)
+    r.top = xt; r.sum = 1.0f; r.rest = 0.0f;
+    r.logp = xt - xt;
+    return r;
+  }
+  const float d = (m - xt) * k;
+  if (d <= 0.0f) {
+    const float odds = s * exp2f(d);
+    r.top = xt; r.sum = 1.0f + odds;
+    r.logp = -log1pf(odds);
+    r.rest = odds / r.sum;
+  } else {   // (NaN as well)
+    r.top = m; r.sum = s + exp2f(-d);
+    r.logp = -d * kLn2 - logf(r.sum);
+    r.rest = s / r.sum;
+  }
+  return r;
+}
+
+// The clipped policy term of one token and its derivative towards logp, and what is reported of it.
+struct PolicyTerm {
+  float loss, dlogp, kl, clipped;
+};
+__device__ __forceinline__ PolicyTerm policy_term(const RowArgs& a, int64_t row, float logp) {
+  const float adv = a.advantages[row / a.advantage_rows];
+  const float ratio = a.old_logp != nullptr ? expf(logp - a.old_logp[row]) : 1.0f;
+  const float bounded = fminf(fmaxf(ratio, a.ratio_min), a.ratio_max);
+  PolicyTerm t;
+  // min(r A, clip(r) A): the bound holds only where it makes the term smaller
+  const bool bound = adv >= 0.0f ? ratio > a.ratio_max : ratio < a.ratio_min;
+  t.loss = -(bound ? bounded : ratio) * adv;
+  t.dlogp = bound ? 0.0f : -adv * ratio;
+  t.clipped = bound ? 1.0f : 0.0f;
+  t.kl = 0.0f;
+  if (a.ref_logp != nullptr) {
+    // exp(d) - d - 1 >= 0 with d = ref - logp: an estimate of KL(policy || reference) that is never negative
+    const float d = a.ref_logp[row] - logp;
+    const float e = expm1f(d);
+    t.kl = e - d;
+    t.loss += a.kl_coef * t.kl;
+    t.dlogp -= a.kl_coef * e;
+  }
+  return t;
+}
+
+// What a row's log-probability comes to: writes the row's outputs (`write`: by one thread) and returns d loss / d logp / T.
+template <int OP>
+__device__ __forceinline__ float finish_target_row(const RowArgs& a, int64_t row, const TargetStats& r, bool write) {
+  if (write && a.logp != nullptr) a.logp[row] = r.logp;
+  if (write && a.lse != nullptr) a.lse[row] = r.top * a.inv_t + logf(r.sum);
+  if constexpr (OP == kPolicy) {
+    const float w = a.weight[row];
+    const PolicyTerm t = policy_term(a, row, r.logp);
+    if (write) {
+      a.terms[row] = w * t.loss;
+      a.terms[a.M + row] = w * t.kl;
+      a.terms[2 * a.M + row] = w * t.clipped;
+    }
+    return w * t.dlogp * a.inv_t;
+  }
+  return a.inv_t;
+}
+
+// A row that is left out (value 0) or whose target is out of range (NaN).
+template <int OP>
+__device__ __forceinline__ void write_left_out(const RowArgs& a, int64_t row, float value) {
+  if (a.logp != nullptr) a.logp[row] = value;
+  if (a.lse != nullptr) a.lse[row] = value;
+  if constexpr (OP == kPolicy) { a.terms[row] = value; a.terms[a.M + row] = value; a.terms[2 * a.M + row] = value; }
+  if constexpr (OP == kDistill) a.terms[row] = value;
+}
+
+__device__ __forceinline__ float read_teacher(const RowArgs& a, int64_t i) {
+  return a.teacher_f32 ? static_cast<const float*>(a.teacher)[i] : to_f32(static_cast<const __nv_bfloat16*>(a.teacher)[i]);
+}
+__device__ __forceinline__ int64_t read_teacher_id(const RowArgs& a, int64_t i) {
+  return a.id_bytes == 8 ? static_cast<const int64_t*>(a.teacher_ids)[i] : static_cast<const int32_t*>(a.teacher_ids)[i];
+}
+
+}  // namespace tokenloss
+}  // namespace mcb

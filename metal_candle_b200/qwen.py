@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from contextlib import contextmanager
 from dataclasses import dataclass
 from typing import Dict, List, Optional, Tuple
 
@@ -23,7 +24,8 @@ import torch
 
 from . import _lib, backend
 from .backend import TrainingError, _ptr, _stream
-from .training import LoRAAdapter, LoRALayer, TargetModule
+from .training import (IGNORE_INDEX, LoRAAdapter, LoRALayer, PolicyLoss, PreferenceLoss, TargetModule, _check_like, _check_preference,
+                       _check_temperature, _FLOATS, _INTEGERS, _policy_terms, _teacher_top, _token_targets)
 
 
 @dataclass
@@ -499,52 +501,224 @@ class Qwen:
         c = self.config
         B, S = input_ids.shape
         M = B * S
-        ids32 = input_ids.to(torch.int32).contiguous().view(-1)
         tgt32 = target_ids.to(torch.int32).contiguous().view(-1)  # u32::MAX wraps to -1 = ignored
-        h = self._embed(ids32)
-        saved = []
-        calls = _LayerCalls(self, B, S, backward=True)
-        for idx in range(len(self.layers)):
-            h, sv = self._layer_fwd(h, idx, B, S, True, calls)
-            saved.append(sv)
-        nf = self._norm(h, self.norm)
+        run = self._forward_saved(input_ids)
+        nf = run["nf"]
         nll = torch.empty(M, dtype=torch.float32, device=self.device)
         count = torch.empty(1, dtype=torch.int32, device=self.device)
         loss = torch.empty(2, dtype=torch.float32, device=self.device)
-        chunk = self.ce_chunk_tokens
-        if chunk == 0:
-            chunk = int(self.lib.mcb_ce_chunk_tokens(M, c.hidden_size))
-        if chunk is None or chunk >= M:
+        chunk = self._chunk_tokens(M)
+        if chunk >= M:
             logits, _ = self._lin(nf, self.lm_head, False)
             _lib.check(self.lib.mcb_cross_entropy(_ptr(logits), _ptr(tgt32), _ptr(nll), _ptr(count), _ptr(loss), M,
                                                   c.vocab_size, 1, self.dt, _stream()))
-            dnf = self._lin_bwd(nf, self.lm_head, logits, None, None, False)
+            run["dnf"] = self._lin_bwd(nf, self.lm_head, logits, None, None, False)
             del logits
         else:
             # lm_head, loss and lm_head backward one chunk of tokens at a time (cross_entropy_loss,
             # src/training/loss.rs:58-147, over logits that never exist for the whole batch)
             _lib.check(self.lib.mcb_cross_entropy_count(_ptr(tgt32), _ptr(count), M, c.vocab_size, _stream()))
-            dnf = torch.empty_like(nf)
-            for c0 in range(0, M, chunk):
-                c1 = min(M, c0 + chunk)
-                logits, _ = self._lin(nf[c0:c1], self.lm_head, False)
+
+            def rows(logits, c0, c1):
                 _lib.check(self.lib.mcb_cross_entropy_chunk(_ptr(logits), _ptr(tgt32[c0:c1]), _ptr(nll[c0:c1]), _ptr(count),
                                                             c1 - c0, c.vocab_size, 1, self.dt, _stream()))
-                backend.lora_linear_backward(None, self.lm_head.weight_t, None, None, 1.0, logits, dx_out=dnf[c0:c1])
-                del logits
+
+            run["dnf"] = self._head_by_chunks(nf, rows)
             _lib.check(self.lib.mcb_cross_entropy_finish(_ptr(nll), _ptr(count), _ptr(loss), M, _stream()))
         self.last_count = count
-        # backward
-        dh, _ = backend.rms_norm_backward(h, self.norm, dnf, c.rms_norm_eps, need_dw=False)
-        del dnf
+        self._backward_saved(run, accumulate)
+        return loss[:1], self._grad_views
+
+    def _forward_saved(self, input_ids: torch.Tensor) -> dict:
+        """The pass up to the final norm, with what the backward pass needs of it."""
+        B, S = input_ids.shape
+        h = self._embed(input_ids.to(torch.int32).contiguous().view(-1))
+        saved = []
+        calls = _LayerCalls(self, B, S, backward=True)
+        for idx in range(len(self.layers)):
+            h, sv = self._layer_fwd(h, idx, B, S, True, calls)
+            saved.append(sv)
+        return dict(B=B, S=S, calls=calls, saved=saved, h=h, nf=self._norm(h, self.norm))
+
+    def _chunk_tokens(self, M: int) -> int:
+        """Tokens per chunk of the lm_head stage (`ce_chunk_tokens`)."""
+        chunk = self.ce_chunk_tokens
+        if chunk == 0:
+            chunk = int(self.lib.mcb_ce_chunk_tokens(M, self.config.hidden_size))
+        return M if chunk is None else min(chunk, M)
+
+    def _head_by_chunks(self, nf: torch.Tensor, rows) -> torch.Tensor:
+        """lm_head, `rows(logits, first, last)`, which turns a chunk's logits into their gradient in place, and the lm_head's
+        backward: the gradient of `nf`."""
+        M = nf.shape[0]
+        chunk = self._chunk_tokens(M)
+        dnf = torch.empty_like(nf)
+        for c0 in range(0, M, chunk):
+            c1 = min(M, c0 + chunk)
+            logits, _ = self._lin(nf[c0:c1], self.lm_head, False)
+            rows(logits, c0, c1)
+            backend.lora_linear_backward(None, self.lm_head.weight_t, None, None, 1.0, logits, dx_out=dnf[c0:c1])
+            del logits
+        return dnf
+
+    def _backward_saved(self, run: dict, accumulate: bool) -> None:
+        """From the gradient of the final norm's output, run["dnf"], to the adapters' gradients."""
+        dh, _ = backend.rms_norm_backward(run["h"], self.norm, run.pop("dnf"), self.config.rms_norm_eps, need_dw=False)
+        saved = run["saved"]
         for idx in range(len(self.layers) - 1, -1, -1):
-            dh = self._layer_bwd(dh, saved[idx], idx, B, S, accumulate, calls)
+            dh = self._layer_bwd(dh, saved[idx], idx, run["B"], run["S"], accumulate, run["calls"])
             saved[idx] = None
             if self.layer_done_hook is not None:
                 self.layer_done_hook(idx)
         if self.backward_done_hook is not None:
             self.backward_done_hook()
-        return loss[:1], self._grad_views
+
+    # -- post-training losses: the same pass with another loss between the lm_head and its backward --
+    @contextmanager
+    def adapter_disabled(self):
+        """The base model for the time of a `with` block: the frozen reference of a preference or policy loss."""
+        lins = [L[m] for L in self.layers for m in self.MODULES]
+        loras = [lin.lora for lin in lins]
+        try:
+            for lin in lins:
+                lin.lora = None
+            yield self
+        finally:
+            for lin, lora in zip(lins, loras):
+                lin.lora = lora
+
+    def _chunk_rows(self, logits: torch.Tensor, temperature: float):
+        n, V = logits.shape
+        return _lib.TokenLogits(logits.data_ptr(), 1, n, V, n * V, V, float(temperature), self.dt)
+
+    def _checked(self, t: torch.Tensor, what: str, shape, dtypes):
+        return _check_like(self.embed_tokens, t, what, shape, dtypes)
+
+    def token_log_probs(self, input_ids: torch.Tensor, target_ids: torch.Tensor, ignore_index: int = IGNORE_INDEX,
+                        temperature: float = 1.0) -> torch.Tensor:
+        """`training.token_log_probs` of the model's logits, [batch, seq] float32, without a backward pass; the logits exist a
+        chunk of tokens at a time."""
+        B, S = input_ids.shape
+        M = B * S
+        targets = self._checked(target_ids, "target_ids", (B, S), _INTEGERS).view(M)
+        _check_temperature(temperature)
+        h = self._embed(input_ids.to(torch.int32).contiguous().view(-1))
+        calls = _LayerCalls(self, B, S, backward=False)
+        for idx in range(len(self.layers)):
+            h, _ = self._layer_fwd(h, idx, B, S, False, calls)
+        nf = self._norm(h, self.norm)
+        logp = torch.empty(M, dtype=torch.float32, device=self.device)
+        chunk = self._chunk_tokens(M)
+        for c0 in range(0, M, chunk):
+            c1 = min(M, c0 + chunk)
+            logits, _ = self._lin(nf[c0:c1], self.lm_head, False)
+            _lib.check(self.lib.mcb_token_logprob_fwd(self._chunk_rows(logits, temperature), _token_targets(targets[c0:c1], ignore_index),
+                                                      _ptr(logp[c0:c1]), None, None, _stream()))
+            del logits
+        return logp.view(B, S)
+
+    def _need_adapter(self, what: str) -> None:
+        if self.lora_adapter is None:
+            raise TrainingError(f"{what} needs an adapter (apply_adapter)")
+
+    def preference_forward_backward(self, input_ids: torch.Tensor, target_ids: torch.Tensor, ref_log_probs: torch.Tensor, beta: float = 0.1,
+                                    label_smoothing: float = 0.0, average_log_probs: bool = False, ignore_index: int = IGNORE_INDEX,
+                                    accumulate: bool = False):
+        """`training.preference_loss` over the model's logits with the adapters' gradients: (PreferenceLoss without grad,
+        gradients).  The coefficient of a token's gradient is known once the whole pair has been seen, and is the same for a
+        sequence: each chunk's logits become d logp / d logits in place, and the coefficients scale the rows of the final norm's
+        gradient, 170 times narrower than the logits, when the last chunk is done."""
+        self._need_adapter("preference_forward_backward")
+        B, S = input_ids.shape
+        M = B * S
+        if B % 2 != 0:
+            raise TrainingError(f"a batch of {B} sequences holds no pairs (the chosen sequences, then the rejected ones)")
+        _check_preference(beta, label_smoothing)
+        targets = self._checked(target_ids, "target_ids", (B, S), _INTEGERS).view(M)
+        ref = self._checked(ref_log_probs, "ref_log_probs", (B,), _FLOATS)
+        run = self._forward_saved(input_ids)
+        logp = torch.empty(M, dtype=torch.float32, device=self.device)
+        out = torch.empty(2 * B + 1, dtype=torch.float32, device=self.device)
+        seq_logp, coef = out[1:B + 1], out[B + 1:]
+
+        def rows(logits, c0, c1):
+            _lib.check(self.lib.mcb_token_logprob_fwd(self._chunk_rows(logits, 1.0), _token_targets(targets[c0:c1], ignore_index),
+                                                      _ptr(logp[c0:c1]), None, _ptr(logits), _stream()))
+
+        run["dnf"] = self._head_by_chunks(run["nf"], rows)
+        _lib.check(self.lib.mcb_preference_finish(_ptr(logp), _token_targets(targets, ignore_index), _ptr(ref), _ptr(seq_logp), _ptr(coef),
+                                                  _ptr(out), B // 2, S, self.config.vocab_size, float(beta), float(label_smoothing),
+                                                  int(bool(average_log_probs)), _stream()))
+        _lib.check(self.lib.mcb_scale_rows(_ptr(run["dnf"]), _ptr(coef), M, self.config.hidden_size, S, self.dt, _stream()))
+        self._backward_saved(run, accumulate)
+        return PreferenceLoss(out[:1], seq_logp, None), self._grad_views
+
+    def policy_forward_backward(self, input_ids: torch.Tensor, target_ids: torch.Tensor, advantages: torch.Tensor,
+                                old_log_probs: Optional[torch.Tensor] = None, ref_log_probs: Optional[torch.Tensor] = None, clip_low: float = 0.2,
+                                clip_high: float = 0.2, kl_coef: float = 0.0, temperature: float = 1.0, sequence_mean: bool = False,
+                                ignore_index: int = IGNORE_INDEX, accumulate: bool = False):
+        """`training.policy_loss` over the model's logits with the adapters' gradients: (PolicyLoss without grad, gradients)."""
+        self._need_adapter("policy_forward_backward")
+        B, S = input_ids.shape
+        M, V = B * S, self.config.vocab_size
+        targets = self._checked(target_ids, "target_ids", (B, S), _INTEGERS).view(M)
+        _check_temperature(temperature)
+        (adv, old, ref), _ = _policy_terms(self.embed_tokens, (B, S), advantages, old_log_probs, ref_log_probs, clip_low, clip_high, kl_coef)
+        adv = (adv if adv.dim() == 2 else adv[:, None].expand(B, S).contiguous()).view(M)   # a chunk may begin inside a sequence
+        old, ref = (None if t is None else t.view(M) for t in (old, ref))
+        run = self._forward_saved(input_ids)
+        weight = torch.empty(M, dtype=torch.float32, device=self.device)
+        logp = torch.empty(M, dtype=torch.float32, device=self.device)
+        parts = []
+        _lib.check(self.lib.mcb_loss_weights(_token_targets(targets, ignore_index), None, _ptr(weight), B, S, V, int(bool(sequence_mean)),
+                                             _stream()))
+
+        def rows(logits, c0, c1):
+            terms = _lib.PolicyTerms(_ptr(adv[c0:c1]), 1, None if old is None else _ptr(old[c0:c1]), None if ref is None else _ptr(ref[c0:c1]),
+                                     float(clip_low), float(clip_high), float(kl_coef), 0)
+            each = torch.empty(3, c1 - c0, dtype=torch.float32, device=self.device)
+            _lib.check(self.lib.mcb_policy_loss_rows(self._chunk_rows(logits, temperature), _token_targets(targets[c0:c1], ignore_index), terms,
+                                                     _ptr(weight[c0:c1]), _ptr(logp[c0:c1]), _ptr(each), _ptr(logits), _stream()))
+            parts.append(each)
+
+        run["dnf"] = self._head_by_chunks(run["nf"], rows)
+        out = self._sum_terms(parts, 3)
+        self._backward_saved(run, accumulate)
+        return PolicyLoss(out[0:1], logp.view(B, S), out[1:2], out[2:3], None), self._grad_views
+
+    def distillation_forward_backward(self, input_ids: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
+                                      mask: Optional[torch.Tensor] = None, temperature: float = 1.0, accumulate: bool = False):
+        """`training.distillation_loss` over the model's logits with the adapters' gradients: (loss, gradients)."""
+        self._need_adapter("distillation_forward_backward")
+        B, S = input_ids.shape
+        M, V = B * S, self.config.vocab_size
+        _check_temperature(temperature)
+        (ids, tl, mask), teacher = _teacher_top(self.embed_tokens, (B, S), teacher_ids, teacher_logits, mask)
+        K = ids.shape[2]
+        ids, tl = ids.view(M, K), tl.view(M, K)
+        run = self._forward_saved(input_ids)
+        weight = torch.empty(M, dtype=torch.float32, device=self.device)
+        parts = []
+        _lib.check(self.lib.mcb_loss_weights(None, _ptr(mask), _ptr(weight), B, S, V, 0, _stream()))
+
+        def rows(logits, c0, c1):
+            part = _lib.TeacherTop(_ptr(ids[c0:c1]), _ptr(tl[c0:c1]), K, teacher.id_bytes, teacher.dtype)
+            each = torch.empty(1, c1 - c0, dtype=torch.float32, device=self.device)
+            _lib.check(self.lib.mcb_distill_loss_rows(self._chunk_rows(logits, temperature), part, _ptr(weight[c0:c1]), _ptr(each), _ptr(logits),
+                                                      _stream()))
+            parts.append(each)
+
+        run["dnf"] = self._head_by_chunks(run["nf"], rows)
+        out = self._sum_terms(parts, 1)
+        self._backward_saved(run, accumulate)
+        return out, self._grad_views
+
+    def _sum_terms(self, parts, n: int) -> torch.Tensor:
+        """The chunks' terms, [n, rows] each, summed: [n] float32."""
+        each = parts[0] if len(parts) == 1 else torch.cat(parts, 1)
+        out = torch.empty(n, dtype=torch.float32, device=self.device)
+        _lib.check(self.lib.mcb_loss_sums(_ptr(each), each.shape[1], n, _ptr(out), _stream()))
+        return out
 
     def capture_forward_backward(self, batch: int, seq: int, keep_hooks: bool = False, pool=None) -> "CapturedStep":
         """Records forward_backward for one (batch, seq) shape into a CUDA graph.  The step is some thousand

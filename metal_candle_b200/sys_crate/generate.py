@@ -23,7 +23,8 @@ TYPES = {
     "size_t": "usize", "char": "c_char", "mcb_adamw_tensor": "mcb_adamw_tensor", "mcb_comm": "mcb_comm",
     "mcb_lora_segment": "mcb_lora_segment", "mcb_qwen": "mcb_qwen", "mcb_qwen_config": "mcb_qwen_config",
     "mcb_qwen_weights": "mcb_qwen_weights", "mcb_qwen_adapter_entry": "mcb_qwen_adapter_entry",
-    "mcb_qwen_layer_call": "mcb_qwen_layer_call",
+    "mcb_qwen_layer_call": "mcb_qwen_layer_call", "uint8_t": "u8", "mcb_token_logits": "mcb_token_logits",
+    "mcb_token_targets": "mcb_token_targets", "mcb_policy_terms": "mcb_policy_terms", "mcb_teacher_top": "mcb_teacher_top",
 }
 
 
@@ -188,6 +189,55 @@ def render(consts, funcs) -> str:
         "    pub scratch: *mut c_void,",
         "    pub saved_bytes: usize,",
         "    pub scratch_bytes: usize,",
+        "}",
+        "",
+        "/// Rows of logits of the token losses (`mcb_token_logprob_*`, `mcb_preference_loss`, ...; host memory).",
+        "#[repr(C)]",
+        "#[derive(Debug, Clone, Copy)]",
+        "pub struct mcb_token_logits {",
+        "    pub logits: *const c_void,",
+        "    pub batch: i64,",
+        "    pub seq: i64,",
+        "    pub vocab: i64,",
+        "    pub batch_stride: i64,",
+        "    pub token_stride: i64,",
+        "    pub temperature: f32,",
+        "    pub dtype: i32,",
+        "}",
+        "",
+        "/// Their target tokens.",
+        "#[repr(C)]",
+        "#[derive(Debug, Clone, Copy)]",
+        "pub struct mcb_token_targets {",
+        "    pub targets: *const c_void,",
+        "    pub target_bytes: i32,",
+        "    pub has_ignore: i32,",
+        "    pub ignore_index: i64,",
+        "}",
+        "",
+        "/// What the clipped policy loss compares with.",
+        "#[repr(C)]",
+        "#[derive(Debug, Clone, Copy)]",
+        "pub struct mcb_policy_terms {",
+        "    pub advantages: *const f32,",
+        "    pub advantage_rows: i64,",
+        "    pub old_logp: *const f32,",
+        "    pub ref_logp: *const f32,",
+        "    pub clip_low: f32,",
+        "    pub clip_high: f32,",
+        "    pub kl_coef: f32,",
+        "    pub pad_: i32,",
+        "}",
+        "",
+        "/// A teacher's largest logits of each row.",
+        "#[repr(C)]",
+        "#[derive(Debug, Clone, Copy)]",
+        "pub struct mcb_teacher_top {",
+        "    pub ids: *const c_void,",
+        "    pub logits: *const c_void,",
+        "    pub top: i64,",
+        "    pub id_bytes: i32,",
+        "    pub dtype: i32,",
         "}",
         "",
         "/// Opaque training-step engine (`mcb_qwen_*`).",

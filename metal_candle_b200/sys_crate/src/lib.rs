@@ -131,6 +131,55 @@ pub struct mcb_qwen_layer_call {
     pub scratch_bytes: usize,
 }
 
+/// Rows of logits of the token losses (`mcb_token_logprob_*`, `mcb_preference_loss`, ...; host memory).
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct mcb_token_logits {
+    pub logits: *const c_void,
+    pub batch: i64,
+    pub seq: i64,
+    pub vocab: i64,
+    pub batch_stride: i64,
+    pub token_stride: i64,
+    pub temperature: f32,
+    pub dtype: i32,
+}
+
+/// Their target tokens.
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct mcb_token_targets {
+    pub targets: *const c_void,
+    pub target_bytes: i32,
+    pub has_ignore: i32,
+    pub ignore_index: i64,
+}
+
+/// What the clipped policy loss compares with.
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct mcb_policy_terms {
+    pub advantages: *const f32,
+    pub advantage_rows: i64,
+    pub old_logp: *const f32,
+    pub ref_logp: *const f32,
+    pub clip_low: f32,
+    pub clip_high: f32,
+    pub kl_coef: f32,
+    pub pad_: i32,
+}
+
+/// A teacher's largest logits of each row.
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct mcb_teacher_top {
+    pub ids: *const c_void,
+    pub logits: *const c_void,
+    pub top: i64,
+    pub id_bytes: i32,
+    pub dtype: i32,
+}
+
 /// Opaque training-step engine (`mcb_qwen_*`).
 #[repr(C)]
 pub struct mcb_qwen {
@@ -213,6 +262,18 @@ extern "C" {
     pub fn mcb_cross_entropy_count(targets: *const i32, count: *mut i32, M: i64, V: i64, stream: *mut c_void) -> c_int;
     pub fn mcb_cross_entropy_chunk(logits: *mut c_void, targets: *const i32, nll: *mut f32, count: *const i32, rows: i64, V: i64, write_grad: c_int, dtype: c_int, stream: *mut c_void) -> c_int;
     pub fn mcb_cross_entropy_finish(nll: *const f32, count: *const i32, loss: *mut f32, M: i64, stream: *mut c_void) -> c_int;
+    pub fn mcb_token_logprob_fwd(logits: *const mcb_token_logits, targets: *const mcb_token_targets, logp: *mut f32, lse: *mut f32, unit_grad: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn mcb_token_logprob_bwd(logits: *const mcb_token_logits, targets: *const mcb_token_targets, logp: *const f32, lse: *const f32, dlogp: *const f32, dlogp_rows: i64, dlogits: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn mcb_token_loss_workspace_bytes(batch: i64, seq: i64) -> usize;
+    pub fn mcb_preference_loss(logits: *const mcb_token_logits, targets: *const mcb_token_targets, ref_logp: *const f32, beta: f32, label_smoothing: f32, average: c_int, seq_logp: *mut f32, loss: *mut f32, dlogits: *mut c_void, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn mcb_policy_loss(logits: *const mcb_token_logits, targets: *const mcb_token_targets, policy: *const mcb_policy_terms, sequence_mean: c_int, logp: *mut f32, out: *mut f32, dlogits: *mut c_void, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn mcb_distill_loss(logits: *const mcb_token_logits, teacher: *const mcb_teacher_top, mask: *const u8, loss: *mut f32, dlogits: *mut c_void, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn mcb_loss_weights(targets: *const mcb_token_targets, mask: *const u8, weight: *mut f32, batch: i64, seq: i64, vocab: i64, sequence_mean: c_int, stream: *mut c_void) -> c_int;
+    pub fn mcb_policy_loss_rows(logits: *const mcb_token_logits, targets: *const mcb_token_targets, policy: *const mcb_policy_terms, weight: *const f32, logp: *mut f32, terms: *mut f32, dlogits: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn mcb_distill_loss_rows(logits: *const mcb_token_logits, teacher: *const mcb_teacher_top, weight: *const f32, terms: *mut f32, dlogits: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn mcb_loss_sums(terms: *const f32, rows: i64, n: c_int, out: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn mcb_preference_finish(logp: *const f32, targets: *const mcb_token_targets, ref_logp: *const f32, seq_logp: *mut f32, coef: *mut f32, loss: *mut f32, pairs: i64, seq: i64, vocab: i64, beta: f32, label_smoothing: f32, average: c_int, stream: *mut c_void) -> c_int;
+    pub fn mcb_scale_rows(x: *mut c_void, coef: *const f32, rows: i64, D: i64, coef_rows: i64, dtype: c_int, stream: *mut c_void) -> c_int;
     pub fn mcb_qwen_arena_bytes(cfg: *const mcb_qwen_config, adapters: *const mcb_qwen_adapter_entry, n_adapters: c_int, rank: c_int, batch: i64, seq: i64) -> usize;
     pub fn mcb_qwen_create(out: *mut *mut mcb_qwen, cfg: *const mcb_qwen_config, weights: *const mcb_qwen_weights, adapters: *const mcb_qwen_adapter_entry, n_adapters: c_int, rank: c_int, scale: f32, arena: *mut c_void, arena_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn mcb_qwen_set_exchange(q: *mut mcb_qwen, comm: *mut mcb_comm, side_stream: *mut c_void, grad_flat: *mut f32, bucket_lo: *const i64, bucket_hi: *const i64, bucket_first_layer: *const c_int, n_buckets: c_int) -> c_int;

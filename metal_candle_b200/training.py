@@ -11,7 +11,7 @@ import struct
 import threading
 from dataclasses import dataclass, field
 from enum import Enum
-from typing import Callable, Dict, Iterable, List, Optional, Tuple
+from typing import Callable, Dict, Iterable, List, NamedTuple, Optional, Tuple
 
 import numpy as np
 import torch
@@ -499,6 +499,215 @@ def cross_entropy_loss(logits: torch.Tensor, targets: torch.Tensor, ignore_index
     if kept == 0:
         raise InvalidConfig("all tokens are ignored, cannot compute loss")
     return (loss[:1], grad) if return_grad else loss[:1]
+
+
+# ---------------------------------------------------------------------------------------------
+# losses over the logits of given tokens
+# ---------------------------------------------------------------------------------------------
+#
+# Post-training beside `cross_entropy_loss`, with its conventions: logits [batch, seq, vocab] (float32 or bfloat16, any
+# strides between rows), targets [batch, seq] integer, explicit gradients instead of autograd (`return_grad`), the logits left
+# untouched.  A target of -1 or `ignore_index` leaves its position out; another one outside the vocabulary makes the loss and that
+# position's outputs NaN.  Nothing waits for the device and nothing is checked there, so every call can be captured into a
+# CUDA graph.  With all positions left out the loss is 0.  `temperature` divides the logits.
+
+class PreferenceLoss(NamedTuple):
+    loss: torch.Tensor                  # [1] float32
+    log_probs: torch.Tensor             # [2 * pairs] float32: the policy's log-probability of each sequence
+    grad: Optional[torch.Tensor]        # d loss / d logits
+
+
+class PolicyLoss(NamedTuple):
+    loss: torch.Tensor                  # [1] float32
+    log_probs: torch.Tensor             # [batch, seq] float32
+    kl: torch.Tensor                    # [1] float32: mean of exp(ref - logp) - (ref - logp) - 1; 0 without a reference
+    clip_fraction: torch.Tensor         # [1] float32: share of the tokens whose ratio the clipping bounds
+    grad: Optional[torch.Tensor]
+
+
+def _on_device(t: torch.Tensor):
+    """The tensor's device as the current one: calls go to that device's current stream."""
+    if not t.is_cuda:
+        raise TrainingError("tensor is not on a CUDA device (this library has no CPU path)")
+    return torch.cuda.device(t.device)
+
+
+def _check_logits(logits: torch.Tensor) -> torch.Tensor:
+    if logits.dim() != 3:
+        raise InvalidConfig(f"logits must be 3D (batch, seq_len, vocab_size), got shape {list(logits.shape)}")
+    if logits.numel() == 0:
+        raise InvalidConfig(f"logits of shape {list(logits.shape)} are empty")
+    backend._dtype_code(logits)
+    return logits if logits.stride(2) == 1 else logits.contiguous()
+
+
+def _check_like(logits: torch.Tensor, t: torch.Tensor, what: str, shape, dtypes) -> torch.Tensor:
+    if t.device != logits.device:
+        raise TrainingError(f"{what} is on {t.device}, the logits are on {logits.device}")
+    if tuple(t.shape) != tuple(shape):
+        raise InvalidConfig(f"{what} must have shape {list(shape)}, got {list(t.shape)}")
+    if t.dtype not in dtypes:
+        raise TrainingError(f"{what} is {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
+    return t.contiguous()
+
+
+_INTEGERS, _FLOATS = (torch.int64, torch.int32), (torch.float32,)
+
+
+def _check_temperature(temperature: float) -> None:
+    if not 1e-6 <= temperature <= 1e6:
+        raise InvalidConfig(f"temperature must be positive and finite (1e-6 to 1e6), got {temperature}")
+
+
+def _token_logits(logits: torch.Tensor, temperature: float):
+    _check_temperature(temperature)
+    B, S, V = logits.shape
+    return _lib.TokenLogits(logits.data_ptr(), B, S, V, logits.stride(0), logits.stride(1), float(temperature), backend._dtype_code(logits))
+
+
+def _token_targets(targets: torch.Tensor, ignore_index: Optional[int]):
+    return _lib.TokenTargets(targets.data_ptr(), targets.element_size(), int(ignore_index is not None), int(ignore_index or 0))
+
+
+def _new_grad(logits: torch.Tensor, wanted: bool) -> Optional[torch.Tensor]:
+    return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if wanted else None
+
+
+def token_log_probs(logits: torch.Tensor, targets: torch.Tensor, ignore_index: Optional[int] = None, temperature: float = 1.0):
+    """log softmax(logits / temperature)[target] and the log-sum-exp of every position: two float32 tensors [batch, seq], 0 where
+    the position is left out."""
+    x = _check_logits(logits)
+    B, S, _ = x.shape
+    t = _check_like(x, targets, "targets", (B, S), _INTEGERS)
+    rows = _token_logits(x, temperature)
+    with _on_device(x):
+        out = torch.empty(2, B, S, dtype=torch.float32, device=x.device)
+        _lib.check(backend._lib_for(x).mcb_token_logprob_fwd(rows, _token_targets(t, ignore_index), out[0].data_ptr(),
+                                                             out[1].data_ptr(), None, backend._stream()))
+    return out[0], out[1]
+
+
+def token_log_probs_backward(logits: torch.Tensor, targets: torch.Tensor, log_probs: torch.Tensor, lse: torch.Tensor, dlogp: torch.Tensor,
+                             ignore_index: Optional[int] = None, temperature: float = 1.0) -> torch.Tensor:
+    """d / d logits of `token_log_probs` given d / d log_probs [batch, seq] float32; log_probs and lse as the forward returned
+    them, for the same logits, targets and temperature."""
+    x = _check_logits(logits)
+    B, S, _ = x.shape
+    t = _check_like(x, targets, "targets", (B, S), _INTEGERS)
+    log_probs, lse, dlogp = (_check_like(x, v, n, (B, S), _FLOATS) for v, n in ((log_probs, "log_probs"), (lse, "lse"), (dlogp, "dlogp")))
+    rows = _token_logits(x, temperature)
+    with _on_device(x):
+        grad = _new_grad(x, True)
+        _lib.check(backend._lib_for(x).mcb_token_logprob_bwd(rows, _token_targets(t, ignore_index), log_probs.data_ptr(),
+                                                             lse.data_ptr(), dlogp.data_ptr(), 1, grad.data_ptr(), backend._stream()))
+    return grad
+
+
+def _check_preference(beta: float, label_smoothing: float) -> None:
+    if not 0.0 < beta < math.inf:
+        raise InvalidConfig(f"beta must be positive and finite, got {beta}")
+    if not 0.0 <= label_smoothing <= 0.5:
+        raise InvalidConfig(f"label_smoothing must be in [0, 0.5], got {label_smoothing}")
+
+
+def preference_loss(logits: torch.Tensor, targets: torch.Tensor, ref_log_probs: torch.Tensor, beta: float = 0.1, label_smoothing: float = 0.0,
+                    average_log_probs: bool = False, ignore_index: Optional[int] = None, return_grad: bool = False) -> PreferenceLoss:
+    """Preference loss of paired log ratios.  The batch holds the chosen sequences first, then the rejected one of each pair in the
+    same order; L is the sum of a sequence's token log-probabilities (average_log_probs: the mean) and ref_log_probs [batch]
+    the frozen reference's, taken the same way.  With z = beta ((L_c - ref_c) - (L_r - ref_r)) the loss is the mean over pairs of
+    -(1 - label_smoothing) log sigmoid(z) - label_smoothing log sigmoid(-z)."""
+    x = _check_logits(logits)
+    B, S, _ = x.shape
+    if B % 2 != 0:
+        raise InvalidConfig(f"a batch of {B} sequences holds no pairs (the chosen sequences, then the rejected ones)")
+    _check_preference(beta, label_smoothing)
+    t = _check_like(x, targets, "targets", (B, S), _INTEGERS)
+    ref = _check_like(x, ref_log_probs, "ref_log_probs", (B,), _FLOATS)
+    with _on_device(x):
+        lib = backend._lib_for(x)
+        grad = _new_grad(x, return_grad)
+        out = torch.empty(B + 1, dtype=torch.float32, device=x.device)
+        ws = backend.workspace(x.device, lib.mcb_token_loss_workspace_bytes(B, S))
+        _lib.check(lib.mcb_preference_loss(_token_logits(x, 1.0), _token_targets(t, ignore_index), ref.data_ptr(), float(beta), float(label_smoothing),
+                                           int(bool(average_log_probs)), out[1:].data_ptr(), out.data_ptr(), backend._ptr(grad), ws.data_ptr(),
+                                           ws.numel(), backend._stream()))
+    return PreferenceLoss(out[:1], out[1:], grad)
+
+
+def _policy_terms(x, shape, advantages, old_log_probs, ref_log_probs, clip_low, clip_high, kl_coef):
+    """The checked tensors (kept alive by the caller) and the library's descriptor of them."""
+    if not (0.0 <= clip_low < math.inf and 0.0 <= clip_high < math.inf):
+        raise InvalidConfig(f"clip_low and clip_high must be finite and not negative, got {clip_low} and {clip_high}")
+    if not 0.0 <= kl_coef < math.inf:
+        raise InvalidConfig(f"kl_coef must be finite and not negative, got {kl_coef}")
+    if kl_coef > 0.0 and ref_log_probs is None:
+        raise InvalidConfig("a KL term needs ref_log_probs")
+    B, S = shape
+    per_token = advantages.dim() == 2
+    adv = _check_like(x, advantages, "advantages", (B, S) if per_token else (B,), _FLOATS)
+    old = None if old_log_probs is None else _check_like(x, old_log_probs, "old_log_probs", (B, S), _FLOATS)
+    ref = None if ref_log_probs is None else _check_like(x, ref_log_probs, "ref_log_probs", (B, S), _FLOATS)
+    terms = _lib.PolicyTerms(adv.data_ptr(), 1 if per_token else S, backend._ptr(old), backend._ptr(ref), float(clip_low), float(clip_high),
+                             float(kl_coef), 0)
+    return (adv, old, ref), terms
+
+
+def policy_loss(logits: torch.Tensor, targets: torch.Tensor, advantages: torch.Tensor, old_log_probs: Optional[torch.Tensor] = None,
+                ref_log_probs: Optional[torch.Tensor] = None, clip_low: float = 0.2, clip_high: float = 0.2, kl_coef: float = 0.0,
+                temperature: float = 1.0, sequence_mean: bool = False, ignore_index: Optional[int] = None,
+                return_grad: bool = False) -> PolicyLoss:
+    """Clipped policy-gradient loss with a KL term.  Per token, with r = exp(logp - old) and d = ref - logp:
+    -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(d) - d - 1); the loss is the mean over the kept tokens, or
+    with sequence_mean over each sequence's tokens first and then over the sequences that keep any.  advantages: [batch]
+    or [batch, seq].  old_log_probs: of the policy that sampled the tokens (None: this one, r = 1 with the gradient of r);
+    ref_log_probs: of a frozen reference, reported as `kl` even with kl_coef = 0.  All float32 [batch, seq], at `temperature`."""
+    x = _check_logits(logits)
+    B, S, _ = x.shape
+    t = _check_like(x, targets, "targets", (B, S), _INTEGERS)
+    held, terms = _policy_terms(x, (B, S), advantages, old_log_probs, ref_log_probs, clip_low, clip_high, kl_coef)
+    rows = _token_logits(x, temperature)
+    with _on_device(x):
+        lib = backend._lib_for(x)
+        grad = _new_grad(x, return_grad)
+        logp = torch.empty(B, S, dtype=torch.float32, device=x.device)
+        out = torch.empty(3, dtype=torch.float32, device=x.device)
+        ws = backend.workspace(x.device, lib.mcb_token_loss_workspace_bytes(B, S))
+        _lib.check(lib.mcb_policy_loss(rows, _token_targets(t, ignore_index), terms, int(bool(sequence_mean)),
+                                       logp.data_ptr(), out.data_ptr(), backend._ptr(grad), ws.data_ptr(), ws.numel(), backend._stream()))
+    del held
+    return PolicyLoss(out[0:1], logp, out[1:2], out[2:3], grad)
+
+
+def _teacher_top(x, shape, teacher_ids, teacher_logits, mask):
+    B, S = shape
+    if teacher_ids.dim() != 3 or not 1 <= teacher_ids.shape[2] <= 1024:
+        raise InvalidConfig(f"teacher_ids must be [batch, seq, 1 to 1024 entries], got shape {list(teacher_ids.shape)}")
+    K = teacher_ids.shape[2]
+    ids = _check_like(x, teacher_ids, "teacher_ids", (B, S, K), _INTEGERS)
+    tl = _check_like(x, teacher_logits, "teacher_logits", (B, S, K), (torch.float32, torch.bfloat16))
+    m = None if mask is None else _check_like(x, mask, "mask", (B, S), (torch.bool, torch.uint8))
+    return (ids, tl, m), _lib.TeacherTop(ids.data_ptr(), tl.data_ptr(), K, ids.element_size(), backend._dtype_code(tl))
+
+
+def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, mask: Optional[torch.Tensor] = None,
+                      temperature: float = 1.0, return_grad: bool = False):
+    """Distillation from a teacher's largest logits: mean over kept positions of temperature^2 KL(q || softmax(logits / temperature)) with
+    q = softmax(teacher_logits / temperature) over the teacher's 1 to 1024 entries of that position.  teacher_ids, teacher_logits:
+    [batch, seq, entries]; an entry of -inf counts for nothing, whatever its id (a position of nothing else adds 0 to the
+    mean); an id that comes twice has the sum of its probabilities.  mask [batch, seq]: 0 leaves a position out.  Returns a
+    1-element float32 tensor; with return_grad also d loss / d logits."""
+    x = _check_logits(logits)
+    B, S, _ = x.shape
+    held, teacher = _teacher_top(x, (B, S), teacher_ids, teacher_logits, mask)
+    rows = _token_logits(x, temperature)
+    with _on_device(x):
+        lib = backend._lib_for(x)
+        grad = _new_grad(x, return_grad)
+        loss = torch.empty(1, dtype=torch.float32, device=x.device)
+        ws = backend.workspace(x.device, lib.mcb_token_loss_workspace_bytes(B, S))
+        _lib.check(lib.mcb_distill_loss(rows, teacher, backend._ptr(held[2]), loss.data_ptr(), backend._ptr(grad),
+                                        ws.data_ptr(), ws.numel(), backend._stream()))
+    return (loss, grad) if return_grad else loss
 
 
 class TrainingStep:
