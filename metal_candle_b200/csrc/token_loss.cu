@@ -69,7 +69,7 @@ token_rows_kernel(const RowArgs a) {
     if constexpr (OP != kDistill) {
       const float xt = to_f32(x[tgt]);
       const TargetStats r = target_stats(m, s, xt, a.k);
-      const float c0 = finish_target_row<OP>(a, row, r, tid == 0);
+      const float c0 = finish_target_row<OP>(a, row, row_inputs<OP>(a, row), r, tid == 0);
       __syncthreads();   // everyone has read the target's logit, which the gradient may lie over
       if (g != nullptr) {
         const float f = -c0 / r.sum;
@@ -167,9 +167,10 @@ token_grad_kernel(const GradArgs ga) {
 
 // The weight of each row in the mean: 1 / kept rows, or 1 / (kept rows of its sequence x sequences that keep any).  Kept are the
 // rows whose mask is not 0, or whose target is not left out; a target out of range gets NaN.  Neither given: all rows.
+// `order`, unless null: the kept rows first, in one fixed order, then the others; and info[0] = how many are kept, info[1] = 0.
 __global__ void __launch_bounds__(1024)
 row_weights_kernel(const void* targets, int target_bytes, int has_ignore, int64_t ignore, const uint8_t* mask, float* weight,
-                   int* done, int64_t M, int64_t S, int V, int sequence_mean) {
+                   int32_t* order, int32_t* info, int64_t M, int64_t S, int V, int sequence_mean) {
   __shared__ int red[32];
   grid_launch_dependents();
   grid_dependency_wait();
@@ -182,38 +183,69 @@ row_weights_kernel(const void* targets, int target_bytes, int has_ignore, int64_
     return t >= 0 ? 1 : t + 1;
   };
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int n = 0;
+  int sequences = 0;
   if (sequence_mean) {
     for (int64_t b = warp; b < M / S; b += 32) {
       int c = 0;
       for (int64_t i = lane; i < S; i += 32) c += kept(b * S + i) != 0;
-      n += __reduce_add_sync(0xffffffffu, c) > 0;
+      sequences += __reduce_add_sync(0xffffffffu, c) > 0;
     }
-    if (lane != 0) n = 0;
-  } else {
-    for (int64_t i = threadIdx.x; i < M; i += 1024) n += kept(i) != 0;
+    if (lane == 0) red[warp] = sequences;
+    __syncthreads();
+    sequences = 0;
+    for (int w = 0; w < 32; ++w) sequences += red[w];
   }
-  n = __reduce_add_sync(0xffffffffu, n);
-  if (lane == 0) red[warp] = n;
-  __syncthreads();
-  n = 0;
-  for (int w = 0; w < 32; ++w) n += red[w];
-  const float share = 1.0f / static_cast<float>(max(1, n));
-  auto put = [&](int64_t row, float value) {
-    const int c = kept(row);
-    weight[row] = c == 0 ? 0.0f : c < 0 ? NAN : value;
-  };
+  // each warp takes 256 rows in a row, eight a lane; how many of those in front of it are kept is counted over the block
+  constexpr int kRows = 8;
+  const int rows = static_cast<int>(M);
+  int total = 0;
+  for (int64_t base = 0; base < M; base += 1024 * kRows) {
+    const int64_t mine = base + warp * 32 * kRows;
+    int keep[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) keep[r] = mine + r * 32 + lane < M ? kept(mine + r * 32 + lane) != 0 : 0;
+    uint32_t votes[kRows];
+    int c = 0;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      votes[r] = __ballot_sync(0xffffffffu, keep[r]);
+      c += __popc(votes[r]);
+    }
+    __syncthreads();   // red is free
+    if (lane == 0) red[warp] = c;
+    __syncthreads();
+    c = red[lane];
+    int at = total + __reduce_add_sync(0xffffffffu, lane < warp ? c : 0);   // kept rows before the warp's r-th 32
+    total += __reduce_add_sync(0xffffffffu, c);
+    if (order == nullptr) continue;
+    const uint32_t below = (1u << lane) - 1u;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const int64_t row = mine + r * 32 + lane;
+      const int k = at + __popc(votes[r] & below);   // kept rows before this one: the others fill the order from its end
+      if (row < M) order[keep[r] ? k : rows - 1 - (static_cast<int>(row) - k)] = static_cast<int32_t>(row);
+      at += __popc(votes[r]);
+    }
+  }
+  if (threadIdx.x == 0 && info != nullptr) { info[0] = total; info[1] = 0; }
   if (sequence_mean) {
+    const float share = 1.0f / static_cast<float>(max(1, sequences));
     for (int64_t b = warp; b < M / S; b += 32) {
       int c = 0;
       for (int64_t i = lane; i < S; i += 32) c += kept(b * S + i) != 0;
       c = __reduce_add_sync(0xffffffffu, c);
-      for (int64_t i = lane; i < S; i += 32) put(b * S + i, share / static_cast<float>(max(1, c)));
+      for (int64_t i = lane; i < S; i += 32) {
+        const int k = kept(b * S + i);
+        weight[b * S + i] = k == 0 ? 0.0f : k < 0 ? NAN : share / static_cast<float>(c);
+      }
     }
   } else {
-    for (int64_t i = threadIdx.x; i < M; i += 1024) put(i, share);
+    const float share = 1.0f / static_cast<float>(total > 0 ? total : 1);
+    for (int64_t i = threadIdx.x; i < M; i += 1024) {
+      const int k = kept(i);
+      weight[i] = k == 0 ? 0.0f : k < 0 ? NAN : share;
+    }
   }
-  if (done != nullptr && threadIdx.x == 0) *done = 0;
 }
 
 // out[i] = sum of terms[i][0 .. M), in one fixed order
@@ -301,8 +333,15 @@ __global__ void __launch_bounds__(256) scale_rows_kernel(T* x, const float* coef
 
 // ---- launches ------------------------------------------------------------------------------------------------------------
 
+int launch_sum(const float* terms, int64_t M, int n, float* out, cudaStream_t st);
+
 template <int OP>
-int launch_rows(const RowArgs& a, int dtype, DeviceState* ds, cudaStream_t st) {
+int launch_rows(const RowArgs& a, const RowPlan& plan, int dtype, DeviceState* ds, cudaStream_t st) {
+  if (OP == kUnit || OP == kDistill || a.grad != nullptr) {
+    bool taken = false;
+    if (int rc = launch_resident_rows(OP, a, plan, dtype, ds, st, &taken)) return rc;
+    if (taken) return MCB_OK;
+  }
   const int64_t most = static_cast<int64_t>(ds->sm_count) * 8;
   const dim3 grid(static_cast<unsigned>(a.M < most ? a.M : most));
   if (dtype == MCB_F32)
@@ -310,7 +349,7 @@ int launch_rows(const RowArgs& a, int dtype, DeviceState* ds, cudaStream_t st) {
   else
     MCB_CHECK_CUDA(launch_kernel(token_rows_kernel<__nv_bfloat16, OP>, grid, dim3(kRowThreads), 0, st, chained_launch(), a));
   MCB_CHECK_LAUNCH("token_rows");
-  return MCB_OK;
+  return plan.sums != nullptr ? launch_sum(a.terms, a.M, plan.n_sums, plan.sums, st) : MCB_OK;
 }
 
 int launch_grad(const GradArgs& ga, int dtype, DeviceState* ds, cudaStream_t st) {
@@ -324,10 +363,10 @@ int launch_grad(const GradArgs& ga, int dtype, DeviceState* ds, cudaStream_t st)
   return MCB_OK;
 }
 
-int launch_weights(const mcb_token_targets* t, const uint8_t* mask, float* weight, int* done, int64_t M, int64_t S, int64_t V,
-                   int sequence_mean, cudaStream_t st) {
+int launch_weights(const mcb_token_targets* t, const uint8_t* mask, float* weight, int32_t* order, int32_t* info, int64_t M, int64_t S,
+                   int64_t V, int sequence_mean, cudaStream_t st) {
   MCB_CHECK_CUDA(launch_kernel(row_weights_kernel, dim3(1), dim3(1024), 0, st, chained_launch(), t ? t->targets : nullptr,
-                               t ? t->target_bytes : 0, t ? t->has_ignore : 0, t ? t->ignore_index : 0, mask, weight, done, M, S,
+                               t ? t->target_bytes : 0, t ? t->has_ignore : 0, t ? t->ignore_index : 0, mask, weight, order, info, M, S,
                                static_cast<int>(V), sequence_mean));
   MCB_CHECK_LAUNCH("row_weights");
   return MCB_OK;
@@ -386,6 +425,17 @@ int check_teacher(const char* what, const mcb_teacher_top* t) {
   return MCB_OK;
 }
 
+// Workspace of a whole loss: a weight, up to three terms and a place in the order for each row, and two counters.
+struct LossWorkspace {
+  float* weight;
+  float* terms;
+  int32_t* order;
+  int32_t* info;
+  LossWorkspace(void* base, int64_t M)
+      : weight(static_cast<float*>(base)), terms(weight + M), order(reinterpret_cast<int32_t*>(terms + 3 * M)), info(order + M) {}
+  RowPlan plan(float* sums, int n) const { return {order, info, sums, n, info + 1}; }
+};
+
 RowArgs row_args(const mcb_token_logits* l, void* grad) {
   RowArgs a = {};
   a.logits = l->logits; a.grad = grad;
@@ -399,7 +449,7 @@ void set_targets(RowArgs& a, const mcb_token_targets* t) {
 }
 void set_policy(RowArgs& a, const mcb_policy_terms* p, const float* weight, float* logp, float* terms) {
   a.weight = weight;
-  a.advantages = p->advantages; a.advantage_rows = p->advantage_rows; a.old_logp = p->old_logp; a.ref_logp = p->ref_logp;
+  a.advantages = p->advantages; a.advantage_rows = p->advantage_rows < kMaxDim ? p->advantage_rows : kMaxDim; a.old_logp = p->old_logp; a.ref_logp = p->ref_logp;
   a.ratio_min = 1.0f - p->clip_low; a.ratio_max = 1.0f + p->clip_high; a.kl_coef = p->kl_coef;
   a.logp = logp; a.terms = terms;
 }
@@ -427,7 +477,7 @@ extern "C" int mcb_token_logprob_fwd(const mcb_token_logits* logits, const mcb_t
   set_targets(a, targets);
   a.logp = logp; a.lse = lse;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return unit_grad ? launch_rows<kUnit>(a, logits->dtype, ds, st) : launch_rows<kStats>(a, logits->dtype, ds, st);
+  return unit_grad ? launch_rows<kUnit>(a, {}, logits->dtype, ds, st) : launch_rows<kStats>(a, {}, logits->dtype, ds, st);
 }
 
 extern "C" int mcb_token_logprob_bwd(const mcb_token_logits* logits, const mcb_token_targets* targets, const float* logp, const float* lse,
@@ -444,7 +494,7 @@ extern "C" int mcb_token_logprob_bwd(const mcb_token_logits* logits, const mcb_t
   ga.a = row_args(logits, dlogits);
   set_targets(ga.a, targets);
   ga.a.logp = const_cast<float*>(logp); ga.a.lse = const_cast<float*>(lse);
-  ga.coef = dlogp; ga.coef_rows = dlogp_rows;
+  ga.coef = dlogp; ga.coef_rows = dlogp_rows < kMaxDim ? dlogp_rows : kMaxDim;
   return launch_grad(ga, logits->dtype, ds, static_cast<cudaStream_t>(stream));
 }
 
@@ -457,7 +507,7 @@ extern "C" int mcb_loss_weights(const mcb_token_targets* targets, const uint8_t*
   if (batch <= 0 || seq <= 0 || vocab <= 0 || vocab > kMaxDim || batch > kMaxDim || seq > kMaxDim || batch * seq > kMaxDim)
     return fail(MCB_ERR_SHAPE, "loss_weights: bad shape");
   if (!current_device_state()) return MCB_ERR_NOT_INIT;
-  return launch_weights(targets, mask, weight, nullptr, batch * seq, seq, vocab, sequence_mean, static_cast<cudaStream_t>(stream));
+  return launch_weights(targets, mask, weight, nullptr, nullptr, batch * seq, seq, vocab, sequence_mean, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int mcb_loss_sums(const float* terms, int64_t rows, int n, float* out, void* stream) {
@@ -480,7 +530,7 @@ extern "C" int mcb_policy_loss_rows(const mcb_token_logits* logits, const mcb_to
   RowArgs a = row_args(logits, dlogits);
   set_targets(a, targets);
   set_policy(a, policy, weight, logp, terms);
-  return launch_rows<kPolicy>(a, logits->dtype, ds, static_cast<cudaStream_t>(stream));
+  return launch_rows<kPolicy>(a, {}, logits->dtype, ds, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int mcb_distill_loss_rows(const mcb_token_logits* logits, const mcb_teacher_top* teacher, const float* weight, float* terms,
@@ -493,12 +543,12 @@ extern "C" int mcb_distill_loss_rows(const mcb_token_logits* logits, const mcb_t
   if (!ds) return MCB_ERR_NOT_INIT;
   RowArgs a = row_args(logits, dlogits);
   set_teacher(a, teacher, weight, terms);
-  return launch_rows<kDistill>(a, logits->dtype, ds, static_cast<cudaStream_t>(stream));
+  return launch_rows<kDistill>(a, {}, logits->dtype, ds, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t mcb_token_loss_workspace_bytes(int64_t batch, int64_t seq) {
   if (batch <= 0 || seq <= 0 || batch > kMaxDim || seq > kMaxDim || batch * seq > kMaxDim) return 0;
-  return (static_cast<size_t>(batch * seq) * 4 + static_cast<size_t>(batch) + 64) * sizeof(float);
+  return (static_cast<size_t>(batch * seq) * 5 + static_cast<size_t>(batch) + 64) * sizeof(float);
 }
 
 extern "C" int mcb_policy_loss(const mcb_token_logits* logits, const mcb_token_targets* targets, const mcb_policy_terms* policy, int sequence_mean,
@@ -514,14 +564,12 @@ extern "C" int mcb_policy_loss(const mcb_token_logits* logits, const mcb_token_t
   if (!ds) return MCB_ERR_NOT_INIT;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t M = logits->batch * logits->seq;
-  float* weight = static_cast<float*>(workspace);
-  float* terms = weight + M;
-  if (int rc = launch_weights(targets, nullptr, weight, nullptr, M, logits->seq, logits->vocab, sequence_mean, st)) return rc;
+  const LossWorkspace ws(workspace, M);
+  if (int rc = launch_weights(targets, nullptr, ws.weight, ws.order, ws.info, M, logits->seq, logits->vocab, sequence_mean, st)) return rc;
   RowArgs a = row_args(logits, dlogits);
   set_targets(a, targets);
-  set_policy(a, policy, weight, logp, terms);
-  if (int rc = launch_rows<kPolicy>(a, logits->dtype, ds, st)) return rc;
-  return launch_sum(terms, M, 3, out, st);
+  set_policy(a, policy, ws.weight, logp, ws.terms);
+  return launch_rows<kPolicy>(a, ws.plan(out, 3), logits->dtype, ds, st);
 }
 
 extern "C" int mcb_distill_loss(const mcb_token_logits* logits, const mcb_teacher_top* teacher, const uint8_t* mask, float* loss, void* dlogits,
@@ -536,13 +584,11 @@ extern "C" int mcb_distill_loss(const mcb_token_logits* logits, const mcb_teache
   if (!ds) return MCB_ERR_NOT_INIT;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t M = logits->batch * logits->seq;
-  float* weight = static_cast<float*>(workspace);
-  float* terms = weight + M;
-  if (int rc = launch_weights(nullptr, mask, weight, nullptr, M, logits->seq, logits->vocab, 0, st)) return rc;
+  const LossWorkspace ws(workspace, M);
+  if (int rc = launch_weights(nullptr, mask, ws.weight, ws.order, ws.info, M, logits->seq, logits->vocab, 0, st)) return rc;
   RowArgs a = row_args(logits, dlogits);
-  set_teacher(a, teacher, weight, terms);
-  if (int rc = launch_rows<kDistill>(a, logits->dtype, ds, st)) return rc;
-  return launch_sum(terms, M, 1, loss, st);
+  set_teacher(a, teacher, ws.weight, ws.terms);
+  return launch_rows<kDistill>(a, ws.plan(loss, 1), logits->dtype, ds, st);
 }
 
 extern "C" int mcb_preference_finish(const float* logp, const mcb_token_targets* targets, const float* ref_logp, float* seq_logp, float* coef,

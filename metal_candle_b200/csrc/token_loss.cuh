@@ -46,9 +46,9 @@ struct RowArgs {
   float* terms;            // kPolicy: [3, M]: loss, KL, clipped; kDistill: [M]; each times the row's weight
 };
 
-__device__ __forceinline__ int64_t row_offset(const RowArgs& a, int64_t row) {
-  const int64_t b = row / a.S;
-  return b * a.batch_stride + (row - b * a.S) * a.token_stride;
+__device__ __forceinline__ int64_t row_offset(const RowArgs& a, int64_t row) {   // (rows and S are below 2^31)
+  const uint32_t r = static_cast<uint32_t>(row), b = r / static_cast<uint32_t>(a.S);
+  return b * a.batch_stride + static_cast<int64_t>(r - b * static_cast<uint32_t>(a.S)) * a.token_stride;
 }
 
 // The row's target, -1 where the row is left out, -2 where it is none of the vocabulary.
@@ -82,8 +82,8 @@ struct TargetStats {
 __device__ __forceinline__ TargetStats target_stats(float m, float s, float xt, float k) {
   TargetStats r;
   if (m == -INFINITY && s == 0.0f) {   // nothing but the target (which, masked itself, has no probability: NaN)
-    r.top = xt; r.sum = 1.0f; r.rest = 0.0f;
-    r.logp = xt - xt;
+    r.logp = r.rest = xt - xt;
+    r.top = xt; r.sum = 1.0f + r.logp;
     return r;
   }
   const float d = (m - xt) * k;
@@ -104,9 +104,24 @@ __device__ __forceinline__ TargetStats target_stats(float m, float s, float xt, 
 struct PolicyTerm {
   float loss, dlogp, kl, clipped;
 };
-__device__ __forceinline__ PolicyTerm policy_term(const RowArgs& a, int64_t row, float logp) {
-  const float adv = a.advantages[row / a.advantage_rows];
-  const float ratio = a.old_logp != nullptr ? expf(logp - a.old_logp[row]) : 1.0f;
+// What the loss reads of a row besides its logits, apart so that it can be asked for ahead.
+struct RowInputs {
+  float weight, advantage, old_logp, ref_logp;
+};
+template <int OP>
+__device__ __forceinline__ RowInputs row_inputs(const RowArgs& a, int64_t row) {
+  RowInputs in = {};
+  if constexpr (OP == kPolicy || OP == kDistill) in.weight = a.weight[row];
+  if constexpr (OP == kPolicy) {
+    in.advantage = a.advantages[static_cast<uint32_t>(row) / static_cast<uint32_t>(a.advantage_rows)];
+    if (a.old_logp != nullptr) in.old_logp = a.old_logp[row];
+    if (a.ref_logp != nullptr) in.ref_logp = a.ref_logp[row];
+  }
+  return in;
+}
+__device__ __forceinline__ PolicyTerm policy_term(const RowArgs& a, const RowInputs& in, float logp) {
+  const float adv = in.advantage;
+  const float ratio = a.old_logp != nullptr ? expf(logp - in.old_logp) : 1.0f;
   const float bounded = fminf(fmaxf(ratio, a.ratio_min), a.ratio_max);
   PolicyTerm t;
   // min(r A, clip(r) A): the bound holds only where it makes the term smaller
@@ -117,7 +132,7 @@ __device__ __forceinline__ PolicyTerm policy_term(const RowArgs& a, int64_t row,
   t.kl = 0.0f;
   if (a.ref_logp != nullptr) {
     // exp(d) - d - 1 >= 0 with d = ref - logp: an estimate of KL(policy || reference) that is never negative
-    const float d = a.ref_logp[row] - logp;
+    const float d = in.ref_logp - logp;
     const float e = expm1f(d);
     t.kl = e - d;
     t.loss += a.kl_coef * t.kl;
@@ -128,12 +143,12 @@ __device__ __forceinline__ PolicyTerm policy_term(const RowArgs& a, int64_t row,
 
 // What a row's log-probability comes to: writes the row's outputs (`write`: by one thread) and returns d loss / d logp / T.
 template <int OP>
-__device__ __forceinline__ float finish_target_row(const RowArgs& a, int64_t row, const TargetStats& r, bool write) {
+__device__ __forceinline__ float finish_target_row(const RowArgs& a, int64_t row, const RowInputs& in, const TargetStats& r, bool write) {
   if (write && a.logp != nullptr) a.logp[row] = r.logp;
   if (write && a.lse != nullptr) a.lse[row] = r.top * a.inv_t + logf(r.sum);
   if constexpr (OP == kPolicy) {
-    const float w = a.weight[row];
-    const PolicyTerm t = policy_term(a, row, r.logp);
+    const float w = in.weight;
+    const PolicyTerm t = policy_term(a, in, r.logp);
     if (write) {
       a.terms[row] = w * t.loss;
       a.terms[a.M + row] = w * t.kl;
@@ -159,6 +174,19 @@ __device__ __forceinline__ float read_teacher(const RowArgs& a, int64_t i) {
 __device__ __forceinline__ int64_t read_teacher_id(const RowArgs& a, int64_t i) {
   return a.id_bytes == 8 ? static_cast<const int64_t*>(a.teacher_ids)[i] : static_cast<const int32_t*>(a.teacher_ids)[i];
 }
+
+// Rows in the order they are to be taken, the kept ones first (as mcb_loss_weights tells them apart), and where the sum of each of
+// the rows' terms goes.  All null for a chunk of rows.
+struct RowPlan {
+  const int32_t* order;
+  const int32_t* kept;
+  float* sums;      // n_sums of them
+  int n_sums;
+  int* done;        // 0 when the kernel starts
+};
+
+// The one-pass kernel (token_resident.cu), where it takes rows of this length: *taken says whether it did.
+int launch_resident_rows(int op, const RowArgs& a, const RowPlan& plan, int dtype, DeviceState* ds, cudaStream_t st, bool* taken);
 
 }  // namespace tokenloss
 }  // namespace mcb
