@@ -59,6 +59,17 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
+// Hands 16 bytes to CTA `to` of the cluster, at the place of `slot` here, and tells the barrier there.  (A plain store with a releasing
+// arrival would first wait for the thread's gradient stores to reach memory.)
+__device__ __forceinline__ void send(uint32_t slot, uint32_t bar, int to, float4 v) {
+  asm volatile("{\n\t.reg .b32 rs, rb;\n\t"
+               "mapa.shared::cluster.u32 rs, %0, %2;\n\t"
+               "mapa.shared::cluster.u32 rb, %1, %2;\n\t"
+               "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [rs], {%3, %4, %5, %6}, [rb];\n\t}"
+               ::"r"(slot), "r"(bar), "r"(to), "r"(__float_as_uint(v.x)), "r"(__float_as_uint(v.y)), "r"(__float_as_uint(v.z)),
+               "r"(__float_as_uint(v.w)) : "memory");
+}
+
 // Bounded like every wait of the library, with acquire at cluster scope: the data came from a peer's store.
 __device__ __forceinline__ void wait_peers(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status) {
   long long t0 = 0;
@@ -106,10 +117,18 @@ struct Lane<float> {
   }
 };
 
-// (m, s) of a warp's lanes: the same in every lane
-__device__ __forceinline__ void warp_combine(float& m, float& s, float k) {
+__device__ __forceinline__ void tmem_ld_wait_on16(uint32_t (&r)[16]) {   // no use of r moves above it
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :: "memory");
+}
+
+// (m, s) of a warp's first `lanes` lanes, a power of two (the others hold nothing: -inf, 0): the same in those lanes
+__device__ __forceinline__ void warp_combine(float& m, float& s, float k, int lanes = 32) {
   const float top = warp_max(m);
-  s = warp_sum(m == -INFINITY ? s : s * ex2((m - top) * k));   // (nothing kept: 0, or NaN if it holds one)
+  s = m == -INFINITY ? s : s * ex2((m - top) * k);   // (nothing kept: 0, or NaN if it holds one)
+  for (int o = lanes >> 1; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   m = top;
 }
 
@@ -147,6 +166,15 @@ struct RowInfo {
   int state;         // 0: to be computed, 1: left out, 2: out of range
   RowInputs in;
 };
+// The group's feeder's notes (see below), in shared memory: they would cost every thread a dozen registers.
+struct Feed {
+  const void* from;      // where the rest of the row's share lies
+  uint32_t fed;          // the place of the row that is being fed, infos[at] if it is among them
+  int at, left;          // left: vectors of the row's share that have not been fed
+  int slot;
+  uint32_t phase;
+};
+
 // SAME: every row of the gradient lies as its logits do relative to 16 bytes, so that whole vectors can be written.
 template <typename T, int OP, bool SAME>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -159,6 +187,7 @@ token_resident_kernel(const RowArgs a, const Resident p) {
   __shared__ __align__(8) uint64_t full[kWarps][kMaxPieces], empty[kWarps][kMaxPieces], slot_bars[kWarps][2];
   __shared__ __align__(16) float4 slots[kWarps / 2][2][8];   // by group, parity and CTA: (maximum, sum, target's logit or loss, whose target it is)
   __shared__ __align__(16) float4 row_end[kWarps / 2][2];    // what the second sweep needs: by group and parity
+  __shared__ Feed feeds[kWarps];
   __shared__ float3 red[2][kWarps];
   __shared__ float edge[kWarps][2][2 * N];                   // the share's elements in vectors that are not the row's alone
   __shared__ float target_logit[kWarps][2];
@@ -192,7 +221,7 @@ token_resident_kernel(const RowArgs a, const Resident p) {
   if (threadIdx.x == 0) *abort_flag = 0;
   if (tid == 0) {
     for (int i = 0; i < p.pieces; ++i) { mbar_init(full0 + 8 * i, 1); mbar_init(empty0 + 8 * i, p.group_warps); }
-    for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&slot_bars[group][i]), ctas); repeats[group][i] = 0; }
+    for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&slot_bars[group][i]), 1); repeats[group][i] = 0; }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async_smem();
   }
@@ -213,64 +242,60 @@ token_resident_kernel(const RowArgs a, const Resident p) {
   // a warp reaches the 32 lanes of its place among four; the warps that share them have 128 columns each
   const uint32_t tmem = p.tmem ? tmem_base + (static_cast<uint32_t>(warp & 3) << 21) + (warp >> 2) * (kTmemChunks * kChunk) : 0;
 
-  const int M = static_cast<int>(a.M);
-  const int kept = p.kept != nullptr ? *from_here(p.kept) : M;
-  auto row_of = [&](int64_t i) -> int { return p.order != nullptr ? from_here(p.order)[i] : static_cast<int>(i); };
-  auto state_of = [&](int64_t i, int row) {   // 0: to be computed, 1: left out, 2: out of range
+  const uint32_t M = static_cast<uint32_t>(a.M);
+  const uint32_t kept = p.kept != nullptr ? static_cast<uint32_t>(*from_here(p.kept)) : M;
+  auto row_of = [&](uint32_t i) -> int { return p.order != nullptr ? from_here(p.order)[i] : static_cast<int>(i); };
+  auto state_of = [&](uint32_t i, int row) {   // 0: to be computed, 1: left out, 2: out of range
     if (OP == kDistill || i >= kept) return i < kept ? 0 : 1;
     const int t = read_target(a.targets, a.target_bytes, a.has_ignore, a.ignore, row, a.V);
     return t >= 0 ? 0 : t == -2 ? 2 : 1;
   };
   auto chunks_of = [&](int n) { return max(1, (n + CV * gd - 1) >> (kLogCv + log_gd)); };
 
-  // One thread of the group's last warp (the first has the row's scalar work) also feeds the ring: pieces in the order they are taken, each when every warp has left the slot it goes to.
-  // fed: the place of the row that is being fed, infos[fed_at] if it is among them.
+  // One thread of the group's last warp (the first has the row's scalar work) also feeds the ring: pieces in the order they are taken,
+  // each when every warp has left the slot it goes to.
   const int feeder = gd - 32;
-  int64_t fed = static_cast<int64_t>(first) - step;
-  const T* from = nullptr;
-  int left = 0, feed_slot = 0, fed_at = -1;   // left: vectors of the row's share that have not been fed
-  uint32_t feed_phase = 1;
+  if (tid == feeder) feeds[group] = {nullptr, static_cast<uint32_t>(first) - static_cast<uint32_t>(step), -1, 0, 0, 1};
   auto feed = [&]() {
-    if (left <= 0) {
+    Feed f = feeds[group];
+    if (f.left <= 0) {
       while (true) {
-        if (fed >= kept) return;
-        fed += step;
-        ++fed_at;
-        if (fed >= kept) return;
-        if (fed_at < info_rows) {
-          const RowInfo& f = infos[fed_at];
-          if (f.state != 0) continue;
-          from = static_cast<const T*>(a.logits) - p.mis + f.share.from;
-          left = f.share.n;
+        f.fed += step; ++f.at;   // (the first time round from 2^32 - something)
+        if (f.fed >= kept) { f.fed -= step; --f.at; feeds[group] = f; return; }
+        if (f.at < info_rows) {
+          const RowInfo& r = infos[f.at];
+          if (r.state != 0) continue;
+          f.from = static_cast<const T*>(a.logits) - p.mis + r.share.from;
+          f.left = r.share.n;
         } else {
-          const int row = row_of(fed);
-          if (state_of(fed, row) != 0) continue;
+          const int row = row_of(f.fed);
+          if (state_of(f.fed, row) != 0) continue;
           const Share s = share_of<N>(a, p, rank, row);
-          from = static_cast<const T*>(a.logits) - p.mis + s.from;
-          left = s.n;
+          f.from = static_cast<const T*>(a.logits) - p.mis + s.from;
+          f.left = s.n;
         }
         break;
       }
     }
-    const int n = max(0, min(left, CV * gd));
-    if (mbar_wait(empty0 + 8 * feed_slot, feed_phase, abort_flag, 55, p.status)) {
-      mbar_expect_tx(full0 + 8 * feed_slot, n * 16);   // a piece with nothing in it completes at once
-      if (n > 0) bulk_load(smem_u32(ring) + feed_slot * piece_bytes, from, n * 16, full0 + 8 * feed_slot);
+    const int n = max(0, min(f.left, CV * gd));
+    if (mbar_wait(empty0 + 8 * f.slot, f.phase, abort_flag, 55, p.status)) {
+      mbar_expect_tx(full0 + 8 * f.slot, n * 16);   // a piece with nothing in it completes at once
+      if (n > 0) bulk_load(smem_u32(ring) + f.slot * piece_bytes, f.from, n * 16, full0 + 8 * f.slot);
     }
-    from += n * N;
-    left -= n;
-    if (++feed_slot == p.pieces) { feed_slot = 0; feed_phase ^= 1; }
+    f.from = static_cast<const T*>(f.from) + n * N;
+    f.left -= n;
+    if (++f.slot == p.pieces) { f.slot = 0; f.phase ^= 1; }
+    feeds[group] = f;
   };
 
   uint32_t phase = 0, slot_phase = 0;   // parities of the ring's current round, and (bit i) of slot barrier i
   int slot = 0, par = 0, at = info_rows;
-  bool started = false;
-  for (int64_t i = first; i < M; i += step, ++at) {
+  for (uint32_t i = first; i < M; i += step, ++at) {   // (M and the step are below 2^31)
     if (at == info_rows) {
       group_sync();   // the last of them is done with
       for (int q = tid; q < info_rows; q += gd) {
-        const int64_t iq = i + static_cast<int64_t>(q) * step;
-        if (iq < M) {
+        const uint32_t iq = i + static_cast<uint32_t>(q) * step;   // (kInfoRows steps are few)
+        if (iq < M && iq >= i) {
           RowInfo f;
           f.row = row_of(iq);
           f.share = share_of<N>(a, p, rank, f.row);
@@ -289,10 +314,11 @@ token_resident_kernel(const RowArgs a, const Resident p) {
       }
       group_sync();
       at = 0;
-      if (started) fed_at -= info_rows;
-      if (!started && tid == feeder)
-        for (int q = 0; q < p.pieces; ++q) feed();
-      started = true;
+      if (tid == feeder) {
+        if (i != static_cast<uint32_t>(first)) feeds[group].at -= info_rows;
+        else
+          for (int q = 0; q < p.pieces; ++q) feed();
+      }
     }
     const RowInfo& info = infos[at];
     if (info.state != 0) {   // the same in every CTA of the cluster
@@ -364,7 +390,8 @@ token_resident_kernel(const RowArgs a, const Resident p) {
     float m = -INFINITY, sw = 0.0f, e[kChunk];
     const int chunks = chunks_of(info.share.n);
     const float2 kk = make_float2(a.k, a.k);
-    auto take = [&](int c, float (&x)[kChunk]) {   // the chunk's exponentials, and the thread's maximum so far, which they are relative to
+    // A chunk on its way into registers; the return value is its largest logit.
+    auto fetch = [&](int c, VT (&raw)[CV]) {
       const Share& s = info.share;
       const int v0 = c << (kLogCv + log_gd), n = min(s.n - v0, CV * gd), e0 = v0 * N;   // the chunk's vectors begin at v0, its elements at e0
       mbar_wait(full0 + 8 * slot, phase, abort_flag, 56, p.status);
@@ -405,7 +432,6 @@ token_resident_kernel(const RowArgs a, const Resident p) {
           third -= t_q[q] * ((xq - x_ref) * a.inv_t);
         }
       }
-      VT raw[CV];
       if (n == CV * gd) {
 #pragma unroll
         for (int j = 0; j < CV; ++j) raw[j].raw = srow[j * gd + tid];
@@ -417,12 +443,15 @@ token_resident_kernel(const RowArgs a, const Resident p) {
           if (j * gd + tid < n) raw[j].raw = srow[j * gd + tid];
         }
       }
-      const float cm = Lane<T>::max_of(raw);
       __syncwarp();
       if (lane == 0) mbar_arrive(empty0 + 8 * slot);   // the warp has taken what it needs of the slot
       if (++slot == p.pieces) { slot = 0; phase ^= 1; }
       if (c > 0 && tid == feeder) feed();              // the slot of the piece before this one
       __syncwarp();
+      return Lane<T>::max_of(raw);
+    };
+    // Its exponentials, relative to the thread's largest logit so far, m.
+    auto exponentials = [&](const VT (&raw)[CV], float cm, float (&x)[kChunk]) {
       const float mm = fmaxf(m, cm);
       if (mm > m && m != -INFINITY) sw *= ex2((m - mm) * a.k);
       m = mm;
@@ -442,20 +471,43 @@ token_resident_kernel(const RowArgs a, const Resident p) {
         }
       }
       sw += s2.x + s2.y;
-      return m;
     };
-#pragma unroll 1
-    for (int c = 0; c < chunks - 1; ++c) {
-      float x[kChunk];
-      refs[c][threadIdx.x] = take(c, x);
-      const uint32_t* w = reinterpret_cast<const uint32_t*>(x);
+    auto keep = [&](int c, const float (&x)[kChunk]) {   // in tensor memory
+      refs[c][threadIdx.x] = m;
       uint32_t half[2][16];
 #pragma unroll
-      for (int q = 0; q < 16; ++q) { half[0][q] = w[q]; half[1][q] = w[16 + q]; }
+      for (int q = 0; q < 16; ++q) { half[0][q] = __float_as_uint(x[q]); half[1][q] = __float_as_uint(x[16 + q]); }
       tmem_st_x16(tmem + c * kChunk, half[0]);
       tmem_st_x16(tmem + c * kChunk + 16, half[1]);
+    };
+    // the next chunk is fetched before this one's arithmetic, where there are registers for two
+    VT raw[CV];
+    float cm;
+    if constexpr (sizeof(T) == 2) {
+      cm = fetch(0, raw);
+#pragma unroll 1
+      for (int c = 0; c < chunks - 1; ++c) {
+        VT next[CV];
+        const float next_cm = fetch(c + 1, next);
+        float x[kChunk];
+        exponentials(raw, cm, x);
+        keep(c, x);
+#pragma unroll
+        for (int j = 0; j < CV; ++j) raw[j] = next[j];
+        cm = next_cm;
+      }
+    } else {
+#pragma unroll 1
+      for (int c = 0; c < chunks - 1; ++c) {
+        float x[kChunk];
+        cm = fetch(c, raw);
+        exponentials(raw, cm, x);
+        keep(c, x);
+      }
+      cm = fetch(chunks - 1, raw);
     }
-    const float ref_e = take(chunks - 1, e);
+    exponentials(raw, cm, e);
+    const float ref_e = m;
     float mw = m;
     warp_combine(mw, sw, a.k);
     if constexpr (OP == kDistill) third = warp_sum(third);
@@ -466,7 +518,7 @@ token_resident_kernel(const RowArgs a, const Resident p) {
       if (tid < 32) {
         const float3 r = lane < p.group_warps ? red[par][group * p.group_warps + lane] : make_float3(-INFINITY, 0.0f, 0.0f);
         mw = r.x; sw = r.y;
-        warp_combine(mw, sw, a.k);
+        warp_combine(mw, sw, a.k, p.group_warps);
         if constexpr (OP == kDistill) third = warp_sum(r.z);
       } else if (tid == feeder) {
         feed();   // the slot of the row's last piece
@@ -487,18 +539,13 @@ token_resident_kernel(const RowArgs a, const Resident p) {
         // Thread q hands this CTA's part to CTA q.  A slot is written again two rows later, when its readers have passed the
         // exchange in between.
         const uint32_t to = smem_u32(&slots[group][par][rank]), bar = smem_u32(&slot_bars[group][par]);
-        if (tid < ctas)
-          asm volatile("{\n\t.reg .b32 rs, rb;\n\t"
-                       "mapa.shared::cluster.u32 rs, %0, %2;\n\t"
-                       "mapa.shared::cluster.u32 rb, %1, %2;\n\t"
-                       "st.shared::cluster.v4.f32 [rs], {%3, %4, %5, %6};\n\t"
-                       "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [rb];\n\t}"
-                       ::"r"(to), "r"(bar), "r"(tid), "f"(mw), "f"(sw), "f"(third), "f"(own ? 1.0f : 0.0f) : "memory");
+        if (tid == 0) mbar_expect_tx(bar, ctas * 16);
+        if (tid < ctas) send(to, bar, tid, make_float4(mw, sw, third, own ? 1.0f : 0.0f));
         wait_peers(bar, (slot_phase >> par) & 1u, abort_flag, p.status);
         slot_phase ^= 1u << par;
         const float4 r = lane < ctas ? slots[group][par][lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
         mw = r.x; sw = r.y;
-        warp_combine(mw, sw, a.k);
+        warp_combine(mw, sw, a.k, ctas);
         if constexpr (OP == kDistill) {
           third = warp_sum(r.z);
         } else {
@@ -532,12 +579,12 @@ token_resident_kernel(const RowArgs a, const Resident p) {
     if (a.grad != nullptr) {
       const Share& s = info.share;
       T* g = static_cast<T*>(a.grad) + s.to;
-      auto put = [&](int c, const float (&x)[kChunk], float r) {
-        const float f = r == -INFINITY ? f_top : f_top * ex2((r - top) * a.k);   // (the thread has seen masked logits only: zeros, or NaN)
+      // vectors [first vector, first vector + count) of chunk c, from their exponentials relative to r
+      auto put = [&](int c, int j0, const float* x, int count, float f) {
         const float2 ff = make_float2(f, f);
 #pragma unroll
-        for (int j = 0; j < CV; ++j) {
-          const int vi = c * CV * gd + j * gd + tid;
+        for (int j = 0; j < count; ++j) {
+          const int vi = ((c * CV + j0 + j) << log_gd) + tid;
           float y[N];
 #pragma unroll
           for (int q = 0; q < N; q += 2) {
@@ -556,18 +603,27 @@ token_resident_kernel(const RowArgs a, const Resident p) {
           }
         }
       };
-      put(chunks - 1, e, ref_e);
+      auto factor = [&](float r) {   // (-inf: the thread has seen masked logits only, whose exponentials are zeros, or NaN)
+        return r == -INFINITY ? f_top : f_top * ex2((r - top) * a.k);
+      };
+      // half a chunk is on its way from tensor memory while the one before is written
+      uint32_t w0[16], w1[16];
+      float x[16];
+      if (chunks > 1) tmem_ld_x16(tmem, w0);
+      put(chunks - 1, 0, e, CV, factor(ref_e));
 #pragma unroll 1
       for (int c = 0; c < chunks - 1; ++c) {
-        {
-          uint32_t w[kChunk];
-          tmem_ld_x32(tmem + c * kChunk, w);
-          tmem_ld_wait_on(w);
-          float x[kChunk];
+        const float f = factor(refs[c][threadIdx.x]);
+        tmem_ld_wait_on16(w0);
+        tmem_ld_x16(tmem + c * kChunk + 16, w1);
 #pragma unroll
-          for (int q = 0; q < kChunk; ++q) x[q] = __uint_as_float(w[q]);
-          put(c, x, refs[c][threadIdx.x]);
-        }
+        for (int q = 0; q < 16; ++q) x[q] = __uint_as_float(w0[q]);
+        put(c, 0, x, CV / 2, f);
+        tmem_ld_wait_on16(w1);
+        if (c + 1 < chunks - 1) tmem_ld_x16(tmem + (c + 1) * kChunk, w0);
+#pragma unroll
+        for (int q = 0; q < 16; ++q) x[q] = __uint_as_float(w1[q]);
+        put(c, CV / 2, x, CV / 2, f);
       }
       const int tl = info.target;
       if (OP != kDistill && own) {
@@ -628,7 +684,7 @@ token_resident_kernel(const RowArgs a, const Resident p) {
       double* sums = reinterpret_cast<double*>(smem);
       for (int t = 0; t < p.n_out; ++t) {
         double acc = 0.0;
-        for (int q = threadIdx.x; q < M; q += kThreads) acc += static_cast<double>(__ldcg(a.terms + static_cast<int64_t>(t) * M + q));
+        for (uint32_t q = threadIdx.x; q < M; q += kThreads) acc += static_cast<double>(__ldcg(a.terms + static_cast<int64_t>(t) * M + q));
         for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
         if (lane == 0) sums[warp] = acc;
         __syncthreads();
@@ -653,10 +709,12 @@ int launch_resident(const RowArgs& a, const RowPlan& plan, DeviceState* ds, cuda
   Resident p;
   p.log_ctas = 0; p.group_warps = 1;
   auto fits = [&]() { return (vecs + (1 << p.log_ctas) - 1) >> p.log_ctas <= static_cast<int64_t>(kMaxChunks) * CV * 32 * p.group_warps; };
+  // As few CTAs a row as can hold it, then as few warps: a row's exchange costs more than the rows in flight gain
+  // (2048 x 151936 bf16 over 8 CTAs with four rows in flight 345 us, over 4 with two 324, over 2 with one 292; 4000 x 32000 over 2 and four
+  // 144 us, by one CTA with two 115, with one 138).
   while (!fits()) {
-    if (p.group_warps < 4) p.group_warps *= 2;
+    if (p.group_warps < kWarps) p.group_warps *= 2;
     else if (p.log_ctas < 3) ++p.log_ctas;
-    else if (p.group_warps < kWarps) p.group_warps *= 2;
     else return MCB_OK;
   }
   p.tmem = (vecs + (1 << p.log_ctas) - 1) >> p.log_ctas > static_cast<int64_t>(CV) * 32 * p.group_warps;
