@@ -37,6 +37,7 @@ constexpr int kChunk = 32;             // elements a thread takes at a time
 constexpr int kTmemChunks = 4;         // chunks it keeps in tensor memory, beside one in registers
 constexpr int kMaxChunks = kTmemChunks + 1;
 constexpr int kMaxPieces = 6;          // ring slots of a group
+constexpr uint32_t kEdges = 1u << 31;
 constexpr int kInfoRows = 128;         // rows a CTA's groups look ahead at, together
 constexpr int kSmem = 200 * 1024;      // dynamic shared memory, at least: with it no other kernel that uses tensor memory fits on the SM
 
@@ -162,7 +163,7 @@ __device__ __forceinline__ Share share_of(const RowArgs& a, const Resident& p, i
 struct RowInfo {
   Share share;
   int row, target;   // the target: within the share, or -1
-  int edges;         // whether the share has vectors that are not the row's alone
+  uint32_t special;  // bit c: chunk c holds the target, is not full, or has vectors that are not the row's alone; kEdges: the share has such
   int state;         // 0: to be computed, 1: left out, 2: out of range
   RowInputs in;
 };
@@ -307,7 +308,11 @@ token_resident_kernel(const RowArgs a, const Resident p) {
               if (t >= f.share.lo && t < f.share.hi) f.target = t;
             }
           }
-          f.edges = f.share.lo > 0 || f.share.hi < f.share.n * N;
+          f.special = 0;
+          const int per = CV * N << log_gd;   // elements of a chunk
+          if (f.target >= 0) f.special |= 1u << (f.target / per);
+          if (f.share.n * N % per != 0 || f.share.n == 0) f.special |= 1u << (chunks_of(f.share.n) - 1);
+          if (f.share.lo > 0 || f.share.hi < f.share.n * N) f.special |= kEdges | 1u | 1u << (chunks_of(f.share.n) - 1);
           f.in = row_inputs<OP>(a, f.row);
           infos[q] = f;
         }
@@ -392,55 +397,55 @@ token_resident_kernel(const RowArgs a, const Resident p) {
     const float2 kk = make_float2(a.k, a.k);
     // A chunk on its way into registers; the return value is its largest logit.
     auto fetch = [&](int c, VT (&raw)[CV]) {
-      const Share& s = info.share;
-      const int v0 = c << (kLogCv + log_gd), n = min(s.n - v0, CV * gd), e0 = v0 * N;   // the chunk's vectors begin at v0, its elements at e0
+      const Raw* srow = reinterpret_cast<const Raw*>(ring + slot * piece_bytes) + tid;
       mbar_wait(full0 + 8 * slot, phase, abort_flag, 56, p.status);
-      Raw* srow = reinterpret_cast<Raw*>(ring + slot * piece_bytes);
-      T* selem = reinterpret_cast<T*>(srow);
-      // What is not to be summed (the neighbouring rows' elements, the target) becomes -inf in the slot, by the thread that reads the
-      // vector below.
-      const int tl = info.target - e0;
-      if (own && tl >= 0 && tl < n * N) {
-        if (((tl / N) & (gd - 1)) == tid) {
-          target_logit[group][par] = to_f32(selem[tl]);
-          selem[tl] = from_f32<T>(-INFINITY);
-          fence_proxy_async_smem();   // the slot's next copy comes behind these stores
-        }
-      }
-      if (info.edges) {
-        bool patched = false;
-        if (c == 0 && s.lo > 0 && tid == 0) {
-          for (int q = 0; q < s.lo; ++q) selem[q] = from_f32<T>(-INFINITY);
-          patched = true;
-        }
-        if (s.hi < s.n * N && s.n - 1 >= v0 && s.n - 1 < v0 + CV * gd && ((s.n - 1) & (gd - 1)) == tid) {
-          for (int q = s.hi; q < s.n * N; ++q) selem[q - e0] = from_f32<T>(-INFINITY);
-          patched = true;
-        }
-        if (patched) fence_proxy_async_smem();
-        if (tid < 2 * N) {   // the row's elements in those vectors are written one by one
-          const int el = tid < N ? s.lo + tid : s.fb * N + tid - N;
-          if (el >= e0 && el < e0 + n * N && (tid < N ? el < min(s.fa * N, s.hi) : el < s.hi)) edge[group][par][tid] = to_f32(selem[el - e0]);
-        }
-      }
       if constexpr (OP == kDistill) {
+        const T* selem = reinterpret_cast<const T*>(ring + slot * piece_bytes);
+        const int e0 = c << (kLogCv + log_gd) << (N == 8 ? 3 : 2);
         for (int q = tid; q < a.K; q += gd) {
           const int el = t_id[q] - e0;
-          if (t_id[q] < 0 || el < 0 || el >= n * N) continue;
+          if (t_id[q] < 0 || el < 0 || el >= CV * N * gd) continue;
           const float xq = to_f32(selem[el]);
           t_x[q] = xq;
           third -= t_q[q] * ((xq - x_ref) * a.inv_t);
         }
       }
-      if (n == CV * gd) {
+      if (!(info.special >> c & 1u)) {
 #pragma unroll
-        for (int j = 0; j < CV; ++j) raw[j].raw = srow[j * gd + tid];
+        for (int j = 0; j < CV; ++j) raw[j].raw = srow[j << log_gd];
       } else {
+        const Share& s = info.share;
+        const int v0 = c << (kLogCv + log_gd), n = min(s.n - v0, CV * gd), e0 = v0 * N;   // the chunk's vectors begin at v0, its elements at e0
+        T* selem = reinterpret_cast<T*>(ring + slot * piece_bytes);
+        const int tl = info.target - e0;
+        if (own && tl >= 0 && tl < n * N) {
+          if (((tl / N) & (gd - 1)) == tid) {
+            target_logit[group][par] = to_f32(selem[tl]);
+            selem[tl] = from_f32<T>(-INFINITY);
+            fence_proxy_async_smem();   // the slot's next copy comes behind these stores
+          }
+        }
+        if (info.special & kEdges) {
+          bool patched = false;
+          if (c == 0 && s.lo > 0 && tid == 0) {
+            for (int q = 0; q < s.lo; ++q) selem[q] = from_f32<T>(-INFINITY);
+            patched = true;
+          }
+          if (s.hi < s.n * N && s.n - 1 >= v0 && s.n - 1 < v0 + CV * gd && ((s.n - 1) & (gd - 1)) == tid) {
+            for (int q = s.hi; q < s.n * N; ++q) selem[q - e0] = from_f32<T>(-INFINITY);
+            patched = true;
+          }
+          if (patched) fence_proxy_async_smem();
+          if (tid < 2 * N) {   // the row's elements in those vectors are written one by one
+            const int el = tid < N ? s.lo + tid : s.fb * N + tid - N;
+            if (el >= e0 && el < e0 + n * N && (tid < N ? el < min(s.fa * N, s.hi) : el < s.hi)) edge[group][par][tid] = to_f32(selem[el - e0]);
+          }
+        }
 #pragma unroll
         for (int j = 0; j < CV; ++j) {
           uint32_t* w = reinterpret_cast<uint32_t*>(&raw[j].raw);
           w[0] = w[1] = w[2] = w[3] = Lane<T>::kMasked;
-          if (j * gd + tid < n) raw[j].raw = srow[j * gd + tid];
+          if (j * gd + tid < n) raw[j].raw = srow[j << log_gd];
         }
       }
       __syncwarp();
@@ -485,11 +490,22 @@ token_resident_kernel(const RowArgs a, const Resident p) {
     float cm;
     if constexpr (sizeof(T) == 2) {
       cm = fetch(0, raw);
+      VT next[CV];
+      float next_cm;
+      int c = 0;
 #pragma unroll 1
-      for (int c = 0; c < chunks - 1; ++c) {
-        VT next[CV];
-        const float next_cm = fetch(c + 1, next);
+      for (; c + 2 < chunks; c += 2) {
         float x[kChunk];
+        next_cm = fetch(c + 1, next);
+        exponentials(raw, cm, x);
+        keep(c, x);
+        cm = fetch(c + 2, raw);
+        exponentials(next, next_cm, x);
+        keep(c + 1, x);
+      }
+      if (c + 1 < chunks) {
+        float x[kChunk];
+        next_cm = fetch(c + 1, next);
         exponentials(raw, cm, x);
         keep(c, x);
 #pragma unroll
@@ -579,27 +595,28 @@ token_resident_kernel(const RowArgs a, const Resident p) {
     if (a.grad != nullptr) {
       const Share& s = info.share;
       T* g = static_cast<T*>(a.grad) + s.to;
-      // vectors [first vector, first vector + count) of chunk c, from their exponentials relative to r
+      // vectors j0 .. j0 + count of chunk c, from their exponentials times f
       auto put = [&](int c, int j0, const float* x, int count, float f) {
         const float2 ff = make_float2(f, f);
+        const int v0 = c << (kLogCv + log_gd);
+        const bool whole = SAME && v0 >= s.fa && v0 + CV * gd <= s.fb;   // all of the chunk's vectors are the row's alone
+        Raw* to = reinterpret_cast<Raw*>(g) + v0 + tid;
 #pragma unroll
         for (int j = 0; j < count; ++j) {
-          const int vi = ((c * CV + j0 + j) << log_gd) + tid;
           float y[N];
 #pragma unroll
           for (int q = 0; q < N; q += 2) {
             const float2 z = __fmul2_rn(make_float2(x[j * N + q], x[j * N + q + 1]), ff);
             y[q] = z.x; y[q + 1] = z.y;
           }
-          if (vi >= s.fa && vi < s.fb) {
-            if (SAME) {
-              VT t;
-              t.from_float(y);
-              __stcs(reinterpret_cast<Raw*>(g) + vi, t.raw);
-            } else {
+          const int vi = v0 + ((j0 + j) << log_gd) + tid;
+          if (SAME) {
+            VT t;
+            t.from_float(y);
+            if (whole || (vi >= s.fa && vi < s.fb)) __stcs(to + ((j0 + j) << log_gd), t.raw);
+          } else if (vi >= s.fa && vi < s.fb) {
 #pragma unroll
-              for (int q = 0; q < N; ++q) g[vi * N + q] = from_f32<T>(y[q]);
-            }
+            for (int q = 0; q < N; ++q) g[vi * N + q] = from_f32<T>(y[q]);
           }
         }
       };
@@ -630,7 +647,7 @@ token_resident_kernel(const RowArgs a, const Resident p) {
         const int tv = tl / N;
         if (tv >= s.fa && tv < s.fb && (tv & (gd - 1)) == tid) g[tl] = from_f32<T>(at_target);   // behind this thread's own vector
       }
-      if (info.edges && tid < 2 * N) {
+      if ((info.special & kEdges) && tid < 2 * N) {
         const int el = tid < N ? s.lo + tid : s.fb * N + tid - N;
         if (tid < N ? el < min(s.fa * N, s.hi) : el < s.hi)
           g[el] = from_f32<T>(el == tl ? at_target : f_top * ex2((edge[group][par][tid] - top) * a.k));
