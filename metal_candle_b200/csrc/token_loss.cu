@@ -27,7 +27,7 @@ __device__ __forceinline__ float block_max(float v, float* red) {
   return t;
 }
 
-// One block a row, two sweeps: maximum and sum, then the gradient.  Any V, alignment and stride.
+// Rows longer than the one-pass kernel takes: one block a row, three sweeps (maximum, sum, gradient).  Any alignment and stride.
 template <typename T, int OP>
 __global__ void __launch_bounds__(kRowThreads)
 token_rows_kernel(const RowArgs a) {
@@ -132,13 +132,7 @@ token_rows_kernel(const RowArgs a) {
   }
 }
 
-// The reverse of token log-probabilities whose softmax is known: dx_j = c (1[j = t] - exp(y_j - lse)), c = dlogp / T, for every
-// row, or one coefficient for each sequence of `coef_rows` rows.
-struct GradArgs {
-  RowArgs a;   // geometry, targets, logp and lse (read here), grad
-  const float* coef;
-  int64_t coef_rows;
-};
+// Gradients in place (see GradArgs): a block a row.
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
 token_grad_kernel(const GradArgs ga) {
@@ -337,11 +331,10 @@ int launch_sum(const float* terms, int64_t M, int n, float* out, cudaStream_t st
 
 template <int OP>
 int launch_rows(const RowArgs& a, const RowPlan& plan, int dtype, DeviceState* ds, cudaStream_t st) {
-  if (OP == kUnit || OP == kDistill || a.grad != nullptr) {
-    bool taken = false;
-    if (int rc = launch_resident_rows(OP, a, plan, dtype, ds, st, &taken)) return rc;
-    if (taken) return MCB_OK;
-  }
+  if (OP == kStats || (OP == kPolicy && a.grad == nullptr)) return launch_stats_rows(OP, a, plan, dtype, ds, st);
+  bool taken = false;
+  if (int rc = launch_resident_rows(OP, a, plan, dtype, ds, st, &taken)) return rc;
+  if (taken) return MCB_OK;
   const int64_t most = static_cast<int64_t>(ds->sm_count) * 8;
   const dim3 grid(static_cast<unsigned>(a.M < most ? a.M : most));
   if (dtype == MCB_F32)
@@ -353,6 +346,9 @@ int launch_rows(const RowArgs& a, const RowPlan& plan, int dtype, DeviceState* d
 }
 
 int launch_grad(const GradArgs& ga, int dtype, DeviceState* ds, cudaStream_t st) {
+  bool taken = false;
+  if (int rc = launch_grad_stream(ga, dtype, ds, st, &taken)) return rc;
+  if (taken) return MCB_OK;
   const int64_t most = static_cast<int64_t>(ds->sm_count) * 8;
   const dim3 grid(static_cast<unsigned>(ga.a.M < most ? ga.a.M : most));
   if (dtype == MCB_F32)

@@ -188,5 +188,17 @@ struct RowPlan {
 // The one-pass kernel (token_resident.cu), where it takes rows of this length: *taken says whether it did.
 int launch_resident_rows(int op, const RowArgs& a, const RowPlan& plan, int dtype, DeviceState* ds, cudaStream_t st, bool* taken);
 
+// The reverse of token log-probabilities whose softmax is known: dx_j = c (1[j = t] - exp(y_j - lse)), c = dlogp / T, dlogp of row i =
+// coef[i / coef_rows]; logp and lse of `a` are read.
+struct GradArgs {
+  RowArgs a;
+  const float* coef;
+  int64_t coef_rows;
+};
+
+// token_stream.cu: kStats, or kPolicy without a gradient; and the gradient, where it is not in place.
+int launch_stats_rows(int op, const RowArgs& a, const RowPlan& plan, int dtype, DeviceState* ds, cudaStream_t st);
+int launch_grad_stream(const GradArgs& ga, int dtype, DeviceState* ds, cudaStream_t st, bool* taken);
+
 }  // namespace tokenloss
 }  // namespace mcb
