@@ -162,51 +162,51 @@ token_grad_kernel(const GradArgs ga) {
 // The weight of each row in the mean: 1 / kept rows, or 1 / (kept rows of its sequence x sequences that keep any).  Kept are the
 // rows whose mask is not 0, or whose target is not left out; a target out of range gets NaN.  Neither given: all rows.
 // `order`, unless null: the kept rows first, in one fixed order, then the others; and info[0] = how many are kept, info[1] = 0.
+// One block: it is the longest chain in front of the losses of few rows, and 32768 targets are 256 KB.  Up to 8192 rows (and 2048
+// sequences) the targets are read once and stay in registers: 600 rows XXX us.
+constexpr int kSeqCounts = 2048;
 __global__ void __launch_bounds__(1024)
 row_weights_kernel(const void* targets, int target_bytes, int has_ignore, int64_t ignore, const uint8_t* mask, float* weight,
-                   int32_t* order, int32_t* info, int64_t M, int64_t S, int V, int sequence_mean) {
+                   int32_t* order, int32_t* info, int M, int S, int V, int sequence_mean) {
   __shared__ int red[32];
+  __shared__ int counts[kSeqCounts];
+  constexpr int kRows = 8, kRound = 1024 * kRows;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int sequences = M / S;
+  const bool counted = sequence_mean && sequences <= kSeqCounts;   // in shared memory, as the rows pass
+  if (counted)
+    for (int b = threadIdx.x; b < sequences; b += 1024) counts[b] = 0;
   grid_launch_dependents();
   grid_dependency_wait();
   targets = from_here(targets);
   mask = from_here(mask);
-  auto kept = [&](int64_t row) {   // 0, 1, or -1 for a target out of range
+  auto kept = [&](int row) {   // 0, 1, or -1 for a target out of range
     if (mask != nullptr) return mask[row] != 0 ? 1 : 0;
     if (targets == nullptr) return 1;
     const int t = read_target(targets, target_bytes, has_ignore, ignore, row, V);
     return t >= 0 ? 1 : t + 1;
   };
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int sequences = 0;
-  if (sequence_mean) {
-    for (int64_t b = warp; b < M / S; b += 32) {
-      int c = 0;
-      for (int64_t i = lane; i < S; i += 32) c += kept(b * S + i) != 0;
-      sequences += __reduce_add_sync(0xffffffffu, c) > 0;
-    }
-    if (lane == 0) red[warp] = sequences;
-    __syncthreads();
-    sequences = 0;
-    for (int w = 0; w < 32; ++w) sequences += red[w];
-  }
   // each warp takes 256 rows in a row, eight a lane; how many of those in front of it are kept is counted over the block
-  constexpr int kRows = 8;
-  const int rows = static_cast<int>(M);
+  int keep[kRows];
   int total = 0;
-  for (int64_t base = 0; base < M; base += 1024 * kRows) {
-    const int64_t mine = base + warp * 32 * kRows;
-    int keep[kRows];
+  for (int64_t base = 0; base < M; base += kRound) {
+    const int64_t mine = base + warp * 32 * kRows + lane;
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) keep[r] = mine + r * 32 + lane < M ? kept(mine + r * 32 + lane) != 0 : 0;
+    for (int r = 0; r < kRows; ++r) keep[r] = mine + r * 32 < M ? kept(static_cast<int>(mine) + r * 32) : 0;
     uint32_t votes[kRows];
     int c = 0;
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      votes[r] = __ballot_sync(0xffffffffu, keep[r]);
+      votes[r] = __ballot_sync(0xffffffffu, keep[r] != 0);
       c += __popc(votes[r]);
     }
-    __syncthreads();   // red is free
+    __syncthreads();   // red is free, counts are cleared
     if (lane == 0) red[warp] = c;
+    if (counted) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r)
+        if (keep[r] != 0) atomicAdd(counts + static_cast<int>(mine + r * 32) / S, 1);
+    }
     __syncthreads();
     c = red[lane];
     int at = total + __reduce_add_sync(0xffffffffu, lane < warp ? c : 0);   // kept rows before the warp's r-th 32
@@ -215,30 +215,57 @@ row_weights_kernel(const void* targets, int target_bytes, int has_ignore, int64_
     const uint32_t below = (1u << lane) - 1u;
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const int64_t row = mine + r * 32 + lane;
-      const int k = at + __popc(votes[r] & below);   // kept rows before this one: the others fill the order from its end
-      if (row < M) order[keep[r] ? k : rows - 1 - (static_cast<int>(row) - k)] = static_cast<int32_t>(row);
+      const int row = static_cast<int>(mine) + r * 32, k = at + __popc(votes[r] & below);
+      // k: kept rows before this one; the others fill the order from its end
+      if (mine + r * 32 < M) order[keep[r] != 0 ? k : M - 1 - (row - k)] = row;
       at += __popc(votes[r]);
     }
   }
   if (threadIdx.x == 0 && info != nullptr) { info[0] = total; info[1] = 0; }
+  float share = 1.0f / static_cast<float>(max(1, total));
   if (sequence_mean) {
-    const float share = 1.0f / static_cast<float>(max(1, sequences));
-    for (int64_t b = warp; b < M / S; b += 32) {
-      int c = 0;
-      for (int64_t i = lane; i < S; i += 32) c += kept(b * S + i) != 0;
-      c = __reduce_add_sync(0xffffffffu, c);
-      for (int64_t i = lane; i < S; i += 32) {
-        const int k = kept(b * S + i);
-        weight[b * S + i] = k == 0 ? 0.0f : k < 0 ? NAN : share / static_cast<float>(c);
+    // the sequences that keep any
+    int n = 0;
+    if (counted) {
+      for (int b = threadIdx.x; b < sequences; b += 1024) n += counts[b] > 0;
+    } else {
+      for (int b = warp; b < sequences; b += 32) {
+        int c = 0;
+        for (int i = lane; i < S; i += 32) c += kept(b * S + i) != 0;
+        c = __reduce_add_sync(0xffffffffu, c);
+        n += lane == 0 && c > 0;
       }
     }
-  } else {
-    const float share = 1.0f / static_cast<float>(total > 0 ? total : 1);
-    for (int64_t i = threadIdx.x; i < M; i += 1024) {
-      const int k = kept(i);
-      weight[i] = k == 0 ? 0.0f : k < 0 ? NAN : share;
+    n = __reduce_add_sync(0xffffffffu, n);
+    __syncthreads();
+    if (lane == 0) red[warp] = n;
+    __syncthreads();
+    n = __reduce_add_sync(0xffffffffu, red[lane]);
+    share = 1.0f / static_cast<float>(max(1, n));
+    if (!counted) {
+      for (int b = warp; b < sequences; b += 32) {
+        int c = 0;
+        for (int i = lane; i < S; i += 32) c += kept(b * S + i) != 0;
+        c = __reduce_add_sync(0xffffffffu, c);
+        for (int i = lane; i < S; i += 32) {
+          const int k = kept(b * S + i);
+          weight[b * S + i] = k == 0 ? 0.0f : k < 0 ? NAN : share / static_cast<float>(c);
+        }
+      }
+      return;
     }
+  }
+  auto put = [&](int row, int k) {
+    weight[row] = k == 0 ? 0.0f : k < 0 ? NAN : counted ? share / static_cast<float>(counts[row / S]) : share;
+  };
+  if (M <= kRound) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const int row = warp * 32 * kRows + lane + r * 32;
+      if (row < M) put(row, keep[r]);
+    }
+  } else {
+    for (int64_t i = threadIdx.x; i < M; i += 1024) put(static_cast<int>(i), kept(static_cast<int>(i)));
   }
 }
 
@@ -362,7 +389,7 @@ int launch_grad(const GradArgs& ga, int dtype, DeviceState* ds, cudaStream_t st)
 int launch_weights(const mcb_token_targets* t, const uint8_t* mask, float* weight, int32_t* order, int32_t* info, int64_t M, int64_t S,
                    int64_t V, int sequence_mean, cudaStream_t st) {
   MCB_CHECK_CUDA(launch_kernel(row_weights_kernel, dim3(1), dim3(1024), 0, st, chained_launch(), t ? t->targets : nullptr,
-                               t ? t->target_bytes : 0, t ? t->has_ignore : 0, t ? t->ignore_index : 0, mask, weight, order, info, M, S,
+                               t ? t->target_bytes : 0, t ? t->has_ignore : 0, t ? t->ignore_index : 0, mask, weight, order, info, static_cast<int>(M), static_cast<int>(S),
                                static_cast<int>(V), sequence_mean));
   MCB_CHECK_LAUNCH("row_weights");
   return MCB_OK;

@@ -734,6 +734,15 @@ int launch_resident(const RowArgs& a, const RowPlan& plan, DeviceState* ds, cuda
     else if (p.log_ctas < 3) ++p.log_ctas;
     else return MCB_OK;
   }
+  // Few rows: more of the SMs for each, first a whole SM (down to two vectors a thread), then a cluster (down to four).
+  while (true) {
+    const int64_t busy = (a.M * p.group_warps + kWarps - 1) / kWarps << p.log_ctas;
+    const int64_t each = vecs / (static_cast<int64_t>(p.group_warps) * 32 << p.log_ctas);   // vectors a thread
+    if (2 * busy > ds->sm_count) break;
+    if (p.group_warps < kWarps && each >= 4) p.group_warps *= 2;
+    else if (p.group_warps == kWarps && p.log_ctas < 3 && each >= 8) ++p.log_ctas;
+    else break;
+  }
   p.tmem = (vecs + (1 << p.log_ctas) - 1) >> p.log_ctas > static_cast<int64_t>(CV) * 32 * p.group_warps;
   p.ctas = 1 << p.log_ctas;
   p.log_groups = 0;

@@ -525,11 +525,11 @@ class PolicyLoss(NamedTuple):
     grad: Optional[torch.Tensor]
 
 
-def _on_device(t: torch.Tensor):
-    """The tensor's device as the current one: calls go to that device's current stream."""
+def _elsewhere(t: torch.Tensor) -> bool:
+    """Whether the tensor's device is not the current one.  (A context manager around every call would cost 3 us of some 20.)"""
     if not t.is_cuda:
         raise TrainingError("tensor is not on a CUDA device (this library has no CPU path)")
-    return torch.cuda.device(t.device)
+    return t.device.index != torch._C._cuda_getDevice()
 
 
 def _check_logits(logits: torch.Tensor) -> torch.Tensor:
@@ -544,11 +544,11 @@ def _check_logits(logits: torch.Tensor) -> torch.Tensor:
 def _check_like(logits: torch.Tensor, t: torch.Tensor, what: str, shape, dtypes) -> torch.Tensor:
     if t.device != logits.device:
         raise TrainingError(f"{what} is on {t.device}, the logits are on {logits.device}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise InvalidConfig(f"{what} must have shape {list(shape)}, got {list(t.shape)}")
     if t.dtype not in dtypes:
         raise TrainingError(f"{what} is {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 _INTEGERS, _FLOATS = (torch.int64, torch.int32), (torch.float32,)
@@ -570,7 +570,7 @@ def _token_targets(targets: torch.Tensor, ignore_index: Optional[int]):
 
 
 def _new_grad(logits: torch.Tensor, wanted: bool) -> Optional[torch.Tensor]:
-    return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if wanted else None
+    return torch.empty_like(logits, memory_format=torch.contiguous_format) if wanted else None
 
 
 def token_log_probs(logits: torch.Tensor, targets: torch.Tensor, ignore_index: Optional[int] = None, temperature: float = 1.0):
@@ -580,11 +580,13 @@ def token_log_probs(logits: torch.Tensor, targets: torch.Tensor, ignore_index: O
     B, S, _ = x.shape
     t = _check_like(x, targets, "targets", (B, S), _INTEGERS)
     rows = _token_logits(x, temperature)
-    with _on_device(x):
-        out = torch.empty(2, B, S, dtype=torch.float32, device=x.device)
-        _lib.check(backend._lib_for(x).mcb_token_logprob_fwd(rows, _token_targets(t, ignore_index), out[0].data_ptr(),
-                                                             out[1].data_ptr(), None, backend._stream()))
-    return out[0], out[1]
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return token_log_probs(x, t, ignore_index, temperature)
+    out = torch.empty(2, B, S, dtype=torch.float32, device=x.device)
+    to = out.data_ptr()
+    _lib.check(backend._lib_for(x).mcb_token_logprob_fwd(rows, _token_targets(t, ignore_index), to, to + 4 * B * S, None, backend._stream()))
+    return out.unbind()
 
 
 def token_log_probs_backward(logits: torch.Tensor, targets: torch.Tensor, log_probs: torch.Tensor, lse: torch.Tensor, dlogp: torch.Tensor,
@@ -596,10 +598,12 @@ def token_log_probs_backward(logits: torch.Tensor, targets: torch.Tensor, log_pr
     t = _check_like(x, targets, "targets", (B, S), _INTEGERS)
     log_probs, lse, dlogp = (_check_like(x, v, n, (B, S), _FLOATS) for v, n in ((log_probs, "log_probs"), (lse, "lse"), (dlogp, "dlogp")))
     rows = _token_logits(x, temperature)
-    with _on_device(x):
-        grad = _new_grad(x, True)
-        _lib.check(backend._lib_for(x).mcb_token_logprob_bwd(rows, _token_targets(t, ignore_index), log_probs.data_ptr(),
-                                                             lse.data_ptr(), dlogp.data_ptr(), 1, grad.data_ptr(), backend._stream()))
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return token_log_probs_backward(x, t, log_probs, lse, dlogp, ignore_index, temperature)
+    grad = _new_grad(x, True)
+    _lib.check(backend._lib_for(x).mcb_token_logprob_bwd(rows, _token_targets(t, ignore_index), log_probs.data_ptr(), lse.data_ptr(),
+                                                         dlogp.data_ptr(), 1, grad.data_ptr(), backend._stream()))
     return grad
 
 
@@ -623,15 +627,18 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, ref_log_probs: 
     _check_preference(beta, label_smoothing)
     t = _check_like(x, targets, "targets", (B, S), _INTEGERS)
     ref = _check_like(x, ref_log_probs, "ref_log_probs", (B,), _FLOATS)
-    with _on_device(x):
-        lib = backend._lib_for(x)
-        grad = _new_grad(x, return_grad)
-        out = torch.empty(B + 1, dtype=torch.float32, device=x.device)
-        ws = backend.workspace(x.device, lib.mcb_token_loss_workspace_bytes(B, S))
-        _lib.check(lib.mcb_preference_loss(_token_logits(x, 1.0), _token_targets(t, ignore_index), ref.data_ptr(), float(beta), float(label_smoothing),
-                                           int(bool(average_log_probs)), out[1:].data_ptr(), out.data_ptr(), backend._ptr(grad), ws.data_ptr(),
-                                           ws.numel(), backend._stream()))
-    return PreferenceLoss(out[:1], out[1:], grad)
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return preference_loss(x, t, ref, beta, label_smoothing, average_log_probs, ignore_index, return_grad)
+    lib = backend._lib_for(x)
+    grad = _new_grad(x, return_grad)
+    out = torch.empty(B + 1, dtype=torch.float32, device=x.device)
+    ws = backend.workspace(x.device, lib.mcb_token_loss_workspace_bytes(B, S))
+    to = out.data_ptr()
+    _lib.check(lib.mcb_preference_loss(_token_logits(x, 1.0), _token_targets(t, ignore_index), ref.data_ptr(), float(beta), float(label_smoothing),
+                                       int(bool(average_log_probs)), to + 4, to, backend._ptr(grad), ws.data_ptr(), ws.numel(),
+                                       backend._stream()))
+    return PreferenceLoss(*out.split((1, B)), grad)
 
 
 def _policy_terms(x, shape, advantages, old_log_probs, ref_log_probs, clip_low, clip_high, kl_coef):
@@ -666,16 +673,18 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, advantages: torch.T
     t = _check_like(x, targets, "targets", (B, S), _INTEGERS)
     held, terms = _policy_terms(x, (B, S), advantages, old_log_probs, ref_log_probs, clip_low, clip_high, kl_coef)
     rows = _token_logits(x, temperature)
-    with _on_device(x):
-        lib = backend._lib_for(x)
-        grad = _new_grad(x, return_grad)
-        logp = torch.empty(B, S, dtype=torch.float32, device=x.device)
-        out = torch.empty(3, dtype=torch.float32, device=x.device)
-        ws = backend.workspace(x.device, lib.mcb_token_loss_workspace_bytes(B, S))
-        _lib.check(lib.mcb_policy_loss(rows, _token_targets(t, ignore_index), terms, int(bool(sequence_mean)),
-                                       logp.data_ptr(), out.data_ptr(), backend._ptr(grad), ws.data_ptr(), ws.numel(), backend._stream()))
-    del held
-    return PolicyLoss(out[0:1], logp, out[1:2], out[2:3], grad)
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return policy_loss(x, t, *held, clip_low, clip_high, kl_coef, temperature, sequence_mean, ignore_index, return_grad)
+    lib = backend._lib_for(x)
+    grad = _new_grad(x, return_grad)
+    logp = torch.empty(B, S, dtype=torch.float32, device=x.device)
+    out = torch.empty(3, dtype=torch.float32, device=x.device)
+    ws = backend.workspace(x.device, lib.mcb_token_loss_workspace_bytes(B, S))
+    _lib.check(lib.mcb_policy_loss(rows, _token_targets(t, ignore_index), terms, int(bool(sequence_mean)), logp.data_ptr(), out.data_ptr(),
+                                   backend._ptr(grad), ws.data_ptr(), ws.numel(), backend._stream()))
+    loss, kl, clipped = out.split(1)
+    return PolicyLoss(loss, logp, kl, clipped, grad)
 
 
 def _teacher_top(x, shape, teacher_ids, teacher_logits, mask):
@@ -700,13 +709,15 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     B, S, _ = x.shape
     held, teacher = _teacher_top(x, (B, S), teacher_ids, teacher_logits, mask)
     rows = _token_logits(x, temperature)
-    with _on_device(x):
-        lib = backend._lib_for(x)
-        grad = _new_grad(x, return_grad)
-        loss = torch.empty(1, dtype=torch.float32, device=x.device)
-        ws = backend.workspace(x.device, lib.mcb_token_loss_workspace_bytes(B, S))
-        _lib.check(lib.mcb_distill_loss(rows, teacher, backend._ptr(held[2]), loss.data_ptr(), backend._ptr(grad),
-                                        ws.data_ptr(), ws.numel(), backend._stream()))
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return distillation_loss(x, *held, temperature, return_grad)
+    lib = backend._lib_for(x)
+    grad = _new_grad(x, return_grad)
+    loss = torch.empty(1, dtype=torch.float32, device=x.device)
+    ws = backend.workspace(x.device, lib.mcb_token_loss_workspace_bytes(B, S))
+    _lib.check(lib.mcb_distill_loss(rows, teacher, backend._ptr(held[2]), loss.data_ptr(), backend._ptr(grad), ws.data_ptr(), ws.numel(),
+                                    backend._stream()))
     return (loss, grad) if return_grad else loss
 
 
