@@ -74,6 +74,12 @@ __device__ __forceinline__ void combine(float& m, float& s, float m2, float s2, 
   m = mm;
 }
 
+// log(1 + x) for x >= 0, with w = 1 + x as rounded: log w scaled by how far w moved from 1 (W. Kahan's form), exact to a few
+// roundings where log w alone would have lost x
+__device__ __forceinline__ float log_plus_one(float x, float w) {
+  return w == 1.0f ? x : w > 2.0f ? logf(w) : logf(w) * __fdividef(x, w - 1.0f);
+}
+
 // A row's softmax around its target: (m, s) are those of the other columns.
 struct TargetStats {
   float top, sum;       // of the whole row
@@ -88,14 +94,14 @@ __device__ __forceinline__ TargetStats target_stats(float m, float s, float xt, 
   }
   const float d = (m - xt) * k;
   if (d <= 0.0f) {
-    const float odds = s * exp2f(d);
+    const float odds = s * ex2(d);
     r.top = xt; r.sum = 1.0f + odds;
-    r.logp = -log1pf(odds);
-    r.rest = odds / r.sum;
+    r.logp = -log_plus_one(odds, r.sum);
+    r.rest = __fdividef(odds, r.sum);
   } else {   // (NaN as well)
-    r.top = m; r.sum = s + exp2f(-d);
+    r.top = m; r.sum = s + ex2(-d);
     r.logp = -d * kLn2 - logf(r.sum);
-    r.rest = s / r.sum;
+    r.rest = __fdividef(s, r.sum);
   }
   return r;
 }
@@ -121,7 +127,7 @@ __device__ __forceinline__ RowInputs row_inputs(const RowArgs& a, int64_t row) {
 }
 __device__ __forceinline__ PolicyTerm policy_term(const RowArgs& a, const RowInputs& in, float logp) {
   const float adv = in.advantage;
-  const float ratio = a.old_logp != nullptr ? expf(logp - in.old_logp) : 1.0f;
+  const float ratio = a.old_logp != nullptr ? ex2((logp - in.old_logp) * kLog2e) : 1.0f;
   const float bounded = fminf(fmaxf(ratio, a.ratio_min), a.ratio_max);
   PolicyTerm t;
   // min(r A, clip(r) A): the bound holds only where it makes the term smaller

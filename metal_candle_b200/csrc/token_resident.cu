@@ -189,11 +189,12 @@ token_resident_kernel(const RowArgs a, const Resident p) {
   __shared__ __align__(16) float4 slots[kWarps / 2][2][8];   // by group, parity and CTA: (maximum, sum, target's logit or loss, whose target it is)
   __shared__ __align__(16) float4 row_end[kWarps / 2][2];    // what the second sweep needs: by group and parity
   __shared__ Feed feeds[kWarps];
-  __shared__ float3 red[2][kWarps];
+  __shared__ float2 red[2][kWarps];
   __shared__ float edge[kWarps][2][2 * N];                   // the share's elements in vectors that are not the row's alone
   __shared__ float target_logit[kWarps][2];
   __shared__ float refs[kTmemChunks][kThreads];              // what the chunks in tensor memory are relative to
-  __shared__ int repeats[kWarps][2];                         // an id that came twice among the row's teacher entries
+  __shared__ int repeats[kWarps][2];                         // whether an id came twice among the row's teacher entries
+  __shared__ __align__(16) float4 teachers[kWarps][2];       // its share of the loss, x_ref, whether it has no entry that counts
   __shared__ int abort_word, last;
   __shared__ uint32_t tmem_base;
   volatile int* abort_flag = &abort_word;
@@ -205,15 +206,15 @@ token_resident_kernel(const RowArgs a, const Resident p) {
   const int first = ((static_cast<int>(blockIdx.x) >> p.log_ctas) << p.log_groups) + group;
   const int step = (static_cast<int>(gridDim.x) >> p.log_ctas) << p.log_groups;
   const int piece_bytes = CV * 16 * gd;
-  // dynamic shared memory: the rows' descriptors, the rings, and (distillation) each group's teacher entries and bitmap of ids
+  // dynamic shared memory: the rows' descriptors, the rings, and (distillation) each group's teacher entries and bitmaps of ids, by parity
   RowInfo* infos = reinterpret_cast<RowInfo*>(smem) + group * (kInfoRows >> p.log_groups);
   const int info_rows = kInfoRows >> p.log_groups;
   uint8_t* ring = smem + kInfoRows * sizeof(RowInfo) + group * p.pieces * piece_bytes;
   const int bit_words = kMaxChunks * kChunk * gd / 32;
-  int* t_id = reinterpret_cast<int*>(smem + kInfoRows * sizeof(RowInfo) + groups * p.pieces * piece_bytes + group * (12 * a.K + 4 * bit_words));
-  float* t_q = reinterpret_cast<float*>(t_id + a.K);
-  float* t_x = t_q + a.K;
-  uint32_t* bits = reinterpret_cast<uint32_t*>(t_x + a.K);
+  int* t_id = reinterpret_cast<int*>(smem + kInfoRows * sizeof(RowInfo) + groups * p.pieces * piece_bytes + group * (24 * a.K + 8 * bit_words));
+  float* t_q = reinterpret_cast<float*>(t_id + 2 * a.K);
+  float* t_x = t_q + 2 * a.K;
+  uint32_t* t_bits = reinterpret_cast<uint32_t*>(t_x + 2 * a.K);
   const uint32_t full0 = smem_u32(full[group]), empty0 = smem_u32(empty[group]);
   auto group_sync = [&]() {
     if (p.group_warps == 1) __syncwarp();
@@ -222,12 +223,12 @@ token_resident_kernel(const RowArgs a, const Resident p) {
   if (threadIdx.x == 0) *abort_flag = 0;
   if (tid == 0) {
     for (int i = 0; i < p.pieces; ++i) { mbar_init(full0 + 8 * i, 1); mbar_init(empty0 + 8 * i, p.group_warps); }
-    for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&slot_bars[group][i]), 1); repeats[group][i] = 0; }
+    for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&slot_bars[group][i]), 1); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async_smem();
   }
   if constexpr (OP == kDistill)
-    for (int i = tid; i < bit_words; i += gd) bits[i] = 0;
+    for (int i = tid; i < 2 * bit_words; i += gd) t_bits[i] = 0;
   if (ctas > 1) cl.sync(); else __syncthreads();   // every CTA's barriers exist before a peer arrives on them
   grid_dependency_wait();
   if (p.tmem) {
@@ -247,7 +248,8 @@ token_resident_kernel(const RowArgs a, const Resident p) {
   const uint32_t kept = p.kept != nullptr ? static_cast<uint32_t>(*from_here(p.kept)) : M;
   auto row_of = [&](uint32_t i) -> int { return p.order != nullptr ? from_here(p.order)[i] : static_cast<int>(i); };
   auto state_of = [&](uint32_t i, int row) {   // 0: to be computed, 1: left out, 2: out of range
-    if (OP == kDistill || i >= kept) return i < kept ? 0 : 1;
+    if (i >= kept) return 1;
+    if (OP == kDistill) return a.weight[row] == 0.0f ? 1 : 0;
     const int t = read_target(a.targets, a.target_bytes, a.has_ignore, a.ignore, row, a.V);
     return t >= 0 ? 0 : t == -2 ? 2 : 1;
   };
@@ -347,49 +349,87 @@ token_resident_kernel(const RowArgs a, const Resident p) {
       }
       continue;
     }
-    float third = 0.0f, x_ref = 0.0f;
-    bool empty_teacher = false;
-    if constexpr (OP == kDistill) {
-      // the teacher's distribution over its entries: each warp takes all of them
-      const int64_t t0 = static_cast<int64_t>(info.row) * a.K;
-      float tm = -INFINITY, ts = 0.0f;
-      for (int q = lane; q < a.K; q += 32) tm = fmaxf(tm, read_teacher(a, t0 + q));
-      tm = warp_max(tm);
-      const float tref = tm == -INFINITY ? 0.0f : tm;
-      int64_t best = -1;
-      for (int q = lane; q < a.K; q += 32) {
-        const float t = read_teacher(a, t0 + q);
-        ts += exp2f((t - tref) * a.k);
-        if (t == tm && best < 0) best = read_teacher_id(a, t0 + q);
-      }
-      ts = warp_sum(ts);
-      empty_teacher = ts == 0.0f;
-      // the student's logit where the teacher's is largest: the loss's logits are taken relative to it
-      const uint32_t who = __ballot_sync(0xffffffffu, best >= 0);
-      best = __shfl_sync(0xffffffffu, best, who == 0 ? 0 : __ffs(who) - 1);
-      if (best >= 0 && best < a.V) x_ref = to_f32(static_cast<const T*>(a.logits)[row_offset(a, info.row) + best]);
-      if (!(fabsf(x_ref) < INFINITY)) x_ref = 0.0f;
-      // its entries within this share: where, how likely, and what they add to the loss besides the student's logit
-      const float inv_ts = 1.0f / ts, log_ts = logf(ts);
-      const Share& s = info.share;
-      for (int q = tid; q < a.K; q += gd) {
-        const float d = read_teacher(a, t0 + q) - tref;   // log q = d / T - log_ts
-        const float prob = empty_teacher ? 0.0f : exp2f(d * a.k) * inv_ts;
-        int el = -1;
-        if (prob != 0.0f) {   // (NaN counts)
-          const int64_t id = read_teacher_id(a, t0 + q);
-          if (id < 0 || id >= a.V) {
-            third = NAN;
-          } else if (id - s.column >= s.lo && id - s.column < s.hi) {
-            el = static_cast<int>(id - s.column);
-            third += prob * (d * a.inv_t - log_ts);
-            if (atomicOr(bits + (el >> 5), 1u << (el & 31)) >> (el & 31) & 1u) repeats[group][par] = 1;
+    float third = 0.0f;
+    // Distillation: the row's teacher, by one warp, in three parts between the first sweep's chunks, so that the global loads of each pass
+    // under a chunk: its entries (two a lane; more than 64 are read where they are needed); q = softmax(t / T), those with -inf
+    // counting for nothing, and of the entries whose column is in this share where it is (or -1), q, and a request for the student's
+    // logit; then the sum of q (log q - (x - x_ref) / T), with x_ref the student's logit where the teacher's is largest.
+    const bool teaches = OP == kDistill && (tid >> 5) == (p.group_warps > 2 ? 1 : 0);
+    float t_in[2] = {-INFINITY, -INFINITY}, x_in[2], x_ref = 0.0f;
+    int64_t id_in[2] = {-1, -1};
+    int taught = 0;   // parts done
+    auto teach = [&]() {
+      if constexpr (OP == kDistill) {
+        const int64_t t0 = static_cast<int64_t>(info.row) * a.K;
+        const T* x_row = static_cast<const T*>(a.logits) + row_offset(a, info.row);
+        if (taught == 0) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (lane + 32 * h < a.K) { t_in[h] = read_teacher(a, t0 + lane + 32 * h); id_in[h] = read_teacher_id(a, t0 + lane + 32 * h); }
+        } else if (taught == 1) {
+          float tm = fmaxf(t_in[0], t_in[1]), ts, loss = 0.0f;
+          for (int q = lane + 64; q < a.K; q += 32) tm = fmaxf(tm, read_teacher(a, t0 + q));
+          tm = warp_max(tm);
+          const float tref = tm == -INFINITY ? 0.0f : tm;
+          ts = exp2f((t_in[0] - tref) * a.k) + exp2f((t_in[1] - tref) * a.k);
+          int64_t best = t_in[0] == tm && lane < a.K ? id_in[0] : t_in[1] == tm && lane + 32 < a.K ? id_in[1] : -1;
+          for (int q = lane + 64; q < a.K; q += 32) {
+            const float t = read_teacher(a, t0 + q);
+            ts += exp2f((t - tref) * a.k);
+            if (t == tm && best < 0) best = read_teacher_id(a, t0 + q);
           }
+          ts = warp_sum(ts);
+          const uint32_t who = __ballot_sync(0xffffffffu, best >= 0);
+          best = __shfl_sync(0xffffffffu, best, who == 0 ? 0 : __ffs(who) - 1);
+          if (best >= 0 && best < a.V) x_ref = to_f32(x_row[best]);
+          const float inv_ts = 1.0f / ts, log_ts = logf(ts);
+          bool twice = false;
+          auto entry = [&](int q, float t, int64_t id) {
+            const float d = t - tref;   // log q = d / T - log_ts
+            const float prob = ts == 0.0f ? 0.0f : exp2f(d * a.k) * inv_ts;
+            int el = -1;
+            if (prob != 0.0f) {   // (NaN counts)
+              if (id < 0 || id >= a.V) {
+                loss = NAN;
+              } else if (id - info.share.column >= info.share.lo && id - info.share.column < info.share.hi) {
+                el = static_cast<int>(id - info.share.column);
+                loss += prob * (d * a.inv_t - log_ts);
+                twice |= atomicOr(t_bits + par * bit_words + (el >> 5), 1u << (el & 31)) >> (el & 31) & 1u;
+              }
+            }
+            t_id[par * a.K + q] = el;
+            t_q[par * a.K + q] = prob;
+            return el;
+          };
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            x_in[h] = 0.0f;
+            if (lane + 32 * h < a.K && entry(lane + 32 * h, t_in[h], id_in[h]) >= 0) x_in[h] = to_f32(x_row[id_in[h]]);
+          }
+          for (int q = lane + 64; q < a.K; q += 32) {
+            const int64_t id = read_teacher_id(a, t0 + q);
+            if (entry(q, read_teacher(a, t0 + q), id) >= 0) t_x[par * a.K + q] = to_f32(x_row[id]);
+          }
+          loss = warp_sum(loss);
+          twice = __any_sync(0xffffffffu, twice);
+          if (lane == 0) { teachers[group][par] = make_float4(loss, 0.0f, ts == 0.0f ? 1.0f : 0.0f, 0.0f); repeats[group][par] = twice; }
+        } else {
+          if (!(fabsf(x_ref) < INFINITY)) x_ref = 0.0f;
+          float loss = 0.0f;
+          for (int q = lane; q < a.K; q += 32) {
+            if (t_id[par * a.K + q] < 0) continue;
+            const float x = q < 32 ? x_in[0] : q < 64 ? x_in[1] : t_x[par * a.K + q];
+            t_x[par * a.K + q] = x;
+            loss -= t_q[par * a.K + q] * ((x - x_ref) * a.inv_t);
+          }
+          loss = warp_sum(loss);
+          if (lane == 0) { teachers[group][par].x += loss; teachers[group][par].y = x_ref; }
         }
-        t_id[q] = el;
-        t_q[q] = prob;
+        ++taught;
+        __syncwarp();
       }
-    }
+    };
+    if (teaches) teach();
     // first sweep
     const bool own = info.target >= 0;
     float m = -INFINITY, sw = 0.0f, e[kChunk];
@@ -399,17 +439,6 @@ token_resident_kernel(const RowArgs a, const Resident p) {
     auto fetch = [&](int c, VT (&raw)[CV]) {
       const Raw* srow = reinterpret_cast<const Raw*>(ring + slot * piece_bytes) + tid;
       mbar_wait(full0 + 8 * slot, phase, abort_flag, 56, p.status);
-      if constexpr (OP == kDistill) {
-        const T* selem = reinterpret_cast<const T*>(ring + slot * piece_bytes);
-        const int e0 = c << (kLogCv + log_gd) << (N == 8 ? 3 : 2);
-        for (int q = tid; q < a.K; q += gd) {
-          const int el = t_id[q] - e0;
-          if (t_id[q] < 0 || el < 0 || el >= CV * N * gd) continue;
-          const float xq = to_f32(selem[el]);
-          t_x[q] = xq;
-          third -= t_q[q] * ((xq - x_ref) * a.inv_t);
-        }
-      }
       if (!(info.special >> c & 1u)) {
 #pragma unroll
         for (int j = 0; j < CV; ++j) raw[j].raw = srow[j << log_gd];
@@ -456,7 +485,7 @@ token_resident_kernel(const RowArgs a, const Resident p) {
       return Lane<T>::max_of(raw);
     };
     // Its exponentials, relative to the thread's largest logit so far, m.
-    auto exponentials = [&](const VT (&raw)[CV], float cm, float (&x)[kChunk]) {
+    auto exponentials = [&](const VT (&raw)[CV], float cm, float (&x)[kChunk], int n = 1 << 20) {   // n: the chunk's vectors, if it may not be full
       const float mm = fmaxf(m, cm);
       if (mm > m && m != -INFINITY) sw *= ex2((m - mm) * a.k);
       m = mm;
@@ -465,6 +494,11 @@ token_resident_kernel(const RowArgs a, const Resident p) {
       float2 s2 = make_float2(0.0f, 0.0f);
 #pragma unroll
       for (int j = 0; j < CV; ++j) {
+        if (j > 0 && (j << log_gd) >= n) {   // nobody has one (the last chunk)
+#pragma unroll
+          for (int q = 0; q < N; ++q) x[j * N + q] = 0.0f;
+          continue;
+        }
         float f[N];
         raw[j].to_float(f);
 #pragma unroll
@@ -499,6 +533,7 @@ token_resident_kernel(const RowArgs a, const Resident p) {
         next_cm = fetch(c + 1, next);
         exponentials(raw, cm, x);
         keep(c, x);
+        if (teaches && taught == 1) teach();
         cm = fetch(c + 2, raw);
         exponentials(next, next_cm, x);
         keep(c + 1, x);
@@ -519,23 +554,24 @@ token_resident_kernel(const RowArgs a, const Resident p) {
         cm = fetch(c, raw);
         exponentials(raw, cm, x);
         keep(c, x);
+        if (teaches && taught == 1) teach();
       }
       cm = fetch(chunks - 1, raw);
     }
-    exponentials(raw, cm, e);
+    if (teaches && taught == 1) teach();
+    exponentials(raw, cm, e, info.share.n - ((chunks - 1) << (kLogCv + log_gd)));
     const float ref_e = m;
+    if (teaches) teach();
     float mw = m;
     warp_combine(mw, sw, a.k);
-    if constexpr (OP == kDistill) third = warp_sum(third);
     if (chunks > 1) tmem_st_wait();
     if (p.group_warps > 1) {
-      if (lane == 0) red[par][warp] = make_float3(mw, sw, third);
+      if (lane == 0) red[par][warp] = make_float2(mw, sw);
       group_sync();
       if (tid < 32) {
-        const float3 r = lane < p.group_warps ? red[par][group * p.group_warps + lane] : make_float3(-INFINITY, 0.0f, 0.0f);
+        const float2 r = lane < p.group_warps ? red[par][group * p.group_warps + lane] : make_float2(-INFINITY, 0.0f);
         mw = r.x; sw = r.y;
         warp_combine(mw, sw, a.k, p.group_warps);
-        if constexpr (OP == kDistill) third = warp_sum(r.z);
       } else if (tid == feeder) {
         feed();   // the slot of the row's last piece
       }
@@ -544,8 +580,8 @@ token_resident_kernel(const RowArgs a, const Resident p) {
       if (tid == feeder) feed();
       __syncwarp();
     }
-    if (OP == kDistill && tid == 0) repeats[group][par ^ 1] = 0;   // the row before is done with it, the next one not begun
-    if (OP != kDistill && own) third = target_logit[group][par];
+    if constexpr (OP == kDistill) third = teachers[group][par].x;
+    else if (own) third = target_logit[group][par];
     const int row = info.row;
     const bool writes = rank == 0 && tid == 0;
     float f_top, top, c0, at_target = 0.0f;   // an element's gradient is f_top 2^((x - top) k)
@@ -572,7 +608,8 @@ token_resident_kernel(const RowArgs a, const Resident p) {
       if constexpr (OP == kDistill) {
         const float w = info.in.weight;
         top = mw == -INFINITY ? 0.0f : mw;
-        const float loss = empty_teacher ? 0.0f : third + ((top - x_ref) * a.inv_t + logf(sw));
+        const bool empty_teacher = teachers[group][par].z != 0.0f;
+        const float loss = empty_teacher ? 0.0f : third + ((top - teachers[group][par].y) * a.inv_t + logf(sw));
         if (writes) a.terms[row] = w * (a.temperature * a.temperature) * loss;
         c0 = empty_teacher ? 0.0f : w * a.temperature + (isnan(loss) ? NAN : 0.0f);
         f_top = empty_teacher ? 0.0f : c0 / sw;
@@ -603,6 +640,7 @@ token_resident_kernel(const RowArgs a, const Resident p) {
         Raw* to = reinterpret_cast<Raw*>(g) + v0 + tid;
 #pragma unroll
         for (int j = 0; j < count; ++j) {
+          if (j > 0 && v0 + ((j0 + j) << log_gd) >= s.fb) break;
           float y[N];
 #pragma unroll
           for (int q = 0; q < N; q += 2) {
@@ -654,28 +692,31 @@ token_resident_kernel(const RowArgs a, const Resident p) {
       }
       if constexpr (OP == kDistill) {
         group_sync();   // the row's softmax is written before its teacher columns are
+        const int* ids = t_id + par * a.K;
+        const float* probs = t_q + par * a.K;
         const bool twice = repeats[group][par] != 0;
         for (int q = tid; q < a.K; q += gd) {
-          const int el = t_id[q];
+          const int el = ids[q];
           if (el < 0) continue;
-          float prob = t_q[q];
+          float prob = probs[q];
           bool mine = true;
           if (twice) {   // the first of those that name the same column writes the sum of them
             prob = 0.0f;
             for (int o = 0; o < a.K; ++o) {
-              if (t_id[o] != el) continue;
+              if (ids[o] != el) continue;
               if (o < q) { mine = false; break; }
-              prob += t_q[o];
+              prob += probs[o];
             }
           }
-          if (mine) g[el] = from_f32<T>(c0 * (exp2f((t_x[q] - top) * a.k) / sw - prob));
+          if (mine) g[el] = from_f32<T>(c0 * (exp2f((t_x[par * a.K + q] - top) * a.k) / sw - prob));
         }
       }
     }
-    if constexpr (OP == kDistill) {
+    if constexpr (OP == kDistill) {   // (this parity's entries are made again behind the next row's first barrier)
+      if (p.group_warps == 1) __syncwarp();
       for (int q = tid; q < a.K; q += gd)
-        if (t_id[q] >= 0) bits[t_id[q] >> 5] = 0;
-      group_sync();   // the entries are free for the next row's
+        if (t_id[par * a.K + q] >= 0) t_bits[par * bit_words + (t_id[par * a.K + q] >> 5)] = 0;
+      if (p.group_warps == 1) __syncwarp();
     }
     par ^= 1;
   }
@@ -751,7 +792,7 @@ int launch_resident(const RowArgs& a, const RowPlan& plan, DeviceState* ds, cuda
   p.order = plan.order; p.kept = plan.kept; p.out = plan.sums; p.n_out = plan.n_sums; p.done = plan.done; p.status = ds->status_word;
   const int64_t fixed = kInfoRows * sizeof(RowInfo), most = 210 * 1024;
   const int64_t slot = static_cast<int64_t>(kThreads) * kChunk * sizeof(T);   // one ring slot of every group
-  auto teacher = [&]() { return OP == kDistill ? (kWarps / p.group_warps) * (12 * static_cast<int64_t>(a.K) + 4 * kMaxChunks * kChunk * p.group_warps) : 0; };
+  auto teacher = [&]() { return OP == kDistill ? (kWarps / p.group_warps) * (24 * static_cast<int64_t>(a.K) + 8 * kMaxChunks * kChunk * p.group_warps) : 0; };
   while (fixed + teacher() + 2 * slot > most) {
     if (p.group_warps == kWarps) return MCB_OK;
     p.group_warps *= 2;

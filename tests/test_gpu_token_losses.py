@@ -492,6 +492,64 @@ def test_gradients_in_place(cuda_device):
             check_grad(unit, wg, 2 * spread)
 
 
+@both
+@pytest.mark.parametrize("V", [300, 2049, 32000, 151936])
+def test_rows_of_a_chunk(cuda_device, dtype, V):
+    """The stages for a caller that makes the logits a chunk at a time: the whole calls' results, in place too, and rows that are left
+    out are not looked at.  How a row is split over the chip depends on how many there are, so the sums' order does: both sides
+    are off by the tolerance above, a gradient by half a step each."""
+
+    def agree(got, want):
+        check_grad(got, want.double(), want.double().abs(), 1e-4 + half(dtype))
+
+    import ctypes as C
+
+    B, S, K = 3, 7, 6
+    x, t, g = make(cuda_device, B, S, V, dtype, 15)
+    ids, tl = teacher(cuda_device, g, B, S, V, K, dtype)
+    t[0, 2] = IGN
+    t[2] = IGN
+    mask = t != IGN
+    A = torch.randn(B, S, device=cuda_device, generator=g)
+    want_p = F.policy_loss(x, t, A, sequence_mean=True, ignore_index=IGN, return_grad=True)
+    want_d = F.distillation_loss(x, ids, tl, mask=mask, temperature=1.5, return_grad=True)
+    x = torch.where(mask[..., None], x, torch.full_like(x, math.nan))
+    lib, st, M = _lib.load(), torch.cuda.current_stream().cuda_stream, B * S
+    code = int(dtype == BF)
+    new = lambda *s: torch.empty(*s, device=cuda_device)  # noqa: E731
+    targets = lambda c: C.byref(_lib.TokenTargets(t.view(M)[c:].data_ptr(), 8, 1, IGN))  # noqa: E731
+    w = new(M)
+    for in_place in (False, True):
+        y = x.clone().view(M, V)
+        to = y if in_place else torch.empty_like(y)
+        _lib.check(lib.mcb_loss_weights(targets(0), None, w.data_ptr(), B, S, V, 1, st))
+        logp, parts = new(M), []
+        for c0, c1 in ((0, 4), (4, 5), (5, 15), (15, M)):
+            rows = C.byref(_lib.TokenLogits(y[c0:].data_ptr(), 1, c1 - c0, V, (c1 - c0) * V, V, 1.0, code))
+            parts.append(new(3, c1 - c0))
+            _lib.check(lib.mcb_policy_loss_rows(rows, targets(c0), C.byref(_lib.PolicyTerms(A.view(M)[c0:].data_ptr(), 1, None, None, 0.2, 0.2, 0.0, 0)),
+                                                w[c0:].data_ptr(), logp[c0:].data_ptr(), parts[-1].data_ptr(), to[c0:].data_ptr(), st))
+        out, terms = new(3), torch.cat(parts, 1)
+        _lib.check(lib.mcb_loss_sums(terms.data_ptr(), M, 3, out.data_ptr(), st))
+        agree(to.view(B, S, V), want_p.grad)
+        assert ((logp.view(B, S) - want_p.log_probs).abs() <= 4e-5 + 2e-6 * want_p.log_probs.abs()).all()
+        assert abs(float(out[0]) - float(want_p.loss)) <= 1e-4
+        y = x.clone().view(M, V)
+        to = y if in_place else torch.empty_like(y)
+        m8 = mask.to(torch.uint8)
+        _lib.check(lib.mcb_loss_weights(None, m8.data_ptr(), w.data_ptr(), B, S, V, 0, st))
+        parts = []
+        for c0, c1 in ((0, 6), (6, 16), (16, M)):
+            rows = C.byref(_lib.TokenLogits(y[c0:].data_ptr(), 1, c1 - c0, V, (c1 - c0) * V, V, 1.5, code))
+            top = C.byref(_lib.TeacherTop(ids.view(M, K)[c0:].data_ptr(), tl.view(M, K)[c0:].data_ptr(), K, 8, code))
+            parts.append(new(c1 - c0))
+            _lib.check(lib.mcb_distill_loss_rows(rows, top, w[c0:].data_ptr(), parts[-1].data_ptr(), to[c0:].data_ptr(), st))
+        terms = torch.cat(parts)
+        _lib.check(lib.mcb_loss_sums(terms.data_ptr(), M, 1, out.data_ptr(), st))
+        agree(to.view(B, S, V), want_d[1])
+        assert abs(float(out[0]) - float(want_d[0])) <= 6e-5 * (1 + float(want_d[0]))
+
+
 def test_another_current_stream_and_memory_around(cuda_device):
     """Nothing but the outputs is written: the bytes around a gradient that starts off a 16-byte boundary stay."""
     import ctypes as C
