@@ -20,6 +20,8 @@
 // have one order.
 #include <cooperative_groups.h>
 
+#include <float.h>
+
 #include <mutex>
 
 #include "token_loss.cuh"
@@ -291,6 +293,108 @@ token_resident_kernel(const RowArgs a, const Resident p) {
     feeds[group] = f;
   };
 
+  // Distillation: a row's teacher, by one warp, in three parts under the row before, so that nothing waits for the global loads of each:
+  // its entries (two a lane; more than 64 are read where they are needed); q = softmax(t / T), those with -inf counting for nothing, and
+  // of the entries whose column is in this share where it is (or -1), q, and a request for the student's logit; then the sum of
+  // q (log q - (x - x_ref) / T), with x_ref the student's logit where the teacher's is largest.
+  const bool teaches = OP == kDistill && (tid >> 5) == (p.group_warps > 1 ? 1 : 0);
+  uint32_t prepared = 0xffffffffu;   // the place of the row that the first part, or the first two, were done for
+  uint32_t t_in[2], x_in[2], x_ref = 0;   // as loaded: a conversion would wait for the load
+  int64_t id_in[2];
+  auto load_bits = [](const T* x) -> uint32_t {
+    if constexpr (sizeof(T) == 2) return *reinterpret_cast<const uint16_t*>(x); else return *reinterpret_cast<const uint32_t*>(x);
+  };
+  auto logit_of = [](uint32_t bits) { return __uint_as_float(sizeof(T) == 2 ? bits << 16 : bits); };
+  auto id_of = [&](int64_t id) { return id >= 0 && id < a.V ? static_cast<int>(id) : -1; };
+  auto teach_load = [&](const RowInfo& info) {
+    const int64_t t0 = static_cast<int64_t>(info.row) * a.K;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int q = lane + 32 * h;
+      t_in[h] = 0;
+      id_in[h] = 0;
+      if (q < a.K) {
+        t_in[h] = a.teacher_f32 ? static_cast<const uint32_t*>(a.teacher)[t0 + q] : static_cast<const uint16_t*>(a.teacher)[t0 + q];
+        id_in[h] = a.id_bytes == 8 ? static_cast<const int64_t*>(a.teacher_ids)[t0 + q] : static_cast<const uint32_t*>(a.teacher_ids)[t0 + q];
+      }
+    }
+  };
+  auto teach_weigh = [&](const RowInfo& info, int into) {
+    const int64_t t0 = static_cast<int64_t>(info.row) * a.K;
+    const T* x_row = static_cast<const T*>(a.logits) + row_offset(a, info.row);
+    float t[2];
+    int id[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      t[h] = lane + 32 * h < a.K ? __uint_as_float(a.teacher_f32 ? t_in[h] : t_in[h] << 16) : -INFINITY;
+      id[h] = id_of(a.id_bytes == 8 ? id_in[h] : static_cast<int32_t>(id_in[h]));
+    }
+    float tm = fmaxf(t[0], t[1]);
+    for (int q = lane + 64; q < a.K; q += 32) tm = fmaxf(tm, read_teacher(a, t0 + q));
+    tm = warp_max(tm);
+    const float tref = tm == -INFINITY ? 0.0f : tm;
+    float e[2] = {ex2((t[0] - tref) * a.k), ex2((t[1] - tref) * a.k)};
+    float ts = e[0] + e[1];
+    int best = t[0] == tm && lane < a.K ? id[0] : t[1] == tm && lane + 32 < a.K ? id[1] : -1;
+    for (int q = lane + 64; q < a.K; q += 32) {
+      const float v = read_teacher(a, t0 + q);
+      ts += ex2((v - tref) * a.k);
+      if (v == tm && best < 0) best = id_of(read_teacher_id(a, t0 + q));
+    }
+    ts = warp_sum(ts);
+    const uint32_t who = __ballot_sync(0xffffffffu, best >= 0);
+    best = __shfl_sync(0xffffffffu, best, who == 0 ? 0 : __ffs(who) - 1);
+    x_ref = best >= 0 ? load_bits(x_row + best) : 0;
+    const float inv_ts = ts == 0.0f ? 0.0f : 1.0f / ts, log_ts = logf(ts);
+    const int column = info.share.column, lo = info.share.lo, hi = info.share.hi;
+    float loss = 0.0f;
+    bool twice = false;
+    auto entry = [&](int q, float v, float exponential, int id) {
+      const float prob = exponential * inv_ts;
+      int el = -1;
+      if (prob != 0.0f) {   // (NaN counts)
+        if (id < 0) {
+          loss = NAN;
+        } else if (id - column >= lo && id - column < hi) {
+          el = id - column;
+          loss += prob * ((v - tref) * a.inv_t - log_ts);   // log q
+          twice |= atomicOr(t_bits + into * bit_words + (el >> 5), 1u << (el & 31)) >> (el & 31) & 1u;
+        }
+      }
+      t_id[into * a.K + q] = el;
+      t_q[into * a.K + q] = prob;
+      return el;
+    };
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      x_in[h] = 0;
+      if (lane + 32 * h < a.K && entry(lane + 32 * h, t[h], e[h], id[h]) >= 0) x_in[h] = load_bits(x_row + id[h]);
+    }
+    for (int q = lane + 64; q < a.K; q += 32) {
+      const int named = id_of(read_teacher_id(a, t0 + q));
+      const float v = read_teacher(a, t0 + q);
+      if (entry(q, v, ex2((v - tref) * a.k), named) >= 0) t_x[into * a.K + q] = to_f32(x_row[named]);
+    }
+    loss = warp_sum(loss);
+    twice = __any_sync(0xffffffffu, twice);
+    if (lane == 0) { teachers[group][into] = make_float4(loss, 0.0f, ts == 0.0f ? 1.0f : 0.0f, 0.0f); repeats[group][into] = twice; }
+    __syncwarp();
+  };
+  auto teach_sum = [&](int into) {
+    float x0 = logit_of(x_ref);
+    if (!(fabsf(x0) < INFINITY)) x0 = 0.0f;
+    float loss = 0.0f;
+    for (int q = lane; q < a.K; q += 32) {
+      if (t_id[into * a.K + q] < 0) continue;
+      const float x = q < 32 ? logit_of(x_in[0]) : q < 64 ? logit_of(x_in[1]) : t_x[into * a.K + q];
+      t_x[into * a.K + q] = x;
+      loss -= t_q[into * a.K + q] * ((x - x0) * a.inv_t);
+    }
+    loss = warp_sum(loss);
+    if (lane == 0) { teachers[group][into].x += loss; teachers[group][into].y = x0; }
+    __syncwarp();
+  };
+
   uint32_t phase = 0, slot_phase = 0;   // parities of the ring's current round, and (bit i) of slot barrier i
   int slot = 0, par = 0, at = info_rows;
   for (uint32_t i = first; i < M; i += step, ++at) {   // (M and the step are below 2^31)
@@ -350,86 +454,13 @@ token_resident_kernel(const RowArgs a, const Resident p) {
       continue;
     }
     float third = 0.0f;
-    // Distillation: the row's teacher, by one warp, in three parts between the first sweep's chunks, so that the global loads of each pass
-    // under a chunk: its entries (two a lane; more than 64 are read where they are needed); q = softmax(t / T), those with -inf
-    // counting for nothing, and of the entries whose column is in this share where it is (or -1), q, and a request for the student's
-    // logit; then the sum of q (log q - (x - x_ref) / T), with x_ref the student's logit where the teacher's is largest.
-    const bool teaches = OP == kDistill && (tid >> 5) == (p.group_warps > 2 ? 1 : 0);
-    float t_in[2] = {-INFINITY, -INFINITY}, x_in[2], x_ref = 0.0f;
-    int64_t id_in[2] = {-1, -1};
-    int taught = 0;   // parts done
-    auto teach = [&]() {
-      if constexpr (OP == kDistill) {
-        const int64_t t0 = static_cast<int64_t>(info.row) * a.K;
-        const T* x_row = static_cast<const T*>(a.logits) + row_offset(a, info.row);
-        if (taught == 0) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (lane + 32 * h < a.K) { t_in[h] = read_teacher(a, t0 + lane + 32 * h); id_in[h] = read_teacher_id(a, t0 + lane + 32 * h); }
-        } else if (taught == 1) {
-          float tm = fmaxf(t_in[0], t_in[1]), ts, loss = 0.0f;
-          for (int q = lane + 64; q < a.K; q += 32) tm = fmaxf(tm, read_teacher(a, t0 + q));
-          tm = warp_max(tm);
-          const float tref = tm == -INFINITY ? 0.0f : tm;
-          ts = exp2f((t_in[0] - tref) * a.k) + exp2f((t_in[1] - tref) * a.k);
-          int64_t best = t_in[0] == tm && lane < a.K ? id_in[0] : t_in[1] == tm && lane + 32 < a.K ? id_in[1] : -1;
-          for (int q = lane + 64; q < a.K; q += 32) {
-            const float t = read_teacher(a, t0 + q);
-            ts += exp2f((t - tref) * a.k);
-            if (t == tm && best < 0) best = read_teacher_id(a, t0 + q);
-          }
-          ts = warp_sum(ts);
-          const uint32_t who = __ballot_sync(0xffffffffu, best >= 0);
-          best = __shfl_sync(0xffffffffu, best, who == 0 ? 0 : __ffs(who) - 1);
-          if (best >= 0 && best < a.V) x_ref = to_f32(x_row[best]);
-          const float inv_ts = 1.0f / ts, log_ts = logf(ts);
-          bool twice = false;
-          auto entry = [&](int q, float t, int64_t id) {
-            const float d = t - tref;   // log q = d / T - log_ts
-            const float prob = ts == 0.0f ? 0.0f : exp2f(d * a.k) * inv_ts;
-            int el = -1;
-            if (prob != 0.0f) {   // (NaN counts)
-              if (id < 0 || id >= a.V) {
-                loss = NAN;
-              } else if (id - info.share.column >= info.share.lo && id - info.share.column < info.share.hi) {
-                el = static_cast<int>(id - info.share.column);
-                loss += prob * (d * a.inv_t - log_ts);
-                twice |= atomicOr(t_bits + par * bit_words + (el >> 5), 1u << (el & 31)) >> (el & 31) & 1u;
-              }
-            }
-            t_id[par * a.K + q] = el;
-            t_q[par * a.K + q] = prob;
-            return el;
-          };
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            x_in[h] = 0.0f;
-            if (lane + 32 * h < a.K && entry(lane + 32 * h, t_in[h], id_in[h]) >= 0) x_in[h] = to_f32(x_row[id_in[h]]);
-          }
-          for (int q = lane + 64; q < a.K; q += 32) {
-            const int64_t id = read_teacher_id(a, t0 + q);
-            if (entry(q, read_teacher(a, t0 + q), id) >= 0) t_x[par * a.K + q] = to_f32(x_row[id]);
-          }
-          loss = warp_sum(loss);
-          twice = __any_sync(0xffffffffu, twice);
-          if (lane == 0) { teachers[group][par] = make_float4(loss, 0.0f, ts == 0.0f ? 1.0f : 0.0f, 0.0f); repeats[group][par] = twice; }
-        } else {
-          if (!(fabsf(x_ref) < INFINITY)) x_ref = 0.0f;
-          float loss = 0.0f;
-          for (int q = lane; q < a.K; q += 32) {
-            if (t_id[par * a.K + q] < 0) continue;
-            const float x = q < 32 ? x_in[0] : q < 64 ? x_in[1] : t_x[par * a.K + q];
-            t_x[par * a.K + q] = x;
-            loss -= t_q[par * a.K + q] * ((x - x_ref) * a.inv_t);
-          }
-          loss = warp_sum(loss);
-          if (lane == 0) { teachers[group][par].x += loss; teachers[group][par].y = x_ref; }
-        }
-        ++taught;
-        __syncwarp();
+    if constexpr (OP == kDistill) {
+      if (teaches) {
+        if (prepared != i) { teach_load(info); teach_weigh(info, par); }   // the first row of a batch
+        teach_sum(par);
+        if (at + 1 < info_rows && i + step < kept && infos[at + 1].state == 0) { prepared = i + step; teach_load(infos[at + 1]); }
       }
-    };
-    if (teaches) teach();
+    }
     // first sweep
     const bool own = info.target >= 0;
     float m = -INFINITY, sw = 0.0f, e[kChunk];
@@ -487,9 +518,9 @@ token_resident_kernel(const RowArgs a, const Resident p) {
     // Its exponentials, relative to the thread's largest logit so far, m.
     auto exponentials = [&](const VT (&raw)[CV], float cm, float (&x)[kChunk], int n = 1 << 20) {   // n: the chunk's vectors, if it may not be full
       const float mm = fmaxf(m, cm);
-      if (mm > m && m != -INFINITY) sw *= ex2((m - mm) * a.k);
+      const float r = mm == -INFINITY ? 0.0f : mm;
+      sw *= ex2((fmaxf(m, -FLT_MAX) - r) * a.k);   // (nothing summed yet: 0, or NaN, times at most 1)
       m = mm;
-      const float r = m == -INFINITY ? 0.0f : m;
       const float2 neg_m = make_float2(-r, -r);
       float2 s2 = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -533,7 +564,6 @@ token_resident_kernel(const RowArgs a, const Resident p) {
         next_cm = fetch(c + 1, next);
         exponentials(raw, cm, x);
         keep(c, x);
-        if (teaches && taught == 1) teach();
         cm = fetch(c + 2, raw);
         exponentials(next, next_cm, x);
         keep(c + 1, x);
@@ -554,14 +584,11 @@ token_resident_kernel(const RowArgs a, const Resident p) {
         cm = fetch(c, raw);
         exponentials(raw, cm, x);
         keep(c, x);
-        if (teaches && taught == 1) teach();
       }
       cm = fetch(chunks - 1, raw);
     }
-    if (teaches && taught == 1) teach();
     exponentials(raw, cm, e, info.share.n - ((chunks - 1) << (kLogCv + log_gd)));
     const float ref_e = m;
-    if (teaches) teach();
     float mw = m;
     warp_combine(mw, sw, a.k);
     if (chunks > 1) tmem_st_wait();
@@ -621,6 +648,9 @@ token_resident_kernel(const RowArgs a, const Resident p) {
         top = r.top == -INFINITY ? 0.0f : r.top;
       }
     }
+    if constexpr (OP == kDistill) {
+      if (teaches && prepared == i + step) teach_weigh(infos[at + 1], par ^ 1);
+    }
     if (p.group_warps > 1) {
       if (tid == 0) row_end[group][par] = make_float4(f_top, top, OP == kDistill ? c0 : at_target, sw);
       group_sync();
@@ -636,25 +666,36 @@ token_resident_kernel(const RowArgs a, const Resident p) {
       auto put = [&](int c, int j0, const float* x, int count, float f) {
         const float2 ff = make_float2(f, f);
         const int v0 = c << (kLogCv + log_gd);
-        const bool whole = SAME && v0 >= s.fa && v0 + CV * gd <= s.fb;   // all of the chunk's vectors are the row's alone
         Raw* to = reinterpret_cast<Raw*>(g) + v0 + tid;
-#pragma unroll
-        for (int j = 0; j < count; ++j) {
-          if (j > 0 && v0 + ((j0 + j) << log_gd) >= s.fb) break;
+        auto scaled = [&](int j) {
+          VT t;
           float y[N];
 #pragma unroll
           for (int q = 0; q < N; q += 2) {
             const float2 z = __fmul2_rn(make_float2(x[j * N + q], x[j * N + q + 1]), ff);
             y[q] = z.x; y[q + 1] = z.y;
           }
-          const int vi = v0 + ((j0 + j) << log_gd) + tid;
-          if (SAME) {
-            VT t;
-            t.from_float(y);
-            if (whole || (vi >= s.fa && vi < s.fb)) __stcs(to + ((j0 + j) << log_gd), t.raw);
-          } else if (vi >= s.fa && vi < s.fb) {
+          t.from_float(y);
+          return t;
+        };
+        if (SAME && v0 >= s.fa && v0 + CV * gd <= s.fb) {   // all of the chunk's vectors are the row's alone
 #pragma unroll
-            for (int q = 0; q < N; ++q) g[vi * N + q] = from_f32<T>(y[q]);
+          for (int j = 0; j < count; ++j) __stcs(to + ((j0 + j) << log_gd), scaled(j).raw);
+          return;
+        }
+#pragma unroll
+        for (int j = 0; j < count; ++j) {
+          if (j > 0 && v0 + ((j0 + j) << log_gd) >= s.fb) break;
+          const VT t = scaled(j);
+          const int vi = v0 + ((j0 + j) << log_gd) + tid;
+          if (vi >= s.fa && vi < s.fb) {
+            if (SAME) {
+              __stcs(to + ((j0 + j) << log_gd), t.raw);
+            } else {
+              const T* y = reinterpret_cast<const T*>(&t.raw);
+#pragma unroll
+              for (int q = 0; q < N; ++q) g[vi * N + q] = y[q];
+            }
           }
         }
       };
