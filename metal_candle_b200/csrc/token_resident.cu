@@ -34,7 +34,12 @@ namespace {
 using namespace tokenloss;
 using namespace umma;
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kThreads = 512, kWarps = kThreads / 32;   // that take rows
+constexpr int kAllThreads = kThreads + 128;              // and four warps that serve them
+// Registers: 640 threads are launched with 96 each, 61440; the row warps take 112, the serving ones keep 32 (512 x 112 + 128 x 32 = 61440),
+// or 104 and 64 where these work out the teacher's part.
+template <int OP> constexpr int kRowRegs = OP == kDistill ? 104 : 112;
+template <int OP> constexpr int kServeRegs = OP == kDistill ? 64 : 32;
 constexpr int kChunk = 32;             // elements a thread takes at a time
 constexpr int kTmemChunks = 4;         // chunks it keeps in tensor memory, beside one in registers
 constexpr int kMaxChunks = kTmemChunks + 1;
@@ -60,6 +65,14 @@ struct Resident {
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// Whether the phase is over, without waiting (the lanes of a warp look at barriers of their own).
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+               "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
 }
 
 // Hands 16 bytes to CTA `to` of the cluster, at the place of `slot` here, and tells the barrier there.  (A plain store with a releasing
@@ -169,28 +182,18 @@ struct RowInfo {
   int state;         // 0: to be computed, 1: left out, 2: out of range
   RowInputs in;
 };
-// The group's feeder's notes (see below), in shared memory: they would cost every thread a dozen registers.
-struct Feed {
-  const void* from;      // where the rest of the row's share lies
-  uint32_t fed;          // the place of the row that is being fed, infos[at] if it is among them
-  int at, left;          // left: vectors of the row's share that have not been fed
-  int slot;
-  uint32_t phase;
-};
-
 // SAME: every row of the gradient lies as its logits do relative to 16 bytes, so that whole vectors can be written.
 template <typename T, int OP, bool SAME>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kAllThreads, 1)
 token_resident_kernel(const RowArgs a, const Resident p) {
   using VT = Vec16<T>;
   using Raw = decltype(VT::raw);
   constexpr int N = VT::N, CV = kChunk / N, kLogCv = CV == 4 ? 2 : 3;   // vectors of a chunk
   static_assert(CV == 1 << kLogCv, "chunks of a power of two");
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(8) uint64_t full[kWarps][kMaxPieces], empty[kWarps][kMaxPieces], slot_bars[kWarps][2];
+  __shared__ __align__(8) uint64_t full[kWarps][kMaxPieces], empty[kWarps][kMaxPieces], slot_bars[kWarps][2], t_full[2][2], t_empty[2][2];
   __shared__ __align__(16) float4 slots[kWarps / 2][2][8];   // by group, parity and CTA: (maximum, sum, target's logit or loss, whose target it is)
   __shared__ __align__(16) float4 row_end[kWarps / 2][2];    // what the second sweep needs: by group and parity
-  __shared__ Feed feeds[kWarps];
   __shared__ float2 red[2][kWarps];
   __shared__ float edge[kWarps][2][2 * N];                   // the share's elements in vectors that are not the row's alone
   __shared__ float target_logit[kWarps][2];
@@ -204,7 +207,9 @@ token_resident_kernel(const RowArgs a, const Resident p) {
   const int ctas = p.ctas, rank = static_cast<int>(cl.block_rank());
   const int groups = 1 << p.log_groups, log_gd = 9 - p.log_groups, gd = 1 << log_gd;   // threads a group
   const int lane = threadIdx.x & 31, warp = static_cast<int>(threadIdx.x) >> 5;
-  const int group = static_cast<int>(threadIdx.x) >> log_gd, tid = threadIdx.x & (gd - 1);   // the thread within its group
+  const bool serves = warp >= kWarps;
+  const int group = serves ? 0 : static_cast<int>(threadIdx.x) >> log_gd;
+  const int tid = serves ? threadIdx.x : threadIdx.x & (gd - 1);   // the thread within its group (those that serve are in none)
   const int first = ((static_cast<int>(blockIdx.x) >> p.log_ctas) << p.log_groups) + group;
   const int step = (static_cast<int>(gridDim.x) >> p.log_ctas) << p.log_groups;
   const int piece_bytes = CV * 16 * gd;
@@ -213,7 +218,8 @@ token_resident_kernel(const RowArgs a, const Resident p) {
   const int info_rows = kInfoRows >> p.log_groups;
   uint8_t* ring = smem + kInfoRows * sizeof(RowInfo) + group * p.pieces * piece_bytes;
   const int bit_words = kMaxChunks * kChunk * gd / 32;
-  int* t_id = reinterpret_cast<int*>(smem + kInfoRows * sizeof(RowInfo) + groups * p.pieces * piece_bytes + group * (24 * a.K + 8 * bit_words));
+  uint8_t* teacher_smem = smem + kInfoRows * sizeof(RowInfo) + groups * p.pieces * piece_bytes;
+  int* t_id = reinterpret_cast<int*>(teacher_smem + group * (24 * a.K + 8 * bit_words));
   float* t_q = reinterpret_cast<float*>(t_id + 2 * a.K);
   float* t_x = t_q + 2 * a.K;
   uint32_t* t_bits = reinterpret_cast<uint32_t*>(t_x + 2 * a.K);
@@ -225,12 +231,14 @@ token_resident_kernel(const RowArgs a, const Resident p) {
   if (threadIdx.x == 0) *abort_flag = 0;
   if (tid == 0) {
     for (int i = 0; i < p.pieces; ++i) { mbar_init(full0 + 8 * i, 1); mbar_init(empty0 + 8 * i, p.group_warps); }
-    for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&slot_bars[group][i]), 1); }
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&slot_bars[group][i]), 1);
+    if (group < 2)
+      for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&t_full[group][i]), 1); mbar_init(smem_u32(&t_empty[group][i]), p.group_warps); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async_smem();
   }
   if constexpr (OP == kDistill)
-    for (int i = tid; i < 2 * bit_words; i += gd) t_bits[i] = 0;
+    for (int i = tid; i < 2 * bit_words && !serves; i += gd) t_bits[i] = 0;
   if (ctas > 1) cl.sync(); else __syncthreads();   // every CTA's barriers exist before a peer arrives on them
   grid_dependency_wait();
   if (p.tmem) {
@@ -257,145 +265,128 @@ token_resident_kernel(const RowArgs a, const Resident p) {
   };
   auto chunks_of = [&](int n) { return max(1, (n + CV * gd - 1) >> (kLogCv + log_gd)); };
 
-  // One thread of the group's last warp (the first has the row's scalar work) also feeds the ring: pieces in the order they are taken,
-  // each when every warp has left the slot it goes to.
-  const int feeder = gd - 32;
-  if (tid == feeder) feeds[group] = {nullptr, static_cast<uint32_t>(first) - static_cast<uint32_t>(step), -1, 0, 0, 1};
-  auto feed = [&]() {
-    Feed f = feeds[group];
-    if (f.left <= 0) {
-      while (true) {
-        f.fed += step; ++f.at;   // (the first time round from 2^32 - something)
-        if (f.fed >= kept) { f.fed -= step; --f.at; feeds[group] = f; return; }
-        if (f.at < info_rows) {
-          const RowInfo& r = infos[f.at];
-          if (r.state != 0) continue;
-          f.from = static_cast<const T*>(a.logits) - p.mis + r.share.from;
-          f.left = r.share.n;
-        } else {
-          const int row = row_of(f.fed);
-          if (state_of(f.fed, row) != 0) continue;
-          const Share s = share_of<N>(a, p, rank, row);
-          f.from = static_cast<const T*>(a.logits) - p.mis + s.from;
-          f.left = s.n;
-        }
-        break;
-      }
+  // Distillation: a row's teacher, by one warp: q = softmax(t / T) over its entries, those with -inf counting for nothing; of the entries
+  // whose column is in this share where it is (or -1), q and the student's logit; and the sum of q (log q - (x - x_ref) / T) over
+  // them, with x_ref the student's logit where the teacher's is largest.
+  auto teach = [&](int g, int row, const Share& s, int into) {
+    const int64_t t0 = static_cast<int64_t>(row) * a.K;
+    const T* x_row = static_cast<const T*>(a.logits) + row_offset(a, row);
+    int* ids = reinterpret_cast<int*>(teacher_smem + g * (24 * a.K + 8 * bit_words)) + into * a.K;
+    float* probs = reinterpret_cast<float*>(ids + 2 * a.K);
+    float* logits = probs + 2 * a.K;
+    uint32_t* bits = reinterpret_cast<uint32_t*>(logits + (2 - into) * a.K) + into * bit_words;
+    auto id_of = [&](int64_t id) { return id >= 0 && id < a.V ? static_cast<int>(id) : -1; };
+    float tm = -INFINITY, ts = 0.0f;
+    for (int q = lane; q < a.K; q += 32) {
+      const float t = read_teacher(a, t0 + q);
+      ids[q] = id_of(read_teacher_id(a, t0 + q));
+      probs[q] = t;
+      tm = fmaxf(tm, t);
     }
-    const int n = max(0, min(f.left, CV * gd));
-    if (mbar_wait(empty0 + 8 * f.slot, f.phase, abort_flag, 55, p.status)) {
-      mbar_expect_tx(full0 + 8 * f.slot, n * 16);   // a piece with nothing in it completes at once
-      if (n > 0) bulk_load(smem_u32(ring) + f.slot * piece_bytes, f.from, n * 16, full0 + 8 * f.slot);
-    }
-    f.from = static_cast<const T*>(f.from) + n * N;
-    f.left -= n;
-    if (++f.slot == p.pieces) { f.slot = 0; f.phase ^= 1; }
-    feeds[group] = f;
-  };
-
-  // Distillation: a row's teacher, by one warp, in three parts under the row before, so that nothing waits for the global loads of each:
-  // its entries (two a lane; more than 64 are read where they are needed); q = softmax(t / T), those with -inf counting for nothing, and
-  // of the entries whose column is in this share where it is (or -1), q, and a request for the student's logit; then the sum of
-  // q (log q - (x - x_ref) / T), with x_ref the student's logit where the teacher's is largest.
-  const bool teaches = OP == kDistill && (tid >> 5) == (p.group_warps > 1 ? 1 : 0);
-  uint32_t prepared = 0xffffffffu;   // the place of the row that the first part, or the first two, were done for
-  uint32_t t_in[2], x_in[2], x_ref = 0;   // as loaded: a conversion would wait for the load
-  int64_t id_in[2];
-  auto load_bits = [](const T* x) -> uint32_t {
-    if constexpr (sizeof(T) == 2) return *reinterpret_cast<const uint16_t*>(x); else return *reinterpret_cast<const uint32_t*>(x);
-  };
-  auto logit_of = [](uint32_t bits) { return __uint_as_float(sizeof(T) == 2 ? bits << 16 : bits); };
-  auto id_of = [&](int64_t id) { return id >= 0 && id < a.V ? static_cast<int>(id) : -1; };
-  auto teach_load = [&](const RowInfo& info) {
-    const int64_t t0 = static_cast<int64_t>(info.row) * a.K;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int q = lane + 32 * h;
-      t_in[h] = 0;
-      id_in[h] = 0;
-      if (q < a.K) {
-        t_in[h] = a.teacher_f32 ? static_cast<const uint32_t*>(a.teacher)[t0 + q] : static_cast<const uint16_t*>(a.teacher)[t0 + q];
-        id_in[h] = a.id_bytes == 8 ? static_cast<const int64_t*>(a.teacher_ids)[t0 + q] : static_cast<const uint32_t*>(a.teacher_ids)[t0 + q];
-      }
-    }
-  };
-  auto teach_weigh = [&](const RowInfo& info, int into) {
-    const int64_t t0 = static_cast<int64_t>(info.row) * a.K;
-    const T* x_row = static_cast<const T*>(a.logits) + row_offset(a, info.row);
-    float t[2];
-    int id[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      t[h] = lane + 32 * h < a.K ? __uint_as_float(a.teacher_f32 ? t_in[h] : t_in[h] << 16) : -INFINITY;
-      id[h] = id_of(a.id_bytes == 8 ? id_in[h] : static_cast<int32_t>(id_in[h]));
-    }
-    float tm = fmaxf(t[0], t[1]);
-    for (int q = lane + 64; q < a.K; q += 32) tm = fmaxf(tm, read_teacher(a, t0 + q));
     tm = warp_max(tm);
     const float tref = tm == -INFINITY ? 0.0f : tm;
-    float e[2] = {ex2((t[0] - tref) * a.k), ex2((t[1] - tref) * a.k)};
-    float ts = e[0] + e[1];
-    int best = t[0] == tm && lane < a.K ? id[0] : t[1] == tm && lane + 32 < a.K ? id[1] : -1;
-    for (int q = lane + 64; q < a.K; q += 32) {
-      const float v = read_teacher(a, t0 + q);
-      ts += ex2((v - tref) * a.k);
-      if (v == tm && best < 0) best = id_of(read_teacher_id(a, t0 + q));
+    int best = -1;
+    for (int q = lane; q < a.K; q += 32) {
+      const float t = probs[q];
+      ts += ex2((t - tref) * a.k);
+      if (t == tm && best < 0) best = ids[q];
     }
     ts = warp_sum(ts);
     const uint32_t who = __ballot_sync(0xffffffffu, best >= 0);
     best = __shfl_sync(0xffffffffu, best, who == 0 ? 0 : __ffs(who) - 1);
-    x_ref = best >= 0 ? load_bits(x_row + best) : 0;
+    float x_ref = best >= 0 ? to_f32(x_row[best]) : 0.0f;
+    if (!(fabsf(x_ref) < INFINITY)) x_ref = 0.0f;
     const float inv_ts = ts == 0.0f ? 0.0f : 1.0f / ts, log_ts = logf(ts);
-    const int column = info.share.column, lo = info.share.lo, hi = info.share.hi;
     float loss = 0.0f;
     bool twice = false;
-    auto entry = [&](int q, float v, float exponential, int id) {
-      const float prob = exponential * inv_ts;
+    for (int q = lane; q < a.K; q += 32) {
+      const float d = probs[q] - tref, prob = ex2(d * a.k) * inv_ts;   // log q = d / T - log_ts
+      const int id = ids[q];
       int el = -1;
       if (prob != 0.0f) {   // (NaN counts)
         if (id < 0) {
           loss = NAN;
-        } else if (id - column >= lo && id - column < hi) {
-          el = id - column;
-          loss += prob * ((v - tref) * a.inv_t - log_ts);   // log q
-          twice |= atomicOr(t_bits + into * bit_words + (el >> 5), 1u << (el & 31)) >> (el & 31) & 1u;
+        } else if (id - s.column >= s.lo && id - s.column < s.hi) {
+          el = id - s.column;
+          const float x = to_f32(x_row[id]);
+          logits[q] = x;
+          loss += prob * ((d * a.inv_t - log_ts) - (x - x_ref) * a.inv_t);
+          twice |= atomicOr(bits + (el >> 5), 1u << (el & 31)) >> (el & 31) & 1u;
         }
       }
-      t_id[into * a.K + q] = el;
-      t_q[into * a.K + q] = prob;
-      return el;
-    };
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      x_in[h] = 0;
-      if (lane + 32 * h < a.K && entry(lane + 32 * h, t[h], e[h], id[h]) >= 0) x_in[h] = load_bits(x_row + id[h]);
-    }
-    for (int q = lane + 64; q < a.K; q += 32) {
-      const int named = id_of(read_teacher_id(a, t0 + q));
-      const float v = read_teacher(a, t0 + q);
-      if (entry(q, v, ex2((v - tref) * a.k), named) >= 0) t_x[into * a.K + q] = to_f32(x_row[named]);
+      ids[q] = el;
+      probs[q] = prob;
     }
     loss = warp_sum(loss);
     twice = __any_sync(0xffffffffu, twice);
-    if (lane == 0) { teachers[group][into] = make_float4(loss, 0.0f, ts == 0.0f ? 1.0f : 0.0f, 0.0f); repeats[group][into] = twice; }
+    if (lane == 0) { teachers[g][into] = make_float4(loss, x_ref, ts == 0.0f ? 1.0f : 0.0f, 0.0f); repeats[g][into] = twice; }
     __syncwarp();
   };
-  auto teach_sum = [&](int into) {
-    float x0 = logit_of(x_ref);
-    if (!(fabsf(x0) < INFINITY)) x0 = 0.0f;
-    float loss = 0.0f;
-    for (int q = lane; q < a.K; q += 32) {
-      if (t_id[into * a.K + q] < 0) continue;
-      const float x = q < 32 ? logit_of(x_in[0]) : q < 64 ? logit_of(x_in[1]) : t_x[into * a.K + q];
-      t_x[into * a.K + q] = x;
-      loss -= t_q[into * a.K + q] * ((x - x0) * a.inv_t);
-    }
-    loss = warp_sum(loss);
-    if (lane == 0) { teachers[group][into].x += loss; teachers[group][into].y = x0; }
-    __syncwarp();
-  };
+  // Serving warps do it up to two rows ahead where an SM has few rows in flight, one for each group; more groups hide their own.
+  const bool taught_ahead = OP == kDistill && groups <= 2;
 
-  uint32_t phase = 0, slot_phase = 0;   // parities of the ring's current round, and (bit i) of slot barrier i
+  if (serves) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kServeRegs<OP>));
+    if (warp == kWarps) {
+      // Lane g feeds group g's ring: pieces in the order they are taken, each when every warp has left the slot it goes to.
+      uint32_t fed = ((blockIdx.x >> p.log_ctas) << p.log_groups) + lane;   // the place of the row
+      bool active = lane < groups && fed < kept;
+      const int g = lane & (kWarps - 1);
+      const T* from = nullptr;
+      int left = -1, slot = 0;   // vectors of the row's share that have not been fed; -1: the row has not been begun
+      uint32_t phase = 1;
+      long long idle = 0;
+      while (__any_sync(0xffffffffu, active)) {
+        bool moved = false;
+        if (active && left < 0) {
+          const int row = row_of(fed);
+          if (state_of(fed, row) == 0) {
+            const Share s = share_of<N>(a, p, rank, row);
+            from = static_cast<const T*>(a.logits) - p.mis + s.from;
+            left = s.n;
+          } else {
+            fed += step;
+            active = fed < kept;
+          }
+          moved = true;
+        }
+        if (active && left >= 0 && mbar_test(smem_u32(&empty[g][slot]), phase)) {
+          const uint32_t bar = smem_u32(&full[g][slot]);
+          const int n = min(left, CV * gd);
+          mbar_expect_tx(bar, n * 16);   // a piece with nothing in it completes at once
+          if (n > 0)
+            bulk_load(smem_u32(smem) + kInfoRows * static_cast<uint32_t>(sizeof(RowInfo)) + (g * p.pieces + slot) * piece_bytes, from, n * 16, bar);
+          from += n * N;
+          left -= n;
+          if (++slot == p.pieces) { slot = 0; phase ^= 1; }
+          if (left == 0) { left = -1; fed += step; active = fed < kept; }
+          moved = true;
+        }
+        if (__any_sync(0xffffffffu, moved)) { idle = 0; continue; }
+        if (*abort_flag != 0) break;
+        const long long now = clock64();
+        if (idle == 0) idle = now;
+        else if (now - idle > kWaitLimitCycles) { *abort_flag = 55; atomicCAS(p.status, 0, 55); break; }
+      }
+      __syncwarp();
+    } else if (taught_ahead && warp - kWarps - 1 < groups) {
+      const int g = warp - kWarps - 1;
+      uint32_t parity = 1;
+      int into = 0;
+      for (uint32_t i = ((blockIdx.x >> p.log_ctas) << p.log_groups) + g; i < kept; i += step) {
+        const int row = row_of(i);
+        if (state_of(i, row) != 0) continue;
+        if (!mbar_wait(smem_u32(&t_empty[g][into]), parity, abort_flag, 57, p.status)) break;
+        teach(g, row, share_of<N>(a, p, rank, row), into);
+        if (lane == 0) mbar_arrive(smem_u32(&t_full[g][into]));
+        if (++into == 2) { into = 0; parity ^= 1; }
+      }
+      __syncwarp();
+    }
+  } else {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegs<OP>));
+
+  uint32_t phase = 0, slot_phase = 0, t_phase = 0;   // parities of the ring's current round, (bit i) of slot barrier i, of the teacher's
   int slot = 0, par = 0, at = info_rows;
   for (uint32_t i = first; i < M; i += step, ++at) {   // (M and the step are below 2^31)
     if (at == info_rows) {
@@ -425,11 +416,6 @@ token_resident_kernel(const RowArgs a, const Resident p) {
       }
       group_sync();
       at = 0;
-      if (tid == feeder) {
-        if (i != static_cast<uint32_t>(first)) feeds[group].at -= info_rows;
-        else
-          for (int q = 0; q < p.pieces; ++q) feed();
-      }
     }
     const RowInfo& info = infos[at];
     if (info.state != 0) {   // the same in every CTA of the cluster
@@ -455,10 +441,9 @@ token_resident_kernel(const RowArgs a, const Resident p) {
     }
     float third = 0.0f;
     if constexpr (OP == kDistill) {
-      if (teaches) {
-        if (prepared != i) { teach_load(info); teach_weigh(info, par); }   // the first row of a batch
-        teach_sum(par);
-        if (at + 1 < info_rows && i + step < kept && infos[at + 1].state == 0) { prepared = i + step; teach_load(infos[at + 1]); }
+      if (!taught_ahead) {
+        if (tid < 32) teach(group, info.row, info.share, par);
+        group_sync();
       }
     }
     // first sweep
@@ -511,8 +496,6 @@ token_resident_kernel(const RowArgs a, const Resident p) {
       __syncwarp();
       if (lane == 0) mbar_arrive(empty0 + 8 * slot);   // the warp has taken what it needs of the slot
       if (++slot == p.pieces) { slot = 0; phase ^= 1; }
-      if (c > 0 && tid == feeder) feed();              // the slot of the piece before this one
-      __syncwarp();
       return Lane<T>::max_of(raw);
     };
     // Its exponentials, relative to the thread's largest logit so far, m.
@@ -599,13 +582,15 @@ token_resident_kernel(const RowArgs a, const Resident p) {
         const float2 r = lane < p.group_warps ? red[par][group * p.group_warps + lane] : make_float2(-INFINITY, 0.0f);
         mw = r.x; sw = r.y;
         warp_combine(mw, sw, a.k, p.group_warps);
-      } else if (tid == feeder) {
-        feed();   // the slot of the row's last piece
       }
     } else {
       __syncwarp();
-      if (tid == feeder) feed();
-      __syncwarp();
+    }
+    if constexpr (OP == kDistill) {
+      if (taught_ahead) {
+        mbar_wait(smem_u32(&t_full[group][par]), t_phase, abort_flag, 57, p.status);
+        t_phase ^= par;   // (both have been waited for)
+      }
     }
     if constexpr (OP == kDistill) third = teachers[group][par].x;
     else if (own) third = target_logit[group][par];
@@ -647,9 +632,6 @@ token_resident_kernel(const RowArgs a, const Resident p) {
         f_top = -c0 / r.sum;
         top = r.top == -INFINITY ? 0.0f : r.top;
       }
-    }
-    if constexpr (OP == kDistill) {
-      if (teaches && prepared == i + step) teach_weigh(infos[at + 1], par ^ 1);
     }
     if (p.group_warps > 1) {
       if (tid == 0) row_end[group][par] = make_float4(f_top, top, OP == kDistill ? c0 : at_target, sw);
@@ -757,10 +739,12 @@ token_resident_kernel(const RowArgs a, const Resident p) {
       if (p.group_warps == 1) __syncwarp();
       for (int q = tid; q < a.K; q += gd)
         if (t_id[par * a.K + q] >= 0) t_bits[par * bit_words + (t_id[par * a.K + q] >> 5)] = 0;
-      if (p.group_warps == 1) __syncwarp();
+      __syncwarp();
+      if (taught_ahead && lane == 0) mbar_arrive(smem_u32(&t_empty[group][par]));
     }
     par ^= 1;
   }
+  }   // (not the serving warps)
   tcgen05_fence_before();
   __syncthreads();
   if (*abort_flag != 0) {
@@ -783,13 +767,13 @@ token_resident_kernel(const RowArgs a, const Resident p) {
       double* sums = reinterpret_cast<double*>(smem);
       for (int t = 0; t < p.n_out; ++t) {
         double acc = 0.0;
-        for (uint32_t q = threadIdx.x; q < M; q += kThreads) acc += static_cast<double>(__ldcg(a.terms + static_cast<int64_t>(t) * M + q));
+        for (uint32_t q = threadIdx.x; q < M; q += kAllThreads) acc += static_cast<double>(__ldcg(a.terms + static_cast<int64_t>(t) * M + q));
         for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
         if (lane == 0) sums[warp] = acc;
         __syncthreads();
         if (threadIdx.x == 0) {
           double total = 0.0;
-          for (int w = 0; w < kWarps; ++w) total += sums[w];
+          for (int w = 0; w < kAllThreads / 32; ++w) total += sums[w];
           p.out[t] = static_cast<float>(total);
         }
         __syncthreads();
@@ -846,7 +830,7 @@ int launch_resident(const RowArgs& a, const RowPlan& plan, DeviceState* ds, cuda
   const bool same = a.grad == nullptr || (((ai ^ ag) & 15u) == 0 && (a.token_stride - a.V) % N == 0 && (a.batch_stride - a.S * a.V) % N == 0);
   const auto kernel = same ? token_resident_kernel<T, OP, true> : token_resident_kernel<T, OP, false>;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.ctas)); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = static_cast<size_t>(smem); cfg.stream = st;
+  cfg.gridDim = dim3(static_cast<unsigned>(p.ctas)); cfg.blockDim = dim3(kAllThreads); cfg.dynamicSmemBytes = static_cast<size_t>(smem); cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = static_cast<unsigned>(p.ctas); attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
