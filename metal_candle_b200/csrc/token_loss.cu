@@ -186,39 +186,49 @@ row_weights_kernel(const void* targets, int target_bytes, int has_ignore, int64_
     const int t = read_target(targets, target_bytes, has_ignore, ignore, row, V);
     return t >= 0 ? 1 : t + 1;
   };
-  // each warp takes 256 rows in a row, eight a lane; how many of those in front of it are kept is counted over the block
+  // eight rows a thread at a time; each warp counts its kept rows and the others, the block those of the warps before it
   int keep[kRows];
   int total = 0;
   for (int64_t base = 0; base < M; base += kRound) {
-    const int64_t mine = base + warp * 32 * kRows + lane;
+    const int64_t mine = base + threadIdx.x;
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) keep[r] = mine + r * 32 < M ? kept(static_cast<int>(mine) + r * 32) : 0;
-    uint32_t votes[kRows];
-    int c = 0;
+    for (int r = 0; r < kRows; ++r) keep[r] = mine + r * 1024 < M ? kept(static_cast<int>(mine) + r * 1024) : 0;
+    uint32_t votes[kRows], others[kRows];
+    int c = 0;   // kept, and 65536 times those that are not (a round has 8192)
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       votes[r] = __ballot_sync(0xffffffffu, keep[r] != 0);
-      c += __popc(votes[r]);
+      others[r] = __ballot_sync(0xffffffffu, mine + r * 1024 < M && keep[r] == 0);
+      c += __popc(votes[r]) + (__popc(others[r]) << 16);
     }
     __syncthreads();   // red is free, counts are cleared
     if (lane == 0) red[warp] = c;
     if (counted) {
 #pragma unroll
-      for (int r = 0; r < kRows; ++r)
-        if (keep[r] != 0) atomicAdd(counts + static_cast<int>(mine + r * 32) / S, 1);
+      for (int r = 0; r < kRows; ++r) {
+        if (votes[r] == 0) continue;
+        const int64_t row0 = mine - lane + r * 1024;
+        const int b0 = static_cast<int>(row0) / S;
+        if (row0 + 31 < static_cast<int64_t>(b0 + 1) * S) {   // all 32 rows of one sequence
+          if (lane == 0) atomicAdd(counts + b0, __popc(votes[r]));
+        } else if (keep[r] != 0) {
+          atomicAdd(counts + static_cast<int>(row0 + lane) / S, 1);
+        }
+      }
     }
     __syncthreads();
     c = red[lane];
-    int at = total + __reduce_add_sync(0xffffffffu, lane < warp ? c : 0);   // kept rows before the warp's r-th 32
-    total += __reduce_add_sync(0xffffffffu, c);
+    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? c : 0);
+    int at = total + (before & 0xffff), out = static_cast<int>(base) - total + (before >> 16);   // places from the order's ends
+    total += __reduce_add_sync(0xffffffffu, c) & 0xffff;
     if (order == nullptr) continue;
     const uint32_t below = (1u << lane) - 1u;
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const int row = static_cast<int>(mine) + r * 32, k = at + __popc(votes[r] & below);
-      // k: kept rows before this one; the others fill the order from its end
-      if (mine + r * 32 < M) order[keep[r] != 0 ? k : M - 1 - (row - k)] = row;
+      const int row = static_cast<int>(mine) + r * 1024;
+      if (mine + r * 1024 < M) order[keep[r] != 0 ? at + __popc(votes[r] & below) : M - 1 - (out + __popc(others[r] & below))] = row;
       at += __popc(votes[r]);
+      out += __popc(others[r]);
     }
   }
   if (threadIdx.x == 0 && info != nullptr) { info[0] = total; info[1] = 0; }
@@ -261,7 +271,7 @@ row_weights_kernel(const void* targets, int target_bytes, int has_ignore, int64_
   if (M <= kRound) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const int row = warp * 32 * kRows + lane + r * 32;
+      const int row = static_cast<int>(threadIdx.x) + r * 1024;
       if (row < M) put(row, keep[r]);
     }
   } else {

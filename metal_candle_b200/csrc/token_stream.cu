@@ -61,8 +61,9 @@ __device__ __forceinline__ void warp_combine(float& m, float& s, float k) {
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // Statistics.  Bound: HBM, one read; per thread eight 16-byte loads are in flight, whose maximum is taken first, so that the running
-// sum is rescaled once in eight vectors.  A row is one block's, or with few rows a cluster's.
-template <typename T, int OP>
+// sum is rescaled once in eight vectors.  A row is one block's, or with few rows a cluster's; SHORT: one warp's (20000 x 1000 bf16 as
+// blocks of a warp each 41 us: as many launches of blocks as rows).
+template <typename T, int OP, bool SHORT>
 __global__ void __launch_bounds__(kThreads)
 token_stats_kernel(const RowArgs a, const RowPlan plan, int log_ctas) {
   using VT = Vec16<T>;
@@ -73,14 +74,17 @@ token_stats_kernel(const RowArgs a, const RowPlan plan, int log_ctas) {
   __shared__ int last;
   cg::cluster_group cl = cg::this_cluster();
   const int ctas = 1 << log_ctas, rank = static_cast<int>(blockIdx.x) & (ctas - 1);
-  const int64_t row = static_cast<int64_t>(blockIdx.x) >> log_ctas;
-  const int tid = threadIdx.x, bd = blockDim.x, lane = tid & 31, warp = tid >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = SHORT ? static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + warp : static_cast<int64_t>(blockIdx.x) >> log_ctas;
+  const int tid = SHORT ? lane : threadIdx.x, bd = SHORT ? 32 : blockDim.x;   // within the row's threads
   if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // (waited for before a peer's memory is touched)
   grid_launch_dependents();
   grid_dependency_wait();
-  const T* x = static_cast<const T*>(from_here(a.logits)) + row_offset(a, row);
-  const int tgt = read_target(from_here(a.targets), a.target_bytes, a.has_ignore, a.ignore, row, a.V);
-  if (tgt < 0) {   // the same in every CTA of the cluster
+  const bool real = !SHORT || row < a.M;
+  const T* x = static_cast<const T*>(from_here(a.logits)) + row_offset(a, real ? row : 0);
+  const int tgt = real ? read_target(from_here(a.targets), a.target_bytes, a.has_ignore, a.ignore, row, a.V) : -1;
+  if (!real) {
+  } else if (tgt < 0) {   // the same in every CTA of the cluster
     if (rank == 0 && tid == 0) write_left_out<OP>(a, row, tgt == -2 ? NAN : 0.0f);
     if (ctas > 1) cluster_wait();
   } else {
@@ -140,9 +144,11 @@ token_stats_kernel(const RowArgs a, const RowPlan plan, int log_ctas) {
       }
     }
     warp_combine(m, s, a.k);
-    if (lane == 0) red[warp] = make_float2(m, s);
-    __syncthreads();
-    if (warp == 0) {
+    if (!SHORT) {
+      if (lane == 0) red[warp] = make_float2(m, s);
+      __syncthreads();
+    }
+    if (!SHORT && warp == 0) {
       const float2 p = lane < bd >> 5 ? red[lane] : make_float2(-INFINITY, 0.0f);
       m = p.x; s = p.y;
       warp_combine(m, s, a.k);
@@ -162,10 +168,11 @@ token_stats_kernel(const RowArgs a, const RowPlan plan, int log_ctas) {
     }
     if (rank == 0 && tid == 0) finish_target_row<OP>(a, row, inputs, target_stats(m, s, to_f32(x[tgt]), a.k), true);
   }
-  if (OP == kPolicy && plan.sums != nullptr && rank == 0) {
-    if (tid == 0) {
+  if (OP == kPolicy && plan.sums != nullptr && rank == 0) {   // the same in every thread of the block
+    __syncthreads();   // the block's rows are done
+    if (threadIdx.x == 0) {
       __threadfence();
-      last = atomicAdd(plan.done, 1) == static_cast<int>(a.M) - 1;
+      last = atomicAdd(plan.done, 1) == static_cast<int>(gridDim.x >> log_ctas) - 1;
     }
     __syncthreads();
     if (last) {
@@ -173,13 +180,13 @@ token_stats_kernel(const RowArgs a, const RowPlan plan, int log_ctas) {
       double* sums = reinterpret_cast<double*>(red);
       for (int t = 0; t < plan.n_sums; ++t) {
         double acc = 0.0;
-        for (int64_t q = tid; q < a.M; q += bd) acc += static_cast<double>(__ldcg(a.terms + t * a.M + q));
+        for (int64_t q = threadIdx.x; q < a.M; q += blockDim.x) acc += static_cast<double>(__ldcg(a.terms + t * a.M + q));
         for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
         if (lane == 0) sums[warp] = acc;
         __syncthreads();
-        if (tid == 0) {
+        if (threadIdx.x == 0) {
           double total = 0.0;
-          for (int w = 0; w < bd >> 5; ++w) total += sums[w];
+          for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) total += sums[w];
           plan.sums[t] = static_cast<float>(total);
         }
         __syncthreads();
@@ -191,17 +198,20 @@ token_stats_kernel(const RowArgs a, const RowPlan plan, int log_ctas) {
 // Gradient: dx_j = c (1[j = t] - p_j).  Bound: HBM, one read and one write.  A block takes `piece` vectors of a row, all of them in
 // flight at once.  The rows are taken from the last to the first: what the statistics' kernel read last may still be in L2.
 // Not in place: other blocks of the row read the target's logit.
-template <typename T>
+// SHORT: a warp does (a row has one piece).
+template <typename T, bool SHORT>
 __global__ void __launch_bounds__(kThreads)
-token_grad_stream_kernel(const GradArgs ga, int pieces, uint32_t blocks) {
+token_grad_stream_kernel(const GradArgs ga, int pieces, uint32_t parts) {
   using VT = Vec16<T>;
   using Raw = decltype(VT::raw);
   constexpr int N = VT::N;
   const RowArgs& a = ga.a;
   grid_launch_dependents();
   grid_dependency_wait();
-  const uint32_t b = blocks - 1 - blockIdx.x, row = b / static_cast<uint32_t>(pieces);
-  const int piece = static_cast<int>(b - row * pieces), tid = threadIdx.x, bd = blockDim.x;
+  const uint32_t part = SHORT ? blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5) : blockIdx.x;
+  if (SHORT && part >= parts) return;
+  const uint32_t b = parts - 1 - part, row = b / static_cast<uint32_t>(pieces);
+  const int piece = static_cast<int>(b - row * pieces), tid = SHORT ? threadIdx.x & 31 : threadIdx.x, bd = SHORT ? 32 : blockDim.x;
   const T* x = static_cast<const T*>(from_here(a.logits)) + row_offset(a, row);
   T* g = static_cast<T*>(a.grad) + static_cast<int64_t>(row) * a.V;
   const T* base;
@@ -276,6 +286,12 @@ int launch_stats(const RowArgs& a, const RowPlan& plan, DeviceState* ds, cudaStr
   int log_ctas = 0;
   while (log_ctas < 3 && a.M << (log_ctas + 1) <= 2 * ds->sm_count && vecs >> (log_ctas + 1) >= kUnroll * threads) ++log_ctas;
   if (a.M << log_ctas > 0x7fffffff) return fail(MCB_ERR_SHAPE, "token_stats: too many rows");
+  if (threads == 32) {
+    MCB_CHECK_CUDA(launch_kernel(token_stats_kernel<T, OP, true>, dim3(static_cast<unsigned>((a.M + kThreads / 32 - 1) / (kThreads / 32))), dim3(kThreads),
+                                 0, st, chained_launch(), a, plan, 0));
+    MCB_CHECK_LAUNCH("token_stats");
+    return MCB_OK;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.M << log_ctas)); cfg.blockDim = dim3(static_cast<unsigned>(threads)); cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -284,7 +300,7 @@ int launch_stats(const RowArgs& a, const RowPlan& plan, DeviceState* ds, cudaStr
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr; cfg.numAttrs = chained_launch() ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, token_stats_kernel<T, OP>, a, plan, log_ctas);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, token_stats_kernel<T, OP, false>, a, plan, log_ctas);
   if (e != cudaSuccess) return cuda_fail(e, "token_stats_kernel launch");
   MCB_CHECK_LAUNCH("token_stats");
   return MCB_OK;
@@ -299,8 +315,12 @@ int launch_stream(const GradArgs& ga, DeviceState* ds, cudaStream_t st, bool* ta
   const int64_t pieces = (vecs + kUnroll * threads - 1) / (kUnroll * threads), blocks = pieces * ga.a.M;
   *taken = ga.a.logits != ga.a.grad && blocks <= 0x7fffffff;
   if (!*taken) return MCB_OK;
-  MCB_CHECK_CUDA(launch_kernel(token_grad_stream_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(static_cast<unsigned>(threads)), 0, st,
-                               chained_launch(), ga, static_cast<int>(pieces), static_cast<uint32_t>(blocks)));
+  if (threads == 32)
+    MCB_CHECK_CUDA(launch_kernel(token_grad_stream_kernel<T, true>, dim3(static_cast<unsigned>((blocks + kThreads / 32 - 1) / (kThreads / 32))),
+                                 dim3(kThreads), 0, st, chained_launch(), ga, static_cast<int>(pieces), static_cast<uint32_t>(blocks)));
+  else
+    MCB_CHECK_CUDA(launch_kernel(token_grad_stream_kernel<T, false>, dim3(static_cast<unsigned>(blocks)), dim3(static_cast<unsigned>(threads)), 0, st,
+                                 chained_launch(), ga, static_cast<int>(pieces), static_cast<uint32_t>(blocks)));
   MCB_CHECK_LAUNCH("token_grad_stream");
   return MCB_OK;
 }
