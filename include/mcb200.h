@@ -511,7 +511,7 @@ int mcb_token_logprob_fwd(const mcb_token_logits* logits, const mcb_token_target
 int mcb_token_logprob_bwd(const mcb_token_logits* logits, const mcb_token_targets* targets, const float* logp, const float* lse,
                           const float* dlogp, int64_t dlogp_rows, void* dlogits, void* stream);
 
-/* Workspace of the three calls below; a call's own, like every workspace. */
+/* Workspace of the three calls below, on a 16-byte boundary; a call's own, like every workspace. */
 size_t mcb_token_loss_workspace_bytes(int64_t batch, int64_t seq);
 /* Preference loss of batch / 2 pairs, the chosen sequences first: with L = sum (average: mean) of a sequence's log-probabilities,
  * z = beta ((L_c - ref_c) - (L_r - ref_r)):  loss[0] = mean of -(1 - label_smoothing) log sigma(z) - label_smoothing log sigma(-z).

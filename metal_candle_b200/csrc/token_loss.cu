@@ -1,6 +1,10 @@
 // Losses over the logits [M, V] of given tokens, with their gradients: token log-probabilities, the preference loss of pairs,
 // the clipped policy loss with a KL term, and distillation from a teacher's top logits.
+#include <cooperative_groups.h>
+
 #include "token_loss.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace mcb {
 namespace {
@@ -53,7 +57,7 @@ token_rows_kernel(const RowArgs a) {
       if (tgt == -2) left_out = NAN;
     }
     if (out) {
-      if (tid == 0) write_left_out<OP>(a, row, left_out);
+      if (tid == 0) write_left_out<OP>(a, row, left_out, nullptr);
       if (g != nullptr)
         for (int c = tid; c < a.V; c += nt) g[c] = from_f32<T>(left_out);
       continue;
@@ -69,7 +73,9 @@ token_rows_kernel(const RowArgs a) {
     if constexpr (OP != kDistill) {
       const float xt = to_f32(x[tgt]);
       const TargetStats r = target_stats(m, s, xt, a.k);
-      const float c0 = finish_target_row<OP>(a, row, row_inputs<OP>(a, row), r, tid == 0);
+      const RowResult res = finish_target_row<OP>(a, row_inputs<OP>(a, row), r);
+      if (tid == 0) write_target_row<OP>(a, row, r, res, nullptr);
+      const float c0 = res.c;
       __syncthreads();   // everyone has read the target's logit, which the gradient may lie over
       if (g != nullptr) {
         const float f = -c0 / r.sum;
@@ -162,20 +168,27 @@ token_grad_kernel(const GradArgs ga) {
 // The weight of each row in the mean: 1 / kept rows, or 1 / (kept rows of its sequence x sequences that keep any).  Kept are the
 // rows whose mask is not 0, or whose target is not left out; a target out of range gets NaN.  Neither given: all rows.
 // `order`, unless null: the kept rows first, in one fixed order, then the others; and info[0] = how many are kept, info[1] = 0.
-// One block: it is the longest chain in front of the losses of few rows, and 32768 targets are 256 KB.  Up to 8192 rows (and 2048
-// sequences) the targets are read once and stay in registers: 600 rows XXX us.
+// One block, or a cluster of 8 with a part of the rows each: it is the longest chain in front of the losses.  Up to 8192 rows a block the
+// targets are read once and stay in registers; up to 2048 sequences are counted as their rows pass, in the first block's memory.
 constexpr int kSeqCounts = 2048;
 __global__ void __launch_bounds__(1024)
 row_weights_kernel(const void* targets, int target_bytes, int has_ignore, int64_t ignore, const uint8_t* mask, float* weight,
                    int32_t* order, int32_t* info, int M, int S, int V, int sequence_mean) {
   __shared__ int red[32];
+  __shared__ int2 totals[8];      // each block's (kept, not kept)
+  __shared__ int nonempty[8];     // and sequences that keep any
   __shared__ int counts[kSeqCounts];
   constexpr int kRows = 8, kRound = 1024 * kRows;
+  cg::cluster_group cl = cg::this_cluster();
+  const int n = static_cast<int>(gridDim.x), rank = static_cast<int>(blockIdx.x);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sequences = M / S;
-  const bool counted = sequence_mean && sequences <= kSeqCounts;   // in shared memory, as the rows pass
+  const bool counted = sequence_mean && sequences <= kSeqCounts;
+  auto all_sync = [&]() { if (n > 1) cl.sync(); else __syncthreads(); };
+  auto there = [&](auto* p, int r) { return n > 1 ? cl.map_shared_rank(p, r) : p; };
   if (counted)
     for (int b = threadIdx.x; b < sequences; b += 1024) counts[b] = 0;
+  all_sync();   // (every block has begun, and its counts are cleared)
   grid_launch_dependents();
   grid_dependency_wait();
   targets = from_here(targets);
@@ -186,117 +199,149 @@ row_weights_kernel(const void* targets, int target_bytes, int has_ignore, int64_
     const int t = read_target(targets, target_bytes, has_ignore, ignore, row, V);
     return t >= 0 ? 1 : t + 1;
   };
-  // eight rows a thread at a time; each warp counts its kept rows and the others, the block those of the warps before it
-  int keep[kRows];
-  int total = 0;
-  for (int64_t base = 0; base < M; base += kRound) {
+  const int64_t per = (static_cast<int64_t>(M) + n - 1) / n, lo = min(static_cast<int64_t>(M), rank * per), hi = min(static_cast<int64_t>(M), lo + per);
+  // eight rows a thread at a time; votes: of each warp's 32, kept and not kept
+  int keep[kRows], ours, theirs;
+  uint32_t votes[kRows], others[kRows];
+  auto look = [&](int64_t base) {
     const int64_t mine = base + threadIdx.x;
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) keep[r] = mine + r * 1024 < M ? kept(static_cast<int>(mine) + r * 1024) : 0;
-    uint32_t votes[kRows], others[kRows];
-    int c = 0;   // kept, and 65536 times those that are not (a round has 8192)
+    for (int r = 0; r < kRows; ++r) keep[r] = mine + r * 1024 < hi ? kept(static_cast<int>(mine + r * 1024)) : 0;
+    ours = theirs = 0;
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       votes[r] = __ballot_sync(0xffffffffu, keep[r] != 0);
-      others[r] = __ballot_sync(0xffffffffu, mine + r * 1024 < M && keep[r] == 0);
-      c += __popc(votes[r]) + (__popc(others[r]) << 16);
+      others[r] = __ballot_sync(0xffffffffu, mine + r * 1024 < hi && keep[r] == 0);
+      ours += __popc(votes[r]);
+      theirs += __popc(others[r]);
     }
-    __syncthreads();   // red is free, counts are cleared
-    if (lane == 0) red[warp] = c;
-    if (counted) {
+  };
+  auto block_total = [&](int v) {   // of a value each warp's lanes share
+    __syncthreads();
+    if (lane == 0) red[warp] = v;
+    __syncthreads();
+    return __reduce_add_sync(0xffffffffu, red[lane]);
+  };
+  int warp_ours = 0, warp_theirs = 0;
+  for (int64_t base = lo; base < hi; base += kRound) {
+    look(base);
+    warp_ours += ours;
+    warp_theirs += theirs;
+    if (!counted) continue;
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        if (votes[r] == 0) continue;
-        const int64_t row0 = mine - lane + r * 1024;
-        const int b0 = static_cast<int>(row0) / S;
-        if (row0 + 31 < static_cast<int64_t>(b0 + 1) * S) {   // all 32 rows of one sequence
-          if (lane == 0) atomicAdd(counts + b0, __popc(votes[r]));
-        } else if (keep[r] != 0) {
-          atomicAdd(counts + static_cast<int>(row0 + lane) / S, 1);
-        }
+    for (int r = 0; r < kRows; ++r) {
+      if (votes[r] == 0) continue;
+      const int64_t row0 = base + warp * 32 + r * 1024;
+      const int b0 = static_cast<int>(row0) / S;
+      if (row0 + 31 < static_cast<int64_t>(b0 + 1) * S) {   // all 32 rows of one sequence
+        if (lane == 0) atomicAdd(there(counts, 0) + b0, __popc(votes[r]));
+      } else if (keep[r] != 0) {
+        atomicAdd(there(counts, 0) + static_cast<int>(row0 + lane) / S, 1);
       }
     }
+  }
+  const int block_ours = block_total(warp_ours), block_theirs = block_total(warp_theirs);
+  int block_sequences = 0;
+  if (sequence_mean && !counted) {
+    for (int64_t b = rank * 32 + warp; b < sequences; b += n * 32) {
+      int c = 0;
+      for (int i = lane; i < S; i += 32) c += kept(static_cast<int>(b * S) + i) != 0;
+      block_sequences += __reduce_add_sync(0xffffffffu, c) > 0;
+    }
+    block_sequences = block_total(block_sequences);
+  }
+  if (static_cast<int>(threadIdx.x) < n) {
+    there(totals, threadIdx.x)[rank] = make_int2(block_ours, block_theirs);
+    there(nonempty, threadIdx.x)[rank] = block_sequences;
+  }
+  all_sync();
+  int total = 0, at0 = 0, out0 = 0, with_any = 0;
+  for (int r = 0; r < n; ++r) {
+    total += totals[r].x;
+    with_any += nonempty[r];
+    if (r < rank) { at0 += totals[r].x; out0 += totals[r].y; }
+  }
+  if (counted) {
+    int c = 0;
+    for (int b = threadIdx.x; b < sequences; b += 1024) c += there(counts, 0)[b] > 0;
+    with_any = block_total(__reduce_add_sync(0xffffffffu, c));
+  }
+  const float share = 1.0f / static_cast<float>(max(1, sequence_mean ? with_any : total));
+  if (rank == 0 && threadIdx.x == 0 && info != nullptr) { info[0] = total; info[1] = 0; }
+  for (int64_t base = lo; base < hi; base += kRound) {
+    if (hi - lo > kRound) look(base);   // (else it has been looked at)
     __syncthreads();
-    c = red[lane];
-    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? c : 0);
-    int at = total + (before & 0xffff), out = static_cast<int>(base) - total + (before >> 16);   // places from the order's ends
-    total += __reduce_add_sync(0xffffffffu, c) & 0xffff;
-    if (order == nullptr) continue;
+    if (lane == 0) red[warp] = ours + (theirs << 16);   // (a round has 8192 of both)
+    __syncthreads();
+    const int c = red[lane];
+    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? c : 0), sum = __reduce_add_sync(0xffffffffu, c);
+    int at = at0 + (before & 0xffff), out = out0 + (before >> 16);   // places from the order's ends
+    at0 += sum & 0xffff;
+    out0 += sum >> 16;
     const uint32_t below = (1u << lane) - 1u;
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const int row = static_cast<int>(mine) + r * 1024;
-      if (mine + r * 1024 < M) order[keep[r] != 0 ? at + __popc(votes[r] & below) : M - 1 - (out + __popc(others[r] & below))] = row;
+      const int64_t row = base + threadIdx.x + r * 1024;
+      if (row < hi) {
+        if (order != nullptr)
+          order[keep[r] != 0 ? at + __popc(votes[r] & below) : M - 1 - (out + __popc(others[r] & below))] = static_cast<int32_t>(row);
+        if (!sequence_mean || counted)
+          weight[row] = keep[r] == 0 ? 0.0f : keep[r] < 0 ? NAN : counted ? share / static_cast<float>(there(counts, 0)[static_cast<int>(row) / S]) : share;
+      }
       at += __popc(votes[r]);
       out += __popc(others[r]);
     }
   }
-  if (threadIdx.x == 0 && info != nullptr) { info[0] = total; info[1] = 0; }
-  float share = 1.0f / static_cast<float>(max(1, total));
-  if (sequence_mean) {
-    // the sequences that keep any
-    int n = 0;
-    if (counted) {
-      for (int b = threadIdx.x; b < sequences; b += 1024) n += counts[b] > 0;
-    } else {
-      for (int b = warp; b < sequences; b += 32) {
-        int c = 0;
-        for (int i = lane; i < S; i += 32) c += kept(b * S + i) != 0;
-        c = __reduce_add_sync(0xffffffffu, c);
-        n += lane == 0 && c > 0;
+  if (sequence_mean && !counted) {
+    for (int64_t b = rank * 32 + warp; b < sequences; b += n * 32) {
+      int c = 0;
+      for (int i = lane; i < S; i += 32) c += kept(static_cast<int>(b * S) + i) != 0;
+      c = __reduce_add_sync(0xffffffffu, c);
+      for (int i = lane; i < S; i += 32) {
+        const int k = kept(static_cast<int>(b * S) + i);
+        weight[b * S + i] = k == 0 ? 0.0f : k < 0 ? NAN : share / static_cast<float>(c);
       }
     }
-    n = __reduce_add_sync(0xffffffffu, n);
-    __syncthreads();
-    if (lane == 0) red[warp] = n;
-    __syncthreads();
-    n = __reduce_add_sync(0xffffffffu, red[lane]);
-    share = 1.0f / static_cast<float>(max(1, n));
-    if (!counted) {
-      for (int b = warp; b < sequences; b += 32) {
-        int c = 0;
-        for (int i = lane; i < S; i += 32) c += kept(b * S + i) != 0;
-        c = __reduce_add_sync(0xffffffffu, c);
-        for (int i = lane; i < S; i += 32) {
-          const int k = kept(b * S + i);
-          weight[b * S + i] = k == 0 ? 0.0f : k < 0 ? NAN : share / static_cast<float>(c);
-        }
-      }
-      return;
-    }
   }
-  auto put = [&](int row, int k) {
-    weight[row] = k == 0 ? 0.0f : k < 0 ? NAN : counted ? share / static_cast<float>(counts[row / S]) : share;
-  };
-  if (M <= kRound) {
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      const int row = static_cast<int>(threadIdx.x) + r * 1024;
-      if (row < M) put(row, keep[r]);
-    }
-  } else {
-    for (int64_t i = threadIdx.x; i < M; i += 1024) put(static_cast<int>(i), kept(static_cast<int>(i)));
-  }
+  if (n > 1) cl.sync();   // no peer still reads here
 }
 
-// out[i] = sum of terms[i][0 .. M), in one fixed order
-__global__ void __launch_bounds__(1024)
+// out[i] = sum of terms[i][0 .. M), i < n <= 8, in one order: a cluster of 8 blocks with a part each, eight loads in flight a thread.
+__global__ void __launch_bounds__(1024) __cluster_dims__(8, 1, 1)
 sum_terms_kernel(const float* terms, int64_t M, int n, float* out) {
-  __shared__ double red[1024];
+  __shared__ double warp_sums[32];
+  __shared__ double parts[8][8];
+  cg::cluster_group cl = cg::this_cluster();
+  const int rank = static_cast<int>(blockIdx.x), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  cl.sync();   // every block has begun
   grid_launch_dependents();
   grid_dependency_wait();
   terms = from_here(terms);
+  const int64_t per = (M + 7) / 8, lo = min(M, rank * per), hi = min(M, lo + per);
   for (int t = 0; t < n; ++t) {
     double acc = 0.0;
-    for (int64_t i = threadIdx.x; i < M; i += 1024) acc += static_cast<double>(terms[t * M + i]);
-    red[threadIdx.x] = acc;
-    __syncthreads();
-    for (int o = 512; o > 0; o >>= 1) {
-      if (threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
-      __syncthreads();
+    for (int64_t i = lo + threadIdx.x; i < hi; i += 8 * 1024) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = i + j * 1024 < hi ? __ldcg(terms + t * M + i + j * 1024) : 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc += static_cast<double>(v[j]);
     }
-    if (threadIdx.x == 0) out[t] = static_cast<float>(red[0]);
+    for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    __syncthreads();   // warp_sums is free
+    if (lane == 0) warp_sums[warp] = acc;
     __syncthreads();
+    if (threadIdx.x == 0) {
+      double total = 0.0;
+      for (int w = 0; w < 32; ++w) total += warp_sums[w];
+      *cl.map_shared_rank(&parts[t][rank], 0) = total;
+    }
+  }
+  cl.sync();
+  if (rank == 0 && static_cast<int>(threadIdx.x) < n) {
+    double total = 0.0;
+    for (int r = 0; r < 8; ++r) total += parts[threadIdx.x][r];
+    out[threadIdx.x] = static_cast<float>(total);
   }
 }
 
@@ -366,12 +411,26 @@ __global__ void __launch_bounds__(256) scale_rows_kernel(T* x, const float* coef
 
 int launch_sum(const float* terms, int64_t M, int n, float* out, cudaStream_t st);
 
+constexpr int64_t kSumInside = 4096;   // rows whose terms the one-pass kernel's last block sums
 template <int OP>
 int launch_rows(const RowArgs& a, const RowPlan& plan, int dtype, DeviceState* ds, cudaStream_t st) {
-  if (OP == kStats || (OP == kPolicy && a.grad == nullptr)) return launch_stats_rows(OP, a, plan, dtype, ds, st);
+  if (OP == kStats || (OP == kPolicy && a.grad == nullptr)) {
+    if (int rc = launch_stats_rows(OP, a, dtype, ds, st)) return rc;
+    return plan.sums != nullptr ? launch_sum(a.terms, a.M, plan.n_sums, plan.sums, st) : MCB_OK;
+  }
   bool taken = false;
-  if (int rc = launch_resident_rows(OP, a, plan, dtype, ds, st, &taken)) return rc;
-  if (taken) return MCB_OK;
+  if (OP != kDistill) {
+    RowArgs b = a;
+    if (plan.sums != nullptr) b.terms = nullptr;   // summed on the way
+    if (int rc = launch_short_rows(OP, b, plan, dtype, ds, st, &taken)) return rc;
+    if (taken) return MCB_OK;
+  }
+  // The sums of many rows by a launch of their own: the last block alone would take 20 us for the three terms of 20000.
+  const bool apart = plan.sums != nullptr && a.M > kSumInside;
+  RowPlan inside = plan;
+  if (apart) inside.sums = nullptr;
+  if (int rc = launch_resident_rows(OP, a, inside, dtype, ds, st, &taken)) return rc;
+  if (taken) return apart ? launch_sum(a.terms, a.M, plan.n_sums, plan.sums, st) : MCB_OK;
   const int64_t most = static_cast<int64_t>(ds->sm_count) * 8;
   const dim3 grid(static_cast<unsigned>(a.M < most ? a.M : most));
   if (dtype == MCB_F32)
@@ -398,15 +457,24 @@ int launch_grad(const GradArgs& ga, int dtype, DeviceState* ds, cudaStream_t st)
 
 int launch_weights(const mcb_token_targets* t, const uint8_t* mask, float* weight, int32_t* order, int32_t* info, int64_t M, int64_t S,
                    int64_t V, int sequence_mean, cudaStream_t st) {
-  MCB_CHECK_CUDA(launch_kernel(row_weights_kernel, dim3(1), dim3(1024), 0, st, chained_launch(), t ? t->targets : nullptr,
-                               t ? t->target_bytes : 0, t ? t->has_ignore : 0, t ? t->ignore_index : 0, mask, weight, order, info, static_cast<int>(M), static_cast<int>(S),
-                               static_cast<int>(V), sequence_mean));
+  cudaLaunchConfig_t cfg = {};
+  const unsigned blocks = M > 2048 ? 8 : 1;   // (each thread of a block alone would take its second two rows in turn)
+  cfg.gridDim = dim3(blocks); cfg.blockDim = dim3(1024); cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr; cfg.numAttrs = chained_launch() ? 2 : 1;
+  MCB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, row_weights_kernel, t ? t->targets : nullptr, t ? t->target_bytes : 0, t ? t->has_ignore : 0,
+                                    t ? t->ignore_index : 0, mask, weight, order, info, static_cast<int>(M), static_cast<int>(S),
+                                    static_cast<int>(V), sequence_mean));
   MCB_CHECK_LAUNCH("row_weights");
   return MCB_OK;
 }
 
 int launch_sum(const float* terms, int64_t M, int n, float* out, cudaStream_t st) {
-  MCB_CHECK_CUDA(launch_kernel(sum_terms_kernel, dim3(1), dim3(1024), 0, st, chained_launch(), terms, M, n, out));
+  MCB_CHECK_CUDA(launch_kernel(sum_terms_kernel, dim3(8), dim3(1024), 0, st, chained_launch(), terms, M, n, out));
   MCB_CHECK_LAUNCH("sum_terms");
   return MCB_OK;
 }
@@ -458,15 +526,17 @@ int check_teacher(const char* what, const mcb_teacher_top* t) {
   return MCB_OK;
 }
 
-// Workspace of a whole loss: a weight, up to three terms and a place in the order for each row, and two counters.
+// Workspace of a whole loss: what the blocks leave to be summed; a weight, up to three terms and a place in the order for each row; and
+// two counters.
 struct LossWorkspace {
+  double* partials;
   float* weight;
   float* terms;
   int32_t* order;
   int32_t* info;
   LossWorkspace(void* base, int64_t M)
-      : weight(static_cast<float*>(base)), terms(weight + M), order(reinterpret_cast<int32_t*>(terms + 3 * M)), info(order + M) {}
-  RowPlan plan(float* sums, int n) const { return {order, info, sums, n, info + 1}; }
+      : partials(static_cast<double*>(base)), weight(reinterpret_cast<float*>(partials + 3 * kMaxPartials)), terms(weight + M), order(reinterpret_cast<int32_t*>(terms + 3 * M)), info(order + M) {}
+  RowPlan plan(float* sums, int n) const { return {order, info, sums, n, info + 1, partials}; }
 };
 
 RowArgs row_args(const mcb_token_logits* l, void* grad) {
@@ -581,7 +651,7 @@ extern "C" int mcb_distill_loss_rows(const mcb_token_logits* logits, const mcb_t
 
 extern "C" size_t mcb_token_loss_workspace_bytes(int64_t batch, int64_t seq) {
   if (batch <= 0 || seq <= 0 || batch > kMaxDim || seq > kMaxDim || batch * seq > kMaxDim) return 0;
-  return (static_cast<size_t>(batch * seq) * 5 + static_cast<size_t>(batch) + 64) * sizeof(float);
+  return (static_cast<size_t>(batch * seq) * 5 + static_cast<size_t>(batch) + 64) * sizeof(float) + 3 * kMaxPartials * sizeof(double);
 }
 
 extern "C" int mcb_policy_loss(const mcb_token_logits* logits, const mcb_token_targets* targets, const mcb_policy_terms* policy, int sequence_mean,
@@ -593,6 +663,7 @@ extern "C" int mcb_policy_loss(const mcb_token_logits* logits, const mcb_token_t
   if (!logp || !out) return fail(MCB_ERR_NULL, "policy_loss: null output");
   if (!workspace || workspace_bytes < mcb_token_loss_workspace_bytes(logits->batch, logits->seq))
     return fail(MCB_ERR_WORKSPACE, "policy_loss: workspace missing or too small");
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return fail(MCB_ERR_ALIGN, "policy_loss: the workspace must lie on a 16-byte boundary");
   DeviceState* ds = current_device_state();
   if (!ds) return MCB_ERR_NOT_INIT;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -613,6 +684,7 @@ extern "C" int mcb_distill_loss(const mcb_token_logits* logits, const mcb_teache
   if (!loss) return fail(MCB_ERR_NULL, "distill_loss: null output");
   if (!workspace || workspace_bytes < mcb_token_loss_workspace_bytes(logits->batch, logits->seq))
     return fail(MCB_ERR_WORKSPACE, "distill_loss: workspace missing or too small");
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return fail(MCB_ERR_ALIGN, "distill_loss: the workspace must lie on a 16-byte boundary");
   DeviceState* ds = current_device_state();
   if (!ds) return MCB_ERR_NOT_INIT;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -43,7 +43,7 @@ struct RowArgs {
   // what a row leaves behind
   float* logp;             // [M] (kDistill: none)
   float* lse;              // [M], or null
-  float* terms;            // kPolicy: [3, M]: loss, KL, clipped; kDistill: [M]; each times the row's weight
+  float* terms;            // kPolicy: [3, M]: loss, KL, clipped; kDistill: [M]; each times the row's weight.  Null: they are summed only
 };
 
 __device__ __forceinline__ int64_t row_offset(const RowArgs& a, int64_t row) {   // (rows and S are below 2^31)
@@ -147,31 +147,42 @@ __device__ __forceinline__ PolicyTerm policy_term(const RowArgs& a, const RowInp
   return t;
 }
 
-// What a row's log-probability comes to: writes the row's outputs (`write`: by one thread) and returns d loss / d logp / T.
+// What a row's log-probability comes to: d loss / d logp / T, and the row's terms.
+struct RowResult {
+  float c, terms[3];
+};
 template <int OP>
-__device__ __forceinline__ float finish_target_row(const RowArgs& a, int64_t row, const RowInputs& in, const TargetStats& r, bool write) {
-  if (write && a.logp != nullptr) a.logp[row] = r.logp;
-  if (write && a.lse != nullptr) a.lse[row] = r.top * a.inv_t + logf(r.sum);
+__device__ __forceinline__ RowResult finish_target_row(const RowArgs& a, const RowInputs& in, const TargetStats& r) {
+  RowResult out = {a.inv_t, {0.0f, 0.0f, 0.0f}};
   if constexpr (OP == kPolicy) {
     const float w = in.weight;
     const PolicyTerm t = policy_term(a, in, r.logp);
-    if (write) {
-      a.terms[row] = w * t.loss;
-      a.terms[a.M + row] = w * t.kl;
-      a.terms[2 * a.M + row] = w * t.clipped;
-    }
-    return w * t.dlogp * a.inv_t;
+    out.c = w * t.dlogp * a.inv_t;
+    out.terms[0] = w * t.loss; out.terms[1] = w * t.kl; out.terms[2] = w * t.clipped;
   }
-  return a.inv_t;
+  return out;
 }
-
+// What the row leaves behind, by one thread.  sums: where its terms are added up, or null.
+template <int OP>
+__device__ __forceinline__ void write_row(const RowArgs& a, int64_t row, float logp, float lse, const float* terms, double* sums) {
+  constexpr int n = OP == kPolicy ? 3 : OP == kDistill ? 1 : 0;
+  if (OP != kDistill && a.logp != nullptr) a.logp[row] = logp;
+  if (OP != kDistill && a.lse != nullptr) a.lse[row] = lse;
+#pragma unroll
+  for (int t = 0; t < n; ++t) {
+    if (a.terms != nullptr) a.terms[t * a.M + row] = terms[t];
+    if (sums != nullptr) sums[t] += static_cast<double>(terms[t]);
+  }
+}
+template <int OP>
+__device__ __forceinline__ void write_target_row(const RowArgs& a, int64_t row, const TargetStats& r, const RowResult& out, double* sums) {
+  write_row<OP>(a, row, r.logp, a.lse != nullptr ? r.top * a.inv_t + logf(r.sum) : 0.0f, out.terms, sums);
+}
 // A row that is left out (value 0) or whose target is out of range (NaN).
 template <int OP>
-__device__ __forceinline__ void write_left_out(const RowArgs& a, int64_t row, float value) {
-  if (a.logp != nullptr) a.logp[row] = value;
-  if (a.lse != nullptr) a.lse[row] = value;
-  if constexpr (OP == kPolicy) { a.terms[row] = value; a.terms[a.M + row] = value; a.terms[2 * a.M + row] = value; }
-  if constexpr (OP == kDistill) a.terms[row] = value;
+__device__ __forceinline__ void write_left_out(const RowArgs& a, int64_t row, float value, double* sums) {
+  const float terms[3] = {value, value, value};
+  write_row<OP>(a, row, value, value, terms, sums);
 }
 
 __device__ __forceinline__ float read_teacher(const RowArgs& a, int64_t i) {
@@ -181,15 +192,47 @@ __device__ __forceinline__ int64_t read_teacher_id(const RowArgs& a, int64_t i) 
   return a.id_bytes == 8 ? static_cast<const int64_t*>(a.teacher_ids)[i] : static_cast<const int32_t*>(a.teacher_ids)[i];
 }
 
-// Rows in the order they are to be taken, the kept ones first (as mcb_loss_weights tells them apart), and where the sum of each of
-// the rows' terms goes.  All null for a chunk of rows.
+// out[t] = sum over i < count of terms[i * step + t * apart] by one block, in an order that depends on its size alone; eight loads in
+// flight a thread.  warp_sums: room for a double a warp.
+template <int THREADS = 0, typename V>   // (0: whatever the block has)
+__device__ __forceinline__ void block_sums(const V* terms, int64_t count, int64_t step, int64_t apart, int n, float* out, double* warp_sums) {
+  const int nt = THREADS > 0 ? THREADS : blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int t = 0; t < n; ++t) {
+    double acc = 0.0;
+    for (int64_t i = threadIdx.x; i < count; i += 8 * nt) {
+      V v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = i + j * nt < count ? __ldcg(terms + t * apart + (i + j * nt) * step) : V(0);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc += static_cast<double>(v[j]);
+    }
+    for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    __syncthreads();   // warp_sums is free
+    if (lane == 0) warp_sums[warp] = acc;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      double total = 0.0;
+      for (int w = 0; w < nt >> 5; ++w) total += warp_sums[w];
+      out[t] = static_cast<float>(total);
+    }
+  }
+}
+
+// Rows in the order they are to be taken, the kept ones first (as mcb_loss_weights tells them apart), and where the sums of the rows'
+// terms go.  The last block to finish makes them, in one order: of the terms, or (short rows, of which there may be many) of what each
+// block has added up over its rows, which are the same from call to call.  All null for a chunk of rows.
+constexpr int kMaxPartials = 2048;   // blocks of such a launch, each with 3 doubles
 struct RowPlan {
   const int32_t* order;
   const int32_t* kept;
   float* sums;      // n_sums of them
   int n_sums;
   int* done;        // 0 when the kernel starts
+  double* partials;
 };
+
+// kUnit and kPolicy, rows of at most 256 vectors, each in the registers of a warp (token_stream.cu).
+int launch_short_rows(int op, const RowArgs& a, const RowPlan& plan, int dtype, DeviceState* ds, cudaStream_t st, bool* taken);
 
 // The one-pass kernel (token_resident.cu), where it takes rows of this length: *taken says whether it did.
 int launch_resident_rows(int op, const RowArgs& a, const RowPlan& plan, int dtype, DeviceState* ds, cudaStream_t st, bool* taken);
@@ -203,7 +246,7 @@ struct GradArgs {
 };
 
 // token_stream.cu: kStats, or kPolicy without a gradient; and the gradient, where it is not in place.
-int launch_stats_rows(int op, const RowArgs& a, const RowPlan& plan, int dtype, DeviceState* ds, cudaStream_t st);
+int launch_stats_rows(int op, const RowArgs& a, int dtype, DeviceState* ds, cudaStream_t st);
 int launch_grad_stream(const GradArgs& ga, int dtype, DeviceState* ds, cudaStream_t st, bool* taken);
 
 }  // namespace tokenloss

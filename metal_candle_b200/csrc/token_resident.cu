@@ -420,7 +420,7 @@ token_resident_kernel(const RowArgs a, const Resident p) {
     const RowInfo& info = infos[at];
     if (info.state != 0) {   // the same in every CTA of the cluster
       const float value = info.state == 2 ? NAN : 0.0f;
-      if (rank == 0 && tid == 0) write_left_out<OP>(a, info.row, value);
+      if (rank == 0 && tid == 0) write_left_out<OP>(a, info.row, value, nullptr);
       if (a.grad != nullptr) {
         const Share& s = info.share;
         T* g = static_cast<T*>(a.grad) + s.to;
@@ -627,7 +627,9 @@ token_resident_kernel(const RowArgs a, const Resident p) {
         f_top = empty_teacher ? 0.0f : c0 / sw;
       } else {
         const TargetStats r = target_stats(mw, sw, third, a.k);
-        c0 = finish_target_row<OP>(a, row, info.in, r, writes);
+        const RowResult out = finish_target_row<OP>(a, info.in, r);
+        if (writes) write_target_row<OP>(a, row, r, out, nullptr);
+        c0 = out.c;
         at_target = c0 * r.rest;
         f_top = -c0 / r.sum;
         top = r.top == -INFINITY ? 0.0f : r.top;
@@ -755,7 +757,7 @@ token_resident_kernel(const RowArgs a, const Resident p) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
   }
   if (ctas > 1) cl.sync();   // no peer still writes here
-  if (p.out != nullptr && rank == 0) {
+  if (OP != kUnit && p.out != nullptr && rank == 0) {
     // the last cluster to finish sums what all have left, in one order whichever it is
     if (threadIdx.x == 0) {
       __threadfence();
@@ -764,20 +766,7 @@ token_resident_kernel(const RowArgs a, const Resident p) {
     __syncthreads();
     if (last) {
       __threadfence();
-      double* sums = reinterpret_cast<double*>(smem);
-      for (int t = 0; t < p.n_out; ++t) {
-        double acc = 0.0;
-        for (uint32_t q = threadIdx.x; q < M; q += kAllThreads) acc += static_cast<double>(__ldcg(a.terms + static_cast<int64_t>(t) * M + q));
-        for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-        if (lane == 0) sums[warp] = acc;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-          double total = 0.0;
-          for (int w = 0; w < kAllThreads / 32; ++w) total += sums[w];
-          p.out[t] = static_cast<float>(total);
-        }
-        __syncthreads();
-      }
+      block_sums<kAllThreads>(a.terms, a.M, 1, a.M, p.n_out, p.out, reinterpret_cast<double*>(smem));
     }
   }
 }

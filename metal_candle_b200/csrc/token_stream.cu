@@ -65,13 +65,12 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // blocks of a warp each 41 us: as many launches of blocks as rows).
 template <typename T, int OP, bool SHORT>
 __global__ void __launch_bounds__(kThreads)
-token_stats_kernel(const RowArgs a, const RowPlan plan, int log_ctas) {
+token_stats_kernel(const RowArgs a, int log_ctas) {
   using VT = Vec16<T>;
   using Raw = decltype(VT::raw);
   constexpr int N = VT::N;
   __shared__ float2 red[kThreads / 32];
   __shared__ float2 parts[8];
-  __shared__ int last;
   cg::cluster_group cl = cg::this_cluster();
   const int ctas = 1 << log_ctas, rank = static_cast<int>(blockIdx.x) & (ctas - 1);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -85,7 +84,7 @@ token_stats_kernel(const RowArgs a, const RowPlan plan, int log_ctas) {
   const int tgt = real ? read_target(from_here(a.targets), a.target_bytes, a.has_ignore, a.ignore, row, a.V) : -1;
   if (!real) {
   } else if (tgt < 0) {   // the same in every CTA of the cluster
-    if (rank == 0 && tid == 0) write_left_out<OP>(a, row, tgt == -2 ? NAN : 0.0f);
+    if (rank == 0 && tid == 0) write_left_out<OP>(a, row, tgt == -2 ? NAN : 0.0f, nullptr);
     if (ctas > 1) cluster_wait();
   } else {
     const T* base;
@@ -166,31 +165,9 @@ token_stats_kernel(const RowArgs a, const RowPlan plan, int log_ctas) {
         warp_combine(m, s, a.k);
       }
     }
-    if (rank == 0 && tid == 0) finish_target_row<OP>(a, row, inputs, target_stats(m, s, to_f32(x[tgt]), a.k), true);
-  }
-  if (OP == kPolicy && plan.sums != nullptr && rank == 0) {   // the same in every thread of the block
-    __syncthreads();   // the block's rows are done
-    if (threadIdx.x == 0) {
-      __threadfence();
-      last = atomicAdd(plan.done, 1) == static_cast<int>(gridDim.x >> log_ctas) - 1;
-    }
-    __syncthreads();
-    if (last) {
-      __threadfence();
-      double* sums = reinterpret_cast<double*>(red);
-      for (int t = 0; t < plan.n_sums; ++t) {
-        double acc = 0.0;
-        for (int64_t q = threadIdx.x; q < a.M; q += blockDim.x) acc += static_cast<double>(__ldcg(a.terms + t * a.M + q));
-        for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-        if (lane == 0) sums[warp] = acc;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-          double total = 0.0;
-          for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) total += sums[w];
-          plan.sums[t] = static_cast<float>(total);
-        }
-        __syncthreads();
-      }
+    if (rank == 0 && tid == 0) {
+      const TargetStats t = target_stats(m, s, to_f32(x[tgt]), a.k);
+      write_target_row<OP>(a, row, t, finish_target_row<OP>(a, inputs, t), nullptr);
     }
   }
 }
@@ -276,8 +253,157 @@ token_grad_stream_kernel(const GradArgs ga, int pieces, uint32_t parts) {
   if (edges) to[edge] = from_f32<T>(edge == te ? at_target : -c0 * ex2(fmaf(to_f32(base[edge]) - ref, a.k, add)));
 }
 
+// Short rows, statistics and gradient: a row in the registers of a warp, as it was read; its exponentials are taken twice (there
+// are few).  Any row may be written over.  20000 x 1000 bf16: XXX us, by the one-pass kernel's warps, whose every row passes
+// through a ring, barriers and a table, 64.  (Distillation is left to that one: its warps wait less for the teacher's entries.)
+constexpr int kShortBlocks = 3;      // blocks an SM, which take rows in turn
 template <typename T, int OP>
-int launch_stats(const RowArgs& a, const RowPlan& plan, DeviceState* ds, cudaStream_t st) {
+__global__ void __launch_bounds__(kThreads, kShortBlocks)
+token_short_kernel(const RowArgs a, const RowPlan plan) {
+  using VT = Vec16<T>;
+  using Raw = decltype(VT::raw);
+  constexpr int N = VT::N, kRows = kThreads / 32;
+  __shared__ double sums[kRows][3];
+  __shared__ int last;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x < kRows * 3) sums[0][threadIdx.x] = 0.0;
+  __syncthreads();
+  grid_launch_dependents();
+  grid_dependency_wait();
+  double* mine = plan.sums != nullptr ? sums[warp] : nullptr;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + warp; row < a.M; row += static_cast<int64_t>(gridDim.x) * kRows) {
+    const T* x = static_cast<const T*>(from_here(a.logits)) + row_offset(a, row);
+    T* g = a.grad != nullptr ? static_cast<T*>(a.grad) + row * a.V : nullptr;
+    const T* base;
+    const RowVecs r = vecs_of(x, a.V, base);
+    const Raw* src = reinterpret_cast<const Raw*>(base);
+    T* to = g - r.lo;
+    const bool same = (reinterpret_cast<uintptr_t>(to) & 15u) == 0;
+    const int edge = lane < N ? r.lo + lane : r.fb * N + lane - N;   // the elements beside the row's own vectors
+    const bool edges = lane < 2 * N && (lane < N ? edge < min(r.fa * N, r.hi) : edge < r.hi);
+    VT v[kUnroll];
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+      const int vi = r.fa + j * 32 + lane;
+      if (vi < r.fb) v[j].raw = src[vi];
+      else fill_masked(v[j]);
+    }
+    const float x_edge = edges ? to_f32(base[edge]) : -INFINITY;
+    auto put = [&](int j) {
+      const int vi = r.fa + j * 32 + lane;
+      if (vi >= r.fb) return;
+      if (same) {
+        __stcs(reinterpret_cast<Raw*>(to) + vi, v[j].raw);
+      } else {
+        const T* e = reinterpret_cast<const T*>(&v[j].raw);
+#pragma unroll
+        for (int q = 0; q < N; ++q) to[vi * N + q] = e[q];
+      }
+    };
+    const RowInputs inputs = row_inputs<OP>(a, row);
+    const int tgt = read_target(a.targets, a.target_bytes, a.has_ignore, a.ignore, row, a.V);
+    if (tgt < 0) {   // the same in every lane
+      const float value = tgt == -2 ? NAN : 0.0f;
+      if (lane == 0) write_left_out<OP>(a, row, value, mine);
+      if (g != nullptr) {
+        float f[N];
+#pragma unroll
+        for (int q = 0; q < N; ++q) f[q] = value;
+#pragma unroll
+        for (int j = 0; j < kUnroll; ++j) { v[j].from_float(f); put(j); }
+        if (edges) to[edge] = from_f32<T>(value);
+      }
+      continue;
+    }
+    // the target: lane, vector and element, or an edge
+    const int te = r.lo + tgt, tv = te / N - r.fa, tq = te % N;
+    const bool own = te / N >= r.fa && te / N < r.fb && (tv & 31) == lane, at_edge = edges && edge == te;
+    float xt = at_edge ? x_edge : 0.0f;
+    if (own) {
+#pragma unroll
+      for (int j = 0; j < kUnroll; ++j)
+        if (j == tv >> 5) {   // out of the sum
+          float f[N];
+          v[j].to_float(f);
+#pragma unroll
+          for (int q = 0; q < N; ++q)
+            if (q == tq) { xt = f[q]; f[q] = -INFINITY; }
+          v[j].from_float(f);
+        }
+    }
+    xt = __shfl_sync(0xffffffffu, xt, __ffs(__ballot_sync(0xffffffffu, own || at_edge)) - 1);
+    const float xe = at_edge ? -INFINITY : x_edge;
+    float m = fmaxf(max_of(v), xe);
+    m = warp_max(m);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    const float2 neg = make_float2(-ref, -ref), kk = make_float2(a.k, a.k);
+    float2 s2 = make_float2(edges ? ex2((xe - ref) * a.k) : 0.0f, 0.0f);
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+      float f[N];
+      v[j].to_float(f);
+#pragma unroll
+      for (int q = 0; q < N; q += 2) {
+        const float2 d = __fmul2_rn(__fadd2_rn(make_float2(f[q], f[q + 1]), neg), kk);
+        s2 = __fadd2_rn(s2, make_float2(ex2(d.x), ex2(d.y)));
+      }
+    }
+    const float s = warp_sum(s2.x + s2.y);
+    const TargetStats t = target_stats(m, s, xt, a.k);
+    const RowResult res = finish_target_row<OP>(a, inputs, t);
+    if (lane == 0) write_target_row<OP>(a, row, t, res, mine);
+    if (g == nullptr) continue;
+    const float top = t.top == -INFINITY ? 0.0f : t.top, scale = -res.c / t.sum, at_target = res.c * t.rest;   // an element's gradient is scale 2^((x - top) k)
+    const float2 neg_top = make_float2(-top, -top), ss = make_float2(scale, scale);
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+      float f[N];
+      v[j].to_float(f);
+#pragma unroll
+      for (int q = 0; q < N; q += 2) {
+        const float2 d = __fmul2_rn(__fadd2_rn(make_float2(f[q], f[q + 1]), neg_top), kk);
+        const float2 e = __fmul2_rn(make_float2(ex2(d.x), ex2(d.y)), ss);
+        f[q] = e.x; f[q + 1] = e.y;
+      }
+      v[j].from_float(f);
+      put(j);
+    }
+    if (own) to[te] = from_f32<T>(at_target);   // behind the vector
+    if (edges) to[edge] = from_f32<T>(at_edge ? at_target : scale * ex2((x_edge - top) * a.k));
+  }
+  if (plan.sums != nullptr) {
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int t = 0; t < plan.n_sums; ++t) {
+        double total = 0.0;
+        for (int w = 0; w < kRows; ++w) total += sums[w][t];
+        plan.partials[3 * blockIdx.x + t] = total;
+      }
+      __threadfence();
+      last = atomicAdd(plan.done, 1) == static_cast<int>(gridDim.x) - 1;
+    }
+    __syncthreads();
+    if (last) {
+      __threadfence();
+      block_sums(plan.partials, gridDim.x, 3, 1, plan.n_sums, plan.sums, sums[0]);
+    }
+  }
+}
+
+template <typename T, int OP>
+int launch_short(const RowArgs& a, const RowPlan& plan, DeviceState* ds, cudaStream_t st, bool* taken) {
+  constexpr int N = Vec16<T>::N, kRows = kThreads / 32;
+  *taken = a.V / N + 1 <= 32 * kUnroll;
+  if (!*taken) return MCB_OK;
+  const int64_t blocks = (a.M + kRows - 1) / kRows, most = kShortBlocks * static_cast<int64_t>(ds->sm_count);
+  const dim3 grid(static_cast<unsigned>(blocks < most ? blocks : most < kMaxPartials ? most : kMaxPartials));
+  MCB_CHECK_CUDA(launch_kernel(token_short_kernel<T, OP>, grid, dim3(kThreads), 0, st, chained_launch(), a, plan));
+  MCB_CHECK_LAUNCH("token_short");
+  return MCB_OK;
+}
+
+template <typename T, int OP>
+int launch_stats(const RowArgs& a, DeviceState* ds, cudaStream_t st) {
   constexpr int N = Vec16<T>::N;
   const int64_t vecs = a.V / N + 1;
   int threads = static_cast<int>((vecs + kUnroll - 1) / kUnroll + 31) / 32 * 32;
@@ -288,7 +414,7 @@ int launch_stats(const RowArgs& a, const RowPlan& plan, DeviceState* ds, cudaStr
   if (a.M << log_ctas > 0x7fffffff) return fail(MCB_ERR_SHAPE, "token_stats: too many rows");
   if (threads == 32) {
     MCB_CHECK_CUDA(launch_kernel(token_stats_kernel<T, OP, true>, dim3(static_cast<unsigned>((a.M + kThreads / 32 - 1) / (kThreads / 32))), dim3(kThreads),
-                                 0, st, chained_launch(), a, plan, 0));
+                                 0, st, chained_launch(), a, 0));
     MCB_CHECK_LAUNCH("token_stats");
     return MCB_OK;
   }
@@ -300,7 +426,7 @@ int launch_stats(const RowArgs& a, const RowPlan& plan, DeviceState* ds, cudaStr
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr; cfg.numAttrs = chained_launch() ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, token_stats_kernel<T, OP, false>, a, plan, log_ctas);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, token_stats_kernel<T, OP, false>, a, log_ctas);
   if (e != cudaSuccess) return cuda_fail(e, "token_stats_kernel launch");
   MCB_CHECK_LAUNCH("token_stats");
   return MCB_OK;
@@ -328,10 +454,15 @@ int launch_stream(const GradArgs& ga, DeviceState* ds, cudaStream_t st, bool* ta
 }  // namespace
 
 namespace tokenloss {
-int launch_stats_rows(int op, const RowArgs& a, const RowPlan& plan, int dtype, DeviceState* ds, cudaStream_t st) {
+int launch_stats_rows(int op, const RowArgs& a, int dtype, DeviceState* ds, cudaStream_t st) {
   const bool f32 = dtype == MCB_F32;
-  if (op == kPolicy) return f32 ? launch_stats<float, kPolicy>(a, plan, ds, st) : launch_stats<__nv_bfloat16, kPolicy>(a, plan, ds, st);
-  return f32 ? launch_stats<float, kStats>(a, plan, ds, st) : launch_stats<__nv_bfloat16, kStats>(a, plan, ds, st);
+  if (op == kPolicy) return f32 ? launch_stats<float, kPolicy>(a, ds, st) : launch_stats<__nv_bfloat16, kPolicy>(a, ds, st);
+  return f32 ? launch_stats<float, kStats>(a, ds, st) : launch_stats<__nv_bfloat16, kStats>(a, ds, st);
+}
+int launch_short_rows(int op, const RowArgs& a, const RowPlan& plan, int dtype, DeviceState* ds, cudaStream_t st, bool* taken) {
+  const bool f32 = dtype == MCB_F32;
+  if (op == kUnit) return f32 ? launch_short<float, kUnit>(a, plan, ds, st, taken) : launch_short<__nv_bfloat16, kUnit>(a, plan, ds, st, taken);
+  return f32 ? launch_short<float, kPolicy>(a, plan, ds, st, taken) : launch_short<__nv_bfloat16, kPolicy>(a, plan, ds, st, taken);
 }
 int launch_grad_stream(const GradArgs& ga, int dtype, DeviceState* ds, cudaStream_t st, bool* taken) {
   return dtype == MCB_F32 ? launch_stream<float>(ga, ds, st, taken) : launch_stream<__nv_bfloat16>(ga, ds, st, taken);

@@ -492,6 +492,45 @@ def test_gradients_in_place(cuda_device):
             check_grad(unit, wg, 2 * spread)
 
 
+@pytest.mark.parametrize("B,S", [(1, 1), (3, 700), (5, 1000), (1, 9001), (9001, 1), (3000, 3), (40, 2500), (1, 70001), (23, 3100)])
+@pytest.mark.parametrize("keep", [0.0, 0.6, 1.0])
+def test_weights_of_the_mean(cuda_device, B, S, keep):
+    """By one block and by a cluster, targets kept in registers and read again, sequences counted in shared memory and one by one; and the
+    loss over the same rows, which takes them in the order the kernel finds."""
+    import ctypes as C
+
+    lib, V, M = _lib.load(), 16, B * S
+    g = torch.Generator(device=cuda_device).manual_seed(B + S)
+    t = torch.randint(0, V, (B, S), device=cuda_device, generator=g)
+    kept = torch.rand(B, S, device=cuda_device, generator=g) < keep
+    if B > 2:
+        kept[1] = False
+    t = torch.where(kept, t, torch.full_like(t, -1)).to(torch.int32)
+    for seq_mean in (0, 1):
+        w = torch.full((B, S), math.nan, device=cuda_device)
+        _lib.check(lib.mcb_loss_weights(C.byref(_lib.TokenTargets(t.data_ptr(), 4, 0, 0)), None, w.data_ptr(), B, S, V, seq_mean,
+                                        torch.cuda.current_stream().cuda_stream))
+        n = kept.sum(1, keepdim=True)
+        want = kept.double() / (n.clamp_min(1) * (n > 0).sum().clamp_min(1) if seq_mean else kept.sum().clamp_min(1))
+        assert ((w.double() - want).abs() <= 3 * 2.0 ** -24 * want).all()   # two divisions and their product
+        m8 = kept.to(torch.uint8)
+        w2 = torch.full_like(w, math.nan)
+        _lib.check(lib.mcb_loss_weights(None, m8.data_ptr(), w2.data_ptr(), B, S, V, seq_mean, torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(w, w2)
+        x = torch.randn(B, S, V, device=cuda_device, generator=g)
+        out = F.policy_loss(x, t, torch.ones(B, S, device=cuda_device), sequence_mean=bool(seq_mean), return_grad=True)
+        assert abs(float(out.loss) + float(want.sum())) <= 1e-5
+        logp = torch.log_softmax(x.double(), -1).gather(-1, t.long().clamp_min(0)[..., None])[..., 0]
+        check_logp(out.log_probs, torch.where(kept, logp, torch.zeros_like(logp)))
+        wg, spread = grad64(torch.softmax(x.double(), -1), t, kept, -want)
+        check_grad(out.grad, wg, 2 * spread)
+        dist, grad = F.distillation_loss(x, t.clamp_min(0)[..., None], torch.zeros(B, S, 1, device=cuda_device), mask=kept, return_grad=True)
+        share = kept.double() / kept.sum().clamp_min(1)
+        assert abs(float(dist) + float((share * logp).sum())) <= 1e-4
+        wg, spread = grad64(torch.softmax(x.double(), -1), t, kept, -share)
+        check_grad(grad, wg, 4 * spread + share[..., None] * torch.softmax(x.double(), -1))
+
+
 @both
 @pytest.mark.parametrize("V", [300, 2049, 32000, 151936])
 def test_rows_of_a_chunk(cuda_device, dtype, V):

@@ -134,6 +134,8 @@ def test_c_arguments_refused():
     lib = _lib.load()
     r, t = C.byref(rows()), C.byref(targets())
     ws = 1 << 40
+    one = C.byref(_lib.PolicyTerms(16, 1, None, None, 0.2, 0.2, 0.0, 0))
+    assert lib.mcb_policy_loss(r, t, one, 0, 16, 16, None, 24, ws, None) == ALIGN
     assert lib.mcb_token_logprob_fwd(None, t, 16, 16, None, None) == NULL
     assert lib.mcb_token_logprob_fwd(r, None, 16, 16, None, None) == NULL
     assert lib.mcb_token_logprob_fwd(r, C.byref(targets(targets=0)), 16, 16, None, None) == NULL
