@@ -684,7 +684,7 @@ class Qwen:
         run["dnf"] = self._head_by_chunks(run["nf"], rows)
         out = self._sum_terms(parts, 3)
         self._backward_saved(run, accumulate)
-        return PolicyLoss(out[0:1], logp.view(B, S), out[1:2], out[2:3], None), self._grad_views
+        return PolicyLoss(out, logp.view(B, S), None), self._grad_views
 
     def distillation_forward_backward(self, input_ids: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
                                       mask: Optional[torch.Tensor] = None, temperature: float = 1.0, accumulate: bool = False):

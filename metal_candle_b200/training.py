@@ -517,12 +517,34 @@ class PreferenceLoss(NamedTuple):
     grad: Optional[torch.Tensor]        # d loss / d logits
 
 
-class PolicyLoss(NamedTuple):
-    loss: torch.Tensor                  # [1] float32
-    log_probs: torch.Tensor             # [batch, seq] float32
-    kl: torch.Tensor                    # [1] float32: mean of exp(ref - logp) - (ref - logp) - 1; 0 without a reference
-    clip_fraction: torch.Tensor         # [1] float32: share of the tokens whose ratio the clipping bounds
-    grad: Optional[torch.Tensor]
+class PolicyLoss:
+    """What `policy_loss` returns; a sequence of (loss, log_probs, kl, clip_fraction, grad)."""
+    __slots__ = ("_sums", "loss", "log_probs", "grad")
+
+    def __init__(self, sums: torch.Tensor, log_probs: torch.Tensor, grad: Optional[torch.Tensor]):
+        self._sums = sums
+        self.loss = sums[:1]            # [1] float32
+        self.log_probs = log_probs      # [batch, seq] float32
+        self.grad = grad                # d loss / d logits, or None
+
+    @property
+    def kl(self) -> torch.Tensor:
+        """[1] float32: mean of exp(ref - logp) - (ref - logp) - 1; 0 without a reference."""
+        return self._sums[1:2]
+
+    @property
+    def clip_fraction(self) -> torch.Tensor:
+        """[1] float32: share of the tokens whose ratio the clipping bounds."""
+        return self._sums[2:3]
+
+    def __iter__(self):
+        return iter((self.loss, self.log_probs, self.kl, self.clip_fraction, self.grad))
+
+    def __getitem__(self, i):
+        return tuple(self)[i]
+
+    def __len__(self):
+        return 5
 
 
 def _elsewhere(t: torch.Tensor) -> bool:
@@ -583,10 +605,11 @@ def token_log_probs(logits: torch.Tensor, targets: torch.Tensor, ignore_index: O
     if _elsewhere(x):
         with torch.cuda.device(x.device):
             return token_log_probs(x, t, ignore_index, temperature)
-    out = torch.empty(2, B, S, dtype=torch.float32, device=x.device)
-    to = out.data_ptr()
-    _lib.check(backend._lib_for(x).mcb_token_logprob_fwd(rows, _token_targets(t, ignore_index), to, to + 4 * B * S, None, backend._stream()))
-    return out.unbind()
+    logp = torch.empty(B, S, dtype=torch.float32, device=x.device)
+    lse = torch.empty_like(logp)
+    _lib.check(backend._lib_for(x).mcb_token_logprob_fwd(rows, _token_targets(t, ignore_index), logp.data_ptr(), lse.data_ptr(), None,
+                                                         backend._stream()))
+    return logp, lse
 
 
 def token_log_probs_backward(logits: torch.Tensor, targets: torch.Tensor, log_probs: torch.Tensor, lse: torch.Tensor, dlogp: torch.Tensor,
@@ -632,13 +655,13 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, ref_log_probs: 
             return preference_loss(x, t, ref, beta, label_smoothing, average_log_probs, ignore_index, return_grad)
     lib = backend._lib_for(x)
     grad = _new_grad(x, return_grad)
-    out = torch.empty(B + 1, dtype=torch.float32, device=x.device)
+    loss = torch.empty(1, dtype=torch.float32, device=x.device)
+    seq_logp = torch.empty_like(ref)
     ws = backend.workspace(x.device, lib.mcb_token_loss_workspace_bytes(B, S))
-    to = out.data_ptr()
     _lib.check(lib.mcb_preference_loss(_token_logits(x, 1.0), _token_targets(t, ignore_index), ref.data_ptr(), float(beta), float(label_smoothing),
-                                       int(bool(average_log_probs)), to + 4, to, backend._ptr(grad), ws.data_ptr(), ws.numel(),
-                                       backend._stream()))
-    return PreferenceLoss(*out.split((1, B)), grad)
+                                       int(bool(average_log_probs)), seq_logp.data_ptr(), loss.data_ptr(), backend._ptr(grad), ws.data_ptr(),
+                                       ws.numel(), backend._stream()))
+    return PreferenceLoss(loss, seq_logp, grad)
 
 
 def _policy_terms(x, shape, advantages, old_log_probs, ref_log_probs, clip_low, clip_high, kl_coef):
@@ -683,8 +706,7 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, advantages: torch.T
     ws = backend.workspace(x.device, lib.mcb_token_loss_workspace_bytes(B, S))
     _lib.check(lib.mcb_policy_loss(rows, _token_targets(t, ignore_index), terms, int(bool(sequence_mean)), logp.data_ptr(), out.data_ptr(),
                                    backend._ptr(grad), ws.data_ptr(), ws.numel(), backend._stream()))
-    loss, kl, clipped = out.split(1)
-    return PolicyLoss(loss, logp, kl, clipped, grad)
+    return PolicyLoss(out, logp, grad)
 
 
 def _teacher_top(x, shape, teacher_ids, teacher_logits, mask):
