@@ -362,9 +362,15 @@ preference_kernel(const float* logp, const void* targets, int target_bytes, int 
   auto sequence = [&](int64_t b, double& total, float& per) {
     double acc = 0.0;
     int c = 0;
-    for (int64_t i = lane; i < S; i += 32) {
-      acc += static_cast<double>(logp[b * S + i]);
-      if (average) c += read_target(targets, target_bytes, has_ignore, ignore, b * S + i, V) != -1;
+    for (int64_t i = lane; i < S; i += 8 * 32) {   // eight loads in flight
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = i + 32 * j < S ? logp[b * S + i + 32 * j] : 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        acc += static_cast<double>(v[j]);
+        if (average && i + 32 * j < S) c += read_target(targets, target_bytes, has_ignore, ignore, b * S + i + 32 * j, V) != -1;
+      }
     }
     for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
     c = __reduce_add_sync(0xffffffffu, c);

@@ -141,8 +141,10 @@ __device__ __forceinline__ PolicyTerm policy_term(const RowArgs& a, const RowInp
     const float d = in.ref_logp - logp;
     const float e = expm1f(d);
     t.kl = e - d;
-    t.loss += a.kl_coef * t.kl;
-    t.dlogp -= a.kl_coef * e;
+    if (a.kl_coef > 0.0f) {   // (0 times an infinite divergence is not a loss)
+      t.loss += a.kl_coef * t.kl;
+      t.dlogp -= a.kl_coef * e;
+    }
   }
   return t;
 }

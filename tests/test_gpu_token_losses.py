@@ -62,7 +62,7 @@ def check_grad(got, want, spread, scale=5e-5):
 
 
 SHAPES = [(1, 1, 1), (2, 3, 2), (1, 1, 17), (2, 5, 50), (2, 7, 1000), (4, 33, 2050), (2, 3, 8193), (2, 4, 32000), (2, 3, 50257), (2, 2, 151936),
-          (2, 1, 420001)]
+          (2, 1, 420001), (2, 2, 700001)]   # the last: longer than the one-pass kernel's rows
 both = pytest.mark.parametrize("dtype", [F32, BF])
 shapes = pytest.mark.parametrize("B,S,V", SHAPES)
 
@@ -194,7 +194,8 @@ def distill64(x, ids, tl, mask, T):
 
 @both
 @pytest.mark.parametrize("B,S,V,K", [(1, 1, 1, 1), (2, 3, 2, 2), (1, 2, 17, 5), (2, 5, 50, 50), (2, 7, 1000, 64), (3, 11, 2050, 33), (2, 3, 8193, 257),
-                                     (2, 4, 32000, 1024), (2, 3, 50257, 101), (2, 2, 151936, 64), (1, 2, 420001, 8)])
+                                     (2, 4, 32000, 1024), (2, 3, 50257, 101), (2, 2, 151936, 64), (1, 2, 420001, 8),
+                                     (2, 2, 700001, 40)])
 @pytest.mark.parametrize("T,tdtype,masked", [(1.0, None, False), (2.0, F32, True), (0.5, BF, True)])
 def test_distillation_loss(cuda_device, dtype, B, S, V, K, T, tdtype, masked):
     x, t, g = make(cuda_device, B, S, V, dtype, 5)
@@ -420,6 +421,63 @@ def test_streams_graphs_and_repeated_calls(cuda_device, dtype, B, S, V):
         torch.cuda.synchronize()
         assert all(same(o, ref) for o, ref in zip(outs, want))
     assert _lib.device_status() == 0
+
+
+def test_infinite_divergence_that_is_only_reported(cuda_device):
+    """kl_coef = 0: a reference that is infinitely far away is seen in `kl` and nowhere else."""
+    x, t, g = make(cuda_device, 2, 3, 100, F32, 16, keep=1.0)
+    A, ref = torch.ones(2, device=cuda_device), torch.zeros(2, 3, device=cuda_device)
+    ref[0, 1] = 500.0
+    far = F.policy_loss(x, t, A, None, ref, return_grad=True)
+    near = F.policy_loss(x, t, A, None, None, return_grad=True)
+    assert far.kl == math.inf and torch.equal(far.loss, near.loss) and torch.equal(far.grad, near.grad)
+
+
+def test_long_sequences_of_pairs(cuda_device):
+    """Sums of many tokens: 9001 log-probabilities a sequence, each good to 2e-5 + 1e-6 |logp| (three logits each, so below 12)."""
+    x, t, g = make(cuda_device, 2, 9001, 3, F32, 17, keep=0.9)
+    logp, _, _, kept = rows64(x, t)
+    for average in (False, True):
+        n = kept.sum(1) if average else torch.ones(2, device=cuda_device)
+        out = F.preference_loss(x, t, (logp.sum(1) / n).float(), average_log_probs=average, ignore_index=IGN)
+        assert ((out.log_probs.double() - logp.sum(1) / n).abs() <= (9001 * 3.2e-5 + 1e-6 * logp.sum(1).abs()) / n).all()
+
+
+def test_first_calls_are_captured(cuda_device):
+    """In a process of its own: nothing that a first call sets up is forbidden under capture."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import torch
+from metal_candle_b200 import _lib
+from metal_candle_b200 import training as F
+_lib.init(0)
+dev = torch.device("cuda", 0)
+cases = []
+for V in (500, 40000, 151936):
+    for dt in (torch.bfloat16, torch.float32):
+        x = torch.randn(2, 6, V, device=dev).to(dt)
+        t = torch.randint(0, V, (2, 6), device=dev)
+        cases.append((x, t, torch.randn(2, device=dev), torch.rand(2, 6, 4, device=dev).argsort(-1), torch.randn(2, 6, 4, device=dev)))
+def run(x, t, a, ids, tl):
+    logp, lse = F.token_log_probs(x, t)
+    return [logp, F.token_log_probs_backward(x, t, logp, lse, logp), *F.policy_loss(x, t, a, return_grad=True),
+            *F.preference_loss(x, t, a, return_grad=True), *F.distillation_loss(x, ids, tl, return_grad=True)]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    captured = [run(*c) for c in cases]
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(u, v) for c, out in zip(cases, captured) for u, v in zip(run(*c), out))
+assert _lib.device_status() == 0
+print("captured")
+"""
+    root = Path(__file__).resolve().parent.parent
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=root)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
 
 
 def test_gradients_against_differences(cuda_device):
