@@ -494,7 +494,8 @@ typedef struct {
   int32_t pad_;
 } mcb_policy_terms;
 /* A teacher's `top` (1 to 1024) largest logits of each row and their vocabulary ids, [batch * seq, top].  An entry whose logit is
- * -inf counts for nothing, whatever its id; another id outside [0, vocab) makes the row NaN; an id that comes twice has the sum. */
+ * -inf, or so low that its probability is 0 in 32 bits, counts for nothing, whatever its id; another id outside [0, vocab)
+ * makes the row NaN; an id that comes twice has the sum. */
 typedef struct {
   const void* ids;      /* int32 or int64 (id_bytes 4 or 8) */
   const void* logits;   /* MCB_F32 or MCB_BF16, by dtype */

@@ -9,10 +9,15 @@
 // keeps its share in tensor memory, 256 KB an SM that nothing else here uses: a thread writes and reads its own lane, up to 4 chunks
 // of 32 columns, and a fifth chunk stays in registers.
 //
-// Between a row's two sweeps lie the exchange over the cluster and the row's own scalar arithmetic, some 6000 cycles, as long as the
-// row's share of the SM's memory time takes twice; so an SM works on four rows at once, each with its own four warps (a GROUP; one
-// warp for short rows, up to sixteen for few or long ones), ring of shared-memory pieces that bulk copies fill ahead, and barriers.
-// With the exponentials in registers alone an SM holds two rows: 4096 rows of 151936 took 784 us instead of XXX.
+// Between a row's two sweeps lie the exchange over the cluster and the row's own scalar arithmetic.  So a row takes as few CTAs and
+// then as few warps as hold it: an exchange less is worth more than rows in flight.  The warps of one row are a GROUP (one to sixteen;
+// more of them, and clusters, where there are few rows), with its own ring of shared-memory pieces that bulk copies fill ahead of it,
+// across the end of a row, and its own barriers; short rows have several groups on an SM.  Four further warps feed the rings and work
+// out the teacher's part of a distillation row ahead of it.
+// 4096 rows of 151936 bf16, all kept: 784 us with the exponentials in registers alone (a row over four CTAs, two rows in flight), 661
+// in tensor memory over eight CTAs with four rows in flight, 493 as here (5.05 TB/s).  Of a row's 17 thousand cycles, where its bytes
+// ask HBM for 13.6: first sweep 8.2, joining the group 1.1, the cluster 0.5 to 1, the row's arithmetic and gradient scale 1.8, second
+// sweep 4.9; the ring's copies run under all of it, the stores under the second sweep alone.
 // One CTA takes a whole SM (its ring excludes other kernels' shared memory), so that tensor memory is its alone and taking it never
 // waits: a cluster that held some of it while it waited for more could wait for a kernel that waits for the cluster.
 //
@@ -363,10 +368,10 @@ token_resident_kernel(const RowArgs a, const Resident p) {
           moved = true;
         }
         if (__any_sync(0xffffffffu, moved)) { idle = 0; continue; }
-        if (*abort_flag != 0) break;
         const long long now = clock64();
         if (idle == 0) idle = now;
-        else if (now - idle > kWaitLimitCycles) { *abort_flag = 55; atomicCAS(p.status, 0, 55); break; }
+        else if (now - idle > kWaitLimitCycles) { *abort_flag = 55; atomicCAS(p.status, 0, 55); }
+        if (__any_sync(0xffffffffu, *abort_flag != 0)) break;   // (all lanes or none)
       }
       __syncwarp();
     } else if (taught_ahead && warp - kWarps - 1 < groups) {
@@ -376,7 +381,7 @@ token_resident_kernel(const RowArgs a, const Resident p) {
       for (uint32_t i = ((blockIdx.x >> p.log_ctas) << p.log_groups) + g; i < kept; i += step) {
         const int row = row_of(i);
         if (state_of(i, row) != 0) continue;
-        if (!mbar_wait(smem_u32(&t_empty[g][into]), parity, abort_flag, 57, p.status)) break;
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&t_empty[g][into]), parity, abort_flag, 57, p.status))) break;
         teach(g, row, share_of<N>(a, p, rank, row), into);
         if (lane == 0) mbar_arrive(smem_u32(&t_full[g][into]));
         if (++into == 2) { into = 0; parity ^= 1; }
@@ -722,7 +727,7 @@ token_resident_kernel(const RowArgs a, const Resident p) {
         const bool twice = repeats[group][par] != 0;
         for (int q = tid; q < a.K; q += gd) {
           const int el = ids[q];
-          if (el < 0) continue;
+          if (el < s.lo || el >= s.hi) continue;   // -1; or what an abandoned wait left there
           float prob = probs[q];
           bool mine = true;
           if (twice) {   // the first of those that name the same column writes the sum of them
@@ -739,8 +744,10 @@ token_resident_kernel(const RowArgs a, const Resident p) {
     }
     if constexpr (OP == kDistill) {   // (this parity's entries are made again behind the next row's first barrier)
       if (p.group_warps == 1) __syncwarp();
-      for (int q = tid; q < a.K; q += gd)
-        if (t_id[par * a.K + q] >= 0) t_bits[par * bit_words + (t_id[par * a.K + q] >> 5)] = 0;
+      for (int q = tid; q < a.K; q += gd) {
+        const int el = t_id[par * a.K + q];
+        if (el >= info.share.lo && el < info.share.hi) t_bits[par * bit_words + (el >> 5)] = 0;
+      }
       __syncwarp();
       if (taught_ahead && lane == 0) mbar_arrive(smem_u32(&t_empty[group][par]));
     }
@@ -771,7 +778,6 @@ token_resident_kernel(const RowArgs a, const Resident p) {
   }
 }
 
-// Clusters of a launch that the device runs at once, kept for each cluster size (the query takes microseconds).
 template <typename T, int OP>
 int launch_resident(const RowArgs& a, const RowPlan& plan, DeviceState* ds, cudaStream_t st, bool* taken) {
   constexpr int N = Vec16<T>::N, CV = kChunk / N;
@@ -826,7 +832,7 @@ int launch_resident(const RowArgs& a, const RowPlan& plan, DeviceState* ds, cuda
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr; cfg.numAttrs = 1;
-  int resident = 0;
+  int resident = 0;   // clusters that the device runs at once, asked for once a cluster size (the query takes microseconds)
   {
     struct Known { const DeviceState* ds; int clusters[4]; };
     static std::mutex mu;

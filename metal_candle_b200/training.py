@@ -724,9 +724,9 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
                       temperature: float = 1.0, return_grad: bool = False):
     """Distillation from a teacher's largest logits: mean over kept positions of temperature^2 KL(q || softmax(logits / temperature)) with
     q = softmax(teacher_logits / temperature) over the teacher's 1 to 1024 entries of that position.  teacher_ids, teacher_logits:
-    [batch, seq, entries]; an entry of -inf counts for nothing, whatever its id (a position of nothing else adds 0 to the
-    mean); an id that comes twice has the sum of its probabilities.  mask [batch, seq]: 0 leaves a position out.  Returns a
-    1-element float32 tensor; with return_grad also d loss / d logits."""
+    [batch, seq, entries]; an entry of -inf, or of a probability that is 0 in 32 bits, counts for nothing, whatever its id (a
+    position of nothing else adds 0 to the mean); an id that comes twice has the sum of its probabilities.  mask [batch, seq]: 0
+    leaves a position out.  Returns a 1-element float32 tensor; with return_grad also d loss / d logits."""
     x = _check_logits(logits)
     B, S, _ = x.shape
     held, teacher = _teacher_top(x, (B, S), teacher_ids, teacher_logits, mask)
