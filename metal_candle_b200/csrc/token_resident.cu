@@ -41,10 +41,9 @@ using namespace umma;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;   // that take rows
 constexpr int kAllThreads = kThreads + 128;              // and four warps that serve them
-// Registers: 640 threads are launched with 96 each, 61440; the row warps take 112, the serving ones keep 32 (512 x 112 + 128 x 32 = 61440),
-// or 104 and 64 where these work out the teacher's part.
-template <int OP> constexpr int kRowRegs = OP == kDistill ? 104 : 112;
-template <int OP> constexpr int kServeRegs = OP == kDistill ? 64 : 32;
+// Registers: 640 threads are launched with 96 each, 61440; the row warps take 112, the serving ones keep 32 (512 x 112 + 128 x 32 = 61440).
+// (Distillation with 104 and 64, so that the teacher's part spills nothing: 3 % slower.)
+constexpr int kRowRegs = 112, kServeRegs = 32;
 constexpr int kChunk = 32;             // elements a thread takes at a time
 constexpr int kTmemChunks = 4;         // chunks it keeps in tensor memory, beside one in registers
 constexpr int kMaxChunks = kTmemChunks + 1;
@@ -224,10 +223,16 @@ token_resident_kernel(const RowArgs a, const Resident p) {
   uint8_t* ring = smem + kInfoRows * sizeof(RowInfo) + group * p.pieces * piece_bytes;
   const int bit_words = kMaxChunks * kChunk * gd / 32;
   uint8_t* teacher_smem = smem + kInfoRows * sizeof(RowInfo) + groups * p.pieces * piece_bytes;
-  int* t_id = reinterpret_cast<int*>(teacher_smem + group * (24 * a.K + 8 * bit_words));
-  float* t_q = reinterpret_cast<float*>(t_id + 2 * a.K);
-  float* t_x = t_q + 2 * a.K;
-  uint32_t* t_bits = reinterpret_cast<uint32_t*>(t_x + 2 * a.K);
+  struct Taught { int* id; float *q, *x; uint32_t* bits; };   // entries: column in the share or -1, probability, student's logit; ids seen
+  auto taught = [&](int g, int parity) {
+    uint8_t* at = teacher_smem + g * (24 * a.K + 8 * bit_words);
+    Taught t;
+    t.id = reinterpret_cast<int*>(at) + parity * a.K;
+    t.q = reinterpret_cast<float*>(at + 8 * a.K) + parity * a.K;
+    t.x = reinterpret_cast<float*>(at + 16 * a.K) + parity * a.K;
+    t.bits = reinterpret_cast<uint32_t*>(at + 24 * a.K) + parity * bit_words;
+    return t;
+  };
   const uint32_t full0 = smem_u32(full[group]), empty0 = smem_u32(empty[group]);
   auto group_sync = [&]() {
     if (p.group_warps == 1) __syncwarp();
@@ -243,7 +248,7 @@ token_resident_kernel(const RowArgs a, const Resident p) {
     fence_proxy_async_smem();
   }
   if constexpr (OP == kDistill)
-    for (int i = tid; i < 2 * bit_words && !serves; i += gd) t_bits[i] = 0;
+    for (int i = tid; i < 2 * bit_words && !serves; i += gd) taught(group, 0).bits[i] = 0;
   if (ctas > 1) cl.sync(); else __syncthreads();   // every CTA's barriers exist before a peer arrives on them
   grid_dependency_wait();
   if (p.tmem) {
@@ -264,7 +269,7 @@ token_resident_kernel(const RowArgs a, const Resident p) {
   auto row_of = [&](uint32_t i) -> int { return p.order != nullptr ? from_here(p.order)[i] : static_cast<int>(i); };
   auto state_of = [&](uint32_t i, int row) {   // 0: to be computed, 1: left out, 2: out of range
     if (i >= kept) return 1;
-    if (OP == kDistill) return a.weight[row] == 0.0f ? 1 : 0;
+    if (OP == kDistill) return p.order == nullptr && a.weight[row] == 0.0f ? 1 : 0;
     const int t = read_target(a.targets, a.target_bytes, a.has_ignore, a.ignore, row, a.V);
     return t >= 0 ? 0 : t == -2 ? 2 : 1;
   };
@@ -276,62 +281,85 @@ token_resident_kernel(const RowArgs a, const Resident p) {
   auto teach = [&](int g, int row, const Share& s, int into) {
     const int64_t t0 = static_cast<int64_t>(row) * a.K;
     const T* x_row = static_cast<const T*>(a.logits) + row_offset(a, row);
-    int* ids = reinterpret_cast<int*>(teacher_smem + g * (24 * a.K + 8 * bit_words)) + into * a.K;
-    float* probs = reinterpret_cast<float*>(ids + 2 * a.K);
-    float* logits = probs + 2 * a.K;
-    uint32_t* bits = reinterpret_cast<uint32_t*>(logits + (2 - into) * a.K) + into * bit_words;
+    const Taught at = taught(g, into);
     auto id_of = [&](int64_t id) { return id >= 0 && id < a.V ? static_cast<int>(id) : -1; };
     float tm = -INFINITY, ts = 0.0f;
-    for (int q = lane; q < a.K; q += 32) {
+#pragma unroll 2
+    for (int q = lane; q < a.K; q += 32) {   // (loads of the student's logits that another CTA has are the same ones it makes)
       const float t = read_teacher(a, t0 + q);
-      ids[q] = id_of(read_teacher_id(a, t0 + q));
-      probs[q] = t;
+      const int id = id_of(read_teacher_id(a, t0 + q));
+      at.x[q] = id >= 0 ? to_f32(x_row[id]) : 0.0f;
+      at.id[q] = id;
+      at.q[q] = t;
       tm = fmaxf(tm, t);
     }
     tm = warp_max(tm);
     const float tref = tm == -INFINITY ? 0.0f : tm;
-    int best = -1;
+    float x_ref = 0.0f;
+    bool best = false;
     for (int q = lane; q < a.K; q += 32) {
-      const float t = probs[q];
+      const float t = at.q[q];
       ts += ex2((t - tref) * a.k);
-      if (t == tm && best < 0) best = ids[q];
+      if (t == tm && !best && at.id[q] >= 0) { best = true; x_ref = at.x[q]; }
     }
     ts = warp_sum(ts);
-    const uint32_t who = __ballot_sync(0xffffffffu, best >= 0);
-    best = __shfl_sync(0xffffffffu, best, who == 0 ? 0 : __ffs(who) - 1);
-    float x_ref = best >= 0 ? to_f32(x_row[best]) : 0.0f;
+    const uint32_t who = __ballot_sync(0xffffffffu, best);
+    x_ref = __shfl_sync(0xffffffffu, x_ref, who == 0 ? 0 : __ffs(who) - 1);
     if (!(fabsf(x_ref) < INFINITY)) x_ref = 0.0f;
     const float inv_ts = ts == 0.0f ? 0.0f : 1.0f / ts, log_ts = logf(ts);
     float loss = 0.0f;
     bool twice = false;
     for (int q = lane; q < a.K; q += 32) {
-      const float d = probs[q] - tref, prob = ex2(d * a.k) * inv_ts;   // log q = d / T - log_ts
-      const int id = ids[q];
+      const float d = at.q[q] - tref, prob = ex2(d * a.k) * inv_ts;   // log q = d / T - log_ts
+      const int id = at.id[q];
       int el = -1;
       if (prob != 0.0f) {   // (NaN counts)
         if (id < 0) {
           loss = NAN;
         } else if (id - s.column >= s.lo && id - s.column < s.hi) {
           el = id - s.column;
-          const float x = to_f32(x_row[id]);
-          logits[q] = x;
-          loss += prob * ((d * a.inv_t - log_ts) - (x - x_ref) * a.inv_t);
-          twice |= atomicOr(bits + (el >> 5), 1u << (el & 31)) >> (el & 31) & 1u;
+          loss += prob * ((d * a.inv_t - log_ts) - (at.x[q] - x_ref) * a.inv_t);
+          twice |= atomicOr(at.bits + (el >> 5), 1u << (el & 31)) >> (el & 31) & 1u;
         }
       }
-      ids[q] = el;
-      probs[q] = prob;
+      at.id[q] = el;
+      at.q[q] = prob;
     }
     loss = warp_sum(loss);
     twice = __any_sync(0xffffffffu, twice);
     if (lane == 0) { teachers[g][into] = make_float4(loss, x_ref, ts == 0.0f ? 1.0f : 0.0f, 0.0f); repeats[g][into] = twice; }
     __syncwarp();
   };
-  // Serving warps do it up to two rows ahead where an SM has few rows in flight, one for each group; more groups hide their own.
+  // The gradient of a row's teacher columns, over what the second sweep wrote there, by threads t of n; clears their bits.
+  auto teacher_columns = [&](int g, int from, const Share& s, float4 row_end, int t, int n) {
+    const Taught at = taught(g, from);
+    const bool twice = repeats[g][from] != 0;
+    T* to = static_cast<T*>(a.grad) + s.to;
+    for (int q = t; q < a.K; q += n) {
+      const int el = at.id[q];
+      if (el < s.lo || el >= s.hi) continue;   // -1; or what an abandoned wait left there
+      at.bits[el >> 5] = 0;
+      if (a.grad == nullptr) continue;
+      float prob = at.q[q];
+      bool mine = true;
+      if (twice) {   // the first of those that name the same column writes the sum of them
+        prob = 0.0f;
+        for (int o = 0; o < a.K; ++o) {
+          if (at.id[o] != el) continue;
+          if (o < q) { mine = false; break; }
+          prob += at.q[o];
+        }
+      }
+      if (mine) to[el] = from_f32<T>(row_end.z * (exp2f((at.x[q] - row_end.y) * a.k) / row_end.w - prob));
+    }
+  };
+  // Serving warps do both where an SM has few rows in flight, one for each group: the teacher's part up to two rows ahead, and its columns
+  // when every warp has written its part of the row (by the row's own warps behind a barrier: 2048 x 151936 bf16 287 us, so 278).
+  // More groups hide their own.
   const bool taught_ahead = OP == kDistill && groups <= 2;
 
   if (serves) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kServeRegs<OP>));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kServeRegs));
     if (warp == kWarps) {
       // Lane g feeds group g's ring: pieces in the order they are taken, each when every warp has left the slot it goes to.
       uint32_t fed = ((blockIdx.x >> p.log_ctas) << p.log_groups) + lane;   // the place of the row
@@ -377,19 +405,33 @@ token_resident_kernel(const RowArgs a, const Resident p) {
     } else if (taught_ahead && warp - kWarps - 1 < groups) {
       const int g = warp - kWarps - 1;
       uint32_t parity = 1;
-      int into = 0;
-      for (uint32_t i = ((blockIdx.x >> p.log_ctas) << p.log_groups) + g; i < kept; i += step) {
+      int into = 0, rows[2] = {-1, -1};   // by parity: whose entries these are
+      auto end_row = [&]() {   // waits for the row that has them, if any, and writes its columns
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&t_empty[g][into]), parity, abort_flag, 57, p.status))) return false;
+        const int before = into == 0 ? rows[0] : rows[1];
+        if (before >= 0) teacher_columns(g, into, share_of<N>(a, p, rank, before), row_end[g][into], lane, 32);
+        __syncwarp();
+        return true;
+      };
+      bool ok = true;
+      for (uint32_t i = ((blockIdx.x >> p.log_ctas) << p.log_groups) + g; i < kept && ok; i += step) {
         const int row = row_of(i);
         if (state_of(i, row) != 0) continue;
-        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&t_empty[g][into]), parity, abort_flag, 57, p.status))) break;
+        ok = end_row();
+        if (!ok) break;
         teach(g, row, share_of<N>(a, p, rank, row), into);
         if (lane == 0) mbar_arrive(smem_u32(&t_full[g][into]));
+        if (into == 0) rows[0] = row; else rows[1] = row;
+        if (++into == 2) { into = 0; parity ^= 1; }
+      }
+      for (int q = 0; q < 2 && ok; ++q) {
+        ok = end_row();
         if (++into == 2) { into = 0; parity ^= 1; }
       }
       __syncwarp();
     }
   } else {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegs<OP>));
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegs));
 
   uint32_t phase = 0, slot_phase = 0, t_phase = 0;   // parities of the ring's current round, (bit i) of slot barrier i, of the teacher's
   int slot = 0, par = 0, at = info_rows;
@@ -720,36 +762,16 @@ token_resident_kernel(const RowArgs a, const Resident p) {
         if (tid < N ? el < min(s.fa * N, s.hi) : el < s.hi)
           g[el] = from_f32<T>(el == tl ? at_target : f_top * ex2((edge[group][par][tid] - top) * a.k));
       }
-      if constexpr (OP == kDistill) {
-        group_sync();   // the row's softmax is written before its teacher columns are
-        const int* ids = t_id + par * a.K;
-        const float* probs = t_q + par * a.K;
-        const bool twice = repeats[group][par] != 0;
-        for (int q = tid; q < a.K; q += gd) {
-          const int el = ids[q];
-          if (el < s.lo || el >= s.hi) continue;   // -1; or what an abandoned wait left there
-          float prob = probs[q];
-          bool mine = true;
-          if (twice) {   // the first of those that name the same column writes the sum of them
-            prob = 0.0f;
-            for (int o = 0; o < a.K; ++o) {
-              if (ids[o] != el) continue;
-              if (o < q) { mine = false; break; }
-              prob += probs[o];
-            }
-          }
-          if (mine) g[el] = from_f32<T>(c0 * (exp2f((t_x[par * a.K + q] - top) * a.k) / sw - prob));
-        }
-      }
     }
-    if constexpr (OP == kDistill) {   // (this parity's entries are made again behind the next row's first barrier)
-      if (p.group_warps == 1) __syncwarp();
-      for (int q = tid; q < a.K; q += gd) {
-        const int el = t_id[par * a.K + q];
-        if (el >= info.share.lo && el < info.share.hi) t_bits[par * bit_words + (el >> 5)] = 0;
+    if constexpr (OP == kDistill) {
+      if (taught_ahead) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&t_empty[group][par]));   // this warp has written its part
+      } else {
+        group_sync();   // the row's softmax is written
+        teacher_columns(group, par, info.share, make_float4(f_top, top, c0, sw), tid, gd);
+        if (p.group_warps == 1) __syncwarp();   // (these entries are made again behind the next row's first barrier)
       }
-      __syncwarp();
-      if (taught_ahead && lane == 0) mbar_arrive(smem_u32(&t_empty[group][par]));
     }
     par ^= 1;
   }
