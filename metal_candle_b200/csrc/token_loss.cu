@@ -365,11 +365,17 @@ preference_kernel(const float* logp, const void* targets, int target_bytes, int 
     for (int64_t i = lane; i < S; i += 8 * 32) {   // eight loads in flight
       float v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = i + 32 * j < S ? logp[b * S + i + 32 * j] : 0.0f;
+      for (int j = 0; j < 8; ++j) v[j] = logp[b * S + min(i + 32 * j, S - 1)];
+      if (average) {
+        int t[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = read_target(targets, target_bytes, has_ignore, ignore, b * S + min(i + 32 * j, S - 1), V);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) c += i + 32 * j < S && t[j] != -1;
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        acc += static_cast<double>(v[j]);
-        if (average && i + 32 * j < S) c += read_target(targets, target_bytes, has_ignore, ignore, b * S + i + 32 * j, V) != -1;
+        acc += i + 32 * j < S ? static_cast<double>(v[j]) : 0.0;
       }
     }
     for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
