@@ -1,7 +1,8 @@
 """Host-side mirror of the reference's `src/training` for the LoRA hot path: `LoRAConfig`, `LoRALayer`,
 `TargetModule`, `LoRAAdapterConfig`, `LoRAAdapter`, `AdamWConfig`, `AdamW`, `LRScheduler`,
 `TrainingConfig`, `StepMetrics`, `TrainingStep`.  Same names, argument meaning, defaults, validation
-messages and step/counter semantics; all arithmetic runs in the CUDA kernels behind the C ABI.
+messages and step/counter semantics; all arithmetic runs in the CUDA kernels behind the C ABI.  Beside the reference's
+cross-entropy: `token_log_probs`, `preference_loss`, `policy_loss` and `distillation_loss`, each with its gradient.
 """
 from __future__ import annotations
 
