@@ -493,11 +493,11 @@ int launch_sum(const float* terms, int64_t M, int n, float* out, cudaStream_t st
 
 // ---- checks of arguments ---------------------------------------------------------------------------------------------------
 
-constexpr int64_t kMaxDim = 0x7fffffff;
+constexpr int64_t kMaxDim = 0x7fffffff, kMaxVocab = 1 << 30;   // (columns are counted in 32 bits, a block's step past the end included)
 
 int check_logits(const char* what, const mcb_token_logits* l, const void* grad) {
   if (!l || !l->logits) return fail(MCB_ERR_NULL, "%s: null pointer", what);
-  if (l->batch <= 0 || l->seq <= 0 || l->vocab <= 0 || l->vocab > kMaxDim || l->batch > kMaxDim || l->seq > kMaxDim ||
+  if (l->batch <= 0 || l->seq <= 0 || l->vocab <= 0 || l->vocab > kMaxVocab || l->batch > kMaxDim || l->seq > kMaxDim ||
       l->batch * l->seq > kMaxDim)
     return fail(MCB_ERR_SHAPE, "%s: %lld x %lld rows of %lld logits", what, (long long)l->batch, (long long)l->seq, (long long)l->vocab);
   if (l->batch_stride < 0 || l->token_stride < 0) return fail(MCB_ERR_SHAPE, "%s: negative strides", what);
@@ -509,6 +509,12 @@ int check_logits(const char* what, const mcb_token_logits* l, const void* grad) 
     return fail(MCB_ERR_ALIGN, "%s: logits and gradient must lie on whole elements", what);
   if (grad == l->logits && (l->token_stride != l->vocab || l->batch_stride != l->seq * l->vocab))
     return fail(MCB_ERR_SHAPE, "%s: a gradient in place needs dense logits", what);
+  if (grad && grad != l->logits) {   // (elements in 128 bits: strides may be anything)
+    const __int128 from = reinterpret_cast<uintptr_t>(l->logits), g = reinterpret_cast<uintptr_t>(grad);
+    const __int128 n = static_cast<__int128>(l->batch - 1) * l->batch_stride + static_cast<__int128>(l->seq - 1) * l->token_stride + l->vocab;
+    if (from < g + static_cast<__int128>(l->batch * l->seq) * l->vocab * size && g < from + n * size)
+      return fail(MCB_ERR_SHAPE, "%s: the gradient overlaps the logits without being in place", what);
+  }
   return MCB_OK;
 }
 int check_targets(const char* what, const mcb_token_targets* t) {
@@ -599,9 +605,9 @@ extern "C" int mcb_token_logprob_bwd(const mcb_token_logits* logits, const mcb_t
                                      const float* dlogp, int64_t dlogp_rows, void* dlogits, void* stream) {
   MCB_NVTX_RANGE("mcb_token_logprob_bwd");
   if (!dlogits) return fail(MCB_ERR_NULL, "token_logprob_bwd: null output");
+  if (!logp || !lse || !dlogp) return fail(MCB_ERR_NULL, "token_logprob_bwd: null pointer");
   if (int rc = check_logits("token_logprob_bwd", logits, dlogits)) return rc;
   if (int rc = check_targets("token_logprob_bwd", targets)) return rc;
-  if (!logp || !lse || !dlogp) return fail(MCB_ERR_NULL, "token_logprob_bwd: null pointer");
   if (dlogp_rows <= 0) return fail(MCB_ERR_SHAPE, "token_logprob_bwd: dlogp_rows %lld", (long long)dlogp_rows);
   DeviceState* ds = current_device_state();
   if (!ds) return MCB_ERR_NOT_INIT;

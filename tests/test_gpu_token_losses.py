@@ -480,6 +480,50 @@ print("captured")
     assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
 
 
+@pytest.mark.parametrize("M,V", [(14402, 151936), (2200002, 1000)])
+def test_offsets_past_32_bits(cuda_device, M, V):
+    """2.2e9 elements of logits and of their gradient: rows at both ends and where a 32-bit offset would turn over."""
+    if torch.cuda.mem_get_info(cuda_device)[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    g = torch.Generator(device=cuda_device).manual_seed(11)
+    x = torch.empty(1, M, V, dtype=BF, device=cuda_device)
+    for part in x[0].split((1 << 28) // V):
+        part.copy_(2.5 * torch.randn(part.shape, device=cuda_device, generator=g))
+    t = torch.randint(0, V, (1, M), device=cuda_device, generator=g)
+    turn = 2 ** 31 // V
+    rows = torch.tensor([0, 1, turn - 1, turn, turn + 1, M - 2, M - 1], device=cuda_device)
+    logp, lse, p, kept = rows64(x[:, rows], t[:, rows])
+
+    def check(grad, coef, spread):
+        wg, size = grad64(p, t[:, rows], kept, coef)
+        check_grad(grad[:, rows], wg, spread * size)
+
+    got, glse = F.token_log_probs(x, t)
+    check_logp(got[:, rows], logp)
+    d = torch.randn(1, M, device=cuda_device, generator=g)
+    check(F.token_log_probs_backward(x, t, got, glse, d), d[:, rows].double(), 2)
+    A = torch.randn(1, M, device=cuda_device, generator=g)
+    out = F.policy_loss(x, t, A, return_grad=True)
+    check_logp(out.log_probs[:, rows], logp)
+    check(out.grad, -A[:, rows].double() / M, 2)
+    del out
+    pair = F.preference_loss(x.view(2, M // 2, V), t.view(2, M // 2), torch.zeros(2, device=cuda_device), beta=1e-4, return_grad=True)
+    z = 1e-4 * (got[0, :M // 2].double().sum() - got[0, M // 2:].double().sum())
+    # each of M log-probabilities is good to 2e-5 + 1e-6 |logp|, and the derivative of sigma is at most 1/4
+    assert abs(float(pair.loss) - math.log1p(math.exp(-float(z)))) <= 1e-4 * M * 4e-5 + 1e-6
+    c = 1e-4 * (torch.sigmoid(z) - 1)
+    sign = torch.where(rows < M // 2, 1.0, -1.0).double()[None]
+    check(pair.grad.view(1, M, V), c * sign, 2 + 1e-4 * M * 4e-5 / 5e-5)
+    del pair
+    ids = torch.randint(0, V, (1, M, 4), device=cuda_device, generator=g)
+    tl = torch.randn(1, M, 4, device=cuda_device, generator=g)
+    loss, grad = F.distillation_loss(x, ids, tl, return_grad=True)
+    wl, wg, parts, size = distill64(x[:, rows], ids[:, rows], tl[:, rows], torch.ones_like(rows, dtype=torch.bool)[None], 1.0)
+    n = len(rows) / M   # distill64 has the mean of these rows
+    check_grad(grad[:, rows], wg * n, parts * n)
+    assert math.isfinite(float(loss))
+
+
 def test_gradients_against_differences(cuda_device):
     """d loss along a direction, against (loss(x + h u) - loss(x - h u)) / 2h of the same entry points in float32: h = 0.02 along a
     direction of unit length; the third derivative of these losses along it is below 10 (0.0007 in the quotient), a loss

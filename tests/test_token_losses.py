@@ -109,6 +109,24 @@ def targets(**change):
 NULL, SHAPE, ALIGN, UNSUPPORTED, WORKSPACE = -1, -2, -3, -4, -5
 
 
+def test_c_vocabularies_that_32_bits_do_not_hold():
+    lib = _lib.load()
+    r = C.byref(rows(vocab=(1 << 30) + 1))
+    assert lib.mcb_token_logprob_fwd(r, C.byref(targets()), 16, None, None, None) == SHAPE
+
+
+@pytest.mark.parametrize("grad", [1024 + 4, 1024 - 4, 1024 + 4 * 47, 1024 - 4 * 47])
+def test_c_gradients_that_overlap_in_part(grad):
+    lib = _lib.load()
+    r = C.byref(rows(logits=1024))
+    assert lib.mcb_token_logprob_fwd(r, C.byref(targets()), 16, None, grad, None) == SHAPE
+    assert lib.mcb_token_logprob_bwd(r, C.byref(targets()), 16, 16, 16, 1, grad, None) == SHAPE
+    assert b"overlaps" in lib.mcb_last_error()
+    # a wide stride between sequences, the gradient in the gap
+    r = C.byref(rows(logits=1024, batch_stride=1 << 40))
+    assert lib.mcb_token_logprob_fwd(r, C.byref(targets()), 16, None, 1024 + 4096, None) == SHAPE
+
+
 @pytest.mark.parametrize("change,code", [
     (dict(logits=0), NULL), (dict(batch=0), SHAPE), (dict(seq=-1), SHAPE), (dict(vocab=0), SHAPE), (dict(vocab=1 << 31), SHAPE),
     (dict(batch=1 << 20, seq=1 << 20), SHAPE), (dict(batch=1 << 62, seq=4), SHAPE), (dict(batch_stride=-1), SHAPE), (dict(token_stride=-8), SHAPE),
