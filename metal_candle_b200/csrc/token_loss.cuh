@@ -85,6 +85,12 @@ struct TargetStats {
   float top, sum;       // of the whole row
   float logp, rest;     // log p_t and 1 - p_t
 };
+// y_t - y_m of a target so far below that (x_t - m) k is no float32 number, though y_t - y_m itself may be one (m > x_t)
+__device__ __forceinline__ float far_below(float xt, float m, float k) {
+  const float inv_t = k * kLn2, d = xt - m;
+  if (d > -INFINITY) return d * inv_t;
+  return m > 0.0f ? xt * inv_t - m * inv_t : d;   // (a difference that overflows has parts of both signs; else x_t is -inf)
+}
 __device__ __forceinline__ TargetStats target_stats(float m, float s, float xt, float k) {
   TargetStats r;
   if (m == -INFINITY && s == 0.0f) {   // nothing but the target (which, masked itself, has no probability: NaN)
@@ -100,7 +106,7 @@ __device__ __forceinline__ TargetStats target_stats(float m, float s, float xt, 
     r.rest = __fdividef(odds, r.sum);
   } else {   // (NaN as well)
     r.top = m; r.sum = s + ex2(-d);
-    r.logp = -d * kLn2 - logf(r.sum);
+    r.logp = (d < INFINITY ? -d * kLn2 : far_below(xt, m, k)) - logf(r.sum);
     r.rest = __fdividef(s, r.sum);
   }
   return r;

@@ -1,0 +1,41 @@
+"""GPU: the losses over given tokens where rows, targets or layouts are out of the ordinary, against float64 at the tolerances of
+ordinary rows (see test_gpu_token_losses)."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from metal_candle_b200 import _lib
+from metal_candle_b200 import training as F
+from tests.test_gpu_token_losses import BF, F32, IGN, both, check_grad, check_logp, grad64, make, rows64, teacher
+
+pytestmark = pytest.mark.gpu
+
+
+@both
+@pytest.mark.parametrize("V", [50, 5001, 50257])
+@pytest.mark.parametrize("T", [0.7, 1.0, 1.5, 2.0])
+def test_log_probabilities_of_the_lowest_values(cuda_device, dtype, V, T):
+    """y_t - lse down to where float32 ends, though y_t log2(e) lies beyond.  Two roundings of relative 2^-24 each may carry a value
+    across that end: within 1e-6 of it both are right."""
+    g = torch.Generator(device=cuda_device).manual_seed(20)
+    x = torch.randn(1, 9, V, device=cuda_device, generator=g).to(dtype)
+    low, most = torch.finfo(dtype).min, torch.finfo(torch.float32).max
+    x[0, 3:6] = 3e38
+    x[0, 6:8] = low
+    x[0, 8, 2:] = -1e38
+    x[0, :, 1] = torch.tensor([low, -2.5e38, -math.inf, low, 0.0, 2e38, -math.inf, low, low], device=cuda_device).to(dtype)
+    t = torch.ones(1, 9, dtype=torch.int64, device=cuda_device)
+    y = x.double()
+    top = y.amax(-1, keepdim=True)
+    want = ((y - top)[..., 1] / T - ((y - top) / T).exp().sum(-1).log())
+    outs = [F.token_log_probs(x, t, temperature=T)[0]]
+    for grad in (False, True):
+        outs.append(F.policy_loss(x, t, torch.zeros(1, device=cuda_device), temperature=T, return_grad=grad).log_probs)
+    for got in outs:
+        for v, w in zip(got[0].tolist(), want[0].tolist()):
+            if w < -most * (1 - 1e-6):
+                assert v == -math.inf or (w > -most * (1 + 1e-6) and v < -most * (1 - 2e-6)), (v, w)
+            else:
+                assert abs(v - w) <= 2e-5 + 1e-6 * abs(w), (v, w)
