@@ -133,7 +133,7 @@ __device__ __forceinline__ RowInputs row_inputs(const RowArgs& a, int64_t row) {
 }
 __device__ __forceinline__ PolicyTerm policy_term(const RowArgs& a, const RowInputs& in, float logp) {
   const float adv = in.advantage;
-  const float ratio = a.old_logp != nullptr ? ex2((logp - in.old_logp) * kLog2e) : 1.0f;
+  const float ratio = a.old_logp != nullptr ? ex2((logp - in.old_logp) * kLog2e) : isnan(logp) ? logp : 1.0f;
   const float bounded = fminf(fmaxf(ratio, a.ratio_min), a.ratio_max);
   PolicyTerm t;
   // min(r A, clip(r) A): the bound holds only where it makes the term smaller

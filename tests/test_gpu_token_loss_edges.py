@@ -39,3 +39,19 @@ def test_log_probabilities_of_the_lowest_values(cuda_device, dtype, V, T):
                 assert v == -math.inf or (w > -most * (1 + 1e-6) and v < -most * (1 - 2e-6)), (v, w)
             else:
                 assert abs(v - w) <= 2e-5 + 1e-6 * abs(w), (v, w)
+
+
+@both
+@pytest.mark.parametrize("V", [50, 5000, 50257, 700001])
+def test_policy_loss_of_nan_logits(cuda_device, dtype, V):
+    """NaN in a row is seen in the loss too, when the ratio is 1 for want of old log-probabilities."""
+    x, t, g = make(cuda_device, 2, 2, V, dtype, 28, keep=1.0)
+    old = torch.zeros(2, 2, device=cuda_device)
+    x[1, 0, (int(t[1, 0]) + 1) % V] = math.nan
+    for grad in (False, True):
+        for o in (None, old):
+            out = F.policy_loss(x, t, torch.ones(2, device=cuda_device), o, return_grad=grad)
+            assert out.loss.isnan() and out.log_probs.isnan().sum() == 1
+    x[1, 0] = -math.inf     # nothing but the target, which is certain
+    x[1, 0, int(t[1, 0])] = 1.0
+    assert F.policy_loss(x, t, torch.ones(2, device=cuda_device)).loss == -1
