@@ -98,6 +98,11 @@ __device__ __forceinline__ TargetStats target_stats(float m, float s, float xt, 
     r.top = xt; r.sum = 1.0f + r.logp;
     return r;
   }
+  if (xt == INFINITY) {   // an overflow, NaN as in any other column
+    r.top = xt;
+    r.logp = r.rest = r.sum = NAN;
+    return r;
+  }
   const float d = (m - xt) * k;
   if (d <= 0.0f) {
     const float odds = s * ex2(d);

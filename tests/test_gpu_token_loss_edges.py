@@ -55,3 +55,30 @@ def test_policy_loss_of_nan_logits(cuda_device, dtype, V):
     x[1, 0] = -math.inf     # nothing but the target, which is certain
     x[1, 0, int(t[1, 0])] = 1.0
     assert F.policy_loss(x, t, torch.ones(2, device=cuda_device)).loss == -1
+
+
+@both
+@pytest.mark.parametrize("V", [50, 5000, 50257, 151936, 700001])
+def test_infinite_logits(cuda_device, dtype, V):
+    """A logit that has overflowed makes its row NaN, at the target as in any other column, and no other row."""
+    g = torch.Generator(device=cuda_device).manual_seed(22)
+    x = torch.randn(2, 3, V, device=cuda_device, generator=g).to(dtype)
+    t = torch.full((2, 3), 2, dtype=torch.int64, device=cuda_device)
+    x[0, 1, 2] = math.inf       # the target
+    x[1, 0, V // 2] = math.inf
+    bad = torch.zeros(2, 3, dtype=torch.bool, device=cuda_device)
+    bad[0, 1] = bad[1, 0] = True
+    logp, lse = F.token_log_probs(x, t)
+    outs = [F.token_log_probs_backward(x, t, logp, lse, torch.ones_like(logp)),
+            F.policy_loss(x, t, torch.ones(2, device=cuda_device), return_grad=True).grad,
+            F.distillation_loss(x, t[..., None], torch.zeros(2, 3, 1, device=cuda_device), return_grad=True)[1]]
+    unit, lp = torch.empty_like(x), torch.empty_like(logp)
+    rows = C.byref(_lib.TokenLogits(x.data_ptr(), 2, 3, V, 3 * V, V, 1.0, int(dtype == BF)))
+    _lib.check(_lib.load().mcb_token_logprob_fwd(rows, C.byref(_lib.TokenTargets(t.data_ptr(), 8, 0, 0)), lp.data_ptr(), None, unit.data_ptr(),
+                                                 torch.cuda.current_stream().cuda_stream))
+    pol = F.policy_loss(x, t, torch.ones(2, device=cuda_device))
+    for v in (logp, lse, lp, pol.log_probs):
+        assert torch.equal(v.isnan(), bad)
+    for v in outs + [unit]:
+        assert torch.equal(v.isnan(), bad[..., None].expand(2, 3, V))
+    assert pol.loss.isnan() and F.preference_loss(x, t, torch.zeros(2, device=cuda_device)).loss.isnan()
