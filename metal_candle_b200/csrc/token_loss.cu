@@ -142,6 +142,7 @@ token_rows_kernel(const RowArgs a) {
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
 token_grad_kernel(const GradArgs ga) {
+  __shared__ float red[kRowThreads / 32];
   const RowArgs& a = ga.a;
   grid_launch_dependents();
   grid_dependency_wait();
@@ -155,11 +156,15 @@ token_grad_kernel(const GradArgs ga) {
     }
     const float c0 = ga.coef[row / ga.coef_rows] * a.inv_t, logp = a.logp[row];
     const float at = c0 * -expm1f(logp);
-    // log2 p_j = (x_j - x_t) k + log2 p_t, which keeps its digits whatever the size of the logits; from the log-sum-exp where the
-    // target itself is masked
-    const bool masked = logp == -INFINITY;
-    const float from = masked ? 0.0f : to_f32(x[tgt]), add = (masked ? -a.lse[row] : logp) * kLog2e;
-    __syncthreads();   // everyone has read the target's logit, which the gradient may lie over
+    float from, add;
+    if (!row_anchor(logp, a.lse[row], to_f32(x[tgt]), from, add)) {   // the same in every thread
+      float m = -INFINITY, s = 0.0f;
+      for (int c = threadIdx.x; c < a.V; c += blockDim.x) m = fmaxf(m, to_f32(x[c]));
+      from = block_max(m, red);
+      for (int c = threadIdx.x; c < a.V; c += blockDim.x) s += ex2((to_f32(x[c]) - from) * a.k);
+      add = -log2f(block_sum(s, red));
+    }
+    __syncthreads();   // everyone has read what the gradient may lie over
     for (int c = threadIdx.x; c < a.V; c += blockDim.x)
       g[c] = from_f32<T>(c == tgt ? at : -c0 * ex2(fmaf(to_f32(x[c]) - from, a.k, add)));
   }

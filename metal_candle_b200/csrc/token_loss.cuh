@@ -258,6 +258,18 @@ struct GradArgs {
   int64_t coef_rows;
 };
 
+// Where the exponents of such a row are taken from: log2 p_j = (x_j - from) k + add, with add 32 bits of log2 p_t (from the target) or of
+// -lse log2(e) (from 0).  Its rounding is an error of p_j relative to p_j, and so is that of x_j k, so the smaller of the two in
+// magnitude is taken: log p_t near 0 keeps its digits however large the logits are, and a target far below the rest (a token that a mask
+// forbids) costs the other columns none.  Where both are large (logits of some thousand, and a target far below) the kernels take the
+// row's maximum and sum again: returns false.  32: an error of 32 x 2^-24 for each of the few roundings, 1e-5.
+__device__ __forceinline__ bool row_anchor(float logp, float lse, float xt, float& from, float& add) {
+  const bool at_target = !(fabsf(logp) > fabsf(lse));   // (NaN: the row is NaN)
+  from = at_target ? xt : 0.0f;
+  add = (at_target ? logp : -lse) * kLog2e;
+  return !(fminf(fabsf(logp), fabsf(lse)) > 32.0f);
+}
+
 // token_stream.cu: kStats, or kPolicy without a gradient; and the gradient, where it is not in place.
 int launch_stats_rows(int op, const RowArgs& a, int dtype, DeviceState* ds, cudaStream_t st);
 int launch_grad_stream(const GradArgs& ga, int dtype, DeviceState* ds, cudaStream_t st, bool* taken);

@@ -172,16 +172,42 @@ token_stats_kernel(const RowArgs a, int log_ctas) {
   }
 }
 
+// A row's maximum and -log2 of its sum of exponentials, by a block or (SHORT) a warp that reads all of it: for the rare row whose known
+// statistics have not the digits (see row_anchor).
+template <typename T, bool SHORT>
+__device__ __forceinline__ void sweep_row(const T* x, int V, float k, int tid, int bd, float* red, float& top, float& minus_log) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto joined = [&](float v, auto join) {
+    for (int o = 16; o > 0; o >>= 1) v = join(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (SHORT) return v;
+    __syncthreads();   // red is free
+    if (lane == 0) red[warp] = v;
+    __syncthreads();
+    v = red[0];
+#pragma unroll 1
+    for (int w = 1; w < bd >> 5; ++w) v = join(v, red[w]);
+    return v;
+  };
+  float m = -INFINITY, s = 0.0f;
+#pragma unroll 1
+  for (int c = tid; c < V; c += bd) m = fmaxf(m, to_f32(x[c]));
+  top = m = joined(m, [](float a, float b) { return fmaxf(a, b); });
+#pragma unroll 1
+  for (int c = tid; c < V; c += bd) s += ex2((to_f32(x[c]) - m) * k);
+  minus_log = -log2f(joined(s, [](float a, float b) { return a + b; }));
+}
+
 // Gradient: dx_j = c (1[j = t] - p_j).  Bound: HBM, one read and one write.  A block takes `piece` vectors of a row, all of them in
 // flight at once.  The rows are taken from the last to the first: what the statistics' kernel read last may still be in L2.
 // Not in place: other blocks of the row read the target's logit.
 // SHORT: a warp does (a row has one piece).
 template <typename T, bool SHORT>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, SHORT ? 4 : 5)   // (the sweep that hardly any row takes would cost 16 registers, and with them a block an SM)
 token_grad_stream_kernel(const GradArgs ga, int pieces, uint32_t parts) {
   using VT = Vec16<T>;
   using Raw = decltype(VT::raw);
   constexpr int N = VT::N;
+  __shared__ float red[kThreads / 32];
   const RowArgs& a = ga.a;
   grid_launch_dependents();
   grid_dependency_wait();
@@ -229,10 +255,13 @@ token_grad_stream_kernel(const GradArgs ga, int pieces, uint32_t parts) {
   for (int j = 0; j < kUnroll; ++j)
     if (v0 + j * bd < r.fb) v[j].raw = __ldcs(src + v0 + j * bd);
   const float c0 = ga.coef[row / static_cast<uint32_t>(ga.coef_rows)] * a.inv_t, logp = a.logp[row];
-  // log2 p_j = (x_j - x_t) k + log2 p_t, which keeps its digits whatever the size of the logits; from the log-sum-exp where the
-  // target itself is masked
-  const bool masked = logp == -INFINITY;
-  const float ref = masked ? 0.0f : to_f32(x[tgt]), add = (masked ? -a.lse[row] : logp) * kLog2e;
+  float ref, add;
+  if (!row_anchor(logp, a.lse[row], to_f32(x[tgt]), ref, add)) {   // the same in every thread of the row
+    sweep_row<T, SHORT>(x, a.V, a.k, tid, bd, red, ref, add);
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j)   // again, so that nothing is kept meanwhile
+      if (v0 + j * bd < r.fb) v[j].raw = __ldcs(src + v0 + j * bd);
+  }
   const float2 neg = make_float2(-ref, -ref), kk = make_float2(a.k, a.k), add2 = make_float2(add, add), cc = make_float2(-c0, -c0);
 #pragma unroll
   for (int j = 0; j < kUnroll; ++j) {

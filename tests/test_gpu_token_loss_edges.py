@@ -82,3 +82,77 @@ def test_infinite_logits(cuda_device, dtype, V):
     for v in outs + [unit]:
         assert torch.equal(v.isnan(), bad[..., None].expand(2, 3, V))
     assert pol.loss.isnan() and F.preference_loss(x, t, torch.zeros(2, device=cuda_device)).loss.isnan()
+
+
+FAR = [-30.0, -100.0, -1e3, -1e4, -1e6, -1e9, None, -math.inf]   # None: the type's lowest value
+
+
+def far_targets(dev, V, dtype, seed=21):
+    """[1, rows, V], the target of every row column 1: of ordinary logits, of logits around 3e4 and of logits whose product with
+    log2(e) overflows."""
+    g = torch.Generator(device=dev).manual_seed(seed + V)
+    n = len(FAR)
+    x = torch.randn(1, 2 * n + 3, V, device=dev, generator=g) * 2.5
+    x[0, n:2 * n] += 3e4
+    x[0, 2 * n:] = 3e38
+    x = x.to(dtype)
+    for i, v in enumerate(FAR + FAR):
+        x[0, i, 1] = torch.finfo(dtype).min if v is None else v
+    x[0, 2 * n, 1] = -math.inf
+    x[0, 2 * n + 1, 1] = 0.0
+    x[0, 2 * n + 2, 1] = torch.finfo(dtype).min
+    return x, torch.ones(x.shape[:2], dtype=torch.int64, device=dev), g
+
+
+def in_place(x, t, logp, lse, d, T):
+    """mcb_token_logprob_bwd over the logits."""
+    B, S, V = x.shape
+    y = x.clone()
+    rows = C.byref(_lib.TokenLogits(y.data_ptr(), B, S, V, S * V, V, T, int(y.dtype == BF)))
+    _lib.check(_lib.load().mcb_token_logprob_bwd(rows, C.byref(_lib.TokenTargets(t.data_ptr(), 8, 0, 0)), logp.data_ptr(), lse.data_ptr(),
+                                                 d.data_ptr(), 1, y.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    return y
+
+
+def softmax64(x, T):
+    """log-probabilities and probabilities with the largest logit taken out first, so that nothing overflows."""
+    z = (x.double() - x.double().amax(-1, keepdim=True)) / T
+    logp = z - z.exp().sum(-1, keepdim=True).log()
+    return logp, logp.exp()
+
+
+@both
+@pytest.mark.parametrize("V", [50, 1000, 5001, 32000, 50257])
+@pytest.mark.parametrize("T", [0.7, 1.0, 2.0])
+def test_targets_far_below_the_rest(cuda_device, dtype, V, T):
+    """A target that the present mask forbids (-1e4, -1e9, the type's lowest value), in the reverse pass: the other columns keep their
+    softmax, at the tolerance of ordinary rows."""
+    x, t, g = far_targets(cuda_device, V, dtype)
+    d = torch.randn(t.shape, device=cuda_device, generator=g)
+    logp, lse = F.token_log_probs(x, t, temperature=T)
+    want, p = softmax64(x, T)
+    most = torch.finfo(F32).max   # (what lies within roundings of float32's end may come out on either side of it)
+    fits, beyond = want[..., 1] > -most * (1 - 1e-6), want[..., 1] < -most * (1 + 1e-6)
+    assert ((logp.double() - want[..., 1])[fits].abs() <= 2e-5 + 1e-6 * want[..., 1][fits].abs()).all()
+    assert (logp[beyond] == -math.inf).all()
+    wg, spread = grad64(p, t, torch.ones_like(t, dtype=torch.bool), d.double() / T)
+    check_grad(F.token_log_probs_backward(x, t, logp, lse, d, temperature=T), wg, 2 * spread)
+    check_grad(in_place(x, t, logp, lse, d, T), wg, 2 * spread)
+
+
+@both
+@pytest.mark.parametrize("V", [50, 1000, 50257])
+def test_pairs_with_targets_far_below_the_rest(cuda_device, dtype, V):
+    """A chosen answer of one forbidden token against one of a likely token: z is so far below 0 that the coefficients are beta / pairs."""
+    x, t, g = far_targets(cuda_device, V, dtype)
+    P = t.shape[1]
+    other = (torch.randn(P, 1, V, device=cuda_device, generator=g)).to(dtype)
+    other[:, 0, 1] = 12.0
+    x, t = torch.cat([x.view(P, 1, V), other]), torch.ones(2 * P, 1, dtype=torch.int64, device=cuda_device)
+    out = F.preference_loss(x, t, torch.zeros(2 * P, device=cuda_device), beta=2.0, return_grad=True)
+    _, p = softmax64(x, 1.0)
+    c = torch.full((2 * P, 1), 2.0 / P, dtype=torch.float64, device=cuda_device)
+    c[:P] *= -1
+    wg, spread = grad64(p, t, torch.ones_like(t, dtype=torch.bool), c)
+    check_grad(out.grad, wg, 2 * spread)
+    assert out.loss == math.inf
