@@ -398,7 +398,8 @@ preference_kernel(const float* logp, const void* targets, int target_bytes, int 
     // sums of some thousand nats whose difference is a few: not rounded before it is taken
     const float z = static_cast<float>(static_cast<double>(beta) * ((won - ref[i]) - (lost - ref[pairs + i])));
     const float tail = log1pf(expf(-fabsf(z)));
-    acc += static_cast<double>((1.0f - eps) * (fmaxf(-z, 0.0f) + tail) + eps * (fmaxf(z, 0.0f) + tail));
+    // (labels that are not smoothed: 0 times the infinite loss of the label that is not there is nothing)
+    acc += static_cast<double>((1.0f - eps) * (fmaxf(-z, 0.0f) + tail) + (eps > 0.0f ? eps * (fmaxf(z, 0.0f) + tail) : 0.0f));
     const float d = (eps - 1.0f / (1.0f + expf(z))) * beta / static_cast<float>(pairs);
     seq_logp[i] = static_cast<float>(won);
     seq_logp[pairs + i] = static_cast<float>(lost);

@@ -156,3 +156,22 @@ def test_pairs_with_targets_far_below_the_rest(cuda_device, dtype, V):
     wg, spread = grad64(p, t, torch.ones_like(t, dtype=torch.bool), c)
     check_grad(out.grad, wg, 2 * spread)
     assert out.loss == math.inf
+
+
+def test_pairs_of_forbidden_tokens(cuda_device):
+    """-inf at the target of a rejected answer: the pair is won for certain, a loss of 0 and no gradient; of a chosen one: an
+    infinite loss, whose gradient is finite.  With smoothed labels either is infinite."""
+    P, S, V, beta = 3, 2, 40, 0.5
+    x, t, g = make(cuda_device, 2 * P, S, V, F32, 23, keep=1.0)
+    ref = torch.zeros(2 * P, device=cuda_device)
+    won, lost = x.clone(), x.clone()
+    won[P + 1, 0, int(t[P + 1, 0])] = -math.inf
+    lost[1, 0, int(t[1, 0])] = -math.inf
+    out = F.preference_loss(won, t, ref, beta=beta, return_grad=True)
+    alone = [F.preference_loss(won[[i, P + i]], t[[i, P + i]], ref[:2], beta=beta) for i in range(P)]
+    assert float(alone[1].loss) == 0.0
+    assert abs(float(out.loss) - (float(alone[0].loss) + float(alone[2].loss)) / P) <= 1e-6 * (1 + float(out.loss))
+    assert (out.grad[[1, P + 1]] == 0).all() and not out.grad.isnan().any()
+    assert F.preference_loss(won, t, ref, beta=beta, label_smoothing=0.1).loss == math.inf
+    out = F.preference_loss(lost, t, ref, beta=beta, return_grad=True)
+    assert out.loss == math.inf and out.grad.isfinite().all() and (out.grad[1] != 0).any()
