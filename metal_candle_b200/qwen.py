@@ -239,6 +239,7 @@ class Qwen:
         self.norm = torch.ones(H, dtype=dtype, device=self.device)
         self.lm_head = _Linear(c.vocab_size, H, False, dtype, self.device, g)
         self.lora_adapter: Optional[LoRAAdapter] = None
+        self._adapter_aside = 0    # adapter_disabled() blocks that are open
         self._grad_flat: Optional[torch.Tensor] = None
         self._grad_views: List[torch.Tensor] = []
         self._grad_slices: Dict[str, Tuple[torch.Tensor, torch.Tensor]] = {}
@@ -256,7 +257,12 @@ class Qwen:
         self.backward_done_hook = None  # called once at the end of forward_backward (joins side-stream work)
 
     # -- adapter management (Qwen::apply_adapter / remove_adapter, src/models/qwen.rs:150-175) --
+    def _may_exchange_adapter(self) -> None:
+        if self._adapter_aside:
+            raise TrainingError("the adapter cannot be exchanged within adapter_disabled(), which puts it back at its end")
+
     def apply_adapter(self, adapter: LoRAAdapter) -> None:
+        self._may_exchange_adapter()
         c = self.config
         for key, layer in adapter.layers():
             _, idx, module = key.split(".")
@@ -286,6 +292,7 @@ class Qwen:
             self._layer_ranges[idx] = (min(lo, start), off)
 
     def remove_adapter(self) -> None:
+        self._may_exchange_adapter()
         for L in self.layers:
             for m in self.MODULES:
                 L[m].lora = None
@@ -576,14 +583,19 @@ class Qwen:
     # -- post-training losses: the same pass with another loss between the lm_head and its backward --
     @contextmanager
     def adapter_disabled(self):
-        """The base model for the time of a `with` block: the frozen reference of a preference or policy loss."""
+        """The base model for the time of a `with` block: the frozen reference of a preference or policy loss.  Meanwhile the model
+        has no adapter: passes that train one are refused, and so are `apply_adapter` and `remove_adapter`."""
         lins = [L[m] for L in self.layers for m in self.MODULES]
-        loras = [lin.lora for lin in lins]
+        loras, adapter = [lin.lora for lin in lins], self.lora_adapter
+        self._adapter_aside += 1
         try:
             for lin in lins:
                 lin.lora = None
+            self.lora_adapter = None
             yield self
         finally:
+            self._adapter_aside -= 1
+            self.lora_adapter = adapter
             for lin, lora in zip(lins, loras):
                 lin.lora = lora
 
