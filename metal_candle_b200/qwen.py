@@ -379,8 +379,13 @@ class Qwen:
             off += l.out_f
         return dict(w=cached[1], wt=cached[2], bias=cached[3], scale=sc, offsets=offs, width=off, lins=lins)
 
+    def _here(self, t: torch.Tensor, what: str) -> torch.Tensor:
+        if t.device != self.embed_tokens.device:
+            raise TrainingError(f"{what} is on {t.device}, the model is on {self.embed_tokens.device}")
+        return t
+
     def _embed(self, ids32: torch.Tensor) -> torch.Tensor:
-        M = ids32.numel()
+        M = self._here(ids32, "input_ids").numel()
         out = torch.empty(M, self.config.hidden_size, dtype=self.dtype, device=self.device)
         _lib.check(self.lib.mcb_embedding_fwd(_ptr(ids32), _ptr(self.embed_tokens), _ptr(out), M, self.config.hidden_size,
                                               self.config.vocab_size, self.dt, _stream()))
@@ -508,7 +513,7 @@ class Qwen:
         c = self.config
         B, S = input_ids.shape
         M = B * S
-        tgt32 = target_ids.to(torch.int32).contiguous().view(-1)  # u32::MAX wraps to -1 = ignored
+        tgt32 = self._here(target_ids, "target_ids").to(torch.int32).contiguous().view(-1)  # u32::MAX wraps to -1 = ignored
         run = self._forward_saved(input_ids)
         nf = run["nf"]
         nll = torch.empty(M, dtype=torch.float32, device=self.device)
