@@ -747,6 +747,7 @@ extern "C" int mcb_preference_loss(const mcb_token_logits* logits, const mcb_tok
   if (logits->batch % 2 != 0) return fail(MCB_ERR_SHAPE, "preference_loss: %lld sequences are no pairs", (long long)logits->batch);
   if (!workspace || workspace_bytes < mcb_token_loss_workspace_bytes(logits->batch, logits->seq))
     return fail(MCB_ERR_WORKSPACE, "preference_loss: workspace missing or too small");
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return fail(MCB_ERR_ALIGN, "preference_loss: the workspace must lie on a 16-byte boundary");
   const int64_t M = logits->batch * logits->seq;
   float* logp = static_cast<float*>(workspace);
   float* lse = logp + M;
