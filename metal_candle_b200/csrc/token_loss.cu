@@ -501,6 +501,10 @@ int launch_sum(const float* terms, int64_t M, int n, float* out, cudaStream_t st
 
 constexpr int64_t kMaxDim = 0x7fffffff, kMaxVocab = 1 << 30;   // (columns are counted in 32 bits, a block's step past the end included)
 
+// The stride of a dimension of one says nothing: taken as that of dense rows.
+int64_t token_stride(const mcb_token_logits* l) { return l->seq == 1 ? l->vocab : l->token_stride; }
+int64_t batch_stride(const mcb_token_logits* l) { return l->batch == 1 ? l->seq * l->vocab : l->batch_stride; }
+
 int check_logits(const char* what, const mcb_token_logits* l, const void* grad) {
   if (!l || !l->logits) return fail(MCB_ERR_NULL, "%s: null pointer", what);
   if (l->batch <= 0 || l->seq <= 0 || l->vocab <= 0 || l->vocab > kMaxVocab || l->batch > kMaxDim || l->seq > kMaxDim ||
@@ -513,7 +517,7 @@ int check_logits(const char* what, const mcb_token_logits* l, const void* grad) 
   const uintptr_t size = l->dtype == MCB_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(l->logits) % size != 0 || reinterpret_cast<uintptr_t>(grad) % size != 0)
     return fail(MCB_ERR_ALIGN, "%s: logits and gradient must lie on whole elements", what);
-  if (grad == l->logits && (l->token_stride != l->vocab || l->batch_stride != l->seq * l->vocab))
+  if (grad == l->logits && (token_stride(l) != l->vocab || batch_stride(l) != l->seq * l->vocab))
     return fail(MCB_ERR_SHAPE, "%s: a gradient in place needs dense logits", what);
   if (grad && grad != l->logits) {   // (elements in 128 bits: strides may be anything)
     const __int128 from = reinterpret_cast<uintptr_t>(l->logits), g = reinterpret_cast<uintptr_t>(grad);
@@ -566,7 +570,7 @@ struct LossWorkspace {
 RowArgs row_args(const mcb_token_logits* l, void* grad) {
   RowArgs a = {};
   a.logits = l->logits; a.grad = grad;
-  a.M = l->batch * l->seq; a.S = l->seq; a.batch_stride = l->batch_stride; a.token_stride = l->token_stride;
+  a.M = l->batch * l->seq; a.S = l->seq; a.batch_stride = batch_stride(l); a.token_stride = token_stride(l);
   a.V = static_cast<int>(l->vocab);
   a.temperature = l->temperature; a.inv_t = 1.0f / l->temperature; a.k = kLog2e / l->temperature;
   return a;

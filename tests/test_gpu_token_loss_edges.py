@@ -175,3 +175,27 @@ def test_pairs_of_forbidden_tokens(cuda_device):
     assert F.preference_loss(won, t, ref, beta=beta, label_smoothing=0.1).loss == math.inf
     out = F.preference_loss(lost, t, ref, beta=beta, return_grad=True)
     assert out.loss == math.inf and out.grad.isfinite().all() and (out.grad[1] != 0).any()
+
+
+@both
+def test_strides_of_single_rows(cuda_device, dtype):
+    """The stride of a dimension of one is any number: such logits are dense all the same, and may be written over."""
+    lib, st = _lib.load(), torch.cuda.current_stream().cuda_stream
+    for B, S, V in ((1, 5, 1001), (4, 1, 1001), (1, 1, 300), (1, 3, 50257)):
+        x, t, g = make(cuda_device, B, S, V, dtype, 24, keep=1.0)
+        logp, lse = F.token_log_probs(x, t)
+        d = torch.randn(B, S, device=cuda_device, generator=g)
+        _, _, p, kept = rows64(x, t)
+        wg, spread = grad64(p, t, kept, d.double())
+        strides = (7 if B == 1 else V if S == 1 else S * V, 5 if S == 1 else V)
+        y = x.clone()
+        rows = C.byref(_lib.TokenLogits(y.data_ptr(), B, S, V, *strides, 1.0, int(dtype == BF)))
+        _lib.check(lib.mcb_token_logprob_bwd(rows, C.byref(_lib.TokenTargets(t.data_ptr(), 8, 0, 0)), logp.data_ptr(), lse.data_ptr(),
+                                             d.data_ptr(), 1, y.data_ptr(), st))
+        check_grad(y, wg, 2 * spread)
+        y = x.clone()
+        rows = C.byref(_lib.TokenLogits(y.data_ptr(), B, S, V, *strides, 1.0, int(dtype == BF)))
+        lp = torch.empty_like(logp)
+        _lib.check(lib.mcb_token_logprob_fwd(rows, C.byref(_lib.TokenTargets(t.data_ptr(), 8, 0, 0)), lp.data_ptr(), None, y.data_ptr(), st))
+        wg, spread = grad64(p, t, kept, torch.ones_like(d).double())
+        check_grad(y, wg, 2 * spread)
