@@ -432,7 +432,8 @@ int launch_sum(const float* terms, int64_t M, int n, float* out, cudaStream_t st
 constexpr int64_t kSumInside = 4096;   // rows whose terms the one-pass kernel's last block sums
 template <int OP>
 int launch_rows(const RowArgs& a, const RowPlan& plan, int dtype, DeviceState* ds, cudaStream_t st) {
-  if (OP == kStats || (OP == kPolicy && a.grad == nullptr)) {
+  static_assert(OP != kStats, "launch_stats_rows");
+  if (OP == kPolicy && a.grad == nullptr) {
     if (int rc = launch_stats_rows(OP, a, dtype, ds, st)) return rc;
     return plan.sums != nullptr ? launch_sum(a.terms, a.M, plan.n_sums, plan.sums, st) : MCB_OK;
   }
@@ -608,7 +609,7 @@ extern "C" int mcb_token_logprob_fwd(const mcb_token_logits* logits, const mcb_t
   set_targets(a, targets);
   a.logp = logp; a.lse = lse;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return unit_grad ? launch_rows<kUnit>(a, {}, logits->dtype, ds, st) : launch_rows<kStats>(a, {}, logits->dtype, ds, st);
+  return unit_grad ? launch_rows<kUnit>(a, {}, logits->dtype, ds, st) : launch_stats_rows(kStats, a, logits->dtype, ds, st);
 }
 
 extern "C" int mcb_token_logprob_bwd(const mcb_token_logits* logits, const mcb_token_targets* targets, const float* logp, const float* lse,

@@ -893,10 +893,7 @@ int launch_resident_rows(int op, const RowArgs& a, const RowPlan& plan, int dtyp
   const bool f32 = dtype == MCB_F32;
   if (op == kUnit) return f32 ? launch_resident<float, kUnit>(a, plan, ds, st, taken) : launch_resident<__nv_bfloat16, kUnit>(a, plan, ds, st, taken);
   if (op == kPolicy) return f32 ? launch_resident<float, kPolicy>(a, plan, ds, st, taken) : launch_resident<__nv_bfloat16, kPolicy>(a, plan, ds, st, taken);
-  if (op == kDistill)
-    return f32 ? launch_resident<float, kDistill>(a, plan, ds, st, taken) : launch_resident<__nv_bfloat16, kDistill>(a, plan, ds, st, taken);
-  *taken = false;
-  return MCB_OK;
+  return f32 ? launch_resident<float, kDistill>(a, plan, ds, st, taken) : launch_resident<__nv_bfloat16, kDistill>(a, plan, ds, st, taken);
 }
 }  // namespace tokenloss
 }  // namespace mcb

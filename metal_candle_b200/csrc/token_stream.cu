@@ -302,7 +302,7 @@ token_short_kernel(const RowArgs a, const RowPlan plan) {
   double* mine = plan.sums != nullptr ? sums[warp] : nullptr;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + warp; row < a.M; row += static_cast<int64_t>(gridDim.x) * kRows) {
     const T* x = static_cast<const T*>(from_here(a.logits)) + row_offset(a, row);
-    T* g = a.grad != nullptr ? static_cast<T*>(a.grad) + row * a.V : nullptr;
+    T* g = static_cast<T*>(a.grad) + row * a.V;
     const T* base;
     const RowVecs r = vecs_of(x, a.V, base);
     const Raw* src = reinterpret_cast<const Raw*>(base);
@@ -334,14 +334,12 @@ token_short_kernel(const RowArgs a, const RowPlan plan) {
     if (tgt < 0) {   // the same in every lane
       const float value = tgt == -2 ? NAN : 0.0f;
       if (lane == 0) write_left_out<OP>(a, row, value, mine);
-      if (g != nullptr) {
-        float f[N];
+      float f[N];
 #pragma unroll
-        for (int q = 0; q < N; ++q) f[q] = value;
+      for (int q = 0; q < N; ++q) f[q] = value;
 #pragma unroll
-        for (int j = 0; j < kUnroll; ++j) { v[j].from_float(f); put(j); }
-        if (edges) to[edge] = from_f32<T>(value);
-      }
+      for (int j = 0; j < kUnroll; ++j) { v[j].from_float(f); put(j); }
+      if (edges) to[edge] = from_f32<T>(value);
       continue;
     }
     // the target: lane, vector and element, or an edge
@@ -381,7 +379,6 @@ token_short_kernel(const RowArgs a, const RowPlan plan) {
     const TargetStats t = target_stats(m, s, xt, a.k);
     const RowResult res = finish_target_row<OP>(a, inputs, t);
     if (lane == 0) write_target_row<OP>(a, row, t, res, mine);
-    if (g == nullptr) continue;
     const float top = t.top == -INFINITY ? 0.0f : t.top, scale = -res.c / t.sum, at_target = res.c * t.rest;   // an element's gradient is scale 2^((x - top) k)
     const float2 neg_top = make_float2(-top, -top), ss = make_float2(scale, scale);
 #pragma unroll
