@@ -300,7 +300,11 @@ token_short_kernel(const RowArgs a, const RowPlan plan) {
   grid_launch_dependents();
   grid_dependency_wait();
   double* mine = plan.sums != nullptr ? sums[warp] : nullptr;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + warp; row < a.M; row += static_cast<int64_t>(gridDim.x) * kRows) {
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kRows + warp, step = static_cast<int64_t>(gridDim.x) * kRows;
+  int64_t next = row0 < a.M ? load_target(a.targets, a.target_bytes, row0) : -1;   // known before the row is asked for: left out, it is not read
+  for (int64_t row = row0; row < a.M; row += step) {
+    const int tgt = judge_target(next, a.has_ignore, a.ignore, a.V);
+    if (row + step < a.M) next = load_target(a.targets, a.target_bytes, row + step);
     const T* x = static_cast<const T*>(from_here(a.logits)) + row_offset(a, row);
     T* g = static_cast<T*>(a.grad) + row * a.V;
     const T* base;
@@ -311,13 +315,6 @@ token_short_kernel(const RowArgs a, const RowPlan plan) {
     const int edge = lane < N ? r.lo + lane : r.fb * N + lane - N;   // the elements beside the row's own vectors
     const bool edges = lane < 2 * N && (lane < N ? edge < min(r.fa * N, r.hi) : edge < r.hi);
     VT v[kUnroll];
-#pragma unroll
-    for (int j = 0; j < kUnroll; ++j) {
-      const int vi = r.fa + j * 32 + lane;
-      if (vi < r.fb) v[j].raw = src[vi];
-      else fill_masked(v[j]);
-    }
-    const float x_edge = edges ? to_f32(base[edge]) : -INFINITY;
     auto put = [&](int j) {
       const int vi = r.fa + j * 32 + lane;
       if (vi >= r.fb) return;
@@ -329,8 +326,6 @@ token_short_kernel(const RowArgs a, const RowPlan plan) {
         for (int q = 0; q < N; ++q) to[vi * N + q] = e[q];
       }
     };
-    const RowInputs inputs = row_inputs<OP>(a, row);
-    const int tgt = read_target(a.targets, a.target_bytes, a.has_ignore, a.ignore, row, a.V);
     if (tgt < 0) {   // the same in every lane
       const float value = tgt == -2 ? NAN : 0.0f;
       if (lane == 0) write_left_out<OP>(a, row, value, mine);
@@ -342,6 +337,14 @@ token_short_kernel(const RowArgs a, const RowPlan plan) {
       if (edges) to[edge] = from_f32<T>(value);
       continue;
     }
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+      const int vi = r.fa + j * 32 + lane;
+      if (vi < r.fb) v[j].raw = src[vi];
+      else fill_masked(v[j]);
+    }
+    const float x_edge = edges ? to_f32(base[edge]) : -INFINITY;
+    const RowInputs inputs = row_inputs<OP>(a, row);
     // the target: lane, vector and element, or an edge
     const int te = r.lo + tgt, tv = te / N - r.fa, tq = te % N;
     const bool own = te / N >= r.fa && te / N < r.fb && (tv & 31) == lane, at_edge = edges && edge == te;

@@ -199,3 +199,22 @@ def test_strides_of_single_rows(cuda_device, dtype):
         _lib.check(lib.mcb_token_logprob_fwd(rows, C.byref(_lib.TokenTargets(t.data_ptr(), 8, 0, 0)), lp.data_ptr(), None, y.data_ptr(), st))
         wg, spread = grad64(p, t, kept, torch.ones_like(d).double())
         check_grad(y, wg, 2 * spread)
+
+
+@both
+@pytest.mark.parametrize("V", [37, 1000])
+def test_many_short_rows_some_left_out(cuda_device, dtype, V):
+    """More rows than the chip has warps for, so that each takes several; what the left-out ones hold does not count."""
+    x, t, g = make(cuda_device, 4, 4001, V, dtype, 29, keep=0.4)
+    t[1, :2000] = -1
+    t[2, 7] = V
+    logp, _, p, kept = rows64(x, t)
+    kept[2, 7] = False
+    A = torch.randn(4, 4001, device=cuda_device, generator=g)
+    wg, spread = grad64(p, torch.where(kept, t, torch.zeros_like(t)), kept, -A.double() / (int(kept.sum()) + 1))
+    x[~kept] = math.nan
+    out = F.policy_loss(x, t, A, ignore_index=IGN, return_grad=True)
+    assert out.grad[2, 7].isnan().all() and out.log_probs.isnan().sum() == 1 and out.loss.isnan()
+    out.grad[2, 7], out.log_probs[2, 7], logp[2, 7] = 0, 0, 0
+    check_logp(out.log_probs, logp)
+    check_grad(out.grad, wg, 2 * spread)
