@@ -156,7 +156,7 @@ __device__ __forceinline__ PolicyTerm policy_term(const RowArgs& a, const RowInp
     // exp(d) - d - 1 >= 0 with d = ref - logp: an estimate of KL(policy || reference) that is never negative
     const float d = in.ref_logp - logp;
     const float e = expm1f(d);
-    t.kl = e - d;
+    t.kl = e < INFINITY ? e - d : e;   // (d = inf, a target that the policy forbids: e - d would be NaN)
     if (a.kl_coef > 0.0f) {   // (0 times an infinite divergence is not a loss)
       t.loss += a.kl_coef * t.kl;
       t.dlogp -= a.kl_coef * e;

@@ -218,3 +218,20 @@ def test_many_short_rows_some_left_out(cuda_device, dtype, V):
     out.grad[2, 7], out.log_probs[2, 7], logp[2, 7] = 0, 0, 0
     check_logp(out.log_probs, logp)
     check_grad(out.grad, wg, 2 * spread)
+
+
+@both
+@pytest.mark.parametrize("V", [100, 5000, 50257, 700001])
+def test_divergence_of_forbidden_tokens(cuda_device, dtype, V):
+    """The policy forbids a token (-inf) that the reference allows: the divergence is infinite, and seen in the loss where it has a weight."""
+    x, t, g = make(cuda_device, 2, 2, V, dtype, 30, keep=1.0)
+    x[0, 1, int(t[0, 1])] = -math.inf
+    A, old = torch.ones(2, device=cuda_device), torch.full((2, 2), -2.0, device=cuda_device)
+    for grad in (False, True):
+        out = F.policy_loss(x, t, A, old, old, return_grad=grad)
+        assert out.kl == math.inf and out.loss.isfinite()
+        assert F.policy_loss(x, t, A, old, old, kl_coef=0.1, return_grad=grad).loss == math.inf
+        nan = old.clone()
+        nan[1, 0] = math.nan
+        assert F.policy_loss(x, t, A, old, nan, return_grad=grad).kl.isnan()
+    assert (out.grad[0, 1] == 0).all() and out.grad.isfinite().all()   # a ratio of 0
