@@ -277,35 +277,31 @@ token_resident_kernel(const RowArgs a, const Resident p) {
 
   // Distillation: a row's teacher, by one warp: q = softmax(t / T) over its entries, those with -inf counting for nothing; of the entries
   // whose column is in this share where it is (or -1), q and the student's logit; and the sum of q (log q - (x - x_ref) / T) over
-  // them, with x_ref the student's logit where the teacher's is largest.
+  // them, with x_ref the largest of the student's logits among all entries: no difference is positive, so that a forbidden token's
+  // loss may be infinite but nothing infinite cancels.
   auto teach = [&](int g, int row, const Share& s, int into) {
     const int64_t t0 = static_cast<int64_t>(row) * a.K;
     const T* x_row = static_cast<const T*>(a.logits) + row_offset(a, row);
     const Taught at = taught(g, into);
     auto id_of = [&](int64_t id) { return id >= 0 && id < a.V ? static_cast<int>(id) : -1; };
-    float tm = -INFINITY, ts = 0.0f;
+    float tm = -INFINITY, ts = 0.0f, x_ref = -INFINITY;
 #pragma unroll 2
     for (int q = lane; q < a.K; q += 32) {   // (loads of the student's logits that another CTA has are the same ones it makes)
       const float t = read_teacher(a, t0 + q);
       const int id = id_of(read_teacher_id(a, t0 + q));
-      at.x[q] = id >= 0 ? to_f32(x_row[id]) : 0.0f;
+      const float x = id >= 0 ? to_f32(x_row[id]) : -INFINITY;
+      at.x[q] = x;
+      x_ref = fmaxf(x_ref, x);
       at.id[q] = id;
       at.q[q] = t;
       tm = fmaxf(tm, t);
     }
     tm = warp_max(tm);
-    const float tref = tm == -INFINITY ? 0.0f : tm;
-    float x_ref = 0.0f;
-    bool best = false;
-    for (int q = lane; q < a.K; q += 32) {
-      const float t = at.q[q];
-      ts += ex2((t - tref) * a.k);
-      if (t == tm && !best && at.id[q] >= 0) { best = true; x_ref = at.x[q]; }
-    }
-    ts = warp_sum(ts);
-    const uint32_t who = __ballot_sync(0xffffffffu, best);
-    x_ref = __shfl_sync(0xffffffffu, x_ref, who == 0 ? 0 : __ffs(who) - 1);
+    x_ref = warp_max(x_ref);
     if (!(fabsf(x_ref) < INFINITY)) x_ref = 0.0f;
+    const float tref = tm == -INFINITY ? 0.0f : tm;
+    for (int q = lane; q < a.K; q += 32) ts += ex2((at.q[q] - tref) * a.k);
+    ts = warp_sum(ts);
     const float inv_ts = ts == 0.0f ? 0.0f : 1.0f / ts, log_ts = logf(ts);
     float loss = 0.0f;
     bool twice = false;

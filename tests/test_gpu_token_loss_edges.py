@@ -235,3 +235,39 @@ def test_divergence_of_forbidden_tokens(cuda_device, dtype, V):
         nan[1, 0] = math.nan
         assert F.policy_loss(x, t, A, old, nan, return_grad=grad).kl.isnan()
     assert (out.grad[0, 1] == 0).all() and out.grad.isfinite().all()   # a ratio of 0
+
+
+@both
+@pytest.mark.parametrize("V", [50, 5001, 50257, 700001])
+@pytest.mark.parametrize("T", [0.5, 1.0, 2.0])
+def test_distillation_of_forbidden_tokens(cuda_device, dtype, V, T):
+    """The student forbids what the teacher likes best or second best: a large or infinite loss, and a gradient of ordinary size."""
+    K = 6
+    g = torch.Generator(device=cuda_device).manual_seed(31)
+    low = torch.finfo(dtype).min
+    masks = [-1e4, -1e9, low, -math.inf]
+    R = 2 * len(masks) + 2
+    x = (torch.randn(1, R, V, device=cuda_device, generator=g) * 2).to(dtype)
+    ids = torch.stack([torch.randperm(V, device=cuda_device, generator=g)[:K] for _ in range(R)]).view(1, R, K)
+    tl = torch.randn(1, R, K, device=cuda_device, generator=g)
+    tl[..., 0], tl[..., 1] = 4.0, 3.5
+    for i, v in enumerate(masks + masks):
+        x[0, i, ids[0, i, i // len(masks)]] = v
+    x[0, R - 2] = 3e38
+    x[0, R - 1] = low
+    q = torch.softmax(tl.double() / T, -1)
+    z = (x.double() - x.double().amax(-1, keepdim=True)) / T
+    logp = z - z.exp().sum(-1, keepdim=True).log()
+    p = logp.exp()
+    _, grad = F.distillation_loss(x, ids, tl, temperature=T, return_grad=True)
+    check_grad(grad, p.scatter_add(-1, ids, -q) * T / R, p.scatter_add(-1, ids, q) * T / R)
+    want = (q * (q.log() - logp.gather(-1, ids))).sum(-1)[0] * T * T
+    for i in range(R):
+        for with_grad in (False, True):
+            out = F.distillation_loss(x[:, i:i + 1], ids[:, i:i + 1], tl[:, i:i + 1], temperature=T, return_grad=with_grad)
+            v, w = float(out[0] if with_grad else out), float(want[i])
+            # terms of size |log q| + loss, each to 3e-5; where y = x / T or the loss, before T^2 or after it, is no float32 any more, the
+            # loss may be infinite
+            near = abs(v - w) <= 3e-5 * (T * T * 20 + w)
+            held = max(w, w / (T * T), float(x[0, i].abs().max()) / T) < torch.finfo(F32).max * (1 - 1e-4)
+            assert near or (v == math.inf and not held), (i, v, w)
