@@ -271,3 +271,91 @@ def test_distillation_of_forbidden_tokens(cuda_device, dtype, V, T):
             near = abs(v - w) <= 3e-5 * (T * T * 20 + w)
             held = max(w, w / (T * T), float(x[0, i].abs().max()) / T) < torch.finfo(F32).max * (1 - 1e-4)
             assert near or (v == math.inf and not held), (i, v, w)
+
+
+@both
+@pytest.mark.parametrize("V", [37, 300, 2051, 50257])
+def test_gradients_at_every_alignment(cuda_device, dtype, V):
+    """Gradients that begin anywhere relative to 16 bytes, while the logits begin on or beside such a boundary, on another stream than
+    the one that made the inputs."""
+    B, S, K = 2, 3, 5
+    x0, t, g = make(cuda_device, B, S, V, dtype, 25)
+    ids, tl = teacher(cuda_device, g, B, S, V, K, dtype)
+    n, lib = B * S * V, _lib.load()
+    A = torch.randn(B, S, device=cuda_device, generator=g)
+    logp64, _, p, kept = rows64(x0, t)
+    w = kept.double() / kept.sum().clamp_min(1)
+    by_target, spread = grad64(p, t, kept, A.double())
+    by_policy = -by_target / kept.sum().clamp_min(1)   # r = 1 without old log-probabilities
+    q = torch.softmax(tl.double(), -1)
+    by_teacher = p.scatter_add(-1, ids, -q) / (B * S)
+    parts = p.scatter_add(-1, ids, q) / (B * S)
+    stream = torch.cuda.Stream()
+    for lo in (0, 1):
+        flat = torch.empty(n + 1, dtype=dtype, device=cuda_device)
+        x = flat[lo:lo + n].view(B, S, V)
+        x.copy_(x0)
+        rows = C.byref(_lib.TokenLogits(x.data_ptr(), B, S, V, S * V, V, 1.0, int(dtype == BF)))
+        tt = C.byref(_lib.TokenTargets(t.data_ptr(), 8, 1, IGN))
+        pol = C.byref(_lib.PolicyTerms(A.data_ptr(), 1, None, None, 0.2, 0.2, 0.0, 0))
+        top = C.byref(_lib.TeacherTop(ids.data_ptr(), tl.data_ptr(), K, 8, int(dtype == BF)))
+        torch.cuda.synchronize()
+        for off in range(8):
+            with torch.cuda.stream(stream):
+                st = stream.cuda_stream
+                ws = torch.empty(lib.mcb_token_loss_workspace_bytes(B, S), dtype=torch.uint8, device=cuda_device)
+                logp, lse, out = (torch.empty(B, S, device=cuda_device) for _ in range(3))
+                bufs = [torch.full((n + 40,), 7.0, dtype=dtype, device=cuda_device) for _ in range(3)]
+                at = [b[16 + off:].data_ptr() for b in bufs]
+                _lib.check(lib.mcb_token_logprob_fwd(rows, tt, logp.data_ptr(), lse.data_ptr(), None, st))
+                _lib.check(lib.mcb_token_logprob_bwd(rows, tt, logp.data_ptr(), lse.data_ptr(), A.data_ptr(), 1, at[0], st))
+                _lib.check(lib.mcb_policy_loss(rows, tt, pol, 0, logp.data_ptr(), out.data_ptr(), at[1], ws.data_ptr(), ws.numel(), st))
+                _lib.check(lib.mcb_distill_loss(rows, top, None, out.data_ptr(), at[2], ws.data_ptr(), ws.numel(), st))
+            stream.synchronize()
+            check_logp(logp, logp64)
+            for b, want, size in zip(bufs, (by_target, by_policy, by_teacher), (spread, spread * w.max(), parts)):
+                check_grad(b[16 + off:16 + off + n].view(B, S, V), want, 2 * size)
+                assert (b[:16 + off] == 7).all() and (b[16 + off + n:] == 7).all()
+
+
+@both
+@pytest.mark.parametrize("eps,average", [(0.0, False), (0.2, True)])
+def test_preference_loss_alone(cuda_device, dtype, eps, average):
+    """Without a gradient: the same loss and log-probabilities, bit for bit."""
+    for B, S, V in ((2, 3, 50), (6, 5, 8193), (4, 7, 50257)):
+        x, t, g = make(cuda_device, B, S, V, dtype, 26)
+        ref = torch.randn(B, device=cuda_device, generator=g)
+        opts = dict(beta=0.3, label_smoothing=eps, average_log_probs=average, ignore_index=IGN)
+        a, b = F.preference_loss(x, t, ref, **opts), F.preference_loss(x, t, ref, return_grad=True, **opts)
+        assert a.grad is None and torch.equal(a.loss, b.loss) and torch.equal(a.log_probs, b.log_probs)
+
+
+LONGEST = {BF: 655353, F32: 655357}   # columns of the longest row that the one-pass kernel takes
+
+
+@both
+@pytest.mark.parametrize("more", [0, 1])
+@pytest.mark.parametrize("lo", [0, 1])
+def test_longest_rows_of_one_pass(cuda_device, dtype, more, lo):
+    """Both sides of the border between the one-pass kernel and the one with three sweeps, from a 16-byte boundary and beside it; rows of
+    an odd length, so that each begins elsewhere."""
+    V, B, S = LONGEST[dtype] + more, 1, 4
+    x0, t, g = make(cuda_device, B, S, V, dtype, 27, keep=1.0)
+    flat = torch.empty(B * S * V + 1, dtype=dtype, device=cuda_device)
+    x = flat[lo:lo + B * S * V].view(B, S, V)
+    x.copy_(x0)
+    logp, _, p, kept = rows64(x, t)
+    A = torch.randn(B, S, device=cuda_device, generator=g)
+    out = F.policy_loss(x, t, A, return_grad=True)
+    check_logp(out.log_probs, logp)
+    wg, spread = grad64(p, t, kept, -A.double() / S)
+    check_grad(out.grad, wg, 2 * spread)
+    ids, tl = teacher(cuda_device, g, B, S, V, 9, dtype)
+    ids[0, :, 0], ids[0, :, 1] = 0, V - 1
+    ids[0, :, 2:] = 1 + ids[0, :, 2:] % (V - 2)
+    loss, grad = F.distillation_loss(x, ids, tl, return_grad=True)
+    q = torch.softmax(tl.double(), -1)
+    check_grad(grad, p.scatter_add(-1, ids, -q) / S, p.scatter_add(-1, ids, q) / S)
+    want = (q * (q.log() - p.gather(-1, ids).log())).sum(-1).mean()
+    assert abs(float(loss) - float(want)) <= 3e-5 * (1 + abs(float(want)) + float((q * q.log().abs()).sum(-1).mean()))
+    assert _lib.device_status() == 0
