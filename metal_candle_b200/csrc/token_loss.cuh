@@ -116,7 +116,7 @@ __device__ __forceinline__ TargetStats target_stats(float m, float s, float xt, 
     r.rest = __fdividef(odds, r.sum);
   } else {   // (NaN as well)
     r.top = m; r.sum = s + ex2(-d);
-    r.logp = (d < INFINITY ? -d * kLn2 : far_below(xt, m, k)) - logf(r.sum);
+    r.logp = d < INFINITY ? fmaf(-d, kLn2, -logf(r.sum)) : far_below(xt, m, k) - logf(r.sum);
     r.rest = __fdividef(s, r.sum);
   }
   return r;
