@@ -466,7 +466,8 @@ int mcb_cross_entropy_finish(const float* nll, const int32_t* count, float* loss
  * structs, read during the call; everything they point to is device memory.
  *
  * Logits [batch, seq, vocab] of MCB_F32 or MCB_BF16: rows of contiguous elements, any non-negative strides (in elements)
- * between them; vocab up to 2^30, batch * seq below 2^31.  y = logits / temperature throughout.  Gradients are dense
+ * between them (of a dimension of one: any number); vocab up to 2^30, batch * seq below 2^31.  A logit of NaN or +inf makes its
+ * position NaN.  y = logits / temperature throughout.  Gradients are dense
  * [batch * seq, vocab] of the logits' type, and may lie over dense logits (in place), or else apart from them; null: none is
  * computed. */
 typedef struct {

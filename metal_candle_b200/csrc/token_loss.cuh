@@ -249,7 +249,7 @@ struct RowPlan {
   double* partials;
 };
 
-// kUnit and kPolicy, rows of at most 256 vectors, each in the registers of a warp (token_stream.cu).
+// kUnit and kPolicy, rows of at most 256 vectors, each held by a warp (token_stream.cu).
 int launch_short_rows(int op, const RowArgs& a, const RowPlan& plan, int dtype, DeviceState* ds, cudaStream_t st, bool* taken);
 
 // The one-pass kernel (token_resident.cu), where it takes rows of this length: *taken says whether it did.

@@ -199,7 +199,7 @@ __device__ __forceinline__ void sweep_row(const T* x, int V, float k, int tid, i
 
 // Gradient: dx_j = c (1[j = t] - p_j).  Bound: HBM, one read and one write.  A block takes `piece` vectors of a row, all of them in
 // flight at once.  The rows are taken from the last to the first: what the statistics' kernel read last may still be in L2.
-// Not in place: other blocks of the row read the target's logit.
+// Not in place: other blocks of the row read the target's logit, or (sweep_row) all of them.
 // SHORT: a warp does (a row has one piece).
 template <typename T, bool SHORT>
 __global__ void __launch_bounds__(kThreads, SHORT ? 4 : 5)   // (the sweep that hardly any row takes would cost 16 registers, and with them a block an SM)
@@ -282,8 +282,9 @@ token_grad_stream_kernel(const GradArgs ga, int pieces, uint32_t parts) {
   if (edges) to[edge] = from_f32<T>(edge == te ? at_target : -c0 * ex2(fmaf(to_f32(base[edge]) - ref, a.k, add)));
 }
 
-// Short rows, statistics and gradient: a row in the registers of a warp, as it was read; its exponentials are taken twice (there
-// are few).  Any row may be written over.  20000 x 1000 bf16: a policy loss 41 us, by the one-pass kernel's warps, whose every row passes
+// Short rows, statistics and gradient: a row held by a warp, as it was read; its exponentials are taken twice (there are few).  (bf16: in
+// registers, but for some 20 words that spill.  float32: the search for the target's vector makes the row an array in local memory, 128
+// bytes a thread.)  Any row may be written over.  20000 x 1000 bf16: a policy loss 40 us, by the one-pass kernel's warps, whose every row passes
 // through a ring, barriers and a table, 64.  (Distillation is left to that one: its warps wait less for the teacher's entries.)
 constexpr int kShortBlocks = 3;      // blocks an SM, which take rows in turn
 template <typename T, int OP>
