@@ -55,12 +55,12 @@ __device__ __forceinline__ int64_t row_offset(const RowArgs& a, int64_t row) {  
 __device__ __forceinline__ int64_t load_target(const void* targets, int target_bytes, int64_t row) {
   return target_bytes == 8 ? static_cast<const int64_t*>(targets)[row] : static_cast<const int32_t*>(targets)[row];
 }
-__device__ __forceinline__ int judge_target(int64_t t, int has_ignore, int64_t ignore, int V) {
+__device__ __forceinline__ int kept_target(int64_t t, int has_ignore, int64_t ignore, int V) {
   if (t == -1 || (has_ignore && t == ignore)) return -1;
   return t >= 0 && t < V ? static_cast<int>(t) : -2;
 }
 __device__ __forceinline__ int read_target(const void* targets, int target_bytes, int has_ignore, int64_t ignore, int64_t row, int V) {
-  return judge_target(load_target(targets, target_bytes, row), has_ignore, ignore, V);
+  return kept_target(load_target(targets, target_bytes, row), has_ignore, ignore, V);
 }
 
 // 2^x, denormal results flushed to zero (one instruction, relative error about 2^-22)

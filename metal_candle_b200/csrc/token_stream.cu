@@ -304,7 +304,7 @@ token_short_kernel(const RowArgs a, const RowPlan plan) {
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kRows + warp, step = static_cast<int64_t>(gridDim.x) * kRows;
   int64_t next = row0 < a.M ? load_target(a.targets, a.target_bytes, row0) : -1;   // known before the row is asked for: left out, it is not read
   for (int64_t row = row0; row < a.M; row += step) {
-    const int tgt = judge_target(next, a.has_ignore, a.ignore, a.V);
+    const int tgt = kept_target(next, a.has_ignore, a.ignore, a.V);
     if (row + step < a.M) next = load_target(a.targets, a.target_bytes, row + step);
     const T* x = static_cast<const T*>(from_here(a.logits)) + row_offset(a, row);
     T* g = static_cast<T*>(a.grad) + row * a.V;
