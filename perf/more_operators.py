@@ -169,9 +169,15 @@ def prepare(case, seed):
         state.update(ids=ids, table=(0.02 * rand(V, case["dim"])).to(dt), dout=rand(M, case["dim"]).to(dt))
         return state
     sizes = _parts(case, case["numel"], case["tensors"], random.Random(case["numel"]))
-    flat = (rand(case["numel"]) * 0.01).to(dt)
-    out = torch.empty_like(flat)
-    return dict(case=case, flat=flat, grads=list(flat.split(sizes)), out_flat=out, out=list(out.split(sizes)))
+    grads = [t.clone() for t in (rand(case["numel"]) * 0.01).to(dt).split(sizes)]
+    out = torch.empty(case["numel"], dtype=dt, device=dev)   # the clipped gradients, one behind the other
+    state.update(grads=grads, out=out)
+    if own:
+        from metal_candle_b200 import training
+
+        # gradient buffers stay where they are from step to step, and so does what knows them
+        state["clipper"] = training.GradClipper(grads, out=list(out.split(sizes)))
+    return state
 
 
 # ---- the plain forms -----------------------------------------------------------------------------------------------------
@@ -252,16 +258,16 @@ def _run_plain(st):
         grad = torch.zeros(case["vocab"], case["dim"], device=ids.device)
         grad.index_add_(0, at, torch.where(kept[:, None], dout * case["scale"], torch.zeros((), device=ids.device)))
         return out, grad
-    g = st["flat"].float()
+    g = torch.cat(st["grads"]).float()
     norm = g.double().square().sum().sqrt().float().view(1)
-    st["out_flat"].copy_(g * (1.0 / (norm + 1e-6)).clamp_max(1.0))
-    return norm, st["out_flat"]
+    st["out"].copy_(g * (1.0 / (norm + 1e-6)).clamp_max(1.0))
+    return norm, st["out"]
 
 
 # ---- the framework's operators --------------------------------------------------------------------------------------------
 
 def _run_own(st):
-    from metal_candle_b200 import backend, training
+    from metal_candle_b200 import backend
 
     case = st["case"]
     kind = case["kind"]
@@ -279,7 +285,7 @@ def _run_own(st):
     if kind == "embedding":
         out = backend.embedding(st["ids"], st["table"], scale=case["scale"])
         return out, backend.embedding_backward(st["ids"], st["dout"], case["vocab"], scale=case["scale"])
-    return training.clip_grad_norm(st["grads"], 1.0, out=st["out"]), st["out_flat"]
+    return st["clipper"].clip(1.0), st["out"]
 
 
 def run(state):
@@ -353,6 +359,6 @@ def exact(case, seed):
         at = torch.where((st["ids"] >= 0) & (st["ids"] < V), st["ids"].long(), torch.full_like(st["ids"], V).long())
         grad = torch.zeros_like(table).index_put_((at,), st["dout"].double() * scale, accumulate=True)
         return table[at] * scale, grad[:V]
-    flat = st["flat"].double()
+    flat = torch.cat(st["grads"]).double()
     norm = torch.linalg.vector_norm(flat)
     return norm.view(1), flat * min(1.0, 1.0 / (float(norm) + 1e-6))
