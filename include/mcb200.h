@@ -280,6 +280,21 @@ int mcb_rmsnorm_bwd_ex(const void* x, const void* w, const void* dy, const void*
 int mcb_rmsnorm_bwd_noalloc(const void* x, const void* w, const void* dy, void* dx, float* dw, int accumulate,
                             int64_t rows, int64_t D, float eps, int dtype, void* stream);
 
+/* ---- layer norm ------------------------------------------------------------------------------ */
+
+/* y = (x - mean) / sqrt(var + eps) (* w) (+ b) over the last dimension, var the mean of the squared differences.  x, y [rows, D]
+ * dtype; w, b [D] dtype or null; mean, rstd [rows] float32 or null.  y may be x.  Any D.  Replaces LayerNormOp
+ * (src/backend/custom_ops.rs:826-1079), which takes the variance as E[x^2] - mean^2. */
+int mcb_layernorm_fwd(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, int64_t rows, int64_t D,
+                      float eps, int dtype, void* stream);
+/* Reverse pass from x alone (mean and rstd are taken again): dx [rows, D] dtype, plus dx_residual if not null (the gradient that reaches
+ * the same tensor along the residual connection); dw, db [D] float32 or null (overwritten unless accumulate).  dx may be dy or
+ * dx_residual.  Sums over rows in a fixed order. */
+size_t mcb_layernorm_bwd_workspace_bytes(int64_t rows, int64_t D);
+int mcb_layernorm_bwd(const void* x, const void* w, const void* dy, const void* dx_residual, void* dx, float* dw, float* db,
+                      int accumulate, int64_t rows, int64_t D, float eps, int dtype, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
 /* ---- softmax ------------------------------------------------------------------------------ */
 
 /* Replaces FusedSoftmaxOp / softmax_fused (src/backend/custom_ops.rs:644-824, kernels.metal:187-261)
@@ -350,6 +365,42 @@ int mcb_attention_causal_bwd_ragged(const void* q, const void* k, const void* v,
                                     int64_t seq, int64_t head_dim, float scale, int dtype, int64_t kv_heads,
                                     int o_token_major, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- attention under document and prefix masks, with capped scores and a distance bias ------------- */
+
+/* Several documents packed into one sequence must not see one another.  document_ids [batch, seq] (int32 or int64: id_bytes 4 or
+ * 8; null: one document): a document is a maximal run of equal, non-negative ids; negative ids are padding, which sees nothing and
+ * is seen by nothing.  A query sees the keys of its own document up to itself, and those of the document's prefix: its leading
+ * positions with prefix [batch, seq] (a byte each) not 0 (null: none; all ones: documents read in both directions).
+ * mcb_attention_mask turns both into per-position intervals and tile ranges once, in `mask` (16-byte aligned device memory of
+ * mcb_attention_mask_bytes, 0 for sizes that are not taken: batch up to 65535, batch * seq below 2^31), for every attention call on
+ * that batch, forward and backward.  The reference has no counterpart (its callers pass an additive mask,
+ * src/models/transformer.rs:269-273). */
+size_t mcb_attention_mask_bytes(int64_t batch, int64_t seq);
+int mcb_attention_mask(const void* document_ids, int id_bytes, const uint8_t* prefix, void* mask, size_t mask_bytes, int64_t batch,
+                       int64_t seq, void* stream);
+/* s = scale q.k; with softcap > 0: s = softcap tanh(s / softcap); with slopes: s -= slopes[head] |i - j|; o = softmax of s over the
+ * visible keys, times v.  A query that sees nothing, or whose every score is -inf, has o = 0, lse = -inf and no gradient; what lies at
+ * positions that a query does not see never reaches it, NaN included.  Layouts as in mcb_attention_causal_fwd_ex with nb = batch *
+ * kv_heads: q [nb, groups * seq, head_dim], k and v [nb, seq, head_dim], lse [nb, groups * seq] float32, o like q or (o_token_major)
+ * [batch * seq, kv_heads * groups * head_dim].  MCB_F32 or MCB_BF16, head_dim a multiple of 8 up to 128, any seq; bfloat16 with
+ * head_dim 64 runs on the tensor cores. */
+typedef struct {
+  const void* mask;        /* as mcb_attention_mask left it, for this batch and seq */
+  size_t mask_bytes;
+  const float* slopes;     /* [kv_heads * groups], device; or null */
+  int64_t batch, seq, kv_heads, groups, head_dim;
+  float scale, softcap;    /* softcap 0: none */
+  int32_t dtype, o_token_major;
+} mcb_masked_attention;
+int mcb_attention_masked_fwd(const mcb_masked_attention* call, const void* q, const void* k, const void* v, void* o, float* lse,
+                             void* stream);
+/* Gradients of the call above from its o and lse: dq like q, dk and dv like k (summed over the group); the slopes have none.
+ * workspace: mcb_attention_masked_workspace_bytes from a 1024-byte boundary. */
+size_t mcb_attention_masked_workspace_bytes(const mcb_masked_attention* call);
+int mcb_attention_masked_bwd(const mcb_masked_attention* call, const void* q, const void* k, const void* v, const void* o,
+                             const float* lse, const void* dout, void* dq, void* dk, void* dv, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
 /* ---- data-parallel exchange ------------------------------------------------------------------- */
 
 /* The reference trains on one device and has no communication layer; these calls are the one exchange step of the
@@ -402,11 +453,45 @@ typedef struct {
 int mcb_adamw_multi(const mcb_adamw_tensor* tensors, int n_tensors, float lr, float beta1, float beta2,
                     float eps, float weight_decay, float grad_scale, void* stream);
 
+/* ---- global gradient norm ---------------------------------------------------------------------- */
+
+/* A gradient of a list: n elements at g (n 0: skipped), MCB_F32 or MCB_BF16.  out receives the clipped gradient (null: in place). */
+typedef struct {
+  const void* g;
+  void* out;
+  int64_t n;
+  int32_t dtype;
+  int32_t pad_;
+} mcb_grad_tensor;
+/* norm[0] = sqrt of the sum of squares over all tensors (a HOST array), right over the whole range of float32; the same bits
+ * every time. */
+size_t mcb_grad_norm_workspace_bytes(int n_tensors);
+int mcb_grad_norm(const mcb_grad_tensor* tensors, int n_tensors, float* norm, void* workspace, size_t workspace_bytes, void* stream);
+/* out = g * min(1, max_norm / (norm + 1e-6)); norm[0], unless null, receives the norm before clipping.  max_norm inf never clips; a
+ * norm of NaN makes every element NaN.  No output may overlap another tensor, or its own gradient in part.  TrainingConfig carries
+ * max_grad_norm (src/training/trainer.rs:16-39), but nothing in the reference reads it. */
+int mcb_clip_grad_norm(const mcb_grad_tensor* tensors, int n_tensors, float max_norm, float* norm, void* workspace,
+                       size_t workspace_bytes, void* stream);
+/* mcb_adamw_multi with the gradients (times grad_scale) clipped so on the way: they stay as they are in memory.  workspace:
+ * mcb_grad_norm_workspace_bytes. */
+int mcb_adamw_multi_clipped(const mcb_adamw_tensor* tensors, int n_tensors, float lr, float beta1, float beta2, float eps,
+                            float weight_decay, float grad_scale, float max_norm, float* norm, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
 /* ---- element-wise frame of the Qwen-shaped training step ------------------------------------- */
 
 /* out[m,:] = table[ids[m],:]  (candle_nn::embedding, src/models/qwen.rs:189).  ids are int32. */
 int mcb_embedding_fwd(const int32_t* ids, const void* table, void* out, int64_t M, int64_t H, int64_t vocab,
                       int dtype, void* stream);
+/* out[m,:] = scale * table[ids[m],:]; an id outside [0, vocab) (padding) gives zeros.  ids int32 or int64 (id_bytes 4 or 8). */
+int mcb_embedding_scaled_fwd(const void* ids, int id_bytes, const void* table, void* out, int64_t M, int64_t H, int64_t vocab,
+                             float scale, int dtype, void* stream);
+/* Its table's gradient, for a table that is trained: dtable[v,:] = scale * sum of dout[m,:] over ids[m] = v, [vocab, H] float32 from a
+ * 16-byte boundary, written whole (accumulate: added to, where a token has the id).  dout [M, H] dtype.  Terms are summed in token
+ * order, in parts of 32: the same bits every time. */
+size_t mcb_embedding_bwd_workspace_bytes(int64_t M, int64_t H);
+int mcb_embedding_bwd(const void* ids, int id_bytes, const void* dout, float* dtable, int accumulate, int64_t M, int64_t H,
+                      int64_t vocab, float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 /* Rotary embedding (half-split, angle = position * theta^(-2i/d); src/models/transformer.rs:47-120)
  * fused with the [B,S,H,d] -> [B,H,S,d] transpose of Attention::forward (transformer.rs:255-257).
  * rotate = 0 only re-lays out (V).  inverse = 1 is the reverse pass: [B,H,S,d] -> [B,S,H,d] with the

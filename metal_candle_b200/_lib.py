@@ -88,6 +88,16 @@ class TeacherTop(C.Structure):
     _fields_ = [("ids", C.c_void_p), ("logits", C.c_void_p), ("top", C.c_int64), ("id_bytes", C.c_int32), ("dtype", C.c_int32)]
 
 
+class MaskedAttention(C.Structure):
+    _fields_ = [("mask", C.c_void_p), ("mask_bytes", C.c_size_t), ("slopes", C.c_void_p), ("batch", C.c_int64), ("seq", C.c_int64),
+                ("kv_heads", C.c_int64), ("groups", C.c_int64), ("head_dim", C.c_int64), ("scale", C.c_float), ("softcap", C.c_float),
+                ("dtype", C.c_int32), ("o_token_major", C.c_int32)]
+
+
+class GradTensor(C.Structure):
+    _fields_ = [("g", C.c_void_p), ("out", C.c_void_p), ("n", C.c_int64), ("dtype", C.c_int32), ("pad_", C.c_int32)]
+
+
 _vp, _i64, _i32, _f32, _sz = C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_size_t
 
 # name -> (restype, argtypes); every symbol include/mcb200.h declares
@@ -160,6 +170,21 @@ SIGNATURES = {
                                                _vp]),
     "mcb_attention_causal_bwd_ragged": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _f32, _i32,
                                                _i64, _i32, _vp, _sz, _vp]),
+    "mcb_attention_mask_bytes": (_sz, [_i64, _i64]),
+    "mcb_attention_mask": (_i32, [_vp, _i32, _vp, _vp, _sz, _i64, _i64, _vp]),
+    "mcb_attention_masked_fwd": (_i32, [C.POINTER(MaskedAttention), _vp, _vp, _vp, _vp, _vp, _vp]),
+    "mcb_attention_masked_workspace_bytes": (_sz, [C.POINTER(MaskedAttention)]),
+    "mcb_attention_masked_bwd": (_i32, [C.POINTER(MaskedAttention), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mcb_layernorm_fwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f32, _i32, _vp]),
+    "mcb_layernorm_bwd_workspace_bytes": (_sz, [_i64, _i64]),
+    "mcb_layernorm_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _f32, _i32, _vp, _sz, _vp]),
+    "mcb_grad_norm_workspace_bytes": (_sz, [_i32]),
+    "mcb_grad_norm": (_i32, [C.POINTER(GradTensor), _i32, _vp, _vp, _sz, _vp]),
+    "mcb_clip_grad_norm": (_i32, [C.POINTER(GradTensor), _i32, _f32, _vp, _vp, _sz, _vp]),
+    "mcb_adamw_multi_clipped": (_i32, [C.POINTER(AdamWTensor), _i32, _f32, _f32, _f32, _f32, _f32, _f32, _f32, _vp, _vp, _sz, _vp]),
+    "mcb_embedding_scaled_fwd": (_i32, [_vp, _i32, _vp, _vp, _i64, _i64, _i64, _f32, _i32, _vp]),
+    "mcb_embedding_bwd_workspace_bytes": (_sz, [_i64, _i64]),
+    "mcb_embedding_bwd": (_i32, [_vp, _i32, _vp, _vp, _i32, _i64, _i64, _i64, _f32, _i32, _vp, _sz, _vp]),
     "mcb_embedding_fwd": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp]),
     "mcb_rope_relayout": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _f32, _i32, _i32, _i32, _vp]),
     "mcb_rope_relayout_qkv": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _i64, _i32, _vp]),

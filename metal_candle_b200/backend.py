@@ -467,6 +467,199 @@ def _attention_backward(entry: str, q, k, v, o, lse, dout, groups: int, scale: f
 
 
 # ---------------------------------------------------------------------------------------------
+# attention under document and prefix masks
+# ---------------------------------------------------------------------------------------------
+
+def _on_device_of(t: torch.Tensor):
+    """A context that makes the tensor's device the current one (streams and launches go by it), or None where it is."""
+    if not t.is_cuda:
+        raise TrainingError("tensor is not on a CUDA device (this library has no CPU path)")
+    return None if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+
+
+def _same_device(like: torch.Tensor, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != like.device:
+            raise TrainingError(f"{name} is on {t.device}, expected {like.device}")
+
+
+class AttentionMask:
+    """What `attention_mask` returns: the intervals of positions that see one another in a batch of packed documents, on the
+    device, for every attention call on that batch."""
+    __slots__ = ("batch", "seq", "block")
+
+    def __init__(self, batch: int, seq: int, block: torch.Tensor):
+        self.batch, self.seq, self.block = batch, seq, block
+
+
+def attention_mask(document_ids: torch.Tensor | None = None, prefix: torch.Tensor | None = None, batch: int | None = None,
+                   seq: int | None = None, device=None) -> AttentionMask:
+    """Mask of a batch of packed documents.  document_ids [batch, seq] (int32 or int64): a document is a maximal run of equal,
+    non-negative ids; negative ids are padding, which sees nothing and is not seen.  A position sees its own document up to itself,
+    and the document's prefix: its leading positions with prefix [batch, seq] (bool or uint8) set.  prefix of all ones: documents
+    read in both directions.  Without document_ids a sequence is one document; without both, give batch, seq and device."""
+    given = document_ids if document_ids is not None else prefix
+    if given is not None:
+        if given.dim() != 2 or given.numel() == 0:
+            raise TrainingError(f"attention_mask: document_ids and prefix are [batch, seq], got {list(given.shape)}")
+        batch, seq = given.shape
+        device = given.device
+    elif batch is None or seq is None or device is None:
+        raise TrainingError("attention_mask: needs document_ids, prefix, or batch, seq and device")
+    if document_ids is not None and document_ids.dtype not in (torch.int32, torch.int64):
+        raise TrainingError(f"attention_mask: document_ids is {document_ids.dtype}, expected torch.int32 or torch.int64")
+    if prefix is not None:
+        if prefix.dtype not in (torch.bool, torch.uint8):
+            raise TrainingError(f"attention_mask: prefix is {prefix.dtype}, expected torch.bool or torch.uint8")
+        if prefix.shape != (batch, seq):
+            raise TrainingError(f"attention_mask: prefix must be [{batch}, {seq}], got {list(prefix.shape)}")
+        _same_device(given, prefix=prefix)
+    device = torch.device(device)
+    if device.type != "cuda":
+        raise TrainingError("attention_mask: needs a CUDA device (this library has no CPU path)")
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return attention_mask(document_ids, prefix, batch, seq, device)
+    ids = None if document_ids is None else document_ids.contiguous()
+    pre = None if prefix is None else prefix.contiguous()
+    lib = _lib.init(index)
+    nbytes = lib.mcb_attention_mask_bytes(batch, seq)
+    if nbytes == 0:
+        raise TrainingError(f"attention_mask: batch={batch} seq={seq} is not supported")
+    block = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    _lib.check(lib.mcb_attention_mask(_ptr(ids), 4 if ids is None else ids.element_size(), _ptr(pre), block.data_ptr(), nbytes, batch, seq,
+                                      _stream()))
+    return AttentionMask(batch, seq, block)
+
+
+def _masked_call(q, k, v, groups: int, scale: float, mask: AttentionMask, softcap: float, slopes, token_major: bool):
+    """The checked descriptor, and the slopes as the kernels read them (kept alive by the caller)."""
+    if k.dim() != 3 or q.dim() != 3:
+        raise TrainingError(f"masked attention: q [nb, groups*S, d] and k [nb, S, d] expected, got {list(q.shape)} and {list(k.shape)}")
+    nb, S, d = k.shape
+    if groups < 1 or q.shape != (nb, groups * S, d) or v.shape != k.shape:
+        raise TrainingError(f"masked attention: q {list(q.shape)}, k {list(k.shape)}, v {list(v.shape)} do not fit groups={groups}")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TrainingError(f"masked attention: q, k and v are {q.dtype}, {k.dtype} and {v.dtype}")
+    if not isinstance(mask, AttentionMask):
+        raise TrainingError("masked attention: mask must come from attention_mask")
+    if mask.seq != S or nb == 0 or nb % mask.batch != 0:
+        raise TrainingError(f"masked attention: a mask of {mask.batch} x {mask.seq} positions does not fit k {list(k.shape)}")
+    _require_cuda(q, k, v, slopes)
+    _same_device(q, k=k, v=v, slopes=slopes, mask=mask.block)
+    kv_heads = nb // mask.batch
+    if slopes is not None and (slopes.shape != (kv_heads * groups,) or slopes.dtype != torch.float32):
+        raise TrainingError(f"masked attention: slopes must be [{kv_heads * groups}] float32, got {list(slopes.shape)} {slopes.dtype}")
+    return _lib.MaskedAttention(mask.block.data_ptr(), mask.block.numel(), _ptr(slopes), mask.batch, S, kv_heads, groups, d, float(scale),
+                                float(softcap), _dtype_code(q), int(bool(token_major)))
+
+
+def attention_masked_forward(q, k, v, groups: int, scale: float, mask: AttentionMask, softcap: float = 0.0, slopes=None,
+                             token_major: bool = False):
+    """Grouped-query attention under `mask`: softmax over the visible keys of s = scale q.k, with softcap > 0 bent to softcap *
+    tanh(s / softcap), with slopes [query heads] float32 lowered by slopes[head] * |i - j|.  q [nb, groups*S, d] (row g*S + s),
+    k and v [nb, S, d], nb = batch * kv_heads; float32 or bfloat16, d a multiple of 8 up to 128.  Returns (o, lse [nb, groups*S]
+    float32); o like q, or token-major [batch*S, kv_heads*groups*d].  A position that sees nothing has o = 0 and lse = -inf."""
+    call = _masked_call(q, k, v, groups, scale, mask, softcap, slopes, token_major)
+    other = _on_device_of(q)
+    if other is not None:
+        with other:
+            return attention_masked_forward(q, k, v, groups, scale, mask, softcap, slopes, token_major)
+    nb, S, d = k.shape
+    o = torch.empty(mask.batch * S, nb // mask.batch * groups * d, dtype=q.dtype, device=q.device) if token_major else torch.empty_like(q)
+    lse = torch.empty(nb, groups * S, dtype=torch.float32, device=q.device)
+    _lib.check(_lib_for(q).mcb_attention_masked_fwd(call, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), _stream()))
+    return o, lse
+
+
+def attention_masked_backward(q, k, v, o, lse, dout, groups: int, scale: float, mask: AttentionMask, softcap: float = 0.0, slopes=None,
+                              token_major: bool = False):
+    """Gradients of `attention_masked_forward` with the same arguments, from its o and lse: (dq like q, dk and dv like k, summed over
+    the group).  The slopes are constants."""
+    call = _masked_call(q, k, v, groups, scale, mask, softcap, slopes, token_major)
+    nb, S, d = k.shape
+    want = (mask.batch * S, nb // mask.batch * groups * d) if token_major else tuple(q.shape)
+    if tuple(o.shape) != want or tuple(dout.shape) != want or o.dtype != q.dtype or dout.dtype != q.dtype:
+        raise TrainingError(f"masked attention backward: o {list(o.shape)} {o.dtype} / dout {list(dout.shape)} {dout.dtype}, expected {list(want)} {q.dtype}")
+    if tuple(lse.shape) != (nb, groups * S) or lse.dtype != torch.float32:
+        raise TrainingError(f"masked attention backward: lse {list(lse.shape)} {lse.dtype}, expected [{nb}, {groups * S}] float32")
+    _require_cuda(o, lse, dout)
+    _same_device(q, o=o, lse=lse, dout=dout)
+    other = _on_device_of(q)
+    if other is not None:
+        with other:
+            return attention_masked_backward(q, k, v, o, lse, dout, groups, scale, mask, softcap, slopes, token_major)
+    lib = _lib_for(q)
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    ws = workspace(q.device, lib.mcb_attention_masked_workspace_bytes(call))
+    _lib.check(lib.mcb_attention_masked_bwd(call, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+                                            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws.numel(), _stream()))
+    return dq, dk, dv
+
+
+# ---------------------------------------------------------------------------------------------
+# embedding lookup with a trained table
+# ---------------------------------------------------------------------------------------------
+
+def _check_ids(ids: torch.Tensor) -> None:
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TrainingError(f"embedding: ids are {ids.dtype}, expected torch.int32 or torch.int64")
+    if ids.numel() == 0:
+        raise TrainingError("embedding: empty ids")
+
+
+def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """`scale * table[ids]`: ids of any shape (int32 or int64), table [vocab, hidden].  An id outside the vocabulary (padding)
+    gives zeros."""
+    _check_ids(ids)
+    if table.dim() != 2 or table.numel() == 0:
+        raise TrainingError(f"embedding: table must be [vocab, hidden], got {list(table.shape)}")
+    dt = _dtype_code(table)
+    ids = ids.contiguous()
+    _require_cuda(ids, table)
+    _same_device(table, ids=ids)
+    other = _on_device_of(table)
+    if other is not None:
+        with other:
+            return embedding(ids, table, scale)
+    V, H = table.shape
+    out = torch.empty(*ids.shape, H, dtype=table.dtype, device=table.device)
+    _lib.check(_lib_for(table).mcb_embedding_scaled_fwd(ids.data_ptr(), ids.element_size(), table.data_ptr(), out.data_ptr(), ids.numel(), H, V,
+                                                        float(scale), dt, _stream()))
+    return out
+
+
+def embedding_backward(ids: torch.Tensor, dout: torch.Tensor, vocab: int, scale: float = 1.0, grad: torch.Tensor | None = None,
+                       accumulate: bool = False) -> torch.Tensor:
+    """Gradient of `embedding` towards its table: float32 [vocab, hidden], written whole, or with accumulate added to `grad`.  Terms
+    of a row are summed in token order: the same tokens give the same bits."""
+    _check_ids(ids)
+    if dout.dim() < 1 or dout.shape[:-1] != ids.shape or dout.shape[-1] == 0:
+        raise TrainingError(f"embedding_backward: dout {list(dout.shape)} does not fit ids {list(ids.shape)}")
+    dt = _dtype_code(dout)
+    H = dout.shape[-1]
+    ids = ids.contiguous()
+    if grad is not None and (grad.shape != (vocab, H) or grad.dtype != torch.float32):
+        raise TrainingError(f"embedding_backward: grad must be [{vocab}, {H}] float32, got {list(grad.shape)} {grad.dtype}")
+    if accumulate and grad is None:
+        raise TrainingError("embedding_backward: accumulate needs grad")
+    _require_cuda(ids, dout, grad)
+    _same_device(dout, ids=ids, grad=grad)
+    other = _on_device_of(dout)
+    if other is not None:
+        with other:
+            return embedding_backward(ids, dout, vocab, scale, grad, accumulate)
+    if grad is None:
+        grad = torch.empty(vocab, H, dtype=torch.float32, device=dout.device)
+    lib = _lib_for(dout)
+    ws = workspace(dout.device, lib.mcb_embedding_bwd_workspace_bytes(ids.numel(), H))
+    _lib.check(lib.mcb_embedding_bwd(ids.data_ptr(), ids.element_size(), dout.data_ptr(), grad.data_ptr(), int(bool(accumulate)), ids.numel(), H,
+                                     int(vocab), float(scale), dt, ws.data_ptr(), ws.numel(), _stream()))
+    return grad
+
+
+# ---------------------------------------------------------------------------------------------
 # RMSNorm
 # ---------------------------------------------------------------------------------------------
 
@@ -537,6 +730,79 @@ def rms_norm_backward(x, weight, dy, eps, need_dw=True, grad_w=None, accumulate=
                                        int(bool(accumulate)), rows, D, float(eps), _dtype_code(x), _ptr(ws), ws.numel(),
                                        _stream()))
     return dx, (grad_w if need_dw else None)
+
+
+# ---------------------------------------------------------------------------------------------
+# layer norm
+# ---------------------------------------------------------------------------------------------
+
+class LayerNormOp:
+    """LayerNormOp::new (src/backend/custom_ops.rs:826-1079): `(x - mean) / sqrt(var + eps)`."""
+
+    def __init__(self, eps: float):
+        self.eps = float(eps)
+
+    def name(self) -> str:
+        return "layer-norm"
+
+    def __call__(self, x):
+        return layer_norm_fused(x, eps=self.eps)
+
+
+def layer_norm_fused(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5,
+                     return_stats: bool = False):
+    """Layer norm over the last dimension, any rank, any size; weight and bias [D] of x's dtype.  With return_stats also the float32
+    mean and 1 / sqrt(var + eps) of every row."""
+    rows, D = _rows(x, "LayerNormOp")
+    dt = _dtype_code(x)
+    _require_cuda(x, weight, bias)
+    _same_device(x, weight=weight, bias=bias)
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and (t.shape != (D,) or t.dtype != x.dtype):
+            raise TrainingError(f"layer norm {name} must be [{D}] of {x.dtype}")
+    other = _on_device_of(x)
+    if other is not None:
+        with other:
+            return layer_norm_fused(x, weight, bias, eps, return_stats)
+    y = torch.empty_like(x)
+    mean, rstd = (torch.empty(rows, dtype=torch.float32, device=x.device) for _ in range(2)) if return_stats else (None, None)
+    _lib.check(_lib_for(x).mcb_layernorm_fwd(_ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _ptr(mean), _ptr(rstd), rows, D, float(eps), dt, _stream()))
+    return (y, mean, rstd) if return_stats else y
+
+
+def layer_norm_backward(x: torch.Tensor, weight: torch.Tensor | None, dy: torch.Tensor, eps: float = 1e-5, need_dw: bool = True,
+                        grad_w: torch.Tensor | None = None, grad_b: torch.Tensor | None = None, accumulate: bool = False,
+                        dx_residual: torch.Tensor | None = None):
+    """(dx, dw, db) of `layer_norm_fused`: dw and db float32 [D], summed over the rows in a fixed order (None without need_dw);
+    accumulate adds to grad_w and grad_b.  `dx_residual` (the gradient along the residual connection) is added to dx inside."""
+    rows, D = _rows(x, "layer_norm_backward")
+    dt = _dtype_code(x)
+    _require_cuda(x, weight, dy, grad_w, grad_b, dx_residual)
+    _same_device(x, weight=weight, dy=dy, grad_w=grad_w, grad_b=grad_b, dx_residual=dx_residual)
+    for name, t in (("dy", dy), ("dx_residual", dx_residual)):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise TrainingError(f"layer_norm_backward: {name} must be {list(x.shape)} of {x.dtype}, got {list(t.shape)} of {t.dtype}")
+    if weight is not None and (weight.shape != (D,) or weight.dtype != x.dtype):
+        raise TrainingError(f"layer norm weight must be [{D}] of {x.dtype}")
+    for name, t in (("grad_w", grad_w), ("grad_b", grad_b)):
+        if t is not None and (t.shape != (D,) or t.dtype != torch.float32):
+            raise TrainingError(f"layer_norm_backward: {name} must be [{D}] float32")
+    if accumulate and need_dw and (grad_w is None or grad_b is None):
+        raise TrainingError("layer_norm_backward: accumulate needs grad_w and grad_b")
+    other = _on_device_of(x)
+    if other is not None:
+        with other:
+            return layer_norm_backward(x, weight, dy, eps, need_dw, grad_w, grad_b, accumulate, dx_residual)
+    lib = _lib_for(x)
+    dx = torch.empty_like(x)
+    if need_dw:
+        grad_w = torch.empty(D, dtype=torch.float32, device=x.device) if grad_w is None else grad_w
+        grad_b = torch.empty(D, dtype=torch.float32, device=x.device) if grad_b is None else grad_b
+    ws = workspace(x.device, lib.mcb_layernorm_bwd_workspace_bytes(rows, D)) if need_dw else None
+    _lib.check(lib.mcb_layernorm_bwd(_ptr(x), _ptr(weight), _ptr(dy), _ptr(dx_residual), _ptr(dx), _ptr(grad_w) if need_dw else None,
+                                     _ptr(grad_b) if need_dw else None, int(bool(accumulate)), rows, D, float(eps), dt, _ptr(ws),
+                                     0 if ws is None else ws.numel(), _stream()))
+    return (dx, grad_w, grad_b) if need_dw else (dx, None, None)
 
 
 # ---------------------------------------------------------------------------------------------

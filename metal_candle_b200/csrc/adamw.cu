@@ -10,7 +10,7 @@
 // candle's scalar division is an affine by 1/rhs.
 #include <algorithm>
 
-#include "common.cuh"
+#include "grad_norm.cuh"
 
 namespace mcb {
 namespace {
@@ -51,9 +51,25 @@ __device__ __forceinline__ void adamw_one(float& p, float g, float& m, float& v,
   v = v_new;
 }
 
-template <int MAX>
+// Clipping by the global norm: every block adds up the partial sums of squares (grad_norm.cu) for itself, which saves a launch
+// and the clipped gradients' way to memory and back.
+struct AdamWClip {
+  const double* part;
+  int parts;
+  float max_norm;
+  float* norm;   // written by one block, or null
+};
+
+template <int MAX, bool CLIP>
 __global__ void __launch_bounds__(256) adamw_multi_kernel(const __grid_constant__ AdamWBatch<MAX> batch,
-                                                          const AdamWScalars s) {
+                                                          const AdamWScalars given, const AdamWClip clip) {
+  AdamWScalars s = given;
+  if constexpr (CLIP) {
+    __shared__ double sums[8];
+    const float norm = gnorm::norm_of(clip.part, clip.parts, sums) * fabsf(s.grad_scale);
+    s.grad_scale *= gnorm::clip_factor(norm, clip.max_norm);
+    if (clip.norm != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) clip.norm[0] = norm;
+  }
   const AdamWTensorDev& t = batch.t[blockIdx.y];
   const int64_t n = t.n;
   const bool vec = ((reinterpret_cast<uintptr_t>(t.p) | reinterpret_cast<uintptr_t>(t.g) |
@@ -119,7 +135,8 @@ bool any_overlap(const mcb_adamw_tensor* tensors, int n) {
 }
 
 template <int MAX>
-int launch_batch(const mcb_adamw_tensor* tensors, int cnt, float beta1, float beta2, const AdamWScalars& s, int sm_count, cudaStream_t st) {
+int launch_batch(const mcb_adamw_tensor* tensors, int cnt, float beta1, float beta2, const AdamWScalars& s, const AdamWClip& clip, int sm_count,
+                 cudaStream_t st) {
   AdamWBatch<MAX> batch;
   int64_t max_n = 0;
   for (int i = 0; i < cnt; ++i) {
@@ -138,7 +155,8 @@ int launch_batch(const mcb_adamw_tensor* tensors, int cnt, float beta1, float be
   const int64_t cap = static_cast<int64_t>(sm_count) * 8;
   if (gx * cnt > cap) gx = (cap + cnt - 1) / cnt;
   dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(cnt));
-  adamw_multi_kernel<MAX><<<grid, 256, 0, st>>>(batch, s);
+  if (clip.part != nullptr) adamw_multi_kernel<MAX, true><<<grid, 256, 0, st>>>(batch, s, clip);
+  else adamw_multi_kernel<MAX, false><<<grid, 256, 0, st>>>(batch, s, clip);
   MCB_CHECK_LAUNCH("adamw_multi");
   return MCB_OK;
 }
@@ -148,9 +166,10 @@ int launch_batch(const mcb_adamw_tensor* tensors, int cnt, float beta1, float be
 
 using namespace mcb;
 
-extern "C" int mcb_adamw_multi(const mcb_adamw_tensor* tensors, int n_tensors, float lr, float beta1, float beta2,
-                               float eps, float weight_decay, float grad_scale, void* stream) {
-  MCB_NVTX_RANGE("mcb_adamw_multi");
+namespace {
+// clip_norm: null, or what receives the norm while the gradients are clipped to max_norm
+int adamw_multi(const mcb_adamw_tensor* tensors, int n_tensors, float lr, float beta1, float beta2, float eps, float weight_decay, float grad_scale,
+                bool clipped, float max_norm, float* clip_norm, void* workspace, size_t workspace_bytes, void* stream) {
   if (n_tensors < 0) return fail(MCB_ERR_SHAPE, "adamw_multi: n_tensors=%d", n_tensors);
   if (n_tensors == 0) return MCB_OK;
   if (!tensors) return fail(MCB_ERR_NULL, "adamw_multi: tensors is null");
@@ -162,6 +181,11 @@ extern "C" int mcb_adamw_multi(const mcb_adamw_tensor* tensors, int n_tensors, f
   if (!(beta2 >= 0.0f && beta2 < 1.0f)) return fail(MCB_ERR_SHAPE, "beta2 must be in [0, 1), got %g", beta2);
   if (!(eps > 0.0f)) return fail(MCB_ERR_SHAPE, "epsilon must be positive");
   if (!(weight_decay >= 0.0f)) return fail(MCB_ERR_SHAPE, "weight decay must be non-negative");
+  if (clipped) {
+    if (!(max_norm >= 0.0f)) return fail(MCB_ERR_SHAPE, "adamw_multi: max_norm must not be negative, got %g", max_norm);
+    if (!workspace || workspace_bytes < gnorm::workspace_bytes(n_tensors) || !aligned16(workspace))
+      return fail(MCB_ERR_WORKSPACE, "adamw_multi: workspace of %zu bytes, 16-byte aligned, needed", gnorm::workspace_bytes(n_tensors));
+  }
   DeviceState* ds = current_device_state();
   if (!ds) return MCB_ERR_NOT_INIT;
   for (int i = 0; i < n_tensors; ++i) {
@@ -175,17 +199,50 @@ extern "C" int mcb_adamw_multi(const mcb_adamw_tensor* tensors, int n_tensors, f
   s.one_m_b1 = 1.0f - beta1; s.one_m_b2 = 1.0f - beta2;
   s.eps = eps; s.lr = lr; s.wd_lr = weight_decay * lr; s.grad_scale = grad_scale;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  AdamWClip clip = {};
+  if (clipped) {
+    clip.part = static_cast<const double*>(workspace);
+    clip.max_norm = max_norm;
+    clip.norm = clip_norm;
+    // as many descriptors at a time as a launch of the sums takes
+    mcb_grad_tensor grads[512];
+    for (int base = 0; base < n_tensors; base += 512) {
+      const int cnt = n_tensors - base < 512 ? n_tensors - base : 512;
+      for (int i = 0; i < cnt; ++i) {
+        grads[i] = mcb_grad_tensor{};
+        grads[i].g = tensors[base + i].g; grads[i].n = tensors[base + i].n; grads[i].dtype = MCB_F32;
+      }
+      int parts = 0;
+      if (int rc = gnorm::launch_squares(grads, cnt, static_cast<double*>(workspace) + clip.parts, &parts, ds, st, "adamw_multi")) return rc;
+      clip.parts += parts;
+    }
+  }
   for (int base = 0; base < n_tensors; base += kMaxTensors) {
     const int cnt = n_tensors - base < kMaxTensors ? n_tensors - base : kMaxTensors;
     if (any_overlap(tensors + base, cnt)) {
       // the update is one tensor after the other: whoever comes second reads what the first has written
       for (int i = 0; i < cnt; ++i)
-        if (int rc = launch_batch<kFewTensors>(tensors + base + i, 1, beta1, beta2, s, ds->sm_count, st)) return rc;
+        if (int rc = launch_batch<kFewTensors>(tensors + base + i, 1, beta1, beta2, s, clip, ds->sm_count, st)) return rc;
       continue;
     }
-    const int rc = cnt <= kFewTensors ? launch_batch<kFewTensors>(tensors + base, cnt, beta1, beta2, s, ds->sm_count, st)
-                                      : launch_batch<kMaxTensors>(tensors + base, cnt, beta1, beta2, s, ds->sm_count, st);
+    const int rc = cnt <= kFewTensors ? launch_batch<kFewTensors>(tensors + base, cnt, beta1, beta2, s, clip, ds->sm_count, st)
+                                      : launch_batch<kMaxTensors>(tensors + base, cnt, beta1, beta2, s, clip, ds->sm_count, st);
     if (rc != MCB_OK) return rc;
+    clip.norm = nullptr;   // the first launch has written it
   }
   return MCB_OK;
+}
+}  // namespace
+
+extern "C" int mcb_adamw_multi(const mcb_adamw_tensor* tensors, int n_tensors, float lr, float beta1, float beta2,
+                               float eps, float weight_decay, float grad_scale, void* stream) {
+  MCB_NVTX_RANGE("mcb_adamw_multi");
+  return adamw_multi(tensors, n_tensors, lr, beta1, beta2, eps, weight_decay, grad_scale, false, 0.0f, nullptr, nullptr, 0, stream);
+}
+
+extern "C" int mcb_adamw_multi_clipped(const mcb_adamw_tensor* tensors, int n_tensors, float lr, float beta1, float beta2, float eps,
+                                       float weight_decay, float grad_scale, float max_norm, float* norm, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+  MCB_NVTX_RANGE("mcb_adamw_multi_clipped");
+  return adamw_multi(tensors, n_tensors, lr, beta1, beta2, eps, weight_decay, grad_scale, true, max_norm, norm, workspace, workspace_bytes, stream);
 }

@@ -1,0 +1,433 @@
+// Embedding lookup with scaling, and the gradient of its table (beside mcb_embedding_fwd, whose table is frozen):
+//   out[i] = scale table[ids[i]];   grad[v] = scale sum of dout[i] over ids[i] = v
+// An id outside [0, vocab) (padding) gives a row of zeros and has no gradient.
+//
+// The gradient goes by sorted tokens: the ids are sorted once with their positions (stable, so a row's terms stay in token order), then
+// every run of equal ids is one sum, held in registers and written once.  Nothing uses floating-point atomics: the same
+// tokens give the same bits, and a token that comes a thousand times costs no more than a thousand different ones.
+//   1. sort (one cluster): radix sort of ceil(log2(vocab + 1)) bits, up to 9 a pass.  A warp owns consecutive tokens; within 32 of them
+//      equal digits are ranked by match; counts of digits go from warp to block to cluster through shared memory.  The other blocks of
+//      the launch write the table's zeros meanwhile (not with accumulate): 0.54 GB for 151936 x 896, which hides the sort.
+//   2. sums: a tile of 32 sorted tokens by as many threads as the columns take; a run that ends inside its tile is written out, one
+//      that goes on leaves its part.  3. The tile where such a run begins adds up the parts, in order.
+// HBM-bound by the table's gradient (float32, written whole) where it is not accumulated.
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace mcb {
+namespace embed {
+namespace {
+
+constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32, kDigits = 512, kTile = 32, kThreads = 128;
+constexpr uint32_t kFull = 0xffffffffu;
+
+// ---- forward -----------------------------------------------------------------------------------------------------------
+// `tx` threads share a row (16 bytes, or one element, at a time), kThreads / tx rows to a block.
+template <typename T, typename I, int N>
+__global__ void __launch_bounds__(kThreads) embed_fwd_kernel(const I* ids, const T* table, T* out, int64_t M, int64_t H, int64_t vocab, float scale, int tx) {
+  grid_launch_dependents();
+  grid_dependency_wait();
+  ids = from_here(ids);
+  table = from_here(table);
+  const int x = threadIdx.x % tx, y = threadIdx.x / tx, rows = kThreads / tx;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * rows + y; row < M; row += static_cast<int64_t>(gridDim.x) * rows) {
+    const int64_t id = static_cast<int64_t>(ids[row]);
+    const bool have = id >= 0 && id < vocab;
+    const T* src = table + (have ? id : 0) * H;
+    for (int64_t c = N * static_cast<int64_t>(x); c < H; c += N * tx) {
+      if constexpr (N == 1) {
+        out[row * H + c] = have ? from_f32<T>(to_f32(src[c]) * scale) : from_f32<T>(0.0f);
+      } else {
+        Vec16<T> v;
+        float f[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] = 0.0f;
+        if (have) {
+          v.raw = *reinterpret_cast<const decltype(v.raw)*>(src + c);
+          v.to_float(f);
+#pragma unroll
+          for (int e = 0; e < N; ++e) f[e] *= scale;
+        }
+        v.from_float(f);
+        *reinterpret_cast<decltype(v.raw)*>(out + row * H + c) = v.raw;
+      }
+    }
+  }
+}
+
+// ---- sort ----------------------------------------------------------------------------------------------------------------
+struct SortParams {
+  const void* ids;
+  uint32_t *key[2], *pos[2];   // the result of pass p is in buffer p & 1
+  float* zero;                 // the table's gradient, or null
+  int64_t zero_n;
+  int64_t vocab;
+  int M, passes, digit_bits;
+};
+
+template <typename I>
+__device__ __forceinline__ uint32_t key_of(const SortParams& p, int pass, int i) {
+  if (pass > 0) return __ldcg(p.key[(pass - 1) & 1] + i);
+  const int64_t id = static_cast<int64_t>(static_cast<const I*>(p.ids)[i]);
+  return id >= 0 && id < p.vocab ? static_cast<uint32_t>(id) : static_cast<uint32_t>(p.vocab);   // the others behind all
+}
+
+template <typename I>
+__global__ void __launch_bounds__(kSortThreads) sort_kernel(const __grid_constant__ SortParams p) {
+  __shared__ uint32_t hist[kSortWarps][kDigits];   // of a warp: counts, then where its next token of a digit goes
+  __shared__ uint32_t total[kDigits];              // of the block; read by the others of the cluster
+  __shared__ uint32_t scan[kSortThreads / 32];
+  cg::cluster_group cl = cg::this_cluster();
+  const int C = static_cast<int>(cl.num_blocks()), rank = static_cast<int>(cl.block_rank());
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  if (blockIdx.x >= static_cast<unsigned>(C)) {
+    // zeros, 16 bytes a store (the start is aligned: checked on the host; the last few elements one by one)
+    const int64_t n4 = p.zero_n >> 2, step = static_cast<int64_t>(gridDim.x - C) * kSortThreads;
+    const int64_t first = static_cast<int64_t>(blockIdx.x - C) * kSortThreads + threadIdx.x;
+    for (int64_t i = first; i < n4; i += step) reinterpret_cast<float4*>(p.zero)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int64_t i = (n4 << 2) + first; i < p.zero_n; i += step) p.zero[i] = 0.0f;
+    return;
+  }
+  const int warps = C * kSortWarps;
+  const int per = ((p.M + warps - 1) / warps + 31) & ~31;   // tokens of a warp
+  const int64_t begin = static_cast<int64_t>(rank * kSortWarps + warp) * per;
+  const int end = static_cast<int>(begin + per < p.M ? begin + per : p.M);
+  for (int pass = 0; pass < p.passes; ++pass) {
+    const int shift = pass * p.digit_bits;
+    const uint32_t mask = (1u << p.digit_bits) - 1u;
+    for (int d = lane; d < kDigits; d += 32) hist[warp][d] = 0;
+    __syncwarp();
+    for (int64_t i0 = begin; i0 < end; i0 += 32) {
+      const int i = static_cast<int>(i0) + lane;
+      const uint32_t have = __ballot_sync(kFull, i < end);
+      if (i < end) {
+        const uint32_t d = (key_of<I>(p, pass, i) >> shift) & mask;
+        const uint32_t peers = __match_any_sync(have, d);
+        if (lane == __ffs(peers) - 1) hist[warp][d] += __popc(peers);
+      }
+      __syncwarp();
+    }
+    __syncthreads();
+    // counts of the warps before, within the block; kDigits == kSortThreads: one digit a thread
+    uint32_t sum = 0;
+    for (int w = 0; w < kSortWarps; ++w) {
+      const uint32_t n = hist[w][threadIdx.x];
+      hist[w][threadIdx.x] = sum;
+      sum += n;
+    }
+    total[threadIdx.x] = sum;
+    cl.sync();
+    uint32_t all = 0, before = 0;   // tokens of this digit in the cluster, and in the blocks before this one
+    for (int r = 0; r < C; ++r) {
+      const uint32_t n = *cl.map_shared_rank(&total[threadIdx.x], r);
+      if (r < rank) before += n;
+      all += n;
+    }
+    // exclusive sum over the digits
+    uint32_t inc = all;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(kFull, inc, o);
+      if (lane >= o) inc += v;
+    }
+    if (lane == 31) scan[warp] = inc;
+    __syncthreads();
+    uint32_t base = inc - all + before;
+    for (int w = 0; w < warp; ++w) base += scan[w];
+    for (int w = 0; w < kSortWarps; ++w) hist[w][threadIdx.x] += base;
+    __syncthreads();
+    uint32_t *key = p.key[pass & 1], *pos = p.pos[pass & 1];
+    for (int64_t i0 = begin; i0 < end; i0 += 32) {
+      const int i = static_cast<int>(i0) + lane;
+      const uint32_t have = __ballot_sync(kFull, i < end);
+      if (i < end) {
+        const uint32_t k = key_of<I>(p, pass, i), d = (k >> shift) & mask;
+        const uint32_t at = pass > 0 ? __ldcg(p.pos[(pass - 1) & 1] + i) : static_cast<uint32_t>(i);
+        const uint32_t peers = __match_any_sync(have, d);
+        const uint32_t to = hist[warp][d] + __popc(peers & ((1u << lane) - 1u));
+        __syncwarp(have);
+        if (lane == __ffs(peers) - 1) hist[warp][d] += __popc(peers);
+        key[to] = k;
+        pos[to] = at;
+      }
+      __syncwarp();
+    }
+    __threadfence();
+    cl.sync();   // the pass is in memory, and nobody reads this block's totals any more
+  }
+}
+
+// ---- sums ------------------------------------------------------------------------------------------------------------------
+struct SumParams {
+  const uint32_t *key, *pos;
+  const void* dout;
+  float* grad;
+  float* part;      // [tiles][2][H]: of the tile's first run where it began before, of its last where it goes on (a run that
+                    // does both is in the first)
+  int64_t H;
+  int64_t vocab;
+  int M, tiles, tx, accumulate;
+  float scale;
+};
+
+template <int N>
+__device__ __forceinline__ void put(float* p, const float (&v)[N]) {
+  if constexpr (N == 1) {
+    p[0] = v[0];
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; e += 4) *reinterpret_cast<float4*>(p + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+  }
+}
+template <int N>
+__device__ __forceinline__ void get_add(const float* p, float (&v)[N]) {
+  if constexpr (N == 1) {
+    v[0] += p[0];
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; e += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(p + e);
+      v[e] += x.x; v[e + 1] += x.y; v[e + 2] += x.z; v[e + 3] += x.w;
+    }
+  }
+}
+template <int N>
+__device__ __forceinline__ void finish(const SumParams& p, uint32_t id, int64_t c, float (&v)[N]) {
+  float* g = p.grad + static_cast<int64_t>(id) * p.H + c;
+#pragma unroll
+  for (int e = 0; e < N; ++e) v[e] *= p.scale;
+  if (p.accumulate) get_add<N>(g, v);
+  put<N>(g, v);
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(kThreads) sum_kernel(const __grid_constant__ SumParams p) {
+  __shared__ uint32_t s_key[kThreads][kTile + 2], s_pos[kThreads][kTile];   // by tile of the block (at most kThreads of them)
+  const int x = threadIdx.x % p.tx, y = threadIdx.x / p.tx, ty = kThreads / p.tx;
+  const int t = blockIdx.x * ty + y;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int64_t i0 = static_cast<int64_t>(t) * kTile;
+  const int n = t < p.tiles ? static_cast<int>(i0 + kTile < p.M ? kTile : p.M - i0) : 0;
+  const uint32_t none = static_cast<uint32_t>(p.vocab);
+  // keys of the tile with one on either side
+  for (int i = x; i < n + 2 && n > 0; i += p.tx) {
+    const int64_t at = i0 + i - 1;
+    s_key[y][i] = at >= 0 && at < p.M ? __ldcg(p.key + at) : none;
+    if (i >= 1 && i <= n) s_pos[y][i - 1] = __ldcg(p.pos + at);
+  }
+  __syncthreads();
+  if (n == 0) return;
+  const int64_t c = N * (static_cast<int64_t>(blockIdx.y) * p.tx + x);
+  if (c >= p.H) return;
+  const T* dout = static_cast<const T*>(p.dout) + c;
+  const bool began = s_key[y][0] == s_key[y][1], goes_on = s_key[y][n] == s_key[y][n + 1] && i0 + n < p.M;
+  float acc[N] = {};
+  bool first = true;   // still in the tile's first run
+  constexpr int kAhead = 8;
+  for (int b = 0; b < n; b += kAhead) {
+    float v[kAhead][N];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[k][e] = 0.0f;
+      if (b + k < n && s_key[y][b + k + 1] != none) {
+        const T* src = dout + static_cast<int64_t>(s_pos[y][b + k]) * p.H;
+        if constexpr (N == 1) {
+          v[k][0] = to_f32(*src);
+        } else {
+          Vec16<T> r;
+          r.raw = *reinterpret_cast<const decltype(r.raw)*>(src);
+          r.to_float(v[k]);
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = b + k;
+      if (i >= n) break;
+      const uint32_t id = s_key[y][i + 1];
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] += v[k][e];
+      const bool last = i == n - 1;
+      if (!last && s_key[y][i + 2] == id) continue;
+      // the run ends here, or goes on behind the tile
+      if (id != none) {
+        if (first && began && i0 > 0) put<N>(p.part + (2 * static_cast<int64_t>(t)) * p.H + c, acc);
+        else if (last && goes_on) put<N>(p.part + (2 * static_cast<int64_t>(t) + 1) * p.H + c, acc);
+        else finish<N>(p, id, c, acc);
+      }
+      first = false;
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] = 0.0f;
+    }
+  }
+}
+
+// The runs that go on behind the tile in which they begin.
+template <int N>
+__global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ SumParams p) {
+  const int x = threadIdx.x % p.tx, y = threadIdx.x / p.tx, ty = kThreads / p.tx;
+  const int t = blockIdx.x * ty + y;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  if (t >= p.tiles) return;
+  const int64_t i0 = static_cast<int64_t>(t) * kTile, i1 = i0 + kTile;
+  if (i1 >= p.M) return;
+  const uint32_t id = __ldcg(p.key + i1 - 1);
+  if (id >= static_cast<uint32_t>(p.vocab) || __ldcg(p.key + i1) != id) return;
+  if (i0 > 0 && __ldcg(p.key + i0 - 1) == id) return;   // it began in a tile before
+  const int64_t c = N * (static_cast<int64_t>(blockIdx.y) * p.tx + x);
+  if (c >= p.H) return;
+  // last token of the run
+  int64_t lo = i1, hi = p.M - 1;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi + 1) >> 1;
+    if (__ldcg(p.key + mid) == id) lo = mid;
+    else hi = mid - 1;
+  }
+  float acc[N] = {};
+  get_add<N>(p.part + (2 * static_cast<int64_t>(t) + 1) * p.H + c, acc);
+#pragma unroll 4
+  for (int64_t q = t + 1; q <= lo / kTile; ++q) get_add<N>(p.part + 2 * q * p.H + c, acc);
+  finish<N>(p, id, c, acc);
+}
+
+inline size_t up256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
+inline int64_t tiles_of(int64_t M) { return (M + kTile - 1) / kTile; }
+// threads that share a row of `n` pieces: a power of two up to kThreads
+inline int row_threads(int64_t n) {
+  int t = 1;
+  while (t < kThreads && t < n) t <<= 1;
+  return t;
+}
+
+template <typename I>
+int launch_sort(const SortParams& p, int sms, cudaStream_t st) {
+  // few tokens: a block alone ranks them sooner than eight that wait for one another three times a pass
+  const int C = p.M <= 1024 ? 1 : 8;
+  int64_t fill = p.zero == nullptr ? 0 : (p.zero_n / 4 + kSortThreads * 4 - 1) / (kSortThreads * 4) + 1;
+  if (fill > 4 * sms) fill = 4 * sms;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(C + (fill + C - 1) / C * C));
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = chained_launch() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = C; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr; cfg.numAttrs = 2;
+  MCB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, sort_kernel<I>, p));
+  MCB_CHECK_LAUNCH("embedding_sort");
+  return MCB_OK;
+}
+
+template <typename T, int N>
+int launch_sums(SumParams& p, cudaStream_t st) {
+  p.tx = row_threads((p.H + N - 1) / N);
+  const int ty = kThreads / p.tx;
+  const int64_t cols = (p.H + static_cast<int64_t>(N) * p.tx - 1) / (static_cast<int64_t>(N) * p.tx);
+  if (cols > 65535) return fail(MCB_ERR_SHAPE, "embedding_bwd: H=%lld", (long long)p.H);
+  const dim3 grid(static_cast<unsigned>((p.tiles + ty - 1) / ty), static_cast<unsigned>(cols));
+  MCB_CHECK_CUDA(launch_kernel(sum_kernel<T, N>, grid, dim3(kThreads), 0, st, chained_launch(), p));
+  MCB_CHECK_LAUNCH("embedding_sum");
+  if (p.tiles > 1) {
+    MCB_CHECK_CUDA(launch_kernel(join_kernel<N>, grid, dim3(kThreads), 0, st, chained_launch(), p));
+    MCB_CHECK_LAUNCH("embedding_join");
+  }
+  return MCB_OK;
+}
+
+int check(const char* who, int id_bytes, int64_t M, int64_t H, int64_t vocab, float scale, int dtype) {
+  if (dtype != MCB_F32 && dtype != MCB_BF16) return fail(MCB_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
+  if (id_bytes != 4 && id_bytes != 8) return fail(MCB_ERR_UNSUPPORTED, "%s: ids of %d bytes (4 or 8)", who, id_bytes);
+  if (M <= 0 || M > 0x3fffffff || H <= 0 || H > 0x7fffff || vocab <= 0 || vocab > 0x3fffffff)
+    return fail(MCB_ERR_SHAPE, "%s: M=%lld H=%lld vocab=%lld", who, (long long)M, (long long)H, (long long)vocab);
+  if (!(scale - scale == 0.0f)) return fail(MCB_ERR_SHAPE, "%s: scale is not finite", who);
+  return MCB_OK;
+}
+
+template <typename T, typename I>
+int launch_fwd(const void* ids, const void* table, void* out, int64_t M, int64_t H, int64_t vocab, float scale, int sms, cudaStream_t st) {
+  constexpr int N = Vec16<T>::N;
+  const bool vec = H % N == 0 && aligned16(table) && aligned16(out);
+  const int tx = row_threads(vec ? H / N : H);
+  const int64_t want = (M + kThreads / tx - 1) / (kThreads / tx), most = 16ll * sms;
+  const dim3 grid(static_cast<unsigned>(want < most ? want : most));
+  if (vec)
+    MCB_CHECK_CUDA(launch_kernel(embed_fwd_kernel<T, I, N>, grid, dim3(kThreads), 0, st, chained_launch(), static_cast<const I*>(ids),
+                                 static_cast<const T*>(table), static_cast<T*>(out), M, H, vocab, scale, tx));
+  else
+    MCB_CHECK_CUDA(launch_kernel(embed_fwd_kernel<T, I, 1>, grid, dim3(kThreads), 0, st, chained_launch(), static_cast<const I*>(ids),
+                                 static_cast<const T*>(table), static_cast<T*>(out), M, H, vocab, scale, tx));
+  MCB_CHECK_LAUNCH("embedding_scaled_fwd");
+  return MCB_OK;
+}
+
+}  // namespace
+}  // namespace embed
+}  // namespace mcb
+
+using namespace mcb;
+
+extern "C" int mcb_embedding_scaled_fwd(const void* ids, int id_bytes, const void* table, void* out, int64_t M, int64_t H, int64_t vocab,
+                                        float scale, int dtype, void* stream) {
+  MCB_NVTX_RANGE("mcb_embedding_scaled_fwd");
+  if (!ids || !table || !out) return fail(MCB_ERR_NULL, "embedding_scaled_fwd: null pointer");
+  if (int rc = embed::check("embedding_scaled_fwd", id_bytes, M, H, vocab, scale, dtype)) return rc;
+  DeviceState* ds = current_device_state();
+  if (!ds) return MCB_ERR_NOT_INIT;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == MCB_F32)
+    return id_bytes == 4 ? embed::launch_fwd<float, int32_t>(ids, table, out, M, H, vocab, scale, ds->sm_count, st)
+                         : embed::launch_fwd<float, int64_t>(ids, table, out, M, H, vocab, scale, ds->sm_count, st);
+  return id_bytes == 4 ? embed::launch_fwd<__nv_bfloat16, int32_t>(ids, table, out, M, H, vocab, scale, ds->sm_count, st)
+                       : embed::launch_fwd<__nv_bfloat16, int64_t>(ids, table, out, M, H, vocab, scale, ds->sm_count, st);
+}
+
+extern "C" size_t mcb_embedding_bwd_workspace_bytes(int64_t M, int64_t H) {
+  if (M <= 0 || H <= 0 || M > 0x3fffffff || H > 0x7fffff) return 0;
+  return 4 * embed::up256(static_cast<size_t>(M) * 4) + static_cast<size_t>(embed::tiles_of(M)) * 2 * H * 4;
+}
+
+extern "C" int mcb_embedding_bwd(const void* ids, int id_bytes, const void* dout, float* dtable, int accumulate, int64_t M, int64_t H,
+                                 int64_t vocab, float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  MCB_NVTX_RANGE("mcb_embedding_bwd");
+  if (!ids || !dout || !dtable) return fail(MCB_ERR_NULL, "embedding_bwd: null pointer");
+  if (int rc = embed::check("embedding_bwd", id_bytes, M, H, vocab, scale, dtype)) return rc;
+  if (!aligned16(dtable)) return fail(MCB_ERR_ALIGN, "embedding_bwd: the table's gradient is not 16-byte aligned");
+  if (!workspace || workspace_bytes < mcb_embedding_bwd_workspace_bytes(M, H) || !aligned16(workspace))
+    return fail(MCB_ERR_WORKSPACE, "embedding_bwd: workspace of %zu bytes, 16-byte aligned, needed", mcb_embedding_bwd_workspace_bytes(M, H));
+  DeviceState* ds = current_device_state();
+  if (!ds) return MCB_ERR_NOT_INIT;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  uint8_t* w = static_cast<uint8_t*>(workspace);
+  const size_t list = embed::up256(static_cast<size_t>(M) * 4);
+  embed::SortParams s = {};
+  s.ids = ids;
+  for (int i = 0; i < 2; ++i) {
+    s.key[i] = reinterpret_cast<uint32_t*>(w + 2 * i * list);
+    s.pos[i] = reinterpret_cast<uint32_t*>(w + (2 * i + 1) * list);
+  }
+  s.zero = accumulate ? nullptr : dtable;
+  s.zero_n = vocab * H; s.vocab = vocab; s.M = static_cast<int>(M);
+  int bits = 1;
+  while ((vocab >> bits) != 0) ++bits;   // of vocab itself, which stands for the ids that count for nothing
+  s.passes = (bits + 8) / 9;
+  s.digit_bits = (bits + s.passes - 1) / s.passes;
+  if (int rc = id_bytes == 4 ? embed::launch_sort<int32_t>(s, ds->sm_count, st) : embed::launch_sort<int64_t>(s, ds->sm_count, st)) return rc;
+  embed::SumParams p = {};
+  p.key = s.key[(s.passes - 1) & 1]; p.pos = s.pos[(s.passes - 1) & 1];
+  p.dout = dout; p.grad = dtable; p.part = reinterpret_cast<float*>(w + 4 * list);
+  p.H = H; p.vocab = vocab; p.M = static_cast<int>(M); p.tiles = static_cast<int>(embed::tiles_of(M)); p.accumulate = accumulate; p.scale = scale;
+  const int n = dtype == MCB_F32 ? 4 : 8;
+  const bool vec = H % n == 0 && aligned16(dout);
+  if (dtype == MCB_F32) return vec ? embed::launch_sums<float, 4>(p, st) : embed::launch_sums<float, 1>(p, st);
+  return vec ? embed::launch_sums<__nv_bfloat16, 8>(p, st) : embed::launch_sums<__nv_bfloat16, 1>(p, st);
+}

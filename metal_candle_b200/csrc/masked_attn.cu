@@ -1,0 +1,499 @@
+// Attention under document / prefix masks, with a score cap and a distance bias, and its gradients:
+//   s = scale q.k;  s = cap tanh(s / cap);  s -= slope |i - j|;  o = sum over visible j of softmax(s) v
+//   P = exp(s - lse);  dv = P^T do;  dS = P (do v^T - do.o) (1 - tanh^2);  dq = scale dS k;  dk = scale dS^T q
+// The entry points, and kernels on CUDA cores for float32 (the validation path) and for bfloat16 heads of other sizes than 64,
+// which flash_attn.cu takes to the tensor cores.
+//
+// CUDA-core kernels: 64 x 64 tiles, 256 threads, a thread has rows ty + 16 i and columns tx + 16 j of a product (four of each, so that
+// one 16-byte shared load of a row serves four multiply-adds in each of four columns).  Tiles are float32 rows of D + 4 elements: the
+// four extra put the sixteen rows that a half warp reads on different banks for every D that is a multiple of 8.  One pass over the
+// keys that some row of the tile sees, with the running maximum and sum; nothing of size seq x seq is stored and no sum uses
+// atomics.  The backward pass is a kernel by query tiles (dq, and delta and lse for the other) and one by key tiles (dk, dv).
+#include "masked_attn.cuh"
+
+namespace mcb {
+namespace mattn {
+namespace {
+
+constexpr int kB = 64, kThreads = 256, kLdP = 68;
+
+__host__ __device__ constexpr int tile_floats(int d) { return kB * (d + 4); }
+inline size_t smem_fwd(int d) { return (3 * tile_floats(d) + kB * kLdP) * sizeof(float); }
+inline size_t smem_dq(int d) { return (4 * tile_floats(d) + kB * kLdP) * sizeof(float); }
+inline size_t smem_dkv(int d) { return (4 * tile_floats(d) + 2 * kB * kLdP) * sizeof(float); }
+
+// rows [first, first + 64) of a [.., S, D] plane as float32; `step` elements between rows; rows outside [0, S) are zeros
+template <typename T>
+__device__ __forceinline__ void load_tile(float* dst, const T* plane, int64_t step, int first, int S, int D) {
+  const int per = D / 4;
+  for (int i = threadIdx.x; i < kB * per; i += kThreads) {
+    const int r = i / per, c = i % per * 4;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (first + r < S) {
+      const T* s = plane + (first + r) * step + c;
+      if constexpr (sizeof(T) == 4) {
+        v = *reinterpret_cast<const float4*>(s);
+      } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(s);
+        v = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+      }
+    }
+    *reinterpret_cast<float4*>(dst + r * (D + 4) + c) = v;
+  }
+}
+
+// acc[i][j] = sum_k a[ty + 16 i][k] b[tx + 16 j][k]
+__device__ __forceinline__ void mul_nt(float (&acc)[4][4], const float* a, const float* b, int D, int ty, int tx) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+  const int ld = D + 4;
+  for (int k = 0; k < D; k += 4) {
+    float4 x[4], y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = *reinterpret_cast<const float4*>(a + (ty + 16 * i) * ld + k);
+      y[i] = *reinterpret_cast<const float4*>(b + (tx + 16 * i) * ld + k);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        acc[i][j] = fmaf(x[i].x, y[j].x, acc[i][j]);
+        acc[i][j] = fmaf(x[i].y, y[j].y, acc[i][j]);
+        acc[i][j] = fmaf(x[i].z, y[j].z, acc[i][j]);
+        acc[i][j] = fmaf(x[i].w, y[j].w, acc[i][j]);
+      }
+  }
+}
+
+// acc[i][jj] += sum_k p[ty + 16 i][k] v[k][4 (tx + 16 jj) ..]
+template <int DV>
+__device__ __forceinline__ void mul_nn(float4 (&acc)[4][DV], const float* p, const float* v, int D, int ty, int tx) {
+  const int ld = D + 4;
+#pragma unroll 4
+  for (int k = 0; k < kB; k += 4) {
+    float4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(p + (ty + 16 * i) * kLdP + k);
+#pragma unroll
+    for (int jj = 0; jj < DV; ++jj) {
+      const int c = 4 * (tx + 16 * jj);
+      if (c >= D) continue;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        const float4 y = *reinterpret_cast<const float4*>(v + (k + kk) * ld + c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float f = kk == 0 ? x[i].x : kk == 1 ? x[i].y : kk == 2 ? x[i].z : x[i].w;
+          acc[i][jj].x = fmaf(f, y.x, acc[i][jj].x);
+          acc[i][jj].y = fmaf(f, y.y, acc[i][jj].y);
+          acc[i][jj].z = fmaf(f, y.z, acc[i][jj].z);
+          acc[i][jj].w = fmaf(f, y.w, acc[i][jj].w);
+        }
+      }
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float4 v) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = v;
+  } else {
+    __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+  }
+}
+// whether the four are finite: x - x is 0 for those and NaN for the others
+__device__ __forceinline__ bool finite4(float4 v) { return (v.x - v.x) + (v.y - v.y) + (v.z - v.z) + (v.w - v.w) == 0.0f; }
+// over the sixteen lanes that share a row
+__device__ __forceinline__ float row_max(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float row_sum(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// A block's item: half of one of the mask's tiles, the longest tiles first, and a head.
+struct Item {
+  int b, first, head;
+};
+__device__ __forceinline__ Item item_of(const Call& c, const int* order, int heads) {
+  const int tiles = static_cast<int>(amask::tiles_of(c.S));
+  const int half = blockIdx.x / heads, t = order[half >> 1];
+  Item w;
+  w.head = blockIdx.x % heads;
+  w.b = t / tiles;
+  w.first = t % tiles * amask::kTile + (half & 1) * kB;
+  return w;
+}
+// The intervals of the tile's rows into shared memory, and the positions that any of them covers.  All threads.
+__device__ __forceinline__ int2 load_ranges(int2* rows, int* ends, const int2* all, const Call& c, const Item& w) {
+  if (threadIdx.x == 0) { ends[0] = 0x7fffffff; ends[1] = 0; }
+  __syncthreads();
+  if (threadIdx.x < kB) {
+    const int s = w.first + threadIdx.x;
+    const int2 r = s < c.S ? all[static_cast<int64_t>(w.b) * c.S + s] : make_int2(0, 0);
+    rows[threadIdx.x] = r;
+    if (r.x < r.y) { atomicMin(&ends[0], r.x); atomicMax(&ends[1], r.y); }
+  }
+  __syncthreads();
+  return make_int2(ends[0], ends[1]);
+}
+
+template <typename T, int DV>
+__global__ void __launch_bounds__(kThreads) masked_fwd_kernel(const __grid_constant__ Call c) {
+  extern __shared__ float4 smem4[];
+  __shared__ int2 rows[kB];
+  __shared__ int ends[2], bad[kB];
+  float* sQ = reinterpret_cast<float*>(smem4);
+  float* sK = sQ + tile_floats(c.D);
+  float* sV = sK + tile_floats(c.D);
+  float* sP = sV + tile_floats(c.D);
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const Item w = item_of(c, c.mask.qorder, c.Hk * c.G);
+  if (w.first >= c.S) return;
+  const int hk = w.head / c.G, g = w.head % c.G;
+  if (threadIdx.x < kB) bad[threadIdx.x] = 0;
+  const int2 range = load_ranges(rows, ends, c.mask.rows, c, w);
+  load_tile(sQ, static_cast<const T*>(c.q) + q_row(c, w.b, hk, g, 0) * c.D, c.D, w.first, c.S, c.D);
+  const float slope2 = c.slopes ? c.slopes[w.head] * kLog2e : 0.0f;
+  float m[4], l[4];
+  float4 acc[4][DV] = {};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { m[i] = kNoScore; l[i] = 0.0f; }
+  for (int j0 = range.x; j0 < range.y; j0 += kB) {
+    __syncthreads();
+    load_tile(sK, static_cast<const T*>(c.k) + k_row(c, w.b, hk, 0) * c.D, c.D, j0, c.S, c.D);
+    load_tile(sV, static_cast<const T*>(c.v) + k_row(c, w.b, hk, 0) * c.D, c.D, j0, c.S, c.D);
+    __syncthreads();
+    float s[4][4];
+    mul_nt(s, sQ, sK, c.D, ty, tx);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int2 sees = rows[ty + 16 * i];
+      const int qpos = w.first + ty + 16 * i;
+      float top = kNoScore;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = j0 + tx + 16 * j;
+        float bent;
+        s[i][j] = key >= sees.x && key < sees.y ? score2(c, s[i][j], slope2, abs(qpos - key), bent) : -INFINITY;
+        top = fmaxf(top, s[i][j]);
+      }
+      top = fmaxf(row_max(top), m[i]);
+      const float old = exp2f(m[i] - top);
+      m[i] = top;
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float p = exp2f(s[i][j] - top);
+        sum += p;
+        sP[(ty + 16 * i) * kLdP + tx + 16 * j] = p;
+      }
+      l[i] = fmaf(l[i], old, row_sum(sum));
+#pragma unroll
+      for (int jj = 0; jj < DV; ++jj) {
+        acc[i][jj].x *= old; acc[i][jj].y *= old; acc[i][jj].z *= old; acc[i][jj].w *= old;
+      }
+    }
+    __syncthreads();
+    mul_nn<DV>(acc, sP, sV, c.D, ty, tx);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int s = w.first + ty + 16 * i;
+    if (s >= c.S) continue;
+    const bool none = l[i] == 0.0f;
+    const float inv = none ? 0.0f : 1.0f / l[i];
+    T* out = static_cast<T*>(c.o) + o_at(c, w.b, hk, g, s);
+#pragma unroll
+    for (int jj = 0; jj < DV; ++jj) {
+      const int col = 4 * (tx + 16 * jj);
+      if (col >= c.D) continue;
+      float4 v = acc[i][jj];
+      v = none ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+      if (!finite4(v)) bad[ty + 16 * i] = 1;
+      store4(out + col, v);
+    }
+    if (c.lse != nullptr && tx == 0) c.lse[q_row(c, w.b, hk, g, s)] = none ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
+  }
+  __syncthreads();
+  for (int r = threadIdx.x >> 5; r < kB; r += kThreads / 32)
+    if (bad[r]) fwd_row<T>(c, w.b, hk, g, w.first + r);
+}
+
+template <typename T, int DV>
+__global__ void __launch_bounds__(kThreads) masked_dq_kernel(const __grid_constant__ Call c) {
+  extern __shared__ float4 smem4[];
+  __shared__ int2 rows[kB];
+  __shared__ int ends[2], bad[kB];
+  __shared__ float s_lse2[kB], s_delta[kB];
+  float* sQ = reinterpret_cast<float*>(smem4);
+  float* sO = sQ + tile_floats(c.D);   // d o
+  float* sK = sO + tile_floats(c.D);
+  float* sV = sK + tile_floats(c.D);
+  float* sS = sV + tile_floats(c.D);
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const Item w = item_of(c, c.mask.qorder, c.Hk * c.G);
+  if (w.first >= c.S) return;
+  const int hk = w.head / c.G, g = w.head % c.G;
+  if (threadIdx.x < kB) bad[threadIdx.x] = 0;
+  const int2 range = load_ranges(rows, ends, c.mask.rows, c, w);
+  const int64_t o0 = o_at(c, w.b, hk, g, 0), ostep = c.o_tok ? static_cast<int64_t>(c.Hk) * c.G * c.D : c.D;
+  load_tile(sQ, static_cast<const T*>(c.q) + q_row(c, w.b, hk, g, 0) * c.D, c.D, w.first, c.S, c.D);
+  load_tile(sO, static_cast<const T*>(c.dout) + o0, ostep, w.first, c.S, c.D);
+  load_tile(sK, static_cast<const T*>(c.o_in) + o0, ostep, w.first, c.S, c.D);
+  __syncthreads();
+  const int64_t pitch = amask::tiles_of(c.S) * amask::kTile;
+  for (int r = threadIdx.x >> 5; r < kB; r += kThreads / 32) {
+    float d = 0.0f;
+    for (int e = threadIdx.x & 31; e < c.D; e += 32) d = fmaf(sO[r * (c.D + 4) + e], sK[r * (c.D + 4) + e], d);
+    d = warp_sum(d);
+    if ((threadIdx.x & 31) == 0) {
+      const int s = w.first + r;
+      float lse2 = INFINITY;   // of a row that sees nothing: P = 0
+      if (s < c.S && rows[r].x < rows[r].y) {
+        const float v = c.lse[q_row(c, w.b, hk, g, s)];
+        if (v != -INFINITY) lse2 = v * kLog2e;
+      }
+      s_lse2[r] = lse2;
+      s_delta[r] = d;
+      const int64_t at = ((static_cast<int64_t>(w.b) * c.Hk + hk) * c.G + g) * pitch + s;
+      c.ndelta[at] = -d;
+      c.nlse2[at] = -lse2;
+    }
+  }
+  const float slope2 = c.slopes ? c.slopes[w.head] * kLog2e : 0.0f;
+  float4 acc[4][DV] = {};
+  for (int j0 = range.x; j0 < range.y; j0 += kB) {
+    __syncthreads();
+    load_tile(sK, static_cast<const T*>(c.k) + k_row(c, w.b, hk, 0) * c.D, c.D, j0, c.S, c.D);
+    load_tile(sV, static_cast<const T*>(c.v) + k_row(c, w.b, hk, 0) * c.D, c.D, j0, c.S, c.D);
+    __syncthreads();
+    float s[4][4], dp[4][4];
+    mul_nt(s, sQ, sK, c.D, ty, tx);
+    mul_nt(dp, sO, sV, c.D, ty, tx);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = ty + 16 * i;
+      const int2 sees = rows[r];
+      const float lse2 = s_lse2[r], delta = s_delta[r];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = j0 + tx + 16 * j;
+        float p, ds = 0.0f;
+        if (key >= sees.x && key < sees.y) ds = pair_ds(c, s[i][j], dp[i][j], slope2, abs(w.first + r - key), lse2, delta, p);
+        sS[r * kLdP + tx + 16 * j] = ds;
+      }
+    }
+    __syncthreads();
+    mul_nn<DV>(acc, sS, sK, c.D, ty, tx);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int s = w.first + ty + 16 * i;
+    if (s >= c.S) continue;
+    T* out = static_cast<T*>(c.dq) + q_row(c, w.b, hk, g, s) * c.D;
+#pragma unroll
+    for (int jj = 0; jj < DV; ++jj) {
+      const int col = 4 * (tx + 16 * jj);
+      if (col >= c.D) continue;
+      float4 v = acc[i][jj];
+      v = make_float4(v.x * c.scale, v.y * c.scale, v.z * c.scale, v.w * c.scale);
+      if (!finite4(v)) bad[ty + 16 * i] = 1;
+      store4(out + col, v);
+    }
+  }
+  __syncthreads();
+  for (int r = threadIdx.x >> 5; r < kB; r += kThreads / 32)
+    if (bad[r]) dq_row<T>(c, w.b, hk, g, w.first + r);
+}
+
+template <typename T, int DV>
+__global__ void __launch_bounds__(kThreads) masked_dkv_kernel(const __grid_constant__ Call c) {
+  extern __shared__ float4 smem4[];
+  __shared__ int2 rows[kB];
+  __shared__ int ends[2], bad[kB];
+  float* sK = reinterpret_cast<float*>(smem4);
+  float* sV = sK + tile_floats(c.D);
+  float* sQ = sV + tile_floats(c.D);
+  float* sO = sQ + tile_floats(c.D);
+  float* sP = sO + tile_floats(c.D);
+  float* sS = sP + kB * kLdP;
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const Item w = item_of(c, c.mask.korder, c.Hk);
+  if (w.first >= c.S) return;
+  const int hk = w.head;
+  if (threadIdx.x < kB) bad[threadIdx.x] = 0;
+  const int2 range = load_ranges(rows, ends, c.mask.keys, c, w);
+  load_tile(sK, static_cast<const T*>(c.k) + k_row(c, w.b, hk, 0) * c.D, c.D, w.first, c.S, c.D);
+  load_tile(sV, static_cast<const T*>(c.v) + k_row(c, w.b, hk, 0) * c.D, c.D, w.first, c.S, c.D);
+  const int64_t pitch = amask::tiles_of(c.S) * amask::kTile, ostep = c.o_tok ? static_cast<int64_t>(c.Hk) * c.G * c.D : c.D;
+  float4 gk[4][DV] = {}, gv[4][DV] = {};
+  for (int g = 0; g < c.G; ++g) {
+    const float slope2 = c.slopes ? c.slopes[hk * c.G + g] * kLog2e : 0.0f;
+    const int64_t srow = ((static_cast<int64_t>(w.b) * c.Hk + hk) * c.G + g) * pitch;
+    for (int i0 = range.x; i0 < range.y; i0 += kB) {
+      __syncthreads();
+      load_tile(sQ, static_cast<const T*>(c.q) + q_row(c, w.b, hk, g, 0) * c.D, c.D, i0, c.S, c.D);
+      load_tile(sO, static_cast<const T*>(c.dout) + o_at(c, w.b, hk, g, 0), ostep, i0, c.S, c.D);
+      __syncthreads();
+      float s[4][4], dp[4][4], lse2[4], delta[4];   // rows: keys, columns: queries
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int qpos = i0 + tx + 16 * j;
+        lse2[j] = qpos < c.S ? -c.nlse2[srow + qpos] : INFINITY;
+        delta[j] = qpos < c.S ? -c.ndelta[srow + qpos] : 0.0f;
+      }
+      mul_nt(s, sK, sQ, c.D, ty, tx);
+      mul_nt(dp, sV, sO, c.D, ty, tx);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = ty + 16 * i;
+        const int2 seen = rows[r];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int qpos = i0 + tx + 16 * j;
+          float p = 0.0f, ds = 0.0f;
+          if (qpos >= seen.x && qpos < seen.y && lse2[j] != INFINITY)
+            ds = pair_ds(c, s[i][j], dp[i][j], slope2, abs(qpos - w.first - r), lse2[j], delta[j], p);
+          sP[r * kLdP + tx + 16 * j] = p;
+          sS[r * kLdP + tx + 16 * j] = ds;
+        }
+      }
+      __syncthreads();
+      mul_nn<DV>(gv, sP, sO, c.D, ty, tx);
+      mul_nn<DV>(gk, sS, sQ, c.D, ty, tx);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int s = w.first + ty + 16 * i;
+    if (s >= c.S) continue;
+    const int64_t at = k_row(c, w.b, hk, s) * c.D;
+#pragma unroll
+    for (int jj = 0; jj < DV; ++jj) {
+      const int col = 4 * (tx + 16 * jj);
+      if (col >= c.D) continue;
+      float4 k = gk[i][jj];
+      k = make_float4(k.x * c.scale, k.y * c.scale, k.z * c.scale, k.w * c.scale);
+      if (!finite4(k) || !finite4(gv[i][jj])) bad[ty + 16 * i] = 1;
+      store4(static_cast<T*>(c.dk) + at + col, k);
+      store4(static_cast<T*>(c.dv) + at + col, gv[i][jj]);
+    }
+  }
+  __syncthreads();
+  for (int r = threadIdx.x >> 5; r < kB; r += kThreads / 32)
+    if (bad[r]) dkv_row<T>(c, w.b, hk, w.first + r);
+}
+
+int launch_one(void (*kernel)(Call), const char* name, int64_t blocks, size_t smem, const Call& c, cudaStream_t st) {
+  if (blocks > 0x7fffffffll) return fail(MCB_ERR_SHAPE, "masked attention: %lld blocks", (long long)blocks);
+  MCB_CHECK_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  MCB_CHECK_CUDA(launch_kernel(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), smem, st, chained_launch(), c));
+  MCB_CHECK_LAUNCH(name);
+  return MCB_OK;
+}
+template <typename T>
+int launch_fwd(const Call& c, cudaStream_t st) {
+  const int64_t halves = 2 * amask::tiles_of(c.S) * c.B;
+  return launch_one(c.D <= 64 ? masked_fwd_kernel<T, 1> : masked_fwd_kernel<T, 2>, "masked_fwd_kernel", halves * c.Hk * c.G, smem_fwd(c.D), c, st);
+}
+template <typename T>
+int launch_bwd(const Call& c, cudaStream_t st) {
+  const int64_t halves = 2 * amask::tiles_of(c.S) * c.B;
+  if (int rc = launch_one(c.D <= 64 ? masked_dq_kernel<T, 1> : masked_dq_kernel<T, 2>, "masked_dq_kernel", halves * c.Hk * c.G, smem_dq(c.D), c, st)) return rc;
+  return launch_one(c.D <= 64 ? masked_dkv_kernel<T, 1> : masked_dkv_kernel<T, 2>, "masked_dkv_kernel", halves * c.Hk, smem_dkv(c.D), c, st);
+}
+
+inline size_t up1k(size_t v) { return (v + 1023) & ~static_cast<size_t>(1023); }
+size_t stat_bytes(const mcb_masked_attention* a) {
+  return up1k(static_cast<size_t>(a->batch) * a->kv_heads * a->groups * amask::tiles_of(a->seq) * amask::kTile * 4);
+}
+
+int fill(Call& c, const mcb_masked_attention* a, const char* who) {
+  if (!a) return fail(MCB_ERR_NULL, "%s: the call is null", who);
+  if (!a->mask) return fail(MCB_ERR_NULL, "%s: mask is null", who);
+  if (a->dtype != MCB_F32 && a->dtype != MCB_BF16) return fail(MCB_ERR_UNSUPPORTED, "%s: dtype %d", who, a->dtype);
+  const size_t need = mcb_attention_mask_bytes(a->batch, a->seq);
+  if (need == 0) return fail(MCB_ERR_SHAPE, "%s: batch=%lld seq=%lld", who, (long long)a->batch, (long long)a->seq);
+  if (a->mask_bytes < need) return fail(MCB_ERR_SHAPE, "%s: a mask of %zu bytes is none of %lld x %lld positions", who, a->mask_bytes, (long long)a->batch, (long long)a->seq);
+  if (a->head_dim < 8 || a->head_dim > 128 || a->head_dim % 8 != 0)
+    return fail(MCB_ERR_UNSUPPORTED, "%s: head dimension %lld (multiples of 8 up to 128)", who, (long long)a->head_dim);
+  // rows and work items are counted in 32 bits, tiles of 128 positions and up to 8 blocks to an item
+  if (a->kv_heads <= 0 || a->groups <= 0 || a->kv_heads > 0x7fffffff || a->groups > 0x7fffffff / a->kv_heads ||
+      a->batch * amask::tiles_of(a->seq) > 0x07ffffffll / (a->kv_heads * a->groups))
+    return fail(MCB_ERR_SHAPE, "%s: batch=%lld kv_heads=%lld groups=%lld seq=%lld", who, (long long)a->batch, (long long)a->kv_heads, (long long)a->groups, (long long)a->seq);
+  if (!(a->scale - a->scale == 0.0f)) return fail(MCB_ERR_SHAPE, "%s: scale is not finite", who);
+  if (!(a->softcap >= 0.0f && a->softcap - a->softcap == 0.0f)) return fail(MCB_ERR_SHAPE, "%s: softcap must be 0 (none) or positive and finite", who);
+  if (!aligned16(a->mask) || (reinterpret_cast<uintptr_t>(a->slopes) & 3) != 0) return fail(MCB_ERR_ALIGN, "%s: alignment of the mask or the slopes", who);
+  c = Call{};
+  c.mask = amask::view(a->mask, a->batch, a->seq);
+  c.slopes = a->slopes;
+  c.B = static_cast<int>(a->batch); c.S = static_cast<int>(a->seq); c.Hk = static_cast<int>(a->kv_heads);
+  c.G = static_cast<int>(a->groups); c.D = static_cast<int>(a->head_dim);
+  c.o_tok = a->o_token_major != 0;
+  c.scale = a->scale; c.cap = a->softcap;
+  return MCB_OK;
+}
+
+}  // namespace
+}  // namespace mattn
+}  // namespace mcb
+
+using namespace mcb;
+
+extern "C" int mcb_attention_masked_fwd(const mcb_masked_attention* a, const void* q, const void* k, const void* v, void* o, float* lse,
+                                        void* stream) {
+  MCB_NVTX_RANGE("mcb_attention_masked_fwd");
+  mattn::Call c;
+  if (int rc = mattn::fill(c, a, "attention_masked_fwd")) return rc;
+  if (!q || !k || !v || !o) return fail(MCB_ERR_NULL, "attention_masked_fwd: q, k, v or o is null");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o)) return fail(MCB_ERR_ALIGN, "attention_masked_fwd: 16-byte alignment");
+  DeviceState* ds = current_device_state();
+  if (!ds) return MCB_ERR_NOT_INIT;
+  c.q = q; c.k = k; c.v = v; c.o = o; c.lse = lse; c.status = ds->status_word;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return a->dtype == MCB_F32 ? mattn::launch_fwd<float>(c, st) : mattn::launch_fwd<__nv_bfloat16>(c, st);
+}
+
+extern "C" size_t mcb_attention_masked_workspace_bytes(const mcb_masked_attention* a) {
+  mattn::Call c;
+  if (mattn::fill(c, a, "attention_masked_workspace_bytes") != MCB_OK) return 0;
+  return 2 * mattn::stat_bytes(a);
+}
+
+extern "C" int mcb_attention_masked_bwd(const mcb_masked_attention* a, const void* q, const void* k, const void* v, const void* o,
+                                        const float* lse, const void* dout, void* dq, void* dk, void* dv, void* workspace,
+                                        size_t workspace_bytes, void* stream) {
+  MCB_NVTX_RANGE("mcb_attention_masked_bwd");
+  mattn::Call c;
+  if (int rc = mattn::fill(c, a, "attention_masked_bwd")) return rc;
+  if (!q || !k || !v || !o || !lse || !dout || !dq || !dk || !dv) return fail(MCB_ERR_NULL, "attention_masked_bwd: a required pointer is null");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv))
+    return fail(MCB_ERR_ALIGN, "attention_masked_bwd: 16-byte alignment");
+  const size_t stat = mattn::stat_bytes(a);
+  if (!workspace || workspace_bytes < 2 * stat || (reinterpret_cast<uintptr_t>(workspace) & 1023u) != 0)
+    return fail(MCB_ERR_WORKSPACE, "attention_masked_bwd: workspace of %zu bytes, 1024-byte aligned, needed", 2 * stat);
+  DeviceState* ds = current_device_state();
+  if (!ds) return MCB_ERR_NOT_INIT;
+  c.q = q; c.k = k; c.v = v; c.o_in = o; c.lse = const_cast<float*>(lse); c.dout = dout; c.dq = dq; c.dk = dk; c.dv = dv;
+  c.ndelta = static_cast<float*>(workspace);
+  c.nlse2 = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + stat);
+  c.status = ds->status_word;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return a->dtype == MCB_F32 ? mattn::launch_bwd<float>(c, st) : mattn::launch_bwd<__nv_bfloat16>(c, st);
+}

@@ -25,6 +25,7 @@ TYPES = {
     "mcb_qwen_weights": "mcb_qwen_weights", "mcb_qwen_adapter_entry": "mcb_qwen_adapter_entry",
     "mcb_qwen_layer_call": "mcb_qwen_layer_call", "uint8_t": "u8", "mcb_token_logits": "mcb_token_logits",
     "mcb_token_targets": "mcb_token_targets", "mcb_policy_terms": "mcb_policy_terms", "mcb_teacher_top": "mcb_teacher_top",
+    "mcb_masked_attention": "mcb_masked_attention", "mcb_grad_tensor": "mcb_grad_tensor",
 }
 
 
@@ -238,6 +239,35 @@ def render(consts, funcs) -> str:
         "    pub top: i64,",
         "    pub id_bytes: i32,",
         "    pub dtype: i32,",
+        "}",
+        "",
+        "/// A call of attention under a document / prefix mask.",
+        "#[repr(C)]",
+        "#[derive(Debug, Clone, Copy)]",
+        "pub struct mcb_masked_attention {",
+        "    pub mask: *const c_void,",
+        "    pub mask_bytes: usize,",
+        "    pub slopes: *const f32,",
+        "    pub batch: i64,",
+        "    pub seq: i64,",
+        "    pub kv_heads: i64,",
+        "    pub groups: i64,",
+        "    pub head_dim: i64,",
+        "    pub scale: f32,",
+        "    pub softcap: f32,",
+        "    pub dtype: i32,",
+        "    pub o_token_major: i32,",
+        "}",
+        "",
+        "/// One gradient of a list whose global norm is taken.",
+        "#[repr(C)]",
+        "#[derive(Debug, Clone, Copy)]",
+        "pub struct mcb_grad_tensor {",
+        "    pub g: *const c_void,",
+        "    pub out: *mut c_void,",
+        "    pub n: i64,",
+        "    pub dtype: i32,",
+        "    pub pad_: i32,",
         "}",
         "",
         "/// Opaque training-step engine (`mcb_qwen_*`).",

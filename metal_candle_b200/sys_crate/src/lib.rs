@@ -180,6 +180,35 @@ pub struct mcb_teacher_top {
     pub dtype: i32,
 }
 
+/// A call of attention under a document / prefix mask.
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct mcb_masked_attention {
+    pub mask: *const c_void,
+    pub mask_bytes: usize,
+    pub slopes: *const f32,
+    pub batch: i64,
+    pub seq: i64,
+    pub kv_heads: i64,
+    pub groups: i64,
+    pub head_dim: i64,
+    pub scale: f32,
+    pub softcap: f32,
+    pub dtype: i32,
+    pub o_token_major: i32,
+}
+
+/// One gradient of a list whose global norm is taken.
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct mcb_grad_tensor {
+    pub g: *const c_void,
+    pub out: *mut c_void,
+    pub n: i64,
+    pub dtype: i32,
+    pub pad_: i32,
+}
+
 /// Opaque training-step engine (`mcb_qwen_*`).
 #[repr(C)]
 pub struct mcb_qwen {
@@ -231,6 +260,9 @@ extern "C" {
     pub fn mcb_rmsnorm_bwd(x: *const c_void, w: *const c_void, dy: *const c_void, dx: *mut c_void, dw: *mut f32, accumulate: c_int, rows: i64, D: i64, eps: f32, dtype: c_int, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn mcb_rmsnorm_bwd_ex(x: *const c_void, w: *const c_void, dy: *const c_void, dx_residual: *const c_void, dx: *mut c_void, dw: *mut f32, accumulate: c_int, rows: i64, D: i64, eps: f32, dtype: c_int, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn mcb_rmsnorm_bwd_noalloc(x: *const c_void, w: *const c_void, dy: *const c_void, dx: *mut c_void, dw: *mut f32, accumulate: c_int, rows: i64, D: i64, eps: f32, dtype: c_int, stream: *mut c_void) -> c_int;
+    pub fn mcb_layernorm_fwd(x: *const c_void, w: *const c_void, b: *const c_void, y: *mut c_void, mean: *mut f32, rstd: *mut f32, rows: i64, D: i64, eps: f32, dtype: c_int, stream: *mut c_void) -> c_int;
+    pub fn mcb_layernorm_bwd_workspace_bytes(rows: i64, D: i64) -> usize;
+    pub fn mcb_layernorm_bwd(x: *const c_void, w: *const c_void, dy: *const c_void, dx_residual: *const c_void, dx: *mut c_void, dw: *mut f32, db: *mut f32, accumulate: c_int, rows: i64, D: i64, eps: f32, dtype: c_int, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn mcb_softmax_fwd(x: *const c_void, y: *mut c_void, rows: i64, D: i64, dtype: c_int, stream: *mut c_void) -> c_int;
     pub fn mcb_softmax_bwd(y: *const c_void, dy: *const c_void, dx: *mut c_void, rows: i64, D: i64, dtype: c_int, stream: *mut c_void) -> c_int;
     pub fn mcb_softmax_causal_fwd(x: *const c_void, y: *mut c_void, rows: i64, D: i64, seq: i64, scale: f32, dtype: c_int, stream: *mut c_void) -> c_int;
@@ -242,6 +274,11 @@ extern "C" {
     pub fn mcb_attention_causal_bwd_ex(q: *const c_void, k: *const c_void, v: *const c_void, o: *const c_void, dout: *const c_void, lse: *const f32, dq: *mut c_void, dk: *mut c_void, dv: *mut c_void, nb: i64, groups: i64, seq: i64, head_dim: i64, scale: f32, dtype: c_int, kv_heads: i64, o_token_major: c_int, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn mcb_attention_causal_fwd_ragged(q: *const c_void, k: *const c_void, v: *const c_void, o: *mut c_void, lse: *mut f32, nb: i64, groups: i64, seq: i64, head_dim: i64, scale: f32, dtype: c_int, kv_heads: i64, o_token_major: c_int, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn mcb_attention_causal_bwd_ragged(q: *const c_void, k: *const c_void, v: *const c_void, o: *const c_void, dout: *const c_void, lse: *const f32, dq: *mut c_void, dk: *mut c_void, dv: *mut c_void, nb: i64, groups: i64, seq: i64, head_dim: i64, scale: f32, dtype: c_int, kv_heads: i64, o_token_major: c_int, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn mcb_attention_mask_bytes(batch: i64, seq: i64) -> usize;
+    pub fn mcb_attention_mask(document_ids: *const c_void, id_bytes: c_int, prefix: *const u8, mask: *mut c_void, mask_bytes: usize, batch: i64, seq: i64, stream: *mut c_void) -> c_int;
+    pub fn mcb_attention_masked_fwd(call: *const mcb_masked_attention, q: *const c_void, k: *const c_void, v: *const c_void, o: *mut c_void, lse: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn mcb_attention_masked_workspace_bytes(call: *const mcb_masked_attention) -> usize;
+    pub fn mcb_attention_masked_bwd(call: *const mcb_masked_attention, q: *const c_void, k: *const c_void, v: *const c_void, o: *const c_void, lse: *const f32, dout: *const c_void, dq: *mut c_void, dk: *mut c_void, dv: *mut c_void, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn mcb_comm_unique_id(id_out: *mut c_void) -> c_int;
     pub fn mcb_comm_init_rank(comm_out: *mut *mut mcb_comm, nranks: c_int, rank: c_int, id: *const c_void, timeout_ms: c_int, flags: c_int) -> c_int;
     pub fn mcb_comm_allreduce_bucket(comm: *mut mcb_comm, buf: *mut f32, count: i64, stream: *mut c_void) -> c_int;
@@ -250,7 +287,14 @@ extern "C" {
     pub fn mcb_comm_info(comm: *const mcb_comm, nranks: *mut c_int, rank: *mut c_int, dead: *mut c_int, nccl_version: *mut c_int) -> c_int;
     pub fn mcb_comm_destroy(comm: *mut mcb_comm) -> c_int;
     pub fn mcb_adamw_multi(tensors: *const mcb_adamw_tensor, n_tensors: c_int, lr: f32, beta1: f32, beta2: f32, eps: f32, weight_decay: f32, grad_scale: f32, stream: *mut c_void) -> c_int;
+    pub fn mcb_grad_norm_workspace_bytes(n_tensors: c_int) -> usize;
+    pub fn mcb_grad_norm(tensors: *const mcb_grad_tensor, n_tensors: c_int, norm: *mut f32, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn mcb_clip_grad_norm(tensors: *const mcb_grad_tensor, n_tensors: c_int, max_norm: f32, norm: *mut f32, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn mcb_adamw_multi_clipped(tensors: *const mcb_adamw_tensor, n_tensors: c_int, lr: f32, beta1: f32, beta2: f32, eps: f32, weight_decay: f32, grad_scale: f32, max_norm: f32, norm: *mut f32, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn mcb_embedding_fwd(ids: *const i32, table: *const c_void, out: *mut c_void, M: i64, H: i64, vocab: i64, dtype: c_int, stream: *mut c_void) -> c_int;
+    pub fn mcb_embedding_scaled_fwd(ids: *const c_void, id_bytes: c_int, table: *const c_void, out: *mut c_void, M: i64, H: i64, vocab: i64, scale: f32, dtype: c_int, stream: *mut c_void) -> c_int;
+    pub fn mcb_embedding_bwd_workspace_bytes(M: i64, H: i64) -> usize;
+    pub fn mcb_embedding_bwd(ids: *const c_void, id_bytes: c_int, dout: *const c_void, dtable: *mut f32, accumulate: c_int, M: i64, H: i64, vocab: i64, scale: f32, dtype: c_int, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn mcb_rope_relayout(src: *const c_void, dst: *mut c_void, B: i64, S: i64, H: i64, d: i64, theta: f32, rotate: c_int, inverse: c_int, dtype: c_int, stream: *mut c_void) -> c_int;
     pub fn mcb_rope_relayout_ex(src: *const c_void, dst: *mut c_void, B: i64, S: i64, H: i64, d: i64, theta: f32, rotate: c_int, inverse: c_int, token_pitch: i64, col_offset: i64, dtype: c_int, stream: *mut c_void) -> c_int;
     pub fn mcb_rope_relayout_qkv(fused: *mut c_void, q: *mut c_void, k: *mut c_void, v: *mut c_void, B: i64, S: i64, Hq: i64, Hk: i64, d: i64, theta: f32, inverse: c_int, token_pitch: i64, dtype: c_int, stream: *mut c_void) -> c_int;

@@ -2,7 +2,8 @@
 `TargetModule`, `LoRAAdapterConfig`, `LoRAAdapter`, `AdamWConfig`, `AdamW`, `LRScheduler`,
 `TrainingConfig`, `StepMetrics`, `TrainingStep`.  Same names, argument meaning, defaults, validation
 messages and step/counter semantics; all arithmetic runs in the CUDA kernels behind the C ABI.  Beside the reference's
-cross-entropy: `token_log_probs`, `preference_loss`, `policy_loss` and `distillation_loss`, each with its gradient.
+cross-entropy: `token_log_probs`, `preference_loss`, `policy_loss` and `distillation_loss`, each with its gradient.  Beside AdamW:
+`grad_norm`, `clip_grad_norm` and `GradClipper`.
 """
 from __future__ import annotations
 
@@ -234,6 +235,79 @@ class LoRAAdapter:
 
 
 # ---------------------------------------------------------------------------------------------
+# global gradient norm
+# ---------------------------------------------------------------------------------------------
+
+class GradClipper:
+    """The global 2-norm of a list of gradients (float32 or bfloat16, contiguous, on one device), and clipping by it, for buffers that
+    stay where they are from step to step: the tensors are held and their table is made once.  out: where the clipped gradients
+    go, a tensor of the same size and type each (None: in place)."""
+
+    def __init__(self, grads: Iterable[torch.Tensor], out: Optional[Iterable[torch.Tensor]] = None):
+        self.grads = list(grads)
+        self.out = None if out is None else list(out)
+        if not self.grads:
+            raise InvalidConfig("no gradients")
+        backend._require_cuda(*self.grads)
+        words, device = [], self.grads[0].device
+        if self.out is not None:
+            if len(self.out) != len(self.grads):
+                raise InvalidConfig(f"{len(self.out)} outputs for {len(self.grads)} gradients")
+            backend._require_cuda(*self.out)
+        for i, g in enumerate(self.grads):
+            o = g if self.out is None else self.out[i]
+            if g.device != device or o.device != device:
+                raise TrainingError(f"gradient {i} is on another device than {device}")
+            if o.dtype != g.dtype or o.numel() != g.numel():
+                raise TrainingError(f"output {i} is {o.numel()} x {o.dtype}, its gradient {g.numel()} x {g.dtype}")
+            words += (g.data_ptr(), 0 if self.out is None else o.data_ptr(), g.numel(), backend._dtype_code(g), 0)
+        self._table = (_lib.GradTensor * len(self.grads))()
+        struct.pack_into("=" + "QQqii" * len(self.grads), self._table, 0, *words)
+        self._bytes = _lib.load().mcb_grad_norm_workspace_bytes(len(self.grads))
+
+    def _call(self, max_norm: Optional[float]) -> torch.Tensor:
+        first = self.grads[0]
+        other = backend._on_device_of(first)
+        if other is not None:
+            with other:
+                return self._call(max_norm)
+        lib = backend._lib_for(first)
+        norm = torch.empty(1, dtype=torch.float32, device=first.device)
+        ws = backend.workspace(first.device, self._bytes)
+        if max_norm is None:
+            _lib.check(lib.mcb_grad_norm(self._table, len(self.grads), norm.data_ptr(), ws.data_ptr(), ws.numel(), backend._stream()))
+        else:
+            _lib.check(lib.mcb_clip_grad_norm(self._table, len(self.grads), max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel(), backend._stream()))
+        return norm
+
+    def norm(self) -> torch.Tensor:
+        """[1] float32: the square root of the sum of all squares."""
+        return self._call(None)
+
+    def clip(self, max_norm: float) -> torch.Tensor:
+        """Multiplies every gradient by min(1, max_norm / (norm + 1e-6)); returns the norm before that, [1] float32.  A norm that is
+        NaN makes every gradient NaN."""
+        return self._call(_check_max_norm(max_norm))
+
+
+def _check_max_norm(max_norm: float) -> float:
+    if not max_norm >= 0.0:
+        raise InvalidConfig(f"max_norm must not be negative, got {max_norm}")
+    return float(max_norm)
+
+
+def grad_norm(grads: Iterable[torch.Tensor]) -> torch.Tensor:
+    """The 2-norm of all gradients taken as one vector, [1] float32 on their device."""
+    return GradClipper(grads).norm()
+
+
+def clip_grad_norm(grads: Iterable[torch.Tensor], max_norm: float, out: Optional[Iterable[torch.Tensor]] = None) -> torch.Tensor:
+    """Scales the gradients (in place, or into `out`) so that their global norm is at most max_norm; returns the norm they had.
+    `GradClipper` does the same for buffers that stay, without making their table again."""
+    return GradClipper(grads, out).clip(max_norm)
+
+
+# ---------------------------------------------------------------------------------------------
 # AdamW (src/training/optimizer.rs)
 # ---------------------------------------------------------------------------------------------
 
@@ -290,7 +364,7 @@ class AdamW:
     def state_of(self, var: torch.Tensor):
         return self.state[self._key(var)]
 
-    def _launch(self, items, grad_scale: float = 1.0) -> None:
+    def _launch(self, items, grad_scale: float = 1.0, max_grad_norm: Optional[float] = None) -> Optional[torch.Tensor]:
         # This loop is most of an update's time on the host: one attribute read per fact and tensor, and the descriptors
         # packed in one go instead of as one ctypes structure per tensor (192 tensors, one update: 416 -> 237 us, 267 with the
         # check of the moments).
@@ -309,8 +383,16 @@ class AdamW:
         struct.pack_into("=" + "QQQQqii" * len(items), table, 0, *words)
         lib = backend._lib_for(items[0][2])
         c = self.config
-        _lib.check(lib.mcb_adamw_multi(table, len(items), c.learning_rate, c.beta1, c.beta2, c.epsilon, c.weight_decay,
-                                       float(grad_scale), backend._stream()))
+        if max_grad_norm is None:
+            _lib.check(lib.mcb_adamw_multi(table, len(items), c.learning_rate, c.beta1, c.beta2, c.epsilon, c.weight_decay,
+                                           float(grad_scale), backend._stream()))
+            return None
+        dev = items[0][2].device
+        norm = torch.empty(1, dtype=torch.float32, device=dev)
+        ws = backend.workspace(dev, lib.mcb_grad_norm_workspace_bytes(len(items)))
+        _lib.check(lib.mcb_adamw_multi_clipped(table, len(items), c.learning_rate, c.beta1, c.beta2, c.epsilon, c.weight_decay,
+                                               float(grad_scale), max_grad_norm, norm.data_ptr(), ws.data_ptr(), ws.numel(), backend._stream()))
+        return norm
 
     def step(self, name, param: torch.Tensor, grad: torch.Tensor) -> torch.Tensor:
         """AdamW::step (src/training/optimizer.rs:227-279).  Updates `param` in place and returns it."""
@@ -328,9 +410,13 @@ class AdamW:
             self.add_parameter(key, var)
         self.step(key, var, grad)
 
-    def step_vars(self, variables: List[torch.Tensor], grads: List[torch.Tensor], grad_scale: float = 1.0) -> None:
+    def step_vars(self, variables: List[torch.Tensor], grads: List[torch.Tensor], grad_scale: float = 1.0,
+                  max_grad_norm: Optional[float] = None) -> Optional[torch.Tensor]:
         """The loop `for var in vars { step_var(var, grad) }` of src/training/trainer.rs:398-402 as one
-        multi-tensor launch: tensor j of this call gets step number step_count + j + 1."""
+        multi-tensor launch: tensor j of this call gets step number step_count + j + 1.  With max_grad_norm the gradients
+        (times grad_scale) are clipped by their global norm on the way into the update (their buffers stay as they are) and
+        that norm is returned, [1] float32."""
+        limit = None if max_grad_norm is None else _check_max_norm(max_grad_norm)
         items, state = [], self.state
         for var, g in zip(variables, grads):
             address, n = var.data_ptr(), var.numel()
@@ -340,8 +426,9 @@ class AdamW:
                 mv = state["var", address, n]
             self.step_count += 1
             items.append((address, n, var, g.contiguous(), mv[0], mv[1], self.step_count))
-        if items:
-            self._launch(items, grad_scale)
+        if not items:
+            return None
+        return self._launch(items, grad_scale) if limit is None else self._launch(items, grad_scale, limit)
 
     def set_lr(self, lr: float) -> None:
         self.config.learning_rate = float(lr)
@@ -433,11 +520,13 @@ class LRScheduler:
 
 @dataclass
 class TrainingConfig:
-    """src/training/trainer.rs:16-39.  `max_grad_norm` is carried but, as in the reference, nothing reads it."""
+    """src/training/trainer.rs:16-39.  As in the reference `max_grad_norm` alone changes nothing; with `clip_gradients` the trainer
+    clips by it."""
     num_epochs: int = 3
     lr_scheduler: LRScheduler = field(default_factory=lambda: LRScheduler.constant(1e-4))
     optimizer_config: AdamWConfig = field(default_factory=AdamWConfig)
     max_grad_norm: Optional[float] = 1.0
+    clip_gradients: bool = False
 
 
 @dataclass
@@ -764,11 +853,15 @@ class TrainingStep:
         return out
 
     def execute(self, input_ids, target_ids, lora_adapter: LoRAAdapter, optimizer: AdamW, learning_rate: float,
-                forward_backward_fn: Callable) -> StepMetrics:
+                forward_backward_fn: Callable, max_grad_norm: Optional[float] = None) -> StepMetrics:
+        """max_grad_norm: the gradients are clipped to that global norm on their way into the update."""
         loss, grads = forward_backward_fn(input_ids, target_ids)
         variables = self.collect_trainable_vars(lora_adapter)
         optimizer.set_lr(learning_rate)
-        optimizer.step_vars(variables, grads)
+        if max_grad_norm is None:
+            optimizer.step_vars(variables, grads)
+        else:
+            optimizer.step_vars(variables, grads, max_grad_norm=max_grad_norm)
         loss_value = float(loss) if not torch.is_tensor(loss) else float(loss.item())  # host sync, trainer.rs:405
         self._step += 1
         return StepMetrics(loss=loss_value, step=self._step, learning_rate=learning_rate)
@@ -800,6 +893,7 @@ class Trainer:
 
         say = print if verbose else (lambda *a, **k: None)
         all_metrics: List[StepMetrics] = []
+        clip = {"max_grad_norm": self.config.max_grad_norm} if self.config.clip_gradients else {}
         say("\nStarting LoRA Training")
         say(f"Epochs: {self.config.num_epochs}")
         say(f"Batches per epoch: {len(dataset)}")
@@ -812,7 +906,7 @@ class Trainer:
             for batch_idx, (input_ids, target_ids) in enumerate(dataset):
                 lr = self.config.lr_scheduler.get_lr(self._global_step)
                 m = self.training_step.execute(input_ids, target_ids, self._lora_adapter, self.optimizer, lr,
-                                               forward_backward_fn)
+                                               forward_backward_fn, **clip)
                 epoch_loss += m.loss
                 all_metrics.append(m)
                 self._global_step += 1
