@@ -125,7 +125,8 @@ __global__ void __launch_bounds__(1024) mask_bits_kernel(const MaskParams p) {
 }
 
 // Tiles by falling block count: a counting sort over 1024 classes of counts, by one block of 128 threads.
-__device__ void sort_tiles(const int2* tiles, int* order, int n, int* bins, int* most) {
+__device__ void sort_tiles(const int2* tiles, int4* work, int n, int per_seq, int* bins, int* most) {
+  tiles = from_here(tiles);
   if (threadIdx.x == 0) *most = 0;
   for (int i = threadIdx.x; i < 1024; i += kTile) bins[i] = 0;
   __syncthreads();
@@ -155,7 +156,10 @@ __device__ void sort_tiles(const int2* tiles, int* order, int n, int* bins, int*
     at += n_here;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kTile) order[atomicAdd(&bins[1023 - static_cast<int>(__ldcg(&tiles[i].y) * 1023ll / top)], 1)] = i;
+  for (int i = threadIdx.x; i < n; i += kTile) {
+    const int first = __ldcg(&tiles[i].x), count = __ldcg(&tiles[i].y);
+    work[atomicAdd(&bins[1023 - static_cast<int>(count * 1023ll / top)], 1)] = make_int4(i / per_seq, i % per_seq, first, count);
+  }
   __syncthreads();
 }
 
@@ -169,6 +173,7 @@ __global__ void __launch_bounds__(kTile) mask_rows_kernel(const MaskParams p) {
   grid_dependency_wait();
   __syncthreads();
   const uint32_t* bits = reinterpret_cast<const uint32_t*>(p.block + p.l.bits) + 2 * static_cast<int64_t>(b) * p.l.bits_per_seq;
+  bits = from_here(bits);
   const Bits runs{bits, p.chunks}, open{bits + p.l.bits_per_seq, p.chunks};
   const int64_t pos = static_cast<int64_t>(t) * kTile + threadIdx.x;
   if (pos < p.S) {
@@ -203,8 +208,8 @@ __global__ void __launch_bounds__(kTile) mask_rows_kernel(const MaskParams p) {
   if (!last) return;
   __threadfence();
   const int n = p.B * tiles;
-  sort_tiles(reinterpret_cast<const int2*>(p.block + p.l.qtiles), p.block + p.l.qorder, n, bins, &most);
-  sort_tiles(reinterpret_cast<const int2*>(p.block + p.l.ktiles), p.block + p.l.korder, n, bins, &most);
+  sort_tiles(reinterpret_cast<const int2*>(p.block + p.l.qtiles), reinterpret_cast<int4*>(p.block + p.l.qwork), n, tiles, bins, &most);
+  sort_tiles(reinterpret_cast<const int2*>(p.block + p.l.ktiles), reinterpret_cast<int4*>(p.block + p.l.kwork), n, tiles, bins, &most);
 }
 
 template <typename I>

@@ -17,8 +17,8 @@ struct Layout {
   int64_t keys;     // int2 [batch, seq]: the queries [x, y) that see key position i
   int64_t qtiles;   // int2 [batch, tiles]: first key block (of 64) and number of blocks that the tile's queries see
   int64_t ktiles;   // int2 [batch, tiles]: first query block (of 64) and number of blocks that see the tile's keys
-  int64_t qorder;   // int [batch * tiles]: the query tiles, the most key blocks first
-  int64_t korder;   // int [batch * tiles]: the key tiles, the most query blocks first
+  int64_t qwork;    // int4 [batch * tiles]: the query tiles, the most key blocks first: sequence, tile, first block, blocks
+  int64_t kwork;    // int4 [batch * tiles]: the key tiles, the most query blocks first
   int64_t ticket;   // int: tiles that are done while the block is being made
   int64_t bits;     // two three-level bitmaps per sequence: where runs begin, where a position is no prefix
   int64_t bits_per_seq;
@@ -32,9 +32,9 @@ __host__ __device__ inline Layout layout(int64_t batch, int64_t seq) {
   l.keys = l.rows + 2 * n;
   l.qtiles = l.keys + 2 * n;
   l.ktiles = l.qtiles + 2 * t;
-  l.qorder = l.ktiles + 2 * t;
-  l.korder = l.qorder + t;
-  l.ticket = l.korder + t;
+  l.qwork = (l.ktiles + 2 * t + 3) & ~static_cast<int64_t>(3);   // 16-byte records
+  l.kwork = l.qwork + 4 * t;
+  l.ticket = l.kwork + 4 * t;
   l.bits = l.ticket + 1;
   l.bits_per_seq = chunks * (1024 + 32 + 1);
   l.words = l.bits + 2 * batch * l.bits_per_seq;
@@ -44,10 +44,8 @@ __host__ __device__ inline Layout layout(int64_t batch, int64_t seq) {
 struct View {
   const int2* rows;
   const int2* keys;
-  const int2* qtiles;
-  const int2* ktiles;
-  const int* qorder;
-  const int* korder;
+  const int4* qwork;
+  const int4* kwork;
 };
 inline View view(const void* mask, int64_t batch, int64_t seq) {
   const Layout l = layout(batch, seq);
@@ -55,10 +53,8 @@ inline View view(const void* mask, int64_t batch, int64_t seq) {
   View v;
   v.rows = reinterpret_cast<const int2*>(w + l.rows);
   v.keys = reinterpret_cast<const int2*>(w + l.keys);
-  v.qtiles = reinterpret_cast<const int2*>(w + l.qtiles);
-  v.ktiles = reinterpret_cast<const int2*>(w + l.ktiles);
-  v.qorder = w + l.qorder;
-  v.korder = w + l.korder;
+  v.qwork = reinterpret_cast<const int4*>(w + l.qwork);
+  v.kwork = reinterpret_cast<const int4*>(w + l.kwork);
   return v;
 }
 

@@ -69,8 +69,8 @@ struct SortParams {
 };
 
 template <typename I>
-__device__ __forceinline__ uint32_t key_of(const SortParams& p, int pass, int i) {
-  if (pass > 0) return __ldcg(p.key[(pass - 1) & 1] + i);
+__device__ __forceinline__ uint32_t key_of(const SortParams& p, const uint32_t* before, int pass, int i) {
+  if (pass > 0) return __ldcg(before + i);
   const int64_t id = static_cast<int64_t>(static_cast<const I*>(p.ids)[i]);
   return id >= 0 && id < p.vocab ? static_cast<uint32_t>(id) : static_cast<uint32_t>(p.vocab);   // the others behind all
 }
@@ -99,6 +99,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const __grid_constan
   const int end = static_cast<int>(begin + per < p.M ? begin + per : p.M);
   for (int pass = 0; pass < p.passes; ++pass) {
     const int shift = pass * p.digit_bits;
+    const uint32_t *from_key = from_here(p.key[(pass + 1) & 1]), *from_pos = from_here(p.pos[(pass + 1) & 1]);   // what the pass before has left
     const uint32_t mask = (1u << p.digit_bits) - 1u;
     for (int d = lane; d < kDigits; d += 32) hist[warp][d] = 0;
     __syncwarp();
@@ -106,7 +107,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const __grid_constan
       const int i = static_cast<int>(i0) + lane;
       const uint32_t have = __ballot_sync(kFull, i < end);
       if (i < end) {
-        const uint32_t d = (key_of<I>(p, pass, i) >> shift) & mask;
+        const uint32_t d = (key_of<I>(p, from_key, pass, i) >> shift) & mask;
         const uint32_t peers = __match_any_sync(have, d);
         if (lane == __ffs(peers) - 1) hist[warp][d] += __popc(peers);
       }
@@ -146,8 +147,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const __grid_constan
       const int i = static_cast<int>(i0) + lane;
       const uint32_t have = __ballot_sync(kFull, i < end);
       if (i < end) {
-        const uint32_t k = key_of<I>(p, pass, i), d = (k >> shift) & mask;
-        const uint32_t at = pass > 0 ? __ldcg(p.pos[(pass - 1) & 1] + i) : static_cast<uint32_t>(i);
+        const uint32_t k = key_of<I>(p, from_key, pass, i), d = (k >> shift) & mask;
+        const uint32_t at = pass > 0 ? __ldcg(from_pos + i) : static_cast<uint32_t>(i);
         const uint32_t peers = __match_any_sync(have, d);
         const uint32_t to = hist[warp][d] + __popc(peers & ((1u << lane) - 1u));
         __syncwarp(have);
@@ -212,14 +213,15 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const __grid_constant__ S
   const int t = blockIdx.x * ty + y;
   grid_launch_dependents();
   grid_dependency_wait();
+  const uint32_t *keys = from_here(p.key), *places = from_here(p.pos);
   const int64_t i0 = static_cast<int64_t>(t) * kTile;
   const int n = t < p.tiles ? static_cast<int>(i0 + kTile < p.M ? kTile : p.M - i0) : 0;
   const uint32_t none = static_cast<uint32_t>(p.vocab);
   // keys of the tile with one on either side
   for (int i = x; i < n + 2 && n > 0; i += p.tx) {
     const int64_t at = i0 + i - 1;
-    s_key[y][i] = at >= 0 && at < p.M ? __ldcg(p.key + at) : none;
-    if (i >= 1 && i <= n) s_pos[y][i - 1] = __ldcg(p.pos + at);
+    s_key[y][i] = at >= 0 && at < p.M ? __ldcg(keys + at) : none;
+    if (i >= 1 && i <= n) s_pos[y][i - 1] = __ldcg(places + at);
   }
   __syncthreads();
   if (n == 0) return;
@@ -277,18 +279,19 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
   grid_launch_dependents();
   grid_dependency_wait();
   if (t >= p.tiles) return;
+  const uint32_t* keys = from_here(p.key);
   const int64_t i0 = static_cast<int64_t>(t) * kTile, i1 = i0 + kTile;
   if (i1 >= p.M) return;
-  const uint32_t id = __ldcg(p.key + i1 - 1);
-  if (id >= static_cast<uint32_t>(p.vocab) || __ldcg(p.key + i1) != id) return;
-  if (i0 > 0 && __ldcg(p.key + i0 - 1) == id) return;   // it began in a tile before
+  const uint32_t id = __ldcg(keys + i1 - 1);
+  if (id >= static_cast<uint32_t>(p.vocab) || __ldcg(keys + i1) != id) return;
+  if (i0 > 0 && __ldcg(keys + i0 - 1) == id) return;   // it began in a tile before
   const int64_t c = N * (static_cast<int64_t>(blockIdx.y) * p.tx + x);
   if (c >= p.H) return;
   // last token of the run
   int64_t lo = i1, hi = p.M - 1;
   while (lo < hi) {
     const int64_t mid = (lo + hi + 1) >> 1;
-    if (__ldcg(p.key + mid) == id) lo = mid;
+    if (__ldcg(keys + mid) == id) lo = mid;
     else hi = mid - 1;
   }
   float acc[N] = {};

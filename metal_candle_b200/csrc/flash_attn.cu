@@ -36,12 +36,20 @@
 // 1024 x 7 x 50 82 instead of 243, 8192 x 7 x 4 563 instead of 605, 4096 x 7 x 16 288 instead of 220 and the relayout
 // of the output, which the fused kernel writes token-major.
 // Every wait is bounded; on expiry the CTA records a code in the device status word and leaves.
+//
+// The same three kernels run under document and prefix masks, with the score capped by tanh and lowered by a distance bias
+// (template parameters MASKED, CAP, BIAS; entry points in masked_attn.cu).  A mask is an interval of keys for each query (attn_mask.cuh), so a thread
+// that owns a query row masks with two registers, and one that owns a key row with the interval of queries that see it.
+// Tiles walk over the key (query) blocks that some row of theirs sees, and the work list has the longest tiles first.
 #include <cuda.h>
 #include <string.h>
 
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "lora_internal.cuh"
+#include "masked_attn.cuh"
 #include "umma_ptx.cuh"
 
 namespace cg = cooperative_groups;
@@ -96,11 +104,89 @@ __device__ __forceinline__ float lg2(float x) {
   return y;
 }
 
+// The call that a kernel under a mask reads; nothing otherwise.
+struct NoCall {
+  NoCall() = default;
+  template <typename T>
+  __device__ explicit NoCall(const T&) {}
+};
+template <bool MASKED>
+using CallOf = std::conditional_t<MASKED, mattn::Call, NoCall>;
+
+// ---- scores that are more than a scaled product -----------------------------------------------------------
+// tanh in float32.  Up to |x| = 1, where capped scores lie all but always, an odd polynomial: tanh(x) / x in powers of x^2, fitted for the
+// smallest relative error over [0, 1] (5e-8; 1.2e-7 as evaluated), seven multiply-adds on pairs and no special function.
+__device__ __forceinline__ float2 tanh_small(float2 x) {
+  const float2 u = __fmul2_rn(x, x);
+  float2 t = f2(0.0010410252725705504f, 0.0010410252725705504f);
+  t = __ffma2_rn(t, u, f2(-0.0062033869326114655f, -0.0062033869326114655f));
+  t = __ffma2_rn(t, u, f2(0.020289989188313484f, 0.020289989188313484f));
+  t = __ffma2_rn(t, u, f2(-0.05345703288912773f, -0.05345703288912773f));
+  t = __ffma2_rn(t, u, f2(0.13325203955173492f, 0.13325203955173492f));
+  t = __ffma2_rn(t, u, f2(-0.33332839608192444f, -0.33332839608192444f));
+  t = __ffma2_rn(t, u, f2(0.9999999403953552f, 0.9999999403953552f));
+  return __fmul2_rn(t, x);
+}
+// Any x: 1 - 2 / (1 + e^2x), two special functions; off by some 1e-7.
+__device__ __forceinline__ float tanh_any(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(x * (2.0f * kLog2e))));
+  return fmaf(-2.0f, r, 1.0f);
+}
+
+// What turns a product into a score in units of log 2, read once by a thread that owns a row.
+template <bool CAP, bool BIAS>
+struct Shape {
+  float in, out, slope2;   // CAP: tanh(product * in) * out; else product * out; then - slope2 * distance
+  __device__ __forceinline__ Shape(const mattn::Call& c) : in(CAP ? c.scale / c.cap : 0.0f), out((CAP ? c.cap : c.scale) * kLog2e), slope2(0.0f) {}
+  // N products (bits) into scores in place; distance of element e: |first + dir * e|.  With CAP, keep(e, tanh^2 of a pair) is called.
+  template <int N, typename F>
+  __device__ __forceinline__ void apply(uint32_t (&v)[N], float first, float dir, F&& keep) const {
+    if constexpr (CAP) {
+      const float2 in2 = f2(in, in), out2 = f2(out, out);
+      float top = 0.0f;
+#pragma unroll
+      for (int e = 0; e < N; e += 2) {
+        const float2 x = __fmul2_rn(f2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), in2);
+        v[e] = __float_as_uint(x.x);
+        v[e + 1] = __float_as_uint(x.y);
+        top = fmax3(top, fabsf(x.x), fabsf(x.y));
+      }
+      const bool small = __all_sync(0xffffffffu, top <= 1.0f);
+#pragma unroll
+      for (int e = 0; e < N; e += 2) {
+        float2 t = f2(__uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+        t = small ? tanh_small(t) : f2(tanh_any(t.x), tanh_any(t.y));
+        keep(e, t);
+        t = __fmul2_rn(t, out2);
+        v[e] = __float_as_uint(t.x);
+        v[e + 1] = __float_as_uint(t.y);
+      }
+    }
+    if constexpr (BIAS) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float far = fabsf(fmaf(dir, static_cast<float>(e), first));
+        const float x = __uint_as_float(v[e]);
+        v[e] = __float_as_uint(CAP ? fmaf(-slope2, far, x) : fmaf(x, out, -slope2 * far));
+      }
+    }
+  }
+};
+// bits [lo - first, hi - first) of a block of 64 (32) positions that starts at `first`
+__device__ __forceinline__ uint32_t interval_bits(int lo, int hi, int first) {
+  const int a = lo - first, b = hi - first;
+  const uint32_t from = a <= 0 ? 0xffffffffu : a >= 32 ? 0u : 0xffffffffu << a;
+  const uint32_t to = b <= 0 ? 0u : b >= 32 ? 0xffffffffu : (1u << b) - 1u;
+  return from & to;
+}
+
 __host__ __device__ __forceinline__ int q_blocks(int S) { return (S + kBQ - 1) / kBQ; }
 
 // Work item t (heavy first): query block qb = nqb-1 - t / (G*nb), then head g and batch*kv-head nb.
 struct FwdTile {
   int qb, g, nb, nkb;
+  int b, hk, kb0;   // sequence and kv head (masked), first key block
   int64_t qrow0;
 };
 __device__ __forceinline__ FwdTile fwd_tile(const FwdParams& p, int t) {
@@ -111,9 +197,46 @@ __device__ __forceinline__ FwdTile fwd_tile(const FwdParams& p, int t) {
   w.g = r % p.G;
   w.nb = r / p.G;
   w.nkb = 2 * w.qb + 2;  // key blocks of 64 up to and including the diagonal
+  w.b = w.hk = w.kb0 = 0;
   w.qrow0 = (static_cast<int64_t>(w.nb) * p.G + w.g) * p.S + static_cast<int64_t>(w.qb) * kBQ;
   return w;
 }
+
+// A CTA's items one after the other.  Under a mask they come from the sorted list, there and back again over the CTAs (the first of
+// one round is the last of the next), each record asked for an item ahead: it would be a trip to L2 in front of every item.
+template <bool MASKED>
+struct Walk {
+  const FwdParams& p;
+  const CallOf<MASKED>& c;
+  int t, n, round;
+  int4 next;
+  __device__ __forceinline__ Walk(const FwdParams& p_, const CallOf<MASKED>& c_) : p(p_), c(c_), t(blockIdx.x), round(0) {
+    if constexpr (MASKED) {
+      n = q_blocks(p.S) * c.B * p.G * c.Hk;
+      next = t < n ? c.mask.qwork[t / (p.G * c.Hk)] : make_int4(0, 0, 0, 0);
+    } else {
+      n = q_blocks(p.S) * p.G * p.NB;
+    }
+  }
+  __device__ __forceinline__ bool get(FwdTile& w) {
+    if (t >= n) return false;
+    if constexpr (MASKED) {
+      const int heads = p.G * c.Hk, r = t % heads;
+      w.b = next.x; w.qb = next.y; w.kb0 = next.z; w.nkb = next.w;
+      w.hk = r / p.G; w.g = r % p.G;
+      w.nb = w.b * c.Hk + w.hk;
+      w.qrow0 = (static_cast<int64_t>(w.nb) * p.G + w.g) * p.S + static_cast<int64_t>(w.qb) * kBQ;
+      ++round;
+      const int64_t to = static_cast<int64_t>(round) * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+      t = to < n ? static_cast<int>(to) : n;
+      if (t < n) next = c.mask.qwork[t / heads];
+    } else {
+      w = fwd_tile(p, t);
+      t += gridDim.x;
+    }
+    return true;
+  }
+};
 
 // Where the 64 values of (kv-head index nb, head g of its group, position s) start in O / dO, in elements, and column
 // and plane of the same head for a tiled copy (its row is the position).
@@ -129,9 +252,10 @@ __device__ __forceinline__ void o_plane(int G, int HKV, int o_tok, int nb, int g
   plane = b;
 }
 
+template <bool MASKED, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 2)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                const __grid_constant__ CUtensorMap tmVt, const FwdParams p) {
+                const __grid_constant__ CUtensorMap tmVt, const FwdParams p, const __grid_constant__ CallOf<MASKED> c) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen_base = smem_raw + (base - smem_u32(smem_raw));
@@ -173,16 +297,18 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   grid_dependency_wait();   // the set-up above ran under the tail of the kernel before
   // S buffers at columns 0 and 64, O at 128, the two P buffers (bf16 pairs: 32 columns each) at 192 and 224
   const uint32_t tO = tmem_base + 128, tP0 = tmem_base + 192;
-  const int n_tiles = q_blocks(p.S) * p.G * p.NB;
+  Walk<MASKED> walk(p, c);
+  FwdTile w;
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       int st = 0;
       uint32_t ph = 0;
       bool ok = true;
-      int it = 0;
-      for (int t = blockIdx.x; ok && t < n_tiles; t += gridDim.x, ++it) {
-        const FwdTile w = fwd_tile(p, t);
+      int it = -1;
+      while (ok && walk.get(w)) {
+        if (MASKED && w.nkb == 0) continue;   // a tile that sees nothing: no loads, no products
+        ++it;
         // the previous item's last S product has read Q
         if (it > 0) ok = mbar_wait(q_free, (it - 1) & 1, abort_flag, 69, p.status);
         if (!ok) break;
@@ -192,17 +318,17 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           ok = mbar_wait(kv_empty0 + 8 * st, ph ^ 1, abort_flag, 71, p.status);
           if (!ok) break;
           mbar_expect_tx(kv_full0 + 8 * st, 2 * kKBytes);
-          tma_load_3d(base + kOffK + st * kKBytes, &tmK, kv_full0 + 8 * st, 0, j * kBK, w.nb);
-          tma_load_3d(base + kOffV + st * kKBytes, &tmVt, kv_full0 + 8 * st, 0, j * kBK, w.nb);
+          tma_load_3d(base + kOffK + st * kKBytes, &tmK, kv_full0 + 8 * st, 0, (w.kb0 + j) * kBK, w.nb);
+          tma_load_3d(base + kOffV + st * kKBytes, &tmVt, kv_full0 + 8 * st, 0, (w.kb0 + j) * kBK, w.nb);
           if (++st == kFwdStages) { st = 0; ph ^= 1; }
         }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       const uint32_t idesc = make_idesc(kBK);  // M = 128, N = 64 for both products
       bool ok = true;
-      int it = 0;
+      int it = -1;
       uint32_t n0 = 0;            // running number of this item's block 0
       int sst = 0;                // ring stage and phase of the next block to get its S product
       uint32_t sph = 0;
@@ -223,10 +349,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         if (++sst == kFwdStages) { sst = 0; sph ^= 1; }
         return true;
       };
-      for (int t = blockIdx.x; ok && t < n_tiles; t += gridDim.x, ++it) {
-        const FwdTile w = fwd_tile(p, t);
+      while (ok && walk.get(w)) {
+        if (MASKED && w.nkb == 0) continue;
+        ++it;
         ok = mbar_wait(q_full, it & 1, abort_flag, 72, p.status);
-        for (int j = 0; ok && j < 2; ++j) ok = issue_s(n0 + j, j == w.nkb - 1);   // nkb >= 2
+        for (int j = 0; ok && j < 2 && j < w.nkb; ++j) ok = issue_s(n0 + j, j == w.nkb - 1);
         for (int j = 0; ok && j < w.nkb; ++j) {
           const uint32_t n = n0 + j;
           if (j + 2 < w.nkb) {
@@ -262,18 +389,35 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
     bool ok = true;
     uint32_t n0 = 0;
-    for (int t = blockIdx.x; ok && t < n_tiles; t += gridDim.x) {
-      const FwdTile w = fwd_tile(p, t);
+    std::conditional_t<MASKED, Shape<CAP, BIAS>, NoCall> shape(c);
+    while (ok && walk.get(w)) {
       const int qpos = w.qb * kBQ + row;
-      float m = -INFINITY, l = 0.0f;   // m: the maximum in use (base-2 logits)
+      // m: the maximum in use (base-2 logits); under a mask a row may see nothing for some blocks, or at all
+      float m = MASKED ? mattn::kNoScore : -INFINITY, l = 0.0f;
+      int2 sees = make_int2(0, 0);
+      float sc = p.sc;
+      if constexpr (MASKED) {
+        if (qpos < p.S) sees = c.mask.rows[static_cast<int64_t>(w.b) * p.S + qpos];
+        if constexpr (BIAS) shape.slope2 = c.slopes[w.hk * p.G + w.g] * kLog2e;
+        if constexpr (CAP || BIAS) sc = 1.0f;
+        if (w.nkb == 0) {   // the tile sees nothing: no block was loaded for it
+          if (qpos < p.S) {
+            uint4* orow = reinterpret_cast<uint4*>(p.O + o_offset(p.S, p.G, p.HKV, p.o_tok, w.nb, w.g, qpos));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) orow[i] = make_uint4(0, 0, 0, 0);
+            if (p.lse != nullptr) p.lse[w.qrow0 + row] = -INFINITY;
+          }
+          continue;
+        }
+      }
       for (int j = 0; j < w.nkb; ++j) {
         const uint32_t n = n0 + j;
         ok = __all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * (n & 1), (n >> 1) & 1, abort_flag, 76, p.status));
         if (!ok) break;
         tcgen05_fence_after();
         const uint32_t tS = tmem_base + (n & 1) * 64;
-        const int key0 = j * kBK;
-        const bool diag = key0 + kBK - 1 > w.qb * kBQ;  // some element of this block may lie above the diagonal
+        const int key0 = (w.kb0 + j) * kBK;
+        const bool diag = !MASKED && key0 + kBK - 1 > w.qb * kBQ;  // some element of this block may lie above the diagonal
         // the row's 64 scores of this block, read from tensor memory once (four loads in flight, one wait)
         uint32_t sv[4][16];
 #pragma unroll
@@ -282,6 +426,20 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_free0 + 8 * (n & 1));   // the buffer may take block n + 2
+        if constexpr (CAP || BIAS) {
+#pragma unroll
+          for (int c4 = 0; c4 < 4; ++c4) shape.apply(sv[c4], static_cast<float>(qpos - key0 - 16 * c4), -1.0f, [](int, float2) {});
+        }
+        if constexpr (MASKED) {
+          if (key0 < sees.x || key0 + kBK > sees.y) {
+            const uint32_t seen[2] = {interval_bits(sees.x, sees.y, key0), interval_bits(sees.x, sees.y, key0 + 32)};
+#pragma unroll
+            for (int c4 = 0; c4 < 4; ++c4)
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if ((seen[c4 >> 1] >> (16 * (c4 & 1) + e) & 1u) == 0) sv[c4][e] = 0xff800000u;
+          }
+        }
         if (diag) {
 #pragma unroll
           for (int c4 = 0; c4 < 4; ++c4)
@@ -299,7 +457,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           mxc[c4] = tmx;
         }
         const float mx = fmaxf(fmax3(mxc[0], mxc[1], mxc[2]), mxc[3]);
-        const float m_true = fmaxf(m, mx * p.sc);  // key 0 is never masked, so this is finite from block 0 on
+        const float m_true = fmaxf(m, mx * sc);  // (without a mask key 0 is always seen, so this is finite from block 0 on)
         const bool raise = m_true > m + 8.0f;       // block 0: m = -inf, always
         if (n >= 2) {
           // the P V product of block n-2 has read the P buffer that this block overwrites
@@ -331,7 +489,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         // tensor memory (the A operand of the P V product: no trip through shared memory)
         // (packed two-wide FMA and add: the special-function unit's 64 exponentials are the only per-element work)
         float2 lsa = f2(0.0f, 0.0f), lsb = f2(0.0f, 0.0f);
-        const float2 sc2 = f2(p.sc, p.sc), nm2 = f2(-m, -m);
+        const float2 sc2 = f2(sc, sc), nm2 = f2(-m, -m);
         const uint32_t tP = tP0 + lane_addr + (n & 1) * 32;
 #pragma unroll
         for (int c2 = 0; c2 < 2; ++c2) {
@@ -361,7 +519,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       ok = __all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * (nl & 1), (nl >> 1) & 1, abort_flag, 78, p.status));
       if (!ok) break;
       tcgen05_fence_after();
-      const float inv = 1.0f / l;
+      const bool none = MASKED && l == 0.0f;   // nothing seen, or scores of -inf alone
+      const float inv = none ? 0.0f : 1.0f / l;
       __nv_bfloat16* orow = p.O + o_offset(p.S, p.G, p.HKV, p.o_tok, w.nb, w.g, w.qb * kBQ + row);
       uint32_t ov[4][16];
 #pragma unroll
@@ -370,7 +529,21 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_free);   // the next item's products may overwrite O
-      if (qpos < p.S) {
+      bool bad = false;
+      if constexpr (MASKED) {
+        // a row that is not finite is taken again from what it sees (masked_attn.cuh)
+        float sum = 0.0f;
+#pragma unroll
+        for (int c4 = 0; c4 < 4; ++c4)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            if (none) ov[c4][e] = 0;
+            const float x = __uint_as_float(ov[c4][e]);
+            sum = fmaf(x, 0.0f, sum);
+          }
+        bad = qpos < p.S && !(sum * inv == 0.0f);
+      }
+      if (qpos < p.S && !bad) {
 #pragma unroll
         for (int c4 = 0; c4 < 4; ++c4) {
           uint32_t ow[8];
@@ -380,7 +553,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           *reinterpret_cast<uint4*>(orow + 16 * c4) = make_uint4(ow[0], ow[1], ow[2], ow[3]);
           *reinterpret_cast<uint4*>(orow + 16 * c4 + 8) = make_uint4(ow[4], ow[5], ow[6], ow[7]);
         }
-        if (p.lse != nullptr) p.lse[w.qrow0 + row] = (m + lg2(l)) * kLn2;
+        if (p.lse != nullptr) p.lse[w.qrow0 + row] = none ? -INFINITY : (m + lg2(l)) * kLn2;
+      }
+      if constexpr (MASKED) {
+        for (uint32_t rows = __ballot_sync(0xffffffffu, bad); rows != 0; rows &= rows - 1)
+          mattn::fwd_row<__nv_bfloat16>(c, w.b, w.hk, w.g, w.qb * kBQ + quad * 32 + __ffs(rows) - 1);
       }
       n0 += static_cast<uint32_t>(w.nkb);
     }
@@ -432,9 +609,11 @@ struct BwdParams {
 // Tensor memory (256 columns): S double-buffered at 0 and 64 (the next blocks' Q K^T run under this block's
 // arithmetic), dP at 128, dQ at 192.  dS (bf16 pairs, 32 columns) is written over the first half of dP, which has
 // been read by then, and is the A operand of dQ += dS K straight from tensor memory.
+template <bool MASKED, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 2)
 attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmdO,
-               const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const BwdParams p) {
+               const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const BwdParams p,
+               const __grid_constant__ CallOf<MASKED> c) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen_base = smem_raw + (base - smem_u32(smem_raw));
@@ -473,16 +652,18 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
   const uint32_t tDP = tmem_base + 128, tDQ = tmem_base + 192;
   FwdParams tp;   // the item order of the forward
   tp.S = p.S; tp.G = p.G; tp.NB = p.NB;
-  const int n_tiles = q_blocks(p.S) * p.G * p.NB;
+  Walk<MASKED> walk(tp, c);
+  FwdTile w;
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       int st = 0;
       uint32_t ph = 0;
       bool ok = true;
-      int it = 0;
-      for (int t = blockIdx.x; ok && t < n_tiles; t += gridDim.x, ++it) {
-        const FwdTile w = fwd_tile(tp, t);
+      int it = -1;
+      while (ok && walk.get(w)) {
+        if (MASKED && w.nkb == 0) continue;
+        ++it;
         // the previous item's last S and dP products have read Q and dO
         if (it > 0) ok = mbar_wait(q_free, (it - 1) & 1, abort_flag, 80, p.status);
         if (!ok) break;
@@ -496,17 +677,17 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
           if (!ok) break;
           const uint32_t sb = base + kDqOffStage + st * kDqStageBytes;
           mbar_expect_tx(kv_full0 + 8 * st, kDqStageBytes);
-          tma_load_3d(sb, &tmK, kv_full0 + 8 * st, 0, j * kBK, w.nb);
-          tma_load_3d(sb + kKBytes, &tmV, kv_full0 + 8 * st, 0, j * kBK, w.nb);
+          tma_load_3d(sb, &tmK, kv_full0 + 8 * st, 0, (w.kb0 + j) * kBK, w.nb);
+          tma_load_3d(sb + kKBytes, &tmV, kv_full0 + 8 * st, 0, (w.kb0 + j) * kBK, w.nb);
           if (++st == kDqStages) { st = 0; ph ^= 1; }
         }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       const uint32_t idesc = make_idesc(kBK);
       bool ok = true;
-      int it = 0;
+      int it = -1;
       uint32_t n0 = 0;
       int sst = 0;                // ring stage and phase of the next block to get its S product
       uint32_t sph = 0;
@@ -524,10 +705,11 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         if (++sst == kDqStages) { sst = 0; sph ^= 1; }
         return true;
       };
-      for (int t = blockIdx.x; ok && t < n_tiles; t += gridDim.x, ++it) {
-        const FwdTile w = fwd_tile(tp, t);
+      while (ok && walk.get(w)) {
+        if (MASKED && w.nkb == 0) continue;
+        ++it;
         ok = mbar_wait(q_full, it & 1, abort_flag, 84, p.status);
-        for (int j = 0; ok && j < 2; ++j) ok = issue_s(n0 + j);   // nkb >= 2
+        for (int j = 0; ok && j < 2 && j < w.nkb; ++j) ok = issue_s(n0 + j);
         for (int j = 0; ok && j < w.nkb; ++j) {
           const uint32_t n = n0 + j;
           const uint32_t sb = base + kDqOffStage + dst * kDqStageBytes;
@@ -566,14 +748,15 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
     bool ok = true;
     uint32_t n0 = 0;
-    int it = 0;
-    for (int t = blockIdx.x; ok && t < n_tiles; t += gridDim.x, ++it) {
-      const FwdTile w = fwd_tile(tp, t);
+    int it = -1;
+    std::conditional_t<MASKED, Shape<CAP, BIAS>, NoCall> shape(c);
+    while (ok && walk.get(w)) {
       const int qpos = w.qb * kBQ + row;
       // delta = sum_d dO * O of this row, straight from global memory (once per item)
       float delta = 0.0f, lse2 = INFINITY;   // of a row behind position S: P = dS = 0
       if (qpos < p.S) {
         lse2 = p.lse[w.qrow0 + row] * kLog2e;
+        if (MASKED && lse2 == -INFINITY) lse2 = INFINITY;   // a row that sees nothing
         const int64_t ooff = o_offset(p.S, p.G, p.HKV, p.o_tok, w.nb, w.g, w.qb * kBQ + row);
         const uint4* o4 = reinterpret_cast<const uint4*>(p.O + ooff);
         const uint4* d4 = reinterpret_cast<const uint4*>(p.dO + ooff);
@@ -591,14 +774,29 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       const int64_t prow = (static_cast<int64_t>(w.nb) * p.G + w.g) * (q_blocks(p.S) * kBQ) + qpos;
       p.ndelta[prow] = -delta;
       p.nlse2[prow] = -lse2;
-      const float2 sc2 = f2(p.sc, p.sc), nl2 = f2(-lse2, -lse2), nd2 = f2(-delta, -delta);
+      int2 sees = make_int2(0, 0);
+      if constexpr (MASKED) {
+        if (qpos < p.S) sees = c.mask.rows[static_cast<int64_t>(w.b) * p.S + qpos];
+        if constexpr (BIAS) shape.slope2 = c.slopes[w.hk * p.G + w.g] * kLog2e;
+        if (w.nkb == 0) {
+          if (qpos < p.S) {
+            uint4* orow = reinterpret_cast<uint4*>(p.dQ + (w.qrow0 + row) * kD);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) orow[i] = make_uint4(0, 0, 0, 0);
+          }
+          continue;
+        }
+      }
+      ++it;
+      const float sc = CAP || BIAS ? 1.0f : p.sc;
+      const float2 sc2 = f2(sc, sc), nl2 = f2(-lse2, -lse2), nd2 = f2(-delta, -delta);
       for (int j = 0; j < w.nkb; ++j) {
         const uint32_t n = n0 + j;
         ok = __all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * (n & 1), (n >> 1) & 1, abort_flag, 88, p.status));
         if (!ok) break;
         tcgen05_fence_after();
-        const int key0 = j * kBK;
-        const bool diag = key0 + kBK - 1 > w.qb * kBQ;
+        const int key0 = (w.kb0 + j) * kBK;
+        const bool diag = !MASKED && key0 + kBK - 1 > w.qb * kBQ;
         // the row's 64 scores, read once; P = 2^(s*sc - lse2) takes their place in the registers
         uint32_t sv[4][16];
 #pragma unroll
@@ -607,12 +805,28 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_free0 + 8 * (n & 1));   // the buffer may take block n + 2
+        uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+        bool edge = false;
+        if constexpr (MASKED) {
+          edge = key0 < sees.x || key0 + kBK > sees.y;
+          if (edge) { seen[0] = interval_bits(sees.x, sees.y, key0); seen[1] = interval_bits(sees.x, sees.y, key0 + 32); }
+        }
 #pragma unroll
         for (int c4 = 0; c4 < 4; ++c4) {
+          float2 slope[CAP ? 8 : 1];   // 1 - tanh^2, which joins P: only their product counts here
+          if constexpr (CAP || BIAS)
+            shape.apply(sv[c4], static_cast<float>(qpos - key0 - 16 * c4), -1.0f, [&](int e, float2 t) {
+              if constexpr (CAP) slope[e >> 1] = __ffma2_rn(t, f2(-t.x, -t.y), f2(1.0f, 1.0f));
+            });
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
             const float2 tt = __ffma2_rn(f2(__uint_as_float(sv[c4][e]), __uint_as_float(sv[c4][e + 1])), sc2, nl2);
             float p0 = ex2(tt.x), p1 = ex2(tt.y);
+            if constexpr (CAP) { p0 *= slope[e >> 1].x; p1 *= slope[e >> 1].y; }
+            if (MASKED && edge) {
+              if ((seen[c4 >> 1] >> (16 * (c4 & 1) + e) & 1u) == 0) p0 = 0.0f;
+              if ((seen[c4 >> 1] >> (16 * (c4 & 1) + e + 1) & 1u) == 0) p1 = 0.0f;
+            }
             if (diag) {
               if (key0 + 16 * c4 + e > qpos) p0 = 0.0f;
               if (key0 + 16 * c4 + e + 1 > qpos) p1 = 0.0f;
@@ -658,7 +872,16 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(dq_free);   // the next item's products may overwrite dQ
-      if (qpos < p.S) {
+      bool bad = false;
+      if constexpr (MASKED) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int c4 = 0; c4 < 4; ++c4)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sum = fmaf(__uint_as_float(qv[c4][e]), 0.0f, sum);
+        bad = qpos < p.S && !(sum == 0.0f);
+      }
+      if (qpos < p.S && !bad) {
         __nv_bfloat16* orow = p.dQ + (w.qrow0 + row) * kD;
 #pragma unroll
         for (int c4 = 0; c4 < 4; ++c4) {
@@ -669,6 +892,10 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
           *reinterpret_cast<uint4*>(orow + 16 * c4) = make_uint4(ow[0], ow[1], ow[2], ow[3]);
           *reinterpret_cast<uint4*>(orow + 16 * c4 + 8) = make_uint4(ow[4], ow[5], ow[6], ow[7]);
         }
+      }
+      if constexpr (MASKED) {
+        for (uint32_t rows = __ballot_sync(0xffffffffu, bad); rows != 0; rows &= rows - 1)
+          mattn::dq_row<__nv_bfloat16>(c, w.b, w.hk, w.g, w.qb * kBQ + quad * 32 + __ffs(rows) - 1);
       }
       n0 += static_cast<uint32_t>(w.nkb);
     }
@@ -707,7 +934,8 @@ constexpr uint32_t kKvOffStage = kKvOffV + kQBytes;   // per stage: Q and dO til
 constexpr uint32_t kKvStageBytes = 2 * kKBytes + 512;
 constexpr uint32_t kKvStageStride = 2 * kKBytes + 1024;
 constexpr uint32_t kKvOffBar = kKvOffStage + kKvStages * kKvStageStride;
-constexpr uint32_t kKvSmem = kKvOffBar + 256 + 1024;
+constexpr uint32_t kKvOffBad = kKvOffBar + 256;
+constexpr uint32_t kKvSmem = kKvOffBad + kBQ * 4 + 1024;
 static_assert(2 * kBQ * kD * 4 <= kKvStages * kKvStageStride, "the parts' sums reuse the load ring");
 
 __device__ __forceinline__ void bulk_load_1d(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -715,9 +943,11 @@ __device__ __forceinline__ void bulk_load_1d(uint32_t dst, const void* src, uint
                ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
+template <bool MASKED, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kKvThreads, 1)
 attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmdO, const BwdParams p) {
+                const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmdO, const BwdParams p,
+                const __grid_constant__ CallOf<MASKED> c) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen_base = smem_raw + (base - smem_u32(smem_raw));
@@ -729,6 +959,8 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
   const uint32_t pds_ready0 = sdp_full0 + 16, out_full = pds_ready0 + 16, tmem_slot = out_full + 8, abort_addr = tmem_slot + 4;
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(gen_base + (tmem_slot - base));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_base + (abort_addr - base));
+  volatile int* bad = reinterpret_cast<volatile int*>(gen_base + kKvOffBad);   // MASKED: key rows that came out not finite
+  if (MASKED && threadIdx.x < kBQ) bad[threadIdx.x] = 0;
 
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
@@ -754,17 +986,28 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
   const uint32_t tDV = tmem_base + 256, tDK = tmem_base + 320, tPT0 = tmem_base + 384;
 
   // all kv heads of key block 0 (the most query steps) start first
-  const int kb = blockIdx.y, part = blockIdx.x % p.kv_parts, nb = blockIdx.x / p.kv_parts;
-  const int nq = (p.S + kBK - 1) / kBK;          // query steps of 64 per head
-  const int i0 = 2 * kb;                         // first query step that sees this key block
-  const int per_head = nq - i0;
+  const int part = blockIdx.x % p.kv_parts;
+  int kb, nb, i0, per_head;   // key block, kv head; first query step (of 64) that sees this key block, steps per head
+  int b = 0, hk = 0;
+  if constexpr (MASKED) {
+    const int item = blockIdx.x / p.kv_parts;
+    const int4 rec = c.mask.kwork[item / c.Hk];
+    hk = item % c.Hk;
+    b = rec.x; kb = rec.y; i0 = rec.z; per_head = rec.w;
+    nb = b * c.Hk + hk;
+  } else {
+    kb = blockIdx.y;
+    nb = blockIdx.x / p.kv_parts;
+    i0 = 2 * kb;
+    per_head = (p.S + kBK - 1) / kBK - i0;
+  }
   // this CTA's steps [t0, t0 + nsteps) of the key block's G * per_head; a part may be empty
   const int all_steps = p.G * per_head;
   const int t0 = static_cast<int>(static_cast<int64_t>(all_steps) * part / p.kv_parts);
   const int nsteps = static_cast<int>(static_cast<int64_t>(all_steps) * (part + 1) / p.kv_parts) - t0;
 
   if (warp == 0) {
-    if (lane == 0 && nsteps > 0) {
+    if (elect_one() && nsteps > 0) {
       mbar_expect_tx(kv_full, 2 * kQBytes);
       tma_load_3d(base + kKvOffK, &tmK, kv_full, 0, kb * kBQ, nb);
       tma_load_3d(base + kKvOffV, &tmV, kv_full, 0, kb * kBQ, nb);
@@ -784,7 +1027,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       const uint32_t idesc = make_idesc(kBK);
       // descriptors of the resident K / V block and of stage 0's Q / dO tiles (K-major for S^T and dP^T, as N-major
       // B operands for dV and dK), built once; a stage or a K slice further is one add
@@ -847,6 +1090,12 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     const int key = kb * kBQ + row;
     const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
     bool ok = true;
+    int2 seen = make_int2(0, 0);   // the queries that see this key
+    if constexpr (MASKED) {
+      if (key < p.S) seen = c.mask.keys[static_cast<int64_t>(b) * p.S + key];
+    }
+    std::conditional_t<MASKED, Shape<CAP, BIAS>, NoCall> shape(c);
+    const float sc = CAP || BIAS ? 1.0f : p.sc;
     for (int t = group; t < nsteps; t += 2) {
       const int st = group;
       const int i = i0 + (t0 + t) % per_head;
@@ -859,13 +1108,25 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
       const float* st_nl2 = reinterpret_cast<const float*>(gen_base + kKvOffStage + (t % kKvStages) * kKvStageStride + 2 * kKBytes) + half * 32;
       const float* st_nd = st_nl2 + 64;
       const int q0 = i * kBK + half * 32;
-      const bool diag = i * kBK < (kb + 1) * kBQ;   // some query of this step lies before some key of the block
-      const float2 sc2 = f2(p.sc, p.sc);
+      const bool diag = !MASKED && i * kBK < (kb + 1) * kBQ;   // some query of this step lies before some key of the block
+      uint32_t bits = 0xffffffffu;
+      bool edge = false;
+      if constexpr (MASKED) {
+        edge = q0 < seen.x || q0 + 32 > seen.y;
+        if (edge) bits = interval_bits(seen.x, seen.y, q0);
+        if constexpr (BIAS) shape.slope2 = c.slopes[hk * p.G + (t0 + t) / per_head] * kLog2e;
+      }
+      const float2 sc2 = f2(sc, sc);
       // the exponentials are taken while dP^T is still on its way from tensor memory
       uint32_t vs[32], vd[32];
       tmem_ld_x32(tS + half * 32, vs);
       tmem_ld_wait_on(vs);
       tmem_ld_x32(tDP + half * 32, vd);
+      float2 slope[CAP ? 16 : 1];   // 1 - tanh^2
+      if constexpr (CAP || BIAS)
+        shape.apply(vs, static_cast<float>(q0 - key), 1.0f, [&](int e, float2 t2) {
+          if constexpr (CAP) slope[e >> 1] = __ffma2_rn(t2, f2(-t2.x, -t2.y), f2(1.0f, 1.0f));
+        });
 #pragma unroll
       for (int e = 0; e < 32; e += 4) {
         const float4 nl = *reinterpret_cast<const float4*>(st_nl2 + e);
@@ -875,6 +1136,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           if (diag && key > q0 + e + x) pr[x] = 0.0f;
+          if (MASKED && edge && (bits >> (e + x) & 1u) == 0) pr[x] = 0.0f;
           vs[e + x] = __float_as_uint(pr[x]);
         }
       }
@@ -884,8 +1146,12 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
       for (int e = 0; e < 32; e += 4) {
         const float4 nd = *reinterpret_cast<const float4*>(st_nd + e);
         const float2 pa = f2(__uint_as_float(vs[e]), __uint_as_float(vs[e + 1])), pb = f2(__uint_as_float(vs[e + 2]), __uint_as_float(vs[e + 3]));
-        const float2 da = __fmul2_rn(pa, __fadd2_rn(f2(__uint_as_float(vd[e]), __uint_as_float(vd[e + 1])), f2(nd.x, nd.y)));
-        const float2 db = __fmul2_rn(pb, __fadd2_rn(f2(__uint_as_float(vd[e + 2]), __uint_as_float(vd[e + 3])), f2(nd.z, nd.w)));
+        float2 da = __fmul2_rn(pa, __fadd2_rn(f2(__uint_as_float(vd[e]), __uint_as_float(vd[e + 1])), f2(nd.x, nd.y)));
+        float2 db = __fmul2_rn(pb, __fadd2_rn(f2(__uint_as_float(vd[e + 2]), __uint_as_float(vd[e + 3])), f2(nd.z, nd.w)));
+        if constexpr (CAP) {
+          da = __fmul2_rn(da, slope[e >> 1]);
+          db = __fmul2_rn(db, slope[(e >> 1) + 1]);
+        }
         wp[e >> 1] = pack_bf16(pa.x, pa.y);
         wp[(e >> 1) + 1] = pack_bf16(pb.x, pb.y);
         wd[e >> 1] = pack_bf16(da.x, da.y);
@@ -909,6 +1175,10 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         uint32_t v[16];
         tmem_ld_x16((group == 0 ? tDV : tDK) + lane_addr + c, v);
         tmem_ld_wait();
+        if (MASKED && nsteps == 0) {   // nothing sees this key block: the accumulators were never written
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[e] = 0;
+        }
         if (p.kv_parts > 1) {
           // this part's sums, column by column, into the load ring (every step's tiles have been read)
           float* at = reinterpret_cast<float*>(gen_base + kKvOffStage) + (group * kD + c) * kBQ + row;
@@ -916,6 +1186,12 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
           for (int e = 0; e < 16; ++e) at[e * kBQ] = nsteps > 0 ? __uint_as_float(v[e]) : 0.0f;
         } else if (key < p.S) {
           uint32_t w[8];
+          if constexpr (MASKED) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sum = fmaf(__uint_as_float(v[e]), 0.0f, sum);
+            if (!(sum == 0.0f)) bad[row] = 1;
+          }
 #pragma unroll
           for (int e = 0; e < 16; e += 2) w[e >> 1] = pack_bf16(__uint_as_float(v[e]) * f, __uint_as_float(v[e + 1]) * f);
           *reinterpret_cast<uint4*>(orow + c) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -944,6 +1220,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
 #pragma unroll
           for (int k = 0; k < 4; ++k) a[k] += peer[k * kBQ];
         }
+        if (MASKED && kb * kBQ + row < p.S && !((a[0] + a[1] + a[2] + a[3]) * 0.0f == 0.0f)) bad[row] = 1;
         if (kb * kBQ + row < p.S) *reinterpret_cast<uint2*>(orow + c) = make_uint2(pack_bf16(a[0] * f, a[1] * f), pack_bf16(a[2] * f, a[3] * f));
       }
     }
@@ -956,6 +1233,12 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
   }
   tcgen05_fence_before();
   __syncthreads();
+  if constexpr (MASKED) {
+    // (a key row's gradients were written by threads of this block, before the barrier)
+    if (warp >= 2)
+      for (int r = warp - 2; r < kBQ; r += kKvThreads / 32 - 2)
+        if (bad[r] != 0) mattn::dkv_row<__nv_bfloat16>(c, b, hk, kb * kBQ + r);
+  }
   if (warp == 1) {
     tcgen05_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
@@ -1058,7 +1341,7 @@ int attention_fwd(const void* q, const void* k, const void* v, void* o, float* l
   int dev = 0;
   MCB_CHECK_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) return fail(MCB_ERR_SHAPE, "attention: device %d out of range", dev);
-  if (int rc = set_attrs_once(reinterpret_cast<const void*>(attn_fwd_kernel), kFwdSmem, &attr_set[dev])) return rc;
+  if (int rc = set_attrs_once(reinterpret_cast<const void*>(attn_fwd_kernel<false, false, false>), kFwdSmem, &attr_set[dev])) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   CUtensorMap tmQ, tmK, tmVt;
   if (int rc = encode(ds, &tmQ, q, kD, seq, nb * groups, kBQ, "Q")) return rc;
@@ -1073,7 +1356,7 @@ int attention_fwd(const void* q, const void* k, const void* v, void* o, float* l
   const int64_t n_tiles = q_blocks(static_cast<int>(seq)) * groups * nb;
   const int64_t slots = 2 * static_cast<int64_t>(ds->sm_count);
   const unsigned grid = static_cast<unsigned>(n_tiles < slots ? n_tiles : slots);
-  MCB_CHECK_CUDA(launch_kernel(attn_fwd_kernel, dim3(grid), dim3(kThreads), kFwdSmem, st, chained_launch(), tmQ, tmK, tmVt, p));
+  MCB_CHECK_CUDA(launch_kernel(attn_fwd_kernel<false, false, false>, dim3(grid), dim3(kThreads), kFwdSmem, st, chained_launch(), tmQ, tmK, tmVt, p, NoCall()));
   MCB_CHECK_LAUNCH("attn_fwd_kernel");
   return MCB_OK;
 }
@@ -1127,8 +1410,8 @@ int attention_bwd(const void* q, const void* k, const void* v, const void* o, co
   int dev = 0;
   MCB_CHECK_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) return fail(MCB_ERR_SHAPE, "attention: device %d out of range", dev);
-  if (int rc = set_attrs_once(reinterpret_cast<const void*>(attn_dq_kernel), kDqSmem, &attr_dq[dev])) return rc;
-  if (int rc = set_attrs_once(reinterpret_cast<const void*>(attn_dkv_kernel), kKvSmem, &attr_kv[dev])) return rc;
+  if (int rc = set_attrs_once(reinterpret_cast<const void*>(attn_dq_kernel<false, false, false>), kDqSmem, &attr_dq[dev])) return rc;
+  if (int rc = set_attrs_once(reinterpret_cast<const void*>(attn_dkv_kernel<false, false, false>), kKvSmem, &attr_kv[dev])) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const size_t rows = static_cast<size_t>(nb) * groups * q_blocks(static_cast<int>(seq)) * kBQ * 4;
   uint8_t* w = static_cast<uint8_t*>(workspace);
@@ -1158,7 +1441,8 @@ int attention_bwd(const void* q, const void* k, const void* v, const void* o, co
   const int64_t n_tiles = q_blocks(static_cast<int>(seq)) * groups * nb;
   const int64_t slots = 2 * static_cast<int64_t>(ds->sm_count);
   const unsigned gq = static_cast<unsigned>(n_tiles < slots ? n_tiles : slots);
-  MCB_CHECK_CUDA(launch_kernel(attn_dq_kernel, dim3(gq), dim3(kThreads), kDqSmem, st, chained_launch(), tmQ128, tmdO128, tmK64, tmV64, p));
+  MCB_CHECK_CUDA(launch_kernel(attn_dq_kernel<false, false, false>, dim3(gq), dim3(kThreads), kDqSmem, st, chained_launch(), tmQ128, tmdO128, tmK64, tmV64, p,
+                               NoCall()));
   MCB_CHECK_LAUNCH("attn_dq_kernel");
   p.kv_parts = dkv_parts(nb, groups, seq, ds->sm_count);
   cudaLaunchConfig_t cfg = {};
@@ -1171,7 +1455,7 @@ int attention_bwd(const void* q, const void* k, const void* v, const void* o, co
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = static_cast<unsigned>(p.kv_parts); attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr; cfg.numAttrs = p.kv_parts > 1 ? 2 : 1;
-  MCB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attn_dkv_kernel, tmK128, tmV128, tmQ64, tmdO64, p));
+  MCB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attn_dkv_kernel<false, false, false>, tmK128, tmV128, tmQ64, tmdO64, p, NoCall()));
   MCB_CHECK_LAUNCH("attn_dkv_kernel");
   return MCB_OK;
 }
@@ -1202,3 +1486,104 @@ extern "C" int mcb_attention_causal_bwd(const void* q, const void* k, const void
   return mcb_attention_causal_bwd_ex(q, k, v, o, dout, lse, dq, dk, dv, nb, groups, seq, head_dim, scale, dtype, 1, 0,
                                      workspace, workspace_bytes, stream);
 }
+
+// ---- under a mask (entry points and checks in masked_attn.cu) ----
+namespace mcb {
+namespace mattn {
+namespace {
+using namespace attn;
+
+// The kernels' instances by what the score has besides the product, and their attributes, set once per device.
+template <bool CAP, bool BIAS>
+struct Form {
+  static constexpr auto fwd = attn_fwd_kernel<true, CAP, BIAS>;
+  static constexpr auto dq = attn_dq_kernel<true, CAP, BIAS>;
+  static constexpr auto dkv = attn_dkv_kernel<true, CAP, BIAS>;
+  static int prepare(int dev) {
+    static bool done[3][64] = {};
+    if (int rc = set_attrs_once(reinterpret_cast<const void*>(fwd), kFwdSmem, &done[0][dev])) return rc;
+    if (int rc = set_attrs_once(reinterpret_cast<const void*>(dq), kDqSmem, &done[1][dev])) return rc;
+    return set_attrs_once(reinterpret_cast<const void*>(dkv), kKvSmem, &done[2][dev]);
+  }
+};
+
+template <bool CAP, bool BIAS>
+int fwd_form(const Call& c, const DeviceState* ds, cudaStream_t st) {
+  int dev = 0;
+  MCB_CHECK_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return fail(MCB_ERR_SHAPE, "masked attention: device %d out of range", dev);
+  if (int rc = Form<CAP, BIAS>::prepare(dev)) return rc;
+  const int64_t nb = static_cast<int64_t>(c.B) * c.Hk;
+  CUtensorMap tmQ, tmK, tmV;
+  if (int rc = encode(ds, &tmQ, c.q, kD, c.S, nb * c.G, kBQ, "Q")) return rc;
+  if (int rc = encode(ds, &tmK, c.k, kD, c.S, nb, kBK, "K")) return rc;
+  if (int rc = encode(ds, &tmV, c.v, kD, c.S, nb, kBK, "V")) return rc;
+  FwdParams p;
+  p.S = c.S; p.G = c.G; p.NB = static_cast<int>(nb); p.HKV = c.Hk; p.o_tok = c.o_tok;
+  p.sc = c.scale * attn::kLog2e;
+  p.O = static_cast<__nv_bfloat16*>(c.o); p.lse = c.lse; p.status = ds->status_word;
+  const int64_t n_tiles = static_cast<int64_t>(q_blocks(c.S)) * c.G * nb, slots = 2 * static_cast<int64_t>(ds->sm_count);
+  MCB_CHECK_CUDA(launch_kernel(Form<CAP, BIAS>::fwd, dim3(static_cast<unsigned>(n_tiles < slots ? n_tiles : slots)), dim3(attn::kThreads), kFwdSmem, st,
+                               chained_launch(), tmQ, tmK, tmV, p, c));
+  MCB_CHECK_LAUNCH("attn_fwd_kernel");
+  return MCB_OK;
+}
+
+template <bool CAP, bool BIAS>
+int bwd_form(const Call& c, const DeviceState* ds, cudaStream_t st) {
+  int dev = 0;
+  MCB_CHECK_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return fail(MCB_ERR_SHAPE, "masked attention: device %d out of range", dev);
+  if (int rc = Form<CAP, BIAS>::prepare(dev)) return rc;
+  const int64_t nb = static_cast<int64_t>(c.B) * c.Hk;
+  const int64_t do_inner = c.o_tok ? static_cast<int64_t>(c.Hk) * c.G * kD : kD, do_planes = c.o_tok ? c.B : nb * c.G;
+  CUtensorMap tmQ128, tmdO128, tmK64, tmV64, tmK128, tmV128, tmQ64, tmdO64;
+  if (int rc = encode(ds, &tmQ128, c.q, kD, c.S, nb * c.G, kBQ, "Q")) return rc;
+  if (int rc = encode(ds, &tmdO128, c.dout, do_inner, c.S, do_planes, kBQ, "dO")) return rc;
+  if (int rc = encode(ds, &tmK64, c.k, kD, c.S, nb, kBK, "K")) return rc;
+  if (int rc = encode(ds, &tmV64, c.v, kD, c.S, nb, kBK, "V")) return rc;
+  if (int rc = encode(ds, &tmK128, c.k, kD, c.S, nb, kBQ, "K block")) return rc;
+  if (int rc = encode(ds, &tmV128, c.v, kD, c.S, nb, kBQ, "V block")) return rc;
+  if (int rc = encode(ds, &tmQ64, c.q, kD, c.S, nb * c.G, kBK, "Q step")) return rc;
+  if (int rc = encode(ds, &tmdO64, c.dout, do_inner, c.S, do_planes, kBK, "dO step")) return rc;
+  BwdParams p;
+  p.S = c.S; p.G = c.G; p.NB = static_cast<int>(nb); p.HKV = c.Hk; p.o_tok = c.o_tok;
+  p.sc = c.scale * attn::kLog2e; p.scale = c.scale;
+  p.O = static_cast<const __nv_bfloat16*>(c.o_in); p.dO = static_cast<const __nv_bfloat16*>(c.dout); p.lse = c.lse;
+  p.ndelta = c.ndelta; p.nlse2 = c.nlse2;
+  p.dQ = static_cast<__nv_bfloat16*>(c.dq); p.dK = static_cast<__nv_bfloat16*>(c.dk); p.dV = static_cast<__nv_bfloat16*>(c.dv);
+  p.status = ds->status_word;
+  const int64_t n_tiles = static_cast<int64_t>(q_blocks(c.S)) * c.G * nb, slots = 2 * static_cast<int64_t>(ds->sm_count);
+  p.kv_parts = 1;
+  MCB_CHECK_CUDA(launch_kernel(Form<CAP, BIAS>::dq, dim3(static_cast<unsigned>(n_tiles < slots ? n_tiles : slots)), dim3(attn::kThreads), kDqSmem, st,
+                               chained_launch(), tmQ128, tmdO128, tmK64, tmV64, p, c));
+  MCB_CHECK_LAUNCH("attn_dq_kernel");
+  p.kv_parts = dkv_parts(nb, c.G, c.S, ds->sm_count);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(nb * q_blocks(c.S) * p.kv_parts));
+  cfg.blockDim = dim3(kKvThreads);
+  cfg.dynamicSmemBytes = kKvSmem; cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = chained_launch() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(p.kv_parts); attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr; cfg.numAttrs = p.kv_parts > 1 ? 2 : 1;
+  MCB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, Form<CAP, BIAS>::dkv, tmK128, tmV128, tmQ64, tmdO64, p, c));
+  MCB_CHECK_LAUNCH("attn_dkv_kernel");
+  return MCB_OK;
+}
+
+}  // namespace
+
+int launch_fwd_umma(const Call& c, const DeviceState* ds, cudaStream_t st) {
+  if (c.cap > 0.0f) return c.slopes ? fwd_form<true, true>(c, ds, st) : fwd_form<true, false>(c, ds, st);
+  return c.slopes ? fwd_form<false, true>(c, ds, st) : fwd_form<false, false>(c, ds, st);
+}
+int launch_bwd_umma(const Call& c, const DeviceState* ds, cudaStream_t st) {
+  if (c.cap > 0.0f) return c.slopes ? bwd_form<true, true>(c, ds, st) : bwd_form<true, false>(c, ds, st);
+  return c.slopes ? bwd_form<false, true>(c, ds, st) : bwd_form<false, false>(c, ds, st);
+}
+
+}  // namespace mattn
+}  // namespace mcb

@@ -24,6 +24,7 @@ __device__ __forceinline__ double block_sum(double v, double* s) {
   return sum;
 }
 __device__ __forceinline__ float norm_of(const double* part, int parts, double* s) {
+  part = from_here(part);
   double v = 0.0;
   for (int i = threadIdx.x; i < parts; i += 256) v += __ldcg(part + i);
   return static_cast<float>(sqrt(block_sum(v, s)));

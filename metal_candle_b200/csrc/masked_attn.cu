@@ -124,13 +124,13 @@ __device__ __forceinline__ float row_sum(float v) {
 struct Item {
   int b, first, head;
 };
-__device__ __forceinline__ Item item_of(const Call& c, const int* order, int heads) {
-  const int tiles = static_cast<int>(amask::tiles_of(c.S));
-  const int half = blockIdx.x / heads, t = order[half >> 1];
+__device__ __forceinline__ Item item_of(const int4* work, int heads) {
+  const int half = blockIdx.x / heads;
+  const int4 t = work[half >> 1];
   Item w;
   w.head = blockIdx.x % heads;
-  w.b = t / tiles;
-  w.first = t % tiles * amask::kTile + (half & 1) * kB;
+  w.b = t.x;
+  w.first = t.y * amask::kTile + (half & 1) * kB;
   return w;
 }
 // The intervals of the tile's rows into shared memory, and the positions that any of them covers.  All threads.
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kThreads) masked_fwd_kernel(const __grid_const
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   grid_launch_dependents();
   grid_dependency_wait();
-  const Item w = item_of(c, c.mask.qorder, c.Hk * c.G);
+  const Item w = item_of(c.mask.qwork, c.Hk * c.G);
   if (w.first >= c.S) return;
   const int hk = w.head / c.G, g = w.head % c.G;
   if (threadIdx.x < kB) bad[threadIdx.x] = 0;
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kThreads) masked_dq_kernel(const __grid_consta
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   grid_launch_dependents();
   grid_dependency_wait();
-  const Item w = item_of(c, c.mask.qorder, c.Hk * c.G);
+  const Item w = item_of(c.mask.qwork, c.Hk * c.G);
   if (w.first >= c.S) return;
   const int hk = w.head / c.G, g = w.head % c.G;
   if (threadIdx.x < kB) bad[threadIdx.x] = 0;
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(kThreads) masked_dkv_kernel(const __grid_const
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   grid_launch_dependents();
   grid_dependency_wait();
-  const Item w = item_of(c, c.mask.korder, c.Hk);
+  const Item w = item_of(c.mask.kwork, c.Hk);
   if (w.first >= c.S) return;
   const int hk = w.head;
   if (threadIdx.x < kB) bad[threadIdx.x] = 0;
@@ -424,6 +424,9 @@ size_t stat_bytes(const mcb_masked_attention* a) {
   return up1k(static_cast<size_t>(a->batch) * a->kv_heads * a->groups * amask::tiles_of(a->seq) * amask::kTile * 4);
 }
 
+// What flash_attn.cu takes: its tiles are built for heads of 64.
+bool tensor_cores(const mcb_masked_attention* a) { return a->dtype == MCB_BF16 && a->head_dim == 64; }
+
 int fill(Call& c, const mcb_masked_attention* a, const char* who) {
   if (!a) return fail(MCB_ERR_NULL, "%s: the call is null", who);
   if (!a->mask) return fail(MCB_ERR_NULL, "%s: mask is null", who);
@@ -437,7 +440,7 @@ int fill(Call& c, const mcb_masked_attention* a, const char* who) {
   if (a->kv_heads <= 0 || a->groups <= 0 || a->kv_heads > 0x7fffffff || a->groups > 0x7fffffff / a->kv_heads ||
       a->batch * amask::tiles_of(a->seq) > 0x07ffffffll / (a->kv_heads * a->groups))
     return fail(MCB_ERR_SHAPE, "%s: batch=%lld kv_heads=%lld groups=%lld seq=%lld", who, (long long)a->batch, (long long)a->kv_heads, (long long)a->groups, (long long)a->seq);
-  if (!(a->scale - a->scale == 0.0f)) return fail(MCB_ERR_SHAPE, "%s: scale is not finite", who);
+  if (!(a->scale > 0.0f && a->scale - a->scale == 0.0f)) return fail(MCB_ERR_SHAPE, "%s: scale must be positive and finite", who);
   if (!(a->softcap >= 0.0f && a->softcap - a->softcap == 0.0f)) return fail(MCB_ERR_SHAPE, "%s: softcap must be 0 (none) or positive and finite", who);
   if (!aligned16(a->mask) || (reinterpret_cast<uintptr_t>(a->slopes) & 3) != 0) return fail(MCB_ERR_ALIGN, "%s: alignment of the mask or the slopes", who);
   c = Call{};
@@ -467,6 +470,7 @@ extern "C" int mcb_attention_masked_fwd(const mcb_masked_attention* a, const voi
   if (!ds) return MCB_ERR_NOT_INIT;
   c.q = q; c.k = k; c.v = v; c.o = o; c.lse = lse; c.status = ds->status_word;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (mattn::tensor_cores(a)) return mattn::launch_fwd_umma(c, ds, st);
   return a->dtype == MCB_F32 ? mattn::launch_fwd<float>(c, st) : mattn::launch_fwd<__nv_bfloat16>(c, st);
 }
 
@@ -495,5 +499,6 @@ extern "C" int mcb_attention_masked_bwd(const mcb_masked_attention* a, const voi
   c.nlse2 = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + stat);
   c.status = ds->status_word;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (mattn::tensor_cores(a)) return mattn::launch_bwd_umma(c, ds, st);
   return a->dtype == MCB_F32 ? mattn::launch_bwd<float>(c, st) : mattn::launch_bwd<__nv_bfloat16>(c, st);
 }

@@ -173,7 +173,8 @@ def test_the_mask_as_intervals(cuda_device, B, S, longest):
         rows, keys = words[:2 * n].view(B, S, 2), words[2 * n:4 * n].view(B, S, 2)
         at = 4 * n
         ranges = words[at:at + 4 * B * tiles].view(2, B, tiles, 2)
-        order = words[at + 4 * B * tiles:at + 6 * B * tiles].view(2, B * tiles)
+        at = (at + 4 * B * tiles + 3) // 4 * 4
+        work = words[at:at + 8 * B * tiles].view(2, B * tiles, 4)
         for b in range(B):
             want_rows, want_keys = expected_intervals(ids[b], None if pre is None else pre[b])
             for got, want, tile in ((rows[b], want_rows, ranges[0, b]), (keys[b], want_keys, ranges[1, b])):
@@ -188,8 +189,10 @@ def test_the_mask_as_intervals(cuda_device, B, S, longest):
                     else:
                         assert first == int(part[:, 0].min()) // 64 and first + count == (int(part[:, 1].max()) + 63) // 64
         for k in range(2):
-            assert sorted(order[k].tolist()) == list(range(B * tiles))
-            counts = ranges[k].reshape(-1, 2)[:, 1][order[k].long()]
+            order = (work[k, :, 0] * tiles + work[k, :, 1]).long()
+            assert sorted(order.tolist()) == list(range(B * tiles))
+            assert torch.equal(work[k, :, 2:], ranges[k].reshape(-1, 2)[order])
+            counts = work[k, :, 3]
             assert (counts[:-1].double() - counts[1:] >= -counts.max().double() / 1023).all()
 
 

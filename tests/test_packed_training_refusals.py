@@ -44,7 +44,8 @@ def attention(**change):
 REFUSED = [(dict(mask=None), NULL), (dict(dtype=2), UNSUPPORTED), (dict(seq=0), SHAPE), (dict(batch=0), SHAPE), (dict(mask_bytes=64), SHAPE),
            (dict(head_dim=0), UNSUPPORTED), (dict(head_dim=4), UNSUPPORTED), (dict(head_dim=60), UNSUPPORTED), (dict(head_dim=136), UNSUPPORTED),
            (dict(kv_heads=0), SHAPE), (dict(groups=0), SHAPE), (dict(kv_heads=1 << 20, groups=1 << 20), SHAPE), (dict(groups=1 << 26), SHAPE),
-           (dict(scale=math.nan), SHAPE), (dict(scale=math.inf), SHAPE), (dict(softcap=-1.0), SHAPE), (dict(softcap=math.nan), SHAPE),
+           (dict(scale=math.nan), SHAPE), (dict(scale=math.inf), SHAPE), (dict(scale=0.0), SHAPE),
+           (dict(scale=-0.1), SHAPE), (dict(softcap=-1.0), SHAPE), (dict(softcap=math.nan), SHAPE),
            (dict(softcap=math.inf), SHAPE), (dict(mask=24), ALIGN), (dict(slopes=17), ALIGN)]
 
 
