@@ -488,7 +488,7 @@ int mcb_embedding_scaled_fwd(const void* ids, int id_bytes, const void* table, v
                              float scale, int dtype, void* stream);
 /* Its table's gradient, for a table that is trained: dtable[v,:] = scale * sum of dout[m,:] over ids[m] = v, [vocab, H] float32 from a
  * 16-byte boundary, written whole (accumulate: added to, where a token has the id).  dout [M, H] dtype.  Terms are summed in token
- * order, in parts of 32: the same bits every time. */
+ * order, in parts of 8 to 32: the same bits every time. */
 size_t mcb_embedding_bwd_workspace_bytes(int64_t M, int64_t H);
 int mcb_embedding_bwd(const void* ids, int id_bytes, const void* dout, float* dtable, int accumulate, int64_t M, int64_t H,
                       int64_t vocab, float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);

@@ -8,7 +8,7 @@
 //   1. sort (one cluster): radix sort of ceil(log2(vocab + 1)) bits, up to 9 a pass.  A warp owns consecutive tokens; within 32 of them
 //      equal digits are ranked by match; counts of digits go from warp to block to cluster through shared memory.  The other blocks of
 //      the launch write the table's zeros meanwhile (not with accumulate): 0.54 GB for 151936 x 896, which hides the sort.
-//   2. sums: a tile of 32 sorted tokens by as many threads as the columns take; a run that ends inside its tile is written out, one
+//   2. sums: a tile of 8 to 32 sorted tokens by as many threads as the columns take; a run that ends inside its tile is written out, one
 //      that goes on leaves its part.  3. The tile where such a run begins adds up the parts, in order.
 // HBM-bound by the table's gradient (float32, written whole) where it is not accumulated.
 #include <cooperative_groups.h>
@@ -21,7 +21,7 @@ namespace mcb {
 namespace embed {
 namespace {
 
-constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32, kDigits = 512, kTile = 32, kThreads = 128;
+constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32, kDigits = 512, kMaxTile = 32, kThreads = 128;
 constexpr uint32_t kFull = 0xffffffffu;
 
 // ---- forward -----------------------------------------------------------------------------------------------------------
@@ -172,7 +172,7 @@ struct SumParams {
                     // does both is in the first)
   int64_t H;
   int64_t vocab;
-  int M, tiles, tx, accumulate;
+  int M, tile, tiles, tx, accumulate;   // tile: sorted tokens of one, 8 to kMaxTile
   float scale;
 };
 
@@ -208,14 +208,14 @@ __device__ __forceinline__ void finish(const SumParams& p, uint32_t id, int64_t 
 
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads) sum_kernel(const __grid_constant__ SumParams p) {
-  __shared__ uint32_t s_key[kThreads][kTile + 2], s_pos[kThreads][kTile];   // by tile of the block (at most kThreads of them)
+  __shared__ uint32_t s_key[kThreads][kMaxTile + 2], s_pos[kThreads][kMaxTile];   // by tile of the block (at most kThreads of them)
   const int x = threadIdx.x % p.tx, y = threadIdx.x / p.tx, ty = kThreads / p.tx;
   const int t = blockIdx.x * ty + y;
   grid_launch_dependents();
   grid_dependency_wait();
   const uint32_t *keys = from_here(p.key), *places = from_here(p.pos);
-  const int64_t i0 = static_cast<int64_t>(t) * kTile;
-  const int n = t < p.tiles ? static_cast<int>(i0 + kTile < p.M ? kTile : p.M - i0) : 0;
+  const int64_t i0 = static_cast<int64_t>(t) * p.tile;
+  const int n = t < p.tiles ? static_cast<int>(i0 + p.tile < p.M ? p.tile : p.M - i0) : 0;
   const uint32_t none = static_cast<uint32_t>(p.vocab);
   // keys of the tile with one on either side
   for (int i = x; i < n + 2 && n > 0; i += p.tx) {
@@ -280,15 +280,19 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
   grid_dependency_wait();
   if (t >= p.tiles) return;
   const uint32_t* keys = from_here(p.key);
-  const int64_t i0 = static_cast<int64_t>(t) * kTile, i1 = i0 + kTile;
+  const int64_t i0 = static_cast<int64_t>(t) * p.tile, i1 = i0 + p.tile;
   if (i1 >= p.M) return;
   const uint32_t id = __ldcg(keys + i1 - 1);
   if (id >= static_cast<uint32_t>(p.vocab) || __ldcg(keys + i1) != id) return;
   if (i0 > 0 && __ldcg(keys + i0 - 1) == id) return;   // it began in a tile before
   const int64_t c = N * (static_cast<int64_t>(blockIdx.y) * p.tx + x);
   if (c >= p.H) return;
-  // last token of the run
+  // last token of the run: steps that double, then halving
   int64_t lo = i1, hi = p.M - 1;
+  for (int64_t far = p.tile; lo + far <= hi; far *= 2) {
+    if (__ldcg(keys + lo + far) != id) { hi = lo + far - 1; break; }
+    lo += far;
+  }
   while (lo < hi) {
     const int64_t mid = (lo + hi + 1) >> 1;
     if (__ldcg(keys + mid) == id) lo = mid;
@@ -297,12 +301,15 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
   float acc[N] = {};
   get_add<N>(p.part + (2 * static_cast<int64_t>(t) + 1) * p.H + c, acc);
 #pragma unroll 4
-  for (int64_t q = t + 1; q <= lo / kTile; ++q) get_add<N>(p.part + 2 * q * p.H + c, acc);
+  for (int64_t q = t + 1; q <= lo / p.tile; ++q) get_add<N>(p.part + 2 * q * p.H + c, acc);
   finish<N>(p, id, c, acc);
 }
 
 inline size_t up256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
-inline int64_t tiles_of(int64_t M) { return (M + kTile - 1) / kTile; }
+// Sorted tokens of a tile: short tiles keep all SMs busy with few tokens (8192 tokens of 896, us: 8 SHORT, 32 LONG), long ones leave
+// fewer parts to join.
+inline int tile_of(int64_t M) { return M <= 16384 ? 8 : M <= 65536 ? 16 : kMaxTile; }
+inline int64_t tiles_of(int64_t M) { return (M + tile_of(M) - 1) / tile_of(M); }
 // threads that share a row of `n` pieces: a power of two up to kThreads
 inline int row_threads(int64_t n) {
   int t = 1;
@@ -428,7 +435,7 @@ extern "C" int mcb_embedding_bwd(const void* ids, int id_bytes, const void* dout
   embed::SumParams p = {};
   p.key = s.key[(s.passes - 1) & 1]; p.pos = s.pos[(s.passes - 1) & 1];
   p.dout = dout; p.grad = dtable; p.part = reinterpret_cast<float*>(w + 4 * list);
-  p.H = H; p.vocab = vocab; p.M = static_cast<int>(M); p.tiles = static_cast<int>(embed::tiles_of(M)); p.accumulate = accumulate; p.scale = scale;
+  p.H = H; p.vocab = vocab; p.M = static_cast<int>(M); p.tile = embed::tile_of(M); p.tiles = static_cast<int>(embed::tiles_of(M)); p.accumulate = accumulate; p.scale = scale;
   const int n = dtype == MCB_F32 ? 4 : 8;
   const bool vec = H % n == 0 && aligned16(dout);
   if (dtype == MCB_F32) return vec ? embed::launch_sums<float, 4>(p, st) : embed::launch_sums<float, 1>(p, st);

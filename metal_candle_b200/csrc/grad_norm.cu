@@ -79,10 +79,10 @@ __device__ __forceinline__ double squares(const float (&v)[16]) {
   return d;
 }
 
+// vec: 16 bytes at a time.  Otherwise neighbouring threads take neighbouring elements, so that a warp's access is whole lines again.
 template <typename F>
-__device__ __forceinline__ void with_piece(const Tensor& t, uint32_t piece, F&& f) {
+__device__ __forceinline__ void with_piece(const Tensor& t, uint32_t piece, bool vec, F&& f) {
   const int64_t at = static_cast<int64_t>(piece - t.first) * kPiece;
-  const bool vec = (reinterpret_cast<uintptr_t>(t.g) & 15u) == 0;
   if (t.dtype == MCB_F32) {
     const float* g = static_cast<const float*>(t.g);
     if (vec) for_piece<float, 4>(g, t.n, at, f);
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant
   double sum = 0.0;
   for (uint32_t piece = blockIdx.x; piece < tab.pieces; piece += gridDim.x) {
     const Tensor& t = tensor_of(tab, piece);
-    with_piece(t, piece, [&](const float (&v)[16]) { sum += squares(v); });
+    with_piece(t, piece, (reinterpret_cast<uintptr_t>(t.g) & 15u) == 0, [&](const float (&v)[16]) { sum += squares(v); });
   }
   sum = block_sum(sum, s);
   if (threadIdx.x == 0) part[blockIdx.x] = sum;
@@ -123,7 +123,7 @@ __device__ __forceinline__ void store_piece(T* out, int64_t n, int64_t at, const
     float w[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) w[e] = v[N * k + e] * f;
-    if (N > 1 && i + N <= n && (reinterpret_cast<uintptr_t>(out) & 15u) == 0) {
+    if (N > 1 && i + N <= n) {
       if constexpr (N > 1) {
         Vec16<T> x;
         x.from_float(w);
@@ -142,11 +142,13 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ 
   grid_dependency_wait();
   const float total = norm_of(part, parts, s), f = clip_factor(total, max_norm);
   if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = total;
-  for (uint32_t piece = blockIdx.x; piece < tab.pieces; piece += gridDim.x) {
+  // from the last piece back: what the sums read last is still in L2
+  for (uint32_t i = blockIdx.x; i < tab.pieces; i += gridDim.x) {
+    const uint32_t piece = tab.pieces - 1 - i;
     const Tensor& t = tensor_of(tab, piece);
     const int64_t at = static_cast<int64_t>(piece - t.first) * kPiece;
-    const bool vec = (reinterpret_cast<uintptr_t>(t.g) & 15u) == 0;
-    with_piece(t, piece, [&](const float (&v)[16]) {
+    const bool vec = ((reinterpret_cast<uintptr_t>(t.g) | reinterpret_cast<uintptr_t>(t.out)) & 15u) == 0;
+    with_piece(t, piece, vec, [&](const float (&v)[16]) {
       if (t.dtype == MCB_F32) {
         if (vec) store_piece<float, 4>(static_cast<float*>(t.out), t.n, at, v, f);
         else store_piece<float, 1>(static_cast<float*>(t.out), t.n, at, v, f);
