@@ -4,10 +4,13 @@
 // The variance is taken from the differences to the mean, which are in registers by then: E[x^2] - mean^2 would lose a row whose
 // mean is large against its spread.  The backward pass takes both from x again instead of reading them: x is read anyway.
 //
-// HBM-bound: the forward reads x and writes y, the backward reads x and dy (and the residual) and writes dx.  A row is read once,
-// into registers, by TPR threads (32 to 512, so that a thread has at most four 16-byte vectors of it, or eight elements of a row that
-// is not made of whole, aligned vectors); longer rows are read again from L2 instead.  Blocks walk over rows; a thread's columns stay its own, so that its parts of
-// dw and db are registers until the block writes them out, a line of partial sums each that a last kernel adds up in order: no atomics.
+// HBM-bound: the forward reads x and writes y, the backward reads x and dy (and the residual) and writes dx.  A row is read once, by TPR
+// threads (8 to 512, so that a thread has at most two 16-byte vectors of it, four where the row needs more than 512 x 2), with the
+// next rows on their way in shared memory.  Blocks walk over rows; a thread's columns stay its own, so that its parts of dw and db
+// are registers until the block writes them out, a line of partial sums each that a last kernel adds up in order: no atomics.
+// Rows that are not whole vectors (D = 777) start at every alignment.  Row r starts (r D) mod N elements behind a vector boundary, which comes
+// back every P = N / gcd(D, N) rows: a block takes rows of one residue mod P, and everything is the aligned case moved by a constant, with
+// a ragged first and last vector.  Longer rows, and operands of different alignments, take a kernel that reads element by element.
 #include <type_traits>
 
 #include "common.cuh"
@@ -22,15 +25,21 @@ struct Params {
   float *mean, *rstd;       // forward, or null
   float *part;              // backward: [blocks][2][D], or null
   int64_t rows;
-  int D;
+  int D, period;            // rows until one starts at the same alignment again
   float eps;
 };
 
 // Sums over the TPR threads of a row, the same bits on all of them.  `buf` has a place for each warp of the block; a call with another
 // buffer lies between two with the same one, whose barrier keeps them apart.
 template <int TPR>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* buf) {
-  v = warp_sum(v);
+  v = lanes_sum<TPR>(v);
   if constexpr (TPR > 32) {
     const int warp = threadIdx.x >> 5;
     constexpr int W = TPR / 32;
@@ -45,9 +54,9 @@ __device__ __forceinline__ float row_sum(float v, float* buf) {
 }
 template <int TPR>
 __device__ __forceinline__ float3 row_sum3(float3 v, float3* buf) {
-  v.x = warp_sum(v.x);
-  v.y = warp_sum(v.y);
-  v.z = warp_sum(v.z);
+  v.x = lanes_sum<TPR>(v.x);
+  v.y = lanes_sum<TPR>(v.y);
+  v.z = lanes_sum<TPR>(v.z);
   if constexpr (TPR > 32) {
     const int warp = threadIdx.x >> 5;
     constexpr int W = TPR / 32;
@@ -61,29 +70,14 @@ __device__ __forceinline__ float3 row_sum3(float3 v, float3* buf) {
   return v;
 }
 
-// N elements of a row as they lie in memory: one 16-byte vector, or (N == 1) the element itself
-template <typename T, int N>
-struct Piece {
-  using Raw = std::conditional_t<N == 1, T, decltype(Vec16<T>::raw)>;
-  Raw raw;
-  __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const Raw*>(p); }
-  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Raw*>(p) = raw; }
-  __device__ __forceinline__ void zero() { raw = Raw(); }
-  __device__ __forceinline__ void to_float(float (&f)[N]) const {
-    if constexpr (N == 1) f[0] = to_f32(raw);
-    else { Vec16<T> v; v.raw = raw; v.to_float(f); }
-  }
-  __device__ __forceinline__ void from_float(const float (&f)[N]) {
-    if constexpr (N == 1) raw = from_f32<T>(f[0]);
-    else { Vec16<T> v; v.from_float(f); raw = v.raw; }
-  }
-};
+// Arithmetic on pairs: one instruction for two elements.
+__device__ __forceinline__ float2 two(const float* v) { return make_float2(v[0], v[1]); }
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ void put2(float* v, float2 x) { v[0] = x.x; v[1] = x.y; }
 
 // ---- rows on their way -------------------------------------------------------------------------------------------------
-// A block has `STAGES - 1` rounds of rows on their way from memory while it works on one (cp.async): the bytes in flight are what the
-// bandwidth is made of, and shared memory has room for them where registers have not.  A thread has the elements [N * (lane + TPR * k), + N) of a row.
-// N > 1 (rows of whole, aligned 16-byte vectors): every thread fetches its own vectors and waits for nobody.  N == 1: rows that start
-// anywhere are fetched as the 16-byte granules that cover them, and the row's threads meet once a round.
+// A block has `STAGES - 1` rounds of rows on their way from memory while it works on one (cp.async, every thread its own vectors):
+// the bytes in flight are what the bandwidth is made of, and shared memory has room for them where registers have not.
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes) {
   const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(bytes) : "memory");
@@ -95,130 +89,158 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 constexpr int block_of(int tpr) { return tpr < 128 ? 128 : tpr; }
 constexpr int stages_of(int tpr, int k) { return k * block_of(tpr) > 1024 ? 2 : 3; }   // (three would not fit for three operands)
 
-template <typename T, int TPR, int K, int N>
-struct Feed {
-  static constexpr int kBlock = block_of(TPR), kRows = kBlock / TPR, STAGES = stages_of(TPR, K);
-  uint8_t* ring;
-  int lane, slot, D, nt, row_bytes;
-  int64_t rows;
-  __host__ __device__ static int bytes_of_row(int D) { return ((D * static_cast<int>(sizeof(T)) + 15) & ~15) + 16; }
-  __host__ static size_t smem(int D, int nt) {
-    return static_cast<size_t>(STAGES) * nt * (N > 1 ? K * kBlock * 16 : kRows * bytes_of_row(D));
+// The rows of a block and a thread's part of them: vectors lane + TPR * k of a row, k < K.  Row r of the block's turn j is j * P + q.  SHIFT: a row
+// begins `off` elements into its first vector.
+template <typename T, int TPR, int K, bool SHIFT>
+struct Rows {
+  static constexpr int N = Vec16<T>::N, kBlock = block_of(TPR), kRows = kBlock / TPR, STAGES = stages_of(TPR, K);
+  uint4* ring;
+  int lane, nt, off, D, P, q;
+  int64_t j, step, rows;
+  static size_t smem(int nt) { return static_cast<size_t>(STAGES) * nt * K * kBlock * 16; }
+  __device__ __forceinline__ Rows(void* base, const Params& p, int nt_) : ring(static_cast<uint4*>(base)), nt(nt_), D(p.D), P(SHIFT ? p.period : 1), rows(p.rows) {
+    lane = threadIdx.x % TPR;
+    q = SHIFT ? blockIdx.x % P : 0;
+    j = static_cast<int64_t>(blockIdx.x / P) * kRows + threadIdx.x / TPR;
+    step = static_cast<int64_t>(gridDim.x / P) * kRows;
+    off = SHIFT ? static_cast<int>(((reinterpret_cast<uintptr_t>(p.x) & 15) / sizeof(T) + static_cast<int64_t>(q) * D) % N) : 0;
   }
-  __device__ __forceinline__ Feed(void* smem_base, int lane_, int slot_, const Params& p, int nt_)
-      : ring(static_cast<uint8_t*>(smem_base)), lane(lane_), slot(slot_), D(p.D), nt(nt_), row_bytes(bytes_of_row(p.D)), rows(p.rows) {}
-  __device__ __forceinline__ uint8_t* at(int stage, int t) const {
-    if constexpr (N > 1) return ring + (static_cast<size_t>(stage * nt + t) * K * kBlock + threadIdx.x) * 16;
-    else return ring + (static_cast<size_t>(stage * nt + t) * kRows + slot) * row_bytes;
-  }
-  __device__ __forceinline__ void fetch(int stage, int t, const T* x, int64_t row) const {
-    if (row >= rows) return;
-    if constexpr (N > 1) {
+  __device__ __forceinline__ int64_t row(int64_t turn) const { return turn * P + q; }
+  __device__ __forceinline__ bool any(int64_t turn) const { return (turn - threadIdx.x / TPR) * P + q < rows; }   // some row of the block's
+  __device__ __forceinline__ int col(int k) const { return N * (lane + TPR * k) - off; }   // of element 0 of a vector; may be below 0
+  __device__ __forceinline__ bool here(int k) const { return col(k) < D; }
+  __device__ __forceinline__ bool whole(int k) const { return !SHIFT || (col(k) >= 0 && col(k) + N <= D); }
+  __device__ __forceinline__ bool in(int k, int e) const { return static_cast<unsigned>(col(k) + e) < static_cast<unsigned>(D); }
+  __device__ __forceinline__ void fetch(int stage, int t, const T* x, int64_t turn) const {
+    const int64_t r = row(turn);
+    if (r >= rows) return;
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int c = N * (lane + TPR * k);
-        if (c < D) cp_async16(at(stage, t) + k * kBlock * 16, x + row * D + c, 16);
+    for (int k = 0; k < K; ++k)
+      if (here(k)) {
+        const T* from = x + r * D + col(k);
+        int bytes = 16;
+        if constexpr (SHIFT) {   // nothing behind the tensor is read (before it, at most the rest of its first 16 bytes)
+          const int64_t left = (rows * D - (r * D + col(k))) * static_cast<int64_t>(sizeof(T));
+          if (left < 16) bytes = static_cast<int>(left);
+        }
+        cp_async16(ring + (static_cast<size_t>(stage * nt + t) * K + k) * kBlock + threadIdx.x, from, bytes);
       }
-    } else {
-      const uintptr_t from = reinterpret_cast<uintptr_t>(x + row * D), first = from & ~static_cast<uintptr_t>(15);
-      const uintptr_t end = reinterpret_cast<uintptr_t>(x + rows * D), row_end = from + static_cast<uintptr_t>(D) * sizeof(T);
-      for (uintptr_t g = first + 16 * lane; g < row_end; g += 16 * TPR)   // nothing behind the tensor is read
-        cp_async16(at(stage, t) + (g - first), reinterpret_cast<const void*>(g), end - g < 16 ? static_cast<int>(end - g) : 16);
-    }
   }
-  __device__ __forceinline__ void get(int stage, int t, const T* x, int64_t row, float (&v)[K][N]) const {
+  // the vectors of a row as float32; elements outside the row are 0
+  __device__ __forceinline__ void get(int stage, int t, int64_t turn, float (&v)[K][N]) const {
+    const bool have = row(turn) < rows;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = N * (lane + TPR * k);
 #pragma unroll
       for (int e = 0; e < N; ++e) v[k][e] = 0.0f;
-      if (row < rows && c < D) {
-        Piece<T, N> piece;
-        if constexpr (N > 1) piece.load(reinterpret_cast<const T*>(at(stage, t) + k * kBlock * 16));
-        else piece.load(reinterpret_cast<const T*>(at(stage, t) + (reinterpret_cast<uintptr_t>(x + row * D) & 15)) + c);
-        piece.to_float(v[k]);
+      if (!have || !here(k)) continue;
+      load(v[k], reinterpret_cast<const T*>(ring + (static_cast<size_t>(stage * nt + t) * K + k) * kBlock + threadIdx.x));
+      drop(v[k], k);
+    }
+  }
+  static __device__ __forceinline__ void load(float (&f)[N], const T* p) {
+    Vec16<T> v;
+    v.raw = *reinterpret_cast<const decltype(v.raw)*>(p);
+    v.to_float(f);
+  }
+  __device__ __forceinline__ void drop(float (&v)[N], int k) const {
+    if constexpr (SHIFT) {
+      if (!whole(k)) {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (!in(k, e)) v[e] = 0.0f;
       }
     }
   }
-  // The round's rows are here (and, N == 1, nobody reads the stage that is filled next).
-  __device__ __forceinline__ void arrived() const {
-    cp_async_wait<STAGES - 2>();
-    if constexpr (N == 1) {
-      if constexpr (TPR > 32) __syncthreads();
-      else __syncwarp();
+  // a vector of a weight [D], `none` where there is no weight
+  __device__ __forceinline__ void weight(float (&f)[N], const T* w, int k, float none) const {
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = none;
+    if (w == nullptr) return;
+    if constexpr (SHIFT) {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (in(k, e)) f[e] = to_f32(w[col(k) + e]);
+    } else {
+      load(f, w + col(k));
+    }
+  }
+  __device__ __forceinline__ void store(T* out, int64_t turn, int k, const float (&f)[N]) const {
+    T* to = out + row(turn) * D + col(k);
+    Vec16<T> v;
+    if (whole(k)) {
+      v.from_float(f);
+      *reinterpret_cast<decltype(v.raw)*>(to) = v.raw;
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (in(k, e)) to[e] = from_f32<T>(f[e]);
     }
   }
 };
 
-template <typename T, int TPR, int K, int N>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) ln_fwd_kernel(const Params p) {
+template <typename T, int TPR, int K, bool SHIFT>
+__global__ void __launch_bounds__(block_of(TPR)) ln_fwd_kernel(const Params p) {
   extern __shared__ uint4 smem4[];
-  using F = Feed<T, TPR, K, N>;
-  __shared__ float buf[2][F::kBlock / 32];
-  const int lane = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+  using R = Rows<T, TPR, K, SHIFT>;
+  constexpr int N = R::N;
+  __shared__ float buf[2][R::kBlock / 32];
   const T *x = static_cast<const T*>(p.x), *w = static_cast<const T*>(p.w), *b = static_cast<const T*>(p.b);
   T* y = static_cast<T*>(p.out);
   const float inv = 1.0f / static_cast<float>(p.D);
-  const int64_t step = static_cast<int64_t>(gridDim.x) * F::kRows;
-  int64_t r0 = static_cast<int64_t>(blockIdx.x) * F::kRows;
-  const F feed(smem4, lane, slot, p, 1);
+  R rows(smem4, p, 1);
   grid_launch_dependents();
   grid_dependency_wait();
+  // a moved weight is read element by element: once, into registers
+  float fw[SHIFT ? K : 1][N], fb[SHIFT ? K : 1][N];
+  if constexpr (SHIFT) {
 #pragma unroll
-  for (int i = 0; i < F::STAGES - 1; ++i) {
-    feed.fetch(i, 0, x, r0 + slot + i * step);
+    for (int k = 0; k < K; ++k) { rows.weight(fw[k], w, k, 1.0f); rows.weight(fb[k], b, k, 0.0f); }
+  }
+#pragma unroll
+  for (int i = 0; i < R::STAGES - 1; ++i) {
+    rows.fetch(i, 0, x, rows.j + i * rows.step);
     cp_async_commit();
   }
-  for (int stage = 0; r0 < p.rows; r0 += step) {
-    const int64_t row = r0 + slot;
+  int stage = 0;
+  for (int64_t j = rows.j; rows.any(j); j += rows.step) {
     float v[K][N];
-    float sum = 0.0f;
-    feed.arrived();
-    feed.fetch(stage == 0 ? F::STAGES - 1 : stage - 1, 0, x, row + (F::STAGES - 1) * step);
+    cp_async_wait<R::STAGES - 2>();
+    rows.get(stage, 0, j, v);
+    rows.fetch(stage == 0 ? R::STAGES - 1 : stage - 1, 0, x, j + (R::STAGES - 1) * rows.step);
     cp_async_commit();
-    feed.get(stage, 0, x, row, v);
-    if (++stage == F::STAGES) stage = 0;
+    if (++stage == R::STAGES) stage = 0;
+    float2 sum = both(0.0f), sq = sum;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int e = 0; e < N; ++e) sum += v[k][e];
-    const float mean = row_sum<TPR>(sum, buf[0]) * inv;
-    float sq = 0.0f;
+      for (int e = 0; e < N; e += 2) sum = __fadd2_rn(two(&v[k][e]), sum);
+    const float mean = row_sum<TPR>(sum.x + sum.y, buf[0]) * inv;
 #pragma unroll
     for (int k = 0; k < K; ++k)
-      if (N * (lane + TPR * k) < p.D) {
+      if (rows.here(k)) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          v[k][e] -= mean;
-          sq = fmaf(v[k][e], v[k][e], sq);
-        }
+        for (int e = 0; e < N; e += 2) put2(&v[k][e], __fadd2_rn(two(&v[k][e]), both(-mean)));
+        rows.drop(v[k], k);
+#pragma unroll
+        for (int e = 0; e < N; e += 2) sq = __ffma2_rn(two(&v[k][e]), two(&v[k][e]), sq);
       }
-    const float rstd = rsqrtf(row_sum<TPR>(sq, buf[1]) * inv + p.eps);
-    if (row >= p.rows) continue;
+    const float rstd = rsqrtf(row_sum<TPR>(sq.x + sq.y, buf[1]) * inv + p.eps);
+    const int64_t row = rows.row(j);
+    if (row >= p.rows) continue;   // (no barrier follows within the round)
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = N * (lane + TPR * k);
-      if (c >= p.D) continue;
-      Piece<T, N> t;
-      float f[N];
+      if (!rows.here(k)) continue;
+      float f[N], g[N];
+      if constexpr (!SHIFT) { rows.weight(f, w, k, 1.0f); rows.weight(g, b, k, 0.0f); }
 #pragma unroll
-      for (int e = 0; e < N; ++e) v[k][e] *= rstd;
-      if (w != nullptr) {
-        t.load(w + c);
-        t.to_float(f);
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[k][e] *= f[e];
+      for (int e = 0; e < N; e += 2) {
+        const float2 n = __fmul2_rn(two(&v[k][e]), both(rstd));
+        put2(&v[k][e], __ffma2_rn(n, two(SHIFT ? &fw[k][e] : &f[e]), two(SHIFT ? &fb[k][e] : &g[e])));
       }
-      if (b != nullptr) {
-        t.load(b + c);
-        t.to_float(f);
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[k][e] += f[e];
-      }
-      t.from_float(v[k]);
-      t.store(y + row * p.D + c);
+      rows.store(y, j, k, v[k]);
     }
-    if (lane == 0) {
+    if (rows.lane == 0) {
       if (p.mean != nullptr) p.mean[row] = mean;
       if (p.rstd != nullptr) p.rstd[row] = rstd;
     }
@@ -227,132 +249,118 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) ln_fwd_kernel(const Par
 
 // After the mean one more round of sums does: of (x - mean)^2, of g and of g (x - mean), from which rstd and both means of the backward
 // formula follow.  SUMS: dw and db are asked for.
-template <typename T, int TPR, int K, int N, bool SUMS>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) ln_bwd_kernel(const Params p) {
+template <typename T, int TPR, int K, bool SHIFT, bool SUMS>
+__global__ void __launch_bounds__(block_of(TPR)) ln_bwd_kernel(const Params p) {
   extern __shared__ uint4 smem4[];
-  using F = Feed<T, TPR, K, N>;
-  __shared__ float buf[F::kBlock / 32];
-  __shared__ float3 buf3[F::kBlock / 32];
-  const int lane = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+  using R = Rows<T, TPR, K, SHIFT>;
+  constexpr int N = R::N;
+  __shared__ float buf[R::kBlock / 32];
+  __shared__ float3 buf3[R::kBlock / 32];
   const T *x = static_cast<const T*>(p.x), *w = static_cast<const T*>(p.w), *dy = static_cast<const T*>(p.dy), *res = static_cast<const T*>(p.res);
   T* dx = static_cast<T*>(p.out);
   const float inv = 1.0f / static_cast<float>(p.D);
-  const int64_t step = static_cast<int64_t>(gridDim.x) * F::kRows;
-  int64_t r0 = static_cast<int64_t>(blockIdx.x) * F::kRows;
-  const F feed(smem4, lane, slot, p, res != nullptr ? 3 : 2);
-  auto fetch = [&](int stage, int64_t row) {
-    feed.fetch(stage, 0, x, row);
-    feed.fetch(stage, 1, dy, row);
-    if (res != nullptr) feed.fetch(stage, 2, res, row);
+  R rows(smem4, p, res != nullptr ? 3 : 2);
+  auto fetch = [&](int stage, int64_t turn) {
+    rows.fetch(stage, 0, x, turn);
+    rows.fetch(stage, 1, dy, turn);
+    if (res != nullptr) rows.fetch(stage, 2, res, turn);
     cp_async_commit();
   };
   grid_launch_dependents();
   grid_dependency_wait();
+  float fw[SHIFT ? K : 1][N];
+  if constexpr (SHIFT) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) rows.weight(fw[k], w, k, 1.0f);
+  }
   float gw[SUMS ? K : 1][N], gb[SUMS ? K : 1][N];
 #pragma unroll
   for (int k = 0; k < (SUMS ? K : 1); ++k)
 #pragma unroll
     for (int e = 0; e < N; ++e) gw[k][e] = gb[k][e] = 0.0f;
 #pragma unroll
-  for (int i = 0; i < F::STAGES - 1; ++i) fetch(i, r0 + slot + i * step);
+  for (int i = 0; i < R::STAGES - 1; ++i) fetch(i, rows.j + i * rows.step);
   int stage = 0;
-  for (; r0 < p.rows; r0 += step) {
-    const int64_t row = r0 + slot;
-    float v[K][N], d[K][N];
-    float sum = 0.0f;
-    feed.arrived();
-    const int here = stage;
-    fetch(stage == 0 ? F::STAGES - 1 : stage - 1, row + (F::STAGES - 1) * step);
-    if (++stage == F::STAGES) stage = 0;
-    feed.get(here, 0, x, row, v);
-    feed.get(here, 1, dy, row, d);
+  for (int64_t j = rows.j; rows.any(j); j += rows.step) {
+    float v[K][N], d[K][N], r[K][N];
+    cp_async_wait<R::STAGES - 2>();
+    rows.get(stage, 0, j, v);
+    rows.get(stage, 1, j, d);
+    const int now = stage;
+    fetch(stage == 0 ? R::STAGES - 1 : stage - 1, j + (R::STAGES - 1) * rows.step);
+    if (++stage == R::STAGES) stage = 0;
+    float2 sum = both(0.0f);
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int e = 0; e < N; ++e) sum += v[k][e];
-    const float mean = row_sum<TPR>(sum, buf) * inv;
-    float3 s = make_float3(0.0f, 0.0f, 0.0f);
+      for (int e = 0; e < N; e += 2) sum = __fadd2_rn(two(&v[k][e]), sum);
+    const float mean = row_sum<TPR>(sum.x + sum.y, buf) * inv;
+    float2 sx = both(0.0f), sy = sx, sz = sx;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = N * (lane + TPR * k);
-      if (c >= p.D) continue;
+      if (!rows.here(k)) continue;
       float f[N];
+      if constexpr (!SHIFT) rows.weight(f, w, k, 1.0f);
 #pragma unroll
-      for (int e = 0; e < N; ++e) f[e] = 1.0f;
-      if (w != nullptr) {
-        Piece<T, N> t;
-        t.load(w + c);
-        t.to_float(f);
-      }
+      for (int e = 0; e < N; e += 2) put2(&v[k][e], __fadd2_rn(two(&v[k][e]), both(-mean)));
+      rows.drop(v[k], k);
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        v[k][e] -= mean;
-        const float g = d[k][e] * f[e];
-        s.x = fmaf(v[k][e], v[k][e], s.x);
-        s.y += g;
-        s.z = fmaf(g, v[k][e], s.z);
+      for (int e = 0; e < N; e += 2) {
+        const float2 o = two(&v[k][e]), g = __fmul2_rn(two(&d[k][e]), two(SHIFT ? &fw[k][e] : &f[e]));
+        sx = __ffma2_rn(o, o, sx);
+        sy = __fadd2_rn(g, sy);
+        sz = __ffma2_rn(g, o, sz);
       }
     }
-    s = row_sum3<TPR>(s, buf3);
+    const float3 s = row_sum3<TPR>(make_float3(sx.x + sx.y, sy.x + sy.y, sz.x + sz.y), buf3);
     const float rstd = rsqrtf(s.x * inv + p.eps);
     const float a = s.y * inv, q = s.z * inv * rstd;
-    if (row >= p.rows) continue;
-    float r[K][N];
-    if (res != nullptr) feed.get(here, 2, res, row, r);
+    if (rows.row(j) >= p.rows) continue;
+    if (res != nullptr) rows.get(now, 2, j, r);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = N * (lane + TPR * k);
-      if (c >= p.D) continue;
-      Piece<T, N> t;
+      if (!rows.here(k)) continue;
       float f[N];
+      if constexpr (!SHIFT) rows.weight(f, w, k, 1.0f);   // (from L1 again: registers for it would cost occupancy)
 #pragma unroll
-      for (int e = 0; e < N; ++e) f[e] = 1.0f;
-      if (w != nullptr) {   // (from L1: registers for it would cost occupancy)
-        t.load(w + c);
-        t.to_float(f);
-      }
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float n = v[k][e] * rstd;
+      for (int e = 0; e < N; e += 2) {
+        const float2 n = __fmul2_rn(two(&v[k][e]), both(rstd)), g = two(&d[k][e]);
         if constexpr (SUMS) {
-          gw[k][e] = fmaf(d[k][e], n, gw[k][e]);
-          gb[k][e] += d[k][e];
+          put2(&gw[k][e], __ffma2_rn(g, n, two(&gw[k][e])));
+          put2(&gb[k][e], __fadd2_rn(g, two(&gb[k][e])));
         }
-        f[e] = fmaf(fmaf(-n, q, fmaf(d[k][e], f[e], -a)), rstd, res != nullptr ? r[k][e] : 0.0f);
+        const float2 t = __ffma2_rn(n, both(-q), __ffma2_rn(g, two(SHIFT ? &fw[k][e] : &f[e]), both(-a)));
+        put2(&f[e], __ffma2_rn(t, both(rstd), res != nullptr ? two(&r[k][e]) : both(0.0f)));
       }
-      t.from_float(f);
-      t.store(dx + row * p.D + c);
+      rows.store(dx, j, k, f);
     }
   }
   if constexpr (SUMS) {
     float* out = p.part + static_cast<int64_t>(blockIdx.x) * 2 * p.D;
-    if constexpr (F::kRows > 1) {
+    if constexpr (R::kRows > 1) {
       cp_async_wait<0>();
       float* sums = reinterpret_cast<float*>(smem4);   // [2][D] of the block's row slots, over the ring
-      for (int s = 0; s < F::kRows; ++s) {
+      for (int s = 0; s < R::kRows; ++s) {
         __syncthreads();
-        if (slot != s) continue;
+        if (static_cast<int>(threadIdx.x / TPR) != s) continue;
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-          for (int e = 0; e < N; ++e) {
-            const int c = N * (lane + TPR * k) + e;
-            if (c < p.D) {
+          for (int e = 0; e < N; ++e)
+            if (rows.in(k, e)) {
+              const int c = rows.col(k) + e;
               sums[c] = (s ? sums[c] : 0.0f) + gw[k][e];
               sums[p.D + c] = (s ? sums[p.D + c] : 0.0f) + gb[k][e];
             }
-          }
       }
       __syncthreads();
-      for (int i = threadIdx.x; i < 2 * p.D; i += F::kBlock) out[i] = sums[i];
+      for (int i = threadIdx.x; i < 2 * p.D; i += R::kBlock) out[i] = sums[i];
     } else {
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const int c = N * (lane + TPR * k) + e;
-          if (c < p.D) { out[c] = gw[k][e]; out[p.D + c] = gb[k][e]; }
-        }
+        for (int e = 0; e < N; ++e)
+          if (rows.in(k, e)) { out[rows.col(k) + e] = gw[k][e]; out[p.D + rows.col(k) + e] = gb[k][e]; }
     }
   }
 }
@@ -444,56 +452,55 @@ int blocks_for(int64_t rows, int per_block, int sms, int per_sm) {
   return static_cast<int>(want < most ? want : most);
 }
 
-// As many blocks as are on the device at once: the rows' sums are kept by block.
-template <typename K>
-int resident(K kernel, int threads, size_t smem, int64_t want, int sms, int* blocks) {
-  int per_sm = 0;
-  MCB_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
-  *blocks = blocks_for(want, 1, sms, per_sm < 1 ? 1 : per_sm);
-  return MCB_OK;
-}
-template <typename T, int N, bool BWD, int TPR, int K>
+template <typename T, bool BWD, bool SHIFT, int TPR, int K>
 int launch_k(const Params& p, int sms, cudaStream_t st, int* blocks) {
-  using F = Feed<T, TPR, K, N>;
-  size_t smem = F::smem(p.D, !BWD ? 1 : p.res != nullptr ? 3 : 2);
-  if (BWD && F::kRows > 1 && smem < 2 * static_cast<size_t>(p.D) * 4) smem = 2 * static_cast<size_t>(p.D) * 4;
-  void (*kernel)(const Params) = ln_fwd_kernel<T, TPR, K, N>;
-  if constexpr (BWD) kernel = p.part != nullptr ? ln_bwd_kernel<T, TPR, K, N, true> : ln_bwd_kernel<T, TPR, K, N, false>;
+  using R = Rows<T, TPR, K, SHIFT>;
+  size_t smem = R::smem(!BWD ? 1 : p.res != nullptr ? 3 : 2);
+  if (BWD && R::kRows > 1 && smem < 2 * static_cast<size_t>(p.D) * 4) smem = 2 * static_cast<size_t>(p.D) * 4;
+  void (*kernel)(const Params) = ln_fwd_kernel<T, TPR, K, SHIFT>;
+  if constexpr (BWD) kernel = p.part != nullptr ? ln_bwd_kernel<T, TPR, K, SHIFT, true> : ln_bwd_kernel<T, TPR, K, SHIFT, false>;
   MCB_CHECK_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  if (int rc = resident(kernel, F::kBlock, smem, (p.rows + F::kRows - 1) / F::kRows, sms, blocks)) return rc;
-  MCB_CHECK_CUDA(launch_kernel(kernel, dim3(*blocks), dim3(F::kBlock), smem, st, chained_launch(), p));
+  // as many blocks as are on the device at once (each leaves a line of sums), a whole number of rounds of the alignments
+  int per_sm = 0;
+  MCB_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, R::kBlock, smem));
+  const int64_t turns = (p.rows + p.period - 1) / p.period;   // rows of an alignment
+  const int each = blocks_for(turns, R::kRows, sms, per_sm < 1 ? 1 : per_sm), most = blocks_for(p.rows, 1, sms, per_sm < 1 ? 1 : per_sm) / p.period;
+  *blocks = p.period * (each < most || most < 1 ? each : most);
+  MCB_CHECK_CUDA(launch_kernel(kernel, dim3(*blocks), dim3(R::kBlock), smem, st, chained_launch(), p));
   MCB_CHECK_LAUNCH("layer_norm");
   return MCB_OK;
 }
-template <typename T, int N, bool BWD, int TPR>
-int launch_tpr(const Params& p, int pieces, int sms, cudaStream_t st, int* blocks) {
-  const int k = (pieces + TPR - 1) / TPR;
-  if (k <= 1) return launch_k<T, N, BWD, TPR, 1>(p, sms, st, blocks);
-  if (k == 2) return launch_k<T, N, BWD, TPR, 2>(p, sms, st, blocks);
-  if constexpr (N > 1) {
-    if (k == 3) return launch_k<T, N, BWD, TPR, 3>(p, sms, st, blocks);
-    return launch_k<T, N, BWD, TPR, 4>(p, sms, st, blocks);
-  } else {
-    if (k <= 4) return launch_k<T, N, BWD, TPR, 4>(p, sms, st, blocks);
-    return launch_k<T, N, BWD, TPR, 8>(p, sms, st, blocks);
-  }
+// A row's threads: as few as have at most two vectors of it each (32768 x 896 bfloat16, backward with its reduction: 64 threads with two
+// 64.5 us, 32 with four 83, 128 with one 68.6: the sums of a thread's columns are registers, and rows in flight go with the threads).
+template <typename T, bool BWD, bool SHIFT>
+int launch_rows(const Params& p, int vecs, int sms, cudaStream_t st, int* blocks) {
+  if (vecs <= 8) return launch_k<T, BWD, SHIFT, 8, 1>(p, sms, st, blocks);
+  if (vecs <= 16) return launch_k<T, BWD, SHIFT, 8, 2>(p, sms, st, blocks);
+  if (vecs <= 32) return launch_k<T, BWD, SHIFT, 32, 1>(p, sms, st, blocks);
+  if (vecs <= 64) return launch_k<T, BWD, SHIFT, 32, 2>(p, sms, st, blocks);
+  if (vecs <= 128) return launch_k<T, BWD, SHIFT, 64, 2>(p, sms, st, blocks);
+  if (vecs <= 256) return launch_k<T, BWD, SHIFT, 128, 2>(p, sms, st, blocks);
+  if (vecs <= 512) return launch_k<T, BWD, SHIFT, 256, 2>(p, sms, st, blocks);
+  if (vecs <= 1024) return launch_k<T, BWD, SHIFT, 512, 2>(p, sms, st, blocks);
+  return launch_k<T, BWD, SHIFT, 512, 4>(p, sms, st, blocks);
 }
-// A row's threads: as few as have at most four 16-byte pieces (or eight elements) of it each.
-template <typename T, bool BWD, int N>
-int launch_n(const Params& p, int sms, cudaStream_t st, int* blocks) {
-  const int pieces = p.D / N;
-  constexpr int most = N > 1 ? 4 : 8;
-  if (pieces <= 32 * most) return launch_tpr<T, N, BWD, 32>(p, pieces, sms, st, blocks);
-  if (pieces <= 128 * most) return launch_tpr<T, N, BWD, 128>(p, pieces, sms, st, blocks);
-  if (pieces <= 512 * most) return launch_tpr<T, N, BWD, 512>(p, pieces, sms, st, blocks);
+template <typename T, bool BWD>
+int launch(Params& p, uintptr_t operands, uintptr_t weights, int sms, cudaStream_t st, int* blocks) {
+  constexpr int N = Vec16<T>::N;
+  // operands: the bits in which the row operands' addresses differ from one another, weights: all bits of the weights' addresses
+  const bool alike = (operands & 15) == 0;
+  const bool whole = p.D % N == 0 && (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && (weights & 15) == 0;
+  const int vecs = whole ? p.D / N : (p.D + 2 * N - 2) / N;
+  p.period = 1;
+  if (alike && vecs <= 2048) {
+    if (whole) return launch_rows<T, BWD, false>(p, vecs, sms, st, blocks);
+    for (p.period = 1; p.D * static_cast<int64_t>(p.period) % N != 0; p.period *= 2) {}
+    return launch_rows<T, BWD, true>(p, vecs, sms, st, blocks);
+  }
   *blocks = blocks_for(p.rows, 1, sms, 4);
   MCB_CHECK_CUDA(launch_kernel(ln_long_kernel<T, BWD>, dim3(*blocks), dim3(512), 0, st, chained_launch(), p));
   MCB_CHECK_LAUNCH("layer_norm");
   return MCB_OK;
-}
-template <typename T, bool BWD>
-int launch(const Params& p, bool vec, int sms, cudaStream_t st, int* blocks) {
-  return vec ? launch_n<T, BWD, Vec16<T>::N>(p, sms, st, blocks) : launch_n<T, BWD, 1>(p, sms, st, blocks);
 }
 
 int check(const char* who, int64_t rows, int64_t D, float eps, int dtype) {
@@ -519,17 +526,17 @@ extern "C" int mcb_layernorm_fwd(const void* x, const void* w, const void* b, vo
   lnorm::Params p = {};
   p.x = x; p.w = w; p.b = b; p.out = y; p.mean = mean; p.rstd = rstd;
   p.rows = rows; p.D = static_cast<int>(D); p.eps = eps;
-  const int size = dtype == MCB_F32 ? 4 : 2;
-  const bool vec = D * size % 16 == 0 && aligned16(x) && aligned16(y) && aligned16(w) && aligned16(b);
+  const auto at = [](const void* v) { return reinterpret_cast<uintptr_t>(v); };
+  const uintptr_t operands = at(x) ^ at(y), weights = at(w) | at(b);
   int blocks = 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == MCB_F32 ? lnorm::launch<float, false>(p, vec, ds->sm_count, st, &blocks)
-                          : lnorm::launch<__nv_bfloat16, false>(p, vec, ds->sm_count, st, &blocks);
+  return dtype == MCB_F32 ? lnorm::launch<float, false>(p, operands, weights, ds->sm_count, st, &blocks)
+                          : lnorm::launch<__nv_bfloat16, false>(p, operands, weights, ds->sm_count, st, &blocks);
 }
 
 extern "C" size_t mcb_layernorm_bwd_workspace_bytes(int64_t rows, int64_t D) {
   if (rows <= 0 || D <= 0) return 0;
-  const int64_t blocks = rows < lnorm::kMaxBlocks ? rows : lnorm::kMaxBlocks;
+  const int64_t blocks = rows < 8 ? 8 : rows < lnorm::kMaxBlocks ? rows : lnorm::kMaxBlocks;   // (one an alignment at least)
   return static_cast<size_t>(blocks) * 2 * D * 4;
 }
 
@@ -547,12 +554,12 @@ extern "C" int mcb_layernorm_bwd(const void* x, const void* w, const void* dy, c
   lnorm::Params p = {};
   p.x = x; p.w = w; p.dy = dy; p.res = dx_residual; p.out = dx; p.part = sums ? static_cast<float*>(workspace) : nullptr;
   p.rows = rows; p.D = static_cast<int>(D); p.eps = eps;
-  const int size = dtype == MCB_F32 ? 4 : 2;
-  const bool vec = D * size % 16 == 0 && aligned16(x) && aligned16(dx) && aligned16(w) && aligned16(dy) && aligned16(dx_residual);
+  const auto at = [](const void* v) { return reinterpret_cast<uintptr_t>(v); };
+  const uintptr_t operands = (at(x) ^ at(dx)) | (at(x) ^ at(dy)) | (dx_residual ? at(x) ^ at(dx_residual) : 0), weights = at(w);
   int blocks = 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (int rc = dtype == MCB_F32 ? lnorm::launch<float, true>(p, vec, ds->sm_count, st, &blocks)
-                                : lnorm::launch<__nv_bfloat16, true>(p, vec, ds->sm_count, st, &blocks)) return rc;
+  if (int rc = dtype == MCB_F32 ? lnorm::launch<float, true>(p, operands, weights, ds->sm_count, st, &blocks)
+                                : lnorm::launch<__nv_bfloat16, true>(p, operands, weights, ds->sm_count, st, &blocks)) return rc;
   if (!sums) return MCB_OK;
   MCB_CHECK_CUDA(launch_kernel(lnorm::ln_reduce_kernel, dim3(static_cast<unsigned>((2 * D + 31) / 32)), dim3(1024), 0, st, chained_launch(),
                                static_cast<const float*>(p.part), blocks, p.D, dw, db, accumulate));

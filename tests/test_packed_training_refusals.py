@@ -89,7 +89,7 @@ def test_layer_norm(lib):
         assert call(eps=-1.0) == SHAPE and call(eps=math.nan) == SHAPE and call(eps=math.inf) == SHAPE
     assert fwd(y=None) == NULL and bwd(dy=None) == NULL and bwd(dx=None) == NULL
     need = lib.mcb_layernorm_bwd_workspace_bytes(4, 8)
-    assert need == 4 * 2 * 8 * 4 and lib.mcb_layernorm_bwd_workspace_bytes(0, 8) == 0
+    assert need == 8 * 2 * 8 * 4 and lib.mcb_layernorm_bwd_workspace_bytes(0, 8) == 0
     assert bwd(ws=None) == WORKSPACE and bwd(n=need - 1) == WORKSPACE and bwd(ws=20) == WORKSPACE and bwd(dw=None, ws=None) == WORKSPACE
 
 
