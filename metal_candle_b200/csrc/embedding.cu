@@ -21,7 +21,7 @@ namespace mcb {
 namespace embed {
 namespace {
 
-constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32, kDigits = 512, kMaxTile = 32, kThreads = 128;
+constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32, kDigits = 512, kMaxTile = 32, kThreads = 128, kJoinThreads = 256;
 constexpr uint32_t kFull = 0xffffffffu;
 
 // ---- forward -----------------------------------------------------------------------------------------------------------
@@ -271,38 +271,52 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const __grid_constant__ S
   }
 }
 
-// The runs that go on behind the tile in which they begin.
+// The runs that go on behind the tile in which they begin, a block to a tile (most have nothing to do and leave).  kJoinThreads / tx groups of
+// threads share the parts of a run, consecutive ones each, and add their sums up in order: a token of a thousand rows waits for memory
+// a few times and not a hundred.
 template <int N>
-__global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ SumParams p) {
-  const int x = threadIdx.x % p.tx, y = threadIdx.x / p.tx, ty = kThreads / p.tx;
-  const int t = blockIdx.x * ty + y;
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ SumParams p) {
+  __shared__ float sums[kJoinThreads * N];
+  __shared__ int64_t found;
+  const int t = blockIdx.x;
   grid_launch_dependents();
   grid_dependency_wait();
-  if (t >= p.tiles) return;
   const uint32_t* keys = from_here(p.key);
   const int64_t i0 = static_cast<int64_t>(t) * p.tile, i1 = i0 + p.tile;
   if (i1 >= p.M) return;
-  const uint32_t id = __ldcg(keys + i1 - 1);
-  if (id >= static_cast<uint32_t>(p.vocab) || __ldcg(keys + i1) != id) return;
-  if (i0 > 0 && __ldcg(keys + i0 - 1) == id) return;   // it began in a tile before
+  const uint32_t id = __ldcg(keys + i1 - 1), next = __ldcg(keys + i1), before = i0 > 0 ? __ldcg(keys + i0 - 1) : static_cast<uint32_t>(p.vocab);
+  if (id >= static_cast<uint32_t>(p.vocab) || next != id || before == id) return;   // no run that begins here goes on
+  // the last tile that it reaches: tile q does where its first key is this id.  32 tiles a look, or 32 groups of 32 where they are not enough
+  if (threadIdx.x < 32) {
+    int64_t last = t + 1;
+    for (int64_t step = 1;;) {
+      const int64_t q = last + step * (threadIdx.x + 1);
+      const int n = __popc(__ballot_sync(kFull, q < p.tiles && __ldcg(keys + q * p.tile) == id));
+      last += step * n;
+      if (n == 32) step *= 32;
+      else if (step == 1) break;
+      else step /= 32;
+    }
+    if (threadIdx.x == 0) found = last;
+  }
+  __syncthreads();
+  const int64_t last = found, count = last - t;   // parts behind this tile's own
+  const int x = threadIdx.x % p.tx, g = threadIdx.x / p.tx, groups = count < 8 ? 1 : kJoinThreads / p.tx;
   const int64_t c = N * (static_cast<int64_t>(blockIdx.y) * p.tx + x);
-  if (c >= p.H) return;
-  // last token of the run: steps that double, then halving
-  int64_t lo = i1, hi = p.M - 1;
-  for (int64_t far = p.tile; lo + far <= hi; far *= 2) {
-    if (__ldcg(keys + lo + far) != id) { hi = lo + far - 1; break; }
-    lo += far;
-  }
-  while (lo < hi) {
-    const int64_t mid = (lo + hi + 1) >> 1;
-    if (__ldcg(keys + mid) == id) lo = mid;
-    else hi = mid - 1;
-  }
   float acc[N] = {};
-  get_add<N>(p.part + (2 * static_cast<int64_t>(t) + 1) * p.H + c, acc);
-#pragma unroll 4
-  for (int64_t q = t + 1; q <= lo / p.tile; ++q) get_add<N>(p.part + 2 * q * p.H + c, acc);
-  finish<N>(p, id, c, acc);
+  if (g < groups && c < p.H) {
+    if (g == 0) get_add<N>(p.part + (2 * static_cast<int64_t>(t) + 1) * p.H + c, acc);
+    const int64_t to = t + 1 + count * (g + 1) / groups;
+#pragma unroll 8
+    for (int64_t q = t + 1 + count * g / groups; q < to; ++q) get_add<N>(p.part + 2 * q * p.H + c, acc);
+  }
+  if (groups > 1) {
+    put<N>(sums + threadIdx.x * N, acc);
+    __syncthreads();
+    if (g == 0)
+      for (int o = 1; o < groups; ++o) get_add<N>(sums + (o * p.tx + x) * N, acc);
+  }
+  if (g == 0 && c < p.H) finish<N>(p, id, c, acc);
 }
 
 inline size_t up256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
@@ -348,7 +362,7 @@ int launch_sums(SumParams& p, cudaStream_t st) {
   MCB_CHECK_CUDA(launch_kernel(sum_kernel<T, N>, grid, dim3(kThreads), 0, st, chained_launch(), p));
   MCB_CHECK_LAUNCH("embedding_sum");
   if (p.tiles > 1) {
-    MCB_CHECK_CUDA(launch_kernel(join_kernel<N>, grid, dim3(kThreads), 0, st, chained_launch(), p));
+    MCB_CHECK_CUDA(launch_kernel(join_kernel<N>, dim3(static_cast<unsigned>(p.tiles), grid.y), dim3(kJoinThreads), 0, st, chained_launch(), p));
     MCB_CHECK_LAUNCH("embedding_join");
   }
   return MCB_OK;

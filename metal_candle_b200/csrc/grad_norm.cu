@@ -41,29 +41,27 @@ __device__ __forceinline__ const Tensor& tensor_of(const Table& tab, uint32_t pi
   return tab.t[lo];
 }
 
-// The 16 elements of a thread in its piece: N at a time, N * (tid + 256 k) on.  at: the piece's first element.
-template <typename T, int N, typename F>
-__device__ __forceinline__ void for_piece(const T* g, int64_t n, int64_t at, F&& f) {
-  float v[16];
+// The 16 elements of a thread in its piece, which begins at element `at`: N at a time, N * (tid + 256 k) on.  VEC: N == 1, or g + at is on a 16-byte boundary.
+// N > 1 without it reads the N elements one by one: they are the same lines, from L1.
+template <typename T, int N, bool VEC>
+__device__ __forceinline__ void load_piece(const T* g, int64_t n, int64_t at, float (&v)[16]) {
 #pragma unroll
   for (int k = 0; k < 16 / N; ++k) {
     const int64_t i = at + N * (threadIdx.x + kThreads * k);
 #pragma unroll
     for (int e = 0; e < N; ++e) v[N * k + e] = 0.0f;
-    if (i + N <= n) {
-      if constexpr (N == 1) {
-        v[k] = to_f32(g[i]);
-      } else {
+    if (N > 1 && VEC && i + N <= n) {
+      if constexpr (N > 1) {
         Vec16<T> x;
         x.raw = *reinterpret_cast<const decltype(x.raw)*>(g + i);
         x.to_float(v + N * k);
       }
     } else {
+#pragma unroll
       for (int e = 0; e < N; ++e)
         if (i + e < n) v[N * k + e] = to_f32(g[i + e]);
     }
   }
-  f(v);
 }
 
 __device__ __forceinline__ double squares(const float (&v)[16]) {
@@ -79,19 +77,14 @@ __device__ __forceinline__ double squares(const float (&v)[16]) {
   return d;
 }
 
-// vec: 16 bytes at a time.  Otherwise neighbouring threads take neighbouring elements, so that a warp's access is whole lines again.
-template <typename F>
-__device__ __forceinline__ void with_piece(const Tensor& t, uint32_t piece, bool vec, F&& f) {
-  const int64_t at = static_cast<int64_t>(piece - t.first) * kPiece;
-  if (t.dtype == MCB_F32) {
-    const float* g = static_cast<const float*>(t.g);
-    if (vec) for_piece<float, 4>(g, t.n, at, f);
-    else for_piece<float, 1>(g, t.n, at, f);
-  } else {
-    const __nv_bfloat16* g = static_cast<const __nv_bfloat16*>(t.g);
-    if (vec) for_piece<__nv_bfloat16, 8>(g, t.n, at, f);
-    else for_piece<__nv_bfloat16, 1>(g, t.n, at, f);
-  }
+template <typename T>
+__device__ __forceinline__ double piece_squares(const Tensor& t, int64_t at) {
+  const T* g = static_cast<const T*>(t.g);
+  float v[16];
+  // (off a boundary neighbouring threads take neighbouring elements, so that a warp's access is whole lines again)
+  if ((reinterpret_cast<uintptr_t>(g) & 15u) == 0) load_piece<T, Vec16<T>::N, true>(g, t.n, at, v);
+  else load_piece<T, 1, true>(g, t.n, at, v);
+  return squares(v);
 }
 
 __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant__ Table tab, double* part) {
@@ -101,7 +94,8 @@ __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant
   double sum = 0.0;
   for (uint32_t piece = blockIdx.x; piece < tab.pieces; piece += gridDim.x) {
     const Tensor& t = tensor_of(tab, piece);
-    with_piece(t, piece, (reinterpret_cast<uintptr_t>(t.g) & 15u) == 0, [&](const float (&v)[16]) { sum += squares(v); });
+    const int64_t at = static_cast<int64_t>(piece - t.first) * kPiece;
+    sum += t.dtype == MCB_F32 ? piece_squares<float>(t, at) : piece_squares<__nv_bfloat16>(t, at);
   }
   sum = block_sum(sum, s);
   if (threadIdx.x == 0) part[blockIdx.x] = sum;
@@ -115,23 +109,33 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const double* part, int 
   if (threadIdx.x == 0) norm[0] = v;
 }
 
-template <typename T, int N>
-__device__ __forceinline__ void store_piece(T* out, int64_t n, int64_t at, const float (&v)[16], float f) {
+// Pieces go by the output's 16-byte boundaries, the first few elements of a tensor by themselves: what is written are whole vectors
+// (written element by element, 250 M elements that lie off the gradients' alignment took 421 us instead of CLIP_US).
+template <typename T>
+__device__ __forceinline__ void clip_piece(const Tensor& t, int64_t piece, float f) {
+  constexpr int N = Vec16<T>::N;
+  const T* g = static_cast<const T*>(t.g);
+  T* out = static_cast<T*>(t.out);
+  const int head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(out) & 15u)) % 16 / sizeof(T));
+  if (piece == 0 && static_cast<int>(threadIdx.x) < head && threadIdx.x < t.n) out[threadIdx.x] = from_f32<T>(to_f32(g[threadIdx.x]) * f);
+  const int64_t at = head + piece * kPiece;
+  float v[16];
+  if ((reinterpret_cast<uintptr_t>(g + head) & 15u) == 0) load_piece<T, N, true>(g, t.n, at, v);
+  else load_piece<T, N, false>(g, t.n, at, v);
 #pragma unroll
   for (int k = 0; k < 16 / N; ++k) {
     const int64_t i = at + N * (threadIdx.x + kThreads * k);
     float w[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) w[e] = v[N * k + e] * f;
-    if (N > 1 && i + N <= n) {
-      if constexpr (N > 1) {
-        Vec16<T> x;
-        x.from_float(w);
-        *reinterpret_cast<decltype(x.raw)*>(out + i) = x.raw;
-      }
+    if (i + N <= t.n) {
+      Vec16<T> x;
+      x.from_float(w);
+      *reinterpret_cast<decltype(x.raw)*>(out + i) = x.raw;
     } else {
+#pragma unroll
       for (int e = 0; e < N; ++e)
-        if (i + e < n) out[i + e] = from_f32<T>(w[e]);
+        if (i + e < t.n) out[i + e] = from_f32<T>(w[e]);
     }
   }
 }
@@ -146,17 +150,8 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ 
   for (uint32_t i = blockIdx.x; i < tab.pieces; i += gridDim.x) {
     const uint32_t piece = tab.pieces - 1 - i;
     const Tensor& t = tensor_of(tab, piece);
-    const int64_t at = static_cast<int64_t>(piece - t.first) * kPiece;
-    const bool vec = ((reinterpret_cast<uintptr_t>(t.g) | reinterpret_cast<uintptr_t>(t.out)) & 15u) == 0;
-    with_piece(t, piece, vec, [&](const float (&v)[16]) {
-      if (t.dtype == MCB_F32) {
-        if (vec) store_piece<float, 4>(static_cast<float*>(t.out), t.n, at, v, f);
-        else store_piece<float, 1>(static_cast<float*>(t.out), t.n, at, v, f);
-      } else {
-        if (vec) store_piece<__nv_bfloat16, 8>(static_cast<__nv_bfloat16*>(t.out), t.n, at, v, f);
-        else store_piece<__nv_bfloat16, 1>(static_cast<__nv_bfloat16*>(t.out), t.n, at, v, f);
-      }
-    });
+    if (t.dtype == MCB_F32) clip_piece<float>(t, piece - t.first, f);
+    else clip_piece<__nv_bfloat16>(t, piece - t.first, f);
   }
 }
 

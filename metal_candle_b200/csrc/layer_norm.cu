@@ -471,13 +471,14 @@ int launch_k(const Params& p, int sms, cudaStream_t st, int* blocks) {
   return MCB_OK;
 }
 // A row's threads: as few as have at most two vectors of it each (32768 x 896 bfloat16, backward with its reduction: 64 threads with two
-// 64.5 us, 32 with four 83, 128 with one 68.6: the sums of a thread's columns are registers, and rows in flight go with the threads).
+// 64.5 us, 32 with four 83, 128 with one 68.6: the sums of a thread's columns are registers, and rows in flight go with the threads.  Forward: 32 with four 23 us, 64 with two 27).
 template <typename T, bool BWD, bool SHIFT>
 int launch_rows(const Params& p, int vecs, int sms, cudaStream_t st, int* blocks) {
   if (vecs <= 8) return launch_k<T, BWD, SHIFT, 8, 1>(p, sms, st, blocks);
   if (vecs <= 16) return launch_k<T, BWD, SHIFT, 8, 2>(p, sms, st, blocks);
   if (vecs <= 32) return launch_k<T, BWD, SHIFT, 32, 1>(p, sms, st, blocks);
   if (vecs <= 64) return launch_k<T, BWD, SHIFT, 32, 2>(p, sms, st, blocks);
+  if (!BWD && vecs <= 128) return launch_k<T, BWD, SHIFT, 32, 4>(p, sms, st, blocks);
   if (vecs <= 128) return launch_k<T, BWD, SHIFT, 64, 2>(p, sms, st, blocks);
   if (vecs <= 256) return launch_k<T, BWD, SHIFT, 128, 2>(p, sms, st, blocks);
   if (vecs <= 512) return launch_k<T, BWD, SHIFT, 256, 2>(p, sms, st, blocks);
