@@ -17,7 +17,7 @@ struct Layout {
   int64_t keys;     // int2 [batch, seq]: the queries [x, y) that see key position i
   int64_t qtiles;   // int2 [batch, tiles]: first key block (of 64) and number of blocks that the tile's queries see
   int64_t ktiles;   // int2 [batch, tiles]: first query block (of 64) and number of blocks that see the tile's keys
-  int64_t qwork;    // int4 [batch * tiles]: the query tiles, the most key blocks first: sequence, tile, first block, blocks
+  int64_t qwork;    // int4 [batch * tiles]: the query tiles, the most key blocks first (of each sequence): sequence, tile, first block, blocks
   int64_t kwork;    // int4 [batch * tiles]: the key tiles, the most query blocks first
   int64_t ticket;   // int: tiles that are done while the block is being made
   int64_t bits;     // two three-level bitmaps per sequence: where runs begin, where a position is no prefix

@@ -6,8 +6,8 @@
 // every run of equal ids is one sum, held in registers and written once.  Nothing uses floating-point atomics: the same
 // tokens give the same bits, and a token that comes a thousand times costs no more than a thousand different ones.
 //   1. sort (one cluster): radix sort of ceil(log2(vocab + 1)) bits, up to 9 a pass.  A warp owns consecutive tokens; within 32 of them
-//      equal digits are ranked by match; counts of digits go from warp to block to cluster through shared memory.  The other blocks of
-//      the launch write the table's zeros meanwhile (not with accumulate): 0.54 GB for 151936 x 896, which hides the sort.
+//      equal digits are ranked by match; counts of digits go from warp to block to cluster through shared memory.  The launch's other
+//      blocks write zeros meanwhile; the rest of the table's are written beside the sums, but for the rows that get one.
 //   2. sums: a tile of 8 to 32 sorted tokens by as many threads as the columns take; a run that ends inside its tile is written out, one
 //      that goes on leaves its part.  3. The tile where such a run begins adds up the parts, in order.
 // HBM-bound by the table's gradient (float32, written whole) where it is not accumulated.
@@ -21,7 +21,8 @@ namespace mcb {
 namespace embed {
 namespace {
 
-constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32, kDigits = 512, kMaxTile = 32, kThreads = 128, kJoinThreads = 256;
+constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32, kDigits = 512, kMaxTile = 32, kThreads = 128, kJoinThreads = 256, kZeroRows = 64;
+constexpr int64_t kEarlyBytes = 64 << 20;   // of zeros beside the sort: about what its 10 us are enough for
 constexpr uint32_t kFull = 0xffffffffu;
 
 // ---- forward -----------------------------------------------------------------------------------------------------------
@@ -62,7 +63,7 @@ __global__ void __launch_bounds__(kThreads) embed_fwd_kernel(const I* ids, const
 struct SortParams {
   const void* ids;
   uint32_t *key[2], *pos[2];   // the result of pass p is in buffer p & 1
-  float* zero;                 // the table's gradient, or null
+  float* zero;                 // zeros for the blocks behind the cluster to write, zero_n elements
   int64_t zero_n;
   int64_t vocab;
   int M, passes, digit_bits;
@@ -75,7 +76,9 @@ __device__ __forceinline__ uint32_t key_of(const SortParams& p, const uint32_t* 
   return id >= 0 && id < p.vocab ? static_cast<uint32_t>(id) : static_cast<uint32_t>(p.vocab);   // the others behind all
 }
 
-template <typename I>
+// KEEP: a warp has at most KEEP x 32 tokens, and keeps keys, positions and ranks in registers between the two walks of a pass.
+// 0: any number, read again.
+template <typename I, int KEEP>
 __global__ void __launch_bounds__(kSortThreads) sort_kernel(const __grid_constant__ SortParams p) {
   __shared__ uint32_t hist[kSortWarps][kDigits];   // of a warp: counts, then where its next token of a digit goes
   __shared__ uint32_t total[kDigits];              // of the block; read by the others of the cluster
@@ -83,52 +86,82 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const __grid_constan
   cg::cluster_group cl = cg::this_cluster();
   const int C = static_cast<int>(cl.num_blocks()), rank = static_cast<int>(cl.block_rank());
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  grid_launch_dependents();
-  grid_dependency_wait();
   if (blockIdx.x >= static_cast<unsigned>(C)) {
-    // zeros, 16 bytes a store (the start is aligned: checked on the host; the last few elements one by one)
+    grid_launch_dependents();
+    grid_dependency_wait();
     const int64_t n4 = p.zero_n >> 2, step = static_cast<int64_t>(gridDim.x - C) * kSortThreads;
-    const int64_t first = static_cast<int64_t>(blockIdx.x - C) * kSortThreads + threadIdx.x;
-    for (int64_t i = first; i < n4; i += step) reinterpret_cast<float4*>(p.zero)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int64_t i = (n4 << 2) + first; i < p.zero_n; i += step) p.zero[i] = 0.0f;
+    const int64_t at = static_cast<int64_t>(blockIdx.x - C) * kSortThreads + threadIdx.x;
+    for (int64_t i = at; i < n4; i += step) __stcs(reinterpret_cast<float4*>(p.zero) + i, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+    for (int64_t i = (n4 << 2) + at; i < p.zero_n; i += step) p.zero[i] = 0.0f;
     return;
   }
   const int warps = C * kSortWarps;
   const int per = ((p.M + warps - 1) / warps + 31) & ~31;   // tokens of a warp
   const int64_t begin = static_cast<int64_t>(rank * kSortWarps + warp) * per;
   const int end = static_cast<int>(begin + per < p.M ? begin + per : p.M);
+  const int digits = 1 << p.digit_bits;
+  for (int d = lane; d < digits; d += 32) hist[warp][d] = 0;
+  grid_launch_dependents();
+  grid_dependency_wait();
   for (int pass = 0; pass < p.passes; ++pass) {
     const int shift = pass * p.digit_bits;
+    const uint32_t mask = static_cast<uint32_t>(digits) - 1u;
     const uint32_t *from_key = from_here(p.key[(pass + 1) & 1]), *from_pos = from_here(p.pos[(pass + 1) & 1]);   // what the pass before has left
-    const uint32_t mask = (1u << p.digit_bits) - 1u;
-    for (int d = lane; d < kDigits; d += 32) hist[warp][d] = 0;
-    __syncwarp();
-    for (int64_t i0 = begin; i0 < end; i0 += 32) {
-      const int i = static_cast<int>(i0) + lane;
-      const uint32_t have = __ballot_sync(kFull, i < end);
-      if (i < end) {
-        const uint32_t d = (key_of<I>(p, from_key, pass, i) >> shift) & mask;
-        const uint32_t peers = __match_any_sync(have, d);
-        if (lane == __ffs(peers) - 1) hist[warp][d] += __popc(peers);
+    uint32_t key[KEEP + 1], at[KEEP + 1], before_me[KEEP + 1];
+    // a walk over 32 tokens: counts their digits into the warp's, and says how many of its digit the warp has had before a token
+    auto count = [&](uint32_t d, uint32_t have) -> uint32_t {
+      const uint32_t peers = __match_any_sync(have, d), base = hist[warp][d];
+      __syncwarp(have);
+      if (lane == __ffs(peers) - 1) hist[warp][d] = base + __popc(peers);
+      return base + __popc(peers & ((1u << lane) - 1u));
+    };
+    if constexpr (KEEP > 0) {
+#pragma unroll
+      for (int n = 0; n < KEEP; ++n) {
+        const int64_t i = begin + 32 * n + lane;
+        key[n] = at[n] = 0;
+        if (i < end) {
+          key[n] = key_of<I>(p, from_key, pass, static_cast<int>(i));
+          at[n] = pass > 0 ? __ldcg(from_pos + i) : static_cast<uint32_t>(i);
+        }
       }
-      __syncwarp();
+#pragma unroll
+      for (int n = 0; n < KEEP; ++n) {
+        const bool in = begin + 32 * n + lane < end;
+        const uint32_t have = __ballot_sync(kFull, in);
+        if (in) before_me[n] = count((key[n] >> shift) & mask, have);
+        __syncwarp();
+      }
+    } else {
+      for (int64_t i0 = begin; i0 < end; i0 += 32) {
+        const int i = static_cast<int>(i0) + lane;
+        const uint32_t have = __ballot_sync(kFull, i < end);
+        if (i < end) count((key_of<I>(p, from_key, pass, i) >> shift) & mask, have);
+        __syncwarp();
+      }
     }
     __syncthreads();
     // counts of the warps before, within the block; kDigits == kSortThreads: one digit a thread
     uint32_t sum = 0;
-    for (int w = 0; w < kSortWarps; ++w) {
-      const uint32_t n = hist[w][threadIdx.x];
-      hist[w][threadIdx.x] = sum;
-      sum += n;
+    if (static_cast<int>(threadIdx.x) < digits) {
+      uint32_t n[kSortWarps];
+#pragma unroll
+      for (int w = 0; w < kSortWarps; ++w) n[w] = hist[w][threadIdx.x];
+#pragma unroll
+      for (int w = 0; w < kSortWarps; ++w) {
+        hist[w][threadIdx.x] = sum;
+        sum += n[w];
+      }
+      total[threadIdx.x] = sum;
     }
-    total[threadIdx.x] = sum;
     cl.sync();
     uint32_t all = 0, before = 0;   // tokens of this digit in the cluster, and in the blocks before this one
-    for (int r = 0; r < C; ++r) {
-      const uint32_t n = *cl.map_shared_rank(&total[threadIdx.x], r);
-      if (r < rank) before += n;
-      all += n;
-    }
+    if (static_cast<int>(threadIdx.x) < digits)
+      for (int r = 0; r < C; ++r) {
+        const uint32_t n = *cl.map_shared_rank(&total[threadIdx.x], r);
+        if (r < rank) before += n;
+        all += n;
+      }
     // exclusive sum over the digits
     uint32_t inc = all;
 #pragma unroll
@@ -140,24 +173,34 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const __grid_constan
     __syncthreads();
     uint32_t base = inc - all + before;
     for (int w = 0; w < warp; ++w) base += scan[w];
-    for (int w = 0; w < kSortWarps; ++w) hist[w][threadIdx.x] += base;
-    __syncthreads();
-    uint32_t *key = p.key[pass & 1], *pos = p.pos[pass & 1];
-    for (int64_t i0 = begin; i0 < end; i0 += 32) {
-      const int i = static_cast<int>(i0) + lane;
-      const uint32_t have = __ballot_sync(kFull, i < end);
-      if (i < end) {
-        const uint32_t k = key_of<I>(p, from_key, pass, i), d = (k >> shift) & mask;
-        const uint32_t at = pass > 0 ? __ldcg(from_pos + i) : static_cast<uint32_t>(i);
-        const uint32_t peers = __match_any_sync(have, d);
-        const uint32_t to = hist[warp][d] + __popc(peers & ((1u << lane) - 1u));
-        __syncwarp(have);
-        if (lane == __ffs(peers) - 1) hist[warp][d] += __popc(peers);
-        key[to] = k;
-        pos[to] = at;
-      }
-      __syncwarp();
+    if (static_cast<int>(threadIdx.x) < digits) {
+#pragma unroll
+      for (int w = 0; w < kSortWarps; ++w) hist[w][threadIdx.x] += base;
     }
+    __syncthreads();
+    uint32_t *to_key = p.key[pass & 1], *to_pos = p.pos[pass & 1];
+    if constexpr (KEEP > 0) {
+#pragma unroll
+      for (int n = 0; n < KEEP; ++n)
+        if (begin + 32 * n + lane < end) {
+          const uint32_t to = hist[warp][(key[n] >> shift) & mask] + before_me[n];
+          to_key[to] = key[n];
+          to_pos[to] = at[n];
+        }
+      __syncwarp();
+    } else {
+      for (int64_t i0 = begin; i0 < end; i0 += 32) {
+        const int i = static_cast<int>(i0) + lane;
+        const uint32_t have = __ballot_sync(kFull, i < end);
+        if (i < end) {
+          const uint32_t k = key_of<I>(p, from_key, pass, i), to = count((k >> shift) & mask, have);
+          to_key[to] = k;
+          to_pos[to] = pass > 0 ? __ldcg(from_pos + i) : static_cast<uint32_t>(i);
+        }
+        __syncwarp();
+      }
+    }
+    for (int d = lane; d < digits; d += 32) hist[warp][d] = 0;
     __threadfence();
     cl.sync();   // the pass is in memory, and nobody reads this block's totals any more
   }
@@ -171,8 +214,9 @@ struct SumParams {
   float* part;      // [tiles][2][H]: of the tile's first run where it began before, of its last where it goes on (a run that
                     // does both is in the first)
   int64_t H;
-  int64_t vocab;
+  int64_t vocab, early;   // early: rows that hold zeros already
   int M, tile, tiles, tx, accumulate;   // tile: sorted tokens of one, 8 to kMaxTile
+  int cols, sum_blocks;                 // blocks to a tile's columns, and of sums in all: the blocks behind them write zeros
   float scale;
 };
 
@@ -206,15 +250,64 @@ __device__ __forceinline__ void finish(const SumParams& p, uint32_t id, int64_t 
   put<N>(g, v);
 }
 
+// Zeros for the rows [first, first + kZeroRows) of the table that no token names, past the L2 (the parts of long runs wait there).
+__device__ __forceinline__ void zero_rows(const SumParams& p, const uint32_t* keys, int64_t first, uint32_t* named) {
+  const int64_t end = first + kZeroRows < p.vocab ? first + kZeroRows : p.vocab;
+  if (threadIdx.x < kZeroRows / 32) named[threadIdx.x] = 0;
+  __syncthreads();
+  // the first sorted token that names a row from `first` on: lo, found by 32 looks at a time; then mark what follows
+  if (threadIdx.x < 32) {
+    int64_t lo = 0, hi = p.M;   // keys before lo are below first, keys from hi on are not
+    while (lo < hi) {
+      const int64_t step = (hi - lo + 31) / 32, q = lo + step * (threadIdx.x + 1) - 1;
+      const int n = __popc(__ballot_sync(kFull, q < hi && __ldcg(keys + q) < first));
+      lo += step * n;
+      hi = lo + step - 1 < hi ? lo + step - 1 : hi;
+    }
+    for (;;) {
+      const int64_t i = lo + threadIdx.x;
+      const bool in = i < p.M && __ldcg(keys + i) < end;
+      if (in) {
+        const uint32_t r = static_cast<uint32_t>(__ldcg(keys + i) - first);
+        atomicOr(&named[r >> 5], 1u << (r & 31));
+      }
+      if (__ballot_sync(kFull, in) != kFull) break;
+      lo += 32;
+    }
+  }
+  __syncthreads();
+  const bool vec = p.H % 4 == 0;
+  uint32_t any = 0;
+  for (int i = 0; i < kZeroRows / 32; ++i) any |= named[i];
+  if (any == 0 && vec) {   // all of them, without the rows between
+    float4* to = reinterpret_cast<float4*>(p.grad + first * p.H);
+    for (int64_t i = threadIdx.x; i < (end - first) * p.H / 4; i += kThreads) __stcs(to + i, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+    return;
+  }
+  for (int64_t r = first; r < end; ++r) {
+    const int k = static_cast<int>(r - first);
+    if (named[k >> 5] >> (k & 31) & 1u) continue;
+    float* row = p.grad + r * p.H;
+    if (vec)
+      for (int64_t i = threadIdx.x; i < p.H / 4; i += kThreads) __stcs(reinterpret_cast<float4*>(row) + i, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+    else
+      for (int64_t i = threadIdx.x; i < p.H; i += kThreads) row[i] = 0.0f;
+  }
+}
+
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads) sum_kernel(const __grid_constant__ SumParams p) {
   __shared__ uint32_t s_key[kThreads][kMaxTile + 2], s_pos[kThreads][kMaxTile];   // by tile of the block (at most kThreads of them)
   const int x = threadIdx.x % p.tx, y = threadIdx.x / p.tx, ty = kThreads / p.tx;
-  const int t = blockIdx.x * ty + y;
+  const int64_t t = static_cast<int64_t>(blockIdx.x / p.cols) * ty + y;
   grid_launch_dependents();
   grid_dependency_wait();
   const uint32_t *keys = from_here(p.key), *places = from_here(p.pos);
-  const int64_t i0 = static_cast<int64_t>(t) * p.tile;
+  if (blockIdx.x >= static_cast<unsigned>(p.sum_blocks)) {
+    zero_rows(p, keys, p.early + static_cast<int64_t>(blockIdx.x - p.sum_blocks) * kZeroRows, s_key[0]);
+    return;
+  }
+  const int64_t i0 = t * p.tile;
   const int n = t < p.tiles ? static_cast<int>(i0 + p.tile < p.M ? p.tile : p.M - i0) : 0;
   const uint32_t none = static_cast<uint32_t>(p.vocab);
   // keys of the tile with one on either side
@@ -225,7 +318,7 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const __grid_constant__ S
   }
   __syncthreads();
   if (n == 0) return;
-  const int64_t c = N * (static_cast<int64_t>(blockIdx.y) * p.tx + x);
+  const int64_t c = N * (static_cast<int64_t>(blockIdx.x % p.cols) * p.tx + x);
   if (c >= p.H) return;
   const T* dout = static_cast<const T*>(p.dout) + c;
   const bool began = s_key[y][0] == s_key[y][1], goes_on = s_key[y][n] == s_key[y][n + 1] && i0 + n < p.M;
@@ -260,8 +353,8 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const __grid_constant__ S
       if (!last && s_key[y][i + 2] == id) continue;
       // the run ends here, or goes on behind the tile
       if (id != none) {
-        if (first && began && i0 > 0) put<N>(p.part + (2 * static_cast<int64_t>(t)) * p.H + c, acc);
-        else if (last && goes_on) put<N>(p.part + (2 * static_cast<int64_t>(t) + 1) * p.H + c, acc);
+        if (first && began && i0 > 0) put<N>(p.part + (2 * t) * p.H + c, acc);
+        else if (last && goes_on) put<N>(p.part + (2 * t + 1) * p.H + c, acc);
         else finish<N>(p, id, c, acc);
       }
       first = false;
@@ -335,9 +428,10 @@ template <typename I>
 int launch_sort(const SortParams& p, int sms, cudaStream_t st) {
   // few tokens: a block alone ranks them sooner than eight that wait for one another three times a pass
   const int C = p.M <= 1024 ? 1 : 8;
-  int64_t fill = p.zero == nullptr ? 0 : (p.zero_n / 4 + kSortThreads * 4 - 1) / (kSortThreads * 4) + 1;
-  if (fill > 4 * sms) fill = 4 * sms;
   cudaLaunchConfig_t cfg = {};
+  int64_t fill = (p.zero_n / 4 + kSortThreads * 4 - 1) / (kSortThreads * 4);
+  if (p.zero_n > 0 && fill == 0) fill = 1;
+  if (fill > 2 * sms) fill = 2 * sms;
   cfg.gridDim = dim3(static_cast<unsigned>(C + (fill + C - 1) / C * C));
   cfg.blockDim = dim3(kSortThreads);
   cfg.stream = st;
@@ -347,7 +441,8 @@ int launch_sort(const SortParams& p, int sms, cudaStream_t st) {
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = C; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr; cfg.numAttrs = 2;
-  MCB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, sort_kernel<I>, p));
+  const bool few = p.M <= C * kSortWarps * 128;
+  MCB_CHECK_CUDA(few ? cudaLaunchKernelEx(&cfg, sort_kernel<I, 4>, p) : cudaLaunchKernelEx(&cfg, sort_kernel<I, 0>, p));
   MCB_CHECK_LAUNCH("embedding_sort");
   return MCB_OK;
 }
@@ -357,12 +452,13 @@ int launch_sums(SumParams& p, cudaStream_t st) {
   p.tx = row_threads((p.H + N - 1) / N);
   const int ty = kThreads / p.tx;
   const int64_t cols = (p.H + static_cast<int64_t>(N) * p.tx - 1) / (static_cast<int64_t>(N) * p.tx);
-  if (cols > 65535) return fail(MCB_ERR_SHAPE, "embedding_bwd: H=%lld", (long long)p.H);
-  const dim3 grid(static_cast<unsigned>((p.tiles + ty - 1) / ty), static_cast<unsigned>(cols));
-  MCB_CHECK_CUDA(launch_kernel(sum_kernel<T, N>, grid, dim3(kThreads), 0, st, chained_launch(), p));
+  const int64_t sums = (p.tiles + ty - 1) / ty * cols, zeros = (p.vocab - p.early + kZeroRows - 1) / kZeroRows;
+  if (cols > 65535 || sums + zeros > 0x7fffffff) return fail(MCB_ERR_SHAPE, "embedding_bwd: H=%lld", (long long)p.H);
+  p.cols = static_cast<int>(cols); p.sum_blocks = static_cast<int>(sums);
+  MCB_CHECK_CUDA(launch_kernel(sum_kernel<T, N>, dim3(static_cast<unsigned>(sums + zeros)), dim3(kThreads), 0, st, chained_launch(), p));
   MCB_CHECK_LAUNCH("embedding_sum");
   if (p.tiles > 1) {
-    MCB_CHECK_CUDA(launch_kernel(join_kernel<N>, dim3(static_cast<unsigned>(p.tiles), grid.y), dim3(kJoinThreads), 0, st, chained_launch(), p));
+    MCB_CHECK_CUDA(launch_kernel(join_kernel<N>, dim3(static_cast<unsigned>(p.tiles), static_cast<unsigned>(cols)), dim3(kJoinThreads), 0, st, chained_launch(), p));
     MCB_CHECK_LAUNCH("embedding_join");
   }
   return MCB_OK;
@@ -439,8 +535,11 @@ extern "C" int mcb_embedding_bwd(const void* ids, int id_bytes, const void* dout
     s.key[i] = reinterpret_cast<uint32_t*>(w + 2 * i * list);
     s.pos[i] = reinterpret_cast<uint32_t*>(w + (2 * i + 1) * list);
   }
-  s.zero = accumulate ? nullptr : dtable;
-  s.zero_n = vocab * H; s.vocab = vocab; s.M = static_cast<int>(M);
+  // what the sort's launch can write while it sorts, the rows behind that with the sums
+  int64_t early = accumulate ? vocab : embed::kEarlyBytes / (H * 4);
+  if (early > vocab) early = vocab;
+  if (!accumulate) { s.zero = dtable; s.zero_n = early * H; }
+  s.vocab = vocab; s.M = static_cast<int>(M);
   int bits = 1;
   while ((vocab >> bits) != 0) ++bits;   // of vocab itself, which stands for the ids that count for nothing
   s.passes = (bits + 8) / 9;
@@ -449,7 +548,7 @@ extern "C" int mcb_embedding_bwd(const void* ids, int id_bytes, const void* dout
   embed::SumParams p = {};
   p.key = s.key[(s.passes - 1) & 1]; p.pos = s.pos[(s.passes - 1) & 1];
   p.dout = dout; p.grad = dtable; p.part = reinterpret_cast<float*>(w + 4 * list);
-  p.H = H; p.vocab = vocab; p.M = static_cast<int>(M); p.tile = embed::tile_of(M); p.tiles = static_cast<int>(embed::tiles_of(M)); p.accumulate = accumulate; p.scale = scale;
+  p.H = H; p.vocab = vocab; p.early = early; p.M = static_cast<int>(M); p.tile = embed::tile_of(M); p.tiles = static_cast<int>(embed::tiles_of(M)); p.accumulate = accumulate; p.scale = scale;
   const int n = dtype == MCB_F32 ? 4 : 8;
   const bool vec = H % n == 0 && aligned16(dout);
   if (dtype == MCB_F32) return vec ? embed::launch_sums<float, 4>(p, st) : embed::launch_sums<float, 1>(p, st);

@@ -42,6 +42,7 @@
 // that owns a query row masks with two registers, and one that owns a key row with the interval of queries that see it.
 // Tiles walk over the key (query) blocks that some row of theirs sees, and the work list has the longest tiles first.
 #include <cuda.h>
+#include <cuda_fp16.h>
 #include <string.h>
 
 #include <cooperative_groups.h>
@@ -609,11 +610,9 @@ struct BwdParams {
 // Tensor memory (256 columns): S double-buffered at 0 and 64 (the next blocks' Q K^T run under this block's
 // arithmetic), dP at 128, dQ at 192.  dS (bf16 pairs, 32 columns) is written over the first half of dP, which has
 // been read by then, and is the A operand of dQ += dS K straight from tensor memory.
-template <bool MASKED, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 2)
 attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmdO,
-               const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const BwdParams p,
-               const __grid_constant__ CallOf<MASKED> c) {
+               const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const BwdParams p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen_base = smem_raw + (base - smem_u32(smem_raw));
@@ -652,18 +651,16 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
   const uint32_t tDP = tmem_base + 128, tDQ = tmem_base + 192;
   FwdParams tp;   // the item order of the forward
   tp.S = p.S; tp.G = p.G; tp.NB = p.NB;
-  Walk<MASKED> walk(tp, c);
-  FwdTile w;
+  const int n_tiles = q_blocks(p.S) * p.G * p.NB;
 
   if (warp == 0) {
     if (elect_one()) {
       int st = 0;
       uint32_t ph = 0;
       bool ok = true;
-      int it = -1;
-      while (ok && walk.get(w)) {
-        if (MASKED && w.nkb == 0) continue;
-        ++it;
+      int it = 0;
+      for (int t = blockIdx.x; ok && t < n_tiles; t += gridDim.x, ++it) {
+        const FwdTile w = fwd_tile(tp, t);
         // the previous item's last S and dP products have read Q and dO
         if (it > 0) ok = mbar_wait(q_free, (it - 1) & 1, abort_flag, 80, p.status);
         if (!ok) break;
@@ -677,8 +674,8 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
           if (!ok) break;
           const uint32_t sb = base + kDqOffStage + st * kDqStageBytes;
           mbar_expect_tx(kv_full0 + 8 * st, kDqStageBytes);
-          tma_load_3d(sb, &tmK, kv_full0 + 8 * st, 0, (w.kb0 + j) * kBK, w.nb);
-          tma_load_3d(sb + kKBytes, &tmV, kv_full0 + 8 * st, 0, (w.kb0 + j) * kBK, w.nb);
+          tma_load_3d(sb, &tmK, kv_full0 + 8 * st, 0, j * kBK, w.nb);
+          tma_load_3d(sb + kKBytes, &tmV, kv_full0 + 8 * st, 0, j * kBK, w.nb);
           if (++st == kDqStages) { st = 0; ph ^= 1; }
         }
       }
@@ -687,7 +684,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     if (elect_one()) {
       const uint32_t idesc = make_idesc(kBK);
       bool ok = true;
-      int it = -1;
+      int it = 0;
       uint32_t n0 = 0;
       int sst = 0;                // ring stage and phase of the next block to get its S product
       uint32_t sph = 0;
@@ -705,11 +702,10 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         if (++sst == kDqStages) { sst = 0; sph ^= 1; }
         return true;
       };
-      while (ok && walk.get(w)) {
-        if (MASKED && w.nkb == 0) continue;
-        ++it;
+      for (int t = blockIdx.x; ok && t < n_tiles; t += gridDim.x, ++it) {
+        const FwdTile w = fwd_tile(tp, t);
         ok = mbar_wait(q_full, it & 1, abort_flag, 84, p.status);
-        for (int j = 0; ok && j < 2 && j < w.nkb; ++j) ok = issue_s(n0 + j);
+        for (int j = 0; ok && j < 2; ++j) ok = issue_s(n0 + j);   // nkb >= 2
         for (int j = 0; ok && j < w.nkb; ++j) {
           const uint32_t n = n0 + j;
           const uint32_t sb = base + kDqOffStage + dst * kDqStageBytes;
@@ -748,15 +744,14 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
     const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
     bool ok = true;
     uint32_t n0 = 0;
-    int it = -1;
-    std::conditional_t<MASKED, Shape<CAP, BIAS>, NoCall> shape(c);
-    while (ok && walk.get(w)) {
+    int it = 0;
+    for (int t = blockIdx.x; ok && t < n_tiles; t += gridDim.x, ++it) {
+      const FwdTile w = fwd_tile(tp, t);
       const int qpos = w.qb * kBQ + row;
       // delta = sum_d dO * O of this row, straight from global memory (once per item)
       float delta = 0.0f, lse2 = INFINITY;   // of a row behind position S: P = dS = 0
       if (qpos < p.S) {
         lse2 = p.lse[w.qrow0 + row] * kLog2e;
-        if (MASKED && lse2 == -INFINITY) lse2 = INFINITY;   // a row that sees nothing
         const int64_t ooff = o_offset(p.S, p.G, p.HKV, p.o_tok, w.nb, w.g, w.qb * kBQ + row);
         const uint4* o4 = reinterpret_cast<const uint4*>(p.O + ooff);
         const uint4* d4 = reinterpret_cast<const uint4*>(p.dO + ooff);
@@ -774,29 +769,14 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       const int64_t prow = (static_cast<int64_t>(w.nb) * p.G + w.g) * (q_blocks(p.S) * kBQ) + qpos;
       p.ndelta[prow] = -delta;
       p.nlse2[prow] = -lse2;
-      int2 sees = make_int2(0, 0);
-      if constexpr (MASKED) {
-        if (qpos < p.S) sees = c.mask.rows[static_cast<int64_t>(w.b) * p.S + qpos];
-        if constexpr (BIAS) shape.slope2 = c.slopes[w.hk * p.G + w.g] * kLog2e;
-        if (w.nkb == 0) {
-          if (qpos < p.S) {
-            uint4* orow = reinterpret_cast<uint4*>(p.dQ + (w.qrow0 + row) * kD);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) orow[i] = make_uint4(0, 0, 0, 0);
-          }
-          continue;
-        }
-      }
-      ++it;
-      const float sc = CAP || BIAS ? 1.0f : p.sc;
-      const float2 sc2 = f2(sc, sc), nl2 = f2(-lse2, -lse2), nd2 = f2(-delta, -delta);
+      const float2 sc2 = f2(p.sc, p.sc), nl2 = f2(-lse2, -lse2), nd2 = f2(-delta, -delta);
       for (int j = 0; j < w.nkb; ++j) {
         const uint32_t n = n0 + j;
         ok = __all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * (n & 1), (n >> 1) & 1, abort_flag, 88, p.status));
         if (!ok) break;
         tcgen05_fence_after();
-        const int key0 = (w.kb0 + j) * kBK;
-        const bool diag = !MASKED && key0 + kBK - 1 > w.qb * kBQ;
+        const int key0 = j * kBK;
+        const bool diag = key0 + kBK - 1 > w.qb * kBQ;
         // the row's 64 scores, read once; P = 2^(s*sc - lse2) takes their place in the registers
         uint32_t sv[4][16];
 #pragma unroll
@@ -805,28 +785,12 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_free0 + 8 * (n & 1));   // the buffer may take block n + 2
-        uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-        bool edge = false;
-        if constexpr (MASKED) {
-          edge = key0 < sees.x || key0 + kBK > sees.y;
-          if (edge) { seen[0] = interval_bits(sees.x, sees.y, key0); seen[1] = interval_bits(sees.x, sees.y, key0 + 32); }
-        }
 #pragma unroll
         for (int c4 = 0; c4 < 4; ++c4) {
-          float2 slope[CAP ? 8 : 1];   // 1 - tanh^2, which joins P: only their product counts here
-          if constexpr (CAP || BIAS)
-            shape.apply(sv[c4], static_cast<float>(qpos - key0 - 16 * c4), -1.0f, [&](int e, float2 t) {
-              if constexpr (CAP) slope[e >> 1] = __ffma2_rn(t, f2(-t.x, -t.y), f2(1.0f, 1.0f));
-            });
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
             const float2 tt = __ffma2_rn(f2(__uint_as_float(sv[c4][e]), __uint_as_float(sv[c4][e + 1])), sc2, nl2);
             float p0 = ex2(tt.x), p1 = ex2(tt.y);
-            if constexpr (CAP) { p0 *= slope[e >> 1].x; p1 *= slope[e >> 1].y; }
-            if (MASKED && edge) {
-              if ((seen[c4 >> 1] >> (16 * (c4 & 1) + e) & 1u) == 0) p0 = 0.0f;
-              if ((seen[c4 >> 1] >> (16 * (c4 & 1) + e + 1) & 1u) == 0) p1 = 0.0f;
-            }
             if (diag) {
               if (key0 + 16 * c4 + e > qpos) p0 = 0.0f;
               if (key0 + 16 * c4 + e + 1 > qpos) p1 = 0.0f;
@@ -872,16 +836,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(dq_free);   // the next item's products may overwrite dQ
-      bool bad = false;
-      if constexpr (MASKED) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int c4 = 0; c4 < 4; ++c4)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) sum = fmaf(__uint_as_float(qv[c4][e]), 0.0f, sum);
-        bad = qpos < p.S && !(sum == 0.0f);
-      }
-      if (qpos < p.S && !bad) {
+      if (qpos < p.S) {
         __nv_bfloat16* orow = p.dQ + (w.qrow0 + row) * kD;
 #pragma unroll
         for (int c4 = 0; c4 < 4; ++c4) {
@@ -893,11 +848,342 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
           *reinterpret_cast<uint4*>(orow + 16 * c4 + 8) = make_uint4(ow[4], ow[5], ow[6], ow[7]);
         }
       }
-      if constexpr (MASKED) {
-        for (uint32_t rows = __ballot_sync(0xffffffffu, bad); rows != 0; rows &= rows - 1)
-          mattn::dq_row<__nv_bfloat16>(c, w.b, w.hk, w.g, w.qb * kBQ + quad * 32 + __ffs(rows) - 1);
-      }
       n0 += static_cast<uint32_t>(w.nkb);
+    }
+  }
+
+  __syncwarp();
+  if (*abort_flag != 0) {
+    for (int k = 0; k < 200; ++k) __nanosleep(1000);
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(256u) : "memory");
+  }
+}
+
+// The same under a mask, with one product more.  delta = sum of P dP over a row is what the gradient of a softmax turns on, and rowsum(dO * O) of
+// the O that was stored in bfloat16 (from probabilities that were rounded for the tensor cores) is off by 2^-9 of |dO| |O|: where a row
+// puts its weight on few keys, P (dP - delta) is a small difference and that error exceeds all others (100 positions, scores of
+// standard deviation 6: gradients off by 0.0054 of their size instead of 0.0023).  So the sum is taken here from P and dP in float32, while the products
+// go on with d~ = rowsum(dO * O), and is put right at the end:
+//   dQ = sum P t (dP - d~) K  -  (delta - d~) sum P t K     (t = 1 - tanh^2 with a cap, else 1)
+// whose second sum needs no more than bfloat16 gives it, its factor being small.  The dK / dV kernel gets the exact delta.
+// Tensor memory (256 columns): S at 0, dP at 64, dQ at 128, the second sum at 192.  P t (bf16 pairs) is written over the first half of S, dS over
+// that of dP, each the A operand of its product; S of the next block is issued behind the product that has read P t, under
+// this block's second half.
+template <bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kThreads, 2)
+attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmdO,
+                      const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const BwdParams p,
+                      const __grid_constant__ mattn::Call c) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* gen_base = smem_raw + (base - smem_u32(smem_raw));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  const uint32_t q_full = base + kDqOffBar, q_free = q_full + 8, dq_full = q_free + 8, dq_free = dq_full + 8;
+  const uint32_t kv_full0 = dq_free + 8, kv_empty0 = kv_full0 + 8 * kDqStages;
+  const uint32_t s_full = kv_empty0 + 8 * kDqStages, p_ready = s_full + 8;
+  const uint32_t dp_full = p_ready + 8, ds_ready = dp_full + 8, tmem_slot = ds_ready + 8, abort_addr = tmem_slot + 4;
+  volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(gen_base + (tmem_slot - base));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_base + (abort_addr - base));
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_free, 1);
+    mbar_init(dq_full, 1);
+    mbar_init(dq_free, 4);
+    for (int s = 0; s < kDqStages; ++s) { mbar_init(kv_full0 + 8 * s, 1); mbar_init(kv_empty0 + 8 * s, 1); }
+    mbar_init(s_full, 1);
+    mbar_init(p_ready, 4);
+    mbar_init(dp_full, 1);
+    mbar_init(ds_ready, 4);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async_smem();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(256u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem_base = *tmem_slot_ptr;
+  grid_launch_dependents();
+  grid_dependency_wait();   // the set-up above ran under the tail of the kernel before
+  const uint32_t tS = tmem_base, tDP = tmem_base + 64, tDQ = tmem_base + 128, tPK = tmem_base + 192;
+  FwdParams tp;   // the item order of the forward
+  tp.S = p.S; tp.G = p.G; tp.NB = p.NB;
+  Walk<true> walk(tp, c);
+  FwdTile w;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int st = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      int it = -1;
+      while (ok && walk.get(w)) {
+        if (w.nkb == 0) continue;
+        ++it;
+        // the previous item's last S and dP products have read Q and dO
+        if (it > 0) ok = mbar_wait(q_free, (it - 1) & 1, abort_flag, 80, p.status);
+        if (!ok) break;
+        mbar_expect_tx(q_full, 2 * kQBytes);
+        tma_load_3d(base + kDqOffQ, &tmQ, q_full, 0, w.qb * kBQ, w.nb * p.G + w.g);
+        int dcol, dplane;
+        o_plane(p.G, p.HKV, p.o_tok, w.nb, w.g, dcol, dplane);
+        tma_load_3d(base + kDqOffDO, &tmdO, q_full, dcol, w.qb * kBQ, dplane);
+        for (int j = 0; j < w.nkb; ++j) {
+          ok = mbar_wait(kv_empty0 + 8 * st, ph ^ 1, abort_flag, 81, p.status);
+          if (!ok) break;
+          const uint32_t sb = base + kDqOffStage + st * kDqStageBytes;
+          mbar_expect_tx(kv_full0 + 8 * st, kDqStageBytes);
+          tma_load_3d(sb, &tmK, kv_full0 + 8 * st, 0, (w.kb0 + j) * kBK, w.nb);
+          tma_load_3d(sb + kKBytes, &tmV, kv_full0 + 8 * st, 0, (w.kb0 + j) * kBK, w.nb);
+          if (++st == kDqStages) { st = 0; ph ^= 1; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t idesc = make_idesc(kBK);
+      bool ok = true;
+      int it = -1;
+      uint32_t n = 0;             // running number of the block that gets its second sum and dQ
+      int sst = 0, dst = 0;       // ring stage of the next block to get its S product, and of block n
+      uint32_t sph = 0;
+      // S of the item's next block: the product that read the P t written over it was issued before this point
+      auto issue_s = [&]() -> bool {
+        if (!mbar_wait(kv_full0 + 8 * sst, sph, abort_flag, 83, p.status)) return false;
+        tcgen05_fence_after();
+        const uint32_t sb = base + kDqOffStage + sst * kDqStageBytes;
+#pragma unroll
+        for (int k4 = 0; k4 < kD / 16; ++k4)
+          umma_bf16(tS, desc_sw128(base + kDqOffQ + k4 * 32), desc_sw128(sb + k4 * 32), idesc, k4 != 0 ? 1u : 0u);
+        umma_commit(s_full);
+        if (++sst == kDqStages) { sst = 0; sph ^= 1; }
+        return true;
+      };
+      // dP of the block in ring stage st; its V tile arrived with the K tile that S has waited for
+      auto issue_dp = [&](int st) {
+        const uint32_t sb = base + kDqOffStage + st * kDqStageBytes;
+#pragma unroll
+        for (int k4 = 0; k4 < kD / 16; ++k4)
+          umma_bf16(tDP, desc_sw128(base + kDqOffDO + k4 * 32), desc_sw128(sb + kKBytes + k4 * 32), idesc, k4 != 0 ? 1u : 0u);
+        umma_commit(dp_full);
+      };
+      while (ok && walk.get(w)) {
+        if (w.nkb == 0) continue;
+        ++it;
+        ok = mbar_wait(q_full, it & 1, abort_flag, 84, p.status) && issue_s();
+        if (!ok) break;
+        issue_dp(dst);
+        if (w.nkb == 1) umma_commit(q_free);
+        for (int j = 0; ok && j < w.nkb; ++j, ++n) {
+          const uint32_t sb = base + kDqOffStage + dst * kDqStageBytes;
+          ok = mbar_wait(p_ready, n & 1, abort_flag, 82, p.status);
+          // the first products of an item overwrite both sums: the previous item's write-out must have read them
+          if (ok && j == 0 && it > 0) ok = mbar_wait(dq_free, (it - 1) & 1, abort_flag, 87, p.status);
+          if (!ok) break;
+          tcgen05_fence_after();
+          // second sum += (P t)_j K_j   (A = [128 x 64 keys] in tensor memory; B = the K tile as it lies: N-major)
+#pragma unroll
+          for (int k4 = 0; k4 < kBK / 16; ++k4)
+            umma_bf16_ts(tPK, tS + k4 * 8, desc_sw128_mn(sb + k4 * 2048, kKBytes, 1024), idesc | (1u << 16), (j | k4) != 0 ? 1u : 0u);
+          if (j + 1 < w.nkb) {
+            ok = issue_s();
+            if (!ok) break;
+          }
+          ok = mbar_wait(ds_ready, n & 1, abort_flag, 86, p.status);
+          if (!ok) break;
+          tcgen05_fence_after();
+          // dQ += dS_j K_j
+#pragma unroll
+          for (int k4 = 0; k4 < kBK / 16; ++k4)
+            umma_bf16_ts(tDQ, tDP + k4 * 8, desc_sw128_mn(sb + k4 * 2048, kKBytes, 1024), idesc | (1u << 16), (j | k4) != 0 ? 1u : 0u);
+          umma_commit(kv_empty0 + 8 * dst);
+          if (++dst == kDqStages) dst = 0;
+          if (j + 1 < w.nkb) {
+            issue_dp(dst);
+            if (j + 2 == w.nkb) umma_commit(q_free);   // Q and dO may be replaced by the next item's
+          } else {
+            umma_commit(dq_full);
+          }
+        }
+      }
+    }
+  } else {
+    const int quad = warp & 3;
+    const int row = quad * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
+    bool ok = true;
+    uint32_t n = 0;   // running number of a block
+    int it = -1;
+    Shape<CAP, BIAS> shape(c);
+    const float sc = CAP || BIAS ? 1.0f : p.sc;
+    const float2 sc2 = f2(sc, sc);
+    while (ok && walk.get(w)) {
+      const int qpos = w.qb * kBQ + row;
+      // d~ = sum_d dO * O of this row, straight from global memory (once per item)
+      float rough = 0.0f, lse2 = INFINITY;   // of a row behind position S, or one that sees nothing: P = dS = 0
+      int2 sees = make_int2(0, 0);
+      if (qpos < p.S) {
+        sees = c.mask.rows[static_cast<int64_t>(w.b) * p.S + qpos];
+        lse2 = p.lse[w.qrow0 + row] * kLog2e;
+        if (lse2 == -INFINITY) lse2 = INFINITY;
+        const int64_t ooff = o_offset(p.S, p.G, p.HKV, p.o_tok, w.nb, w.g, qpos);
+        const uint4* o4 = reinterpret_cast<const uint4*>(p.O + ooff);
+        const uint4* d4 = reinterpret_cast<const uint4*>(p.dO + ooff);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint4 a = o4[k], b = d4[k];
+          const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            rough = fmaf(__uint_as_float(aw[e] << 16), __uint_as_float(bw[e] << 16), rough);
+            rough = fmaf(__uint_as_float(aw[e] & 0xffff0000u), __uint_as_float(bw[e] & 0xffff0000u), rough);
+          }
+        }
+      }
+      const int64_t prow = (static_cast<int64_t>(w.nb) * p.G + w.g) * (q_blocks(p.S) * kBQ) + qpos;
+      p.nlse2[prow] = -lse2;
+      if constexpr (BIAS) shape.slope2 = c.slopes[w.hk * p.G + w.g] * kLog2e;
+      if (w.nkb == 0) {   // the tile sees nothing: no block was loaded for it
+        p.ndelta[prow] = 0.0f;
+        if (qpos < p.S) {
+          uint4* orow = reinterpret_cast<uint4*>(p.dQ + (w.qrow0 + row) * kD);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) orow[i] = make_uint4(0, 0, 0, 0);
+        }
+        continue;
+      }
+      ++it;
+      const float2 nl2 = f2(-lse2, -lse2), nd2 = f2(-rough, -rough);
+      float2 exact = f2(0.0f, 0.0f);   // delta
+      for (int j = 0; j < w.nkb; ++j, ++n) {
+        ok = __all_sync(0xffffffffu, mbar_wait(s_full, n & 1, abort_flag, 88, p.status));
+        if (!ok) break;
+        tcgen05_fence_after();
+        const int key0 = (w.kb0 + j) * kBK;
+        // the row's 64 scores, read once; P takes their place in the registers, P t in tensor memory
+        uint32_t sv[4][16];
+#pragma unroll
+        for (int c4 = 0; c4 < 4; ++c4) tmem_ld_x16(tS + lane_addr + 16 * c4, sv[c4]);
+        tmem_ld_wait();
+        const bool edge = key0 < sees.x || key0 + kBK > sees.y;
+        uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+        if (edge) { seen[0] = interval_bits(sees.x, sees.y, key0); seen[1] = interval_bits(sees.x, sees.y, key0 + 32); }
+        __half2 bend[CAP ? 32 : 1];   // t, to 2^-12 of itself
+#pragma unroll
+        for (int c2 = 0; c2 < 2; ++c2) {
+          uint32_t pw[16];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int c4 = 2 * c2 + h;
+            float2 slope[CAP ? 8 : 1];
+            if constexpr (CAP || BIAS)
+              shape.apply(sv[c4], static_cast<float>(qpos - key0 - 16 * c4), -1.0f, [&](int e, float2 t) {
+                if constexpr (CAP) {
+                  slope[e >> 1] = __ffma2_rn(t, f2(-t.x, -t.y), f2(1.0f, 1.0f));
+                  bend[8 * c4 + (e >> 1)] = __float22half2_rn(slope[e >> 1]);
+                }
+              });
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              const float2 tt = __ffma2_rn(f2(__uint_as_float(sv[c4][e]), __uint_as_float(sv[c4][e + 1])), sc2, nl2);
+              float2 pr = f2(ex2(tt.x), ex2(tt.y));
+              if (edge) {
+                if ((seen[c2] >> (16 * h + e) & 1u) == 0) pr.x = 0.0f;
+                if ((seen[c2] >> (16 * h + e + 1) & 1u) == 0) pr.y = 0.0f;
+              }
+              sv[c4][e] = __float_as_uint(pr.x);
+              sv[c4][e + 1] = __float_as_uint(pr.y);
+              if constexpr (CAP) pr = __fmul2_rn(pr, slope[e >> 1]);
+              pw[8 * h + (e >> 1)] = pack_bf16(pr.x, pr.y);
+            }
+          }
+          tmem_st_x16(tS + lane_addr + 16 * c2, pw);
+        }
+        tmem_st_wait();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready);
+        // dS = P t (dP - d~), bf16 pairs written over the half of dP already read
+        ok = __all_sync(0xffffffffu, mbar_wait(dp_full, n & 1, abort_flag, 89, p.status));
+        if (!ok) break;
+        tcgen05_fence_after();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t vd[2][16];
+          tmem_ld_x16(tDP + lane_addr + 32 * h, vd[0]);
+          tmem_ld_x16(tDP + lane_addr + 32 * h + 16, vd[1]);
+          tmem_ld_wait();
+          if (edge) {   // what lies at a masked position may be anything
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if ((seen[h] >> e & 1u) == 0) vd[e >> 4][e & 15] = 0;
+          }
+          uint32_t dw[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const uint32_t* pv = &sv[2 * h + (e >> 4)][e & 15];
+            const uint32_t* dv = &vd[e >> 4][e & 15];
+            const float2 pr = f2(__uint_as_float(pv[0]), __uint_as_float(pv[1])), d = f2(__uint_as_float(dv[0]), __uint_as_float(dv[1]));
+            exact = __ffma2_rn(pr, d, exact);
+            float2 r2 = __fmul2_rn(pr, __fadd2_rn(d, nd2));
+            if constexpr (CAP) r2 = __fmul2_rn(r2, __half22float2(bend[16 * h + (e >> 1)]));
+            dw[e >> 1] = pack_bf16(r2.x, r2.y);
+          }
+          tmem_st_x16(tDP + lane_addr + 16 * h, dw);
+        }
+        tmem_st_wait();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ds_ready);
+      }
+      if (!ok) break;
+      const float delta = exact.x + exact.y, put_right = rough - delta;
+      p.ndelta[prow] = -delta;
+      ok = __all_sync(0xffffffffu, mbar_wait(dq_full, it & 1, abort_flag, 90, p.status));
+      if (!ok) break;
+      tcgen05_fence_after();
+      uint32_t qv[4][16];
+      float sum = 0.0f;
+#pragma unroll
+      for (int c4 = 0; c4 < 4; ++c4) {
+        uint32_t kv[16];
+        tmem_ld_x16(tDQ + lane_addr + 16 * c4, qv[c4]);
+        tmem_ld_x16(tPK + lane_addr + 16 * c4, kv);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float x = fmaf(put_right, __uint_as_float(kv[e]), __uint_as_float(qv[c4][e])) * p.scale;
+          qv[c4][e] = __float_as_uint(x);
+          sum = fmaf(x, 0.0f, sum);
+        }
+      }
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(dq_free);   // the next item's products may overwrite both sums
+      const bool bad = qpos < p.S && !(sum == 0.0f);
+      if (qpos < p.S && !bad) {
+        __nv_bfloat16* orow = p.dQ + (w.qrow0 + row) * kD;
+#pragma unroll
+        for (int c4 = 0; c4 < 4; ++c4) {
+          uint32_t ow[8];
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) ow[e >> 1] = pack_bf16(__uint_as_float(qv[c4][e]), __uint_as_float(qv[c4][e + 1]));
+          *reinterpret_cast<uint4*>(orow + 16 * c4) = make_uint4(ow[0], ow[1], ow[2], ow[3]);
+          *reinterpret_cast<uint4*>(orow + 16 * c4 + 8) = make_uint4(ow[4], ow[5], ow[6], ow[7]);
+        }
+      }
+      for (uint32_t rows = __ballot_sync(0xffffffffu, bad); rows != 0; rows &= rows - 1)
+        mattn::dq_row<__nv_bfloat16>(c, w.b, w.hk, w.g, w.qb * kBQ + quad * 32 + __ffs(rows) - 1);
     }
   }
 
@@ -1410,7 +1696,7 @@ int attention_bwd(const void* q, const void* k, const void* v, const void* o, co
   int dev = 0;
   MCB_CHECK_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) return fail(MCB_ERR_SHAPE, "attention: device %d out of range", dev);
-  if (int rc = set_attrs_once(reinterpret_cast<const void*>(attn_dq_kernel<false, false, false>), kDqSmem, &attr_dq[dev])) return rc;
+  if (int rc = set_attrs_once(reinterpret_cast<const void*>(attn_dq_kernel), kDqSmem, &attr_dq[dev])) return rc;
   if (int rc = set_attrs_once(reinterpret_cast<const void*>(attn_dkv_kernel<false, false, false>), kKvSmem, &attr_kv[dev])) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const size_t rows = static_cast<size_t>(nb) * groups * q_blocks(static_cast<int>(seq)) * kBQ * 4;
@@ -1441,8 +1727,7 @@ int attention_bwd(const void* q, const void* k, const void* v, const void* o, co
   const int64_t n_tiles = q_blocks(static_cast<int>(seq)) * groups * nb;
   const int64_t slots = 2 * static_cast<int64_t>(ds->sm_count);
   const unsigned gq = static_cast<unsigned>(n_tiles < slots ? n_tiles : slots);
-  MCB_CHECK_CUDA(launch_kernel(attn_dq_kernel<false, false, false>, dim3(gq), dim3(kThreads), kDqSmem, st, chained_launch(), tmQ128, tmdO128, tmK64, tmV64, p,
-                               NoCall()));
+  MCB_CHECK_CUDA(launch_kernel(attn_dq_kernel, dim3(gq), dim3(kThreads), kDqSmem, st, chained_launch(), tmQ128, tmdO128, tmK64, tmV64, p));
   MCB_CHECK_LAUNCH("attn_dq_kernel");
   p.kv_parts = dkv_parts(nb, groups, seq, ds->sm_count);
   cudaLaunchConfig_t cfg = {};
@@ -1497,7 +1782,7 @@ using namespace attn;
 template <bool CAP, bool BIAS>
 struct Form {
   static constexpr auto fwd = attn_fwd_kernel<true, CAP, BIAS>;
-  static constexpr auto dq = attn_dq_kernel<true, CAP, BIAS>;
+  static constexpr auto dq = attn_dq_masked_kernel<CAP, BIAS>;
   static constexpr auto dkv = attn_dkv_kernel<true, CAP, BIAS>;
   static int prepare(int dev) {
     static bool done[3][64] = {};
@@ -1557,7 +1842,7 @@ int bwd_form(const Call& c, const DeviceState* ds, cudaStream_t st) {
   p.kv_parts = 1;
   MCB_CHECK_CUDA(launch_kernel(Form<CAP, BIAS>::dq, dim3(static_cast<unsigned>(n_tiles < slots ? n_tiles : slots)), dim3(attn::kThreads), kDqSmem, st,
                                chained_launch(), tmQ128, tmdO128, tmK64, tmV64, p, c));
-  MCB_CHECK_LAUNCH("attn_dq_kernel");
+  MCB_CHECK_LAUNCH("attn_dq_masked_kernel");
   p.kv_parts = dkv_parts(nb, c.G, c.S, ds->sm_count);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(nb * q_blocks(c.S) * p.kv_parts));

@@ -19,7 +19,7 @@ constexpr int kB = 64, kThreads = 256, kLdP = 68;
 
 __host__ __device__ constexpr int tile_floats(int d) { return kB * (d + 4); }
 inline size_t smem_fwd(int d) { return (3 * tile_floats(d) + kB * kLdP) * sizeof(float); }
-inline size_t smem_dq(int d) { return (4 * tile_floats(d) + kB * kLdP) * sizeof(float); }
+inline size_t smem_dq(int d) { return (4 * tile_floats(d) + 2 * kB * kLdP) * sizeof(float); }
 inline size_t smem_dkv(int d) { return (4 * tile_floats(d) + 2 * kB * kLdP) * sizeof(float); }
 
 // rows [first, first + 64) of a [.., S, D] plane as float32; `step` elements between rows; rows outside [0, S) are zeros
@@ -231,6 +231,8 @@ __global__ void __launch_bounds__(kThreads) masked_fwd_kernel(const __grid_const
     if (bad[r]) fwd_row<T>(c, w.b, hk, g, w.first + r);
 }
 
+// bfloat16: delta = sum of P dP is taken here and not from the rounded o, and what that changes put right at the end, by a second sum (see
+// attn_dq_masked_kernel).
 template <typename T, int DV>
 __global__ void __launch_bounds__(kThreads) masked_dq_kernel(const __grid_constant__ Call c) {
   extern __shared__ float4 smem4[];
@@ -242,6 +244,8 @@ __global__ void __launch_bounds__(kThreads) masked_dq_kernel(const __grid_consta
   float* sK = sO + tile_floats(c.D);
   float* sV = sK + tile_floats(c.D);
   float* sS = sV + tile_floats(c.D);
+  float* sP = sS + kB * kLdP;
+  constexpr bool kExact = sizeof(T) == 2;
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   grid_launch_dependents();
   grid_dependency_wait();
@@ -270,12 +274,13 @@ __global__ void __launch_bounds__(kThreads) masked_dq_kernel(const __grid_consta
       s_lse2[r] = lse2;
       s_delta[r] = d;
       const int64_t at = ((static_cast<int64_t>(w.b) * c.Hk + hk) * c.G + g) * pitch + s;
-      c.ndelta[at] = -d;
+      if (!kExact) c.ndelta[at] = -d;
       c.nlse2[at] = -lse2;
     }
   }
   const float slope2 = c.slopes ? c.slopes[w.head] * kLog2e : 0.0f;
-  float4 acc[4][DV] = {};
+  float4 acc[4][DV] = {}, acc2[kExact ? 4 : 1][DV] = {};
+  float exact[4] = {};
   for (int j0 = range.x; j0 < range.y; j0 += kB) {
     __syncthreads();
     load_tile(sK, static_cast<const T*>(c.k) + k_row(c, w.b, hk, 0) * c.D, c.D, j0, c.S, c.D);
@@ -292,17 +297,30 @@ __global__ void __launch_bounds__(kThreads) masked_dq_kernel(const __grid_consta
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int key = j0 + tx + 16 * j;
-        float p, ds = 0.0f;
-        if (key >= sees.x && key < sees.y) ds = pair_ds(c, s[i][j], dp[i][j], slope2, abs(w.first + r - key), lse2, delta, p);
+        float p, t, ds = 0.0f, pt = 0.0f;
+        if (key >= sees.x && key < sees.y) {
+          p = pair_p(c, s[i][j], slope2, abs(w.first + r - key), lse2, t);
+          pt = p * t;
+          ds = p * (dp[i][j] - delta) * t;
+          exact[i] = fmaf(p, dp[i][j], exact[i]);
+        }
         sS[r * kLdP + tx + 16 * j] = ds;
+        if (kExact) sP[r * kLdP + tx + 16 * j] = pt;
       }
     }
     __syncthreads();
     mul_nn<DV>(acc, sS, sK, c.D, ty, tx);
+    if constexpr (kExact) mul_nn<DV>(acc2, sP, sK, c.D, ty, tx);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int s = w.first + ty + 16 * i;
+    float put_right = 0.0f;
+    if constexpr (kExact) {
+      const float d = row_sum(exact[i]);
+      put_right = s_delta[ty + 16 * i] - d;
+      if (tx == 0) c.ndelta[((static_cast<int64_t>(w.b) * c.Hk + hk) * c.G + g) * pitch + s] = -d;
+    }
     if (s >= c.S) continue;
     T* out = static_cast<T*>(c.dq) + q_row(c, w.b, hk, g, s) * c.D;
 #pragma unroll
@@ -310,6 +328,10 @@ __global__ void __launch_bounds__(kThreads) masked_dq_kernel(const __grid_consta
       const int col = 4 * (tx + 16 * jj);
       if (col >= c.D) continue;
       float4 v = acc[i][jj];
+      if constexpr (kExact) {
+        const float4 k = acc2[i][jj];
+        v = make_float4(fmaf(put_right, k.x, v.x), fmaf(put_right, k.y, v.y), fmaf(put_right, k.z, v.z), fmaf(put_right, k.w, v.w));
+      }
       v = make_float4(v.x * c.scale, v.y * c.scale, v.z * c.scale, v.w * c.scale);
       if (!finite4(v)) bad[ty + 16 * i] = 1;
       store4(out + col, v);

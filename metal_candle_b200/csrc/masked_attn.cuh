@@ -108,49 +108,63 @@ __device__ __noinline__ void fwd_row(const Call& c, int b, int hk, int g, int s)
   if (c.lse != nullptr && (threadIdx.x & 31) == 0) c.lse[q_row(c, b, hk, g, s)] = none ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
-// P and dS of a pair, from the log-sum-exp (base 2) and delta of the query's row
-__device__ __forceinline__ float pair_ds(const Call& c, float dot, float dp, float slope2, int distance, float lse2, float delta, float& p) {
+// P of a pair from the log-sum-exp (base 2) of the query's row, and t = 1 - tanh^2
+__device__ __forceinline__ float pair_p(const Call& c, float dot, float slope2, int distance, float lse2, float& t) {
   float bent;
-  p = exp2f(score2(c, dot, slope2, distance, bent) - lse2);
-  return p * (dp - delta) * (1.0f - bent * bent);
+  const float p = exp2f(score2(c, dot, slope2, distance, bent) - lse2);
+  t = 1.0f - bent * bent;
+  return p;
+}
+// and dS, with delta of that row
+__device__ __forceinline__ float pair_ds(const Call& c, float dot, float dp, float slope2, int distance, float lse2, float delta, float& p) {
+  float t;
+  p = pair_p(c, dot, slope2, distance, lse2, t);
+  return p * (dp - delta) * t;
 }
 
 template <typename T>
 __device__ __noinline__ void dq_row(const Call& c, int b, int hk, int g, int s) {
   const int2 sees = c.mask.rows[static_cast<int64_t>(b) * c.S + s];
   const int64_t qr = q_row(c, b, hk, g, s), oa = o_at(c, b, hk, g, s);
-  const RowData<T> q(static_cast<const T*>(c.q) + qr * c.D, c.D), o(static_cast<const T*>(c.o_in) + oa, c.D);
-  const RowData<T> go(static_cast<const T*>(c.dout) + oa, c.D);
-  const float slope2 = c.slopes ? c.slopes[hk * c.G + g] * kLog2e : 0.0f, lse2 = c.lse[qr] * kLog2e, delta = go.dot(o);
+  const RowData<T> q(static_cast<const T*>(c.q) + qr * c.D, c.D), go(static_cast<const T*>(c.dout) + oa, c.D);
+  const float slope2 = c.slopes ? c.slopes[hk * c.G + g] * kLog2e : 0.0f, lse2 = c.lse[qr] * kLog2e;
   float acc[4] = {};
-  if (lse2 != -INFINITY)
-    for (int j = sees.x; j < sees.y; ++j) {
-      const int64_t kr = k_row(c, b, hk, j) * c.D;
-      const RowData<T> k(static_cast<const T*>(c.k) + kr, c.D), v(static_cast<const T*>(c.v) + kr, c.D);
-      float p;
-      const float ds = pair_ds(c, q.dot(k), go.dot(v), slope2, abs(s - j), lse2, delta, p);
+  if (lse2 != -INFINITY) {
+    float delta = 0.0f;
+    for (int turn = 0; turn < 2; ++turn)   // delta = sum of P dP first
+      for (int j = sees.x; j < sees.y; ++j) {
+        const int64_t kr = k_row(c, b, hk, j) * c.D;
+        const RowData<T> k(static_cast<const T*>(c.k) + kr, c.D), v(static_cast<const T*>(c.v) + kr, c.D);
+        float p;
+        const float dp = go.dot(v), ds = pair_ds(c, q.dot(k), dp, slope2, abs(s - j), lse2, delta, p);
+        if (turn == 0) {
+          acc[0] = fmaf(p, dp, acc[0]);
+        } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = fmaf(ds, k.v[e], acc[e]);
-    }
+          for (int e = 0; e < 4; ++e) acc[e] = fmaf(ds, k.v[e], acc[e]);
+        }
+        if (turn == 0 && j == sees.y - 1) { delta = acc[0]; acc[0] = 0.0f; }
+      }
+  }
   row_store(static_cast<T*>(c.dq) + qr * c.D, acc, c.scale, c.D);
 }
 
+// (delta and the log-sum-exp of the queries as the dq kernel has left them)
 template <typename T>
 __device__ __noinline__ void dkv_row(const Call& c, int b, int hk, int s) {
   const int2 seen = c.mask.keys[static_cast<int64_t>(b) * c.S + s];
-  const int64_t kr = k_row(c, b, hk, s) * c.D;
+  const int64_t kr = k_row(c, b, hk, s) * c.D, pitch = amask::tiles_of(c.S) * amask::kTile;
   const RowData<T> k(static_cast<const T*>(c.k) + kr, c.D), v(static_cast<const T*>(c.v) + kr, c.D);
   float gk[4] = {}, gv[4] = {};
   for (int g = 0; g < c.G; ++g) {
     const float slope2 = c.slopes ? c.slopes[hk * c.G + g] * kLog2e : 0.0f;
     for (int i = seen.x; i < seen.y; ++i) {
-      const int64_t qr = q_row(c, b, hk, g, i), oa = o_at(c, b, hk, g, i);
-      const float lse2 = c.lse[qr] * kLog2e;
-      if (lse2 == -INFINITY) continue;
-      const RowData<T> q(static_cast<const T*>(c.q) + qr * c.D, c.D), o(static_cast<const T*>(c.o_in) + oa, c.D);
-      const RowData<T> go(static_cast<const T*>(c.dout) + oa, c.D);
+      const int64_t at = ((static_cast<int64_t>(b) * c.Hk + hk) * c.G + g) * pitch + i;
+      const float lse2 = -c.nlse2[at];
+      if (lse2 == INFINITY) continue;
+      const RowData<T> q(static_cast<const T*>(c.q) + q_row(c, b, hk, g, i) * c.D, c.D), go(static_cast<const T*>(c.dout) + o_at(c, b, hk, g, i), c.D);
       float p;
-      const float ds = pair_ds(c, q.dot(k), go.dot(v), slope2, abs(s - i), lse2, go.dot(o), p);
+      const float ds = pair_ds(c, q.dot(k), go.dot(v), slope2, abs(s - i), lse2, -c.ndelta[at], p);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         gk[e] = fmaf(ds, q.v[e], gk[e]);
