@@ -9,7 +9,11 @@
 // four extra put the sixteen rows that a half warp reads on different banks for every D that is a multiple of 8.  One pass over the
 // keys that some row of the tile sees, with the running maximum and sum; nothing of size seq x seq is stored and no sum uses
 // atomics.  The backward pass is a kernel by query tiles (dq, and delta and lse for the other) and one by key tiles (dk, dv).
+#include <cooperative_groups.h>
+
 #include "masked_attn.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace mcb {
 namespace mattn {
@@ -42,41 +46,61 @@ __device__ __forceinline__ void load_tile(float* dst, const T* plane, int64_t st
   }
 }
 
-// acc[i][j] = sum_k a[ty + 16 i][k] b[tx + 16 j][k]
-__device__ __forceinline__ void mul_nt(float (&acc)[4][4], const float* a, const float* b, int D, int ty, int tx) {
+// acc[i][j] = sum_k a[ty + 16 i][k] b[tx + 16 j][k] for i < ni, j < nj (rows and columns that exist; others stay 0).  Even and odd k are summed
+// apart, two multiply-adds to an instruction.
+__device__ __forceinline__ void mul_nt(float (&acc)[4][4], const float* a, const float* b, int D, int ty, int tx, int ni, int nj) {
+  float2 sum[4][4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+    for (int j = 0; j < 4; ++j) sum[i][j] = make_float2(0.0f, 0.0f);
   const int ld = D + 4;
-  for (int k = 0; k < D; k += 4) {
-    float4 x[4], y[4];
+  if (ni == 4 && nj == 4) {
+    for (int k = 0; k < D; k += 4) {
+      float4 x[4], y[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = *reinterpret_cast<const float4*>(a + (ty + 16 * i) * ld + k);
-      y[i] = *reinterpret_cast<const float4*>(b + (tx + 16 * i) * ld + k);
+      for (int i = 0; i < 4; ++i) {
+        x[i] = *reinterpret_cast<const float4*>(a + (ty + 16 * i) * ld + k);
+        y[i] = *reinterpret_cast<const float4*>(b + (tx + 16 * i) * ld + k);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          sum[i][j] = __ffma2_rn(make_float2(x[i].x, x[i].y), make_float2(y[j].x, y[j].y), sum[i][j]);
+          sum[i][j] = __ffma2_rn(make_float2(x[i].z, x[i].w), make_float2(y[j].z, y[j].w), sum[i][j]);
+        }
     }
+  } else {
+    for (int k = 0; k < D; k += 4)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i) {
+        if (i >= ni) break;
+        const float4 x = *reinterpret_cast<const float4*>(a + (ty + 16 * i) * ld + k);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        acc[i][j] = fmaf(x[i].x, y[j].x, acc[i][j]);
-        acc[i][j] = fmaf(x[i].y, y[j].y, acc[i][j]);
-        acc[i][j] = fmaf(x[i].z, y[j].z, acc[i][j]);
-        acc[i][j] = fmaf(x[i].w, y[j].w, acc[i][j]);
+        for (int j = 0; j < 4; ++j) {
+          if (j >= nj) break;
+          const float4 y = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * ld + k);
+          sum[i][j] = __ffma2_rn(make_float2(x.x, x.y), make_float2(y.x, y.y), sum[i][j]);
+          sum[i][j] = __ffma2_rn(make_float2(x.z, x.w), make_float2(y.z, y.w), sum[i][j]);
+        }
       }
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = sum[i][j].x + sum[i][j].y;
 }
 
-// acc[i][jj] += sum_k p[ty + 16 i][k] v[k][4 (tx + 16 jj) ..]
+// acc[i][jj] += sum_k p[ty + 16 i][k] v[k][4 (tx + 16 jj) ..] for k < K (a multiple of 4 up to 64), i < ni
 template <int DV>
-__device__ __forceinline__ void mul_nn(float4 (&acc)[4][DV], const float* p, const float* v, int D, int ty, int tx) {
+__device__ __forceinline__ void mul_nn(float4 (&acc)[4][DV], const float* p, const float* v, int D, int ty, int tx, int K, int ni) {
   const int ld = D + 4;
 #pragma unroll 4
-  for (int k = 0; k < kB; k += 4) {
+  for (int k = 0; k < K; k += 4) {
     float4 x[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(p + (ty + 16 * i) * kLdP + k);
+    for (int i = 0; i < 4; ++i) x[i] = i < ni ? *reinterpret_cast<const float4*>(p + (ty + 16 * i) * kLdP + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int jj = 0; jj < DV; ++jj) {
       const int c = 4 * (tx + 16 * jj);
@@ -86,16 +110,19 @@ __device__ __forceinline__ void mul_nn(float4 (&acc)[4][DV], const float* p, con
         const float4 y = *reinterpret_cast<const float4*>(v + (k + kk) * ld + c);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
+          if (i >= ni) break;
           const float f = kk == 0 ? x[i].x : kk == 1 ? x[i].y : kk == 2 ? x[i].z : x[i].w;
-          acc[i][jj].x = fmaf(f, y.x, acc[i][jj].x);
-          acc[i][jj].y = fmaf(f, y.y, acc[i][jj].y);
-          acc[i][jj].z = fmaf(f, y.z, acc[i][jj].z);
-          acc[i][jj].w = fmaf(f, y.w, acc[i][jj].w);
+          const float2 a = __ffma2_rn(make_float2(f, f), make_float2(y.x, y.y), make_float2(acc[i][jj].x, acc[i][jj].y));
+          const float2 b = __ffma2_rn(make_float2(f, f), make_float2(y.z, y.w), make_float2(acc[i][jj].z, acc[i][jj].w));
+          acc[i][jj] = make_float4(a.x, a.y, b.x, b.y);
         }
       }
     }
   }
 }
+// sixteens of rows that a tile from position `first` has, and its positions rounded up to fours
+__device__ __forceinline__ int sixteens(int first, int end) { return end - first >= kB ? 4 : (end - first + 15) / 16; }
+__device__ __forceinline__ int fours(int first, int end) { return end - first >= kB ? kB : (end - first + 3) & ~3; }
 
 template <typename T>
 __device__ __forceinline__ void store4(T* p, float4 v) {
@@ -124,11 +151,11 @@ __device__ __forceinline__ float row_sum(float v) {
 struct Item {
   int b, first, head;
 };
-__device__ __forceinline__ Item item_of(const int4* work, int heads) {
-  const int half = blockIdx.x / heads;
+__device__ __forceinline__ Item item_of(const int4* work, int heads, int block) {
+  const int half = block / heads;
   const int4 t = work[half >> 1];
   Item w;
-  w.head = blockIdx.x % heads;
+  w.head = block % heads;
   w.b = t.x;
   w.first = t.y * amask::kTile + (half & 1) * kB;
   return w;
@@ -159,13 +186,14 @@ __global__ void __launch_bounds__(kThreads) masked_fwd_kernel(const __grid_const
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   grid_launch_dependents();
   grid_dependency_wait();
-  const Item w = item_of(c.mask.qwork, c.Hk * c.G);
+  const Item w = item_of(c.mask.qwork, c.Hk * c.G, blockIdx.x);
   if (w.first >= c.S) return;
   const int hk = w.head / c.G, g = w.head % c.G;
   if (threadIdx.x < kB) bad[threadIdx.x] = 0;
   const int2 range = load_ranges(rows, ends, c.mask.rows, c, w);
   load_tile(sQ, static_cast<const T*>(c.q) + q_row(c, w.b, hk, g, 0) * c.D, c.D, w.first, c.S, c.D);
   const float slope2 = c.slopes ? c.slopes[w.head] * kLog2e : 0.0f;
+  const int ni = sixteens(w.first, c.S);
   float m[4], l[4];
   float4 acc[4][DV] = {};
 #pragma unroll
@@ -176,9 +204,10 @@ __global__ void __launch_bounds__(kThreads) masked_fwd_kernel(const __grid_const
     load_tile(sV, static_cast<const T*>(c.v) + k_row(c, w.b, hk, 0) * c.D, c.D, j0, c.S, c.D);
     __syncthreads();
     float s[4][4];
-    mul_nt(s, sQ, sK, c.D, ty, tx);
+    mul_nt(s, sQ, sK, c.D, ty, tx, ni, sixteens(j0, range.y));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      if (i >= ni) break;
       const int2 sees = rows[ty + 16 * i];
       const int qpos = w.first + ty + 16 * i;
       float top = kNoScore;
@@ -206,7 +235,7 @@ __global__ void __launch_bounds__(kThreads) masked_fwd_kernel(const __grid_const
       }
     }
     __syncthreads();
-    mul_nn<DV>(acc, sP, sV, c.D, ty, tx);
+    mul_nn<DV>(acc, sP, sV, c.D, ty, tx, fours(j0, range.y), ni);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -249,7 +278,7 @@ __global__ void __launch_bounds__(kThreads) masked_dq_kernel(const __grid_consta
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   grid_launch_dependents();
   grid_dependency_wait();
-  const Item w = item_of(c.mask.qwork, c.Hk * c.G);
+  const Item w = item_of(c.mask.qwork, c.Hk * c.G, blockIdx.x);
   if (w.first >= c.S) return;
   const int hk = w.head / c.G, g = w.head % c.G;
   if (threadIdx.x < kB) bad[threadIdx.x] = 0;
@@ -279,6 +308,7 @@ __global__ void __launch_bounds__(kThreads) masked_dq_kernel(const __grid_consta
     }
   }
   const float slope2 = c.slopes ? c.slopes[w.head] * kLog2e : 0.0f;
+  const int ni = sixteens(w.first, c.S);
   float4 acc[4][DV] = {}, acc2[kExact ? 4 : 1][DV] = {};
   float exact[4] = {};
   for (int j0 = range.x; j0 < range.y; j0 += kB) {
@@ -287,10 +317,12 @@ __global__ void __launch_bounds__(kThreads) masked_dq_kernel(const __grid_consta
     load_tile(sV, static_cast<const T*>(c.v) + k_row(c, w.b, hk, 0) * c.D, c.D, j0, c.S, c.D);
     __syncthreads();
     float s[4][4], dp[4][4];
-    mul_nt(s, sQ, sK, c.D, ty, tx);
-    mul_nt(dp, sO, sV, c.D, ty, tx);
+    const int nj = sixteens(j0, range.y);
+    mul_nt(s, sQ, sK, c.D, ty, tx, ni, nj);
+    mul_nt(dp, sO, sV, c.D, ty, tx, ni, nj);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      if (i >= ni) break;
       const int r = ty + 16 * i;
       const int2 sees = rows[r];
       const float lse2 = s_lse2[r], delta = s_delta[r];
@@ -309,8 +341,8 @@ __global__ void __launch_bounds__(kThreads) masked_dq_kernel(const __grid_consta
       }
     }
     __syncthreads();
-    mul_nn<DV>(acc, sS, sK, c.D, ty, tx);
-    if constexpr (kExact) mul_nn<DV>(acc2, sP, sK, c.D, ty, tx);
+    mul_nn<DV>(acc, sS, sK, c.D, ty, tx, fours(j0, range.y), ni);
+    if constexpr (kExact) mul_nn<DV>(acc2, sP, sK, c.D, ty, tx, fours(j0, range.y), ni);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -356,19 +388,25 @@ __global__ void __launch_bounds__(kThreads) masked_dkv_kernel(const __grid_const
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   grid_launch_dependents();
   grid_dependency_wait();
-  const Item w = item_of(c.mask.kwork, c.Hk);
-  if (w.first >= c.S) return;
-  const int hk = w.head;
+  // the blocks of a cluster share a tile's steps (a head and 64 queries each), consecutive ones each
+  cg::cluster_group cl = cg::this_cluster();
+  const int parts = static_cast<int>(cl.num_blocks()), part = static_cast<int>(cl.block_rank());
+  const Item w = item_of(c.mask.kwork, c.Hk, blockIdx.x / parts);
+  if (w.first >= c.S) return;   // (all of the cluster)
+  const int hk = w.head, ni = sixteens(w.first, c.S);
   if (threadIdx.x < kB) bad[threadIdx.x] = 0;
   const int2 range = load_ranges(rows, ends, c.mask.keys, c, w);
   load_tile(sK, static_cast<const T*>(c.k) + k_row(c, w.b, hk, 0) * c.D, c.D, w.first, c.S, c.D);
   load_tile(sV, static_cast<const T*>(c.v) + k_row(c, w.b, hk, 0) * c.D, c.D, w.first, c.S, c.D);
   const int64_t pitch = amask::tiles_of(c.S) * amask::kTile, ostep = c.o_tok ? static_cast<int64_t>(c.Hk) * c.G * c.D : c.D;
   float4 gk[4][DV] = {}, gv[4][DV] = {};
-  for (int g = 0; g < c.G; ++g) {
+  const int per_head = range.y > range.x ? (range.y - range.x + kB - 1) / kB : 0;
+  const int64_t steps = static_cast<int64_t>(c.G) * per_head;
+  for (int64_t step = steps * part / parts; step < steps * (part + 1) / parts; ++step) {
+    const int g = static_cast<int>(step / per_head), i0 = range.x + static_cast<int>(step % per_head) * kB;
     const float slope2 = c.slopes ? c.slopes[hk * c.G + g] * kLog2e : 0.0f;
     const int64_t srow = ((static_cast<int64_t>(w.b) * c.Hk + hk) * c.G + g) * pitch;
-    for (int i0 = range.x; i0 < range.y; i0 += kB) {
+    {
       __syncthreads();
       load_tile(sQ, static_cast<const T*>(c.q) + q_row(c, w.b, hk, g, 0) * c.D, c.D, i0, c.S, c.D);
       load_tile(sO, static_cast<const T*>(c.dout) + o_at(c, w.b, hk, g, 0), ostep, i0, c.S, c.D);
@@ -380,10 +418,12 @@ __global__ void __launch_bounds__(kThreads) masked_dkv_kernel(const __grid_const
         lse2[j] = qpos < c.S ? -c.nlse2[srow + qpos] : INFINITY;
         delta[j] = qpos < c.S ? -c.ndelta[srow + qpos] : 0.0f;
       }
-      mul_nt(s, sK, sQ, c.D, ty, tx);
-      mul_nt(dp, sV, sO, c.D, ty, tx);
+      const int nj = sixteens(i0, range.y);
+      mul_nt(s, sK, sQ, c.D, ty, tx, ni, nj);
+      mul_nt(dp, sV, sO, c.D, ty, tx, ni, nj);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
+        if (i >= ni) break;
         const int r = ty + 16 * i;
         const int2 seen = rows[r];
 #pragma unroll
@@ -397,9 +437,39 @@ __global__ void __launch_bounds__(kThreads) masked_dkv_kernel(const __grid_const
         }
       }
       __syncthreads();
-      mul_nn<DV>(gv, sP, sO, c.D, ty, tx);
-      mul_nn<DV>(gk, sS, sQ, c.D, ty, tx);
+      mul_nn<DV>(gv, sP, sO, c.D, ty, tx, fours(i0, range.y), ni);
+      mul_nn<DV>(gk, sS, sQ, c.D, ty, tx, fours(i0, range.y), ni);
     }
+  }
+  if (parts > 1) {
+    // every block's sums into its own shared memory (over Q and d O), then the first adds the others' to its own, in order
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int jj = 0; jj < DV; ++jj) {
+        const int col = 4 * (tx + 16 * jj);
+        if (col >= c.D) continue;
+        *reinterpret_cast<float4*>(sQ + (ty + 16 * i) * (c.D + 4) + col) = gk[i][jj];
+        *reinterpret_cast<float4*>(sO + (ty + 16 * i) * (c.D + 4) + col) = gv[i][jj];
+      }
+    cl.sync();
+    if (part == 0)
+      for (int q = 1; q < parts; ++q) {
+        const float *pk = cl.map_shared_rank(sQ, q), *pv = cl.map_shared_rank(sO, q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int jj = 0; jj < DV; ++jj) {
+            const int col = 4 * (tx + 16 * jj);
+            if (col >= c.D || i >= ni) continue;
+            const float4 x = *reinterpret_cast<const float4*>(pk + (ty + 16 * i) * (c.D + 4) + col), y = *reinterpret_cast<const float4*>(pv + (ty + 16 * i) * (c.D + 4) + col);
+            gk[i][jj] = make_float4(gk[i][jj].x + x.x, gk[i][jj].y + x.y, gk[i][jj].z + x.z, gk[i][jj].w + x.w);
+            gv[i][jj] = make_float4(gv[i][jj].x + y.x, gv[i][jj].y + y.y, gv[i][jj].z + y.z, gv[i][jj].w + y.w);
+          }
+      }
+    cl.sync();   // no block leaves while the first reads its sums
+    if (part != 0) return;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -422,23 +492,37 @@ __global__ void __launch_bounds__(kThreads) masked_dkv_kernel(const __grid_const
     if (bad[r]) dkv_row<T>(c, w.b, hk, w.first + r);
 }
 
-int launch_one(void (*kernel)(Call), const char* name, int64_t blocks, size_t smem, const Call& c, cudaStream_t st) {
+int launch_one(void (*kernel)(Call), const char* name, int64_t blocks, int cluster, size_t smem, const Call& c, cudaStream_t st) {
   if (blocks > 0x7fffffffll) return fail(MCB_ERR_SHAPE, "masked attention: %lld blocks", (long long)blocks);
   MCB_CHECK_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  MCB_CHECK_CUDA(launch_kernel(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), smem, st, chained_launch(), c));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = chained_launch() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster); attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr; cfg.numAttrs = cluster > 1 ? 2 : 1;
+  MCB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, c));
   MCB_CHECK_LAUNCH(name);
   return MCB_OK;
 }
 template <typename T>
 int launch_fwd(const Call& c, cudaStream_t st) {
   const int64_t halves = 2 * amask::tiles_of(c.S) * c.B;
-  return launch_one(c.D <= 64 ? masked_fwd_kernel<T, 1> : masked_fwd_kernel<T, 2>, "masked_fwd_kernel", halves * c.Hk * c.G, smem_fwd(c.D), c, st);
+  return launch_one(c.D <= 64 ? masked_fwd_kernel<T, 1> : masked_fwd_kernel<T, 2>, "masked_fwd_kernel", halves * c.Hk * c.G, 1, smem_fwd(c.D), c, st);
 }
 template <typename T>
-int launch_bwd(const Call& c, cudaStream_t st) {
+int launch_bwd(const Call& c, int sms, cudaStream_t st) {
   const int64_t halves = 2 * amask::tiles_of(c.S) * c.B;
-  if (int rc = launch_one(c.D <= 64 ? masked_dq_kernel<T, 1> : masked_dq_kernel<T, 2>, "masked_dq_kernel", halves * c.Hk * c.G, smem_dq(c.D), c, st)) return rc;
-  return launch_one(c.D <= 64 ? masked_dkv_kernel<T, 1> : masked_dkv_kernel<T, 2>, "masked_dkv_kernel", halves * c.Hk, smem_dkv(c.D), c, st);
+  if (int rc = launch_one(c.D <= 64 ? masked_dq_kernel<T, 1> : masked_dq_kernel<T, 2>, "masked_dq_kernel", halves * c.Hk * c.G, 1, smem_dq(c.D), c, st)) return rc;
+  // few key tiles: clusters share one's steps, as long as the device has room and a part has a step (2 x 3 heads of 19 positions: 45 us alone, SHARED by 4)
+  const int64_t tiles = halves * c.Hk, steps = static_cast<int64_t>(c.G) * ((c.S + kB - 1) / kB);
+  int parts = 1;
+  while (parts < 8 && tiles * parts * 2 <= sms && parts * 2 <= steps) parts *= 2;
+  return launch_one(c.D <= 64 ? masked_dkv_kernel<T, 1> : masked_dkv_kernel<T, 2>, "masked_dkv_kernel", tiles * parts, parts, smem_dkv(c.D), c, st);
 }
 
 inline size_t up1k(size_t v) { return (v + 1023) & ~static_cast<size_t>(1023); }
@@ -522,5 +606,5 @@ extern "C" int mcb_attention_masked_bwd(const mcb_masked_attention* a, const voi
   c.status = ds->status_word;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (mattn::tensor_cores(a)) return mattn::launch_bwd_umma(c, ds, st);
-  return a->dtype == MCB_F32 ? mattn::launch_bwd<float>(c, st) : mattn::launch_bwd<__nv_bfloat16>(c, st);
+  return a->dtype == MCB_F32 ? mattn::launch_bwd<float>(c, ds->sm_count, st) : mattn::launch_bwd<__nv_bfloat16>(c, ds->sm_count, st);
 }
