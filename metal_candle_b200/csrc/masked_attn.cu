@@ -4,8 +4,8 @@
 // The entry points, and kernels on CUDA cores for float32 (the validation path) and for bfloat16 heads of other sizes than 64,
 // which flash_attn.cu takes to the tensor cores.
 //
-// CUDA-core kernels: 64 x 64 tiles, 256 threads, a thread has rows ty + 16 i and columns tx + 16 j of a product (four of each, so that
-// one 16-byte shared load of a row serves four multiply-adds in each of four columns).  Tiles are float32 rows of D + 4 elements: the
+// CUDA-core kernels: tiles of 32 x 64, 256 threads, a thread has rows ty + 16 i and columns tx + 16 j of a product (two by four: the longest
+// block's chain of tiles is what a launch takes at the sizes this is for, 12 heads x 1200 positions, forward: HERE us, 64 x 64 tiles by 256 threads 282).  Tiles are float32 rows of D + 4 elements: the
 // four extra put the sixteen rows that a half warp reads on different banks for every D that is a multiple of 8.  One pass over the
 // keys that some row of the tile sees, with the running maximum and sum; nothing of size seq x seq is stored and no sum uses
 // atomics.  The backward pass is a kernel by query tiles (dq, and delta and lse for the other) and one by key tiles (dk, dv).
@@ -19,19 +19,22 @@ namespace mcb {
 namespace mattn {
 namespace {
 
-constexpr int kB = 64, kThreads = 256, kLdP = 68;
+constexpr int kRows = 32, kB = 64, kThreads = 256, kLdP = 68;   // rows of a block's tile, and of the tiles it walks over
+constexpr int kR = 2;   // rows of a thread: ty, ty + 16
 
 __host__ __device__ constexpr int tile_floats(int d) { return kB * (d + 4); }
-inline size_t smem_fwd(int d) { return (3 * tile_floats(d) + kB * kLdP) * sizeof(float); }
-inline size_t smem_dq(int d) { return (4 * tile_floats(d) + 2 * kB * kLdP) * sizeof(float); }
-inline size_t smem_dkv(int d) { return (4 * tile_floats(d) + 2 * kB * kLdP) * sizeof(float); }
+__host__ __device__ constexpr int rows_floats(int d) { return kRows * (d + 4); }
+inline size_t smem_fwd(int d) { return (rows_floats(d) + 2 * tile_floats(d) + kRows * kLdP) * sizeof(float); }
+inline size_t smem_bwd(int d) { return (2 * rows_floats(d) + 2 * tile_floats(d) + 2 * kRows * kLdP) * sizeof(float); }
 
-// rows [first, first + 64) of a [.., S, D] plane as float32; `step` elements between rows; rows outside [0, S) are zeros
-template <typename T>
+// rows [first, first + COUNT) of a [.., S, D] plane as float32; `step` elements between rows; rows outside [0, S) are zeros
+template <int COUNT, typename T>
 __device__ __forceinline__ void load_tile(float* dst, const T* plane, int64_t step, int first, int S, int D) {
-  const int per = D / 4;
-  for (int i = threadIdx.x; i < kB * per; i += kThreads) {
-    const int r = i / per, c = i % per * 4;
+  // half a warp to a row of up to 64 elements, a warp to a longer one
+  const int wide = D > 64 ? 32 : 16, c = threadIdx.x % wide * 4;
+  if (c >= D) return;
+#pragma unroll 4
+  for (int r = threadIdx.x / wide; r < COUNT; r += kThreads / wide) {
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (first + r < S) {
       const T* s = plane + (first + r) * step + c;
@@ -48,79 +51,84 @@ __device__ __forceinline__ void load_tile(float* dst, const T* plane, int64_t st
 
 // acc[i][j] = sum_k a[ty + 16 i][k] b[tx + 16 j][k] for i < ni, j < nj (rows and columns that exist; others stay 0).  Even and odd k are summed
 // apart, two multiply-adds to an instruction.
-__device__ __forceinline__ void mul_nt(float (&acc)[4][4], const float* a, const float* b, int D, int ty, int tx, int ni, int nj) {
-  float2 sum[4][4];
+__device__ __forceinline__ void mul_nt(float (&acc)[kR][4], const float* a, const float* b, int D, int ty, int tx, int ni, int nj) {
+  float2 sum[kR][4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < kR; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) sum[i][j] = make_float2(0.0f, 0.0f);
   const int ld = D + 4;
-  if (ni == 4 && nj == 4) {
+  a += ty * ld;
+  b += tx * ld;
+  if (ni == kR && nj == 4) {
+#pragma unroll 2
     for (int k = 0; k < D; k += 4) {
-      float4 x[4], y[4];
+      float4 x[kR], y[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = *reinterpret_cast<const float4*>(a + (ty + 16 * i) * ld + k);
-        y[i] = *reinterpret_cast<const float4*>(b + (tx + 16 * i) * ld + k);
-      }
+      for (int i = 0; i < kR; ++i) x[i] = *reinterpret_cast<const float4*>(a + 16 * i * ld + k);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4*>(b + 16 * j * ld + k);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          sum[i][j] = __ffma2_rn(make_float2(x[i].x, x[i].y), make_float2(y[j].x, y[j].y), sum[i][j]);
-          sum[i][j] = __ffma2_rn(make_float2(x[i].z, x[i].w), make_float2(y[j].z, y[j].w), sum[i][j]);
-        }
+      for (int i = 0; i < kR; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[i][j] = __ffma2_rn(make_float2(x[i].x, x[i].y), make_float2(y[j].x, y[j].y), sum[i][j]);
+#pragma unroll
+      for (int i = 0; i < kR; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[i][j] = __ffma2_rn(make_float2(x[i].z, x[i].w), make_float2(y[j].z, y[j].w), sum[i][j]);
     }
   } else {
     for (int k = 0; k < D; k += 4)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kR; ++i) {
         if (i >= ni) break;
-        const float4 x = *reinterpret_cast<const float4*>(a + (ty + 16 * i) * ld + k);
+        const float4 x = *reinterpret_cast<const float4*>(a + 16 * i * ld + k);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (j >= nj) break;
-          const float4 y = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * ld + k);
+          const float4 y = *reinterpret_cast<const float4*>(b + 16 * j * ld + k);
           sum[i][j] = __ffma2_rn(make_float2(x.x, x.y), make_float2(y.x, y.y), sum[i][j]);
           sum[i][j] = __ffma2_rn(make_float2(x.z, x.w), make_float2(y.z, y.w), sum[i][j]);
         }
       }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < kR; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = sum[i][j].x + sum[i][j].y;
 }
 
 // acc[i][jj] += sum_k p[ty + 16 i][k] v[k][4 (tx + 16 jj) ..] for k < K (a multiple of 4 up to 64), i < ni
 template <int DV>
-__device__ __forceinline__ void mul_nn(float4 (&acc)[4][DV], const float* p, const float* v, int D, int ty, int tx, int K, int ni) {
+__device__ __forceinline__ void mul_nn(float4 (&acc)[kR][DV], const float* p, const float* v, int D, int ty, int tx, int K, int ni) {
   const int ld = D + 4;
+  p += ty * kLdP;
+  v += 4 * tx;
 #pragma unroll 4
   for (int k = 0; k < K; k += 4) {
-    float4 x[4];
+    float4 x[kR];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = i < ni ? *reinterpret_cast<const float4*>(p + (ty + 16 * i) * kLdP + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i = 0; i < kR; ++i) x[i] = i < ni ? *reinterpret_cast<const float4*>(p + 16 * i * kLdP + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int jj = 0; jj < DV; ++jj) {
-      const int c = 4 * (tx + 16 * jj);
-      if (c >= D) continue;
+      if (4 * (tx + 16 * jj) >= D) continue;
+      float4 y[4];
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        const float4 y = *reinterpret_cast<const float4*>(v + (k + kk) * ld + c);
+      for (int kk = 0; kk < 4; ++kk) y[kk] = *reinterpret_cast<const float4*>(v + (k + kk) * ld + 64 * jj);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (i >= ni) break;
+      for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int i = 0; i < kR; ++i) {
           const float f = kk == 0 ? x[i].x : kk == 1 ? x[i].y : kk == 2 ? x[i].z : x[i].w;
-          const float2 a = __ffma2_rn(make_float2(f, f), make_float2(y.x, y.y), make_float2(acc[i][jj].x, acc[i][jj].y));
-          const float2 b = __ffma2_rn(make_float2(f, f), make_float2(y.z, y.w), make_float2(acc[i][jj].z, acc[i][jj].w));
+          const float2 a = __ffma2_rn(make_float2(f, f), make_float2(y[kk].x, y[kk].y), make_float2(acc[i][jj].x, acc[i][jj].y));
+          const float2 b = __ffma2_rn(make_float2(f, f), make_float2(y[kk].z, y[kk].w), make_float2(acc[i][jj].z, acc[i][jj].w));
           acc[i][jj] = make_float4(a.x, a.y, b.x, b.y);
         }
-      }
     }
   }
 }
-// sixteens of rows that a tile from position `first` has, and its positions rounded up to fours
+// sixteens of rows and of columns that a tile from position `first` has, and its positions rounded up to fours
+__device__ __forceinline__ int row_sixteens(int first, int end) { return end - first > 16 ? 2 : 1; }
 __device__ __forceinline__ int sixteens(int first, int end) { return end - first >= kB ? 4 : (end - first + 15) / 16; }
 __device__ __forceinline__ int fours(int first, int end) { return end - first >= kB ? kB : (end - first + 3) & ~3; }
 
@@ -147,24 +155,24 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
-// A block's item: half of one of the mask's tiles, the longest tiles first, and a head.
+// A block's item: a quarter of one of the mask's tiles, the longest tiles first, and a head.
 struct Item {
   int b, first, head;
 };
 __device__ __forceinline__ Item item_of(const int4* work, int heads, int block) {
-  const int half = block / heads;
-  const int4 t = work[half >> 1];
+  const int quarter = block / heads;
+  const int4 t = work[quarter >> 2];
   Item w;
   w.head = block % heads;
   w.b = t.x;
-  w.first = t.y * amask::kTile + (half & 1) * kB;
+  w.first = t.y * amask::kTile + (quarter & 3) * kRows;
   return w;
 }
 // The intervals of the tile's rows into shared memory, and the positions that any of them covers.  All threads.
 __device__ __forceinline__ int2 load_ranges(int2* rows, int* ends, const int2* all, const Call& c, const Item& w) {
   if (threadIdx.x == 0) { ends[0] = 0x7fffffff; ends[1] = 0; }
   __syncthreads();
-  if (threadIdx.x < kB) {
+  if (threadIdx.x < kRows) {
     const int s = w.first + threadIdx.x;
     const int2 r = s < c.S ? all[static_cast<int64_t>(w.b) * c.S + s] : make_int2(0, 0);
     rows[threadIdx.x] = r;
@@ -175,12 +183,12 @@ __device__ __forceinline__ int2 load_ranges(int2* rows, int* ends, const int2* a
 }
 
 template <typename T, int DV>
-__global__ void __launch_bounds__(kThreads) masked_fwd_kernel(const __grid_constant__ Call c) {
+__global__ void __launch_bounds__(kThreads, 3) masked_fwd_kernel(const __grid_constant__ Call c) {
   extern __shared__ float4 smem4[];
-  __shared__ int2 rows[kB];
-  __shared__ int ends[2], bad[kB];
+  __shared__ int2 rows[kRows];
+  __shared__ int ends[2], bad[kRows];
   float* sQ = reinterpret_cast<float*>(smem4);
-  float* sK = sQ + tile_floats(c.D);
+  float* sK = sQ + rows_floats(c.D);
   float* sV = sK + tile_floats(c.D);
   float* sP = sV + tile_floats(c.D);
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
@@ -189,24 +197,24 @@ __global__ void __launch_bounds__(kThreads) masked_fwd_kernel(const __grid_const
   const Item w = item_of(c.mask.qwork, c.Hk * c.G, blockIdx.x);
   if (w.first >= c.S) return;
   const int hk = w.head / c.G, g = w.head % c.G;
-  if (threadIdx.x < kB) bad[threadIdx.x] = 0;
+  if (threadIdx.x < kRows) bad[threadIdx.x] = 0;
   const int2 range = load_ranges(rows, ends, c.mask.rows, c, w);
-  load_tile(sQ, static_cast<const T*>(c.q) + q_row(c, w.b, hk, g, 0) * c.D, c.D, w.first, c.S, c.D);
+  load_tile<kRows>(sQ, static_cast<const T*>(c.q) + q_row(c, w.b, hk, g, 0) * c.D, c.D, w.first, c.S, c.D);
   const float slope2 = c.slopes ? c.slopes[w.head] * kLog2e : 0.0f;
-  const int ni = sixteens(w.first, c.S);
-  float m[4], l[4];
-  float4 acc[4][DV] = {};
+  const int ni = row_sixteens(w.first, c.S);
+  float m[kR], l[kR];
+  float4 acc[kR][DV] = {};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) { m[i] = kNoScore; l[i] = 0.0f; }
+  for (int i = 0; i < kR; ++i) { m[i] = kNoScore; l[i] = 0.0f; }
   for (int j0 = range.x; j0 < range.y; j0 += kB) {
     __syncthreads();
-    load_tile(sK, static_cast<const T*>(c.k) + k_row(c, w.b, hk, 0) * c.D, c.D, j0, c.S, c.D);
-    load_tile(sV, static_cast<const T*>(c.v) + k_row(c, w.b, hk, 0) * c.D, c.D, j0, c.S, c.D);
+    load_tile<kB>(sK, static_cast<const T*>(c.k) + k_row(c, w.b, hk, 0) * c.D, c.D, j0, c.S, c.D);
+    load_tile<kB>(sV, static_cast<const T*>(c.v) + k_row(c, w.b, hk, 0) * c.D, c.D, j0, c.S, c.D);
     __syncthreads();
-    float s[4][4];
+    float s[kR][4];
     mul_nt(s, sQ, sK, c.D, ty, tx, ni, sixteens(j0, range.y));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kR; ++i) {
       if (i >= ni) break;
       const int2 sees = rows[ty + 16 * i];
       const int qpos = w.first + ty + 16 * i;
@@ -238,7 +246,7 @@ __global__ void __launch_bounds__(kThreads) masked_fwd_kernel(const __grid_const
     mul_nn<DV>(acc, sP, sV, c.D, ty, tx, fours(j0, range.y), ni);
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kR; ++i) {
     const int s = w.first + ty + 16 * i;
     if (s >= c.S) continue;
     const bool none = l[i] == 0.0f;
@@ -256,7 +264,7 @@ __global__ void __launch_bounds__(kThreads) masked_fwd_kernel(const __grid_const
     if (c.lse != nullptr && tx == 0) c.lse[q_row(c, w.b, hk, g, s)] = none ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
   }
   __syncthreads();
-  for (int r = threadIdx.x >> 5; r < kB; r += kThreads / 32)
+  for (int r = threadIdx.x >> 5; r < kRows; r += kThreads / 32)
     if (bad[r]) fwd_row<T>(c, w.b, hk, g, w.first + r);
 }
 
@@ -265,15 +273,15 @@ __global__ void __launch_bounds__(kThreads) masked_fwd_kernel(const __grid_const
 template <typename T, int DV>
 __global__ void __launch_bounds__(kThreads) masked_dq_kernel(const __grid_constant__ Call c) {
   extern __shared__ float4 smem4[];
-  __shared__ int2 rows[kB];
-  __shared__ int ends[2], bad[kB];
-  __shared__ float s_lse2[kB], s_delta[kB];
+  __shared__ int2 rows[kRows];
+  __shared__ int ends[2], bad[kRows];
+  __shared__ float s_lse2[kRows], s_delta[kRows];
   float* sQ = reinterpret_cast<float*>(smem4);
-  float* sO = sQ + tile_floats(c.D);   // d o
-  float* sK = sO + tile_floats(c.D);
+  float* sO = sQ + rows_floats(c.D);   // d o
+  float* sK = sO + rows_floats(c.D);
   float* sV = sK + tile_floats(c.D);
   float* sS = sV + tile_floats(c.D);
-  float* sP = sS + kB * kLdP;
+  float* sP = sS + kRows * kLdP;
   constexpr bool kExact = sizeof(T) == 2;
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   grid_launch_dependents();
@@ -281,15 +289,15 @@ __global__ void __launch_bounds__(kThreads) masked_dq_kernel(const __grid_consta
   const Item w = item_of(c.mask.qwork, c.Hk * c.G, blockIdx.x);
   if (w.first >= c.S) return;
   const int hk = w.head / c.G, g = w.head % c.G;
-  if (threadIdx.x < kB) bad[threadIdx.x] = 0;
+  if (threadIdx.x < kRows) bad[threadIdx.x] = 0;
   const int2 range = load_ranges(rows, ends, c.mask.rows, c, w);
   const int64_t o0 = o_at(c, w.b, hk, g, 0), ostep = c.o_tok ? static_cast<int64_t>(c.Hk) * c.G * c.D : c.D;
-  load_tile(sQ, static_cast<const T*>(c.q) + q_row(c, w.b, hk, g, 0) * c.D, c.D, w.first, c.S, c.D);
-  load_tile(sO, static_cast<const T*>(c.dout) + o0, ostep, w.first, c.S, c.D);
-  load_tile(sK, static_cast<const T*>(c.o_in) + o0, ostep, w.first, c.S, c.D);
+  load_tile<kRows>(sQ, static_cast<const T*>(c.q) + q_row(c, w.b, hk, g, 0) * c.D, c.D, w.first, c.S, c.D);
+  load_tile<kRows>(sO, static_cast<const T*>(c.dout) + o0, ostep, w.first, c.S, c.D);
+  load_tile<kRows>(sK, static_cast<const T*>(c.o_in) + o0, ostep, w.first, c.S, c.D);
   __syncthreads();
   const int64_t pitch = amask::tiles_of(c.S) * amask::kTile;
-  for (int r = threadIdx.x >> 5; r < kB; r += kThreads / 32) {
+  for (int r = threadIdx.x >> 5; r < kRows; r += kThreads / 32) {
     float d = 0.0f;
     for (int e = threadIdx.x & 31; e < c.D; e += 32) d = fmaf(sO[r * (c.D + 4) + e], sK[r * (c.D + 4) + e], d);
     d = warp_sum(d);
@@ -308,20 +316,20 @@ __global__ void __launch_bounds__(kThreads) masked_dq_kernel(const __grid_consta
     }
   }
   const float slope2 = c.slopes ? c.slopes[w.head] * kLog2e : 0.0f;
-  const int ni = sixteens(w.first, c.S);
-  float4 acc[4][DV] = {}, acc2[kExact ? 4 : 1][DV] = {};
-  float exact[4] = {};
+  const int ni = row_sixteens(w.first, c.S);
+  float4 acc[kR][DV] = {}, acc2[kExact ? kR : 1][DV] = {};
+  float exact[kR] = {};
   for (int j0 = range.x; j0 < range.y; j0 += kB) {
     __syncthreads();
-    load_tile(sK, static_cast<const T*>(c.k) + k_row(c, w.b, hk, 0) * c.D, c.D, j0, c.S, c.D);
-    load_tile(sV, static_cast<const T*>(c.v) + k_row(c, w.b, hk, 0) * c.D, c.D, j0, c.S, c.D);
+    load_tile<kB>(sK, static_cast<const T*>(c.k) + k_row(c, w.b, hk, 0) * c.D, c.D, j0, c.S, c.D);
+    load_tile<kB>(sV, static_cast<const T*>(c.v) + k_row(c, w.b, hk, 0) * c.D, c.D, j0, c.S, c.D);
     __syncthreads();
-    float s[4][4], dp[4][4];
+    float s[kR][4], dp[kR][4];
     const int nj = sixteens(j0, range.y);
     mul_nt(s, sQ, sK, c.D, ty, tx, ni, nj);
     mul_nt(dp, sO, sV, c.D, ty, tx, ni, nj);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kR; ++i) {
       if (i >= ni) break;
       const int r = ty + 16 * i;
       const int2 sees = rows[r];
@@ -345,7 +353,7 @@ __global__ void __launch_bounds__(kThreads) masked_dq_kernel(const __grid_consta
     if constexpr (kExact) mul_nn<DV>(acc2, sP, sK, c.D, ty, tx, fours(j0, range.y), ni);
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kR; ++i) {
     const int s = w.first + ty + 16 * i;
     float put_right = 0.0f;
     if constexpr (kExact) {
@@ -370,21 +378,21 @@ __global__ void __launch_bounds__(kThreads) masked_dq_kernel(const __grid_consta
     }
   }
   __syncthreads();
-  for (int r = threadIdx.x >> 5; r < kB; r += kThreads / 32)
+  for (int r = threadIdx.x >> 5; r < kRows; r += kThreads / 32)
     if (bad[r]) dq_row<T>(c, w.b, hk, g, w.first + r);
 }
 
 template <typename T, int DV>
 __global__ void __launch_bounds__(kThreads) masked_dkv_kernel(const __grid_constant__ Call c) {
   extern __shared__ float4 smem4[];
-  __shared__ int2 rows[kB];
-  __shared__ int ends[2], bad[kB];
+  __shared__ int2 rows[kRows];
+  __shared__ int ends[2], bad[kRows];
   float* sK = reinterpret_cast<float*>(smem4);
-  float* sV = sK + tile_floats(c.D);
-  float* sQ = sV + tile_floats(c.D);
+  float* sV = sK + rows_floats(c.D);
+  float* sQ = sV + rows_floats(c.D);
   float* sO = sQ + tile_floats(c.D);
   float* sP = sO + tile_floats(c.D);
-  float* sS = sP + kB * kLdP;
+  float* sS = sP + kRows * kLdP;
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   grid_launch_dependents();
   grid_dependency_wait();
@@ -393,13 +401,13 @@ __global__ void __launch_bounds__(kThreads) masked_dkv_kernel(const __grid_const
   const int parts = static_cast<int>(cl.num_blocks()), part = static_cast<int>(cl.block_rank());
   const Item w = item_of(c.mask.kwork, c.Hk, blockIdx.x / parts);
   if (w.first >= c.S) return;   // (all of the cluster)
-  const int hk = w.head, ni = sixteens(w.first, c.S);
-  if (threadIdx.x < kB) bad[threadIdx.x] = 0;
+  const int hk = w.head, ni = row_sixteens(w.first, c.S);
+  if (threadIdx.x < kRows) bad[threadIdx.x] = 0;
   const int2 range = load_ranges(rows, ends, c.mask.keys, c, w);
-  load_tile(sK, static_cast<const T*>(c.k) + k_row(c, w.b, hk, 0) * c.D, c.D, w.first, c.S, c.D);
-  load_tile(sV, static_cast<const T*>(c.v) + k_row(c, w.b, hk, 0) * c.D, c.D, w.first, c.S, c.D);
+  load_tile<kRows>(sK, static_cast<const T*>(c.k) + k_row(c, w.b, hk, 0) * c.D, c.D, w.first, c.S, c.D);
+  load_tile<kRows>(sV, static_cast<const T*>(c.v) + k_row(c, w.b, hk, 0) * c.D, c.D, w.first, c.S, c.D);
   const int64_t pitch = amask::tiles_of(c.S) * amask::kTile, ostep = c.o_tok ? static_cast<int64_t>(c.Hk) * c.G * c.D : c.D;
-  float4 gk[4][DV] = {}, gv[4][DV] = {};
+  float4 gk[kR][DV] = {}, gv[kR][DV] = {};
   const int per_head = range.y > range.x ? (range.y - range.x + kB - 1) / kB : 0;
   const int64_t steps = static_cast<int64_t>(c.G) * per_head;
   for (int64_t step = steps * part / parts; step < steps * (part + 1) / parts; ++step) {
@@ -408,10 +416,10 @@ __global__ void __launch_bounds__(kThreads) masked_dkv_kernel(const __grid_const
     const int64_t srow = ((static_cast<int64_t>(w.b) * c.Hk + hk) * c.G + g) * pitch;
     {
       __syncthreads();
-      load_tile(sQ, static_cast<const T*>(c.q) + q_row(c, w.b, hk, g, 0) * c.D, c.D, i0, c.S, c.D);
-      load_tile(sO, static_cast<const T*>(c.dout) + o_at(c, w.b, hk, g, 0), ostep, i0, c.S, c.D);
+      load_tile<kB>(sQ, static_cast<const T*>(c.q) + q_row(c, w.b, hk, g, 0) * c.D, c.D, i0, c.S, c.D);
+      load_tile<kB>(sO, static_cast<const T*>(c.dout) + o_at(c, w.b, hk, g, 0), ostep, i0, c.S, c.D);
       __syncthreads();
-      float s[4][4], dp[4][4], lse2[4], delta[4];   // rows: keys, columns: queries
+      float s[kR][4], dp[kR][4], lse2[4], delta[4];   // rows: keys, columns: queries
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int qpos = i0 + tx + 16 * j;
@@ -422,7 +430,7 @@ __global__ void __launch_bounds__(kThreads) masked_dkv_kernel(const __grid_const
       mul_nt(s, sK, sQ, c.D, ty, tx, ni, nj);
       mul_nt(dp, sV, sO, c.D, ty, tx, ni, nj);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kR; ++i) {
         if (i >= ni) break;
         const int r = ty + 16 * i;
         const int2 seen = rows[r];
@@ -445,7 +453,7 @@ __global__ void __launch_bounds__(kThreads) masked_dkv_kernel(const __grid_const
     // every block's sums into its own shared memory (over Q and d O), then the first adds the others' to its own, in order
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < kR; ++i)
 #pragma unroll
       for (int jj = 0; jj < DV; ++jj) {
         const int col = 4 * (tx + 16 * jj);
@@ -458,7 +466,7 @@ __global__ void __launch_bounds__(kThreads) masked_dkv_kernel(const __grid_const
       for (int q = 1; q < parts; ++q) {
         const float *pk = cl.map_shared_rank(sQ, q), *pv = cl.map_shared_rank(sO, q);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < kR; ++i)
 #pragma unroll
           for (int jj = 0; jj < DV; ++jj) {
             const int col = 4 * (tx + 16 * jj);
@@ -472,7 +480,7 @@ __global__ void __launch_bounds__(kThreads) masked_dkv_kernel(const __grid_const
     if (part != 0) return;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kR; ++i) {
     const int s = w.first + ty + 16 * i;
     if (s >= c.S) continue;
     const int64_t at = k_row(c, w.b, hk, s) * c.D;
@@ -488,7 +496,7 @@ __global__ void __launch_bounds__(kThreads) masked_dkv_kernel(const __grid_const
     }
   }
   __syncthreads();
-  for (int r = threadIdx.x >> 5; r < kB; r += kThreads / 32)
+  for (int r = threadIdx.x >> 5; r < kRows; r += kThreads / 32)
     if (bad[r]) dkv_row<T>(c, w.b, hk, w.first + r);
 }
 
@@ -511,18 +519,19 @@ int launch_one(void (*kernel)(Call), const char* name, int64_t blocks, int clust
 }
 template <typename T>
 int launch_fwd(const Call& c, cudaStream_t st) {
-  const int64_t halves = 2 * amask::tiles_of(c.S) * c.B;
-  return launch_one(c.D <= 64 ? masked_fwd_kernel<T, 1> : masked_fwd_kernel<T, 2>, "masked_fwd_kernel", halves * c.Hk * c.G, 1, smem_fwd(c.D), c, st);
+  const int64_t quarters = 4 * amask::tiles_of(c.S) * c.B;
+  return launch_one(c.D <= 64 ? masked_fwd_kernel<T, 1> : masked_fwd_kernel<T, 2>, "masked_fwd_kernel", quarters * c.Hk * c.G, 1, smem_fwd(c.D), c, st);
 }
 template <typename T>
 int launch_bwd(const Call& c, int sms, cudaStream_t st) {
-  const int64_t halves = 2 * amask::tiles_of(c.S) * c.B;
-  if (int rc = launch_one(c.D <= 64 ? masked_dq_kernel<T, 1> : masked_dq_kernel<T, 2>, "masked_dq_kernel", halves * c.Hk * c.G, 1, smem_dq(c.D), c, st)) return rc;
-  // few key tiles: clusters share one's steps, as long as the device has room and a part has a step (2 x 3 heads of 19 positions: 45 us alone, SHARED by 4)
-  const int64_t tiles = halves * c.Hk, steps = static_cast<int64_t>(c.G) * ((c.S + kB - 1) / kB);
+  const int64_t quarters = 4 * amask::tiles_of(c.S) * c.B;
+  if (int rc = launch_one(c.D <= 64 ? masked_dq_kernel<T, 1> : masked_dq_kernel<T, 2>, "masked_dq_kernel", quarters * c.Hk * c.G, 1, smem_bwd(c.D), c, st)) return rc;
+  // clusters share a key tile's steps as long as a part has one and there are not many blocks to an SM: the longest tile's chain of steps is what
+  // the launch takes (2 kv heads of 7 x 1200 positions of 80, whole backward pass: 2516 us unshared, SHARED by 8)
+  const int64_t tiles = quarters * c.Hk, steps = static_cast<int64_t>(c.G) * ((c.S + kB - 1) / kB);
   int parts = 1;
-  while (parts < 8 && tiles * parts * 2 <= sms && parts * 2 <= steps) parts *= 2;
-  return launch_one(c.D <= 64 ? masked_dkv_kernel<T, 1> : masked_dkv_kernel<T, 2>, "masked_dkv_kernel", tiles * parts, parts, smem_dkv(c.D), c, st);
+  while (parts < 8 && tiles * parts * 2 <= 8 * sms && parts * 2 <= steps) parts *= 2;
+  return launch_one(c.D <= 64 ? masked_dkv_kernel<T, 1> : masked_dkv_kernel<T, 2>, "masked_dkv_kernel", tiles * parts, parts, smem_bwd(c.D), c, st);
 }
 
 inline size_t up1k(size_t v) { return (v + 1023) & ~static_cast<size_t>(1023); }
