@@ -1229,11 +1229,9 @@ __device__ __forceinline__ void bulk_load_1d(uint32_t dst, const void* src, uint
                ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
-template <bool MASKED, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kKvThreads, 1)
 attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmdO, const BwdParams p,
-                const __grid_constant__ CallOf<MASKED> c) {
+                const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmdO, const BwdParams p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen_base = smem_raw + (base - smem_u32(smem_raw));
@@ -1245,8 +1243,6 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
   const uint32_t pds_ready0 = sdp_full0 + 16, out_full = pds_ready0 + 16, tmem_slot = out_full + 8, abort_addr = tmem_slot + 4;
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(gen_base + (tmem_slot - base));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_base + (abort_addr - base));
-  volatile int* bad = reinterpret_cast<volatile int*>(gen_base + kKvOffBad);   // MASKED: key rows that came out not finite
-  if (MASKED && threadIdx.x < kBQ) bad[threadIdx.x] = 0;
 
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
@@ -1272,21 +1268,10 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
   const uint32_t tDV = tmem_base + 256, tDK = tmem_base + 320, tPT0 = tmem_base + 384;
 
   // all kv heads of key block 0 (the most query steps) start first
-  const int part = blockIdx.x % p.kv_parts;
-  int kb, nb, i0, per_head;   // key block, kv head; first query step (of 64) that sees this key block, steps per head
-  int b = 0, hk = 0;
-  if constexpr (MASKED) {
-    const int item = blockIdx.x / p.kv_parts;
-    const int4 rec = c.mask.kwork[item / c.Hk];
-    hk = item % c.Hk;
-    b = rec.x; kb = rec.y; i0 = rec.z; per_head = rec.w;
-    nb = b * c.Hk + hk;
-  } else {
-    kb = blockIdx.y;
-    nb = blockIdx.x / p.kv_parts;
-    i0 = 2 * kb;
-    per_head = (p.S + kBK - 1) / kBK - i0;
-  }
+  const int kb = blockIdx.y, part = blockIdx.x % p.kv_parts, nb = blockIdx.x / p.kv_parts;
+  const int nq = (p.S + kBK - 1) / kBK;          // query steps of 64 per head
+  const int i0 = 2 * kb;                         // first query step that sees this key block
+  const int per_head = nq - i0;
   // this CTA's steps [t0, t0 + nsteps) of the key block's G * per_head; a part may be empty
   const int all_steps = p.G * per_head;
   const int t0 = static_cast<int>(static_cast<int64_t>(all_steps) * part / p.kv_parts);
@@ -1376,12 +1361,6 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     const int key = kb * kBQ + row;
     const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
     bool ok = true;
-    int2 seen = make_int2(0, 0);   // the queries that see this key
-    if constexpr (MASKED) {
-      if (key < p.S) seen = c.mask.keys[static_cast<int64_t>(b) * p.S + key];
-    }
-    std::conditional_t<MASKED, Shape<CAP, BIAS>, NoCall> shape(c);
-    const float sc = CAP || BIAS ? 1.0f : p.sc;
     for (int t = group; t < nsteps; t += 2) {
       const int st = group;
       const int i = i0 + (t0 + t) % per_head;
@@ -1394,25 +1373,13 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
       const float* st_nl2 = reinterpret_cast<const float*>(gen_base + kKvOffStage + (t % kKvStages) * kKvStageStride + 2 * kKBytes) + half * 32;
       const float* st_nd = st_nl2 + 64;
       const int q0 = i * kBK + half * 32;
-      const bool diag = !MASKED && i * kBK < (kb + 1) * kBQ;   // some query of this step lies before some key of the block
-      uint32_t bits = 0xffffffffu;
-      bool edge = false;
-      if constexpr (MASKED) {
-        edge = q0 < seen.x || q0 + 32 > seen.y;
-        if (edge) bits = interval_bits(seen.x, seen.y, q0);
-        if constexpr (BIAS) shape.slope2 = c.slopes[hk * p.G + (t0 + t) / per_head] * kLog2e;
-      }
-      const float2 sc2 = f2(sc, sc);
+      const bool diag = i * kBK < (kb + 1) * kBQ;   // some query of this step lies before some key of the block
+      const float2 sc2 = f2(p.sc, p.sc);
       // the exponentials are taken while dP^T is still on its way from tensor memory
       uint32_t vs[32], vd[32];
       tmem_ld_x32(tS + half * 32, vs);
       tmem_ld_wait_on(vs);
       tmem_ld_x32(tDP + half * 32, vd);
-      float2 slope[CAP ? 16 : 1];   // 1 - tanh^2
-      if constexpr (CAP || BIAS)
-        shape.apply(vs, static_cast<float>(q0 - key), 1.0f, [&](int e, float2 t2) {
-          if constexpr (CAP) slope[e >> 1] = __ffma2_rn(t2, f2(-t2.x, -t2.y), f2(1.0f, 1.0f));
-        });
 #pragma unroll
       for (int e = 0; e < 32; e += 4) {
         const float4 nl = *reinterpret_cast<const float4*>(st_nl2 + e);
@@ -1422,7 +1389,6 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           if (diag && key > q0 + e + x) pr[x] = 0.0f;
-          if (MASKED && edge && (bits >> (e + x) & 1u) == 0) pr[x] = 0.0f;
           vs[e + x] = __float_as_uint(pr[x]);
         }
       }
@@ -1432,12 +1398,8 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
       for (int e = 0; e < 32; e += 4) {
         const float4 nd = *reinterpret_cast<const float4*>(st_nd + e);
         const float2 pa = f2(__uint_as_float(vs[e]), __uint_as_float(vs[e + 1])), pb = f2(__uint_as_float(vs[e + 2]), __uint_as_float(vs[e + 3]));
-        float2 da = __fmul2_rn(pa, __fadd2_rn(f2(__uint_as_float(vd[e]), __uint_as_float(vd[e + 1])), f2(nd.x, nd.y)));
-        float2 db = __fmul2_rn(pb, __fadd2_rn(f2(__uint_as_float(vd[e + 2]), __uint_as_float(vd[e + 3])), f2(nd.z, nd.w)));
-        if constexpr (CAP) {
-          da = __fmul2_rn(da, slope[e >> 1]);
-          db = __fmul2_rn(db, slope[(e >> 1) + 1]);
-        }
+        const float2 da = __fmul2_rn(pa, __fadd2_rn(f2(__uint_as_float(vd[e]), __uint_as_float(vd[e + 1])), f2(nd.x, nd.y)));
+        const float2 db = __fmul2_rn(pb, __fadd2_rn(f2(__uint_as_float(vd[e + 2]), __uint_as_float(vd[e + 3])), f2(nd.z, nd.w)));
         wp[e >> 1] = pack_bf16(pa.x, pa.y);
         wp[(e >> 1) + 1] = pack_bf16(pb.x, pb.y);
         wd[e >> 1] = pack_bf16(da.x, da.y);
@@ -1461,10 +1423,6 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         uint32_t v[16];
         tmem_ld_x16((group == 0 ? tDV : tDK) + lane_addr + c, v);
         tmem_ld_wait();
-        if (MASKED && nsteps == 0) {   // nothing sees this key block: the accumulators were never written
-#pragma unroll
-          for (int e = 0; e < 16; ++e) v[e] = 0;
-        }
         if (p.kv_parts > 1) {
           // this part's sums, column by column, into the load ring (every step's tiles have been read)
           float* at = reinterpret_cast<float*>(gen_base + kKvOffStage) + (group * kD + c) * kBQ + row;
@@ -1472,12 +1430,6 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
           for (int e = 0; e < 16; ++e) at[e * kBQ] = nsteps > 0 ? __uint_as_float(v[e]) : 0.0f;
         } else if (key < p.S) {
           uint32_t w[8];
-          if constexpr (MASKED) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) sum = fmaf(__uint_as_float(v[e]), 0.0f, sum);
-            if (!(sum == 0.0f)) bad[row] = 1;
-          }
 #pragma unroll
           for (int e = 0; e < 16; e += 2) w[e >> 1] = pack_bf16(__uint_as_float(v[e]) * f, __uint_as_float(v[e + 1]) * f);
           *reinterpret_cast<uint4*>(orow + c) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -1506,7 +1458,6 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
 #pragma unroll
           for (int k = 0; k < 4; ++k) a[k] += peer[k * kBQ];
         }
-        if (MASKED && kb * kBQ + row < p.S && !((a[0] + a[1] + a[2] + a[3]) * 0.0f == 0.0f)) bad[row] = 1;
         if (kb * kBQ + row < p.S) *reinterpret_cast<uint2*>(orow + c) = make_uint2(pack_bf16(a[0] * f, a[1] * f), pack_bf16(a[2] * f, a[3] * f));
       }
     }
@@ -1519,15 +1470,302 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
   }
   tcgen05_fence_before();
   __syncthreads();
-  if constexpr (MASKED) {
-    // (a key row's gradients were written by threads of this block, before the barrier)
-    if (warp >= 2)
-      for (int r = warp - 2; r < kBQ; r += kKvThreads / 32 - 2)
-        if (bad[r] != 0) mattn::dkv_row<__nv_bfloat16>(c, b, hk, kb * kBQ + r);
-  }
   if (warp == 1) {
     tcgen05_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+  }
+}
+
+// The same under a mask: two CTAs of half the tensor memory (256 columns) on an SM instead of one of all of it, so that one's loads, first
+// products and write-out pass under the other's steps: documents make many short key blocks of what would be few long ones.  One group of eight element-wise
+// warps: a warp has a quadrant's 32 key rows and 32 of a step's 64 queries.  Tensor memory: S^T at 0, dP^T at 64, dV at 128, dK at 192; a warp
+// writes P^T and dS^T (bf16 pairs) over the first half of the columns of S^T and dP^T that it has read itself.  The next step's S^T is issued
+// behind the product that has read P^T, its dP^T behind the one that has read dS^T.  Backward pass, 14 heads over 2 of 4 x 1024 .. HERE
+constexpr int kKvmThreads = 320;
+template <bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kKvmThreads, 2)
+attn_dkv_masked_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                       const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmdO, const BwdParams p,
+                       const __grid_constant__ mattn::Call c) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* gen_base = smem_raw + (base - smem_u32(smem_raw));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  const uint32_t kv_full = base + kKvOffBar, ld_full0 = kv_full + 8, ld_empty0 = ld_full0 + 8 * kKvStages;
+  const uint32_t s_full = ld_empty0 + 8 * kKvStages, dp_full = s_full + 8, p_ready = dp_full + 8, ds_ready = p_ready + 8;
+  const uint32_t out_full = ds_ready + 8, tmem_slot = out_full + 8, abort_addr = tmem_slot + 4;
+  volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(gen_base + (tmem_slot - base));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_base + (abort_addr - base));
+  volatile int* bad = reinterpret_cast<volatile int*>(gen_base + kKvOffBad);   // key rows that came out not finite
+  if (threadIdx.x < kBQ) bad[threadIdx.x] = 0;
+
+  if (threadIdx.x == 0) {
+    mbar_init(kv_full, 1);
+    for (int s = 0; s < kKvStages; ++s) { mbar_init(ld_full0 + 8 * s, 1); mbar_init(ld_empty0 + 8 * s, 1); }
+    mbar_init(s_full, 1);
+    mbar_init(dp_full, 1);
+    mbar_init(p_ready, 8);
+    mbar_init(ds_ready, 8);
+    mbar_init(out_full, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async_smem();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(256u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem_base = *tmem_slot_ptr;
+  grid_launch_dependents();
+  grid_dependency_wait();   // the set-up above ran under the tail of the kernel before
+  const uint32_t tS = tmem_base, tDP = tmem_base + 64, tDV = tmem_base + 128, tDK = tmem_base + 192;
+
+  const int part = blockIdx.x % p.kv_parts, item = blockIdx.x / p.kv_parts;
+  const int4 rec = c.mask.kwork[item / c.Hk];
+  const int hk = item % c.Hk, b = rec.x, kb = rec.y, nb = b * c.Hk + hk;
+  const int i0 = rec.z, per_head = rec.w;   // first query step (of 64) that sees this key block, steps per head
+  // this CTA's steps [t0, t0 + nsteps) of the key block's G * per_head; a part may be empty
+  const int all_steps = p.G * per_head;
+  const int t0 = static_cast<int>(static_cast<int64_t>(all_steps) * part / p.kv_parts);
+  const int nsteps = static_cast<int>(static_cast<int64_t>(all_steps) * (part + 1) / p.kv_parts) - t0;
+
+  if (warp == 0) {
+    if (elect_one() && nsteps > 0) {
+      mbar_expect_tx(kv_full, 2 * kQBytes);
+      tma_load_3d(base + kKvOffK, &tmK, kv_full, 0, kb * kBQ, nb);
+      tma_load_3d(base + kKvOffV, &tmV, kv_full, 0, kb * kBQ, nb);
+      for (int t = 0; t < nsteps; ++t) {
+        const int st = t % kKvStages;
+        const int g = (t0 + t) / per_head, i = i0 + (t0 + t) % per_head;
+        if (!mbar_wait(ld_empty0 + 8 * st, ((t / kKvStages) & 1) ^ 1, abort_flag, 91, p.status)) break;
+        const int64_t prow = (static_cast<int64_t>(nb) * p.G + g) * (q_blocks(p.S) * kBQ) + i * kBK;
+        const uint32_t sb = base + kKvOffStage + st * kKvStageStride, fb = ld_full0 + 8 * st;
+        mbar_expect_tx(fb, kKvStageBytes);
+        tma_load_3d(sb, &tmQ, fb, 0, i * kBK, nb * p.G + g);
+        int dcol, dplane;
+        o_plane(p.G, p.HKV, p.o_tok, nb, g, dcol, dplane);
+        tma_load_3d(sb + kKBytes, &tmdO, fb, dcol, i * kBK, dplane);
+        bulk_load_1d(sb + 2 * kKBytes, p.nlse2 + prow, 256, fb);
+        bulk_load_1d(sb + 2 * kKBytes + 256, p.ndelta + prow, 256, fb);
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t idesc = make_idesc(kBK);
+      const uint64_t dK = desc_sw128(base + kKvOffK), dV = desc_sw128(base + kKvOffV);
+      const uint64_t dQk = desc_sw128(base + kKvOffStage), dQn = desc_sw128_mn(base + kKvOffStage, kKBytes, 1024);
+      // S^T = K Q^T of the step in ring stage st, and dP^T = V dO^T
+      auto issue_s = [&](int st) {
+        const uint32_t so = static_cast<uint32_t>(st) * kKvStageStride;
+#pragma unroll
+        for (int k4 = 0; k4 < kD / 16; ++k4)
+          umma_bf16(tS, desc_advance(dK, k4 * 32), desc_advance(dQk, so + k4 * 32), idesc, k4 != 0 ? 1u : 0u);
+        umma_commit(s_full);
+      };
+      auto issue_dp = [&](int st) {
+        const uint32_t so = static_cast<uint32_t>(st) * kKvStageStride + kKBytes;
+#pragma unroll
+        for (int k4 = 0; k4 < kD / 16; ++k4)
+          umma_bf16(tDP, desc_advance(dV, k4 * 32), desc_advance(dQk, so + k4 * 32), idesc, k4 != 0 ? 1u : 0u);
+        umma_commit(dp_full);
+      };
+      bool ok = nsteps > 0 && mbar_wait(kv_full, 0, abort_flag, 92, p.status) && mbar_wait(ld_full0, 0, abort_flag, 93, p.status);
+      if (ok) {
+        tcgen05_fence_after();
+        issue_s(0);
+        issue_dp(0);
+      }
+      for (int t = 0; ok && t < nsteps; ++t) {
+        const int st = t % kKvStages, next = (t + 1) % kKvStages;
+        const uint32_t so = static_cast<uint32_t>(st) * kKvStageStride;
+        const uint32_t acc = t != 0 ? 1u : 0u;
+        ok = mbar_wait(p_ready, t & 1, abort_flag, 94, p.status);
+        if (!ok) break;
+        tcgen05_fence_after();
+        // dV += P^T dO   (A = P^T [128 keys x 64 queries] in tensor memory, 16 queries = 8 columns, the second 32 queries 32 columns on; B =
+        // the dO tile as it lies, [64 queries x 64 d]: N-major, 16 queries further = two 8-row groups of 1024 bytes)
+#pragma unroll
+        for (int k4 = 0; k4 < kBK / 16; ++k4)
+          umma_bf16_ts(tDV, tS + (k4 >> 1) * 32 + (k4 & 1) * 8, desc_advance(dQn, so + kKBytes + k4 * 2048), idesc | (1u << 16), k4 != 0 ? 1u : acc);
+        if (t + 1 < nsteps) {
+          ok = mbar_wait(ld_full0 + 8 * next, ((t + 1) / kKvStages) & 1, abort_flag, 93, p.status);
+          if (!ok) break;
+          tcgen05_fence_after();
+          issue_s(next);
+        }
+        ok = mbar_wait(ds_ready, t & 1, abort_flag, 95, p.status);
+        if (!ok) break;
+        tcgen05_fence_after();
+        // dK += dS^T Q
+#pragma unroll
+        for (int k4 = 0; k4 < kBK / 16; ++k4)
+          umma_bf16_ts(tDK, tDP + (k4 >> 1) * 32 + (k4 & 1) * 8, desc_advance(dQn, so + k4 * 2048), idesc | (1u << 16), k4 != 0 ? 1u : acc);
+        umma_commit(ld_empty0 + 8 * st);
+        if (t + 1 < nsteps) issue_dp(next);
+        else umma_commit(out_full);
+      }
+    }
+  } else {
+    const int quad = warp & 3;                // tensor-memory lane quadrant of this warp
+    const int half = ((warp - 2) >> 2) & 1;   // which 32 of the 64 query columns
+    const int row = quad * 32 + lane;
+    const int key = kb * kBQ + row;
+    const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t aS = tS + lane_addr + half * 32, aDP = tDP + lane_addr + half * 32;
+    bool ok = true;
+    int2 seen = make_int2(0, 0);   // the queries that see this key
+    if (key < p.S) seen = c.mask.keys[static_cast<int64_t>(b) * p.S + key];
+    Shape<CAP, BIAS> shape(c);
+    const float sc = CAP || BIAS ? 1.0f : p.sc;
+    const float2 sc2 = f2(sc, sc);
+    for (int t = 0; t < nsteps; ++t) {
+      const int q0 = (i0 + (t0 + t) % per_head) * kBK + half * 32;
+      ok = __all_sync(0xffffffffu, mbar_wait(s_full, t & 1, abort_flag, 96, p.status));
+      if (!ok) break;
+      tcgen05_fence_after();
+      const float* st_nl2 = reinterpret_cast<const float*>(gen_base + kKvOffStage + (t % kKvStages) * kKvStageStride + 2 * kKBytes) + half * 32;
+      const float* st_nd = st_nl2 + 64;
+      const bool edge = q0 < seen.x || q0 + 32 > seen.y;
+      const uint32_t bits = edge ? interval_bits(seen.x, seen.y, q0) : 0xffffffffu;
+      if constexpr (BIAS) shape.slope2 = c.slopes[hk * p.G + (t0 + t) / per_head] * kLog2e;
+      uint32_t vs[32];
+      tmem_ld_x32(aS, vs);
+      tmem_ld_wait_on(vs);
+      __half2 bend[CAP ? 16 : 1];   // 1 - tanh^2, to 2^-12 of itself
+      if constexpr (CAP || BIAS)
+        shape.apply(vs, static_cast<float>(q0 - key), 1.0f, [&](int e, float2 t2) {
+          if constexpr (CAP) bend[e >> 1] = __float22half2_rn(__ffma2_rn(t2, f2(-t2.x, -t2.y), f2(1.0f, 1.0f)));
+        });
+      uint32_t wp[16];
+#pragma unroll
+      for (int e = 0; e < 32; e += 4) {
+        const float4 nl = *reinterpret_cast<const float4*>(st_nl2 + e);
+        const float2 ta = __ffma2_rn(f2(__uint_as_float(vs[e]), __uint_as_float(vs[e + 1])), sc2, f2(nl.x, nl.y));
+        const float2 tb = __ffma2_rn(f2(__uint_as_float(vs[e + 2]), __uint_as_float(vs[e + 3])), sc2, f2(nl.z, nl.w));
+        float pr[4] = {ex2(ta.x), ex2(ta.y), ex2(tb.x), ex2(tb.y)};
+        if (edge) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if ((bits >> (e + x) & 1u) == 0) pr[x] = 0.0f;
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) vs[e + x] = __float_as_uint(pr[x]);
+        wp[e >> 1] = pack_bf16(pr[0], pr[1]);
+        wp[(e >> 1) + 1] = pack_bf16(pr[2], pr[3]);
+      }
+      tmem_st_x16(aS, wp);
+      tmem_st_wait();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_ready);
+      ok = __all_sync(0xffffffffu, mbar_wait(dp_full, t & 1, abort_flag, 97, p.status));
+      if (!ok) break;
+      tcgen05_fence_after();
+      uint32_t vd[32];
+      tmem_ld_x32(aDP, vd);
+      tmem_ld_wait_on(vd);
+      uint32_t wd[16];
+#pragma unroll
+      for (int e = 0; e < 32; e += 4) {
+        const float4 nd = *reinterpret_cast<const float4*>(st_nd + e);
+        float2 da = __fmul2_rn(f2(__uint_as_float(vs[e]), __uint_as_float(vs[e + 1])),
+                               __fadd2_rn(f2(__uint_as_float(vd[e]), __uint_as_float(vd[e + 1])), f2(nd.x, nd.y)));
+        float2 db = __fmul2_rn(f2(__uint_as_float(vs[e + 2]), __uint_as_float(vs[e + 3])),
+                               __fadd2_rn(f2(__uint_as_float(vd[e + 2]), __uint_as_float(vd[e + 3])), f2(nd.z, nd.w)));
+        if constexpr (CAP) {
+          da = __fmul2_rn(da, __half22float2(bend[e >> 1]));
+          db = __fmul2_rn(db, __half22float2(bend[(e >> 1) + 1]));
+        }
+        wd[e >> 1] = pack_bf16(da.x, da.y);
+        wd[(e >> 1) + 1] = pack_bf16(db.x, db.y);
+      }
+      tmem_st_x16(aDP, wd);
+      tmem_st_wait();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_ready);
+    }
+    if (ok && nsteps > 0) ok = __all_sync(0xffffffffu, mbar_wait(out_full, 0, abort_flag, 98, p.status));
+    if (ok) {
+      tcgen05_fence_after();
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {   // this warp's 32 columns of dV, then of dK, 16 at a time
+        const bool is_dk = k >= 2;
+        const int col = half * 32 + (k & 1) * 16;
+        uint32_t v[16];
+        tmem_ld_x16((is_dk ? tDK : tDV) + lane_addr + col, v);
+        tmem_ld_wait();
+        if (nsteps == 0) {   // nothing sees this key block: the accumulators were never written
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[e] = 0;
+        }
+        const float f = is_dk ? p.scale : 1.0f;
+        if (p.kv_parts > 1) {
+          // this part's sums, column by column, into the load ring (every step's tiles have been read)
+          float* at = reinterpret_cast<float*>(gen_base + kKvOffStage) + ((is_dk ? kD : 0) + col) * kBQ + row;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) at[e * kBQ] = __uint_as_float(v[e]);
+        } else if (key < p.S) {
+          uint32_t w[8];
+          float sum = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sum = fmaf(__uint_as_float(v[e]), 0.0f, sum);
+          if (!(sum == 0.0f)) bad[row] = 1;
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) w[e >> 1] = pack_bf16(__uint_as_float(v[e]) * f, __uint_as_float(v[e + 1]) * f);
+          __nv_bfloat16* orow = (is_dk ? p.dK : p.dV) + (static_cast<int64_t>(nb) * p.S + key) * kD + col;
+          *reinterpret_cast<uint4*>(orow) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(orow + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+        }
+      }
+    }
+  }
+
+  if (p.kv_parts > 1) {
+    // each CTA of the cluster adds up its share of the key rows from all parts, in their order
+    __syncwarp();
+    cg::cluster_group cl = cg::this_cluster();
+    cl.sync();
+    if (warp >= 2) {
+      const int rows = kBQ / p.kv_parts, cols = kD / p.kv_parts;   // rows of this CTA, columns of a thread
+      const int e = threadIdx.x - 64;
+      const int row = part * rows + e % rows, c0 = e / rows * cols;    // columns 0..63 are dV, 64..127 dK
+      const float* src = reinterpret_cast<const float*>(gen_base + kKvOffStage) + c0 * kBQ + row;
+      const float f = c0 < kD ? 1.0f : p.scale;
+      __nv_bfloat16* orow = (c0 < kD ? p.dV : p.dK) + (static_cast<int64_t>(nb) * p.S + kb * kBQ + row) * kD + (c0 & (kD - 1));
+      for (int k = 0; k < cols; k += 4) {
+        float a[4] = {};
+        for (int q = 0; q < p.kv_parts; ++q) {
+          const float* peer = cl.map_shared_rank(src, q) + k * kBQ;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) a[x] += peer[x * kBQ];
+        }
+        if (kb * kBQ + row < p.S) {
+          if (!((a[0] + a[1] + a[2] + a[3]) * 0.0f == 0.0f)) bad[row] = 1;
+          *reinterpret_cast<uint2*>(orow + k) = make_uint2(pack_bf16(a[0] * f, a[1] * f), pack_bf16(a[2] * f, a[3] * f));
+        }
+      }
+    }
+    cl.sync();   // no CTA leaves while another reads its sums
+  }
+
+  __syncwarp();
+  if (*abort_flag != 0) {
+    for (int k = 0; k < 200; ++k) __nanosleep(1000);
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  // (a key row's gradients were written by threads of this block, before the barrier)
+  if (warp >= 2)
+    for (int r = warp - 2; r < kBQ; r += kKvmThreads / 32 - 2)
+      if (bad[r] != 0) mattn::dkv_row<__nv_bfloat16>(c, b, hk, kb * kBQ + r);
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(256u) : "memory");
   }
 }
 
@@ -1697,7 +1935,7 @@ int attention_bwd(const void* q, const void* k, const void* v, const void* o, co
   MCB_CHECK_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) return fail(MCB_ERR_SHAPE, "attention: device %d out of range", dev);
   if (int rc = set_attrs_once(reinterpret_cast<const void*>(attn_dq_kernel), kDqSmem, &attr_dq[dev])) return rc;
-  if (int rc = set_attrs_once(reinterpret_cast<const void*>(attn_dkv_kernel<false, false, false>), kKvSmem, &attr_kv[dev])) return rc;
+  if (int rc = set_attrs_once(reinterpret_cast<const void*>(attn_dkv_kernel), kKvSmem, &attr_kv[dev])) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const size_t rows = static_cast<size_t>(nb) * groups * q_blocks(static_cast<int>(seq)) * kBQ * 4;
   uint8_t* w = static_cast<uint8_t*>(workspace);
@@ -1740,7 +1978,7 @@ int attention_bwd(const void* q, const void* k, const void* v, const void* o, co
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = static_cast<unsigned>(p.kv_parts); attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr; cfg.numAttrs = p.kv_parts > 1 ? 2 : 1;
-  MCB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attn_dkv_kernel<false, false, false>, tmK128, tmV128, tmQ64, tmdO64, p, NoCall()));
+  MCB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attn_dkv_kernel, tmK128, tmV128, tmQ64, tmdO64, p));
   MCB_CHECK_LAUNCH("attn_dkv_kernel");
   return MCB_OK;
 }
@@ -1783,7 +2021,7 @@ template <bool CAP, bool BIAS>
 struct Form {
   static constexpr auto fwd = attn_fwd_kernel<true, CAP, BIAS>;
   static constexpr auto dq = attn_dq_masked_kernel<CAP, BIAS>;
-  static constexpr auto dkv = attn_dkv_kernel<true, CAP, BIAS>;
+  static constexpr auto dkv = attn_dkv_masked_kernel<CAP, BIAS>;
   static int prepare(int dev) {
     static bool done[3][64] = {};
     if (int rc = set_attrs_once(reinterpret_cast<const void*>(fwd), kFwdSmem, &done[0][dev])) return rc;
@@ -1846,7 +2084,7 @@ int bwd_form(const Call& c, const DeviceState* ds, cudaStream_t st) {
   p.kv_parts = dkv_parts(nb, c.G, c.S, ds->sm_count);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(nb * q_blocks(c.S) * p.kv_parts));
-  cfg.blockDim = dim3(kKvThreads);
+  cfg.blockDim = dim3(kKvmThreads);
   cfg.dynamicSmemBytes = kKvSmem; cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1855,7 +2093,7 @@ int bwd_form(const Call& c, const DeviceState* ds, cudaStream_t st) {
   attr[1].val.clusterDim.x = static_cast<unsigned>(p.kv_parts); attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr; cfg.numAttrs = p.kv_parts > 1 ? 2 : 1;
   MCB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, Form<CAP, BIAS>::dkv, tmK128, tmV128, tmQ64, tmdO64, p, c));
-  MCB_CHECK_LAUNCH("attn_dkv_kernel");
+  MCB_CHECK_LAUNCH("attn_dkv_masked_kernel");
   return MCB_OK;
 }
 
