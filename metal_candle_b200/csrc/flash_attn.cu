@@ -326,59 +326,66 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       }
     }
   } else if (warp == 1) {
-    if (elect_one()) {
-      const uint32_t idesc = make_idesc(kBK);  // M = 128, N = 64 for both products
-      bool ok = true;
-      int it = -1;
-      uint32_t n0 = 0;            // running number of this item's block 0
-      int sst = 0;                // ring stage and phase of the next block to get its S product
-      uint32_t sph = 0;
-      int pst = 0;                // ring stage of the next block to get its P V product
-      // S_j = Q K_j^T for block j of the current item (running number n) into tensor-memory buffer n & 1; the
-      // buffer is free once the softmax warps have read block n - 2 into registers (s_free)
-      auto issue_s = [&](uint32_t n, bool last) -> bool {
-        if (n >= 2 && !mbar_wait(s_free0 + 8 * (n & 1), ((n - 2) >> 1) & 1, abort_flag, 70, p.status)) return false;
-        if (!mbar_wait(kv_full0 + 8 * sst, sph, abort_flag, 75, p.status)) return false;
-        tcgen05_fence_after();
-        const uint32_t tS = tmem_base + (n & 1) * 64;
+    // The whole warp walks through the blocks and waits; one lane issues.  Only so do the operands of an MMA stay the warp's own (uniform registers),
+    // and an MMA of 32 to 64 cycles is not issued in 100: FWDUS
+    const uint32_t idesc = make_idesc(kBK);  // M = 128, N = 64 for both products
+    auto wait = [&](uint32_t bar, uint32_t parity, int code) -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, code, p.status));
+    };
+    bool ok = true;
+    int it = -1;
+    uint32_t n0 = 0;            // running number of this item's block 0
+    int sst = 0;                // ring stage and phase of the next block to get its S product
+    uint32_t sph = 0;
+    int pst = 0;                // ring stage of the next block to get its P V product
+    // S_j = Q K_j^T for block j of the current item (running number n) into tensor-memory buffer n & 1; the
+    // buffer is free once the softmax warps have read block n - 2 into registers (s_free)
+    auto issue_s = [&](uint32_t n, bool last) -> bool {
+      if (n >= 2 && !wait(s_free0 + 8 * (n & 1), ((n - 2) >> 1) & 1, 70)) return false;
+      if (!wait(kv_full0 + 8 * sst, sph, 75)) return false;
+      tcgen05_fence_after();
+      const uint32_t tS = tmem_base + (n & 1) * 64;
+      const uint64_t dQ = desc_sw128(base + kOffQ), dK = desc_sw128(base + kOffK + sst * kKBytes);
+      if (elect_one()) {
 #pragma unroll
-        for (int k4 = 0; k4 < kD / 16; ++k4)
-          umma_bf16(tS, desc_sw128(base + kOffQ + k4 * 32), desc_sw128(base + kOffK + sst * kKBytes + k4 * 32), idesc,
-                    k4 != 0 ? 1u : 0u);
+        for (int k4 = 0; k4 < kD / 16; ++k4) umma_bf16(tS, desc_advance(dQ, k4 * 32), desc_advance(dK, k4 * 32), idesc, k4 != 0 ? 1u : 0u);
         umma_commit(s_full0 + 8 * (n & 1));
         if (last) umma_commit(q_free);   // Q may be replaced by the next item's
-        if (++sst == kFwdStages) { sst = 0; sph ^= 1; }
-        return true;
-      };
-      while (ok && walk.get(w)) {
-        if (MASKED && w.nkb == 0) continue;
-        ++it;
-        ok = mbar_wait(q_full, it & 1, abort_flag, 72, p.status);
-        for (int j = 0; ok && j < 2 && j < w.nkb; ++j) ok = issue_s(n0 + j, j == w.nkb - 1);
-        for (int j = 0; ok && j < w.nkb; ++j) {
-          const uint32_t n = n0 + j;
-          if (j + 2 < w.nkb) {
-            ok = issue_s(n + 2, j + 2 == w.nkb - 1);
-            if (!ok) break;
-          }
-          ok = mbar_wait(p_ready0 + 8 * (n & 1), (n >> 1) & 1, abort_flag, 74, p.status);
-          // the first product of an item overwrites O: the previous item's write-out must have read it
-          if (ok && j == 0 && it > 0) ok = mbar_wait(o_free, (it - 1) & 1, abort_flag, 68, p.status);
+      }
+      __syncwarp();
+      if (++sst == kFwdStages) { sst = 0; sph ^= 1; }
+      return true;
+    };
+    while (ok && walk.get(w)) {
+      if (MASKED && w.nkb == 0) continue;
+      ++it;
+      ok = wait(q_full, it & 1, 72);
+      for (int j = 0; ok && j < 2 && j < w.nkb; ++j) ok = issue_s(n0 + j, j == w.nkb - 1);
+      for (int j = 0; ok && j < w.nkb; ++j) {
+        const uint32_t n = n0 + j;
+        if (j + 2 < w.nkb) {
+          ok = issue_s(n + 2, j + 2 == w.nkb - 1);
           if (!ok) break;
-          tcgen05_fence_after();
-          // O += P_j V_j   (A = P [128 x 64 keys] in tensor memory, 16 keys = 8 columns; B = the V tile as it lies,
-          // [64 keys x 64 d]: N-major, 16 keys further = two 8-row groups of 1024 bytes)
+        }
+        ok = wait(p_ready0 + 8 * (n & 1), (n >> 1) & 1, 74);
+        // the first product of an item overwrites O: the previous item's write-out must have read it
+        if (ok && j == 0 && it > 0) ok = wait(o_free, (it - 1) & 1, 68);
+        if (!ok) break;
+        tcgen05_fence_after();
+        // O += P_j V_j   (A = P [128 x 64 keys] in tensor memory, 16 keys = 8 columns; B = the V tile as it lies,
+        // [64 keys x 64 d]: N-major, 16 keys further = two 8-row groups of 1024 bytes)
+        const uint64_t dV = desc_sw128_mn(base + kOffV + pst * kKBytes, kKBytes, 1024);
+        const uint32_t tP = tP0 + (n & 1) * 32, acc = j != 0 ? 1u : 0u;
+        if (elect_one()) {
 #pragma unroll
-          for (int k4 = 0; k4 < kBK / 16; ++k4)
-            umma_bf16_ts(tO, tP0 + (n & 1) * 32 + k4 * 8,
-                         desc_sw128_mn(base + kOffV + pst * kKBytes + k4 * 2048, kKBytes, 1024), idesc | (1u << 16),
-                         (j | k4) != 0 ? 1u : 0u);
+          for (int k4 = 0; k4 < kBK / 16; ++k4) umma_bf16_ts(tO, tP + k4 * 8, desc_advance(dV, k4 * 2048), idesc | (1u << 16), k4 != 0 ? 1u : acc);
           umma_commit(pv_done0 + 8 * (n & 1));
           umma_commit(kv_empty0 + 8 * pst);
-          if (++pst == kFwdStages) pst = 0;
         }
-        n0 += static_cast<uint32_t>(w.nkb);
+        __syncwarp();
+        if (++pst == kFwdStages) pst = 0;
       }
+      n0 += static_cast<uint32_t>(w.nkb);
     }
   } else {
     // ---------------- online softmax, one query row per thread ----------------
@@ -950,71 +957,79 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
       }
     }
   } else if (warp == 1) {
-    if (elect_one()) {
-      const uint32_t idesc = make_idesc(kBK);
-      bool ok = true;
-      int it = -1;
-      uint32_t n = 0;             // running number of the block that gets its second sum and dQ
-      int sst = 0, dst = 0;       // ring stage of the next block to get its S product, and of block n
-      uint32_t sph = 0;
-      // S of the item's next block: the product that read the P t written over it was issued before this point
-      auto issue_s = [&]() -> bool {
-        if (!mbar_wait(kv_full0 + 8 * sst, sph, abort_flag, 83, p.status)) return false;
-        tcgen05_fence_after();
-        const uint32_t sb = base + kDqOffStage + sst * kDqStageBytes;
+    // (the whole warp walks and waits, one lane issues: see the forward)
+    const uint32_t idesc = make_idesc(kBK);
+    auto wait = [&](uint32_t bar, uint32_t parity, int code) -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, code, p.status));
+    };
+    bool ok = true;
+    int it = -1;
+    uint32_t n = 0;             // running number of the block that gets its second sum and dQ
+    int sst = 0, dst = 0;       // ring stage of the next block to get its S product, and of block n
+    uint32_t sph = 0;
+    const uint64_t dQ = desc_sw128(base + kDqOffQ), dO = desc_sw128(base + kDqOffDO);
+    // S of the item's next block: the product that read the P t written over it was issued before this point
+    auto issue_s = [&]() -> bool {
+      if (!wait(kv_full0 + 8 * sst, sph, 83)) return false;
+      tcgen05_fence_after();
+      const uint64_t dK = desc_sw128(base + kDqOffStage + sst * kDqStageBytes);
+      if (elect_one()) {
 #pragma unroll
-        for (int k4 = 0; k4 < kD / 16; ++k4)
-          umma_bf16(tS, desc_sw128(base + kDqOffQ + k4 * 32), desc_sw128(sb + k4 * 32), idesc, k4 != 0 ? 1u : 0u);
+        for (int k4 = 0; k4 < kD / 16; ++k4) umma_bf16(tS, desc_advance(dQ, k4 * 32), desc_advance(dK, k4 * 32), idesc, k4 != 0 ? 1u : 0u);
         umma_commit(s_full);
-        if (++sst == kDqStages) { sst = 0; sph ^= 1; }
-        return true;
-      };
-      // dP of the block in ring stage st; its V tile arrived with the K tile that S has waited for
-      auto issue_dp = [&](int st) {
-        const uint32_t sb = base + kDqOffStage + st * kDqStageBytes;
+      }
+      __syncwarp();
+      if (++sst == kDqStages) { sst = 0; sph ^= 1; }
+      return true;
+    };
+    // dP of the block in ring stage st; its V tile arrived with the K tile that S has waited for
+    auto issue_dp = [&](int st, bool last) {
+      const uint64_t dV = desc_sw128(base + kDqOffStage + st * kDqStageBytes + kKBytes);
+      if (elect_one()) {
 #pragma unroll
-        for (int k4 = 0; k4 < kD / 16; ++k4)
-          umma_bf16(tDP, desc_sw128(base + kDqOffDO + k4 * 32), desc_sw128(sb + kKBytes + k4 * 32), idesc, k4 != 0 ? 1u : 0u);
+        for (int k4 = 0; k4 < kD / 16; ++k4) umma_bf16(tDP, desc_advance(dO, k4 * 32), desc_advance(dV, k4 * 32), idesc, k4 != 0 ? 1u : 0u);
         umma_commit(dp_full);
-      };
-      while (ok && walk.get(w)) {
-        if (w.nkb == 0) continue;
-        ++it;
-        ok = mbar_wait(q_full, it & 1, abort_flag, 84, p.status) && issue_s();
+        if (last) umma_commit(q_free);   // Q and dO may be replaced by the next item's
+      }
+      __syncwarp();
+    };
+    while (ok && walk.get(w)) {
+      if (w.nkb == 0) continue;
+      ++it;
+      ok = wait(q_full, it & 1, 84) && issue_s();
+      if (!ok) break;
+      issue_dp(dst, w.nkb == 1);
+      for (int j = 0; ok && j < w.nkb; ++j, ++n) {
+        const uint64_t dKn = desc_sw128_mn(base + kDqOffStage + dst * kDqStageBytes, kKBytes, 1024);
+        const uint32_t acc = j != 0 ? 1u : 0u;
+        ok = wait(p_ready, n & 1, 82);
+        // the first products of an item overwrite both sums: the previous item's write-out must have read them
+        if (ok && j == 0 && it > 0) ok = wait(dq_free, (it - 1) & 1, 87);
         if (!ok) break;
-        issue_dp(dst);
-        if (w.nkb == 1) umma_commit(q_free);
-        for (int j = 0; ok && j < w.nkb; ++j, ++n) {
-          const uint32_t sb = base + kDqOffStage + dst * kDqStageBytes;
-          ok = mbar_wait(p_ready, n & 1, abort_flag, 82, p.status);
-          // the first products of an item overwrite both sums: the previous item's write-out must have read them
-          if (ok && j == 0 && it > 0) ok = mbar_wait(dq_free, (it - 1) & 1, abort_flag, 87, p.status);
-          if (!ok) break;
-          tcgen05_fence_after();
-          // second sum += (P t)_j K_j   (A = [128 x 64 keys] in tensor memory; B = the K tile as it lies: N-major)
+        tcgen05_fence_after();
+        // second sum += (P t)_j K_j   (A = [128 x 64 keys] in tensor memory; B = the K tile as it lies: N-major)
+        if (elect_one()) {
 #pragma unroll
-          for (int k4 = 0; k4 < kBK / 16; ++k4)
-            umma_bf16_ts(tPK, tS + k4 * 8, desc_sw128_mn(sb + k4 * 2048, kKBytes, 1024), idesc | (1u << 16), (j | k4) != 0 ? 1u : 0u);
-          if (j + 1 < w.nkb) {
-            ok = issue_s();
-            if (!ok) break;
-          }
-          ok = mbar_wait(ds_ready, n & 1, abort_flag, 86, p.status);
-          if (!ok) break;
-          tcgen05_fence_after();
-          // dQ += dS_j K_j
-#pragma unroll
-          for (int k4 = 0; k4 < kBK / 16; ++k4)
-            umma_bf16_ts(tDQ, tDP + k4 * 8, desc_sw128_mn(sb + k4 * 2048, kKBytes, 1024), idesc | (1u << 16), (j | k4) != 0 ? 1u : 0u);
-          umma_commit(kv_empty0 + 8 * dst);
-          if (++dst == kDqStages) dst = 0;
-          if (j + 1 < w.nkb) {
-            issue_dp(dst);
-            if (j + 2 == w.nkb) umma_commit(q_free);   // Q and dO may be replaced by the next item's
-          } else {
-            umma_commit(dq_full);
-          }
+          for (int k4 = 0; k4 < kBK / 16; ++k4) umma_bf16_ts(tPK, tS + k4 * 8, desc_advance(dKn, k4 * 2048), idesc | (1u << 16), k4 != 0 ? 1u : acc);
         }
+        __syncwarp();
+        if (j + 1 < w.nkb) {
+          ok = issue_s();
+          if (!ok) break;
+        }
+        ok = wait(ds_ready, n & 1, 86);
+        if (!ok) break;
+        tcgen05_fence_after();
+        // dQ += dS_j K_j
+        if (elect_one()) {
+#pragma unroll
+          for (int k4 = 0; k4 < kBK / 16; ++k4) umma_bf16_ts(tDQ, tDP + k4 * 8, desc_advance(dKn, k4 * 2048), idesc | (1u << 16), k4 != 0 ? 1u : acc);
+          umma_commit(kv_empty0 + 8 * dst);
+          if (j + 1 == w.nkb) umma_commit(dq_full);
+        }
+        __syncwarp();
+        if (++dst == kDqStages) dst = 0;
+        if (j + 1 < w.nkb) issue_dp(dst, j + 2 == w.nkb);
       }
     }
   } else {
@@ -1554,60 +1569,72 @@ attn_dkv_masked_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
       }
     }
   } else if (warp == 1) {
-    if (elect_one()) {
-      const uint32_t idesc = make_idesc(kBK);
-      const uint64_t dK = desc_sw128(base + kKvOffK), dV = desc_sw128(base + kKvOffV);
-      const uint64_t dQk = desc_sw128(base + kKvOffStage), dQn = desc_sw128_mn(base + kKvOffStage, kKBytes, 1024);
-      // S^T = K Q^T of the step in ring stage st, and dP^T = V dO^T
-      auto issue_s = [&](int st) {
-        const uint32_t so = static_cast<uint32_t>(st) * kKvStageStride;
+    // (the whole warp walks and waits, one lane issues: see the forward)
+    const uint32_t idesc = make_idesc(kBK);
+    auto wait = [&](uint32_t bar, uint32_t parity, int code) -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, code, p.status));
+    };
+    const uint64_t dK = desc_sw128(base + kKvOffK), dV = desc_sw128(base + kKvOffV);
+    const uint64_t dQk = desc_sw128(base + kKvOffStage), dQn = desc_sw128_mn(base + kKvOffStage, kKBytes, 1024);
+    // S^T = K Q^T of the step in ring stage st, and dP^T = V dO^T
+    auto issue_s = [&](int st) {
+      const uint64_t dQ = desc_advance(dQk, static_cast<uint32_t>(st) * kKvStageStride);
+      if (elect_one()) {
 #pragma unroll
-        for (int k4 = 0; k4 < kD / 16; ++k4)
-          umma_bf16(tS, desc_advance(dK, k4 * 32), desc_advance(dQk, so + k4 * 32), idesc, k4 != 0 ? 1u : 0u);
+        for (int k4 = 0; k4 < kD / 16; ++k4) umma_bf16(tS, desc_advance(dK, k4 * 32), desc_advance(dQ, k4 * 32), idesc, k4 != 0 ? 1u : 0u);
         umma_commit(s_full);
-      };
-      auto issue_dp = [&](int st) {
-        const uint32_t so = static_cast<uint32_t>(st) * kKvStageStride + kKBytes;
+      }
+      __syncwarp();
+    };
+    auto issue_dp = [&](int st) {
+      const uint64_t dO = desc_advance(dQk, static_cast<uint32_t>(st) * kKvStageStride + kKBytes);
+      if (elect_one()) {
 #pragma unroll
-        for (int k4 = 0; k4 < kD / 16; ++k4)
-          umma_bf16(tDP, desc_advance(dV, k4 * 32), desc_advance(dQk, so + k4 * 32), idesc, k4 != 0 ? 1u : 0u);
+        for (int k4 = 0; k4 < kD / 16; ++k4) umma_bf16(tDP, desc_advance(dV, k4 * 32), desc_advance(dO, k4 * 32), idesc, k4 != 0 ? 1u : 0u);
         umma_commit(dp_full);
-      };
-      bool ok = nsteps > 0 && mbar_wait(kv_full, 0, abort_flag, 92, p.status) && mbar_wait(ld_full0, 0, abort_flag, 93, p.status);
-      if (ok) {
-        tcgen05_fence_after();
-        issue_s(0);
-        issue_dp(0);
       }
-      for (int t = 0; ok && t < nsteps; ++t) {
-        const int st = t % kKvStages, next = (t + 1) % kKvStages;
-        const uint32_t so = static_cast<uint32_t>(st) * kKvStageStride;
-        const uint32_t acc = t != 0 ? 1u : 0u;
-        ok = mbar_wait(p_ready, t & 1, abort_flag, 94, p.status);
-        if (!ok) break;
-        tcgen05_fence_after();
-        // dV += P^T dO   (A = P^T [128 keys x 64 queries] in tensor memory, 16 queries = 8 columns, the second 32 queries 32 columns on; B =
-        // the dO tile as it lies, [64 queries x 64 d]: N-major, 16 queries further = two 8-row groups of 1024 bytes)
+      __syncwarp();
+    };
+    bool ok = nsteps > 0 && wait(kv_full, 0, 92) && wait(ld_full0, 0, 93);
+    if (ok) {
+      tcgen05_fence_after();
+      issue_s(0);
+      issue_dp(0);
+    }
+    for (int t = 0; ok && t < nsteps; ++t) {
+      const int st = t % kKvStages, next = (t + 1) % kKvStages;
+      const uint64_t dQ = desc_advance(dQn, static_cast<uint32_t>(st) * kKvStageStride), dO = desc_advance(dQ, kKBytes);
+      const uint32_t acc = t != 0 ? 1u : 0u;
+      ok = wait(p_ready, t & 1, 94);
+      if (!ok) break;
+      tcgen05_fence_after();
+      // dV += P^T dO   (A = P^T [128 keys x 64 queries] in tensor memory, 16 queries = 8 columns, the second 32 queries 32 columns on; B =
+      // the dO tile as it lies, [64 queries x 64 d]: N-major, 16 queries further = two 8-row groups of 1024 bytes)
+      if (elect_one()) {
 #pragma unroll
         for (int k4 = 0; k4 < kBK / 16; ++k4)
-          umma_bf16_ts(tDV, tS + (k4 >> 1) * 32 + (k4 & 1) * 8, desc_advance(dQn, so + kKBytes + k4 * 2048), idesc | (1u << 16), k4 != 0 ? 1u : acc);
-        if (t + 1 < nsteps) {
-          ok = mbar_wait(ld_full0 + 8 * next, ((t + 1) / kKvStages) & 1, abort_flag, 93, p.status);
-          if (!ok) break;
-          tcgen05_fence_after();
-          issue_s(next);
-        }
-        ok = mbar_wait(ds_ready, t & 1, abort_flag, 95, p.status);
+          umma_bf16_ts(tDV, tS + (k4 >> 1) * 32 + (k4 & 1) * 8, desc_advance(dO, k4 * 2048), idesc | (1u << 16), k4 != 0 ? 1u : acc);
+      }
+      __syncwarp();
+      if (t + 1 < nsteps) {
+        ok = wait(ld_full0 + 8 * next, ((t + 1) / kKvStages) & 1, 93);
         if (!ok) break;
         tcgen05_fence_after();
-        // dK += dS^T Q
+        issue_s(next);
+      }
+      ok = wait(ds_ready, t & 1, 95);
+      if (!ok) break;
+      tcgen05_fence_after();
+      // dK += dS^T Q
+      if (elect_one()) {
 #pragma unroll
         for (int k4 = 0; k4 < kBK / 16; ++k4)
-          umma_bf16_ts(tDK, tDP + (k4 >> 1) * 32 + (k4 & 1) * 8, desc_advance(dQn, so + k4 * 2048), idesc | (1u << 16), k4 != 0 ? 1u : acc);
+          umma_bf16_ts(tDK, tDP + (k4 >> 1) * 32 + (k4 & 1) * 8, desc_advance(dQ, k4 * 2048), idesc | (1u << 16), k4 != 0 ? 1u : acc);
         umma_commit(ld_empty0 + 8 * st);
-        if (t + 1 < nsteps) issue_dp(next);
-        else umma_commit(out_full);
+        if (t + 1 == nsteps) umma_commit(out_full);
       }
+      __syncwarp();
+      if (t + 1 < nsteps) issue_dp(next);
     }
   } else {
     const int quad = warp & 3;                // tensor-memory lane quadrant of this warp
@@ -1823,6 +1850,17 @@ int dkv_parts(int64_t nb, int64_t groups, int64_t seq, int sms) {
     if (i == 0 || t < best_t) { best = 1 << i; best_t = t; }
   }
   return best;
+}
+
+// The same under a mask, where a CTA starts under another's steps and the steps of a key block are not known here: parts until one and a half CTAs wait for
+// every place on the device, while a part is likely to have some steps.  Whole backward pass with 1 / 2 / 4 parts, us: 4 kv heads x 7
+// x 4096 positions in documents of 585: 262 / 174 / 127, one document: 796 / 486 / 321; 16 x 7 x 2048 of 400: 285 / 204 / 202; 32 x 2 x 1024, capped:
+// 160 / 130 / 147; 36 x 1 x 777 of 240: 44 / 48 / 63; 48 x 1 x 1024 of 340: 48 / 67 / 91.
+int masked_dkv_parts(int64_t nb, int64_t groups, int64_t seq, int sms) {
+  const int64_t items = nb * q_blocks(static_cast<int>(seq)), steps = (seq + kBK - 1) / kBK, most = groups * (steps < 16 ? 1 : steps / 16);
+  int parts = 1;
+  while (parts < 8 && items * parts < 3ll * sms && 2 * parts <= most) parts *= 2;
+  return parts;
 }
 
 }  // namespace
@@ -2081,7 +2119,7 @@ int bwd_form(const Call& c, const DeviceState* ds, cudaStream_t st) {
   MCB_CHECK_CUDA(launch_kernel(Form<CAP, BIAS>::dq, dim3(static_cast<unsigned>(n_tiles < slots ? n_tiles : slots)), dim3(attn::kThreads), kDqSmem, st,
                                chained_launch(), tmQ128, tmdO128, tmK64, tmV64, p, c));
   MCB_CHECK_LAUNCH("attn_dq_masked_kernel");
-  p.kv_parts = dkv_parts(nb, c.G, c.S, ds->sm_count);
+  p.kv_parts = masked_dkv_parts(nb, c.G, c.S, ds->sm_count);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(nb * q_blocks(c.S) * p.kv_parts));
   cfg.blockDim = dim3(kKvmThreads);
