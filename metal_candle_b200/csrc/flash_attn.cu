@@ -76,7 +76,8 @@ constexpr int kFwdStages = 4;                         // K / V ring: a load has 
 constexpr uint32_t kOffK = kOffQ + kQBytes;
 constexpr uint32_t kOffV = kOffK + kFwdStages * kKBytes;
 constexpr uint32_t kOffBar = kOffV + kFwdStages * kKBytes;
-constexpr uint32_t kFwdSmem = kOffBar + 256 + 1024;
+constexpr uint32_t kOffAnswers = kOffBar + 256;       // of the item requests (see Answers): two of 16 bytes, then their barriers
+constexpr uint32_t kFwdSmem = kOffAnswers + 64 + 1024;
 
 struct FwdParams {
   int S, G, NB;
@@ -203,38 +204,99 @@ __device__ __forceinline__ FwdTile fwd_tile(const FwdParams& p, int t) {
   return w;
 }
 
-// A CTA's items one after the other.  Under a mask they come from the sorted list, there and back again over the CTAs (the first of
-// one round is the last of the next), each record asked for an item ahead: it would be a trip to L2 in front of every item.
+// ---- a CTA's items one after the other ----
+// Without a mask: item t, t + gridDim, ..  Under one the tiles' lengths differ too much to be dealt out beforehand (documents of 585: 40 % between the
+// longest CTA and the mean): the grid has a CTA for every item, the longest first, and those that run take over items of CTAs that have not started
+// (cluster launch control).  A request's answer lies in shared memory, two by turns, with a barrier that it
+// completes and one on which all readers let go of it: the loading thread, the MMA warp and four softmax warps.
+struct Answers {
+  uint32_t full0, empty0, at0;   // two barriers each; two answers of 16 bytes
+};
+constexpr uint32_t kAnswerReaders = 6;
+__device__ __forceinline__ void request_item(uint32_t answer, uint32_t bar) {
+  mbar_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
+}
+// the item that was taken over, or -1: none is left
+__device__ __forceinline__ int read_answer(uint32_t answer) {
+  uint32_t got, x, y, z;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
+      "ld.shared.b128 r, [%4];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, %3, _}, r;\n\t}"
+      : "=r"(got), "=r"(x), "=r"(y), "=r"(z)
+      : "r"(answer)
+      : "memory");
+  return got ? static_cast<int>(x) : -1;
+}
+
 template <bool MASKED>
-struct Walk {
+struct Walk;
+template <>
+struct Walk<false> {
   const FwdParams& p;
-  const CallOf<MASKED>& c;
-  int t, n, round;
-  int4 next;
-  __device__ __forceinline__ Walk(const FwdParams& p_, const CallOf<MASKED>& c_) : p(p_), c(c_), t(blockIdx.x), round(0) {
-    if constexpr (MASKED) {
-      n = q_blocks(p.S) * c.B * p.G * c.Hk;
-      next = t < n ? c.mask.qwork[t / (p.G * c.Hk)] : make_int4(0, 0, 0, 0);
-    } else {
-      n = q_blocks(p.S) * p.G * p.NB;
-    }
-  }
+  int t, n;
+  __device__ __forceinline__ Walk(const FwdParams& p_, const NoCall&, const Answers&, volatile int*) : p(p_), t(blockIdx.x), n(q_blocks(p_.S) * p_.G * p_.NB) {}
+  __device__ __forceinline__ bool get_as_loader(FwdTile& w) { return get(w); }
   __device__ __forceinline__ bool get(FwdTile& w) {
     if (t >= n) return false;
-    if constexpr (MASKED) {
-      const int heads = p.G * c.Hk, r = t % heads;
-      w.b = next.x; w.qb = next.y; w.kb0 = next.z; w.nkb = next.w;
-      w.hk = r / p.G; w.g = r % p.G;
-      w.nb = w.b * c.Hk + w.hk;
-      w.qrow0 = (static_cast<int64_t>(w.nb) * p.G + w.g) * p.S + static_cast<int64_t>(w.qb) * kBQ;
-      ++round;
-      const int64_t to = static_cast<int64_t>(round) * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-      t = to < n ? static_cast<int>(to) : n;
-      if (t < n) next = c.mask.qwork[t / heads];
-    } else {
-      w = fwd_tile(p, t);
-      t += gridDim.x;
+    w = fwd_tile(p, t);
+    t += gridDim.x;
+    return true;
+  }
+};
+template <>
+struct Walk<true> {
+  const FwdParams& p;
+  const mattn::Call& c;
+  const Answers ans;
+  volatile int* abort_flag;
+  int t, k;      // item, and how many came before it
+  int4 rec;      // its record
+  __device__ __forceinline__ Walk(const FwdParams& p_, const mattn::Call& c_, const Answers& a, volatile int* abort)
+      : p(p_), c(c_), ans(a), abort_flag(abort), t(blockIdx.x), k(0), rec(c_.mask.qwork[blockIdx.x / (p_.G * c_.Hk)]) {}
+  __device__ __forceinline__ void fill(FwdTile& w) const {
+    const int r = t % (p.G * c.Hk);
+    w.b = rec.x; w.qb = rec.y; w.kb0 = rec.z; w.nkb = rec.w;
+    w.hk = r / p.G; w.g = r % p.G;
+    w.nb = w.b * c.Hk + w.hk;
+    w.qrow0 = (static_cast<int64_t>(w.nb) * p.G + w.g) * p.S + static_cast<int64_t>(w.qb) * kBQ;
+  }
+  // answer k >= 1 is number (k - 1) / 2 in its place
+  __device__ __forceinline__ bool arrived(int n) const { return mbar_wait(ans.full0 + 8 * (n & 1), ((n - 1) >> 1) & 1, abort_flag, 99, c.status); }
+  // by one thread: its next item.  Asked for when the loads of the one before are on their way, some blocks ahead of their use, and no sooner: a CTA that
+  // asks as it starts takes over items whose CTAs would have started beside it (64 x 2 heads of 1024 positions, forward: 45 us, asked at the start 58)
+  __device__ __forceinline__ bool get_as_loader(FwdTile& w) {
+    if (k > 0) {
+      if (k >= 3 && !mbar_wait(ans.empty0 + 8 * (k & 1), ((k - 3) >> 1) & 1, abort_flag, 100, c.status)) return false;
+      request_item(ans.at0 + 16 * (k & 1), ans.full0 + 8 * (k & 1));
+      if (!arrived(k)) return false;
+      t = read_answer(ans.at0 + 16 * (k & 1));
+      fence_proxy_async_smem();
+      mbar_arrive(ans.empty0 + 8 * (k & 1));
+      if (t < 0) return false;
+      rec = c.mask.qwork[t / (p.G * c.Hk)];
     }
+    ++k;
+    fill(w);
+    return true;
+  }
+  // by a whole warp: its next item
+  __device__ __forceinline__ bool get(FwdTile& w) {
+    if (k > 0) {
+      if (!__all_sync(0xffffffffu, arrived(k))) return false;
+      t = read_answer(ans.at0 + 16 * (k & 1));
+      fence_proxy_async_smem();
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(ans.empty0 + 8 * (k & 1));
+      if (t < 0) return false;
+      rec = c.mask.qwork[t / (p.G * c.Hk)];
+    }
+    ++k;
+    fill(w);
     return true;
   }
 };
@@ -271,6 +333,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   const uint32_t kv_empty0 = kv_full0 + 8 * kFwdStages;
   const uint32_t s_full0 = kv_empty0 + 8 * kFwdStages, p_ready0 = s_full0 + 16, pv_done0 = p_ready0 + 16;
   const uint32_t s_free0 = pv_done0 + 16, tmem_slot = s_free0 + 16, abort_addr = tmem_slot + 4;
+  const Answers ans = {base + kOffAnswers + 32, base + kOffAnswers + 48, base + kOffAnswers};
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(gen_base + (tmem_slot - base));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_base + (abort_addr - base));
 
@@ -282,6 +345,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     for (int s = 0; s < 2; ++s) {
       mbar_init(s_full0 + 8 * s, 1); mbar_init(p_ready0 + 8 * s, 4); mbar_init(pv_done0 + 8 * s, 1); mbar_init(s_free0 + 8 * s, 4);
     }
+    if (MASKED)
+      for (int s = 0; s < 2; ++s) { mbar_init(ans.full0 + 8 * s, 1); mbar_init(ans.empty0 + 8 * s, kAnswerReaders); }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async_smem();
@@ -298,7 +363,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   grid_dependency_wait();   // the set-up above ran under the tail of the kernel before
   // S buffers at columns 0 and 64, O at 128, the two P buffers (bf16 pairs: 32 columns each) at 192 and 224
   const uint32_t tO = tmem_base + 128, tP0 = tmem_base + 192;
-  Walk<MASKED> walk(p, c);
+  Walk<MASKED> walk(p, c, ans, abort_flag);
   FwdTile w;
 
   if (warp == 0) {
@@ -307,7 +372,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       uint32_t ph = 0;
       bool ok = true;
       int it = -1;
-      while (ok && walk.get(w)) {
+      while (ok && walk.get_as_loader(w)) {
         if (MASKED && w.nkb == 0) continue;   // a tile that sees nothing: no loads, no products
         ++it;
         // the previous item's last S product has read Q
@@ -593,7 +658,8 @@ constexpr int kDqStages = 4;
 constexpr uint32_t kDqOffStage = kDqOffDO + kQBytes;     // stages of a K and a V tile (8 KB each)
 constexpr uint32_t kDqStageBytes = 2 * kKBytes;
 constexpr uint32_t kDqOffBar = kDqOffStage + kDqStages * kDqStageBytes;
-constexpr uint32_t kDqSmem = kDqOffBar + 256 + 1024;
+constexpr uint32_t kDqOffAnswers = kDqOffBar + 256;
+constexpr uint32_t kDqSmem = kDqOffAnswers + 64 + 1024;
 
 struct BwdParams {
   int S, G, NB;
@@ -895,6 +961,7 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   const uint32_t kv_full0 = dq_free + 8, kv_empty0 = kv_full0 + 8 * kDqStages;
   const uint32_t s_full = kv_empty0 + 8 * kDqStages, p_ready = s_full + 8;
   const uint32_t dp_full = p_ready + 8, ds_ready = dp_full + 8, tmem_slot = ds_ready + 8, abort_addr = tmem_slot + 4;
+  const Answers ans = {base + kDqOffAnswers + 32, base + kDqOffAnswers + 48, base + kDqOffAnswers};
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(gen_base + (tmem_slot - base));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_base + (abort_addr - base));
 
@@ -908,6 +975,7 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     mbar_init(p_ready, 4);
     mbar_init(dp_full, 1);
     mbar_init(ds_ready, 4);
+    for (int s = 0; s < 2; ++s) { mbar_init(ans.full0 + 8 * s, 1); mbar_init(ans.empty0 + 8 * s, kAnswerReaders); }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async_smem();
@@ -925,7 +993,7 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   const uint32_t tS = tmem_base, tDP = tmem_base + 64, tDQ = tmem_base + 128, tPK = tmem_base + 192;
   FwdParams tp;   // the item order of the forward
   tp.S = p.S; tp.G = p.G; tp.NB = p.NB;
-  Walk<true> walk(tp, c);
+  Walk<true> walk(tp, c, ans, abort_flag);
   FwdTile w;
 
   if (warp == 0) {
@@ -934,7 +1002,7 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
       uint32_t ph = 0;
       bool ok = true;
       int it = -1;
-      while (ok && walk.get(w)) {
+      while (ok && walk.get_as_loader(w)) {
         if (w.nkb == 0) continue;
         ++it;
         // the previous item's last S and dP products have read Q and dO
@@ -2083,8 +2151,8 @@ int fwd_form(const Call& c, const DeviceState* ds, cudaStream_t st) {
   p.S = c.S; p.G = c.G; p.NB = static_cast<int>(nb); p.HKV = c.Hk; p.o_tok = c.o_tok;
   p.sc = c.scale * attn::kLog2e;
   p.O = static_cast<__nv_bfloat16*>(c.o); p.lse = c.lse; p.status = ds->status_word;
-  const int64_t n_tiles = static_cast<int64_t>(q_blocks(c.S)) * c.G * nb, slots = 2 * static_cast<int64_t>(ds->sm_count);
-  MCB_CHECK_CUDA(launch_kernel(Form<CAP, BIAS>::fwd, dim3(static_cast<unsigned>(n_tiles < slots ? n_tiles : slots)), dim3(attn::kThreads), kFwdSmem, st,
+  const int64_t n_tiles = static_cast<int64_t>(q_blocks(c.S)) * c.G * nb;   // (those that run take over the rest, see Walk)
+  MCB_CHECK_CUDA(launch_kernel(Form<CAP, BIAS>::fwd, dim3(static_cast<unsigned>(n_tiles)), dim3(attn::kThreads), kFwdSmem, st,
                                chained_launch(), tmQ, tmK, tmV, p, c));
   MCB_CHECK_LAUNCH("attn_fwd_kernel");
   return MCB_OK;
@@ -2114,9 +2182,9 @@ int bwd_form(const Call& c, const DeviceState* ds, cudaStream_t st) {
   p.ndelta = c.ndelta; p.nlse2 = c.nlse2;
   p.dQ = static_cast<__nv_bfloat16*>(c.dq); p.dK = static_cast<__nv_bfloat16*>(c.dk); p.dV = static_cast<__nv_bfloat16*>(c.dv);
   p.status = ds->status_word;
-  const int64_t n_tiles = static_cast<int64_t>(q_blocks(c.S)) * c.G * nb, slots = 2 * static_cast<int64_t>(ds->sm_count);
+  const int64_t n_tiles = static_cast<int64_t>(q_blocks(c.S)) * c.G * nb;   // (those that run take over the rest, see Walk)
   p.kv_parts = 1;
-  MCB_CHECK_CUDA(launch_kernel(Form<CAP, BIAS>::dq, dim3(static_cast<unsigned>(n_tiles < slots ? n_tiles : slots)), dim3(attn::kThreads), kDqSmem, st,
+  MCB_CHECK_CUDA(launch_kernel(Form<CAP, BIAS>::dq, dim3(static_cast<unsigned>(n_tiles)), dim3(attn::kThreads), kDqSmem, st,
                                chained_launch(), tmQ128, tmdO128, tmK64, tmV64, p, c));
   MCB_CHECK_LAUNCH("attn_dq_masked_kernel");
   p.kv_parts = masked_dkv_parts(nb, c.G, c.S, ds->sm_count);
