@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(block_of(TPR)) ln_fwd_kernel(const Params p) {
 // After the mean one more round of sums does: of (x - mean)^2, of g and of g (x - mean), from which rstd and both means of the backward
 // formula follow.  SUMS: dw and db are asked for.
 template <typename T, int TPR, int K, bool SHIFT, bool SUMS>
-__global__ void __launch_bounds__(block_of(TPR)) ln_bwd_kernel(const Params p) {
+__global__ void __launch_bounds__(block_of(TPR), TPR == 256 ? 2 : 1) ln_bwd_kernel(const Params p) {
   extern __shared__ uint4 smem4[];
   using R = Rows<T, TPR, K, SHIFT>;
   constexpr int N = R::N;
@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(1024) ln_reduce_kernel(const float* part, int 
   part = from_here(part);
   float v = 0.0f;
   if (c < 2 * D)
-#pragma unroll 4
+#pragma unroll 8
     for (int i = strand; i < blocks; i += 32) v += part[static_cast<int64_t>(i) * 2 * D + c];
   s[strand][threadIdx.x & 31] = v;
   __syncthreads();

@@ -106,8 +106,11 @@ class _LayerCalls:
         self.model, self.batch, self.seq, self.backward = model, batch, seq, backward
         self.cfg = ctypes.byref(_lib.QwenConfig(c.vocab_size, c.hidden_size, c.intermediate_size, c.num_hidden_layers,
                                                 c.num_attention_heads, c.num_key_value_heads, c.rms_norm_eps, c.rope_theta))
-        # what the library's layer takes; other models and settings run kernel by kernel
-        self.usable = (model.dtype == torch.bfloat16 and c.head_dim == 64 and c.intermediate_size % 8 == 0 and c.vocab_size % 8 == 0
+        mask = model._mask
+        if mask is not None and (mask.batch, mask.seq) != (batch, seq):
+            raise TrainingError(f"packed() was given documents of {mask.batch} x {mask.seq} positions, the batch has {batch} x {seq}")
+        # what the library's layer takes; other models and settings (and packed documents) run kernel by kernel
+        self.usable = (mask is None and model.dtype == torch.bfloat16 and c.head_dim == 64 and c.intermediate_size % 8 == 0 and c.vocab_size % 8 == 0
                        and model.fuse_swiglu_bwd)
         H, I = c.hidden_size, c.intermediate_size
         W3 = H + 2 * c.kv_size
@@ -212,6 +215,8 @@ class Qwen:
     """Random-init weights N(0, 0.02^2) for embedding and projections, norm weights 1, biases 0."""
 
     MODULES = ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj")
+
+    _mask: Optional[backend.AttentionMask] = None   # of the packed() block that is open
 
     def __init__(self, config: ModelConfig, device, dtype=torch.bfloat16, seed: int = 0):
         config.validate()
@@ -411,6 +416,10 @@ class Qwen:
         dtypes and head sizes materialise the probabilities P as the reference does."""
         c = self.config
         Hk, G, d = c.num_key_value_heads, c.num_attention_heads // c.num_key_value_heads, c.head_dim
+        if self._mask is not None:
+            O, lse = backend.attention_masked_forward(Qr.view(B * Hk, G * S, d), Kr.view(B * Hk, S, d), Vr.view(B * Hk, S, d), G,
+                                                      1.0 / math.sqrt(d), self._mask, token_major=True)
+            return None, O, lse
         if backend.attention_ragged_supported(Qr):
             # the fused kernel writes its output token-major, [B*S, hidden]: the o_proj input as it is
             O, lse = backend.attention_causal_ragged_forward(Qr.view(B * Hk, G * S, d), Kr.view(B * Hk, S, d),
@@ -426,6 +435,9 @@ class Qwen:
     def _attention_bwd(self, Qr, Kr, Vr, P, O, lse, dO, B, S):
         c = self.config
         Hk, G, d = c.num_key_value_heads, c.num_attention_heads // c.num_key_value_heads, c.head_dim
+        if self._mask is not None:
+            return backend.attention_masked_backward(Qr.view(B * Hk, G * S, d), Kr.view(B * Hk, S, d), Vr.view(B * Hk, S, d), O, lse, dO, G,
+                                                     1.0 / math.sqrt(d), self._mask, token_major=True)
         if P is None:
             # fused: O and dO are token-major [B*S, hidden] (o_proj's input and its gradient as they are)
             return backend.attention_causal_ragged_backward(Qr.view(B * Hk, G * S, d), Kr.view(B * Hk, S, d),
@@ -584,6 +596,25 @@ class Qwen:
                 self.layer_done_hook(idx)
         if self.backward_done_hook is not None:
             self.backward_done_hook()
+
+    # -- several documents in a sequence --
+    @contextmanager
+    def packed(self, document_ids: torch.Tensor, prefix: Optional[torch.Tensor] = None):
+        """Within the `with` block the model's passes (`forward`, `forward_backward`, the post-training ones) take batches of packed
+        documents: document_ids [batch, seq] and prefix as `backend.attention_mask` takes them, so that no token sees another
+        document.  Rotary positions go on over the sequence, which scores do not depend on: they turn on differences.  The targets are the
+        caller's: the last token of a document has none.  Every batch has a block of its own; a pass cannot be captured within one."""
+        if document_ids.dim() != 2:
+            raise TrainingError(f"document_ids must be [batch, seq], got {list(document_ids.shape)}")
+        for t, what in ((document_ids, "document_ids"), (prefix, "prefix")):
+            if t is not None:
+                self._here(t, what)
+        before = self._mask
+        self._mask = backend.attention_mask(document_ids, prefix)
+        try:
+            yield self
+        finally:
+            self._mask = before
 
     # -- post-training losses: the same pass with another loss between the lm_head and its backward --
     @contextmanager
@@ -749,6 +780,8 @@ class Qwen:
         `pool` (another capture's `graph.pool()`) lets graphs that are never replayed concurrently share memory."""
         if self.lora_adapter is None:
             raise TrainingError("capture_forward_backward needs an adapter (apply_adapter)")
+        if self._mask is not None:
+            raise TrainingError("capture_forward_backward within packed(): the graph would read the mask after the block has let go of it")
         ids = torch.zeros(batch, seq, dtype=torch.int32, device=self.device)
         targets = torch.full((batch, seq), -1, dtype=torch.int32, device=self.device)
         hook, done_hook = self.layer_done_hook, self.backward_done_hook
