@@ -470,17 +470,20 @@ def _attention_backward(entry: str, q, k, v, o, lse, dout, groups: int, scale: f
 # attention under document and prefix masks
 # ---------------------------------------------------------------------------------------------
 
-def _on_device_of(t: torch.Tensor):
-    """A context that makes the tensor's device the current one (streams and launches go by it), or None where it is."""
-    if not t.is_cuda:
-        raise TrainingError("tensor is not on a CUDA device (this library has no CPU path)")
-    return None if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
-
-
-def _same_device(like: torch.Tensor, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != like.device:
-            raise TrainingError(f"{name} is on {t.device}, expected {like.device}")
+def _together(like: torch.Tensor, names: str, *tensors) -> int:
+    """The device index of `like`, which every tensor has to share (None: not given), all contiguous.  One look at each: a call of a few
+    microseconds notices two."""
+    index = like.get_device()
+    good = index >= 0 and like.is_contiguous()
+    for t in tensors:
+        if t is not None and (t.get_device() != index or not t.is_contiguous()):
+            good = False
+    if not good:
+        _require_cuda(like, *tensors)
+        for name, t in zip(names.split(), tensors):
+            if t is not None and t.device != like.device:
+                raise TrainingError(f"{name} is on {t.device}, expected {like.device}")
+    return index
 
 
 class AttentionMask:
@@ -513,7 +516,8 @@ def attention_mask(document_ids: torch.Tensor | None = None, prefix: torch.Tenso
             raise TrainingError(f"attention_mask: prefix is {prefix.dtype}, expected torch.bool or torch.uint8")
         if prefix.shape != (batch, seq):
             raise TrainingError(f"attention_mask: prefix must be [{batch}, {seq}], got {list(prefix.shape)}")
-        _same_device(given, prefix=prefix)
+        if prefix.device != given.device:
+            raise TrainingError(f"prefix is on {prefix.device}, expected {given.device}")
     device = torch.device(device)
     if device.type != "cuda":
         raise TrainingError("attention_mask: needs a CUDA device (this library has no CPU path)")
@@ -546,8 +550,7 @@ def _masked_call(q, k, v, groups: int, scale: float, mask: AttentionMask, softca
         raise TrainingError("masked attention: mask must come from attention_mask")
     if mask.seq != S or nb == 0 or nb % mask.batch != 0:
         raise TrainingError(f"masked attention: a mask of {mask.batch} x {mask.seq} positions does not fit k {list(k.shape)}")
-    _require_cuda(q, k, v, slopes)
-    _same_device(q, k=k, v=v, slopes=slopes, mask=mask.block)
+    _together(q, "k v slopes mask", k, v, slopes, mask.block)
     kv_heads = nb // mask.batch
     if slopes is not None and (slopes.shape != (kv_heads * groups,) or slopes.dtype != torch.float32):
         raise TrainingError(f"masked attention: slopes must be [{kv_heads * groups}] float32, got {list(slopes.shape)} {slopes.dtype}")
@@ -562,9 +565,8 @@ def attention_masked_forward(q, k, v, groups: int, scale: float, mask: Attention
     k and v [nb, S, d], nb = batch * kv_heads; float32 or bfloat16, d a multiple of 8 up to 128.  Returns (o, lse [nb, groups*S]
     float32); o like q, or token-major [batch*S, kv_heads*groups*d].  A position that sees nothing has o = 0 and lse = -inf."""
     call = _masked_call(q, k, v, groups, scale, mask, softcap, slopes, token_major)
-    other = _on_device_of(q)
-    if other is not None:
-        with other:
+    if q.get_device() != torch._C._cuda_getDevice():
+        with torch.cuda.device(q.device):
             return attention_masked_forward(q, k, v, groups, scale, mask, softcap, slopes, token_major)
     nb, S, d = k.shape
     o = torch.empty(mask.batch * S, nb // mask.batch * groups * d, dtype=q.dtype, device=q.device) if token_major else torch.empty_like(q)
@@ -584,11 +586,9 @@ def attention_masked_backward(q, k, v, o, lse, dout, groups: int, scale: float, 
         raise TrainingError(f"masked attention backward: o {list(o.shape)} {o.dtype} / dout {list(dout.shape)} {dout.dtype}, expected {list(want)} {q.dtype}")
     if tuple(lse.shape) != (nb, groups * S) or lse.dtype != torch.float32:
         raise TrainingError(f"masked attention backward: lse {list(lse.shape)} {lse.dtype}, expected [{nb}, {groups * S}] float32")
-    _require_cuda(o, lse, dout)
-    _same_device(q, o=o, lse=lse, dout=dout)
-    other = _on_device_of(q)
-    if other is not None:
-        with other:
+    _together(q, "o lse dout", o, lse, dout)
+    if q.get_device() != torch._C._cuda_getDevice():
+        with torch.cuda.device(q.device):
             return attention_masked_backward(q, k, v, o, lse, dout, groups, scale, mask, softcap, slopes, token_major)
     lib = _lib_for(q)
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
@@ -617,11 +617,8 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> tor
         raise TrainingError(f"embedding: table must be [vocab, hidden], got {list(table.shape)}")
     dt = _dtype_code(table)
     ids = ids.contiguous()
-    _require_cuda(ids, table)
-    _same_device(table, ids=ids)
-    other = _on_device_of(table)
-    if other is not None:
-        with other:
+    if _together(table, "ids", ids) != torch._C._cuda_getDevice():
+        with torch.cuda.device(table.device):
             return embedding(ids, table, scale)
     V, H = table.shape
     out = torch.empty(*ids.shape, H, dtype=table.dtype, device=table.device)
@@ -644,11 +641,8 @@ def embedding_backward(ids: torch.Tensor, dout: torch.Tensor, vocab: int, scale:
         raise TrainingError(f"embedding_backward: grad must be [{vocab}, {H}] float32, got {list(grad.shape)} {grad.dtype}")
     if accumulate and grad is None:
         raise TrainingError("embedding_backward: accumulate needs grad")
-    _require_cuda(ids, dout, grad)
-    _same_device(dout, ids=ids, grad=grad)
-    other = _on_device_of(dout)
-    if other is not None:
-        with other:
+    if _together(dout, "ids grad", ids, grad) != torch._C._cuda_getDevice():
+        with torch.cuda.device(dout.device):
             return embedding_backward(ids, dout, vocab, scale, grad, accumulate)
     if grad is None:
         grad = torch.empty(vocab, H, dtype=torch.float32, device=dout.device)
@@ -755,14 +749,12 @@ def layer_norm_fused(x: torch.Tensor, weight: torch.Tensor | None = None, bias: 
     mean and 1 / sqrt(var + eps) of every row."""
     rows, D = _rows(x, "LayerNormOp")
     dt = _dtype_code(x)
-    _require_cuda(x, weight, bias)
-    _same_device(x, weight=weight, bias=bias)
+    index = _together(x, "weight bias", weight, bias)
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None and (t.shape != (D,) or t.dtype != x.dtype):
             raise TrainingError(f"layer norm {name} must be [{D}] of {x.dtype}")
-    other = _on_device_of(x)
-    if other is not None:
-        with other:
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(x.device):
             return layer_norm_fused(x, weight, bias, eps, return_stats)
     y = torch.empty_like(x)
     mean, rstd = (torch.empty(rows, dtype=torch.float32, device=x.device) for _ in range(2)) if return_stats else (None, None)
@@ -777,8 +769,7 @@ def layer_norm_backward(x: torch.Tensor, weight: torch.Tensor | None, dy: torch.
     accumulate adds to grad_w and grad_b.  `dx_residual` (the gradient along the residual connection) is added to dx inside."""
     rows, D = _rows(x, "layer_norm_backward")
     dt = _dtype_code(x)
-    _require_cuda(x, weight, dy, grad_w, grad_b, dx_residual)
-    _same_device(x, weight=weight, dy=dy, grad_w=grad_w, grad_b=grad_b, dx_residual=dx_residual)
+    index = _together(x, "weight dy grad_w grad_b dx_residual", weight, dy, grad_w, grad_b, dx_residual)
     for name, t in (("dy", dy), ("dx_residual", dx_residual)):
         if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
             raise TrainingError(f"layer_norm_backward: {name} must be {list(x.shape)} of {x.dtype}, got {list(t.shape)} of {t.dtype}")
@@ -789,9 +780,8 @@ def layer_norm_backward(x: torch.Tensor, weight: torch.Tensor | None, dy: torch.
             raise TrainingError(f"layer_norm_backward: {name} must be [{D}] float32")
     if accumulate and need_dw and (grad_w is None or grad_b is None):
         raise TrainingError("layer_norm_backward: accumulate needs grad_w and grad_b")
-    other = _on_device_of(x)
-    if other is not None:
-        with other:
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(x.device):
             return layer_norm_backward(x, weight, dy, eps, need_dw, grad_w, grad_b, accumulate, dx_residual)
     lib = _lib_for(x)
     dx = torch.empty_like(x)

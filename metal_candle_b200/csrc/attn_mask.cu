@@ -318,8 +318,8 @@ __global__ void __launch_bounds__(kTile) mask_rows_kernel(const MaskParams p) {
 template <typename I>
 int launch(const MaskParams& p, cudaStream_t st) {
   if (p.S <= kChunk) {
-    // a thousand or two positions a block
-    const int C = p.S <= 2048 ? 1 : p.S <= 4096 ? 2 : p.S <= 8192 ? 4 : 8;
+    // a thousand positions a block, more from 8192 on
+    const int C = p.S <= 1024 ? 1 : p.S <= 2048 ? 2 : p.S <= 4096 ? 4 : 8;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(p.B * C));
     cfg.blockDim = dim3(1024);

@@ -11,6 +11,7 @@
 // Rows that are not whole vectors (D = 777) start at every alignment.  Row r starts (r D) mod N elements behind a vector boundary, which comes
 // back every P = N / gcd(D, N) rows: a block takes rows of one residue mod P, and everything is the aligned case moved by a constant, with
 // a ragged first and last vector.  Longer rows, and operands of different alignments, take a kernel that reads element by element.
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -459,10 +460,21 @@ int launch_k(const Params& p, int sms, cudaStream_t st, int* blocks) {
   if (BWD && R::kRows > 1 && smem < 2 * static_cast<size_t>(p.D) * 4) smem = 2 * static_cast<size_t>(p.D) * 4;
   void (*kernel)(const Params) = ln_fwd_kernel<T, TPR, K, SHIFT>;
   if constexpr (BWD) kernel = p.part != nullptr ? ln_bwd_kernel<T, TPR, K, SHIFT, true> : ln_bwd_kernel<T, TPR, K, SHIFT, false>;
-  MCB_CHECK_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  // as many blocks as are on the device at once (each leaves a line of sums), a whole number of rounds of the alignments
-  int per_sm = 0;
-  MCB_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, R::kBlock, smem));
+  // as many blocks as are on the device at once (each leaves a line of sums), a whole number of rounds of the alignments; asked once for
+  // every kernel, device and size of shared memory (a word, so that threads that meet here read a whole answer)
+  static std::atomic<uint64_t> answer[2][64];
+  int dev = 0, per_sm = 0;
+  MCB_CHECK_CUDA(cudaGetDevice(&dev));
+  std::atomic<uint64_t>& known = answer[BWD && p.part != nullptr][dev & 63];
+  const uint64_t seen = known.load(std::memory_order_relaxed);
+  if (static_cast<uint32_t>(seen) == smem + 1) {
+    per_sm = static_cast<int>(seen >> 32);
+  } else {
+    const size_t most = R::smem(3) > smem ? R::smem(3) : smem;   // (of any call of this kernel: another thread's launch must not find less)
+    MCB_CHECK_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most)));
+    MCB_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, R::kBlock, smem));
+    if (dev < 64) known.store(static_cast<uint64_t>(per_sm) << 32 | (smem + 1), std::memory_order_relaxed);
+  }
   const int64_t turns = (p.rows + p.period - 1) / p.period;   // rows of an alignment
   const int each = blocks_for(turns, R::kRows, sms, per_sm < 1 ? 1 : per_sm), most = blocks_for(p.rows, 1, sms, per_sm < 1 ? 1 : per_sm) / p.period;
   *blocks = p.period * (each < most || most < 1 ? each : most);

@@ -502,7 +502,8 @@ __global__ void __launch_bounds__(kThreads) masked_dkv_kernel(const __grid_const
 
 int launch_one(void (*kernel)(Call), const char* name, int64_t blocks, int cluster, size_t smem, const Call& c, cudaStream_t st) {
   if (blocks > 0x7fffffffll) return fail(MCB_ERR_SHAPE, "masked attention: %lld blocks", (long long)blocks);
-  MCB_CHECK_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  // (the most of any call: another thread's launch of the same kernel must not find less)
+  MCB_CHECK_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bwd(128))));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
   cfg.blockDim = dim3(kThreads);

@@ -267,9 +267,8 @@ class GradClipper:
 
     def _call(self, max_norm: Optional[float]) -> torch.Tensor:
         first = self.grads[0]
-        other = backend._on_device_of(first)
-        if other is not None:
-            with other:
+        if first.get_device() != torch._C._cuda_getDevice():
+            with torch.cuda.device(first.device):
                 return self._call(max_norm)
         lib = backend._lib_for(first)
         norm = torch.empty(1, dtype=torch.float32, device=first.device)
