@@ -106,6 +106,11 @@ __device__ __forceinline__ float lg2(float x) {
   return y;
 }
 
+__device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+               "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+
 // The call that a kernel under a mask reads; nothing otherwise.
 struct NoCall {
   NoCall() = default;
@@ -1163,34 +1168,30 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         if (edge) { seen[0] = interval_bits(sees.x, sees.y, key0); seen[1] = interval_bits(sees.x, sees.y, key0 + 32); }
         __half2 bend[CAP ? 32 : 1];   // t, to 2^-12 of itself
 #pragma unroll
-        for (int c2 = 0; c2 < 2; ++c2) {
-          uint32_t pw[16];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int c4 = 2 * c2 + h;
-            float2 slope[CAP ? 8 : 1];
-            if constexpr (CAP || BIAS)
-              shape.apply(sv[c4], static_cast<float>(qpos - key0 - 16 * c4), -1.0f, [&](int e, float2 t) {
-                if constexpr (CAP) {
-                  slope[e >> 1] = __ffma2_rn(t, f2(-t.x, -t.y), f2(1.0f, 1.0f));
-                  bend[8 * c4 + (e >> 1)] = __float22half2_rn(slope[e >> 1]);
-                }
-              });
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              const float2 tt = __ffma2_rn(f2(__uint_as_float(sv[c4][e]), __uint_as_float(sv[c4][e + 1])), sc2, nl2);
-              float2 pr = f2(ex2(tt.x), ex2(tt.y));
-              if (edge) {
-                if ((seen[c2] >> (16 * h + e) & 1u) == 0) pr.x = 0.0f;
-                if ((seen[c2] >> (16 * h + e + 1) & 1u) == 0) pr.y = 0.0f;
+        for (int c4 = 0; c4 < 4; ++c4) {
+          uint32_t pw[8];
+          float2 slope[CAP ? 8 : 1];
+          if constexpr (CAP || BIAS)
+            shape.apply(sv[c4], static_cast<float>(qpos - key0 - 16 * c4), -1.0f, [&](int e, float2 t) {
+              if constexpr (CAP) {
+                slope[e >> 1] = __ffma2_rn(t, f2(-t.x, -t.y), f2(1.0f, 1.0f));
+                bend[8 * c4 + (e >> 1)] = __float22half2_rn(slope[e >> 1]);
               }
-              sv[c4][e] = __float_as_uint(pr.x);
-              sv[c4][e + 1] = __float_as_uint(pr.y);
-              if constexpr (CAP) pr = __fmul2_rn(pr, slope[e >> 1]);
-              pw[8 * h + (e >> 1)] = pack_bf16(pr.x, pr.y);
+            });
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            const float2 tt = __ffma2_rn(f2(__uint_as_float(sv[c4][e]), __uint_as_float(sv[c4][e + 1])), sc2, nl2);
+            float2 pr = f2(ex2(tt.x), ex2(tt.y));
+            if (edge) {
+              if ((seen[c4 >> 1] >> (16 * (c4 & 1) + e) & 1u) == 0) pr.x = 0.0f;
+              if ((seen[c4 >> 1] >> (16 * (c4 & 1) + e + 1) & 1u) == 0) pr.y = 0.0f;
             }
+            sv[c4][e] = __float_as_uint(pr.x);
+            sv[c4][e + 1] = __float_as_uint(pr.y);
+            if constexpr (CAP) pr = __fmul2_rn(pr, slope[e >> 1]);
+            pw[e >> 1] = pack_bf16(pr.x, pr.y);
           }
-          tmem_st_x16(tS + lane_addr + 16 * c2, pw);
+          tmem_st_x8(tS + lane_addr + 8 * c4, pw);
         }
         tmem_st_wait();
         tcgen05_fence_before();
