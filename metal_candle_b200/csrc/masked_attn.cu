@@ -556,8 +556,10 @@ int fill(Call& c, const mcb_masked_attention* a, const char* who) {
   if (a->kv_heads <= 0 || a->groups <= 0 || a->kv_heads > 0x7fffffff || a->groups > 0x7fffffff / a->kv_heads ||
       a->batch * amask::tiles_of(a->seq) > 0x07ffffffll / (a->kv_heads * a->groups))
     return fail(MCB_ERR_SHAPE, "%s: batch=%lld kv_heads=%lld groups=%lld seq=%lld", who, (long long)a->batch, (long long)a->kv_heads, (long long)a->groups, (long long)a->seq);
-  if (!(a->scale > 0.0f && a->scale - a->scale == 0.0f)) return fail(MCB_ERR_SHAPE, "%s: scale must be positive and finite", who);
-  if (!(a->softcap >= 0.0f && a->softcap - a->softcap == 0.0f)) return fail(MCB_ERR_SHAPE, "%s: softcap must be 0 (none) or positive and finite", who);
+  const auto finite = [](float v) { return v - v == 0.0f; };
+  if (!(a->scale > 0.0f && finite(a->scale * kLog2e))) return fail(MCB_ERR_SHAPE, "%s: scale must be positive and finite", who);
+  if (!(a->softcap >= 0.0f && finite(a->softcap * kLog2e) && (a->softcap == 0.0f || finite(a->scale / a->softcap))))
+    return fail(MCB_ERR_SHAPE, "%s: softcap must be 0 (none) or positive and finite, and scale / softcap finite", who);
   if (!aligned16(a->mask) || (reinterpret_cast<uintptr_t>(a->slopes) & 3) != 0) return fail(MCB_ERR_ALIGN, "%s: alignment of the mask or the slopes", who);
   c = Call{};
   c.mask = amask::view(a->mask, a->batch, a->seq);

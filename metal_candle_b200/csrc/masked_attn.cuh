@@ -58,7 +58,8 @@ __device__ __forceinline__ float score2(const Call& c, float dot, float slope2, 
 //
 // A tile's product takes a masked probability of 0 times whatever lies at the masked position: an infinity or a NaN there (memory
 // that nothing has written behind a document, a diverged neighbour) makes the sum NaN although the row does not see it.  A row that
-// comes out not finite is therefore computed again from the positions that it sees alone, here.  With finite inputs none is.
+// comes out not finite is therefore computed again from the positions that it sees alone, here.  With finite inputs none is, and a row
+// that is NaN by right (a diverged run) is left as soon as that shows.
 // Head dimensions up to 128: lane l has the elements l, l + 32, l + 64, l + 96.
 template <typename T>
 struct RowData {
@@ -97,6 +98,7 @@ __device__ __noinline__ void fwd_row(const Call& c, int b, int hk, int g, int s)
     const float top = t > m ? t : m;   // (a NaN score leaves the maximum and makes the sums NaN)
     const float old = exp2f(m - top), p = exp2f(t - top);
     l = fmaf(l, old, p);
+    if (l != l) break;   // (the same on all lanes) every element is NaN
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] = fmaf(p, v.v[e], acc[e] * old);
     m = top;
@@ -139,6 +141,9 @@ __device__ __noinline__ void dq_row(const Call& c, int b, int hk, int g, int s) 
         const float dp = go.dot(v), ds = pair_ds(c, q.dot(k), dp, slope2, abs(s - j), lse2, delta, p);
         if (turn == 0) {
           acc[0] = fmaf(p, dp, acc[0]);
+        } else if (ds != ds) {
+          acc[0] = acc[1] = acc[2] = acc[3] = ds;   // every element is NaN
+          break;
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[e] = fmaf(ds, k.v[e], acc[e]);
@@ -165,6 +170,11 @@ __device__ __noinline__ void dkv_row(const Call& c, int b, int hk, int s) {
       const RowData<T> q(static_cast<const T*>(c.q) + q_row(c, b, hk, g, i) * c.D, c.D), go(static_cast<const T*>(c.dout) + o_at(c, b, hk, g, i), c.D);
       float p;
       const float ds = pair_ds(c, q.dot(k), go.dot(v), slope2, abs(s - i), lse2, -c.ndelta[at], p);
+      if (p != p) {   // every element of both is NaN
+        g = c.G;
+        for (int e = 0; e < 4; ++e) gk[e] = gv[e] = p;
+        break;
+      }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         gk[e] = fmaf(ds, q.v[e], gk[e]);

@@ -282,3 +282,77 @@ def test_streams_graphs_and_two_at_once(cuda_device):
         expect = step(q, k, v, dout)["o"]
         ids_t.copy_(old)
         assert torch.equal(changed, expect) and not torch.equal(changed, want["o"])
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 64), (F32, 40)])
+def test_values_that_are_not_finite_stay_in_their_document(cuda_device, dtype, d):
+    """A NaN query, key, value or output gradient makes its own document's rows NaN as the formulas say and leaves the others what they are.
+
+    Not to the bit: a row of a tile that meets the NaN (0 x NaN in a product) is computed again by itself, and there the weights are not
+    rounded to bfloat16 (u_p of the bounds is 0 there), so both results are within the bounds and differ by no more than their sum."""
+    B, S, Hk, G = 1, 300, 1, 2
+    ids = [[0] * 130 + [1] * 170]
+    mask = mask_of(cuda_device, ids, None)
+    base = inputs(cuda_device, B, S, Hk, G, d, dtype, False, 12)
+    want = ref.attention(*base, ids, None, G, 0.125, 0.0, None, False, dtype, dtype == BF16)
+    for which, at in (("q", 40), ("k", 40), ("v", 40), ("dout", 40)):
+        q, k, v, dout = (t.clone() for t in base)
+        t = dict(q=q, k=k, v=v, dout=dout)[which]
+        t[0, at, 3] = math.nan   # head 0 of the first document
+        got = run(q, k, v, dout, G, 0.125, mask, 0.0, None, False)
+        o, dq = got["o"].view(G, S, d), got["dq"].view(G, S, d)
+        nan = {name: torch.isnan(got[name]).view(-1, S, d).any(0).any(-1).cpu() for name in ("o", "dq", "dk", "dv")}
+        seen = torch.zeros(S, dtype=torch.bool)
+        if which == "q":     # one query row: its o; dq of it; dk and dv of the keys that it sees
+            seen[:41] = True
+            assert nan["o"].nonzero().flatten().tolist() == [40] and nan["dq"].nonzero().flatten().tolist() == [40]
+            assert torch.equal(nan["dk"], seen) and torch.equal(nan["dv"], seen)
+        elif which == "k":   # the queries that see it
+            seen[40:130] = True
+            assert torch.equal(nan["o"], seen) and torch.equal(nan["dq"], seen)
+        elif which == "v":
+            seen[40:130] = True
+            assert torch.equal(nan["o"], seen) and torch.equal(nan["dq"], seen)
+            assert torch.isfinite(o[:, :130, :3]).all() and torch.isnan(o[:, 40:130, 3]).all()   # the other columns are what they are
+        else:
+            seen[:41] = True
+            assert not nan["o"].any() and nan["dq"].nonzero().flatten().tolist() == [40]
+            assert torch.equal(nan["dk"], seen)
+        for name in ("o", "dq", "dk", "dv"):
+            ref.check(got[name].view(-1, S, d)[:, 130:], tuple(t.view(-1, S, d)[:, 130:] for t in want[name]), f"{name} with {which}")
+
+
+def test_one_mask_on_two_streams_and_prefix_alone(cuda_device):
+    B, S, Hk, G, d = 2, 900, 2, 3, 64
+    prefix = torch.zeros(B, S, dtype=torch.uint8, device=cuda_device)
+    prefix[0, :333] = 1
+    prefix[1, 5:] = 1   # not leading: counts for nothing
+    mask = backend.attention_mask(prefix=prefix)
+    a, b = inputs(cuda_device, B, S, Hk, G, d, BF16, True, 1), inputs(cuda_device, B, S, Hk, G, d, BF16, True, 2)
+    want = [run(*t, G, 0.125, mask, 0.0, None, True) for t in (a, b)]
+    value = ref.attention(*a, [[0] * S] * B, prefix.bool().tolist(), G, 0.125, 0.0, None, True, BF16, True)
+    for name, v in value.items():
+        ref.check(want[0][name], v, name)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(8):
+        for stream, t in zip(streams, (a, b)):
+            with torch.cuda.stream(stream):
+                got.append(run(*t, G, 0.125, mask, 0.0, None, True))
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        assert all(torch.equal(out[n], want[i % 2][n]) for n in out)
+
+
+def test_many_short_items(cuda_device):
+    """More items than CTAs by far, most of them of one block, some of none: every one is done once."""
+    B, S, Hk, G, d = 600, 40, 2, 2, 64
+    rng = random.Random(3)
+    ids = [[-1] * S if rng.random() < 0.3 else [i // rng.randint(1, 9) for i in range(S)] for _ in range(B)]
+    mask = mask_of(cuda_device, ids, None)
+    q, k, v, dout = inputs(cuda_device, B, S, Hk, G, d, BF16, False, 4)
+    got = run(q, k, v, dout, G, 0.125, mask, 0.0, None, False)
+    want = ref.attention(q, k, v, dout, ids, None, G, 0.125, 0.0, None, False, BF16, True)
+    for name, value in want.items():
+        ref.check(got[name], value, name)

@@ -112,6 +112,36 @@ def test_layer_norm_off_alignment_and_in_parts(cuda_device, dtype):
     ref.check(gb, want["db"], "db in parts")
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D,start", [(896, 0), (896, 3), (777, 0), (777, 5), (33, 1), (2500, 0)])
+def test_layer_norm_in_place(cuda_device, dtype, D, start):
+    """y over x, dx over dy and over the residual's gradient, for rows that start anywhere."""
+    from metal_candle_b200 import _lib
+
+    lib, rows, code = _lib.load(), 300, 0 if dtype == F32 else 1
+    stream = torch.cuda.current_stream().cuda_stream
+    flat = lambda seed: rand(cuda_device, rows * D + 8, seed=seed, dtype=dtype)[start:start + rows * D].view(rows, D)  # noqa: E731
+    x, dy, res, w, b = flat(1), flat(2), flat(3), rand(cuda_device, D, seed=4, dtype=dtype), rand(cuda_device, D, seed=5, dtype=dtype)
+    want = layer_norm_64(x, w, b, dy, res, 1e-5, dtype)
+    ws = torch.empty(lib.mcb_layernorm_bwd_workspace_bytes(rows, D), dtype=torch.uint8, device=cuda_device)
+    for over in ("dy", "res"):
+        d, r, dw, db = dy.clone(), res.clone(), torch.empty(D, device=cuda_device), torch.empty(D, device=cuda_device)
+        dc, rc = (torch.empty(rows * D + 8, dtype=dtype, device=cuda_device)[start:start + rows * D].view(rows, D) for _ in range(2))
+        dc.copy_(d), rc.copy_(r)
+        out = dc if over == "dy" else rc
+        _lib.check(lib.mcb_layernorm_bwd(x.data_ptr(), w.data_ptr(), dc.data_ptr(), rc.data_ptr(), out.data_ptr(), dw.data_ptr(), db.data_ptr(), 0, rows, D,
+                                         1e-5, code, ws.data_ptr(), ws.numel(), stream))
+        for name, t in (("dx", out), ("dw", dw), ("db", db)):
+            ref.check(t, want[name], f"{name} over {over}")
+        # one of the two sums alone
+        only = torch.empty(D, device=cuda_device)
+        _lib.check(lib.mcb_layernorm_bwd(x.data_ptr(), w.data_ptr(), d.data_ptr(), None, torch.empty_like(d).data_ptr(), None, only.data_ptr(), 0, rows, D,
+                                         1e-5, code, ws.data_ptr(), ws.numel(), stream))
+        ref.check(only, want["db"], "db alone")
+    _lib.check(lib.mcb_layernorm_fwd(x.data_ptr(), w.data_ptr(), b.data_ptr(), x.data_ptr(), None, None, rows, D, 1e-5, code, stream))
+    ref.check(x, want["y"], "y over x")
+
+
 # ---- embedding -------------------------------------------------------------------------------------------------------------
 
 def embedding_64(ids, dout, vocab, scale):
@@ -202,6 +232,11 @@ def test_norm_and_clip(cuda_device, sizes, dtype):
             assert ((o.double() - want).abs() <= (2.0 ** -22 + half_step(g.dtype)) * want.abs() + 1e-44).all()
         assert near(clip_grad_norm(copies, limit), whole)
         assert all(torch.equal(o, c) for o, c in zip(out, copies))
+
+
+def test_norm_of_nothing(cuda_device):
+    empty = [torch.empty(0, device=cuda_device), torch.empty(0, 5, dtype=BF16, device=cuda_device)]
+    assert float(grad_norm(empty)) == 0.0 and float(clip_grad_norm(empty, 1.0)) == 0.0
 
 
 def test_norm_at_the_ends_of_float32(cuda_device):

@@ -46,7 +46,7 @@ REFUSED = [(dict(mask=None), NULL), (dict(dtype=2), UNSUPPORTED), (dict(seq=0), 
            (dict(kv_heads=0), SHAPE), (dict(groups=0), SHAPE), (dict(kv_heads=1 << 20, groups=1 << 20), SHAPE), (dict(groups=1 << 26), SHAPE),
            (dict(scale=math.nan), SHAPE), (dict(scale=math.inf), SHAPE), (dict(scale=0.0), SHAPE),
            (dict(scale=-0.1), SHAPE), (dict(softcap=-1.0), SHAPE), (dict(softcap=math.nan), SHAPE),
-           (dict(softcap=math.inf), SHAPE), (dict(mask=24), ALIGN), (dict(slopes=17), ALIGN)]
+           (dict(softcap=math.inf), SHAPE), (dict(softcap=3e38), SHAPE), (dict(softcap=1e-42), SHAPE), (dict(scale=3e38), SHAPE), (dict(mask=24), ALIGN), (dict(slopes=17), ALIGN)]
 
 
 @pytest.mark.parametrize("change,status", REFUSED)
