@@ -76,8 +76,9 @@ constexpr int kFwdStages = 4;                         // K / V ring: a load has 
 constexpr uint32_t kOffK = kOffQ + kQBytes;
 constexpr uint32_t kOffV = kOffK + kFwdStages * kKBytes;
 constexpr uint32_t kOffBar = kOffV + kFwdStages * kKBytes;
-constexpr uint32_t kOffAnswers = kOffBar + 256;       // of the item requests (see Answers): two of 16 bytes, then their barriers
-constexpr uint32_t kFwdSmem = kOffAnswers + 64 + 1024;
+constexpr uint32_t kOffItems = kOffBar + 256;         // see Items
+constexpr uint32_t kItemsBytes = 128;
+constexpr uint32_t kFwdSmem = kOffItems + kItemsBytes + 1024;
 
 struct FwdParams {
   int S, G, NB;
@@ -212,31 +213,41 @@ __device__ __forceinline__ FwdTile fwd_tile(const FwdParams& p, int t) {
 // ---- a CTA's items one after the other ----
 // Without a mask: item t, t + gridDim, ..  Under one the tiles' lengths differ too much to be dealt out beforehand (documents of 585: 40 % between the
 // longest CTA and the mean): the grid has a CTA for every item, the longest first, and those that run take over items of CTAs that have not started
-// (cluster launch control).  A request's answer lies in shared memory, two by turns, with a barrier that it
-// completes and one on which all readers let go of it: the loading thread, the MMA warp and four softmax warps.
-struct Answers {
-  uint32_t full0, empty0, at0;   // two barriers each; two answers of 16 bytes
+// (cluster launch control).  The loading thread asks; the item and its record go to the MMA warp and the softmax warps through shared memory, two
+// places by turns with a barrier that fills one and one on which its readers let go of it.
+struct Items {
+  uint32_t at;     // bytes from here: the request's answer (16), two records (16 each), two items (4 each), then the barriers (8 each): of the
+  uint8_t* gen;    // request, of the places filled, of the places read
+  static constexpr uint32_t kReaders = 5;
+  __device__ __forceinline__ uint32_t asked() const { return at + 56; }
+  __device__ __forceinline__ uint32_t full(int k) const { return at + 64 + 8 * (k & 1); }
+  __device__ __forceinline__ uint32_t empty(int k) const { return at + 80 + 8 * (k & 1); }
+  __device__ __forceinline__ volatile int4* record(int k) const { return reinterpret_cast<volatile int4*>(gen + 16 + 16 * (k & 1)); }
+  __device__ __forceinline__ volatile int* item(int k) const { return reinterpret_cast<volatile int*>(gen + 48 + 4 * (k & 1)); }
+  __device__ __forceinline__ void init() const {
+    mbar_init(asked(), 1);
+    for (int s = 0; s < 2; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), kReaders); }
+  }
+  __device__ __forceinline__ void request() const {
+    mbar_expect_tx(asked(), 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(at), "r"(asked()) : "memory");
+  }
+  // the item that was taken over, or -1: none is left
+  __device__ __forceinline__ int answer() const {
+    uint32_t got, x, y, z;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
+        "ld.shared.b128 r, [%4];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "mov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, %3, _}, r;\n\t}"
+        : "=r"(got), "=r"(x), "=r"(y), "=r"(z)
+        : "r"(at)
+        : "memory");
+    return got ? static_cast<int>(x) : -1;
+  }
 };
-constexpr uint32_t kAnswerReaders = 6;
-__device__ __forceinline__ void request_item(uint32_t answer, uint32_t bar) {
-  mbar_expect_tx(bar, 16);
-  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
-}
-// the item that was taken over, or -1: none is left
-__device__ __forceinline__ int read_answer(uint32_t answer) {
-  uint32_t got, x, y, z;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
-      "ld.shared.b128 r, [%4];\n\t"
-      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t"
-      "mov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
-      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, %3, _}, r;\n\t}"
-      : "=r"(got), "=r"(x), "=r"(y), "=r"(z)
-      : "r"(answer)
-      : "memory");
-  return got ? static_cast<int>(x) : -1;
-}
 
 template <bool MASKED>
 struct Walk;
@@ -244,7 +255,7 @@ template <>
 struct Walk<false> {
   const FwdParams& p;
   int t, n;
-  __device__ __forceinline__ Walk(const FwdParams& p_, const NoCall&, const Answers&, volatile int*) : p(p_), t(blockIdx.x), n(q_blocks(p_.S) * p_.G * p_.NB) {}
+  __device__ __forceinline__ Walk(const FwdParams& p_, const NoCall&, const Items&, volatile int*) : p(p_), t(blockIdx.x), n(q_blocks(p_.S) * p_.G * p_.NB) {}
   __device__ __forceinline__ bool get_as_loader(FwdTile& w) { return get(w); }
   __device__ __forceinline__ bool get(FwdTile& w) {
     if (t >= n) return false;
@@ -257,12 +268,12 @@ template <>
 struct Walk<true> {
   const FwdParams& p;
   const mattn::Call& c;
-  const Answers ans;
+  const Items items;
   volatile int* abort_flag;
   int t, k;      // item, and how many came before it
   int4 rec;      // its record
-  __device__ __forceinline__ Walk(const FwdParams& p_, const mattn::Call& c_, const Answers& a, volatile int* abort)
-      : p(p_), c(c_), ans(a), abort_flag(abort), t(blockIdx.x), k(0), rec(c_.mask.qwork[blockIdx.x / (p_.G * c_.Hk)]) {}
+  __device__ __forceinline__ Walk(const FwdParams& p_, const mattn::Call& c_, const Items& i, volatile int* abort)
+      : p(p_), c(c_), items(i), abort_flag(abort), t(blockIdx.x), k(0), rec(c_.mask.qwork[blockIdx.x / (p_.G * c_.Hk)]) {}
   __device__ __forceinline__ void fill(FwdTile& w) const {
     const int r = t % (p.G * c.Hk);
     w.b = rec.x; w.qb = rec.y; w.kb0 = rec.z; w.nkb = rec.w;
@@ -270,20 +281,22 @@ struct Walk<true> {
     w.nb = w.b * c.Hk + w.hk;
     w.qrow0 = (static_cast<int64_t>(w.nb) * p.G + w.g) * p.S + static_cast<int64_t>(w.qb) * kBQ;
   }
-  // answer k >= 1 is number (k - 1) / 2 in its place
-  __device__ __forceinline__ bool arrived(int n) const { return mbar_wait(ans.full0 + 8 * (n & 1), ((n - 1) >> 1) & 1, abort_flag, 99, c.status); }
+  // (item k >= 1 is use (k - 1) / 2 of its place)
   // by one thread: its next item.  Asked for when the loads of the one before are on their way, some blocks ahead of their use, and no sooner: a CTA that
-  // asks as it starts takes over items whose CTAs would have started beside it (64 x 2 heads of 1024 positions, forward: 45 us, asked at the start 58)
+  // asks as it starts takes over items whose CTAs would have started beside it (4 x 16 heads of 1024 positions, forward: 45 us, asked at the start 58)
   __device__ __forceinline__ bool get_as_loader(FwdTile& w) {
     if (k > 0) {
-      if (k >= 3 && !mbar_wait(ans.empty0 + 8 * (k & 1), ((k - 3) >> 1) & 1, abort_flag, 100, c.status)) return false;
-      request_item(ans.at0 + 16 * (k & 1), ans.full0 + 8 * (k & 1));
-      if (!arrived(k)) return false;
-      t = read_answer(ans.at0 + 16 * (k & 1));
-      fence_proxy_async_smem();
-      mbar_arrive(ans.empty0 + 8 * (k & 1));
+      items.request();
+      if (!mbar_wait(items.asked(), (k - 1) & 1, abort_flag, 99, c.status)) return false;
+      t = items.answer();
+      fence_proxy_async_smem();   // (the next answer is written by another proxy)
+      if (t >= 0) rec = c.mask.qwork[t / (p.G * c.Hk)];
+      if (k >= 3 && !mbar_wait(items.empty(k), ((k - 3) >> 1) & 1, abort_flag, 100, c.status)) return false;
+      volatile int4* at = items.record(k);
+      at->x = rec.x; at->y = rec.y; at->z = rec.z; at->w = rec.w;
+      *items.item(k) = t;
+      mbar_arrive(items.full(k));
       if (t < 0) return false;
-      rec = c.mask.qwork[t / (p.G * c.Hk)];
     }
     ++k;
     fill(w);
@@ -292,13 +305,13 @@ struct Walk<true> {
   // by a whole warp: its next item
   __device__ __forceinline__ bool get(FwdTile& w) {
     if (k > 0) {
-      if (!__all_sync(0xffffffffu, arrived(k))) return false;
-      t = read_answer(ans.at0 + 16 * (k & 1));
-      fence_proxy_async_smem();
+      if (!__all_sync(0xffffffffu, mbar_wait(items.full(k), ((k - 1) >> 1) & 1, abort_flag, 99, c.status))) return false;
+      t = *items.item(k);
+      volatile int4* at = items.record(k);
+      rec = make_int4(at->x, at->y, at->z, at->w);
       __syncwarp();
-      if ((threadIdx.x & 31) == 0) mbar_arrive(ans.empty0 + 8 * (k & 1));
+      if ((threadIdx.x & 31) == 0) mbar_arrive(items.empty(k));
       if (t < 0) return false;
-      rec = c.mask.qwork[t / (p.G * c.Hk)];
     }
     ++k;
     fill(w);
@@ -338,7 +351,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   const uint32_t kv_empty0 = kv_full0 + 8 * kFwdStages;
   const uint32_t s_full0 = kv_empty0 + 8 * kFwdStages, p_ready0 = s_full0 + 16, pv_done0 = p_ready0 + 16;
   const uint32_t s_free0 = pv_done0 + 16, tmem_slot = s_free0 + 16, abort_addr = tmem_slot + 4;
-  const Answers ans = {base + kOffAnswers + 32, base + kOffAnswers + 48, base + kOffAnswers};
+  const Items items = {base + kOffItems, gen_base + kOffItems};
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(gen_base + (tmem_slot - base));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_base + (abort_addr - base));
 
@@ -350,8 +363,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     for (int s = 0; s < 2; ++s) {
       mbar_init(s_full0 + 8 * s, 1); mbar_init(p_ready0 + 8 * s, 4); mbar_init(pv_done0 + 8 * s, 1); mbar_init(s_free0 + 8 * s, 4);
     }
-    if (MASKED)
-      for (int s = 0; s < 2; ++s) { mbar_init(ans.full0 + 8 * s, 1); mbar_init(ans.empty0 + 8 * s, kAnswerReaders); }
+    if (MASKED) items.init();
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async_smem();
@@ -368,7 +380,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   grid_dependency_wait();   // the set-up above ran under the tail of the kernel before
   // S buffers at columns 0 and 64, O at 128, the two P buffers (bf16 pairs: 32 columns each) at 192 and 224
   const uint32_t tO = tmem_base + 128, tP0 = tmem_base + 192;
-  Walk<MASKED> walk(p, c, ans, abort_flag);
+  Walk<MASKED> walk(p, c, items, abort_flag);
   FwdTile w;
 
   if (warp == 0) {
@@ -468,14 +480,24 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     bool ok = true;
     uint32_t n0 = 0;
     std::conditional_t<MASKED, Shape<CAP, BIAS>, NoCall> shape(c);
-    while (ok && walk.get(w)) {
+    int2 sees = make_int2(0, 0), sees_next = make_int2(0, 0);
+    auto row_of = [&](const FwdTile& t) {
+      const int at = t.qb * kBQ + row;
+      if constexpr (MASKED)
+        if (at < p.S) return c.mask.rows[static_cast<int64_t>(t.b) * p.S + at];
+      return make_int2(0, 0);
+    };
+    FwdTile next;
+    bool more = walk.get(next);
+    if (more) sees_next = row_of(next);
+    while (ok && more) {
+      w = next;
+      sees = sees_next;
       const int qpos = w.qb * kBQ + row;
       // m: the maximum in use (base-2 logits); under a mask a row may see nothing for some blocks, or at all
       float m = MASKED ? mattn::kNoScore : -INFINITY, l = 0.0f;
-      int2 sees = make_int2(0, 0);
       float sc = p.sc;
       if constexpr (MASKED) {
-        if (qpos < p.S) sees = c.mask.rows[static_cast<int64_t>(w.b) * p.S + qpos];
         if constexpr (BIAS) shape.slope2 = c.slopes[w.hk * p.G + w.g] * kLog2e;
         if constexpr (CAP || BIAS) sc = 1.0f;
         if (w.nkb == 0) {   // the tile sees nothing: no block was loaded for it
@@ -485,6 +507,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             for (int i = 0; i < 8; ++i) orow[i] = make_uint4(0, 0, 0, 0);
             if (p.lse != nullptr) p.lse[w.qrow0 + row] = -INFINITY;
           }
+          more = walk.get(next);
+          if (more) sees_next = row_of(next);
           continue;
         }
       }
@@ -592,6 +616,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         if (lane == 0) mbar_arrive(p_ready0 + 8 * (n & 1));
       }
       if (!ok) break;
+      // (the next item's row is read under this one's write-out)
+      more = walk.get(next);
+      if (more) sees_next = row_of(next);
       // write-out: the item's last P V product has landed
       const uint32_t nl = n0 + static_cast<uint32_t>(w.nkb) - 1;
       ok = __all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * (nl & 1), (nl >> 1) & 1, abort_flag, 78, p.status));
@@ -663,8 +690,8 @@ constexpr int kDqStages = 4;
 constexpr uint32_t kDqOffStage = kDqOffDO + kQBytes;     // stages of a K and a V tile (8 KB each)
 constexpr uint32_t kDqStageBytes = 2 * kKBytes;
 constexpr uint32_t kDqOffBar = kDqOffStage + kDqStages * kDqStageBytes;
-constexpr uint32_t kDqOffAnswers = kDqOffBar + 256;
-constexpr uint32_t kDqSmem = kDqOffAnswers + 64 + 1024;
+constexpr uint32_t kDqOffItems = kDqOffBar + 256;
+constexpr uint32_t kDqSmem = kDqOffItems + kItemsBytes + 1024;
 
 struct BwdParams {
   int S, G, NB;
@@ -954,7 +981,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
 // this block's second half.
 template <bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 2)
-attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmdO,
+attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmdO, const __grid_constant__ CUtensorMap tmO,
                       const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const BwdParams p,
                       const __grid_constant__ mattn::Call c) {
   extern __shared__ uint8_t smem_raw[];
@@ -966,13 +993,13 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   const uint32_t kv_full0 = dq_free + 8, kv_empty0 = kv_full0 + 8 * kDqStages;
   const uint32_t s_full = kv_empty0 + 8 * kDqStages, p_ready = s_full + 8;
   const uint32_t dp_full = p_ready + 8, ds_ready = dp_full + 8, tmem_slot = ds_ready + 8, abort_addr = tmem_slot + 4;
-  const Answers ans = {base + kDqOffAnswers + 32, base + kDqOffAnswers + 48, base + kDqOffAnswers};
+  const Items items = {base + kDqOffItems, gen_base + kDqOffItems};
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(gen_base + (tmem_slot - base));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_base + (abort_addr - base));
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    mbar_init(q_free, 1);
+    mbar_init(q_free, 5);   // the last S and dP products, and the four warps that have read dO
     mbar_init(dq_full, 1);
     mbar_init(dq_free, 4);
     for (int s = 0; s < kDqStages; ++s) { mbar_init(kv_full0 + 8 * s, 1); mbar_init(kv_empty0 + 8 * s, 1); }
@@ -980,7 +1007,7 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     mbar_init(p_ready, 4);
     mbar_init(dp_full, 1);
     mbar_init(ds_ready, 4);
-    for (int s = 0; s < 2; ++s) { mbar_init(ans.full0 + 8 * s, 1); mbar_init(ans.empty0 + 8 * s, kAnswerReaders); }
+    items.init();
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async_smem();
@@ -998,7 +1025,7 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   const uint32_t tS = tmem_base, tDP = tmem_base + 64, tDQ = tmem_base + 128, tPK = tmem_base + 192;
   FwdParams tp;   // the item order of the forward
   tp.S = p.S; tp.G = p.G; tp.NB = p.NB;
-  Walk<true> walk(tp, c, ans, abort_flag);
+  Walk<true> walk(tp, c, items, abort_flag);
   FwdTile w;
 
   if (warp == 0) {
@@ -1018,13 +1045,18 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         int dcol, dplane;
         o_plane(p.G, p.HKV, p.o_tok, w.nb, w.g, dcol, dplane);
         tma_load_3d(base + kDqOffDO, &tmdO, q_full, dcol, w.qb * kBQ, dplane);
-        for (int j = 0; j < w.nkb; ++j) {
+        // O takes a place of the ring, then the blocks
+        for (int j = -1; j < w.nkb; ++j) {
           ok = mbar_wait(kv_empty0 + 8 * st, ph ^ 1, abort_flag, 81, p.status);
           if (!ok) break;
           const uint32_t sb = base + kDqOffStage + st * kDqStageBytes;
           mbar_expect_tx(kv_full0 + 8 * st, kDqStageBytes);
-          tma_load_3d(sb, &tmK, kv_full0 + 8 * st, 0, (w.kb0 + j) * kBK, w.nb);
-          tma_load_3d(sb + kKBytes, &tmV, kv_full0 + 8 * st, 0, (w.kb0 + j) * kBK, w.nb);
+          if (j < 0) {
+            tma_load_3d(sb, &tmO, kv_full0 + 8 * st, dcol, w.qb * kBQ, dplane);
+          } else {
+            tma_load_3d(sb, &tmK, kv_full0 + 8 * st, 0, (w.kb0 + j) * kBK, w.nb);
+            tma_load_3d(sb + kKBytes, &tmV, kv_full0 + 8 * st, 0, (w.kb0 + j) * kBK, w.nb);
+          }
           if (++st == kDqStages) { st = 0; ph ^= 1; }
         }
       }
@@ -1069,6 +1101,9 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     while (ok && walk.get(w)) {
       if (w.nkb == 0) continue;
       ++it;
+      const int o_st = dst;   // the ring's place that holds O
+      if (++sst == kDqStages) { sst = 0; sph ^= 1; }
+      if (++dst == kDqStages) dst = 0;
       ok = wait(q_full, it & 1, 84) && issue_s();
       if (!ok) break;
       issue_dp(dst, w.nkb == 1);
@@ -1076,6 +1111,7 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         const uint64_t dKn = desc_sw128_mn(base + kDqOffStage + dst * kDqStageBytes, kKBytes, 1024);
         const uint32_t acc = j != 0 ? 1u : 0u;
         ok = wait(p_ready, n & 1, 82);
+        if (ok && j == 0 && lane == 0) mbar_arrive(kv_empty0 + 8 * o_st);   // the four warps have read O
         // the first products of an item overwrite both sums: the previous item's write-out must have read them
         if (ok && j == 0 && it > 0) ok = wait(dq_free, (it - 1) & 1, 87);
         if (!ok) break;
@@ -1115,29 +1151,25 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     Shape<CAP, BIAS> shape(c);
     const float sc = CAP || BIAS ? 1.0f : p.sc;
     const float2 sc2 = f2(sc, sc);
-    while (ok && walk.get(w)) {
+    int2 sees_next = make_int2(0, 0);
+    float lse_next = -INFINITY;
+    auto row_of = [&](const FwdTile& t) {
+      const int at = t.qb * kBQ + row;
+      sees_next = make_int2(0, 0);
+      lse_next = -INFINITY;
+      if (at >= p.S) return;
+      sees_next = c.mask.rows[static_cast<int64_t>(t.b) * p.S + at];
+      lse_next = p.lse[t.qrow0 + row];
+    };
+    FwdTile next;
+    bool more = walk.get(next);
+    if (more) row_of(next);
+    while (ok && more) {
+      w = next;
+      const int2 sees = sees_next;
       const int qpos = w.qb * kBQ + row;
-      // d~ = sum_d dO * O of this row, straight from global memory (once per item)
-      float rough = 0.0f, lse2 = INFINITY;   // of a row behind position S, or one that sees nothing: P = dS = 0
-      int2 sees = make_int2(0, 0);
-      if (qpos < p.S) {
-        sees = c.mask.rows[static_cast<int64_t>(w.b) * p.S + qpos];
-        lse2 = p.lse[w.qrow0 + row] * kLog2e;
-        if (lse2 == -INFINITY) lse2 = INFINITY;
-        const int64_t ooff = o_offset(p.S, p.G, p.HKV, p.o_tok, w.nb, w.g, qpos);
-        const uint4* o4 = reinterpret_cast<const uint4*>(p.O + ooff);
-        const uint4* d4 = reinterpret_cast<const uint4*>(p.dO + ooff);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint4 a = o4[k], b = d4[k];
-          const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            rough = fmaf(__uint_as_float(aw[e] << 16), __uint_as_float(bw[e] << 16), rough);
-            rough = fmaf(__uint_as_float(aw[e] & 0xffff0000u), __uint_as_float(bw[e] & 0xffff0000u), rough);
-          }
-        }
-      }
+      float lse2 = lse_next * kLog2e;
+      if (lse2 == -INFINITY) lse2 = INFINITY;   // of a row behind position S, or one that sees nothing: P = dS = 0
       const int64_t prow = (static_cast<int64_t>(w.nb) * p.G + w.g) * (q_blocks(p.S) * kBQ) + qpos;
       p.nlse2[prow] = -lse2;
       if constexpr (BIAS) shape.slope2 = c.slopes[w.hk * p.G + w.g] * kLog2e;
@@ -1148,9 +1180,35 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
 #pragma unroll
           for (int i = 0; i < 8; ++i) orow[i] = make_uint4(0, 0, 0, 0);
         }
+        more = walk.get(next);
+        if (more) row_of(next);
         continue;
       }
       ++it;
+      // d~ = sum_d dO * O of this row: its tile of O is the ring's entry before the item's blocks.  (2 x 4096 positions, 14 heads,
+      // documents of 585, backward: 122 us with O and dO read from global memory, a row a lane, 112 so.)  Positions behind S are zeros.
+      const uint32_t entry = n + static_cast<uint32_t>(it), o_st = entry % kDqStages;
+      ok = __all_sync(0xffffffffu, mbar_wait(q_full, it & 1, abort_flag, 84, p.status) &&
+                                       mbar_wait(kv_full0 + 8 * o_st, (entry / kDqStages) & 1, abort_flag, 85, p.status));
+      if (!ok) break;
+      float rough = 0.0f;
+      {
+        const uint8_t* o_row = gen_base + kDqOffStage + o_st * kDqStageBytes + row * 128;
+        const uint8_t* do_row = gen_base + kDqOffDO + row * 128;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {   // (16-byte pieces of a row lie by its number's low bits)
+          const int at = (k ^ (row & 7)) * 16;
+          const uint4 a = *reinterpret_cast<const uint4*>(o_row + at), b = *reinterpret_cast<const uint4*>(do_row + at);
+          const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            rough = fmaf(__uint_as_float(aw[e] << 16), __uint_as_float(bw[e] << 16), rough);
+            rough = fmaf(__uint_as_float(aw[e] & 0xffff0000u), __uint_as_float(bw[e] & 0xffff0000u), rough);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_free);
       const float2 nl2 = f2(-lse2, -lse2), nd2 = f2(-rough, -rough);
       float2 exact = f2(0.0f, 0.0f);   // delta
       for (int j = 0; j < w.nkb; ++j, ++n) {
@@ -1231,6 +1289,8 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         if (lane == 0) mbar_arrive(ds_ready);
       }
       if (!ok) break;
+      more = walk.get(next);
+      if (more) row_of(next);
       const float delta = exact.x + exact.y, put_right = rough - delta;
       p.ndelta[prow] = -delta;
       ok = __all_sync(0xffffffffu, mbar_wait(dq_full, it & 1, abort_flag, 90, p.status));
@@ -2167,9 +2227,10 @@ int bwd_form(const Call& c, const DeviceState* ds, cudaStream_t st) {
   if (int rc = Form<CAP, BIAS>::prepare(dev)) return rc;
   const int64_t nb = static_cast<int64_t>(c.B) * c.Hk;
   const int64_t do_inner = c.o_tok ? static_cast<int64_t>(c.Hk) * c.G * kD : kD, do_planes = c.o_tok ? c.B : nb * c.G;
-  CUtensorMap tmQ128, tmdO128, tmK64, tmV64, tmK128, tmV128, tmQ64, tmdO64;
+  CUtensorMap tmQ128, tmdO128, tmO128, tmK64, tmV64, tmK128, tmV128, tmQ64, tmdO64;
   if (int rc = encode(ds, &tmQ128, c.q, kD, c.S, nb * c.G, kBQ, "Q")) return rc;
   if (int rc = encode(ds, &tmdO128, c.dout, do_inner, c.S, do_planes, kBQ, "dO")) return rc;
+  if (int rc = encode(ds, &tmO128, c.o_in, do_inner, c.S, do_planes, kBQ, "O")) return rc;
   if (int rc = encode(ds, &tmK64, c.k, kD, c.S, nb, kBK, "K")) return rc;
   if (int rc = encode(ds, &tmV64, c.v, kD, c.S, nb, kBK, "V")) return rc;
   if (int rc = encode(ds, &tmK128, c.k, kD, c.S, nb, kBQ, "K block")) return rc;
@@ -2186,7 +2247,7 @@ int bwd_form(const Call& c, const DeviceState* ds, cudaStream_t st) {
   const int64_t n_tiles = static_cast<int64_t>(q_blocks(c.S)) * c.G * nb;   // (those that run take over the rest, see Walk)
   p.kv_parts = 1;
   MCB_CHECK_CUDA(launch_kernel(Form<CAP, BIAS>::dq, dim3(static_cast<unsigned>(n_tiles)), dim3(attn::kThreads), kDqSmem, st,
-                               chained_launch(), tmQ128, tmdO128, tmK64, tmV64, p, c));
+                               chained_launch(), tmQ128, tmdO128, tmO128, tmK64, tmV64, p, c));
   MCB_CHECK_LAUNCH("attn_dq_masked_kernel");
   p.kv_parts = masked_dkv_parts(nb, c.G, c.S, ds->sm_count);
   cudaLaunchConfig_t cfg = {};
