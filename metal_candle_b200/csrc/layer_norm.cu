@@ -53,8 +53,19 @@ __device__ __forceinline__ float row_sum(float v, float* buf) {
   }
   return v;
 }
+// Three at a time.  Where a warp has a row to itself two halves, then quarters of it take a sum each: nine exchanges instead of fifteen, in a
+// longer chain (which costs the larger rows' kernels more than the exchanges do: 16384 x 1024 float32, backward: 50 us, 47 without).
 template <int TPR>
 __device__ __forceinline__ float3 row_sum3(float3 v, float3* buf) {
+  if constexpr (TPR == 32) {
+    constexpr uint32_t all = 0xffffffffu;
+    const bool up = threadIdx.x & 16, right = threadIdx.x & 8;
+    const float xy = (up ? v.y : v.x) + __shfl_xor_sync(all, up ? v.x : v.y, 16), z = v.z + __shfl_xor_sync(all, v.z, 16);
+    float c = (right ? z : xy) + __shfl_xor_sync(all, right ? xy : z, 8);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) c += __shfl_xor_sync(all, c, o);
+    return make_float3(__shfl_sync(all, c, 0), __shfl_sync(all, c, 16), __shfl_sync(all, c, 8));
+  }
   v.x = lanes_sum<TPR>(v.x);
   v.y = lanes_sum<TPR>(v.y);
   v.z = lanes_sum<TPR>(v.z);
@@ -87,6 +98,7 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int LEFT>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
+constexpr bool staged(int tpr, int k) { return tpr == 32 && k == 4; }   // see the backward kernel
 constexpr int block_of(int tpr) { return tpr < 128 ? 128 : tpr; }
 constexpr int stages_of(int tpr, int k) { return k * block_of(tpr) > 1024 ? 2 : 3; }   // (three would not fit for three operands)
 
@@ -98,13 +110,18 @@ struct Rows {
   uint4* ring;
   int lane, nt, off, D, P, q;
   int64_t j, step, rows;
-  static size_t smem(int nt) { return static_cast<size_t>(STAGES) * nt * K * kBlock * 16; }
+  static __host__ __device__ size_t smem(int nt) { return static_cast<size_t>(STAGES) * nt * K * kBlock * 16; }
   __device__ __forceinline__ Rows(void* base, const Params& p, int nt_) : ring(static_cast<uint4*>(base)), nt(nt_), D(p.D), P(SHIFT ? p.period : 1), rows(p.rows) {
     lane = threadIdx.x % TPR;
     q = SHIFT ? blockIdx.x % P : 0;
     j = static_cast<int64_t>(blockIdx.x / P) * kRows + threadIdx.x / TPR;
     step = static_cast<int64_t>(gridDim.x / P) * kRows;
     off = SHIFT ? static_cast<int>(((reinterpret_cast<uintptr_t>(p.x) & 15) / sizeof(T) + static_cast<int64_t>(q) * D) % N) : 0;
+    // places of vectors that a row does not have are never loaded: they stay 0
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (!here(k))
+        for (int i = 0; i < STAGES * nt; ++i) ring[(static_cast<size_t>(i) * K + k) * kBlock + threadIdx.x] = make_uint4(0, 0, 0, 0);
   }
   __device__ __forceinline__ int64_t row(int64_t turn) const { return turn * P + q; }
   __device__ __forceinline__ bool any(int64_t turn) const { return (turn - threadIdx.x / TPR) * P + q < rows; }   // some row of the block's
@@ -127,15 +144,14 @@ struct Rows {
         cp_async16(ring + (static_cast<size_t>(stage * nt + t) * K + k) * kBlock + threadIdx.x, from, bytes);
       }
   }
-  // the vectors of a row as float32; elements outside the row are 0
-  __device__ __forceinline__ void get(int stage, int t, int64_t turn, float (&v)[K][N]) const {
-    const bool have = row(turn) < rows;
+  // the vectors of a row as float32; elements outside the row are 0 (what a row that does not exist has is anything)
+  __device__ __forceinline__ void get_vector(int stage, int t, int k, float (&f)[N]) const {
+    load(f, reinterpret_cast<const T*>(ring + (static_cast<size_t>(stage * nt + t) * K + k) * kBlock + threadIdx.x));
+  }
+  __device__ __forceinline__ void get(int stage, int t, float (&v)[K][N]) const {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-#pragma unroll
-      for (int e = 0; e < N; ++e) v[k][e] = 0.0f;
-      if (!have || !here(k)) continue;
-      load(v[k], reinterpret_cast<const T*>(ring + (static_cast<size_t>(stage * nt + t) * K + k) * kBlock + threadIdx.x));
+      get_vector(stage, t, k, v[k]);
       drop(v[k], k);
     }
   }
@@ -155,16 +171,13 @@ struct Rows {
   }
   // a vector of a weight [D], `none` where there is no weight
   __device__ __forceinline__ void weight(float (&f)[N], const T* w, int k, float none) const {
+    if (!SHIFT && w != nullptr) return load(f, w + col(k));
 #pragma unroll
     for (int e = 0; e < N; ++e) f[e] = none;
     if (w == nullptr) return;
-    if constexpr (SHIFT) {
 #pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (in(k, e)) f[e] = to_f32(w[col(k) + e]);
-    } else {
-      load(f, w + col(k));
-    }
+    for (int e = 0; e < N; ++e)
+      if (in(k, e)) f[e] = to_f32(w[col(k) + e]);
   }
   __device__ __forceinline__ void store(T* out, int64_t turn, int k, const float (&f)[N]) const {
     T* to = out + row(turn) * D + col(k);
@@ -192,22 +205,22 @@ __global__ void __launch_bounds__(block_of(TPR)) ln_fwd_kernel(const Params p) {
   R rows(smem4, p, 1);
   grid_launch_dependents();
   grid_dependency_wait();
+#pragma unroll
+  for (int i = 0; i < R::STAGES - 1; ++i) {
+    rows.fetch(i, 0, x, rows.j + i * rows.step);
+    cp_async_commit();
+  }
   // a moved weight is read element by element: once, into registers
   float fw[SHIFT ? K : 1][N], fb[SHIFT ? K : 1][N];
   if constexpr (SHIFT) {
 #pragma unroll
     for (int k = 0; k < K; ++k) { rows.weight(fw[k], w, k, 1.0f); rows.weight(fb[k], b, k, 0.0f); }
   }
-#pragma unroll
-  for (int i = 0; i < R::STAGES - 1; ++i) {
-    rows.fetch(i, 0, x, rows.j + i * rows.step);
-    cp_async_commit();
-  }
   int stage = 0;
   for (int64_t j = rows.j; rows.any(j); j += rows.step) {
     float v[K][N];
     cp_async_wait<R::STAGES - 2>();
-    rows.get(stage, 0, j, v);
+    rows.get(stage, 0, v);
     rows.fetch(stage == 0 ? R::STAGES - 1 : stage - 1, 0, x, j + (R::STAGES - 1) * rows.step);
     cp_async_commit();
     if (++stage == R::STAGES) stage = 0;
@@ -269,11 +282,6 @@ __global__ void __launch_bounds__(block_of(TPR), TPR == 256 ? 2 : 1) ln_bwd_kern
   };
   grid_launch_dependents();
   grid_dependency_wait();
-  float fw[SHIFT ? K : 1][N];
-  if constexpr (SHIFT) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) rows.weight(fw[k], w, k, 1.0f);
-  }
   float gw[SUMS ? K : 1][N], gb[SUMS ? K : 1][N];
 #pragma unroll
   for (int k = 0; k < (SUMS ? K : 1); ++k)
@@ -281,12 +289,42 @@ __global__ void __launch_bounds__(block_of(TPR), TPR == 256 ? 2 : 1) ln_bwd_kern
     for (int e = 0; e < N; ++e) gw[k][e] = gb[k][e] = 0.0f;
 #pragma unroll
   for (int i = 0; i < R::STAGES - 1; ++i) fetch(i, rows.j + i * rows.step);
+  // the weight of a vector: where a thread has four, float32 in shared memory behind the ring; else from L1, or, where the row's vectors are not the
+  // weight's, read element by element into registers once
+  constexpr bool STAGED = staged(TPR, K), KEPT = SHIFT && !STAGED;
+  float fw[KEPT ? K : 1][N];
+  float* ws = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(smem4) + R::smem(rows.nt));
+  if constexpr (KEPT) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) rows.weight(fw[k], w, k, 1.0f);
+  }
+  if constexpr (STAGED) {
+    for (int i = threadIdx.x; i < TPR * K * N; i += R::kBlock) {
+      const int c = i - rows.off;
+      ws[i] = static_cast<unsigned>(c) >= static_cast<unsigned>(p.D) ? 0.0f : w != nullptr ? to_f32(w[c]) : 1.0f;
+    }
+    __syncthreads();
+  }
+  auto weight = [&](float (&f)[N], int k) {
+    if constexpr (STAGED) {
+#pragma unroll
+      for (int e = 0; e < N; e += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(ws + N * (rows.lane + TPR * k) + e);
+        f[e] = v.x; f[e + 1] = v.y; f[e + 2] = v.z; f[e + 3] = v.w;
+      }
+    } else if constexpr (KEPT) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) f[e] = fw[k][e];
+    } else {
+      rows.weight(f, w, k, 1.0f);
+    }
+  };
   int stage = 0;
   for (int64_t j = rows.j; rows.any(j); j += rows.step) {
-    float v[K][N], d[K][N], r[K][N];
+    float v[K][N], d[K][N];
     cp_async_wait<R::STAGES - 2>();
-    rows.get(stage, 0, j, v);
-    rows.get(stage, 1, j, d);
+    rows.get(stage, 0, v);
+    rows.get(stage, 1, d);
     const int now = stage;
     fetch(stage == 0 ? R::STAGES - 1 : stage - 1, j + (R::STAGES - 1) * rows.step);
     if (++stage == R::STAGES) stage = 0;
@@ -301,13 +339,13 @@ __global__ void __launch_bounds__(block_of(TPR), TPR == 256 ? 2 : 1) ln_bwd_kern
     for (int k = 0; k < K; ++k) {
       if (!rows.here(k)) continue;
       float f[N];
-      if constexpr (!SHIFT) rows.weight(f, w, k, 1.0f);
+      weight(f, k);
 #pragma unroll
       for (int e = 0; e < N; e += 2) put2(&v[k][e], __fadd2_rn(two(&v[k][e]), both(-mean)));
       rows.drop(v[k], k);
 #pragma unroll
       for (int e = 0; e < N; e += 2) {
-        const float2 o = two(&v[k][e]), g = __fmul2_rn(two(&d[k][e]), two(SHIFT ? &fw[k][e] : &f[e]));
+        const float2 o = two(&v[k][e]), g = __fmul2_rn(two(&d[k][e]), two(&f[e]));
         sx = __ffma2_rn(o, o, sx);
         sy = __fadd2_rn(g, sy);
         sz = __ffma2_rn(g, o, sz);
@@ -317,12 +355,11 @@ __global__ void __launch_bounds__(block_of(TPR), TPR == 256 ? 2 : 1) ln_bwd_kern
     const float rstd = rsqrtf(s.x * inv + p.eps);
     const float a = s.y * inv, q = s.z * inv * rstd;
     if (rows.row(j) >= p.rows) continue;
-    if (res != nullptr) rows.get(now, 2, j, r);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (!rows.here(k)) continue;
       float f[N];
-      if constexpr (!SHIFT) rows.weight(f, w, k, 1.0f);   // (from L1 again: registers for it would cost occupancy)
+      weight(f, k);   // (again: registers for it would cost occupancy)
 #pragma unroll
       for (int e = 0; e < N; e += 2) {
         const float2 n = __fmul2_rn(two(&v[k][e]), both(rstd)), g = two(&d[k][e]);
@@ -330,8 +367,16 @@ __global__ void __launch_bounds__(block_of(TPR), TPR == 256 ? 2 : 1) ln_bwd_kern
           put2(&gw[k][e], __ffma2_rn(g, n, two(&gw[k][e])));
           put2(&gb[k][e], __fadd2_rn(g, two(&gb[k][e])));
         }
-        const float2 t = __ffma2_rn(n, both(-q), __ffma2_rn(g, two(SHIFT ? &fw[k][e] : &f[e]), both(-a)));
-        put2(&f[e], __ffma2_rn(t, both(rstd), res != nullptr ? two(&r[k][e]) : both(0.0f)));
+        put2(&f[e], __ffma2_rn(n, both(-q), __ffma2_rn(g, two(&f[e]), both(-a))));
+      }
+      if (res != nullptr) {
+        float r[N];
+        rows.get_vector(now, 2, k, r);
+#pragma unroll
+        for (int e = 0; e < N; e += 2) put2(&f[e], __ffma2_rn(two(&f[e]), both(rstd), two(&r[e])));
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; e += 2) put2(&f[e], __fmul2_rn(two(&f[e]), both(rstd)));
       }
       rows.store(dx, j, k, f);
     }
@@ -456,7 +501,8 @@ int blocks_for(int64_t rows, int per_block, int sms, int per_sm) {
 template <typename T, bool BWD, bool SHIFT, int TPR, int K>
 int launch_k(const Params& p, int sms, cudaStream_t st, int* blocks) {
   using R = Rows<T, TPR, K, SHIFT>;
-  size_t smem = R::smem(!BWD ? 1 : p.res != nullptr ? 3 : 2);
+  constexpr size_t kWeight = BWD && staged(TPR, K) ? static_cast<size_t>(TPR) * K * R::N * 4 : 0;
+  size_t smem = R::smem(!BWD ? 1 : p.res != nullptr ? 3 : 2) + kWeight;
   if (BWD && R::kRows > 1 && smem < 2 * static_cast<size_t>(p.D) * 4) smem = 2 * static_cast<size_t>(p.D) * 4;
   void (*kernel)(const Params) = ln_fwd_kernel<T, TPR, K, SHIFT>;
   if constexpr (BWD) kernel = p.part != nullptr ? ln_bwd_kernel<T, TPR, K, SHIFT, true> : ln_bwd_kernel<T, TPR, K, SHIFT, false>;
@@ -470,7 +516,7 @@ int launch_k(const Params& p, int sms, cudaStream_t st, int* blocks) {
   if (static_cast<uint32_t>(seen) == smem + 1) {
     per_sm = static_cast<int>(seen >> 32);
   } else {
-    const size_t most = R::smem(3) > smem ? R::smem(3) : smem;   // (of any call of this kernel: another thread's launch must not find less)
+    const size_t most = R::smem(3) + kWeight > smem ? R::smem(3) + kWeight : smem;   // (of any call of this kernel: another thread's launch must not find less)
     MCB_CHECK_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most)));
     MCB_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, R::kBlock, smem));
     if (dev < 64) known.store(static_cast<uint64_t>(per_sm) << 32 | (smem + 1), std::memory_order_relaxed);
@@ -482,15 +528,17 @@ int launch_k(const Params& p, int sms, cudaStream_t st, int* blocks) {
   MCB_CHECK_LAUNCH("layer_norm");
   return MCB_OK;
 }
-// A row's threads: as few as have at most two vectors of it each (32768 x 896 bfloat16, backward with its reduction: 64 threads with two
-// 64.5 us, 32 with four 83, 128 with one 68.6: the sums of a thread's columns are registers, and rows in flight go with the threads.  Forward: 32 with four 23 us, 64 with two 27).
+// A row's threads: as few as have at most two vectors of it each, but a warp for up to four where that was the faster: forward (32768 x 896
+// bfloat16, us: 32 threads with four 23, 64 with two 27), and backward of aligned bfloat16 rows, with the weight in shared memory (with the residual,
+// reduction included: 55, 64 with two 60, 128 with one 69; aligned float32 30000 x 512: 57, 64 with two 54; moved bfloat16 20000 x 1001: 64 and 54).
 template <typename T, bool BWD, bool SHIFT>
 int launch_rows(const Params& p, int vecs, int sms, cudaStream_t st, int* blocks) {
   if (vecs <= 8) return launch_k<T, BWD, SHIFT, 8, 1>(p, sms, st, blocks);
   if (vecs <= 16) return launch_k<T, BWD, SHIFT, 8, 2>(p, sms, st, blocks);
   if (vecs <= 32) return launch_k<T, BWD, SHIFT, 32, 1>(p, sms, st, blocks);
   if (vecs <= 64) return launch_k<T, BWD, SHIFT, 32, 2>(p, sms, st, blocks);
-  if (!BWD && vecs <= 128) return launch_k<T, BWD, SHIFT, 32, 4>(p, sms, st, blocks);
+  if constexpr (!BWD || (!SHIFT && sizeof(T) == 2))
+    if (vecs <= 128) return launch_k<T, BWD, SHIFT, 32, 4>(p, sms, st, blocks);
   if (vecs <= 128) return launch_k<T, BWD, SHIFT, 64, 2>(p, sms, st, blocks);
   if (vecs <= 256) return launch_k<T, BWD, SHIFT, 128, 2>(p, sms, st, blocks);
   if (vecs <= 512) return launch_k<T, BWD, SHIFT, 256, 2>(p, sms, st, blocks);
