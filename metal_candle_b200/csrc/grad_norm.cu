@@ -78,13 +78,17 @@ __device__ __forceinline__ double squares(const float (&v)[16]) {
 }
 
 template <typename T>
-__device__ __forceinline__ double piece_squares(const Tensor& t, int64_t at) {
+__device__ __forceinline__ void load_tensor(const Tensor& t, int64_t at, float (&v)[16]) {
   const T* g = static_cast<const T*>(t.g);
-  float v[16];
   // (off a boundary neighbouring threads take neighbouring elements, so that a warp's access is whole lines again)
   if ((reinterpret_cast<uintptr_t>(g) & 15u) == 0) load_piece<T, Vec16<T>::N, true>(g, t.n, at, v);
   else load_piece<T, 1, true>(g, t.n, at, v);
-  return squares(v);
+}
+__device__ __forceinline__ void load_number(const Table& tab, uint32_t piece, float (&v)[16]) {
+  const Tensor& t = tensor_of(tab, piece);
+  const int64_t at = static_cast<int64_t>(piece - t.first) * kPiece;
+  if (t.dtype == MCB_F32) load_tensor<float>(t, at, v);
+  else load_tensor<__nv_bfloat16>(t, at, v);
 }
 
 __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant__ Table tab, double* part) {
@@ -92,10 +96,18 @@ __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant
   grid_launch_dependents();
   grid_dependency_wait();
   double sum = 0.0;
-  for (uint32_t piece = blockIdx.x; piece < tab.pieces; piece += gridDim.x) {
-    const Tensor& t = tensor_of(tab, piece);
-    const int64_t at = static_cast<int64_t>(piece - t.first) * kPiece;
-    sum += t.dtype == MCB_F32 ? piece_squares<float>(t, at) : piece_squares<__nv_bfloat16>(t, at);
+  // the next piece is on its way while one is summed
+  float v[2][16];
+  uint32_t piece = blockIdx.x;
+  if (piece < tab.pieces) load_number(tab, piece, v[0]);
+  while (piece < tab.pieces) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (piece >= tab.pieces) break;
+      if (piece + gridDim.x < tab.pieces) load_number(tab, piece + gridDim.x, v[1 - i]);
+      sum += squares(v[i]);
+      piece += gridDim.x;
+    }
   }
   sum = block_sum(sum, s);
   if (threadIdx.x == 0) part[blockIdx.x] = sum;
@@ -110,18 +122,28 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const double* part, int 
 }
 
 // Pieces go by the output's 16-byte boundaries, the first few elements of a tensor by themselves: what is written are whole vectors
-// (written element by element, 250 M elements that lie off the gradients' alignment took 421 us instead of CLIP_US).
+// (written element by element, 250 M elements that lie off the gradients' alignment took 421 us instead of 350).
 template <typename T>
-__device__ __forceinline__ void clip_piece(const Tensor& t, int64_t piece, float f) {
+__device__ __forceinline__ int head_of(const Tensor& t) {
+  return static_cast<int>((16 - (reinterpret_cast<uintptr_t>(t.out) & 15u)) % 16 / sizeof(T));
+}
+template <typename T>
+__device__ __forceinline__ void load_for_clip(const Tensor& t, int64_t piece, float (&v)[16]) {
+  constexpr int N = Vec16<T>::N;
+  const T* g = static_cast<const T*>(t.g);
+  const int head = head_of<T>(t);
+  const int64_t at = head + piece * kPiece;
+  if ((reinterpret_cast<uintptr_t>(g + head) & 15u) == 0) load_piece<T, N, true>(g, t.n, at, v);
+  else load_piece<T, N, false>(g, t.n, at, v);
+}
+template <typename T>
+__device__ __forceinline__ void clip_piece(const Tensor& t, int64_t piece, float f, const float (&v)[16]) {
   constexpr int N = Vec16<T>::N;
   const T* g = static_cast<const T*>(t.g);
   T* out = static_cast<T*>(t.out);
-  const int head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(out) & 15u)) % 16 / sizeof(T));
+  const int head = head_of<T>(t);
   if (piece == 0 && static_cast<int>(threadIdx.x) < head && threadIdx.x < t.n) out[threadIdx.x] = from_f32<T>(to_f32(g[threadIdx.x]) * f);
   const int64_t at = head + piece * kPiece;
-  float v[16];
-  if ((reinterpret_cast<uintptr_t>(g + head) & 15u) == 0) load_piece<T, N, true>(g, t.n, at, v);
-  else load_piece<T, N, false>(g, t.n, at, v);
 #pragma unroll
   for (int k = 0; k < 16 / N; ++k) {
     const int64_t i = at + N * (threadIdx.x + kThreads * k);
@@ -144,14 +166,34 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ 
   __shared__ double s[kThreads / 32];
   grid_launch_dependents();
   grid_dependency_wait();
+  // from the last piece back: what the sums read last is still in L2
+  auto tensor = [&](uint32_t i, int64_t& piece) -> const Tensor& {
+    const Tensor& t = tensor_of(tab, tab.pieces - 1 - i);
+    piece = tab.pieces - 1 - i - t.first;
+    return t;
+  };
+  auto load = [&](uint32_t i, float (&v)[16]) {
+    int64_t piece;
+    const Tensor& t = tensor(i, piece);
+    if (t.dtype == MCB_F32) load_for_clip<float>(t, piece, v);
+    else load_for_clip<__nv_bfloat16>(t, piece, v);
+  };
+  float v[2][16];
+  uint32_t i = blockIdx.x;
   const float total = norm_of(part, parts, s), f = clip_factor(total, max_norm);
   if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = total;
-  // from the last piece back: what the sums read last is still in L2
-  for (uint32_t i = blockIdx.x; i < tab.pieces; i += gridDim.x) {
-    const uint32_t piece = tab.pieces - 1 - i;
-    const Tensor& t = tensor_of(tab, piece);
-    if (t.dtype == MCB_F32) clip_piece<float>(t, piece - t.first, f);
-    else clip_piece<__nv_bfloat16>(t, piece - t.first, f);
+  if (i < tab.pieces) load(i, v[0]);
+  while (i < tab.pieces) {
+#pragma unroll
+    for (int turn = 0; turn < 2; ++turn) {
+      if (i >= tab.pieces) break;
+      if (i + gridDim.x < tab.pieces) load(i + gridDim.x, v[1 - turn]);
+      int64_t piece;
+      const Tensor& t = tensor(i, piece);
+      if (t.dtype == MCB_F32) clip_piece<float>(t, piece, f, v[turn]);
+      else clip_piece<__nv_bfloat16>(t, piece, f, v[turn]);
+      i += gridDim.x;
+    }
   }
 }
 
