@@ -13,6 +13,8 @@
 // HBM-bound by the table's gradient (float32, written whole) where it is not accumulated.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace cg = cooperative_groups;
@@ -295,62 +297,64 @@ __device__ __forceinline__ void zero_rows(const SumParams& p, const uint32_t* ke
   }
 }
 
+template <typename T>
+struct One {   // (as Vec16)
+  T raw;
+  __device__ __forceinline__ void to_float(float* f) const { f[0] = to_f32(raw); }
+};
+__host__ __device__ constexpr int list_words(int tile) { return 2 * tile + 2; }
+
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads) sum_kernel(const __grid_constant__ SumParams p) {
-  __shared__ uint32_t s_key[kThreads][kMaxTile + 2], s_pos[kThreads][kMaxTile];   // by tile of the block (at most kThreads of them)
+  extern __shared__ uint32_t lists[];   // by tile of the block: its keys with one on either side, its positions
   const int x = threadIdx.x % p.tx, y = threadIdx.x / p.tx, ty = kThreads / p.tx;
   const int64_t t = static_cast<int64_t>(blockIdx.x / p.cols) * ty + y;
   grid_launch_dependents();
   grid_dependency_wait();
   const uint32_t *keys = from_here(p.key), *places = from_here(p.pos);
   if (blockIdx.x >= static_cast<unsigned>(p.sum_blocks)) {
-    zero_rows(p, keys, p.early + static_cast<int64_t>(blockIdx.x - p.sum_blocks) * kZeroRows, s_key[0]);
+    zero_rows(p, keys, p.early + static_cast<int64_t>(blockIdx.x - p.sum_blocks) * kZeroRows, lists);
     return;
   }
+  uint32_t *s_key = lists + y * list_words(p.tile), *s_pos = s_key + p.tile + 2;
   const int64_t i0 = t * p.tile;
   const int n = t < p.tiles ? static_cast<int>(i0 + p.tile < p.M ? p.tile : p.M - i0) : 0;
   const uint32_t none = static_cast<uint32_t>(p.vocab);
   // keys of the tile with one on either side
   for (int i = x; i < n + 2 && n > 0; i += p.tx) {
     const int64_t at = i0 + i - 1;
-    s_key[y][i] = at >= 0 && at < p.M ? __ldcg(keys + at) : none;
-    if (i >= 1 && i <= n) s_pos[y][i - 1] = __ldcg(places + at);
+    s_key[i] = at >= 0 && at < p.M ? __ldcg(keys + at) : none;
+    if (i >= 1 && i <= n) s_pos[i - 1] = __ldcg(places + at);
   }
   __syncthreads();
   if (n == 0) return;
   const int64_t c = N * (static_cast<int64_t>(blockIdx.x % p.cols) * p.tx + x);
   if (c >= p.H) return;
   const T* dout = static_cast<const T*>(p.dout) + c;
-  const bool began = s_key[y][0] == s_key[y][1], goes_on = s_key[y][n] == s_key[y][n + 1] && i0 + n < p.M;
+  const bool began = s_key[0] == s_key[1], goes_on = s_key[n] == s_key[n + 1] && i0 + n < p.M;
   float acc[N] = {};
   bool first = true;   // still in the tile's first run
   constexpr int kAhead = 8;
   for (int b = 0; b < n; b += kAhead) {
-    float v[kAhead][N];
+    std::conditional_t<N == 1, One<T>, Vec16<T>> v[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-#pragma unroll
-      for (int e = 0; e < N; ++e) v[k][e] = 0.0f;
-      if (b + k < n && s_key[y][b + k + 1] != none) {
-        const T* src = dout + static_cast<int64_t>(s_pos[y][b + k]) * p.H;
-        if constexpr (N == 1) {
-          v[k][0] = to_f32(*src);
-        } else {
-          Vec16<T> r;
-          r.raw = *reinterpret_cast<const decltype(r.raw)*>(src);
-          r.to_float(v[k]);
-        }
-      }
+      if constexpr (N == 1) v[k].raw = from_f32<T>(0.0f);
+      else v[k].raw = {};
+      if (b + k < n && s_key[b + k + 1] != none)
+        v[k].raw = *reinterpret_cast<const decltype(v[k].raw)*>(dout + static_cast<int64_t>(s_pos[b + k]) * p.H);
     }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       const int i = b + k;
       if (i >= n) break;
-      const uint32_t id = s_key[y][i + 1];
+      const uint32_t id = s_key[i + 1];
+      float f[N];
+      v[k].to_float(f);
 #pragma unroll
-      for (int e = 0; e < N; ++e) acc[e] += v[k][e];
+      for (int e = 0; e < N; ++e) acc[e] += f[e];
       const bool last = i == n - 1;
-      if (!last && s_key[y][i + 2] == id) continue;
+      if (!last && s_key[i + 2] == id) continue;
       // the run ends here, or goes on behind the tile
       if (id != none) {
         if (first && began && i0 > 0) put<N>(p.part + (2 * t) * p.H + c, acc);
@@ -413,7 +417,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 }
 
 inline size_t up256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
-// Sorted tokens of a tile: short tiles keep all SMs busy with few tokens (8192 tokens of 896, us: 8 SHORT, 32 LONG), long ones leave
+// Sorted tokens of a tile: short tiles keep all SMs busy with few tokens (sums of 8192 tokens of 896, us: 16 with tiles of 8, 25 with 32), long ones leave
 // fewer parts to join.
 inline int tile_of(int64_t M) { return M <= 16384 ? 8 : M <= 65536 ? 16 : kMaxTile; }
 inline int64_t tiles_of(int64_t M) { return (M + tile_of(M) - 1) / tile_of(M); }
@@ -455,7 +459,8 @@ int launch_sums(SumParams& p, cudaStream_t st) {
   const int64_t sums = (p.tiles + ty - 1) / ty * cols, zeros = (p.vocab - p.early + kZeroRows - 1) / kZeroRows;
   if (cols > 65535 || sums + zeros > 0x7fffffff) return fail(MCB_ERR_SHAPE, "embedding_bwd: H=%lld", (long long)p.H);
   p.cols = static_cast<int>(cols); p.sum_blocks = static_cast<int>(sums);
-  MCB_CHECK_CUDA(launch_kernel(sum_kernel<T, N>, dim3(static_cast<unsigned>(sums + zeros)), dim3(kThreads), 0, st, chained_launch(), p));
+  MCB_CHECK_CUDA(launch_kernel(sum_kernel<T, N>, dim3(static_cast<unsigned>(sums + zeros)), dim3(kThreads),
+                               static_cast<size_t>(ty) * list_words(p.tile) * 4, st, chained_launch(), p));
   MCB_CHECK_LAUNCH("embedding_sum");
   if (p.tiles > 1) {
     MCB_CHECK_CUDA(launch_kernel(join_kernel<N>, dim3(static_cast<unsigned>(p.tiles), static_cast<unsigned>(cols)), dim3(kJoinThreads), 0, st, chained_launch(), p));
