@@ -5,7 +5,8 @@
 // which flash_attn.cu takes to the tensor cores.
 //
 // CUDA-core kernels: tiles of 32 x 64, 256 threads, a thread has rows ty + 16 i and columns tx + 16 j of a product (two by four: the longest
-// block's chain of tiles is what a launch takes at the sizes this is for, 12 heads x 1200 positions, forward: HERE us, 64 x 64 tiles by 256 threads 282).  Tiles are float32 rows of D + 4 elements: the
+// block's chain of tiles is what a launch takes at the sizes this is for, 12 heads x 1200 positions, forward: 184 us, 64 x 64 tiles by 256
+// threads 282).  Bound by the operands' way from shared memory: 12 of 72 TFLOP/s.  Tiles are float32 rows of D + 4 elements: the
 // four extra put the sixteen rows that a half warp reads on different banks for every D that is a multiple of 8.  One pass over the
 // keys that some row of the tile sees, with the running maximum and sum; nothing of size seq x seq is stored and no sum uses
 // atomics.  The backward pass is a kernel by query tiles (dq, and delta and lse for the other) and one by key tiles (dk, dv).
@@ -528,7 +529,7 @@ int launch_bwd(const Call& c, int sms, cudaStream_t st) {
   const int64_t quarters = 4 * amask::tiles_of(c.S) * c.B;
   if (int rc = launch_one(c.D <= 64 ? masked_dq_kernel<T, 1> : masked_dq_kernel<T, 2>, "masked_dq_kernel", quarters * c.Hk * c.G, 1, smem_bwd(c.D), c, st)) return rc;
   // clusters share a key tile's steps as long as a part has one and there are not many blocks to an SM: the longest tile's chain of steps is what
-  // the launch takes (2 kv heads of 7 x 1200 positions of 80, whole backward pass: 2516 us unshared, SHARED by 8)
+  // the launch takes (2 kv heads of 7 x 1200 positions of 80, whole backward pass: 2516 us unshared, 722 by 8)
   const int64_t tiles = quarters * c.Hk, steps = static_cast<int64_t>(c.G) * ((c.S + kB - 1) / kB);
   int parts = 1;
   while (parts < 8 && tiles * parts * 2 <= 8 * sms && parts * 2 <= steps) parts *= 2;
