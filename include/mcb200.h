@@ -395,7 +395,7 @@ typedef struct {
 int mcb_attention_masked_fwd(const mcb_masked_attention* call, const void* q, const void* k, const void* v, void* o, float* lse,
                              void* stream);
 /* Gradients of the call above from its o and lse: dq like q, dk and dv like k (summed over the group); the slopes have none.
- * workspace: mcb_attention_masked_workspace_bytes from a 1024-byte boundary. */
+ * workspace: mcb_attention_masked_workspace_bytes from a 1024-byte boundary.  In both calls no output may overlap an input or another output. */
 size_t mcb_attention_masked_workspace_bytes(const mcb_masked_attention* call);
 int mcb_attention_masked_bwd(const mcb_masked_attention* call, const void* q, const void* k, const void* v, const void* o,
                              const float* lse, const void* dout, void* dq, void* dk, void* dv, void* workspace,

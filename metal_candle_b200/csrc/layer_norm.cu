@@ -507,11 +507,11 @@ int launch_k(const Params& p, int sms, cudaStream_t st, int* blocks) {
   void (*kernel)(const Params) = ln_fwd_kernel<T, TPR, K, SHIFT>;
   if constexpr (BWD) kernel = p.part != nullptr ? ln_bwd_kernel<T, TPR, K, SHIFT, true> : ln_bwd_kernel<T, TPR, K, SHIFT, false>;
   // as many blocks as are on the device at once (each leaves a line of sums), a whole number of rounds of the alignments; asked once for
-  // every kernel, device and size of shared memory (a word, so that threads that meet here read a whole answer)
-  static std::atomic<uint64_t> answer[2][64];
+  // every kernel, number of operands, device and size of shared memory (a word, so that threads that meet here read a whole answer)
+  static std::atomic<uint64_t> answer[4][64];
   int dev = 0, per_sm = 0;
   MCB_CHECK_CUDA(cudaGetDevice(&dev));
-  std::atomic<uint64_t>& known = answer[BWD && p.part != nullptr][dev & 63];
+  std::atomic<uint64_t>& known = answer[(BWD && p.part != nullptr) + 2 * (BWD && p.res != nullptr)][dev & 63];
   const uint64_t seen = known.load(std::memory_order_relaxed);
   if (static_cast<uint32_t>(seen) == smem + 1) {
     per_sm = static_cast<int>(seen >> 32);

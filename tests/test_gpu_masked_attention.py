@@ -356,3 +356,22 @@ def test_many_short_items(cuda_device):
     want = ref.attention(q, k, v, dout, ids, None, G, 0.125, 0.0, None, False, BF16, True)
     for name, value in want.items():
         ref.check(got[name], value, name)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_sequences_beyond_one_launch_of_the_mask(cuda_device, dtype):
+    """40000 positions: the mask is made in two launches; documents at the start, across position 32768 and at the end."""
+    S, Hk, G, d = 40000, 1, 2, 64
+    rng, ids, spans = random.Random(5), [], []
+    while len(ids) < S:
+        n = min(S - len(ids), rng.randint(1, 400))
+        spans.append((len(ids), len(ids) + n))
+        ids += [len(spans) % 3] * n
+    q, k, v, dout = inputs(cuda_device, 1, S, Hk, G, d, dtype, False, 9)
+    got = run(q, k, v, dout, G, 0.125, mask_of(cuda_device, [ids], None), 0.0, None, False)
+    for a, e in [spans[0], next(s for s in spans if s[0] <= 32768 < s[1]), spans[-1]]:
+        part = lambda t, n: t.view(n, S, -1)[:, a:e].reshape(1, n * (e - a), -1).contiguous()  # noqa: E731
+        want = ref.attention(part(q, G), part(k, 1), part(v, 1), part(dout, G), [[0] * (e - a)], None, G, 0.125, 0.0, None, False, dtype, dtype == BF16)
+        for name, n in (("o", G), ("dq", G), ("dk", 1), ("dv", 1)):
+            ref.check(part(got[name], n), want[name], f"{name} of [{a}, {e})")
+        ref.check(got["lse"].view(G, S)[:, a:e].reshape(1, -1), want["lse"], "lse")

@@ -80,4 +80,24 @@ def test_refusals(cuda_device):
         with model.packed(docs[0]):
             pass
     assert model._mask is None
+    with pytest.raises(TrainingError, match="prefix"):
+        with model.packed(docs, torch.zeros_like(docs[:, 1:], dtype=torch.uint8)):
+            pass
+    assert model._mask is None
     model.forward(ids[:, :-1].contiguous())
+
+
+def test_blocks_within_blocks_and_after_an_error(cuda_device):
+    model, ids, targets, _ = small_model(cuda_device, torch.bfloat16)
+    one, many = torch.zeros_like(ids), torch.arange(ids.shape[1], device=cuda_device, dtype=ids.dtype).expand_as(ids).contiguous() // 4
+    plain = model.forward(ids)
+    with model.packed(many):
+        apart = model.forward(ids)
+        with model.packed(one):
+            whole = model.forward(ids)
+        assert torch.equal(model.forward(ids), apart)
+    with pytest.raises(KeyError):
+        with model.packed(many):
+            raise KeyError("a step that failed")
+    assert torch.equal(model.forward(ids), plain)
+    assert not torch.equal(whole, apart) and torch.equal(whole[:, :4], apart[:, :4])

@@ -396,3 +396,50 @@ def test_a_training_step_over_packed_documents(cuda_device):
         step = 1e-2 * moment / (square.sqrt() + 1e-8) + 1e-2 * 0.01 * before.cpu().double()
         clear = g.abs() > 1e-4
         assert clear.any() and ((before - after).cpu().double() - step)[clear].abs().max() <= 1e-5
+
+
+def test_chained_launches_change_nothing(cuda_device):
+    """Kernels launched while the one before still runs, against launches that wait for it: every call reads what the last one wrote."""
+    from metal_candle_b200 import _lib
+
+    lib = _lib.load()
+    B, S, Hk, G, d, V = 2, 300, 2, 3, 64, 500
+    D = Hk * G * d
+    gen = torch.Generator(device=cuda_device).manual_seed(8)
+    ids = torch.randint(-1, V, (B, S), device=cuda_device, generator=gen, dtype=torch.int32)
+    docs = (torch.arange(S, device=cuda_device) // 70).expand(B, S).contiguous()
+    begin = {dtype: (rand(cuda_device, V, D, seed=1, dtype=dtype), rand(cuda_device, D, seed=2, dtype=dtype)) for dtype in (BF16, F32)}
+
+    def chain():
+        out = []
+        for dtype, (table, w) in begin.items():
+            for _ in range(2):
+                mask = backend.attention_mask(docs)
+                x = backend.embedding(ids, table, 2.0).view(B * S, D)
+                n = backend.layer_norm_fused(x, w, w)
+                q = n.view(B * Hk, G * S, d)
+                k = q[:, :S].contiguous()
+                how = dict(groups=G, scale=0.125, mask=mask, token_major=True)
+                o, lse = backend.attention_masked_forward(q, k, k, **how)
+                dq, dk, dv = backend.attention_masked_backward(q, k, k, o, lse, n, **how)
+                dx, dw, db = backend.layer_norm_backward(x, w, dq.view(B * S, D), dx_residual=n)
+                grad = backend.embedding_backward(ids, dx.view(B, S, D), V, 2.0)
+                norm = clip_grad_norm([grad, dw, db, dk, dv], 1.0)
+                table, w = grad.to(dtype), (w + dw.to(dtype))
+                out += [o, lse, dq, dk, dv, dx, dw, db, grad, norm]
+        return out
+
+    try:
+        _lib.check(lib.mcb_set_option(_lib.MCB_OPT_PDL, 0))
+        want = chain()
+        torch.cuda.synchronize()
+    finally:
+        _lib.check(lib.mcb_set_option(_lib.MCB_OPT_PDL, 1))
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(chain(), want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = chain()
+    for _ in range(3):
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(captured, want))

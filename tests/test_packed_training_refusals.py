@@ -62,19 +62,39 @@ def test_attention_pointers(lib):
     assert lib.mcb_attention_masked_fwd(None, 16, 16, 16, 16, None, None) == NULL
     for i in range(4):
         for value, status in ((None, NULL), (24, ALIGN)):
-            args = [16] * 4
+            args = [(i + 2) << 41 for i in range(4)]
             args[i] = value
             assert lib.mcb_attention_masked_fwd(C.byref(call), *args, None, None) == status
     for i in range(9):
-        args = [16] * 9
+        args = [(i + 2) << 41 for i in range(9)]
         args[i] = None
-        assert lib.mcb_attention_masked_bwd(C.byref(call), *args, 1024, HUGE, None) == NULL
-        args[i] = 24
-        assert lib.mcb_attention_masked_bwd(C.byref(call), *args, 1024, HUGE, None) == (ALIGN if i != 4 else NOT_INIT)   # lse is float32
+        assert lib.mcb_attention_masked_bwd(C.byref(call), *args, 1 << 50, HUGE, None) == NULL
+        args[i] = 24 + (1 << 52)
+        assert lib.mcb_attention_masked_bwd(C.byref(call), *args, 1 << 50, HUGE, None) == (ALIGN if i != 4 else NOT_INIT)   # lse is float32
     need = lib.mcb_attention_masked_workspace_bytes(C.byref(call))
     assert need >= 2 * 2 * 2 * 3 * 100 * 4
     for ws, n in ((None, HUGE), (1024, need - 1), (1040, HUGE)):
-        assert lib.mcb_attention_masked_bwd(C.byref(call), *[16] * 9, ws, n, None) == WORKSPACE
+        assert lib.mcb_attention_masked_bwd(C.byref(call), *[(i + 2) << 41 for i in range(9)], ws, n, None) == WORKSPACE
+
+
+def test_attention_outputs_overlap_nothing(lib):
+    call = attention()
+    size = 2 * 2 * 3 * 100 * 64 * (4 if call.dtype == 0 else 2)   # of q
+    assert size == call.batch * call.kv_heads * call.groups * call.seq * call.head_dim * (4 if call.dtype == 0 else 2)
+    far = [(i + 2) << 41 for i in range(9)]
+    fwd = lambda *a: lib.mcb_attention_masked_fwd(C.byref(call), *a, None)                 # noqa: E731
+    bwd = lambda *a: lib.mcb_attention_masked_bwd(C.byref(call), *a, 1 << 50, HUGE, None)   # noqa: E731
+    assert fwd(*far[:5]) == bwd(*far) == NOT_INIT
+    for other in (far[0], far[1], far[2]):
+        assert fwd(*far[:3], other, far[4]) == SHAPE and fwd(*far[:4], other + 16) == SHAPE
+    assert fwd(far[0], far[1], far[2], far[0] + size - 16, None) == SHAPE and fwd(far[0], far[1], far[2], far[0] + size, None) == NOT_INIT
+    assert fwd(far[0], far[1], far[2], far[0] - size, None) == NOT_INIT
+    for out in (6, 7, 8):
+        for i in range(9):
+            args = list(far)
+            args[out] = args[i]
+            assert bwd(*args) == (NOT_INIT if i == out else SHAPE)
+    assert lib.mcb_attention_masked_bwd(C.byref(call), *far, far[0], HUGE, None) == SHAPE
 
 
 def test_layer_norm(lib):
