@@ -375,3 +375,27 @@ def test_sequences_beyond_one_launch_of_the_mask(cuda_device, dtype):
         for name, n in (("o", G), ("dq", G), ("dk", 1), ("dv", 1)):
             ref.check(part(got[name], n), want[name], f"{name} of [{a}, {e})")
         ref.check(got["lse"].view(G, S)[:, a:e].reshape(1, -1), want["lse"], "lse")
+
+
+def test_ids_of_64_bits(cuda_device):
+    """Neighbouring documents whose ids agree in their low 32 bits are two, and so is a negative id whose low half is not."""
+    ids = [0] * 5 + [1 << 32] * 7 + [(1 << 32) + 1] * 3 + [1] * 9 + [-(1 << 32) + 1] * 4 + [1] * 6 + [(1 << 63) - 1] * 8
+    small = [0] * 5 + [1] * 7 + [2] * 3 + [3] * 9 + [-1] * 4 + [3] * 6 + [4] * 8
+    n = 4 * len(ids)
+    a, b = (mask_of(cuda_device, [x], None, torch.int64).block.view(torch.int32)[:n] for x in (ids, small))
+    assert torch.equal(a, b)
+
+
+def test_heads_beyond_2_to_the_31_elements(cuda_device):
+    """33 heads of a million positions in documents of 100: offsets pass 32 bits in q, o and the gradients."""
+    S, G, d, doc = 1 << 20, 33, 64, 100
+    gen = torch.Generator(device=cuda_device).manual_seed(1)
+    ids = (torch.arange(S, device=cuda_device, dtype=torch.int32) // doc).view(1, S)
+    rand = lambda *s: torch.randn(*s, device=cuda_device, generator=gen, dtype=BF16)  # noqa: E731
+    q, k, v, dout = rand(1, G * S, d), rand(1, S, d), rand(1, S, d), rand(1, G * S, d)
+    got = run(q, k, v, dout, G, 0.125, backend.attention_mask(ids), 0.0, None, False)
+    for first in (0, (S // 2) // doc * doc, S // doc * doc - doc):
+        part = lambda t, n: t.view(n, S, -1)[:, first:first + doc].reshape(1, n * doc, -1).contiguous()  # noqa: E731
+        want = ref.attention(part(q, G), part(k, 1), part(v, 1), part(dout, G), [[0] * doc], None, G, 0.125, 0.0, None, False, BF16, True)
+        for name, n in (("o", G), ("dq", G), ("dk", 1), ("dv", 1)):
+            ref.check(part(got[name], n), want[name], f"{name} from {first}")

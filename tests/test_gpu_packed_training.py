@@ -443,3 +443,51 @@ def test_chained_launches_change_nothing(cuda_device):
     for _ in range(3):
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(captured, want))
+
+
+def test_ids_of_64_bits_and_rows_beyond_2_to_the_31_elements(cuda_device):
+    """Ids whose low 32 bits alone would be in the vocabulary are outside it; a table of more than 2^31 elements is reached to its end."""
+    V, H = 600_001, 3600
+    table = torch.zeros(V, H, dtype=BF16, device=cuda_device)
+    table[V - 1] = rand(cuda_device, H, seed=1, dtype=BF16)
+    table[7] = 3.0
+    ids = torch.tensor([V - 1, 7, (1 << 32) + 7, -(1 << 32) + 7, V, V - 1, -1], device=cuda_device)
+    out = backend.embedding(ids, table, 2.0)
+    assert torch.equal(out[0], table[V - 1] * 2) and torch.equal(out[5], out[0]) and (out[1] == 6.0).all()
+    assert (out[[2, 3, 4, 6]] == 0).all()
+    del table
+    grad = torch.full((V, H), math.nan, device=cuda_device)
+    dout = rand(cuda_device, 7, H, seed=2)
+    backend.embedding_backward(ids, dout, V, 1.0, grad=grad)
+    assert torch.equal(grad[V - 1], dout[0] + dout[5]) and torch.equal(grad[7], dout[1])
+    grad[V - 1], grad[7] = 0.0, 0.0
+    assert all(int(torch.count_nonzero(part)) == 0 for part in grad.split(100_000))
+
+
+def test_layer_norm_beyond_2_to_the_31_elements(cuda_device):
+    rows, D = 2_400_000, 904
+    x = torch.empty(rows, D, dtype=BF16, device=cuda_device)
+    head, tail = rand(cuda_device, 300, D, seed=1, dtype=BF16), rand(cuda_device, 300, D, seed=2, dtype=BF16)
+    x.zero_()
+    x[:300], x[-300:] = head, tail
+    dy = torch.zeros_like(x)
+    dy[:300], dy[-300:] = tail, head
+    w = rand(cuda_device, D, seed=3, dtype=BF16)
+    y = backend.layer_norm_fused(x, w, w)
+    dx, dw, db = backend.layer_norm_backward(x, w, dy)
+    want = layer_norm_64(torch.cat([head, tail]), w, w, torch.cat([tail, head]), None, 1e-5, BF16)
+    ref.check(torch.cat([y[:300], y[-300:]]), want["y"], "y")
+    ref.check(torch.cat([dx[:300], dx[-300:]]), want["dx"], "dx")
+    for name, t in (("dw", dw), ("db", db)):   # rows of zeros add exact zeros: the sums are those of the 600 rows, in another order
+        ref.check(t, want[name], name)
+
+
+def test_clipping_beyond_2_to_the_31_elements(cuda_device):
+    n = (1 << 31) + 4099
+    g = torch.zeros(n, dtype=BF16, device=cuda_device)
+    g[0], g[1 << 31], g[-1] = 2.0, 6.0, 9.0
+    assert abs(float(clip_grad_norm([g], 1.1)) - 11.0) <= 11 * 2.0 ** -23
+    f = torch.tensor([2.0, 6.0, 9.0], dtype=BF16) * (1.1 / (11 + 1e-6))   # (a tenth of each, to a rounding of bfloat16)
+    got = torch.stack([g[0], g[1 << 31], g[-1]]).cpu()
+    assert ((got.float() - f.float()).abs() <= 2 * 2.0 ** -8 * f.float()).all()
+    assert int(torch.count_nonzero(g)) == 3
