@@ -1296,6 +1296,9 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
       more = walk.get(next);
       if (more) row_of(next);
       const float delta = exact.x + exact.y, put_right = rough - delta;
+      // one key alone has P = 1 whatever the score: no dq.  (Its dS in the next kernel is P dP (1 - P), the rounding of P; P = 1 set here would make that 0
+      // as well, and cost 2 to 5 % of the backward pass.)
+      const float scale = sees.y - sees.x == 1 ? 0.0f : p.scale;
       p.ndelta[prow] = -delta;
       ok = __all_sync(0xffffffffu, mbar_wait(dq_full, it & 1, abort_flag, 90, p.status));
       if (!ok) break;
@@ -1310,7 +1313,7 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float x = fmaf(put_right, __uint_as_float(kv[e]), __uint_as_float(qv[c4][e])) * p.scale;
+          const float x = fmaf(put_right, __uint_as_float(kv[e]), __uint_as_float(qv[c4][e])) * scale;
           qv[c4][e] = __float_as_uint(x);
           sum = fmaf(x, 0.0f, sum);
         }

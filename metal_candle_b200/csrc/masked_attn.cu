@@ -335,6 +335,7 @@ __global__ void __launch_bounds__(kThreads) masked_dq_kernel(const __grid_consta
       const int r = ty + 16 * i;
       const int2 sees = rows[r];
       const float lse2 = s_lse2[r], delta = s_delta[r];
+      const bool single = sees.y - sees.x == 1;   // P = 1 whatever the score: delta is its dP, to the bit, and dS = 0 here and in the next kernel
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int key = j0 + tx + 16 * j;
@@ -342,7 +343,9 @@ __global__ void __launch_bounds__(kThreads) masked_dq_kernel(const __grid_consta
         if (key >= sees.x && key < sees.y) {
           p = pair_p(c, s[i][j], slope2, abs(w.first + r - key), lse2, t);
           pt = p * t;
-          ds = p * (dp[i][j] - delta) * t;
+          if (single) p = fmaf(p, 0.0f, 1.0f);
+          pt = single ? 0.0f : pt;
+          ds = p * (single ? dp[i][j] * 0.0f : dp[i][j] - delta) * t;
           exact[i] = fmaf(p, dp[i][j], exact[i]);
         }
         sS[r * kLdP + tx + 16 * j] = ds;
@@ -357,9 +360,10 @@ __global__ void __launch_bounds__(kThreads) masked_dq_kernel(const __grid_consta
   for (int i = 0; i < kR; ++i) {
     const int s = w.first + ty + 16 * i;
     float put_right = 0.0f;
-    if constexpr (kExact) {
-      const float d = row_sum(exact[i]);
-      put_right = s_delta[ty + 16 * i] - d;
+    const float d = row_sum(exact[i]);
+    const int2 sees = rows[ty + 16 * i];
+    if constexpr (kExact) put_right = s_delta[ty + 16 * i] - d;
+    if (kExact || sees.y - sees.x == 1) {
       if (tx == 0) c.ndelta[((static_cast<int64_t>(w.b) * c.Hk + hk) * c.G + g) * pitch + s] = -d;
     }
     if (s >= c.S) continue;

@@ -377,6 +377,30 @@ def test_sequences_beyond_one_launch_of_the_mask(cuda_device, dtype):
         ref.check(got["lse"].view(G, S)[:, a:e].reshape(1, -1), want["lse"], "lse")
 
 
+@pytest.mark.parametrize("dtype,d", [(BF16, 64), (F32, 64), (F32, 40), (BF16, 128)])
+@pytest.mark.parametrize("softcap,bias", [(0.0, False), (30.0, True)])
+def test_documents_of_one_token(cuda_device, dtype, d, softcap, bias):
+    """A softmax over one key does not depend on the score: dq is 0, exactly, and so is dk (on the tensor cores up to the rounding of P)."""
+    exact = not (dtype == BF16 and d == 64)
+    B, S, Hk, G = 2, 150, 2, 3
+    q, k, v, dout = inputs(cuda_device, B, S, Hk, G, d, dtype, False, 21)
+    slopes = torch.rand(Hk * G, device=cuda_device) if bias else None
+    mask = mask_of(cuda_device, [list(range(S))] * B, None)
+    got = run(q, k, v, dout, G, d ** -0.5, mask, softcap, slopes, False)
+    assert int(torch.count_nonzero(got["dq"])) == 0 and (not exact or int(torch.count_nonzero(got["dk"])) == 0)
+    want = ref.attention(q, k, v, dout, [list(range(S))] * B, None, G, d ** -0.5, softcap, slopes, False, dtype, dtype == BF16 and d == 64)
+    for name in ("o", "lse", "dv", "dk"):
+        ref.check(got[name], want[name], name)
+    mixed = [[0] * 40 + list(range(1, 31)) + [31] * 80] * B
+    mask = mask_of(cuda_device, mixed, None)
+    got = run(q, k, v, dout, G, d ** -0.5, mask, softcap, slopes, False)
+    assert int(torch.count_nonzero(got["dq"].view(B, Hk, G, S, d)[..., [0, 40, 55, 69, 70], :])) == 0
+    assert not exact or int(torch.count_nonzero(got["dk"].view(B, Hk, S, d)[..., 40:70, :])) == 0
+    want = ref.attention(q, k, v, dout, mixed, None, G, d ** -0.5, softcap, slopes, False, dtype, dtype == BF16)
+    for name, value in want.items():
+        ref.check(got[name], value, name)
+
+
 def test_ids_of_64_bits(cuda_device):
     """Neighbouring documents whose ids agree in their low 32 bits are two, and so is a negative id whose low half is not."""
     ids = [0] * 5 + [1 << 32] * 7 + [(1 << 32) + 1] * 3 + [1] * 9 + [-(1 << 32) + 1] * 4 + [1] * 6 + [(1 << 63) - 1] * 8
