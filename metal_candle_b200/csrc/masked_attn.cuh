@@ -141,14 +141,19 @@ __device__ __noinline__ void dq_row(const Call& c, int b, int hk, int g, int s) 
         const float dp = go.dot(v), ds = pair_ds(c, q.dot(k), dp, slope2, abs(s - j), lse2, delta, p);
         if (turn == 0) {
           acc[0] = fmaf(p, dp, acc[0]);
-        } else if (ds != ds) {
-          acc[0] = acc[1] = acc[2] = acc[3] = ds;   // every element is NaN
+          if (acc[0] == acc[0]) {
+            if (j == sees.y - 1) { delta = acc[0]; acc[0] = 0.0f; }
+            continue;
+          }
+        }
+        if (turn == 0 || ds != ds) {   // delta, or a dS, is NaN: so is every element
+          acc[0] = acc[1] = acc[2] = acc[3] = turn == 0 ? acc[0] : ds;
+          turn = 2;
           break;
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[e] = fmaf(ds, k.v[e], acc[e]);
         }
-        if (turn == 0 && j == sees.y - 1) { delta = acc[0]; acc[0] = 0.0f; }
       }
   }
   row_store(static_cast<T*>(c.dq) + qr * c.D, acc, c.scale, c.D);
