@@ -78,7 +78,9 @@ constexpr uint32_t kOffV = kOffK + kFwdStages * kKBytes;
 constexpr uint32_t kOffBar = kOffV + kFwdStages * kKBytes;
 constexpr uint32_t kOffItems = kOffBar + 256;         // see Items
 constexpr uint32_t kItemsBytes = 128;
-constexpr uint32_t kFwdSmem = kOffItems + kItemsBytes + 1024;
+constexpr uint32_t kOffAgain = kOffItems + kItemsBytes;   // see Again
+constexpr uint32_t kAgainBytes = 544;
+constexpr uint32_t kFwdSmem = kOffAgain + kAgainBytes + 1024;
 
 struct FwdParams {
   int S, G, NB;
@@ -250,6 +252,47 @@ struct Items {
   }
 };
 
+// Rows that come out not finite are taken again from what they see (masked_attn.cuh), which takes as long as that is.  It is done behind the CTA's last
+// item, when nobody waits for anybody any more: within an item a row of some 10^5 positions would outlast the other warps' bounded waits.  A
+// warp notes such rows of its quadrant, and once one has, the loader takes over no more items: those that are left start as CTAs of their own.  The
+// loader hands on item n when all readers have item n - 2, and a warp takes item k + 1 before it notes rows of item k: item k + 5 is
+// asked for behind the note, so that a warp has at most five.
+struct Again {
+  static constexpr int kNotes = 8;
+  uint8_t* gen;   // notes [4][kNotes] of 16 bytes (sequence, query block, head, rows as bits), the four warps' numbers of them, whether there is any
+  __device__ __forceinline__ volatile int4* note(int quad, int i) const { return reinterpret_cast<volatile int4*>(gen) + quad * kNotes + i; }
+  __device__ __forceinline__ volatile int* count(int quad) const { return reinterpret_cast<volatile int*>(gen + 4 * kNotes * 16) + quad; }
+  __device__ __forceinline__ volatile int* any() const { return count(4); }
+  __device__ __forceinline__ void init() const {
+    for (int i = 0; i < 5; ++i) *count(i) = 0;
+  }
+  // by a whole warp
+  __device__ __forceinline__ void add(const FwdTile& w, int heads, int quad, bool bad) const {
+    const uint32_t rows = __ballot_sync(0xffffffffu, bad);
+    if (rows == 0 || (threadIdx.x & 31) != 0) return;
+    const int i = *count(quad);
+    volatile int4* at = note(quad, i);
+    at->x = w.b; at->y = w.qb; at->z = w.hk * heads + w.g; at->w = static_cast<int>(rows);
+    *count(quad) = i + 1;
+    *any() = 1;
+  }
+  // by all warps of the CTA, behind a barrier: row(sequence, kv head, head of its group, position) for every row that was noted, a warp to a row
+  template <typename F>
+  __device__ __forceinline__ void run(int heads, F&& row) const {
+    if (*any() == 0) return;
+    const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    int n = 0;
+    for (int quad = 0; quad < 4; ++quad)
+      for (int i = 0; i < *count(quad); ++i) {
+        volatile int4* at = note(quad, i);
+        const int b = at->x, first = at->y * kBQ + quad * 32, head = at->z;
+        for (uint32_t rows = static_cast<uint32_t>(at->w); rows != 0; rows &= rows - 1)
+          if (n++ % warps == warp) row(b, head / heads, head % heads, first + __ffs(rows) - 1);
+      }
+  }
+};
+static_assert(4 * Again::kNotes * 16 + 5 * 4 <= kAgainBytes, "room for the notes");
+
 template <bool MASKED>
 struct Walk;
 template <>
@@ -257,7 +300,7 @@ struct Walk<false> {
   const FwdParams& p;
   int t, n;
   bool back;
-  __device__ __forceinline__ Walk(const FwdParams& p_, const NoCall&, const Items&, volatile int*)
+  __device__ __forceinline__ Walk(const FwdParams& p_, const NoCall&, const Items&, const Again&, volatile int*)
       : p(p_), t(blockIdx.x), n(q_blocks(p_.S) * p_.G * p_.NB), back(false) {}
   __device__ __forceinline__ bool get_as_loader(FwdTile& w) { return get(w); }
   __device__ __forceinline__ bool get(FwdTile& w) {
@@ -273,11 +316,12 @@ struct Walk<true> {
   const FwdParams& p;
   const mattn::Call& c;
   const Items items;
+  const Again again;
   volatile int* abort_flag;
   int t, k;      // item, and how many came before it
   int4 rec;      // its record
-  __device__ __forceinline__ Walk(const FwdParams& p_, const mattn::Call& c_, const Items& i, volatile int* abort)
-      : p(p_), c(c_), items(i), abort_flag(abort), t(blockIdx.x), k(0), rec(c_.mask.qwork[blockIdx.x / (p_.G * c_.Hk)]) {}
+  __device__ __forceinline__ Walk(const FwdParams& p_, const mattn::Call& c_, const Items& i, const Again& a, volatile int* abort)
+      : p(p_), c(c_), items(i), again(a), abort_flag(abort), t(blockIdx.x), k(0), rec(c_.mask.qwork[blockIdx.x / (p_.G * c_.Hk)]) {}
   __device__ __forceinline__ void fill(FwdTile& w) const {
     const int r = t % (p.G * c.Hk);
     w.b = rec.x; w.qb = rec.y; w.kb0 = rec.z; w.nkb = rec.w;
@@ -290,11 +334,14 @@ struct Walk<true> {
   // asks as it starts takes over items whose CTAs would have started beside it (4 x 16 heads of 1024 positions, forward: 45 us, asked at the start 58)
   __device__ __forceinline__ bool get_as_loader(FwdTile& w) {
     if (k > 0) {
-      items.request();
-      if (!mbar_wait(items.asked(), (k - 1) & 1, abort_flag, 99, c.status)) return false;
-      t = items.answer();
-      fence_proxy_async_smem();   // (the next answer is written by another proxy)
-      if (t >= 0) rec = c.mask.qwork[t / (p.G * c.Hk)];
+      t = -1;
+      if (*again.any() == 0) {
+        items.request();
+        if (!mbar_wait(items.asked(), (k - 1) & 1, abort_flag, 99, c.status)) return false;
+        t = items.answer();
+        fence_proxy_async_smem();   // (the next answer is written by another proxy)
+        if (t >= 0) rec = c.mask.qwork[t / (p.G * c.Hk)];
+      }
       if (k >= 3 && !mbar_wait(items.empty(k), ((k - 3) >> 1) & 1, abort_flag, 100, c.status)) return false;
       volatile int4* at = items.record(k);
       at->x = rec.x; at->y = rec.y; at->z = rec.z; at->w = rec.w;
@@ -356,6 +403,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   const uint32_t s_full0 = kv_empty0 + 8 * kFwdStages, p_ready0 = s_full0 + 16, pv_done0 = p_ready0 + 16;
   const uint32_t s_free0 = pv_done0 + 16, tmem_slot = s_free0 + 16, abort_addr = tmem_slot + 4;
   const Items items = {base + kOffItems, gen_base + kOffItems};
+  const Again again = {gen_base + kOffAgain};
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(gen_base + (tmem_slot - base));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_base + (abort_addr - base));
 
@@ -367,7 +415,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     for (int s = 0; s < 2; ++s) {
       mbar_init(s_full0 + 8 * s, 1); mbar_init(p_ready0 + 8 * s, 4); mbar_init(pv_done0 + 8 * s, 1); mbar_init(s_free0 + 8 * s, 4);
     }
-    if (MASKED) items.init();
+    if (MASKED) { items.init(); again.init(); }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async_smem();
@@ -384,7 +432,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   grid_dependency_wait();   // the set-up above ran under the tail of the kernel before
   // S buffers at columns 0 and 64, O at 128, the two P buffers (bf16 pairs: 32 columns each) at 192 and 224
   const uint32_t tO = tmem_base + 128, tP0 = tmem_base + 192;
-  Walk<MASKED> walk(p, c, items, abort_flag);
+  Walk<MASKED> walk(p, c, items, again, abort_flag);
   FwdTile w;
 
   if (warp == 0) {
@@ -640,7 +688,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       if (lane == 0) mbar_arrive(o_free);   // the next item's products may overwrite O
       bool bad = false;
       if constexpr (MASKED) {
-        // a row that is not finite is taken again from what it sees (masked_attn.cuh)
+        // a row that is not finite is taken again from what it sees
         float sum = 0.0f;
 #pragma unroll
         for (int c4 = 0; c4 < 4; ++c4)
@@ -664,10 +712,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         }
         if (p.lse != nullptr) p.lse[w.qrow0 + row] = none ? -INFINITY : (m + lg2(l)) * kLn2;
       }
-      if constexpr (MASKED) {
-        for (uint32_t rows = __ballot_sync(0xffffffffu, bad); rows != 0; rows &= rows - 1)
-          mattn::fwd_row<__nv_bfloat16>(c, w.b, w.hk, w.g, w.qb * kBQ + quad * 32 + __ffs(rows) - 1);
-      }
+      if constexpr (MASKED) again.add(w, p.G, quad, bad);
       n0 += static_cast<uint32_t>(w.nkb);
     }
   }
@@ -682,6 +727,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     tcgen05_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(256u) : "memory");
   }
+  if constexpr (MASKED)
+    if (*abort_flag == 0) again.run(p.G, [&](int b, int hk, int g, int pos) { mattn::fwd_row<__nv_bfloat16>(c, b, hk, g, pos); });
 }
 
 
@@ -695,7 +742,8 @@ constexpr uint32_t kDqOffStage = kDqOffDO + kQBytes;     // stages of a K and a 
 constexpr uint32_t kDqStageBytes = 2 * kKBytes;
 constexpr uint32_t kDqOffBar = kDqOffStage + kDqStages * kDqStageBytes;
 constexpr uint32_t kDqOffItems = kDqOffBar + 256;
-constexpr uint32_t kDqSmem = kDqOffItems + kItemsBytes + 1024;
+constexpr uint32_t kDqOffAgain = kDqOffItems + kItemsBytes;
+constexpr uint32_t kDqSmem = kDqOffAgain + kAgainBytes + 1024;
 
 struct BwdParams {
   int S, G, NB;
@@ -998,6 +1046,7 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   const uint32_t s_full = kv_empty0 + 8 * kDqStages, p_ready = s_full + 8;
   const uint32_t dp_full = p_ready + 8, ds_ready = dp_full + 8, tmem_slot = ds_ready + 8, abort_addr = tmem_slot + 4;
   const Items items = {base + kDqOffItems, gen_base + kDqOffItems};
+  const Again again = {gen_base + kDqOffAgain};
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(gen_base + (tmem_slot - base));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_base + (abort_addr - base));
 
@@ -1012,6 +1061,7 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     mbar_init(dp_full, 1);
     mbar_init(ds_ready, 4);
     items.init();
+    again.init();
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async_smem();
@@ -1029,7 +1079,7 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   const uint32_t tS = tmem_base, tDP = tmem_base + 64, tDQ = tmem_base + 128, tPK = tmem_base + 192;
   FwdParams tp;   // the item order of the forward
   tp.S = p.S; tp.G = p.G; tp.NB = p.NB;
-  Walk<true> walk(tp, c, items, abort_flag);
+  Walk<true> walk(tp, c, items, again, abort_flag);
   FwdTile w;
 
   if (warp == 0) {
@@ -1333,8 +1383,7 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
           *reinterpret_cast<uint4*>(orow + 16 * c4 + 8) = make_uint4(ow[4], ow[5], ow[6], ow[7]);
         }
       }
-      for (uint32_t rows = __ballot_sync(0xffffffffu, bad); rows != 0; rows &= rows - 1)
-        mattn::dq_row<__nv_bfloat16>(c, w.b, w.hk, w.g, w.qb * kBQ + quad * 32 + __ffs(rows) - 1);
+      again.add(w, p.G, quad, bad);
     }
   }
 
@@ -1348,6 +1397,7 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     tcgen05_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(256u) : "memory");
   }
+  if (*abort_flag == 0) again.run(p.G, [&](int b, int hk, int g, int pos) { mattn::dq_row<__nv_bfloat16>(c, b, hk, g, pos); });
 }
 
 // ---------------------------------------------------------------------------------------------------------

@@ -60,47 +60,87 @@ __device__ __forceinline__ float score2(const Call& c, float dot, float slope2, 
 // that nothing has written behind a document, a diverged neighbour) makes the sum NaN although the row does not see it.  A row that
 // comes out not finite is therefore computed again from the positions that it sees alone, here.  With finite inputs none is, and a row
 // that is NaN by right (a diverged run) is left as soon as that shows.
-// Head dimensions up to 128: lane l has the elements l, l + 32, l + 64, l + 96.
+// 32 positions at a time: a lane takes the products of one of them by itself, then the warp adds their rows up, a lane the four elements from 4 l
+// on (head dimensions up to 128).  Bound by latency: 2 heads of 16384 positions with every row taken again 45 ms forward and 107 backward,
+// beside 0.2 and 0.47 where none is.  (Four rows and two pieces at a time, and no more: the kernels that call this hold its registers with theirs.
+// With eight each 36 and 92, but the forward of a finite 16384 with a prefix took 447 us instead of 402.)
 template <typename T>
-struct RowData {
-  float v[4];
-  __device__ __forceinline__ RowData(const T* p, int d) {
-    const int lane = threadIdx.x & 31;
+__device__ __forceinline__ float lane_dot(const T* a, const T* b, int d) {
+  constexpr int N = Vec16<T>::N;
+  float s = 0.0f;
+#pragma unroll 2
+  for (int at = 0; at < d; at += N) {
+    Vec16<T> x, y;
+    x.raw = *reinterpret_cast<const decltype(x.raw)*>(a + at);
+    y.raw = *reinterpret_cast<const decltype(y.raw)*>(b + at);
+    float fx[N], fy[N];
+    x.to_float(fx);
+    y.to_float(fy);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = lane + 32 * e < d ? to_f32(p[lane + 32 * e]) : 0.0f;
+    for (int e = 0; e < N; ++e) s = fmaf(fx[e], fy[e], s);
   }
-  __device__ __forceinline__ float dot(const RowData& o) const {
-    float s = 0.0f;
+  return s;
+}
+template <typename T>
+__device__ __forceinline__ void load4(float (&x)[4], const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u);
+    x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
+  }
+}
+// acc += the sum over the lanes i of `which` of their f times row i (`step` elements apart).  Every load is made,
+// of a row and a piece that exist, so that four are on their way at a time.
+template <typename T>
+__device__ __forceinline__ void add_rows(float (&acc)[4], float f, uint32_t which, const T* rows, int64_t step, int d) {
+  if (which == 0) return;
+  const int lane = threadIdx.x & 31, some = __ffs(which) - 1;
+  rows += min(4 * lane, d - 4);
+  for (int i0 = 0; i0 < 32; i0 += 4) {
+    if ((which >> i0 & 15u) == 0) continue;
+    float x[4][4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s = fmaf(v[e], o.v[e], s);
-    return warp_sum(s);
+    for (int i = 0; i < 4; ++i) load4(x[i], rows + ((which >> (i0 + i) & 1u) != 0 ? i0 + i : some) * step);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float w = __shfl_sync(0xffffffffu, f, i0 + i);
+      if ((which >> (i0 + i) & 1u) == 0) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, x[i][e], acc[e]);
+    }
   }
-};
+}
+__device__ __forceinline__ void all_nan(float (&v)[4]) { v[0] = v[1] = v[2] = v[3] = __int_as_float(0x7fffffff); }
 template <typename T>
 __device__ __forceinline__ void row_store(T* p, const float (&v)[4], float f, int d) {
-  const int lane = threadIdx.x & 31;
+  const int at = 4 * (threadIdx.x & 31);
+  if (at >= d) return;
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (lane + 32 * e < d) p[lane + 32 * e] = from_f32<T>(v[e] * f);
+  for (int e = 0; e < 4; ++e) p[at + e] = from_f32<T>(v[e] * f);
 }
 
 template <typename T>
 __device__ __noinline__ void fwd_row(const Call& c, int b, int hk, int g, int s) {
   const int2 sees = c.mask.rows[static_cast<int64_t>(b) * c.S + s];
-  const RowData<T> q(static_cast<const T*>(c.q) + q_row(c, b, hk, g, s) * c.D, c.D);
+  const int64_t kv = k_row(c, b, hk, 0) * c.D;
+  const T *q = static_cast<const T*>(c.q) + q_row(c, b, hk, g, s) * c.D, *k = static_cast<const T*>(c.k) + kv, *v = static_cast<const T*>(c.v) + kv;
   const float slope2 = c.slopes ? c.slopes[hk * c.G + g] * kLog2e : 0.0f;
   float m = kNoScore, l = 0.0f, acc[4] = {};
-  for (int j = sees.x; j < sees.y; ++j) {
-    const int64_t kr = k_row(c, b, hk, j) * c.D;
-    const RowData<T> k(static_cast<const T*>(c.k) + kr, c.D), v(static_cast<const T*>(c.v) + kr, c.D);
-    float bent;
-    const float t = score2(c, q.dot(k), slope2, abs(s - j), bent);
-    const float top = t > m ? t : m;   // (a NaN score leaves the maximum and makes the sums NaN)
-    const float old = exp2f(m - top), p = exp2f(t - top);
-    l = fmaf(l, old, p);
+  for (int j0 = sees.x; j0 < sees.y; j0 += 32) {
+    const int j = j0 + (threadIdx.x & 31);
+    const bool in = j < sees.y;
+    float t = -INFINITY, bent;
+    if (in) t = score2(c, lane_dot(q, k + static_cast<int64_t>(j) * c.D, c.D), slope2, abs(s - j), bent);
+    const float top = fmaxf(m, warp_max(t));   // (a NaN score leaves the maximum and makes the sums NaN)
+    const float old = exp2f(m - top), p = in ? exp2f(t - top) : 0.0f;
+    l = fmaf(l, old, warp_sum(p));
     if (l != l) break;   // (the same on all lanes) every element is NaN
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] = fmaf(p, v.v[e], acc[e] * old);
+    for (int e = 0; e < 4; ++e) acc[e] *= old;
+    add_rows(acc, p, __ballot_sync(0xffffffffu, in), v + static_cast<int64_t>(j0) * c.D, c.D, c.D);
     m = top;
   }
   const bool none = l == 0.0f;
@@ -127,35 +167,31 @@ __device__ __forceinline__ float pair_ds(const Call& c, float dot, float dp, flo
 template <typename T>
 __device__ __noinline__ void dq_row(const Call& c, int b, int hk, int g, int s) {
   const int2 sees = c.mask.rows[static_cast<int64_t>(b) * c.S + s];
-  const int64_t qr = q_row(c, b, hk, g, s), oa = o_at(c, b, hk, g, s);
-  const RowData<T> q(static_cast<const T*>(c.q) + qr * c.D, c.D), go(static_cast<const T*>(c.dout) + oa, c.D);
+  const int64_t qr = q_row(c, b, hk, g, s), kv = k_row(c, b, hk, 0) * c.D;
+  const T *q = static_cast<const T*>(c.q) + qr * c.D, *go = static_cast<const T*>(c.dout) + o_at(c, b, hk, g, s);
+  const T *k = static_cast<const T*>(c.k) + kv, *v = static_cast<const T*>(c.v) + kv;
   const float slope2 = c.slopes ? c.slopes[hk * c.G + g] * kLog2e : 0.0f, lse2 = c.lse[qr] * kLog2e;
-  float acc[4] = {};
-  if (lse2 != -INFINITY) {
-    float delta = 0.0f;
-    for (int turn = 0; turn < 2; ++turn)   // delta = sum of P dP first
-      for (int j = sees.x; j < sees.y; ++j) {
-        const int64_t kr = k_row(c, b, hk, j) * c.D;
-        const RowData<T> k(static_cast<const T*>(c.k) + kr, c.D), v(static_cast<const T*>(c.v) + kr, c.D);
+  float acc[4] = {}, delta = 0.0f;
+  bool nan = false;
+  for (int turn = 0; turn < 2 && !nan && lse2 != -INFINITY; ++turn) {   // delta = sum of P dP first
+    float part = 0.0f;
+    for (int j0 = sees.x; j0 < sees.y; j0 += 32) {
+      const int j = j0 + (threadIdx.x & 31);
+      const bool in = j < sees.y;
+      float ds = 0.0f;
+      if (in) {
         float p;
-        const float dp = go.dot(v), ds = pair_ds(c, q.dot(k), dp, slope2, abs(s - j), lse2, delta, p);
-        if (turn == 0) {
-          acc[0] = fmaf(p, dp, acc[0]);
-          if (acc[0] == acc[0]) {
-            if (j == sees.y - 1) { delta = acc[0]; acc[0] = 0.0f; }
-            continue;
-          }
-        }
-        if (turn == 0 || ds != ds) {   // delta, or a dS, is NaN: so is every element
-          acc[0] = acc[1] = acc[2] = acc[3] = turn == 0 ? acc[0] : ds;
-          turn = 2;
-          break;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e] = fmaf(ds, k.v[e], acc[e]);
-        }
+        const float dp = lane_dot(go, v + static_cast<int64_t>(j) * c.D, c.D);
+        ds = pair_ds(c, lane_dot(q, k + static_cast<int64_t>(j) * c.D, c.D), dp, slope2, abs(s - j), lse2, delta, p);
+        if (turn == 0) ds = part = fmaf(p, dp, part);
       }
+      nan = __any_sync(0xffffffffu, ds != ds);   // delta, or a dS: every element is NaN
+      if (nan) break;
+      if (turn == 1) add_rows(acc, ds, __ballot_sync(0xffffffffu, in), k + static_cast<int64_t>(j0) * c.D, c.D, c.D);
+    }
+    delta = warp_sum(part);
   }
+  if (nan) all_nan(acc);
   row_store(static_cast<T*>(c.dq) + qr * c.D, acc, c.scale, c.D);
 }
 
@@ -163,30 +199,30 @@ __device__ __noinline__ void dq_row(const Call& c, int b, int hk, int g, int s) 
 template <typename T>
 __device__ __noinline__ void dkv_row(const Call& c, int b, int hk, int s) {
   const int2 seen = c.mask.keys[static_cast<int64_t>(b) * c.S + s];
-  const int64_t kr = k_row(c, b, hk, s) * c.D, pitch = amask::tiles_of(c.S) * amask::kTile;
-  const RowData<T> k(static_cast<const T*>(c.k) + kr, c.D), v(static_cast<const T*>(c.v) + kr, c.D);
+  const int64_t kr = k_row(c, b, hk, s) * c.D, pitch = amask::tiles_of(c.S) * amask::kTile, ostep = c.o_tok ? static_cast<int64_t>(c.Hk) * c.G * c.D : c.D;
+  const T *k = static_cast<const T*>(c.k) + kr, *v = static_cast<const T*>(c.v) + kr;
   float gk[4] = {}, gv[4] = {};
-  for (int g = 0; g < c.G; ++g) {
+  bool nan = false;
+  for (int g = 0; g < c.G && !nan; ++g) {
     const float slope2 = c.slopes ? c.slopes[hk * c.G + g] * kLog2e : 0.0f;
-    for (int i = seen.x; i < seen.y; ++i) {
-      const int64_t at = ((static_cast<int64_t>(b) * c.Hk + hk) * c.G + g) * pitch + i;
-      const float lse2 = -c.nlse2[at];
-      if (lse2 == INFINITY) continue;
-      const RowData<T> q(static_cast<const T*>(c.q) + q_row(c, b, hk, g, i) * c.D, c.D), go(static_cast<const T*>(c.dout) + o_at(c, b, hk, g, i), c.D);
-      float p;
-      const float ds = pair_ds(c, q.dot(k), go.dot(v), slope2, abs(s - i), lse2, -c.ndelta[at], p);
-      if (p != p) {   // every element of both is NaN
-        g = c.G;
-        for (int e = 0; e < 4; ++e) gk[e] = gv[e] = p;
-        break;
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        gk[e] = fmaf(ds, q.v[e], gk[e]);
-        gv[e] = fmaf(p, go.v[e], gv[e]);
-      }
+    const T *q = static_cast<const T*>(c.q) + q_row(c, b, hk, g, 0) * c.D, *go = static_cast<const T*>(c.dout) + o_at(c, b, hk, g, 0);
+    const int64_t first = ((static_cast<int64_t>(b) * c.Hk + hk) * c.G + g) * pitch;
+    for (int i0 = seen.x; i0 < seen.y; i0 += 32) {
+      const int i = i0 + (threadIdx.x & 31);
+      const float lse2 = i < seen.y ? -c.nlse2[first + i] : INFINITY;
+      const bool in = lse2 != INFINITY;
+      float p = 0.0f, ds = 0.0f;
+      if (in)
+        ds = pair_ds(c, lane_dot(k, q + static_cast<int64_t>(i) * c.D, c.D), lane_dot(v, go + i * ostep, c.D), slope2, abs(s - i), lse2,
+                     -c.ndelta[first + i], p);
+      nan = __any_sync(0xffffffffu, p != p);   // every element of both is NaN
+      if (nan) break;
+      const uint32_t which = __ballot_sync(0xffffffffu, in);
+      add_rows(gk, ds, which, q + static_cast<int64_t>(i0) * c.D, c.D, c.D);
+      add_rows(gv, p, which, go + i0 * ostep, ostep, c.D);
     }
   }
+  if (nan) { all_nan(gk); all_nan(gv); }
   row_store(static_cast<T*>(c.dk) + kr, gk, c.scale, c.D);
   row_store(static_cast<T*>(c.dv) + kr, gv, 1.0f, c.D);
 }

@@ -4,7 +4,8 @@ import math
 import pytest
 import torch
 
-from metal_candle_b200 import backend
+from metal_candle_b200 import _lib, backend
+from tests.support import packed_reference as ref
 from tests.test_gpu_masked_attention import inputs, run
 
 pytestmark = pytest.mark.gpu
@@ -42,3 +43,122 @@ def test_rows_that_are_nan_by_right_are_left_at_once(cuda_device, dtype):
         assert torch.isnan(t).all(), name
     took = fastest(lambda: run(q, k, v, dout, G, 0.125, mask, 0.0, None, False))
     assert took <= 4 * finite + 1, (took, finite)
+
+
+def document_64(q, k, v, dout, scale, dtype):
+    """{name: (value, bound)} of one causal document and head, [n, d] each, in float64 on the GPU, a piece of the queries at a time.  Formulas and
+    bounds: tests/support/packed_reference.py, for the tensor cores."""
+    n, d = q.shape
+    u = up = torch.finfo(dtype).eps / 2
+    w = 2.0 ** -22
+    q, k, v, dout = (t.double() for t in (q, k, v, dout))
+    out = {name: (torch.zeros(n, d, dtype=torch.float64, device=q.device), torch.zeros(n, d, dtype=torch.float64, device=q.device))
+           for name in ("o", "dq", "dk", "dv")}
+    out["lse"] = tuple(torch.zeros(n, dtype=torch.float64, device=q.device) for _ in range(2))
+    step = 512
+    for a in range(0, n, step):
+        e = min(n, a + step)
+        qc, go, kc, vc = q[a:e], dout[a:e], k[:e], v[:e]
+        unseen = torch.arange(e, device=q.device)[None, :] > torch.arange(a, e, device=q.device)[:, None]
+        s = (qc @ kc.T).mul_(scale).masked_fill_(unseen, -math.inf)
+        z = torch.logsumexp(s, 1)
+        p = torch.exp(s - z[:, None])
+        top = s.masked_fill_(unseen, 0.0).abs_().amax(1)
+        dots = (qc.abs() @ kc.abs().T).mul_(scale).masked_fill_(unseen, 0.0).amax(1)
+        ds = (d + 4) * w * dots + 2.0 ** -21 * top.clamp_min(1.0)
+        pe = 2 * ds + up + e * w
+        o = p @ vc
+        eo = pe[:, None] * (p @ vc.abs()) + u * o.abs()
+        delta = (go * o).sum(1)
+        ddelta = ((u + d * w) * go.abs() * o.abs()).sum(1) + (go.abs() * eo).sum(1)
+        grad = (go @ vc.T).sub_(delta[:, None]).mul_(p)
+        ge = grad.abs().mul_(pe[:, None]).add_((go.abs() @ vc.abs().T).mul_(d * w).add_(ddelta[:, None]).mul_(p))
+        dq = grad @ kc * scale
+        for name, value, bound in (("o", o, eo), ("lse", z, ds + e * w + 2.0 ** -21 * z.abs()), ("dq", dq, ge @ kc.abs() * scale + u * dq.abs())):
+            out[name][0][a:e], out[name][1][a:e] = value, bound
+        for name, value, bound in (("dk", grad.T @ qc * scale, ge.T @ qc.abs() * scale), ("dv", p.T @ go, (p * pe[:, None]).T @ go.abs())):
+            out[name][0][:e] += value
+            out[name][1][:e] += bound
+    for name in ("dk", "dv"):
+        out[name][1].add_(u * out[name][0].abs())
+    return out
+
+
+def check(got, want, name):
+    value, bound = want
+    got = got.double()
+    assert torch.isfinite(got).all(), name
+    off = float(((got - value).abs() - bound).max())
+    assert off <= 1e-30, f"{name}: {off:.3g} over its bound"
+
+
+def test_a_long_document_behind_one_that_is_not_finite(cuda_device):
+    """131109 positions, of which the first ten are NaN and another document's: the long one's first block of keys holds them, so that every one of its
+    rows comes out NaN at first (0 x NaN) and is taken again from up to 131099 keys.  However long that is, no wait may run out meanwhile."""
+    S, d, first = 131109, 64, 10
+    q, k, v, dout = inputs(cuda_device, 1, S, 1, 1, d, BF16, False, 5)
+    for t in (q, k, v, dout):
+        t[:, :first] = math.nan
+    ids = torch.ones(1, S, dtype=torch.int32, device=cuda_device)
+    ids[:, :first] = 0
+    assert _lib.device_status() == 0
+    got = run(q, k, v, dout, 1, 0.125, backend.attention_mask(ids), 0.0, None, False)
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 0
+    want = document_64(*(t[0, first:] for t in (q, k, v, dout)), 0.125, BF16)
+    for name, value in want.items():
+        check(got[name][0, first:], value, name)
+        assert torch.isnan(got[name][0, :first]).all(), name
+
+
+def test_a_nan_late_in_a_long_document(cuda_device):
+    """One NaN key at position 100000 of 131072: the queries before it are what they are without it, those from it on are NaN, each behind a walk over all
+    keys before that one, and so is every key's gradient."""
+    S, d, at = 131072, 64, 100000
+    q, k, v, dout = inputs(cuda_device, 1, S, 1, 1, d, BF16, False, 6)
+    mask = backend.attention_mask(batch=1, seq=S, device=cuda_device)
+    clean = run(q, k, v, dout, 1, 0.125, mask, 0.0, None, False)
+    k[0, at, 7] = math.nan
+    assert _lib.device_status() == 0
+    got = run(q, k, v, dout, 1, 0.125, mask, 0.0, None, False)
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 0
+    tile = at // 128 * 128
+    for name in ("o", "lse", "dq"):
+        assert torch.equal(got[name][0, :tile], clean[name][0, :tile]), name
+        assert torch.isfinite(got[name][0, tile:at]).all() and torch.isnan(got[name][0, at:]).all(), name
+    for name in ("dk", "dv"):
+        assert torch.isnan(got[name][0, :at + 1]).all(), name
+
+
+def test_many_rows_taken_again(cuda_device):
+    """More items than the CTAs that run at once, most of them with rows to take again, of every quadrant: each is done, once.  Documents of 100
+    positions, every third NaN."""
+    B, S, G, d, doc = 40, 4000, 3, 64, 100
+    q, k, v, dout = inputs(cuda_device, B, S, 1, G, d, BF16, True, 7)
+    number = torch.arange(S, device=cuda_device) // doc
+    ids = (number % 7).to(torch.int32).expand(B, S).contiguous()
+    mask = backend.attention_mask(ids)
+    dirty = number % 3 == 1
+    q.view(B, G, S, d)[:, :, dirty] = math.nan
+    k[:, dirty] = v[:, dirty] = math.nan
+    dout.view(B, S, G * d)[:, dirty] = math.nan
+    got = run(q, k, v, dout, G, 0.125, mask, 0.0, None, True)
+    again = run(q, k, v, dout, G, 0.125, mask, 0.0, None, True)
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 0
+    rows = lambda t: t.view(B, G, S, -1).transpose(1, 2) if t.shape[:2] == (B, G * S) else t.view(B, S, -1)  # noqa: E731
+    for name in got:
+        a, b = rows(got[name]), rows(again[name])
+        assert torch.isnan(a[:, dirty]).all(), name
+        assert torch.isfinite(a[:, ~dirty]).all() and torch.equal(a[:, ~dirty], b[:, ~dirty]), name
+    for b in (0, 23, B - 1):
+        for at in range(0, S, doc):
+            if dirty[at]:
+                continue
+            part = lambda t: t.view(B, -1, S, t.shape[-1])[b, :, at:at + doc].reshape(1, -1, t.shape[-1])  # noqa: E731
+            token = lambda t: t.view(B, S, G * d)[b, at:at + doc]  # noqa: E731
+            want = ref.attention(part(q), part(k), part(v), token(dout), [[0] * doc], None, G, 0.125, 0.0, None, True, BF16, True)
+            for name, value in want.items():
+                x = token(got[name]) if name == "o" else part(got[name][..., None]).view(1, -1) if name == "lse" else part(got[name])
+                ref.check(x, value, f"{name} of {b}, {at}")
