@@ -257,23 +257,34 @@ __device__ __forceinline__ void zero_rows(const SumParams& p, const uint32_t* ke
   const int64_t end = first + kZeroRows < p.vocab ? first + kZeroRows : p.vocab;
   if (threadIdx.x < kZeroRows / 32) named[threadIdx.x] = 0;
   __syncthreads();
-  // the first sorted token that names a row from `first` on: lo, found by 32 looks at a time; then mark what follows
+  // from the first sorted token that names a row of these on, mark what the tokens name, 32 of them at a time; 32 of one row are followed by a jump
+  // behind the last of that row, so that a row named by half of all tokens takes some looks more and not one for every 32 of them (65536 tokens, half of
+  // them the same: the whole gradient 882 us without, 476 with)
   if (threadIdx.x < 32) {
-    int64_t lo = 0, hi = p.M;   // keys before lo are below first, keys from hi on are not
-    while (lo < hi) {
-      const int64_t step = (hi - lo + 31) / 32, q = lo + step * (threadIdx.x + 1) - 1;
-      const int n = __popc(__ballot_sync(kFull, q < hi && __ldcg(keys + q) < first));
-      lo += step * n;
-      hi = lo + step - 1 < hi ? lo + step - 1 : hi;
-    }
+    // the first token from lo on whose row is not below `bound`, by 32 looks at a time
+    auto seek = [&](int64_t lo, int64_t bound) {
+      int64_t hi = p.M;   // keys before lo are below bound, keys from hi on are not
+      while (lo < hi) {
+        const int64_t step = (hi - lo + 31) / 32, q = lo + step * (threadIdx.x + 1) - 1;
+        const int n = __popc(__ballot_sync(kFull, q < hi && __ldcg(keys + q) < bound));
+        lo += step * n;
+        hi = lo + step - 1 < hi ? lo + step - 1 : hi;
+      }
+      return lo;
+    };
+    int64_t lo = seek(0, first);
     for (;;) {
       const int64_t i = lo + threadIdx.x;
-      const bool in = i < p.M && __ldcg(keys + i) < end;
-      if (in) {
-        const uint32_t r = static_cast<uint32_t>(__ldcg(keys + i) - first);
-        atomicOr(&named[r >> 5], 1u << (r & 31));
+      const uint32_t key = i < p.M ? __ldcg(keys + i) : static_cast<uint32_t>(p.vocab);
+      const bool in = key < end;
+      const uint32_t r = key - static_cast<uint32_t>(first), one = __shfl_sync(kFull, r, 0);
+      if (__all_sync(kFull, in && r == one)) {
+        if (threadIdx.x == 0) atomicOr(&named[one >> 5], 1u << (one & 31));
+        lo = seek(lo + 32, first + one + 1);
+        continue;
       }
-      if (__ballot_sync(kFull, in) != kFull) break;
+      if (in) atomicOr(&named[r >> 5], 1u << (r & 31));
+      if (!__all_sync(kFull, in)) break;
       lo += 32;
     }
   }
