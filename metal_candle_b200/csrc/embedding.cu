@@ -379,13 +379,17 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const __grid_constant__ S
   }
 }
 
-// The runs that go on behind the tile in which they begin, a block to a tile (most have nothing to do and leave).  kJoinThreads / tx groups of
+// The runs that go on behind the tile in which they begin, a block to a tile (most have nothing to do and leave).  kJoinThreads / width groups of
 // threads share the parts of a run, consecutive ones each, and add their sums up in order: a token of a thousand rows waits for memory
-// a few times and not a hundred.
+// a few times and not a hundred.  A run of kShare parts or more has its columns shared as well, by the blocks of its first tiles: kSlice threads wide each, so
+// that there are 32 groups (896 columns, 32768 tokens of one id, this kernel: 330 us by one block, 29 so; below 64 parts the looks that
+// the other blocks need are what the shares save).
+constexpr int kShare = 64, kSlice = 8;
+static_assert(kThreads / kSlice <= 32 && kThreads / kSlice <= kShare, "one look finds the run's begin, and it has a block for every slice");
 template <int N>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ SumParams p) {
   __shared__ float sums[kJoinThreads * N];
-  __shared__ int64_t found;
+  __shared__ int64_t found[2];   // the tiles in which the run begins and ends
   const int t = blockIdx.x;
   grid_launch_dependents();
   grid_dependency_wait();
@@ -393,11 +397,20 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   const int64_t i0 = static_cast<int64_t>(t) * p.tile, i1 = i0 + p.tile;
   if (i1 >= p.M) return;
   const uint32_t id = __ldcg(keys + i1 - 1), next = __ldcg(keys + i1), before = i0 > 0 ? __ldcg(keys + i0 - 1) : static_cast<uint32_t>(p.vocab);
-  if (id >= static_cast<uint32_t>(p.vocab) || next != id || before == id) return;   // no run that begins here goes on
-  // the last tile that it reaches: tile q does where its first key is this id.  32 tiles a look, or 32 groups of 32 where they are not enough
+  if (id >= static_cast<uint32_t>(p.vocab) || next != id) return;   // no run goes on behind this tile
+  const int slices = p.tx > kSlice ? p.tx / kSlice : 1;
+  if (before == id && slices == 1) return;   // it begins before, and is not shared
   if (threadIdx.x < 32) {
+    int64_t begin = t;
+    if (before == id) {
+      // this tile and the n before it begin with the id
+      const int64_t q = t - 1 - static_cast<int64_t>(threadIdx.x);
+      begin -= __popc(__ballot_sync(kFull, q >= 0 && __ldcg(keys + q * p.tile) == id));
+      if (begin > 0 && __ldcg(keys + begin * p.tile - 1) == id) --begin;
+    }
+    // the last tile that it reaches: tile q does where its first key is this id.  32 tiles a look, or 32 groups of 32 where they are not enough
     int64_t last = t + 1;
-    for (int64_t step = 1;;) {
+    for (int64_t step = 1; t - begin < slices;) {
       const int64_t q = last + step * (threadIdx.x + 1);
       const int n = __popc(__ballot_sync(kFull, q < p.tiles && __ldcg(keys + q * p.tile) == id));
       last += step * n;
@@ -405,24 +418,26 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
       else if (step == 1) break;
       else step /= 32;
     }
-    if (threadIdx.x == 0) found = last;
+    if (threadIdx.x == 0) { found[0] = begin; found[1] = last; }
   }
   __syncthreads();
-  const int64_t last = found, count = last - t;   // parts behind this tile's own
-  const int x = threadIdx.x % p.tx, g = threadIdx.x / p.tx, groups = count < 8 ? 1 : kJoinThreads / p.tx;
-  const int64_t c = N * (static_cast<int64_t>(blockIdx.y) * p.tx + x);
+  const int64_t begin = found[0], count = found[1] - begin;   // parts behind the first tile's own
+  const bool shared = count >= kShare && slices > 1;
+  if (t - begin >= (shared ? slices : 1)) return;
+  const int width = shared ? kSlice : p.tx, x = threadIdx.x % width, g = threadIdx.x / width, groups = count < 8 ? 1 : kJoinThreads / width;
+  const int64_t c = N * (static_cast<int64_t>(blockIdx.y) * p.tx + (t - begin) * width + x);
   float acc[N] = {};
   if (g < groups && c < p.H) {
-    if (g == 0) get_add<N>(p.part + (2 * static_cast<int64_t>(t) + 1) * p.H + c, acc);
-    const int64_t to = t + 1 + count * (g + 1) / groups;
+    if (g == 0) get_add<N>(p.part + (2 * begin + 1) * p.H + c, acc);
+    const int64_t to = begin + 1 + count * (g + 1) / groups;
 #pragma unroll 8
-    for (int64_t q = t + 1 + count * g / groups; q < to; ++q) get_add<N>(p.part + 2 * q * p.H + c, acc);
+    for (int64_t q = begin + 1 + count * g / groups; q < to; ++q) get_add<N>(p.part + 2 * q * p.H + c, acc);
   }
   if (groups > 1) {
     put<N>(sums + threadIdx.x * N, acc);
     __syncthreads();
     if (g == 0)
-      for (int o = 1; o < groups; ++o) get_add<N>(sums + (o * p.tx + x) * N, acc);
+      for (int o = 1; o < groups; ++o) get_add<N>(sums + (o * width + x) * N, acc);
   }
   if (g == 0 && c < p.H) finish<N>(p, id, c, acc);
 }

@@ -31,7 +31,7 @@ def fastest(call, times=5):
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_a_token_that_comes_half_the_time(cuda_device, dtype):
     """Padding by an id at the end of a large vocabulary: the same sums, and no longer than by an id at its start, whose rows hold zeros already when
-    the sums begin."""
+    the sums begin, or than as many different tokens."""
     M, H, V, hot = 65536, 896, 151936, 151645
     gen = torch.Generator(device=cuda_device).manual_seed(1)
     spread = torch.randint(0, V, (M,), device=cuda_device, generator=gen, dtype=torch.int32)
@@ -45,8 +45,8 @@ def test_a_token_that_comes_half_the_time(cuda_device, dtype):
     named[ids.long()] = True
     assert not grad[~named].any()
     low = torch.where(ids == hot, torch.full_like(ids, 7), ids)
-    start, late = (fastest(lambda: backend.embedding_backward(x, dout, V, grad=grad)) for x in (low, ids))
-    assert late <= 1.25 * start, (late, start)
+    even, start, late = (fastest(lambda: backend.embedding_backward(x, dout, V, grad=grad)) for x in (spread, low, ids))
+    assert late <= 1.25 * start and max(start, late) <= 1.5 * even, (late, start, even)
 
 
 def test_rows_named_once_and_often_side_by_side(cuda_device):
@@ -64,3 +64,35 @@ def test_rows_named_once_and_often_side_by_side(cuda_device):
     named = torch.zeros(V, dtype=torch.bool, device=cuda_device)
     named[ids[ids >= 0]] = True
     assert not grad[~named].any() and torch.isfinite(grad).all()
+
+
+@pytest.mark.parametrize("dtype,H", [(BF16, 896), (F32, 896), (F32, 130), (BF16, 64), (F32, 17), (BF16, 2056)])
+def test_runs_of_any_length_from_any_place(cuda_device, dtype, H):
+    """Runs of a few to a thousand parts (8 tokens each), ending and beginning at the parts' borders and between, one behind the other; alone in
+    the batch; with gradients added to."""
+    parts = [1, 2, 7, 8, 9, 15, 16, 17, 62, 63, 64, 65, 66, 127]
+    lengths = [8 * n + off for n in parts for off in (0, 1, 7)] + [3, 5]
+    order = torch.randperm(len(lengths), generator=torch.Generator().manual_seed(H)).tolist()
+    V = len(lengths) + 3
+    gen = torch.Generator(device=cuda_device).manual_seed(2)
+    for sizes in ([lengths[i] for i in order], [8 * 512], [8 * 513 + 1, 8 * 300], [513, 8 * 64 + 1, 519]):
+        ids = torch.cat([torch.full((n,), i + 1, device=cuda_device, dtype=torch.int32) for i, n in enumerate(sizes)])
+        assert len(ids) <= 16384
+        ids = ids[torch.randperm(len(ids), device=cuda_device, generator=gen)]
+        dout = rand(cuda_device, len(ids), H, seed=4, dtype=dtype)
+        value = embedding_64(ids, dout, V, 3.0)
+        grad = backend.embedding_backward(ids, dout, V, 3.0)
+        ref.check(grad, value, "grad")
+        assert torch.equal(grad, backend.embedding_backward(ids, dout, V, 3.0))
+        before = rand(cuda_device, V, H, seed=5)
+        more = backend.embedding_backward(ids, dout, V, 3.0, grad=before.clone(), accumulate=True)
+        at = before.cpu().double()
+        ref.check(more, (at + value[0], value[1] + 2.0 ** -24 * (at.abs() + value[0].abs())), "accumulated")
+
+
+def test_one_token_alone(cuda_device):
+    """All of 300000 tokens the same: parts of 32, some ten thousand of them."""
+    M, H = 300000, 96
+    ids = torch.full((M,), 2, device=cuda_device, dtype=torch.int32)
+    dout = rand(cuda_device, M, H, seed=6, dtype=BF16)
+    ref.check(backend.embedding_backward(ids, dout, 4), embedding_64(ids, dout, 4, 1.0), "grad")
