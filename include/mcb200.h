@@ -463,17 +463,17 @@ typedef struct {
   int32_t dtype;
   int32_t pad_;
 } mcb_grad_tensor;
-/* norm[0] = sqrt of the sum of squares over all tensors (a HOST array), right over the whole range of float32; the same bits
- * every time. */
+/* norm[0] = sqrt of the sum of squares over all tensors (a HOST array), taken in float64: right wherever in float32 the elements lie, inf where
+ * it passes the largest float32; the same bits every time. */
 size_t mcb_grad_norm_workspace_bytes(int n_tensors);
 int mcb_grad_norm(const mcb_grad_tensor* tensors, int n_tensors, float* norm, void* workspace, size_t workspace_bytes, void* stream);
-/* out = g * min(1, max_norm / (norm + 1e-6)); norm[0], unless null, receives the norm before clipping.  max_norm inf never clips; a
- * norm of NaN makes every element NaN.  No output may overlap another tensor, or its own gradient in part.  TrainingConfig carries
+/* out = g * min(1, max_norm / (norm + 1e-6)); norm[0], unless null, receives the norm before clipping.  max_norm inf never clips; with any other
+ * a norm of NaN makes every element NaN.  Finite gradients are clipped to max_norm also where norm[0] reads inf.  No output may overlap another tensor, or its own gradient in part.  TrainingConfig carries
  * max_grad_norm (src/training/trainer.rs:16-39), but nothing in the reference reads it. */
 int mcb_clip_grad_norm(const mcb_grad_tensor* tensors, int n_tensors, float max_norm, float* norm, void* workspace,
                        size_t workspace_bytes, void* stream);
-/* mcb_adamw_multi with the gradients (times grad_scale) clipped so on the way: they stay as they are in memory.  workspace:
- * mcb_grad_norm_workspace_bytes. */
+/* mcb_adamw_multi with the gradients (times grad_scale, which counts in the norm) clipped so on the way: they stay as they are in memory.
+ * workspace: mcb_grad_norm_workspace_bytes.  Without tensors nothing is written, norm[0] neither. */
 int mcb_adamw_multi_clipped(const mcb_adamw_tensor* tensors, int n_tensors, float lr, float beta1, float beta2, float eps,
                             float weight_decay, float grad_scale, float max_norm, float* norm, void* workspace,
                             size_t workspace_bytes, void* stream);

@@ -64,12 +64,16 @@ template <int MAX, bool CLIP>
 __global__ void __launch_bounds__(256) adamw_multi_kernel(const __grid_constant__ AdamWBatch<MAX> batch,
                                                           const AdamWScalars given, const AdamWClip clip) {
   AdamWScalars s = given;
+  float first = 1.0f;   // a gradient is multiplied by this and by s.grad_scale in turn (see clip_factor)
   if constexpr (CLIP) {
     __shared__ double sums[8];
-    const float norm = gnorm::norm_of(clip.part, clip.parts, sums) * fabsf(s.grad_scale);
-    s.grad_scale *= gnorm::clip_factor(norm, clip.max_norm);
-    if (clip.norm != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) clip.norm[0] = norm;
+    const double norm = gnorm::norm_of(clip.part, clip.parts, sums) * fabs(static_cast<double>(s.grad_scale));
+    const float2 f = gnorm::clip_factor(norm, clip.max_norm, s.grad_scale);
+    first = f.x;
+    s.grad_scale = f.y;
+    if (clip.norm != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) clip.norm[0] = static_cast<float>(norm);
   }
+  auto scaled = [&](float g) { return CLIP ? __fmul_rn(g, first) : g; };
   const AdamWTensorDev& t = batch.t[blockIdx.y];
   const int64_t n = t.n;
   const bool vec = ((reinterpret_cast<uintptr_t>(t.p) | reinterpret_cast<uintptr_t>(t.g) |
@@ -83,23 +87,23 @@ __global__ void __launch_bounds__(256) adamw_multi_kernel(const __grid_constant_
       const float4 g = reinterpret_cast<const float4*>(t.g)[i];
       float4 m = reinterpret_cast<float4*>(t.m)[i];
       float4 v = reinterpret_cast<float4*>(t.v)[i];
-      adamw_one(p.x, g.x, m.x, v.x, s, t.inv_bc1, t.inv_bc2);
-      adamw_one(p.y, g.y, m.y, v.y, s, t.inv_bc1, t.inv_bc2);
-      adamw_one(p.z, g.z, m.z, v.z, s, t.inv_bc1, t.inv_bc2);
-      adamw_one(p.w, g.w, m.w, v.w, s, t.inv_bc1, t.inv_bc2);
+      adamw_one(p.x, scaled(g.x), m.x, v.x, s, t.inv_bc1, t.inv_bc2);
+      adamw_one(p.y, scaled(g.y), m.y, v.y, s, t.inv_bc1, t.inv_bc2);
+      adamw_one(p.z, scaled(g.z), m.z, v.z, s, t.inv_bc1, t.inv_bc2);
+      adamw_one(p.w, scaled(g.w), m.w, v.w, s, t.inv_bc1, t.inv_bc2);
       reinterpret_cast<float4*>(t.p)[i] = p;
       reinterpret_cast<float4*>(t.m)[i] = m;
       reinterpret_cast<float4*>(t.v)[i] = v;
     }
     for (int64_t i = (n4 << 2) + tid; i < n; i += stride) {
       float p = t.p[i], m = t.m[i], v = t.v[i];
-      adamw_one(p, t.g[i], m, v, s, t.inv_bc1, t.inv_bc2);
+      adamw_one(p, scaled(t.g[i]), m, v, s, t.inv_bc1, t.inv_bc2);
       t.p[i] = p; t.m[i] = m; t.v[i] = v;
     }
   } else {
     for (int64_t i = tid; i < n; i += stride) {
       float p = t.p[i], m = t.m[i], v = t.v[i];
-      adamw_one(p, t.g[i], m, v, s, t.inv_bc1, t.inv_bc2);
+      adamw_one(p, scaled(t.g[i]), m, v, s, t.inv_bc1, t.inv_bc2);
       t.p[i] = p; t.m[i] = m; t.v[i] = v;
     }
   }

@@ -8,7 +8,8 @@
 // elements that are dealt out over all blocks, so that tensors of a thousand and of a hundred million elements share a launch.
 //
 // Squares are summed in float32 by a thread (16 elements, then in float64).  Where a thread's largest magnitude is outside [2^-50, 2^50] its squares are
-// taken in float64: the norm of gradients near either end of float32 is right, and inf or NaN only if an element is.
+// taken in float64: the norm of gradients near either end of float32 is right.  It is NaN or inf where an element is, and reads inf where it passes the largest
+// float32, which does not keep finite gradients from being clipped by it.
 #include "grad_norm.cuh"
 
 namespace mcb {
@@ -117,8 +118,8 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const double* part, int 
   __shared__ double s[kThreads / 32];
   grid_launch_dependents();
   grid_dependency_wait();
-  const float v = norm_of(part, parts, s);
-  if (threadIdx.x == 0) norm[0] = v;
+  const double v = norm_of(part, parts, s);
+  if (threadIdx.x == 0) norm[0] = static_cast<float>(v);
 }
 
 // Pieces go by the output's 16-byte boundaries, the first few elements of a tensor by themselves: what is written are whole vectors
@@ -137,19 +138,19 @@ __device__ __forceinline__ void load_for_clip(const Tensor& t, int64_t piece, fl
   else load_piece<T, N, false>(g, t.n, at, v);
 }
 template <typename T>
-__device__ __forceinline__ void clip_piece(const Tensor& t, int64_t piece, float f, const float (&v)[16]) {
+__device__ __forceinline__ void clip_piece(const Tensor& t, int64_t piece, float2 f, const float (&v)[16]) {
   constexpr int N = Vec16<T>::N;
   const T* g = static_cast<const T*>(t.g);
   T* out = static_cast<T*>(t.out);
   const int head = head_of<T>(t);
-  if (piece == 0 && static_cast<int>(threadIdx.x) < head && threadIdx.x < t.n) out[threadIdx.x] = from_f32<T>(to_f32(g[threadIdx.x]) * f);
+  if (piece == 0 && static_cast<int>(threadIdx.x) < head && threadIdx.x < t.n) out[threadIdx.x] = from_f32<T>(to_f32(g[threadIdx.x]) * f.x * f.y);
   const int64_t at = head + piece * kPiece;
 #pragma unroll
   for (int k = 0; k < 16 / N; ++k) {
     const int64_t i = at + N * (threadIdx.x + kThreads * k);
     float w[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) w[e] = v[N * k + e] * f;
+    for (int e = 0; e < N; ++e) w[e] = v[N * k + e] * f.x * f.y;
     if (i + N <= t.n) {
       Vec16<T> x;
       x.from_float(w);
@@ -180,8 +181,9 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ 
   };
   float v[2][16];
   uint32_t i = blockIdx.x;
-  const float total = norm_of(part, parts, s), f = clip_factor(total, max_norm);
-  if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = total;
+  const double total = norm_of(part, parts, s);
+  const float2 f = clip_factor(total, max_norm, 1.0f);
+  if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = static_cast<float>(total);
   if (i < tab.pieces) load(i, v[0]);
   while (i < tab.pieces) {
 #pragma unroll

@@ -1,0 +1,44 @@
+"""Clipping by the global norm at the ends of float32."""
+import math
+
+import pytest
+import torch
+
+from metal_candle_b200.training import AdamW, AdamWConfig, clip_grad_norm
+from tests.test_gpu_packed_training import rand
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def test_clipping_where_the_norm_passes_float32(cuda_device):
+    """Finite gradients whose norm is above 3.4e38: the norm reads inf, and they are scaled to max_norm all the same."""
+    for dtype in (F32, BF16):
+        for n in (2, 5000):
+            g = torch.full((n,), 3e38, device=cuda_device).to(dtype)
+            g[1] = -1e38
+            whole = math.sqrt(float(g.double().square().sum()))
+            for limit in (1.0, 1e-3, 1e30):
+                clipped = [g.clone()]
+                norm = float(clip_grad_norm(clipped, limit))
+                assert norm == math.inf if whole > 3.41e38 else abs(norm - whole) <= 2.0 ** -19 * whole
+                want = g.double() * (limit / whole)
+                # 16 float32 additions at most in the norm, the factor's and the products' roundings, the output's
+                assert ((clipped[0].double() - want).abs() <= (2.0 ** -19 + torch.finfo(dtype).eps / 2) * want.abs()).all()
+
+
+@pytest.mark.parametrize("size,grad_scale", [(3e38, 2.0 ** -100), (3e38, 1e-30), (1e-40, 2.0 ** 100), (1e38, 1.0)])
+def test_adamw_clips_by_the_norm_of_the_scaled_gradients(cuda_device, size, grad_scale):
+    """The norm counts after grad_scale, wherever in float32 the gradients lie before it."""
+    n, limit = 1000, 0.5
+    g = rand(cuda_device, n, seed=1).clamp(-1, 1) * size
+    p, a = torch.zeros(n, device=cuda_device), AdamW(AdamWConfig(learning_rate=1e-2, beta1=0.5, beta2=0.5, weight_decay=0.0))
+    norm = a.step_vars([p], [g], grad_scale=grad_scale, max_grad_norm=limit)
+    scale = float(torch.tensor(grad_scale, dtype=F32))
+    whole = math.sqrt(float((g.double() * scale).square().sum()))
+    assert abs(float(norm) - whole) <= 2.0 ** -19 * whole if whole < 3.4e38 else float(norm) == math.inf
+    want = g.double() * scale * min(1.0, limit / (whole + 1e-6))
+    m = a.state_of(p)[0].double()   # (1 - beta1) of the gradient that the update has seen, exactly
+    # the norm's 16 additions, the factor, two products; a gradient below 2^-126 before it is scaled has lost digits already
+    assert ((2 * m - want).abs() <= 2.0 ** -18 * want.abs() + 1e-44).all() and float(m.abs().max()) > 0
