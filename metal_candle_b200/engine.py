@@ -90,6 +90,7 @@ class QwenEngine:
                                                   first, n))
 
     def _check_batch(self, ids, targets):
+        self.model._refuse_packed("a step of QwenEngine")
         if ids.dtype != torch.int32 or targets.dtype != torch.int32 or not ids.is_cuda or not targets.is_cuda:
             raise TrainingError("QwenEngine takes int32 CUDA tensors of token ids and targets (ignored positions: -1)")
         if ids.shape != targets.shape or ids.dim() != 2 or not ids.is_contiguous() or not targets.is_contiguous():

@@ -82,13 +82,17 @@ class _Linear:
 class CapturedStep:
     """forward_backward of a fixed shape as a CUDA graph (Qwen.capture_forward_backward)."""
 
-    def __init__(self, graph, ids, targets, loss, grads, count=None):
+    def __init__(self, graph, ids, targets, loss, grads, count=None, model: Optional["Qwen"] = None):
         self.graph, self.ids, self.targets, self.loss, self.grads = graph, ids, targets, loss, grads
+        self.model = model
         self.count = count   # int32 [1]: targets of the last replayed batch that were not ignored
 
     def __call__(self, input_ids: torch.Tensor, target_ids: torch.Tensor):
         """Copies the batch into the graph's input buffers (device to device, or from pinned host memory) and
-        replays; returns (loss, grads) like Qwen.forward_backward - the same tensors on every call."""
+        replays; returns (loss, grads) like Qwen.forward_backward - the same tensors on every call.  Refused within the
+        model's packed(): the graph has no documents."""
+        if self.model is not None:
+            self.model._refuse_packed("a captured step")
         self.ids.copy_(input_ids, non_blocking=True)
         self.targets.copy_(target_ids, non_blocking=True)
         self.graph.replay()
@@ -603,7 +607,8 @@ class Qwen:
         """Within the `with` block the model's passes (`forward`, `forward_backward`, the post-training ones) take batches of packed
         documents: document_ids [batch, seq] and prefix as `backend.attention_mask` takes them, so that no token sees another
         document.  Rotary positions go on over the sequence, which scores do not depend on: they turn on differences.  The targets are the
-        caller's: the last token of a document has none.  Every batch has a block of its own; a pass cannot be captured within one."""
+        caller's: the last token of a document has none.  Every batch has a block of its own; a pass cannot be captured within one, and steps that were
+        captured before, or the engine's, are refused: they have no documents."""
         if document_ids.dim() != 2:
             raise TrainingError(f"document_ids must be [batch, seq], got {list(document_ids.shape)}")
         for t, what in ((document_ids, "document_ids"), (prefix, "prefix")):
@@ -615,6 +620,10 @@ class Qwen:
             yield self
         finally:
             self._mask = before
+
+    def _refuse_packed(self, what: str) -> None:
+        if self._mask is not None:
+            raise TrainingError(f"{what} within packed(): it would run the batch without the documents")
 
     # -- post-training losses: the same pass with another loss between the lm_head and its backward --
     @contextmanager
@@ -797,7 +806,7 @@ class Qwen:
         finally:
             self.layer_done_hook, self.backward_done_hook = hook, done_hook
             _lib.profile_enable(was_profiling)
-        return CapturedStep(graph, ids, targets, loss, grads, count=self.last_count)
+        return CapturedStep(graph, ids, targets, loss, grads, count=self.last_count, model=self)
 
     def _layer_bwd(self, dh3, sv, idx, B, S, accumulate, calls: _LayerCalls):
         c = self.config
