@@ -113,6 +113,8 @@ class _LayerCalls:
         mask = model._mask
         if mask is not None and (mask.batch, mask.seq) != (batch, seq):
             raise TrainingError(f"packed() was given documents of {mask.batch} x {mask.seq} positions, the batch has {batch} x {seq}")
+        if mask is not None and not model._mask_recorded and torch._C._cuda_isCurrentStreamCapturing():
+            raise TrainingError("a pass is captured within packed() that was opened before: the graph would read the mask after the block has let go of it")
         # what the library's layer takes; other models and settings (and packed documents) run kernel by kernel
         self.usable = (mask is None and model.dtype == torch.bfloat16 and c.head_dim == 64 and c.intermediate_size % 8 == 0 and c.vocab_size % 8 == 0
                        and model.fuse_swiglu_bwd)
@@ -221,6 +223,7 @@ class Qwen:
     MODULES = ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj")
 
     _mask: Optional[backend.AttentionMask] = None   # of the packed() block that is open
+    _mask_recorded = False                          # whether that block was opened under a capture, whose graph makes the mask anew
 
     def __init__(self, config: ModelConfig, device, dtype=torch.bfloat16, seed: int = 0):
         config.validate()
@@ -607,19 +610,20 @@ class Qwen:
         """Within the `with` block the model's passes (`forward`, `forward_backward`, the post-training ones) take batches of packed
         documents: document_ids [batch, seq] and prefix as `backend.attention_mask` takes them, so that no token sees another
         document.  Rotary positions go on over the sequence, which scores do not depend on: they turn on differences.  The targets are the
-        caller's: the last token of a document has none.  Every batch has a block of its own; a pass cannot be captured within one, and steps that were
-        captured before, or the engine's, are refused: they have no documents."""
+        caller's: the last token of a document has none.  Every batch has a block of its own.  Steps that were captured before, or
+        the engine's, are refused within one: they have no documents.  A pass that is captured (by `torch.cuda.graph`) takes its block into the capture: the
+        graph then makes the mask of what document_ids and prefix hold when it is replayed."""
         if document_ids.dim() != 2:
             raise TrainingError(f"document_ids must be [batch, seq], got {list(document_ids.shape)}")
         for t, what in ((document_ids, "document_ids"), (prefix, "prefix")):
             if t is not None:
                 self._here(t, what)
-        before = self._mask
-        self._mask = backend.attention_mask(document_ids, prefix)
+        before = self._mask, self._mask_recorded
+        self._mask, self._mask_recorded = backend.attention_mask(document_ids, prefix), torch._C._cuda_isCurrentStreamCapturing()
         try:
             yield self
         finally:
-            self._mask = before
+            self._mask, self._mask_recorded = before
 
     def _refuse_packed(self, what: str) -> None:
         if self._mask is not None:

@@ -28,3 +28,27 @@ def test_steps_without_documents_are_refused_within_packed(cuda_device):
                 call()
     assert torch.equal(step(ids, targets)[0], loss)
     engine.forward_backward(ids32, targets32)
+
+
+def test_a_capture_by_hand_holds_its_own_documents(cuda_device):
+    """packed() opened while a graph is recorded belongs to it; a block opened before does not, and the graph would outlive it."""
+    model, ids, targets, _ = small_model(cuda_device, BF16)
+    docs = torch.arange(ids.shape[1], device=cuda_device, dtype=torch.int32).expand(ids.shape).contiguous() // 7
+    with model.packed(docs):
+        want = model.forward_backward(ids, targets)[0].clone()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(TrainingError, match="packed"):
+            with torch.cuda.graph(graph):
+                model.forward_backward(ids, targets)
+    plain = model.forward_backward(ids, targets)[0].clone()
+    graph, held = torch.cuda.CUDAGraph(), docs.clone()
+    with torch.cuda.graph(graph):
+        with model.packed(held):
+            loss, grads = model.forward_backward(ids, targets)
+    graph.replay()
+    assert torch.equal(loss, want) and not torch.equal(loss, plain)
+    held.zero_()   # other documents, the same graph
+    graph.replay()
+    one = loss.clone()
+    with model.packed(torch.zeros_like(docs)):
+        assert torch.equal(model.forward_backward(ids, targets)[0], one)
