@@ -530,10 +530,11 @@ class TrainingConfig:
 
 @dataclass
 class StepMetrics:
-    """src/training/trainer.rs:264-274."""
+    """src/training/trainer.rs:264-274; with clipping also the gradients' norm before it."""
     loss: float
     step: int
     learning_rate: float
+    grad_norm: Optional[float] = None
 
 
 IGNORE_INDEX = 0xFFFFFFFF  # u32::MAX, what TrainingStep passes (src/training/trainer.rs:385)
@@ -853,17 +854,18 @@ class TrainingStep:
 
     def execute(self, input_ids, target_ids, lora_adapter: LoRAAdapter, optimizer: AdamW, learning_rate: float,
                 forward_backward_fn: Callable, max_grad_norm: Optional[float] = None) -> StepMetrics:
-        """max_grad_norm: the gradients are clipped to that global norm on their way into the update."""
+        """max_grad_norm: the gradients are clipped to that global norm on their way into the update; the metrics have the norm before."""
         loss, grads = forward_backward_fn(input_ids, target_ids)
         variables = self.collect_trainable_vars(lora_adapter)
         optimizer.set_lr(learning_rate)
+        norm = None
         if max_grad_norm is None:
             optimizer.step_vars(variables, grads)
         else:
-            optimizer.step_vars(variables, grads, max_grad_norm=max_grad_norm)
+            norm = optimizer.step_vars(variables, grads, max_grad_norm=max_grad_norm)
         loss_value = float(loss) if not torch.is_tensor(loss) else float(loss.item())  # host sync, trainer.rs:405
         self._step += 1
-        return StepMetrics(loss=loss_value, step=self._step, learning_rate=learning_rate)
+        return StepMetrics(loss=loss_value, step=self._step, learning_rate=learning_rate, grad_norm=None if norm is None else float(norm))
 
     def step(self) -> int:
         return self._step

@@ -1,10 +1,11 @@
-"""Clipping by the global norm at the ends of float32."""
+"""Clipping by the global norm at the ends of float32, and the norm in a step's metrics."""
 import math
 
 import pytest
 import torch
 
-from metal_candle_b200.training import AdamW, AdamWConfig, clip_grad_norm
+from metal_candle_b200 import training
+from metal_candle_b200.training import AdamW, AdamWConfig, clip_grad_norm, grad_norm
 from tests.test_gpu_packed_training import rand
 
 pytestmark = pytest.mark.gpu
@@ -42,3 +43,19 @@ def test_adamw_clips_by_the_norm_of_the_scaled_gradients(cuda_device, size, grad
     m = a.state_of(p)[0].double()   # (1 - beta1) of the gradient that the update has seen, exactly
     # the norm's 16 additions, the factor, two products; a gradient below 2^-126 before it is scaled has lost digits already
     assert ((2 * m - want).abs() <= 2.0 ** -18 * want.abs() + 1e-44).all() and float(m.abs().max()) > 0
+
+
+def test_the_norm_reaches_the_metrics(cuda_device):
+    params = [rand(cuda_device, 5, seed=1), rand(cuda_device, 7, seed=2)]
+
+    class Adapter:
+        def layers(self):
+            return [("layers.0.q_proj", self)]
+
+        def trainable_variables(self):
+            return params
+
+    grads = [rand(cuda_device, 5, seed=3), rand(cuda_device, 7, seed=4)]
+    step = lambda **how: training.TrainingStep().execute(None, None, Adapter(), AdamW(), 1e-3, lambda i, t: (1.0, grads), **how)  # noqa: E731
+    assert step().grad_norm is None
+    assert step(max_grad_norm=1e-3).grad_norm == float(grad_norm(grads))
