@@ -364,6 +364,10 @@ class AdamW:
         return self.state[self._key(var)]
 
     def _launch(self, items, grad_scale: float = 1.0, max_grad_norm: Optional[float] = None) -> Optional[torch.Tensor]:
+        first = items[0][2]
+        if first.is_cuda and first.get_device() != torch._C._cuda_getDevice():
+            with torch.cuda.device(first.device):
+                return self._launch(items, grad_scale, max_grad_norm)
         # This loop is most of an update's time on the host: one attribute read per fact and tensor, and the descriptors
         # packed in one go instead of as one ctypes structure per tensor (192 tensors, one update: 416 -> 237 us, 267 with the
         # check of the moments).

@@ -59,3 +59,31 @@ def test_the_norm_reaches_the_metrics(cuda_device):
     step = lambda **how: training.TrainingStep().execute(None, None, Adapter(), AdamW(), 1e-3, lambda i, t: (1.0, grads), **how)  # noqa: E731
     assert step().grad_norm is None
     assert step(max_grad_norm=1e-3).grad_norm == float(grad_norm(grads))
+
+
+@pytest.mark.parametrize("limit", [None, 0.5])
+def test_adamw_on_another_device_than_the_current_one(cuda_device, monkeypatch, limit):
+    """The update is launched with the parameters' device as the current one (seen here by a current device that is only said to be another)."""
+    p, g = rand(cuda_device, 40, seed=1), rand(cuda_device, 40, seed=2)
+    other, made = p.clone(), []
+    AdamW().step_vars([p], [g], max_grad_norm=limit)
+    now = [cuda_device.index + 1]
+
+    class Device:
+        def __init__(self, device):
+            self.index = torch.device(device).index
+
+        def __enter__(self):
+            made.append(self.index)
+            self.before, now[0] = now[0], self.index
+
+        def __exit__(self, *_):
+            now[0] = self.before
+
+    a = AdamW()
+    a.add_parameter(a._key(other), other)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    a.step_vars([other], [g], max_grad_norm=limit)
+    monkeypatch.undo()
+    assert made and set(made) == {cuda_device.index} and torch.equal(p, other)
