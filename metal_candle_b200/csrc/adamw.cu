@@ -189,6 +189,7 @@ int adamw_multi(const mcb_adamw_tensor* tensors, int n_tensors, float lr, float 
     if (!(max_norm >= 0.0f)) return fail(MCB_ERR_SHAPE, "adamw_multi: max_norm must not be negative, got %g", max_norm);
     if (!workspace || workspace_bytes < gnorm::workspace_bytes(n_tensors) || !aligned16(workspace))
       return fail(MCB_ERR_WORKSPACE, "adamw_multi: workspace of %zu bytes, 16-byte aligned, needed", gnorm::workspace_bytes(n_tensors));
+    if (!on_boundary(4, clip_norm)) return fail(MCB_ERR_ALIGN, "adamw_multi: norm is not aligned to its elements");
   }
   DeviceState* ds = current_device_state();
   if (!ds) return MCB_ERR_NOT_INIT;
@@ -196,6 +197,7 @@ int adamw_multi(const mcb_adamw_tensor* tensors, int n_tensors, float lr, float 
     const mcb_adamw_tensor& t = tensors[i];
     if (!t.p || !t.g || !t.m || !t.v) return fail(MCB_ERR_NULL, "adamw_multi: tensor %d has a null pointer", i);
     if (t.n <= 0) return fail(MCB_ERR_SHAPE, "adamw_multi: tensor %d has n=%lld", i, (long long)t.n);
+    if (!on_boundary(4, t.p, t.g, t.m, t.v)) return fail(MCB_ERR_ALIGN, "adamw_multi: tensor %d is not aligned to its elements", i);
     if (t.t <= 0) return fail(MCB_ERR_SHAPE, "adamw_multi: tensor %d has step t=%d (must be >= 1)", i, t.t);
   }
   AdamWScalars s;

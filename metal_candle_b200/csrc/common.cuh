@@ -92,6 +92,12 @@ inline cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// Whether all of these (null: not given) lie on boundaries of `bytes`, a power of two: an element's size, where nothing more is needed.
+template <typename... P>
+inline bool on_boundary(size_t bytes, const P*... p) {
+  return ((reinterpret_cast<uintptr_t>(p) | ... | uintptr_t{0}) & (bytes - 1)) == 0;
+}
+inline size_t element_bytes(int dtype) { return dtype == MCB_F32 ? 4 : 2; }
 
 // ---- device-side helpers -----------------------------------------------------------------
 

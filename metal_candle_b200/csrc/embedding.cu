@@ -532,6 +532,8 @@ extern "C" int mcb_embedding_scaled_fwd(const void* ids, int id_bytes, const voi
   MCB_NVTX_RANGE("mcb_embedding_scaled_fwd");
   if (!ids || !table || !out) return fail(MCB_ERR_NULL, "embedding_scaled_fwd: null pointer");
   if (int rc = embed::check("embedding_scaled_fwd", id_bytes, M, H, vocab, scale, dtype)) return rc;
+  if (!on_boundary(id_bytes, ids) || !on_boundary(element_bytes(dtype), table, out))
+    return fail(MCB_ERR_ALIGN, "embedding_scaled_fwd: a pointer is not aligned to its elements");
   DeviceState* ds = current_device_state();
   if (!ds) return MCB_ERR_NOT_INIT;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -553,6 +555,8 @@ extern "C" int mcb_embedding_bwd(const void* ids, int id_bytes, const void* dout
   if (!ids || !dout || !dtable) return fail(MCB_ERR_NULL, "embedding_bwd: null pointer");
   if (int rc = embed::check("embedding_bwd", id_bytes, M, H, vocab, scale, dtype)) return rc;
   if (!aligned16(dtable)) return fail(MCB_ERR_ALIGN, "embedding_bwd: the table's gradient is not 16-byte aligned");
+  if (!on_boundary(id_bytes, ids) || !on_boundary(element_bytes(dtype), dout))
+    return fail(MCB_ERR_ALIGN, "embedding_bwd: a pointer is not aligned to its elements");
   if (!workspace || workspace_bytes < mcb_embedding_bwd_workspace_bytes(M, H) || !aligned16(workspace))
     return fail(MCB_ERR_WORKSPACE, "embedding_bwd: workspace of %zu bytes, 16-byte aligned, needed", mcb_embedding_bwd_workspace_bytes(M, H));
   DeviceState* ds = current_device_state();

@@ -295,6 +295,7 @@ extern "C" int mcb_grad_norm(const mcb_grad_tensor* tensors, int n_tensors, floa
   MCB_NVTX_RANGE("mcb_grad_norm");
   if (int rc = gnorm::check(tensors, n_tensors, "grad_norm")) return rc;
   if (!norm) return fail(MCB_ERR_NULL, "grad_norm: norm is null");
+  if (!on_boundary(4, norm)) return fail(MCB_ERR_ALIGN, "grad_norm: norm is not aligned to its elements");
   if (!workspace || workspace_bytes < gnorm::workspace_bytes(n_tensors) || !aligned16(workspace))
     return fail(MCB_ERR_WORKSPACE, "grad_norm: workspace of %zu bytes, 16-byte aligned, needed", gnorm::workspace_bytes(n_tensors));
   DeviceState* ds = current_device_state();
@@ -313,6 +314,7 @@ extern "C" int mcb_clip_grad_norm(const mcb_grad_tensor* tensors, int n_tensors,
   MCB_NVTX_RANGE("mcb_clip_grad_norm");
   if (int rc = gnorm::check(tensors, n_tensors, "clip_grad_norm")) return rc;
   if (!(max_norm >= 0.0f)) return fail(MCB_ERR_SHAPE, "clip_grad_norm: max_norm must not be negative, got %g", max_norm);
+  if (!on_boundary(4, norm)) return fail(MCB_ERR_ALIGN, "clip_grad_norm: norm is not aligned to its elements");
   if (!workspace || workspace_bytes < gnorm::workspace_bytes(n_tensors) || !aligned16(workspace))
     return fail(MCB_ERR_WORKSPACE, "clip_grad_norm: workspace of %zu bytes, 16-byte aligned, needed", gnorm::workspace_bytes(n_tensors));
   try {

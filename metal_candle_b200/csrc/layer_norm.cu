@@ -582,6 +582,8 @@ extern "C" int mcb_layernorm_fwd(const void* x, const void* w, const void* b, vo
   MCB_NVTX_RANGE("mcb_layernorm_fwd");
   if (!x || !y) return fail(MCB_ERR_NULL, "layernorm_fwd: x or y is null");
   if (int rc = lnorm::check("layernorm_fwd", rows, D, eps, dtype)) return rc;
+  if (!on_boundary(element_bytes(dtype), x, w, b, y) || !on_boundary(4, mean, rstd))
+    return fail(MCB_ERR_ALIGN, "layernorm_fwd: a pointer is not aligned to its elements");
   DeviceState* ds = current_device_state();
   if (!ds) return MCB_ERR_NOT_INIT;
   lnorm::Params p = {};
@@ -610,6 +612,8 @@ extern "C" int mcb_layernorm_bwd(const void* x, const void* w, const void* dy, c
   const bool sums = dw != nullptr || db != nullptr;
   if (sums && (!workspace || workspace_bytes < mcb_layernorm_bwd_workspace_bytes(rows, D) || !aligned16(workspace)))
     return fail(MCB_ERR_WORKSPACE, "layernorm_bwd: workspace of %zu bytes, 16-byte aligned, needed", mcb_layernorm_bwd_workspace_bytes(rows, D));
+  if (!on_boundary(element_bytes(dtype), x, w, dy, dx_residual, dx) || !on_boundary(4, dw, db))
+    return fail(MCB_ERR_ALIGN, "layernorm_bwd: a pointer is not aligned to its elements");
   DeviceState* ds = current_device_state();
   if (!ds) return MCB_ERR_NOT_INIT;
   lnorm::Params p = {};

@@ -606,6 +606,7 @@ extern "C" int mcb_attention_masked_fwd(const mcb_masked_attention* a, const voi
   if (int rc = mattn::fill(c, a, "attention_masked_fwd")) return rc;
   if (!q || !k || !v || !o) return fail(MCB_ERR_NULL, "attention_masked_fwd: q, k, v or o is null");
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o)) return fail(MCB_ERR_ALIGN, "attention_masked_fwd: 16-byte alignment");
+  if (!on_boundary(4, lse)) return fail(MCB_ERR_ALIGN, "attention_masked_fwd: lse is not aligned to its elements");
   const size_t kb = mattn::k_bytes(a), qb = kb * a->groups;
   const mattn::Range ranges[] = {{o, qb}, {lse, mattn::lse_bytes(a)}, {q, qb}, {k, kb}, {v, kb}, {a->mask, mcb_attention_mask_bytes(a->batch, a->seq)}};
   if (mattn::outputs_overlap(ranges, 2)) return fail(MCB_ERR_SHAPE, "attention_masked_fwd: o or lse overlaps an input or the other");
@@ -632,6 +633,7 @@ extern "C" int mcb_attention_masked_bwd(const mcb_masked_attention* a, const voi
   if (!q || !k || !v || !o || !lse || !dout || !dq || !dk || !dv) return fail(MCB_ERR_NULL, "attention_masked_bwd: a required pointer is null");
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv))
     return fail(MCB_ERR_ALIGN, "attention_masked_bwd: 16-byte alignment");
+  if (!on_boundary(4, lse)) return fail(MCB_ERR_ALIGN, "attention_masked_bwd: lse is not aligned to its elements");
   const size_t stat = mattn::stat_bytes(a);
   if (!workspace || workspace_bytes < 2 * stat || (reinterpret_cast<uintptr_t>(workspace) & 1023u) != 0)
     return fail(MCB_ERR_WORKSPACE, "attention_masked_bwd: workspace of %zu bytes, 1024-byte aligned, needed", 2 * stat);

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from metal_candle_b200 import training
+from metal_candle_b200 import _lib, training
 from metal_candle_b200.training import AdamW, AdamWConfig, clip_grad_norm, grad_norm
 from tests.test_gpu_packed_training import rand
 
@@ -87,3 +87,15 @@ def test_adamw_on_another_device_than_the_current_one(cuda_device, monkeypatch, 
     a.step_vars([other], [g], max_grad_norm=limit)
     monkeypatch.undo()
     assert made and set(made) == {cuda_device.index} and torch.equal(p, other)
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_adamw_refuses_pointers_off_their_elements(cuda_device, which):
+    t = [torch.zeros(8, device=cuda_device) for _ in range(4)]
+    at = [x.data_ptr() for x in t]
+    at[which] += 2
+    table = (_lib.AdamWTensor * 1)(_lib.AdamWTensor(*at, 4, 1, 0))
+    lib = _lib.init(cuda_device.index)
+    assert lib.mcb_adamw_multi(table, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1.0, None) == -3
+    torch.cuda.synchronize()
+    assert not any(x.any() for x in t)
