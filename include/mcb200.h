@@ -283,13 +283,13 @@ int mcb_rmsnorm_bwd_noalloc(const void* x, const void* w, const void* dy, void* 
 /* ---- layer norm ------------------------------------------------------------------------------ */
 
 /* y = (x - mean) / sqrt(var + eps) (* w) (+ b) over the last dimension, var the mean of the squared differences.  x, y [rows, D]
- * dtype; w, b [D] dtype or null; mean, rstd [rows] float32 or null.  y may be x.  Any D.  Replaces LayerNormOp
+ * dtype; w, b [D] dtype or null; mean, rstd [rows] float32 or null.  y may be x; no output may overlap anything else in part or whole.  Any D.  Replaces LayerNormOp
  * (src/backend/custom_ops.rs:826-1079), which takes the variance as E[x^2] - mean^2. */
 int mcb_layernorm_fwd(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, int64_t rows, int64_t D,
                       float eps, int dtype, void* stream);
 /* Reverse pass from x alone (mean and rstd are taken again): dx [rows, D] dtype, plus dx_residual if not null (the gradient that reaches
  * the same tensor along the residual connection); dw, db [D] float32 or null (overwritten unless accumulate).  dx may be dy or
- * dx_residual.  Sums over rows in a fixed order. */
+ * dx_residual; no gradient may overlap anything else in part or whole.  Sums over rows in a fixed order. */
 size_t mcb_layernorm_bwd_workspace_bytes(int64_t rows, int64_t D);
 int mcb_layernorm_bwd(const void* x, const void* w, const void* dy, const void* dx_residual, void* dx, float* dw, float* db,
                       int accumulate, int64_t rows, int64_t D, float eps, int dtype, void* workspace, size_t workspace_bytes,
@@ -488,7 +488,8 @@ int mcb_embedding_scaled_fwd(const void* ids, int id_bytes, const void* table, v
                              float scale, int dtype, void* stream);
 /* Its table's gradient, for a table that is trained: dtable[v,:] = scale * sum of dout[m,:] over ids[m] = v, [vocab, H] float32 from a
  * 16-byte boundary, written whole (accumulate: added to, where a token has the id).  dout [M, H] dtype.  Terms are summed in token
- * order, in parts of 8 to 32: the same bits every time. */
+ * order, in parts of 8 to 32: the same bits every time.  Neither
+ * dtable nor (above) out may overlap an input. */
 size_t mcb_embedding_bwd_workspace_bytes(int64_t M, int64_t H);
 int mcb_embedding_bwd(const void* ids, int id_bytes, const void* dout, float* dtable, int accumulate, int64_t M, int64_t H,
                       int64_t vocab, float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);

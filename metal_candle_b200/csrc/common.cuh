@@ -97,6 +97,22 @@ template <typename... P>
 inline bool on_boundary(size_t bytes, const P*... p) {
   return ((reinterpret_cast<uintptr_t>(p) | ... | uintptr_t{0}) & (bytes - 1)) == 0;
 }
+// Whether an output (the first `outputs` of the ranges; null: not given) overlaps another range: a block would read what another has written already.
+struct Range {
+  const void* p;
+  size_t bytes;
+};
+inline bool overlap(const Range& r, const Range& s) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(r.p), b = reinterpret_cast<uintptr_t>(s.p);
+  return a != 0 && b != 0 && a < b + s.bytes && b < a + r.bytes;
+}
+template <int N>
+bool outputs_overlap(const Range (&r)[N], int outputs) {
+  for (int i = 0; i < outputs; ++i)
+    for (int j = i + 1; j < N; ++j)
+      if (overlap(r[i], r[j])) return true;
+  return false;
+}
 inline size_t element_bytes(int dtype) { return dtype == MCB_F32 ? 4 : 2; }
 
 // ---- device-side helpers -----------------------------------------------------------------

@@ -534,6 +534,9 @@ extern "C" int mcb_embedding_scaled_fwd(const void* ids, int id_bytes, const voi
   if (int rc = embed::check("embedding_scaled_fwd", id_bytes, M, H, vocab, scale, dtype)) return rc;
   if (!on_boundary(id_bytes, ids) || !on_boundary(element_bytes(dtype), table, out))
     return fail(MCB_ERR_ALIGN, "embedding_scaled_fwd: a pointer is not aligned to its elements");
+  const size_t row = static_cast<size_t>(H) * element_bytes(dtype);
+  const Range ranges[] = {{out, M * row}, {table, vocab * row}, {ids, static_cast<size_t>(M) * id_bytes}};
+  if (outputs_overlap(ranges, 1)) return fail(MCB_ERR_SHAPE, "embedding_scaled_fwd: the output overlaps an input");
   DeviceState* ds = current_device_state();
   if (!ds) return MCB_ERR_NOT_INIT;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -559,6 +562,9 @@ extern "C" int mcb_embedding_bwd(const void* ids, int id_bytes, const void* dout
     return fail(MCB_ERR_ALIGN, "embedding_bwd: a pointer is not aligned to its elements");
   if (!workspace || workspace_bytes < mcb_embedding_bwd_workspace_bytes(M, H) || !aligned16(workspace))
     return fail(MCB_ERR_WORKSPACE, "embedding_bwd: workspace of %zu bytes, 16-byte aligned, needed", mcb_embedding_bwd_workspace_bytes(M, H));
+  const Range ranges[] = {{dtable, static_cast<size_t>(vocab) * H * sizeof(float)}, {workspace, mcb_embedding_bwd_workspace_bytes(M, H)},
+                          {dout, static_cast<size_t>(M) * H * element_bytes(dtype)}, {ids, static_cast<size_t>(M) * id_bytes}};
+  if (outputs_overlap(ranges, 2)) return fail(MCB_ERR_SHAPE, "embedding_bwd: the gradient or the workspace overlaps an input or one another");
   DeviceState* ds = current_device_state();
   if (!ds) return MCB_ERR_NOT_INIT;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

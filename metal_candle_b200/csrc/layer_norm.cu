@@ -584,6 +584,9 @@ extern "C" int mcb_layernorm_fwd(const void* x, const void* w, const void* b, vo
   if (int rc = lnorm::check("layernorm_fwd", rows, D, eps, dtype)) return rc;
   if (!on_boundary(element_bytes(dtype), x, w, b, y) || !on_boundary(4, mean, rstd))
     return fail(MCB_ERR_ALIGN, "layernorm_fwd: a pointer is not aligned to its elements");
+  const size_t row = static_cast<size_t>(D) * element_bytes(dtype), all = rows * row;
+  const Range ranges[] = {{y, all}, {mean, rows * sizeof(float)}, {rstd, rows * sizeof(float)}, {y == x ? nullptr : x, all}, {w, row}, {b, row}};
+  if (outputs_overlap(ranges, 3)) return fail(MCB_ERR_SHAPE, "layernorm_fwd: an output overlaps an input (but for y = x) or another output");
   DeviceState* ds = current_device_state();
   if (!ds) return MCB_ERR_NOT_INIT;
   lnorm::Params p = {};
@@ -614,6 +617,12 @@ extern "C" int mcb_layernorm_bwd(const void* x, const void* w, const void* dy, c
     return fail(MCB_ERR_WORKSPACE, "layernorm_bwd: workspace of %zu bytes, 16-byte aligned, needed", mcb_layernorm_bwd_workspace_bytes(rows, D));
   if (!on_boundary(element_bytes(dtype), x, w, dy, dx_residual, dx) || !on_boundary(4, dw, db))
     return fail(MCB_ERR_ALIGN, "layernorm_bwd: a pointer is not aligned to its elements");
+  const size_t row = static_cast<size_t>(D) * element_bytes(dtype), all = rows * row, sum = D * sizeof(float);
+  const auto other = [&](const void* v) { return dx == v ? nullptr : v; };   // (dx may be what it is made of, row for row)
+  const Range ranges[] = {{dx, all}, {dw, sum}, {db, sum}, {sums ? workspace : nullptr, mcb_layernorm_bwd_workspace_bytes(rows, D)},
+                          {other(x), all}, {other(dy), all}, {other(dx_residual), all}, {w, row}};
+  if (outputs_overlap(ranges, 4))
+    return fail(MCB_ERR_SHAPE, "layernorm_bwd: a gradient or the workspace overlaps an input (but for dx = dy or dx_residual) or one another");
   DeviceState* ds = current_device_state();
   if (!ds) return MCB_ERR_NOT_INIT;
   lnorm::Params p = {};

@@ -545,21 +545,8 @@ size_t stat_bytes(const mcb_masked_attention* a) {
   return up1k(static_cast<size_t>(a->batch) * a->kv_heads * a->groups * amask::tiles_of(a->seq) * amask::kTile * 4);
 }
 
-// Whether an output (the first `outputs` of the ranges) overlaps another range: a block would read what another has written already.
-struct Range {
-  const void* p;
-  size_t bytes;
-};
-template <int N>
-bool outputs_overlap(const Range (&r)[N], int outputs) {
-  for (int i = 0; i < outputs; ++i)
-    for (int j = i + 1; j < N; ++j) {
-      const uintptr_t a = reinterpret_cast<uintptr_t>(r[i].p), b = reinterpret_cast<uintptr_t>(r[j].p);
-      if (a != 0 && b != 0 && a < b + r[j].bytes && b < a + r[i].bytes) return true;
-    }
-  return false;
-}
 size_t k_bytes(const mcb_masked_attention* a) { return static_cast<size_t>(a->batch) * a->kv_heads * a->seq * a->head_dim * (a->dtype == MCB_F32 ? 4 : 2); }
+size_t slopes_bytes(const mcb_masked_attention* a) { return static_cast<size_t>(a->kv_heads) * a->groups * 4; }
 size_t lse_bytes(const mcb_masked_attention* a) { return static_cast<size_t>(a->batch) * a->kv_heads * a->groups * a->seq * 4; }
 
 // What flash_attn.cu takes: its tiles are built for heads of 64.
@@ -608,8 +595,9 @@ extern "C" int mcb_attention_masked_fwd(const mcb_masked_attention* a, const voi
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o)) return fail(MCB_ERR_ALIGN, "attention_masked_fwd: 16-byte alignment");
   if (!on_boundary(4, lse)) return fail(MCB_ERR_ALIGN, "attention_masked_fwd: lse is not aligned to its elements");
   const size_t kb = mattn::k_bytes(a), qb = kb * a->groups;
-  const mattn::Range ranges[] = {{o, qb}, {lse, mattn::lse_bytes(a)}, {q, qb}, {k, kb}, {v, kb}, {a->mask, mcb_attention_mask_bytes(a->batch, a->seq)}};
-  if (mattn::outputs_overlap(ranges, 2)) return fail(MCB_ERR_SHAPE, "attention_masked_fwd: o or lse overlaps an input or the other");
+  const Range ranges[] = {{o, qb}, {lse, mattn::lse_bytes(a)}, {q, qb}, {k, kb}, {v, kb}, {a->mask, mcb_attention_mask_bytes(a->batch, a->seq)},
+                          {a->slopes, mattn::slopes_bytes(a)}};
+  if (outputs_overlap(ranges, 2)) return fail(MCB_ERR_SHAPE, "attention_masked_fwd: o or lse overlaps an input or the other");
   DeviceState* ds = current_device_state();
   if (!ds) return MCB_ERR_NOT_INIT;
   c.q = q; c.k = k; c.v = v; c.o = o; c.lse = lse; c.status = ds->status_word;
@@ -638,8 +626,9 @@ extern "C" int mcb_attention_masked_bwd(const mcb_masked_attention* a, const voi
   if (!workspace || workspace_bytes < 2 * stat || (reinterpret_cast<uintptr_t>(workspace) & 1023u) != 0)
     return fail(MCB_ERR_WORKSPACE, "attention_masked_bwd: workspace of %zu bytes, 1024-byte aligned, needed", 2 * stat);
   const size_t kb = mattn::k_bytes(a), qb = kb * a->groups;
-  const mattn::Range ranges[] = {{dq, qb}, {dk, kb}, {dv, kb}, {workspace, 2 * stat}, {q, qb}, {k, kb}, {v, kb}, {o, qb}, {dout, qb}, {lse, mattn::lse_bytes(a)}, {a->mask, mcb_attention_mask_bytes(a->batch, a->seq)}};
-  if (mattn::outputs_overlap(ranges, 4)) return fail(MCB_ERR_SHAPE, "attention_masked_bwd: a gradient or the workspace overlaps an input or one another");
+  const Range ranges[] = {{dq, qb}, {dk, kb}, {dv, kb}, {workspace, 2 * stat}, {q, qb}, {k, kb}, {v, kb}, {o, qb}, {dout, qb}, {lse, mattn::lse_bytes(a)},
+                          {a->mask, mcb_attention_mask_bytes(a->batch, a->seq)}, {a->slopes, mattn::slopes_bytes(a)}};
+  if (outputs_overlap(ranges, 4)) return fail(MCB_ERR_SHAPE, "attention_masked_bwd: a gradient or the workspace overlaps an input or one another");
   DeviceState* ds = current_device_state();
   if (!ds) return MCB_ERR_NOT_INIT;
   c.q = q; c.k = k; c.v = v; c.o_in = o; c.lse = const_cast<float*>(lse); c.dout = dout; c.dq = dq; c.dk = dk; c.dv = dv;

@@ -52,3 +52,70 @@ def test_statistics_off_their_elements(lib):
         assert lib.mcb_clip_grad_norm(grads, 1, 1.0, f[1] + off, 16, HUGE, None) == status
         table = (_lib.AdamWTensor * 1)(_lib.AdamWTensor(f[0], f[1], f[2], f[3], 4, 1, 0))
         assert lib.mcb_adamw_multi_clipped(table, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1.0, 1.0, f[4] + off, 16, HUGE, None) == status
+
+
+def test_layer_norm_outputs_overlap_nothing_else(lib):
+    rows, D = 4, 8
+    all_, row, stat = rows * D * 4, D * 4, rows * 4
+    f = FAR
+    fwd = lambda p: lib.mcb_layernorm_fwd(p[0], p[1], p[2], p[3], p[4], p[5], rows, D, 1e-5, F32, None)  # noqa: E731
+    sizes = [all_, row, row, all_, stat, stat]   # x, w, b, y, mean, rstd
+    for out in (3, 4, 5):
+        for i in range(6):
+            if i == out:
+                continue
+            for at, status in ((f[i], NOT_INIT if (out, i) == (3, 0) else SHAPE), (f[i] + sizes[i] - 4, SHAPE), (f[i] + sizes[i], NOT_INIT),
+                               (f[i] - sizes[out] + 4, SHAPE), (f[i] - sizes[out], NOT_INIT)):
+                args = f[:6]
+                args[out] = at
+                assert fwd(args) == status, (out, i, at - f[i])
+    ws = lib.mcb_layernorm_bwd_workspace_bytes(rows, D)
+    bwd = lambda p: lib.mcb_layernorm_bwd(p[0], p[1], p[2], p[3], p[4], p[5], p[6], 0, rows, D, 1e-5, F32, p[7], HUGE, None)  # noqa: E731
+    sizes = [all_, row, all_, all_, all_, row, row, ws]   # x, w, dy, dx_residual, dx, dw, db, workspace
+    for out in (4, 5, 6, 7):
+        for i in range(8):
+            if i == out:
+                continue
+            for at, status in ((f[i], NOT_INIT if out == 4 and i in (0, 2, 3) else SHAPE), (f[i] + sizes[i] - 16, SHAPE), (f[i] + sizes[i], NOT_INIT),
+                               (f[i] - sizes[out] + 16, SHAPE), (f[i] - sizes[out], NOT_INIT)):
+                args = f[:8]
+                args[out] = at
+                assert bwd(args) == status, (out, i, at - f[i])
+    both = f[:8]
+    both[2] = both[3] = both[4] = f[0]
+    assert bwd(both) == NOT_INIT
+    alone = list(f[:8])
+    alone[5], alone[6], alone[7] = None, None, f[0]   # no sums: the workspace is not used
+    assert bwd(alone) == NOT_INIT
+
+
+def test_embedding_outputs_overlap_nothing(lib):
+    M, H, V, f = 4, 8, 10, FAR
+    for id_bytes in (4, 8):
+        fwd = lambda ids, table, out: lib.mcb_embedding_scaled_fwd(ids, id_bytes, table, out, M, H, V, 1.0, BF16, None)  # noqa: E731
+        assert fwd(f[0], f[1], f[1] + 2 * V * H) == NOT_INIT and fwd(f[0], f[1], f[1] + 2 * V * H - 2) == SHAPE
+        assert fwd(f[0], f[1], f[1] - 2 * M * H) == NOT_INIT and fwd(f[0], f[1], f[1]) == SHAPE
+        assert fwd(f[0], f[1], f[0] + id_bytes * M) == NOT_INIT and fwd(f[0], f[1], f[0] + id_bytes * M - 2) == SHAPE
+        bwd = lambda ids, dout, grad, ws: lib.mcb_embedding_bwd(ids, id_bytes, dout, grad, 0, M, H, V, 1.0, F32, ws, HUGE, None)  # noqa: E731
+        need = lib.mcb_embedding_bwd_workspace_bytes(M, H)
+        assert bwd(f[0], f[1], f[2], f[3]) == NOT_INIT
+        for other, size in ((f[0], id_bytes * M), (f[1], 4 * M * H)):
+            assert bwd(f[0], f[1], other, f[3]) == SHAPE and bwd(f[0], f[1], other + size - 16, f[3]) == SHAPE and bwd(f[0], f[1], other + size, f[3]) == NOT_INIT
+            assert bwd(f[0], f[1], f[2], other - need + 16) == SHAPE and bwd(f[0], f[1], f[2], other - need) == NOT_INIT
+        assert bwd(f[0], f[1], f[2], f[2] + 4 * V * H - 16) == SHAPE and bwd(f[0], f[1], f[2], f[2] + 4 * V * H) == NOT_INIT
+
+
+def test_attention_outputs_do_not_overlap_the_slopes(lib):
+    call = _lib.MaskedAttention(16, HUGE, FAR[9], 2, 100, 2, 3, 64, 0.125, 0.0, BF16, 0)
+    f = FAR
+    assert lib.mcb_attention_masked_fwd(C.byref(call), *f[:5], None) == NOT_INIT
+    for i in (3, 4):
+        args = f[:5]
+        args[i] = f[9] + 16
+        assert lib.mcb_attention_masked_fwd(C.byref(call), *args, None) == SHAPE
+    for i in (6, 7, 8):
+        args = f[:9]
+        args[i] = f[9] + 16
+        assert lib.mcb_attention_masked_bwd(C.byref(call), *args, 1 << 50, HUGE, None) == SHAPE
+    assert lib.mcb_attention_masked_bwd(C.byref(call), *f[:9], f[9], HUGE, None) == SHAPE
+    assert lib.mcb_attention_masked_bwd(C.byref(call), *f[:9], f[9] + 1024, HUGE, None) == NOT_INIT
