@@ -505,6 +505,12 @@ def attention_mask(document_ids: torch.Tensor | None = None, prefix: torch.Tenso
     if given is not None:
         if given.dim() != 2 or given.numel() == 0:
             raise TrainingError(f"attention_mask: document_ids and prefix are [batch, seq], got {list(given.shape)}")
+        if batch not in (None, given.shape[0]) or seq not in (None, given.shape[1]):
+            raise TrainingError(f"attention_mask: batch={batch} and seq={seq} do not fit {list(given.shape)}")
+        if device is not None:
+            device = torch.device(device)
+            if device.type != given.device.type or device.index not in (None, given.device.index):
+                raise TrainingError(f"attention_mask: device {device}, but document_ids or prefix on {given.device}")
         batch, seq = given.shape
         device = given.device
     elif batch is None or seq is None or device is None:

@@ -2,8 +2,10 @@
 import ctypes as C
 
 import pytest
+import torch
 
-from metal_candle_b200 import _lib
+from metal_candle_b200 import _lib, backend
+from metal_candle_b200.backend import TrainingError
 
 NULL, SHAPE, ALIGN, UNSUPPORTED, WORKSPACE, NOT_INIT = -1, -2, -3, -4, -5, -6
 F32, BF16 = _lib.MCB_F32, _lib.MCB_BF16
@@ -119,3 +121,12 @@ def test_attention_outputs_do_not_overlap_the_slopes(lib):
         assert lib.mcb_attention_masked_bwd(C.byref(call), *args, 1 << 50, HUGE, None) == SHAPE
     assert lib.mcb_attention_masked_bwd(C.byref(call), *f[:9], f[9], HUGE, None) == SHAPE
     assert lib.mcb_attention_masked_bwd(C.byref(call), *f[:9], f[9] + 1024, HUGE, None) == NOT_INIT
+
+
+def test_a_mask_of_other_sizes_than_its_documents():
+    ids, marks = torch.zeros(2, 5, dtype=torch.int32, device="meta"), torch.zeros(2, 5, dtype=torch.bool, device="meta")
+    for given in (dict(document_ids=ids), dict(prefix=marks), dict(document_ids=ids, prefix=marks)):
+        for other, message in ((dict(batch=3), "do not fit"), (dict(seq=4), "do not fit"), (dict(batch=2, seq=10), "do not fit"), (dict(device="cuda"), "but document_ids"),
+                               (dict(batch=2, seq=5, device="meta"), "CUDA device"), (dict(), "CUDA device")):
+            with pytest.raises(TrainingError, match=message):
+                backend.attention_mask(**given, **other)
