@@ -20,7 +20,7 @@ struct Layout {
   int64_t qwork;    // int4 [batch * tiles]: the query tiles, the most key blocks first (of each sequence): sequence, tile, first block, blocks
   int64_t kwork;    // int4 [batch * tiles]: the key tiles, the most query blocks first
   int64_t ticket;   // int: tiles that are done while the block is being made
-  int64_t bits;     // two three-level bitmaps per sequence: where runs begin, where a position is no prefix
+  int64_t bits;     // two three-level bitmaps per sequence: where runs begin, where a position is no prefix (of sequences beyond kChunk)
   int64_t bits_per_seq;
   int64_t words;    // in all
 };
@@ -36,7 +36,7 @@ __host__ __device__ inline Layout layout(int64_t batch, int64_t seq) {
   l.kwork = l.qwork + 4 * t;
   l.ticket = l.kwork + 4 * t;
   l.bits = l.ticket + 1;
-  l.bits_per_seq = chunks * (1024 + 32 + 1);
+  l.bits_per_seq = seq > kChunk ? chunks * (1024 + 32 + 1) : 0;   // (shorter ones' bitmaps are in shared memory)
   l.words = l.bits + 2 * batch * l.bits_per_seq;
   return l;
 }

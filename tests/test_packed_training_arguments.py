@@ -130,3 +130,11 @@ def test_a_mask_of_other_sizes_than_its_documents():
                                (dict(batch=2, seq=5, device="meta"), "CUDA device"), (dict(), "CUDA device")):
             with pytest.raises(TrainingError, match=message):
                 backend.attention_mask(**given, **other)
+
+
+@pytest.mark.parametrize("batch,seq", [(1, 1), (65535, 1), (2, 4096), (8, 128), (1, 32768), (3, 1000), (1, 32769), (2, 70001)])
+def test_bytes_of_a_mask(lib, batch, seq):
+    """Four numbers a position, twelve a tile of 128 and, beyond 32768 positions, two bitmaps of three levels, a word for 32 each."""
+    tiles, chunks = (seq + 127) // 128, (seq + 32767) // 32768
+    words = batch * (4 * seq + 12 * tiles + (2 * chunks * 1057 if seq > 32768 else 0))
+    assert 4 * words <= lib.mcb_attention_mask_bytes(batch, seq) <= 4 * words + 48
