@@ -8,8 +8,8 @@ namespace mattn {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // Stands for "no score yet" as the running maximum: finite, so that a row that sees nothing has exponentials 2^(-inf - m) = 0
-// and not NaN, and below any score that counts.
-constexpr float kNoScore = -3e38f;
+// and not NaN, and no finite score lies below.
+constexpr float kNoScore = -3.4028235e38f;
 
 struct Call {
   amask::View mask;

@@ -162,3 +162,20 @@ def test_many_rows_taken_again(cuda_device):
             for name, value in want.items():
                 x = token(got[name]) if name == "o" else part(got[name][..., None]).view(1, -1) if name == "lse" else part(got[name])
                 ref.check(x, value, f"{name} of {b}, {at}")
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 64), (F32, 8)])
+def test_scores_near_the_lowest_number(cuda_device, dtype, d):
+    """Scores of -2.25e38, -3.25e38 in units of log 2, are scores: a row that has no others takes the mean of its keys."""
+    S = 70
+    q, k, v, _ = inputs(cuda_device, 1, S, 1, 1, d, dtype, False, 8)
+    q.zero_()
+    k.zero_()
+    q[..., 0], k[..., 0] = 1.5e19, -1.5e19
+    o, lse = backend.attention_masked_forward(q, k, v, 1, 1.0, backend.attention_mask(batch=1, seq=S, device=cuda_device))
+    score = float(q[0, 0, 0].double() * k[0, 0, 0].double())
+    assert ((lse.double() - score).abs() <= 2.0 ** -21 * abs(score)).all()
+    for i in range(S):   # all scores equal: weights of 1, summed and divided in float32, the result rounded
+        want = v[0, :i + 1].double().mean(0)
+        bound = (torch.finfo(dtype).eps / 2 + (S + 2) * 2.0 ** -22) * v[0, :i + 1].double().abs().mean(0)
+        assert ((o[0, i].double() - want).abs() <= bound).all(), i
