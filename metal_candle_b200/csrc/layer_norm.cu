@@ -110,7 +110,7 @@ struct Rows {
   uint4* ring;
   int lane, nt, off, D, P, q;
   int64_t j, step, rows;
-  static __host__ __device__ size_t smem(int nt) { return static_cast<size_t>(STAGES) * nt * K * kBlock * 16; }
+  static __host__ __device__ constexpr size_t smem(int nt) { return static_cast<size_t>(STAGES) * nt * K * kBlock * 16; }
   __device__ __forceinline__ Rows(void* base, const Params& p, int nt_) : ring(static_cast<uint4*>(base)), nt(nt_), D(p.D), P(SHIFT ? p.period : 1), rows(p.rows) {
     lane = threadIdx.x % TPR;
     q = SHIFT ? blockIdx.x % P : 0;
@@ -502,27 +502,27 @@ template <typename T, bool BWD, bool SHIFT, int TPR, int K>
 int launch_k(const Params& p, int sms, cudaStream_t st, int* blocks) {
   using R = Rows<T, TPR, K, SHIFT>;
   constexpr size_t kWeight = BWD && staged(TPR, K) ? static_cast<size_t>(TPR) * K * R::N * 4 : 0;
-  size_t smem = R::smem(!BWD ? 1 : p.res != nullptr ? 3 : 2) + kWeight;
-  if (BWD && R::kRows > 1 && smem < 2 * static_cast<size_t>(p.D) * 4) smem = 2 * static_cast<size_t>(p.D) * 4;
+  const size_t smem = R::smem(!BWD ? 1 : p.res != nullptr ? 3 : 2) + kWeight;
+  static_assert(!BWD || R::kRows == 1 || 2 * sizeof(float) * TPR * K * R::N <= R::smem(2), "dw and db of the block's row slots lie over the ring");
   void (*kernel)(const Params) = ln_fwd_kernel<T, TPR, K, SHIFT>;
   if constexpr (BWD) kernel = p.part != nullptr ? ln_bwd_kernel<T, TPR, K, SHIFT, true> : ln_bwd_kernel<T, TPR, K, SHIFT, false>;
   // as many blocks as are on the device at once (each leaves a line of sums), a whole number of rounds of the alignments; asked once for
-  // every kernel, number of operands, device and size of shared memory (a word, so that threads that meet here read a whole answer)
-  static std::atomic<uint64_t> answer[4][64];
-  int dev = 0, per_sm = 0;
+  // every kernel, number of operands and device
+  static std::atomic<int> answer[4][64];
+  int dev = 0;
   MCB_CHECK_CUDA(cudaGetDevice(&dev));
-  std::atomic<uint64_t>& known = answer[(BWD && p.part != nullptr) + 2 * (BWD && p.res != nullptr)][dev & 63];
-  const uint64_t seen = known.load(std::memory_order_relaxed);
-  if (static_cast<uint32_t>(seen) == smem + 1) {
-    per_sm = static_cast<int>(seen >> 32);
-  } else {
-    const size_t most = R::smem(3) + kWeight > smem ? R::smem(3) + kWeight : smem;   // (of any call of this kernel: another thread's launch must not find less)
+  if (dev >= 64) return fail(MCB_ERR_SHAPE, "layer norm: device %d out of range", dev);
+  std::atomic<int>& known = answer[(BWD && p.part != nullptr) + 2 * (BWD && p.res != nullptr)][dev];
+  int per_sm = known.load(std::memory_order_relaxed);
+  if (per_sm == 0) {
+    const size_t most = R::smem(BWD ? 3 : 1) + kWeight;   // (of any call of this kernel: another thread's launch must not find less)
     MCB_CHECK_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most)));
     MCB_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, R::kBlock, smem));
-    if (dev < 64) known.store(static_cast<uint64_t>(per_sm) << 32 | (smem + 1), std::memory_order_relaxed);
+    if (per_sm < 1) per_sm = 1;
+    known.store(per_sm, std::memory_order_relaxed);
   }
   const int64_t turns = (p.rows + p.period - 1) / p.period;   // rows of an alignment
-  const int each = blocks_for(turns, R::kRows, sms, per_sm < 1 ? 1 : per_sm), most = blocks_for(p.rows, 1, sms, per_sm < 1 ? 1 : per_sm) / p.period;
+  const int each = blocks_for(turns, R::kRows, sms, per_sm), most = blocks_for(p.rows, 1, sms, per_sm) / p.period;
   *blocks = p.period * (each < most || most < 1 ? each : most);
   MCB_CHECK_CUDA(launch_kernel(kernel, dim3(*blocks), dim3(R::kBlock), smem, st, chained_launch(), p));
   MCB_CHECK_LAUNCH("layer_norm");
