@@ -389,7 +389,7 @@ typedef struct {
   size_t mask_bytes;
   const float* slopes;     /* [kv_heads * groups], device; or null */
   int64_t batch, seq, kv_heads, groups, head_dim;
-  float scale, softcap;    /* scale > 0; softcap 0: none */
+  float scale, softcap;    /* scale > 0; softcap 0: none, else scale / softcap a normal number */
   int32_t dtype, o_token_major;
 } mcb_masked_attention;
 int mcb_attention_masked_fwd(const mcb_masked_attention* call, const void* q, const void* k, const void* v, void* o, float* lse,

@@ -567,8 +567,10 @@ int fill(Call& c, const mcb_masked_attention* a, const char* who) {
     return fail(MCB_ERR_SHAPE, "%s: batch=%lld kv_heads=%lld groups=%lld seq=%lld", who, (long long)a->batch, (long long)a->kv_heads, (long long)a->groups, (long long)a->seq);
   const auto finite = [](float v) { return v - v == 0.0f; };
   if (!(a->scale > 0.0f && finite(a->scale * kLog2e))) return fail(MCB_ERR_SHAPE, "%s: scale must be positive and finite", who);
-  if (!(a->softcap >= 0.0f && finite(a->softcap * kLog2e) && (a->softcap == 0.0f || finite(a->scale / a->softcap))))
-    return fail(MCB_ERR_SHAPE, "%s: softcap must be 0 (none) or positive and finite, and scale / softcap finite", who);
+  // (a quotient below 2^-126 has lost digits that every score would be short of)
+  const float bend = a->scale / a->softcap;
+  if (!(a->softcap >= 0.0f && finite(a->softcap * kLog2e) && (a->softcap == 0.0f || (finite(bend) && bend >= 0x1p-126f))))
+    return fail(MCB_ERR_SHAPE, "%s: softcap must be 0 (none) or positive and finite, and scale / softcap within float32's normal numbers", who);
   if (!aligned16(a->mask) || (reinterpret_cast<uintptr_t>(a->slopes) & 3) != 0) return fail(MCB_ERR_ALIGN, "%s: alignment of the mask or the slopes", who);
   c = Call{};
   c.mask = amask::view(a->mask, a->batch, a->seq);

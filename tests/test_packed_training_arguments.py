@@ -138,3 +138,12 @@ def test_bytes_of_a_mask(lib, batch, seq):
     tiles, chunks = (seq + 127) // 128, (seq + 32767) // 32768
     words = batch * (4 * seq + 12 * tiles + (2 * chunks * 1057 if seq > 32768 else 0))
     assert 4 * words <= lib.mcb_attention_mask_bytes(batch, seq) <= 4 * words + 48
+
+
+@pytest.mark.parametrize("scale,softcap,status", [(0.125, 1.7e38, SHAPE), (0.125, 2.0 ** 124, SHAPE), (0.125, 2.0 ** 123, NOT_INIT), (2.0 ** -100, 2.0 ** 27, SHAPE),
+                                                  (2.0 ** -100, 2.0 ** 26, NOT_INIT), (1.0, 0.0, NOT_INIT), (1e-38, 0.0, NOT_INIT)])
+def test_caps_whose_quotient_has_lost_digits(lib, scale, softcap, status):
+    """scale / softcap below 2^-126 is held with fewer digits: the scores would be wrong by as much."""
+    call = _lib.MaskedAttention(16, HUGE, None, 2, 100, 2, 3, 64, scale, softcap, F32, 0)
+    assert lib.mcb_attention_masked_fwd(C.byref(call), *FAR[:5], None) == status
+    assert lib.mcb_attention_masked_bwd(C.byref(call), *FAR[:9], 1 << 50, HUGE, None) == status
