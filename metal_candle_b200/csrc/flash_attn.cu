@@ -689,7 +689,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       if (lane == 0) mbar_arrive(o_free);   // the next item's products may overwrite O
       bool bad = false;
       if constexpr (MASKED) {
-        // a row that is not finite is taken again from what it sees
+        // a row that is not finite is taken again from what it sees, unless the sum of its weights is NaN: then one that it sees is, and every element is
         float sum = 0.0f;
 #pragma unroll
         for (int c4 = 0; c4 < 4; ++c4)
@@ -699,7 +699,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             const float x = __uint_as_float(ov[c4][e]);
             sum = fmaf(x, 0.0f, sum);
           }
-        bad = qpos < p.S && !(sum * inv == 0.0f);
+        bad = qpos < p.S && l == l && !(sum * inv == 0.0f);
       }
       if (qpos < p.S && !bad) {
 #pragma unroll
@@ -1372,7 +1372,7 @@ attn_dq_masked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(dq_free);   // the next item's products may overwrite both sums
-      const bool bad = qpos < p.S && !(sum == 0.0f);
+      const bool bad = qpos < p.S && delta == delta && !(sum == 0.0f);   // (delta NaN, of what the row sees alone: every element is)
       if (qpos < p.S && !bad) {
         __nv_bfloat16* orow = p.dQ + (w.qrow0 + row) * kD;
 #pragma unroll

@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 3) masked_fwd_kernel(const __grid_co
       if (col >= c.D) continue;
       float4 v = acc[i][jj];
       v = none ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-      if (!finite4(v)) bad[ty + 16 * i] = 1;
+      if (!finite4(v) && l[i] == l[i]) bad[ty + 16 * i] = 1;   // (a sum of weights that is NaN: so is every element, by right)
       store4(out + col, v);
     }
     if (c.lse != nullptr && tx == 0) c.lse[q_row(c, w.b, hk, g, s)] = none ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(kThreads) masked_dq_kernel(const __grid_consta
         v = make_float4(fmaf(put_right, k.x, v.x), fmaf(put_right, k.y, v.y), fmaf(put_right, k.z, v.z), fmaf(put_right, k.w, v.w));
       }
       v = make_float4(v.x * c.scale, v.y * c.scale, v.z * c.scale, v.w * c.scale);
-      if (!finite4(v)) bad[ty + 16 * i] = 1;
+      if (!finite4(v) && d == d) bad[ty + 16 * i] = 1;   // (delta, of what the row sees alone, NaN: so is every element)
       store4(out + col, v);
     }
   }

@@ -202,7 +202,18 @@ __device__ __noinline__ void dkv_row(const Call& c, int b, int hk, int s) {
   const int64_t kr = k_row(c, b, hk, s) * c.D, pitch = amask::tiles_of(c.S) * amask::kTile, ostep = c.o_tok ? static_cast<int64_t>(c.Hk) * c.G * c.D : c.D;
   const T *k = static_cast<const T*>(c.k) + kr, *v = static_cast<const T*>(c.v) + kr;
   float gk[4] = {}, gv[4] = {};
+  // a query whose log-sum-exp is NaN makes every element NaN: sooner seen than from its products
   bool nan = false;
+  for (int g = 0; g < c.G && !nan; ++g) {
+    const float* of = c.nlse2 + ((static_cast<int64_t>(b) * c.Hk + hk) * c.G + g) * pitch;
+    float sum = 0.0f;
+#pragma unroll 4
+    for (int i = seen.x + (threadIdx.x & 31); i < seen.y; i += 32) {
+      const float x = of[i];
+      if (x != x) sum = x;
+    }
+    nan = __any_sync(0xffffffffu, sum != sum);
+  }
   for (int g = 0; g < c.G && !nan; ++g) {
     const float slope2 = c.slopes ? c.slopes[hk * c.G + g] * kLog2e : 0.0f;
     const T *q = static_cast<const T*>(c.q) + q_row(c, b, hk, g, 0) * c.D, *go = static_cast<const T*>(c.dout) + o_at(c, b, hk, g, 0);

@@ -179,3 +179,23 @@ def test_scores_near_the_lowest_number(cuda_device, dtype, d):
         want = v[0, :i + 1].double().mean(0)
         bound = (torch.finfo(dtype).eps / 2 + (S + 2) * 2.0 ** -22) * v[0, :i + 1].double().abs().mean(0)
         assert ((o[0, i].double() - want).abs() <= bound).all(), i
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_late_nan_takes_no_walk_over_the_keys_before_it(cuda_device, dtype):
+    """A query from the NaN key on has weights whose sum is NaN, and a key before it a query whose log-sum-exp is: NaN by right, which shows without taking
+    the row again.  (What is left are the rows of one tile before the key.)"""
+    S, G, d = (16384 if dtype == BF16 else 4096), 2, 64
+    at = S // 2 + 1   # a tile's second position
+    q, k, v, dout = inputs(cuda_device, 1, S, 1, G, d, dtype, False, 3)
+    mask = backend.attention_mask(batch=1, seq=S, device=cuda_device)
+    finite = fastest(lambda: run(q, k, v, dout, G, 0.125, mask, 0.0, None, False))
+    k[0, at, 3] = math.nan
+    got = run(q, k, v, dout, G, 0.125, mask, 0.0, None, False)
+    for name in ("o", "lse", "dq"):
+        t = got[name].view(G, S, -1)
+        assert torch.isfinite(t[:, :at]).all() and torch.isnan(t[:, at:]).all(), name
+    assert torch.isnan(got["dk"]).all() and torch.isnan(got["dv"]).all()
+    took = fastest(lambda: run(q, k, v, dout, G, 0.125, mask, 0.0, None, False))
+    # one row a head, of half the sequence, by one warp: 256 (64) steps of some microseconds, three times
+    assert took <= 4 * finite + 6, (took, finite)
