@@ -380,7 +380,8 @@ int mcb_attention_mask(const void* document_ids, int id_bytes, const uint8_t* pr
                        int64_t seq, void* stream);
 /* s = scale q.k; with softcap > 0: s = softcap tanh(s / softcap); with slopes: s -= slopes[head] |i - j|; o = softmax of s over the
  * visible keys, times v.  A query that sees nothing, or whose every score is -inf, has o = 0, lse = -inf and no gradient; what lies at
- * positions that a query does not see never reaches it, NaN included.  Layouts as in mcb_attention_causal_fwd_ex with nb = batch *
+ * positions that a query does not see never reaches it, NaN included (where some are not finite, rows beside them are computed again one by one: slow
+ * for long documents, so padding is better left finite).  Layouts as in mcb_attention_causal_fwd_ex with nb = batch *
  * kv_heads: q [nb, groups * seq, head_dim], k and v [nb, seq, head_dim], lse [nb, groups * seq] float32, o like q or (o_token_major)
  * [batch * seq, kv_heads * groups * head_dim].  MCB_F32 or MCB_BF16, head_dim a multiple of 8 up to 128, any seq; bfloat16 with
  * head_dim 64 runs on the tensor cores. */

@@ -569,7 +569,9 @@ def attention_masked_forward(q, k, v, groups: int, scale: float, mask: Attention
     """Grouped-query attention under `mask`: softmax over the visible keys of s = scale q.k, with softcap > 0 bent to softcap *
     tanh(s / softcap), with slopes [query heads] float32 lowered by slopes[head] * |i - j|.  q [nb, groups*S, d] (row g*S + s),
     k and v [nb, S, d], nb = batch * kv_heads; float32 or bfloat16, d a multiple of 8 up to 128.  Returns (o, lse [nb, groups*S]
-    float32); o like q, or token-major [batch*S, kv_heads*groups*d].  A position that sees nothing has o = 0 and lse = -inf."""
+    float32); o like q, or token-major [batch*S, kv_heads*groups*d].  A position that sees nothing has o = 0 and lse = -inf.
+    Values at positions that a row does not see never reach it; where some are not finite, rows beside them are computed again one by one, which is
+    slow in long documents: padding is better left finite."""
     call = _masked_call(q, k, v, groups, scale, mask, softcap, slopes, token_major)
     if q.get_device() != torch._C._cuda_getDevice():
         with torch.cuda.device(q.device):

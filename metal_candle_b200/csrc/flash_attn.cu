@@ -1023,7 +1023,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
 }
 
 // The same under a mask, with one product more.  delta = sum of P dP over a row is what the gradient of a softmax turns on, and rowsum(dO * O) of
-// the O that was stored in bfloat16 (from probabilities that were rounded for the tensor cores) is off by 2^-9 of |dO| |O|: where a row
+// the O that was stored in bfloat16 (from probabilities that were rounded for the tensor cores) is off by up to 2^-8 of |dO| |O|: where a row
 // puts its weight on few keys, P (dP - delta) is a small difference and that error exceeds all others (100 positions, scores of
 // standard deviation 6: gradients off by 0.0054 of their size instead of 0.0023).  So the sum is taken here from P and dP in float32, while the products
 // go on with d~ = rowsum(dO * O), and is put right at the end:

@@ -302,7 +302,7 @@ def grad_norm(grads: Iterable[torch.Tensor]) -> torch.Tensor:
 
 def clip_grad_norm(grads: Iterable[torch.Tensor], max_norm: float, out: Optional[Iterable[torch.Tensor]] = None) -> torch.Tensor:
     """Scales the gradients (in place, or into `out`) so that their global norm is at most max_norm; returns the norm they had.
-    `GradClipper` does the same for buffers that stay, without making their table again."""
+    `GradClipper` does the same for buffers that stay, without making their table again (1 us of host time a tensor)."""
     return GradClipper(grads, out).clip(max_norm)
 
 
