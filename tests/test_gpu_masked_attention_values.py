@@ -199,3 +199,39 @@ def test_a_late_nan_takes_no_walk_over_the_keys_before_it(cuda_device, dtype):
     took = fastest(lambda: run(q, k, v, dout, G, 0.125, mask, 0.0, None, False))
     # one row a head, of half the sequence, by one warp: 256 (64) steps of some microseconds, three times
     assert took <= 4 * finite + 6, (took, finite)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_rows_taken_again_on_two_streams_and_in_a_graph(cuda_device, dtype):
+    """The same bits whatever runs beside them, eager, on two streams at a time, and replayed; and finite passes between them."""
+    B, S, G, d = 3, 1500, 4, 64
+    ids = (torch.arange(S, device=cuda_device) // 170).to(torch.int32).expand(B, S).contiguous()
+    mask = backend.attention_mask(ids)
+    clean = inputs(cuda_device, B, S, 1, G, d, dtype, True, 4)
+    dirty = [t.clone() for t in clean]
+    odd = ids[0] % 2 == 1
+    dirty[0].view(B, G, S, d)[:, :, odd] = math.nan
+    dirty[1][:, odd] = dirty[2][:, odd] = math.inf
+    step = lambda t: run(*t, G, 0.125, mask, 15.0, None, True)  # noqa: E731
+    bits = lambda out: {n: t.view(torch.int16 if t.dtype == BF16 else torch.int32).clone() for n, t in out.items()}  # noqa: E731
+    want = [bits(step(t)) for t in (clean, dirty)]
+    assert all(torch.isfinite(t.view(dtype if n != "lse" else F32)).all() for n, t in want[0].items())
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for i in range(8):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append((step(dirty if i % 4 < 2 else clean), i % 4 < 2))
+    torch.cuda.synchronize()
+    for out, bad in outs:
+        assert all(torch.equal(x, want[bad][n]) for n, x in bits(out).items())
+    buf = [t.clone() for t in clean]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(buf)
+    for bad in (1, 0, 1):
+        for b, t in zip(buf, (clean, dirty)[bad]):
+            b.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, want[bad][n]) for n, x in bits(held).items())
+    assert _lib.device_status() == 0
